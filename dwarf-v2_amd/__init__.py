@@ -18,17 +18,22 @@ Public surface (reference names, Lanerra/dwarf-v2):
   interference_pool, interference_packet,
   interference_packet_forward                        train/train_dwarf.py (InterferencePacket)
   q6: pack_kv, unpack_kv, q6_prefill, q6_decode      (no reference counterpart)
+  layer_norm; rotary_plan, RotaryPlan, rotary_embed;
+  linear_attention, linear_attention_step            (no reference counterpart)
 """
 
-from . import _lib, block, lattice, npci, ops, packet, planner, probe, q6
+from . import _lib, block, lattice, linattn, norm, npci, ops, packet, planner, probe, q6, rotary
 from .block import dsqg_block_forward
 from .dsqg import (_DSQGProbedFn, _DSQGV18GroupedFn, dsqg_attention_v18_grouped, dsqg_attention_with_probes,
                    dsqg_backward, dsqg_forward)
 from .ema import bounded_ema_factor, causal_ema_scan, inverse_bounded_ema_factor
+from .linattn import linear_attention, linear_attention_step
+from .norm import layer_norm
 from .npci import npci_rotate
 from .packet import _InterferencePacketFn, _InterferencePoolFn, interference_packet, interference_packet_forward, interference_pool
 from .planner import _normalize_grouping_args, _plan_sparse_groups, _verify_sparse_plan
 from .probe import _PhaseProbeFn, phase_probe_features
+from .rotary import RotaryPlan, rotary_embed, rotary_plan
 from .lattice import (
     ALL_OFFSETS,
     GROUPED_MODE_IDS,
@@ -44,6 +49,7 @@ __all__ = [
     "ALL_OFFSETS",
     "GROUPED_MODE_IDS",
     "R_PLANES",
+    "RotaryPlan",
     "_DSQGProbedFn",
     "_DSQGV18GroupedFn",
     "_InterferencePacketFn",
@@ -68,9 +74,14 @@ __all__ = [
     "interference_packet_forward",
     "interference_pool",
     "inverse_bounded_ema_factor",
+    "layer_norm",
+    "linear_attention",
+    "linear_attention_step",
     "npci_rotate",
     "phase_probe_features",
     "q6",
+    "rotary_embed",
+    "rotary_plan",
 ]
 
 

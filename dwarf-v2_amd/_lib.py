@@ -13,7 +13,7 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t
 
 LIB_NAME = "libdwarf_dsqg.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 DWARF_OK = 0
 DWARF_ERR_INVALID_ARGUMENT = 1
@@ -23,6 +23,7 @@ DWARF_ERR_WORKSPACE = 4
 
 DWARF_BF16 = 0
 DWARF_F32 = 1
+DWARF_F16 = 2   # the entry points of dwarf_mixer.h only
 
 EXPORTED_SYMBOLS = (
     "dwarf_abi_version",
@@ -320,6 +321,87 @@ class HeadGateBwdArgs(ctypes.Structure):
     ]
 
 
+# ---- include/dwarf_mixer.h ----
+MIXER_SYMBOLS = ("dwarf_layer_norm_fwd", "dwarf_layer_norm_bwd_workspace_bytes", "dwarf_layer_norm_bwd", "dwarf_rotary",
+                 "dwarf_linear_attention_segment", "dwarf_linear_attention_states_bytes", "dwarf_linear_attention_fwd",
+                 "dwarf_linear_attention_bwd_workspace_bytes", "dwarf_linear_attention_bwd",
+                 "dwarf_linear_attention_step")
+
+
+class LayerNormFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("groups", c_int32), ("D", c_int32),
+        ("dtype", c_int32), ("eps", c_float),
+        ("x", c_void_p), ("x_stride", _i64(2)),
+        ("weight", c_void_p), ("bias", c_void_p),
+        ("y", c_void_p), ("y_stride", _i64(2)),
+    ]
+
+
+class LayerNormBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", LayerNormFwdArgs),
+        ("dy", c_void_p), ("dy_stride", _i64(2)),
+        ("dx", c_void_p), ("dx_stride", _i64(2)),
+        ("dweight", c_void_p), ("dbias", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", c_int32), ("H", c_int32), ("H_kv", c_int32), ("N", c_int32), ("D", c_int32), ("pairs", c_int32),
+        ("dtype", c_int32), ("interleaved", c_int32), ("inverse", c_int32), ("position_bytes", c_int32),
+        ("magnitude", c_float),
+        ("q", c_void_p), ("q_stride", _i64(4)),
+        ("k", c_void_p), ("k_stride", _i64(4)),
+        ("positions", c_void_p), ("position_stride", _i64(2)),
+        ("turns", c_void_p),
+        ("q_out", c_void_p), ("q_out_stride", _i64(4)),
+        ("k_out", c_void_p), ("k_out_stride", _i64(4)),
+    ]
+
+
+class LinearAttentionFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", c_int32), ("H", c_int32), ("H_kv", c_int32), ("N", c_int32), ("head_dim", c_int32),
+        ("dtype", c_int32), ("scale", c_float),
+        ("q", c_void_p), ("q_stride", _i64(4)),
+        ("k", c_void_p), ("k_stride", _i64(4)),
+        ("v", c_void_p), ("v_stride", _i64(4)),
+        ("log_decay", c_void_p), ("lengths", c_void_p), ("initial", c_void_p),
+        ("out", c_void_p), ("out_stride", _i64(4)),
+        ("final", c_void_p),
+        ("states", c_void_p), ("states_bytes", c_size_t),
+    ]
+
+
+class LinearAttentionBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", LinearAttentionFwdArgs),
+        ("dout", c_void_p), ("dout_stride", _i64(4)),
+        ("dfinal", c_void_p),
+        ("dq", c_void_p), ("dq_stride", _i64(4)),
+        ("dk", c_void_p), ("dk_stride", _i64(4)),
+        ("dv", c_void_p), ("dv_stride", _i64(4)),
+        ("dlog_decay", c_void_p), ("dinitial", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class LinearAttentionStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("S", c_int32), ("H", c_int32), ("H_kv", c_int32), ("pool", c_int32), ("head_dim", c_int32),
+        ("dtype", c_int32), ("scale", c_float),
+        ("q", c_void_p), ("q_stride", _i64(3)),
+        ("k", c_void_p), ("k_stride", _i64(3)),
+        ("v", c_void_p), ("v_stride", _i64(3)),
+        ("log_decay", c_void_p), ("slots", c_void_p),
+        ("state", c_void_p), ("new_state", c_void_p), ("slot_stride", c_int64),
+        ("out", c_void_p), ("out_stride", _i64(3)),
+    ]
+
+
 class NativeLibraryError(RuntimeError):
     """The HIP library is missing, stale or failed a call."""
 
@@ -426,6 +508,26 @@ def load() -> ctypes.CDLL:
     lib.dwarf_head_gate_bwd_workspace_bytes.argtypes = [POINTER(HeadGateBwdArgs)]
     lib.dwarf_head_gate_bwd.restype = c_int
     lib.dwarf_head_gate_bwd.argtypes = [POINTER(HeadGateBwdArgs), c_void_p]
+    lib.dwarf_layer_norm_fwd.restype = c_int
+    lib.dwarf_layer_norm_fwd.argtypes = [POINTER(LayerNormFwdArgs), c_void_p]
+    lib.dwarf_layer_norm_bwd_workspace_bytes.restype = c_size_t
+    lib.dwarf_layer_norm_bwd_workspace_bytes.argtypes = [POINTER(LayerNormBwdArgs)]
+    lib.dwarf_layer_norm_bwd.restype = c_int
+    lib.dwarf_layer_norm_bwd.argtypes = [POINTER(LayerNormBwdArgs), c_void_p]
+    lib.dwarf_rotary.restype = c_int
+    lib.dwarf_rotary.argtypes = [POINTER(RotaryArgs), c_void_p]
+    lib.dwarf_linear_attention_segment.restype = c_int32
+    lib.dwarf_linear_attention_segment.argtypes = [c_int32, c_int32, c_int32]
+    lib.dwarf_linear_attention_states_bytes.restype = c_size_t
+    lib.dwarf_linear_attention_states_bytes.argtypes = [POINTER(LinearAttentionFwdArgs)]
+    lib.dwarf_linear_attention_fwd.restype = c_int
+    lib.dwarf_linear_attention_fwd.argtypes = [POINTER(LinearAttentionFwdArgs), c_void_p]
+    lib.dwarf_linear_attention_bwd_workspace_bytes.restype = c_size_t
+    lib.dwarf_linear_attention_bwd_workspace_bytes.argtypes = [POINTER(LinearAttentionBwdArgs)]
+    lib.dwarf_linear_attention_bwd.restype = c_int
+    lib.dwarf_linear_attention_bwd.argtypes = [POINTER(LinearAttentionBwdArgs), c_void_p]
+    lib.dwarf_linear_attention_step.restype = c_int
+    lib.dwarf_linear_attention_step.argtypes = [POINTER(LinearAttentionStepArgs), c_void_p]
     _LIB = lib
     return lib
 

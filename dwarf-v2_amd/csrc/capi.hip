@@ -10,6 +10,7 @@
 #include "dsqg_internal.h"
 #include "dwarf_block.h"
 #include "dwarf_dsqg.h"
+#include "dwarf_mixer.h"
 
 namespace dwarf {
 size_t ema_fwd_workspace(int B, int N, int D);
@@ -50,6 +51,16 @@ hipError_t launch_normalize_probes(const float* q, const float* k, float* out, h
 size_t head_gate_bwd_workspace(const dwarf_head_gate_bwd_args& a);
 hipError_t launch_head_gate_fwd(const dwarf_head_gate_fwd_args& a, hipStream_t stream);
 hipError_t launch_head_gate_bwd(const dwarf_head_gate_bwd_args& a, hipStream_t stream);
+size_t layer_norm_bwd_workspace(const dwarf_layer_norm_bwd_args& a);
+hipError_t launch_layer_norm_fwd(const dwarf_layer_norm_fwd_args& a, hipStream_t stream);
+hipError_t launch_layer_norm_bwd(const dwarf_layer_norm_bwd_args& a, hipStream_t stream);
+hipError_t launch_rotary(const dwarf_rotary_args& a, hipStream_t stream);
+int linear_attention_segment(int B, int H, int N);
+size_t linear_attention_states_bytes(const dwarf_linear_attention_fwd_args& a);
+size_t linear_attention_bwd_workspace(const dwarf_linear_attention_bwd_args& a);
+hipError_t launch_linear_attention_fwd(const dwarf_linear_attention_fwd_args& a, hipStream_t stream);
+hipError_t launch_linear_attention_bwd(const dwarf_linear_attention_bwd_args& a, hipStream_t stream);
+hipError_t launch_linear_attention_step(const dwarf_linear_attention_step_args& a, hipStream_t stream);
 }  // namespace dwarf
 
 namespace {
@@ -91,7 +102,7 @@ int zero_floats(float* p, int64_t n, hipStream_t stream, const char* what) {
 
 constexpr int kMaxOffsets = 256;  // LDS tables of the DSQG kernels
 
-size_t elem_size(int dtype) { return dtype == DWARF_BF16 ? 2 : 4; }
+size_t elem_size(int dtype) { return dtype == DWARF_F32 ? 4 : 2; }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -838,6 +849,191 @@ int dwarf_head_gate_bwd(const dwarf_head_gate_bwd_args* args, dwarf_stream_t str
   if (!a.workspace || a.workspace_bytes < need || !aligned16(a.workspace))
     return fail(DWARF_ERR_WORKSPACE, "workspace needs %zu bytes, 16-byte aligned, got %zu", need, a.workspace_bytes);
   return hip_status(dwarf::launch_head_gate_bwd(a, reinterpret_cast<hipStream_t>(stream)), "dwarf_head_gate_bwd");
+}
+
+// ---- layer norm, rotary positions, decayed linear attention (dwarf_mixer.h) ----
+static bool mixer_dtype(int dtype) { return dtype == DWARF_BF16 || dtype == DWARF_F16 || dtype == DWARF_F32; }
+static bool finite_f32(float x) { return x - x == 0.f; }
+
+static int check_elements(const char* name, const void* p, int dtype) {
+  if (!p) return fail(DWARF_ERR_INVALID_ARGUMENT, "%s is NULL", name);
+  if (reinterpret_cast<uintptr_t>(p) % elem_size(dtype))
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "%s is not aligned to its elements", name);
+  return DWARF_OK;
+}
+
+static int check_norm(const dwarf_layer_norm_fwd_args& a) {
+  if (a.rows < 0 || a.groups < 1 || a.D < 1)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "bad sizes rows=%lld groups=%d D=%d", static_cast<long long>(a.rows), a.groups, a.D);
+  if (!mixer_dtype(a.dtype)) return fail(DWARF_ERR_INVALID_ARGUMENT, "dtype=%d", a.dtype);
+  if (!(a.eps >= 0.f) || !finite_f32(a.eps)) return fail(DWARF_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+  if (a.groups > 65535 || a.D > (1 << 24) || static_cast<int64_t>(a.groups) * a.D >= (int64_t(1) << 30) ||
+      a.rows >= (int64_t(1) << 40))
+    return fail(DWARF_ERR_UNSUPPORTED, "groups up to 65535, D up to 2^24 and groups * D below 2^30");
+  return a.rows ? check_elements("x", a.x, a.dtype) : DWARF_OK;
+}
+
+int dwarf_layer_norm_fwd(const dwarf_layer_norm_fwd_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  int rc = check_norm(*args);
+  if (rc || args->rows == 0) return rc ? rc : ok();
+  if ((rc = check_elements("y", args->y, args->dtype))) return rc;
+  return hip_status(dwarf::launch_layer_norm_fwd(*args, reinterpret_cast<hipStream_t>(stream)), "dwarf_layer_norm_fwd");
+}
+
+size_t dwarf_layer_norm_bwd_workspace_bytes(const dwarf_layer_norm_bwd_args* args) {
+  return args && check_norm(args->fwd) == DWARF_OK && args->fwd.rows ? dwarf::layer_norm_bwd_workspace(*args) : 0;
+}
+
+int dwarf_layer_norm_bwd(const dwarf_layer_norm_bwd_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_layer_norm_bwd_args& a = *args;
+  int rc = check_norm(a.fwd);
+  if (rc) return rc;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (a.fwd.rows == 0) {   // the weights' gradients are sums over nothing
+    const int64_t n = static_cast<int64_t>(a.fwd.groups) * a.fwd.D;
+    rc = zero_floats(a.dweight, n, s, "dwarf_layer_norm_bwd");
+    return rc ? rc : zero_floats(a.dbias, n, s, "dwarf_layer_norm_bwd");
+  }
+  if ((rc = check_elements("dy", a.dy, a.fwd.dtype))) return rc;
+  if (a.dx && (rc = check_elements("dx", a.dx, a.fwd.dtype))) return rc;
+  if (!a.dx && !a.dweight && !a.dbias) return ok();
+  const size_t need = dwarf::layer_norm_bwd_workspace(a);
+  if (need && (!a.workspace || a.workspace_bytes < need || !aligned16(a.workspace)))
+    return fail(DWARF_ERR_WORKSPACE, "workspace needs %zu bytes, 16-byte aligned, got %zu", need, a.workspace_bytes);
+  return hip_status(dwarf::launch_layer_norm_bwd(a, s), "dwarf_layer_norm_bwd");
+}
+
+int dwarf_rotary(const dwarf_rotary_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_rotary_args& a = *args;
+  if (a.B < 0 || a.N < 0 || a.H < 1 || (a.k && a.H_kv < 1) || a.D < 2 || a.D % 2)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "bad sizes B=%d H=%d H_kv=%d N=%d D=%d (D even)", a.B, a.H, a.H_kv, a.N, a.D);
+  if (a.pairs < 1 || a.pairs > a.D / 2)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "pairs=%d outside [1, D/2=%d]", a.pairs, a.D / 2);
+  if (!mixer_dtype(a.dtype)) return fail(DWARF_ERR_INVALID_ARGUMENT, "dtype=%d", a.dtype);
+  if (a.position_bytes != 4 && a.position_bytes != 8)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "position_bytes=%d (4 or 8)", a.position_bytes);
+  if (!finite_f32(a.magnitude)) return fail(DWARF_ERR_INVALID_ARGUMENT, "magnitude must be finite");
+  if (a.D > 65536 || a.H > 65536 || (a.k && a.H_kv > 65536) ||
+      static_cast<double>(a.B) * a.N * a.D * (static_cast<double>(a.H) + (a.k ? a.H_kv : 0)) >= 0x1p38)
+    return fail(DWARF_ERR_UNSUPPORTED, "D and heads up to 65536, fewer than 2^38 elements");
+  if (static_cast<int64_t>(a.B) * a.N == 0) return ok();
+  if (!a.positions || !a.turns) return fail(DWARF_ERR_INVALID_ARGUMENT, "positions or turns is NULL");
+  const struct { const char* name; const void* p; const int64_t* s; bool used; } rows[] = {
+      {"q", a.q, a.q_stride, true}, {"q_out", a.q_out, a.q_out_stride, true},
+      {"k", a.k, a.k_stride, a.k != nullptr}, {"k_out", a.k_out, a.k_out_stride, a.k != nullptr}};
+  for (const auto& r : rows) {
+    if (!r.used) continue;
+    const int rc = check_elements(r.name, r.p, a.dtype);
+    if (rc) return rc;
+    if (r.s[3] != 1) return fail(DWARF_ERR_INVALID_ARGUMENT, "%s needs unit stride on D", r.name);
+    if (a.interleaved && (reinterpret_cast<uintptr_t>(r.p) % (2 * elem_size(a.dtype)) || r.s[0] % 2 || r.s[1] % 2 || r.s[2] % 2))
+      return fail(DWARF_ERR_INVALID_ARGUMENT, "%s: interleaved pairs need even strides and pair alignment", r.name);
+  }
+  return hip_status(dwarf::launch_rotary(a, reinterpret_cast<hipStream_t>(stream)), "dwarf_rotary");
+}
+
+static int check_heads(int B, int H, int H_kv, int hd, int dtype, float scale) {
+  if (B < 0 || H < 1 || H_kv < 1) return fail(DWARF_ERR_INVALID_ARGUMENT, "bad sizes B=%d H=%d H_kv=%d", B, H, H_kv);
+  if (H % H_kv) return fail(DWARF_ERR_INVALID_ARGUMENT, "num query heads H=%d must be divisible by KV heads H_kv=%d", H, H_kv);
+  if (hd != dwarf::kHeadDim)
+    return fail(DWARF_ERR_UNSUPPORTED, "linear attention is built for head_dim %d (got %d)", dwarf::kHeadDim, hd);
+  if (!mixer_dtype(dtype)) return fail(DWARF_ERR_INVALID_ARGUMENT, "dtype=%d", dtype);
+  if (!finite_f32(scale)) return fail(DWARF_ERR_INVALID_ARGUMENT, "scale must be finite");
+  return DWARF_OK;
+}
+
+static int check_linear_attention(const dwarf_linear_attention_fwd_args& a) {
+  int rc = check_heads(a.B, a.H, a.H_kv, a.head_dim, a.dtype, a.scale);
+  if (rc) return rc;
+  if (a.N < 0) return fail(DWARF_ERR_INVALID_ARGUMENT, "N=%d", a.N);
+  if (a.N > (1 << 24) || static_cast<double>(a.B) * a.H * (a.N / 64 + 16) >= 0x1p31)
+    return fail(DWARF_ERR_UNSUPPORTED, "N up to 2^24 and B * H * N / 64 below 2^31");
+  if (a.B == 0) return DWARF_OK;
+  if (!a.log_decay) return fail(DWARF_ERR_INVALID_ARGUMENT, "log_decay is NULL");
+  if (a.N == 0) return DWARF_OK;
+  if ((rc = check_rows("q", a.q, a.q_stride, 3, a.dtype))) return rc;
+  if ((rc = check_rows("k", a.k, a.k_stride, 3, a.dtype))) return rc;
+  if ((rc = check_rows("v", a.v, a.v_stride, 3, a.dtype))) return rc;
+  const size_t need = dwarf::linear_attention_states_bytes(a);
+  if (need && (!a.states || a.states_bytes < need || !aligned16(a.states)))
+    return fail(DWARF_ERR_WORKSPACE, "states needs %zu bytes, 16-byte aligned, got %zu", need, a.states_bytes);
+  return DWARF_OK;
+}
+
+int32_t dwarf_linear_attention_segment(int32_t B, int32_t H, int32_t N) {
+  return B > 0 && H > 0 && N > 0 ? dwarf::linear_attention_segment(B, H, N) : 64;
+}
+
+size_t dwarf_linear_attention_states_bytes(const dwarf_linear_attention_fwd_args* args) {
+  return args && args->B > 0 && args->H > 0 && args->N > 0 ? dwarf::linear_attention_states_bytes(*args) : 0;
+}
+
+int dwarf_linear_attention_fwd(const dwarf_linear_attention_fwd_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  int rc = check_linear_attention(*args);
+  if (rc || args->B == 0) return rc ? rc : ok();
+  if (args->N && (rc = check_rows("out", args->out, args->out_stride, 3, args->dtype))) return rc;
+  if (args->N == 0 && !args->final) return ok();
+  return hip_status(dwarf::launch_linear_attention_fwd(*args, reinterpret_cast<hipStream_t>(stream)),
+                    "dwarf_linear_attention_fwd");
+}
+
+size_t dwarf_linear_attention_bwd_workspace_bytes(const dwarf_linear_attention_bwd_args* args) {
+  return args && args->fwd.B > 0 && args->fwd.H > 0 && args->fwd.H_kv > 0 && args->fwd.N >= 0
+             ? dwarf::linear_attention_bwd_workspace(*args) : 0;
+}
+
+int dwarf_linear_attention_bwd(const dwarf_linear_attention_bwd_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_linear_attention_bwd_args& a = *args;
+  int rc = check_linear_attention(a.fwd);
+  if (rc) return rc;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (a.fwd.B == 0) return zero_floats(a.dlog_decay, a.fwd.H, s, "dwarf_linear_attention_bwd");
+  if (a.fwd.N) {
+    if ((rc = check_rows("dout", a.dout, a.dout_stride, 3, a.fwd.dtype))) return rc;
+    if ((rc = check_rows("dq", a.dq, a.dq_stride, 3, a.fwd.dtype))) return rc;
+    if ((rc = check_rows("dk", a.dk, a.dk_stride, 3, a.fwd.dtype))) return rc;
+    if ((rc = check_rows("dv", a.dv, a.dv_stride, 3, a.fwd.dtype))) return rc;
+  }
+  if (a.dlog_decay && a.dfinal && !a.fwd.final)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "dlog_decay with dfinal needs the final state");
+  const size_t need = dwarf::linear_attention_bwd_workspace(a);
+  if (need && (!a.workspace || a.workspace_bytes < need || !aligned16(a.workspace)))
+    return fail(DWARF_ERR_WORKSPACE, "workspace needs %zu bytes, 16-byte aligned, got %zu", need, a.workspace_bytes);
+  return hip_status(dwarf::launch_linear_attention_bwd(a, s), "dwarf_linear_attention_bwd");
+}
+
+int dwarf_linear_attention_step(const dwarf_linear_attention_step_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_linear_attention_step_args& a = *args;
+  int rc = check_heads(a.S, a.H, a.H_kv, a.head_dim, a.dtype, a.scale);
+  if (rc) return rc;
+  if (static_cast<int64_t>(a.S) * a.H >= (int64_t(1) << 30)) return fail(DWARF_ERR_UNSUPPORTED, "S * H must stay below 2^30");
+  if (a.S == 0) return ok();
+  if (!a.log_decay) return fail(DWARF_ERR_INVALID_ARGUMENT, "log_decay is NULL");
+  if ((rc = check_rows("q", a.q, a.q_stride, 2, a.dtype))) return rc;
+  if ((rc = check_rows("k", a.k, a.k_stride, 2, a.dtype))) return rc;
+  if ((rc = check_rows("v", a.v, a.v_stride, 2, a.dtype))) return rc;
+  if ((rc = check_rows("out", a.out, a.out_stride, 2, a.dtype))) return rc;
+  if (a.pool < 0 || (!a.slots && a.pool < a.S))
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "pool=%d holds fewer states than the %d rows", a.pool, a.S);
+  if (a.pool == 0) return fail(DWARF_ERR_INVALID_ARGUMENT, "the pool is empty");
+  if (!a.state || !a.new_state || !aligned16(a.state) || !aligned16(a.new_state))
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "state and new_state must be 16-byte aligned");
+  const int64_t each = static_cast<int64_t>(a.H) * dwarf::kHeadDim * dwarf::kHeadDim;
+  if (a.slot_stride < each || a.slot_stride % 4)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "slot_stride=%lld must be a multiple of 4 and at least %lld",
+                static_cast<long long>(a.slot_stride), static_cast<long long>(each));
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.state), y = reinterpret_cast<uintptr_t>(a.new_state);
+  const uintptr_t span = (static_cast<uintptr_t>(a.pool - 1) * a.slot_stride + each) * sizeof(float);
+  if (x != y && x < y + span && y < x + span)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "state and new_state overlap: give one pool twice, or two apart");
+  return hip_status(dwarf::launch_linear_attention_step(a, reinterpret_cast<hipStream_t>(stream)),
+                    "dwarf_linear_attention_step");
 }
 
 }  // extern "C"

@@ -1,0 +1,574 @@
+// Linear attention with a decay for each head (g = exp(log_decay), at most 1):
+//   S_t = g S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t
+// in chunks of 64 tokens.  With a chunk's n live tokens counted from 0,
+//   o_i = scale [ sum_{j <= i} g^{i-j} (q_i.k_j) v_j + g^{i+1} q_i S_in ]
+//   S_out = g^n S_in + sum_j g^{n-1-j} k_j v_j^T
+// so only non-negative powers of g appear.  The backward is the same sum in
+// other roles: with G the adjoint of the state behind a chunk,
+//   dq_i = scale [ sum_{j <= i} g^{i-j} (do_i.v_j) k_j + g^{i+1} do_i S_in^T ]
+//   dv_j = scale sum_{i >= j} g^{i-j} (k_j.q_i) do_i + g^{n-1-j} k_j G
+//   dk_j = scale sum_{i >= j} g^{i-j} (v_j.do_i) q_i + g^{n-1-j} v_j G^T
+//   G_in = g^n G + scale sum_i g^{i+1} q_i do_i^T
+// and, with tau the token's place in its segment counted from 1,
+//   dlog_decay = sum_segments [ sum_t tau (q.dq - k.dk) + n <S_out, G_out> ],
+// where tau is taken from the segment's middle, so that the two sums, which
+// nearly cancel, stay small.
+//
+// A sequence is cut into segments.  la_local forms each segment's own sum, the
+// scan joins them into the state in front of each segment (behind it, for G),
+// and la_rows walks a segment's chunks with the state in registers.  One
+// segment needs la_rows alone.
+#include "mixer.h"
+#include "mfma.h"
+
+namespace dwarf {
+namespace {
+
+constexpr int kHd = 64;
+constexpr int kChunk = 64;
+constexpr int kLaThreads = 256;
+constexpr int kState = kHd * kHd;
+constexpr int kRowStride = 68;   // LDS rows read as 16-byte vectors
+constexpr int kColStride = 65;   // LDS rows read down the columns: rows 16 apart lie 16 banks apart
+constexpr float kLog2E = 1.4426950408889634f;
+
+struct LaRows {
+  const void* p;
+  int64_t s0, s1, s2;
+};
+struct LaGeom {
+  int B, H, Hkv, N, seg, segs;
+  float scale;
+  const float* log_decay;
+  const int32_t* lengths;
+};
+
+// log2 of the head's decay: values above 0 count as 0, and the smallest keep g^0 = 1 (-inf would make it NaN).
+__device__ __forceinline__ float la_log2_decay(const LaGeom& gm, int h) {
+  const float ld = gm.log_decay[h];
+  const float x = ld > 0.f ? 0.f : ld;
+  return (x < -1e4f ? -1e4f : x) * kLog2E;
+}
+__device__ __forceinline__ float la_power(float lg, int n) { return __builtin_amdgcn_exp2f(lg * static_cast<float>(n)); }
+
+__device__ __forceinline__ int la_length(const LaGeom& gm, int b) {
+  if (!gm.lengths) return gm.N;
+  const int n = gm.lengths[b];
+  return n < 0 ? 0 : n > gm.N ? gm.N : n;
+}
+
+// Sixteen elements from column 16 (threadIdx.x % 4) of row r, zeros where it is not live.
+template <typename T>
+__device__ __forceinline__ void la_load16(const T* row, bool live, float* x) {
+  constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 16 / kPer; ++i) {
+    if (live) {
+      load_vec<T, kPer>(row + i * kPer, x + i * kPer);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[i * kPer + e] = 0.f;
+    }
+  }
+}
+
+// A 64-row tile into LDS rows of STRIDE floats.
+template <typename T, int STRIDE>
+__device__ __forceinline__ void la_tile(const T* base, int64_t stride, int n, float* s) {
+  const int r = threadIdx.x / 4, c = 16 * (threadIdx.x % 4);
+  float x[16];
+  la_load16<T>(base + r * stride + c, r < n, x);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[r * STRIDE + c + i] = x[i];
+}
+
+// The chunk's weights in the state's sum, in LDS: forward g^{n-1-j}, reverse g^{j+1}.
+template <bool REV>
+__device__ __forceinline__ void la_weights(float lg, int n, float* s_w) {
+  if (threadIdx.x < kChunk) {
+    const int j = threadIdx.x;
+    s_w[j] = j < n ? la_power(lg, REV ? j + 1 : n - 1 - j) : 0.f;
+  }
+}
+
+// acc = g^n acc + us sum_j w_j B_j C_j^T; wave w holds rows [16w, 16w + 16).
+template <int BSTRIDE>
+__device__ __forceinline__ void la_update(const float* sB, const float* sC, const float* s_w, float shrink, float us,
+                                          f32x4* acc) {
+  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave, g = l / 16, c = l % 16;
+  f32x4 add[4] = {zero4(), zero4(), zero4(), zero4()};
+#pragma unroll
+  for (int kk = 0; kk < 16; ++kk) {
+    const int j = 16 * g + kk;
+    const float a = sB[j * BSTRIDE + 16 * w + c] * s_w[j];
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct) add[ct] = mfma16_f32(a, sC[j * kColStride + 16 * ct + c], add[ct]);
+  }
+#pragma unroll
+  for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[ct][r] = fmaf(shrink, acc[ct][r], us * add[ct][r]);
+}
+
+// Segment sums: local[b][h][seg] = sum over the segment of us w B C^T.
+template <typename T, bool REV>
+__global__ __launch_bounds__(kLaThreads) void la_local_kernel(LaRows B_, int bh, LaRows C_, int ch, LaGeom gm, float us,
+                                                              float* __restrict__ local) {
+  __shared__ float sB[kChunk * kColStride], sC[kChunk * kColStride], s_w[kChunk];
+  const int seg = blockIdx.x % gm.segs, h = blockIdx.x / gm.segs % gm.H, b = blockIdx.x / gm.segs / gm.H;
+  const int len = la_length(gm, b), t0 = seg * gm.seg;
+  if (t0 >= len) return;
+  const int t1 = t0 + gm.seg < len ? t0 + gm.seg : len;
+  const float lg = la_log2_decay(gm, h);
+  const T* pb = static_cast<const T*>(B_.p) + b * B_.s0 + (h / (gm.H / bh)) * B_.s1;
+  const T* pc = static_cast<const T*>(C_.p) + b * C_.s0 + (h / (gm.H / ch)) * C_.s1;
+  f32x4 acc[4] = {zero4(), zero4(), zero4(), zero4()};
+  const int chunks = (t1 - t0 + kChunk - 1) / kChunk;
+  for (int i = 0; i < chunks; ++i) {
+    const int t = t0 + (REV ? chunks - 1 - i : i) * kChunk;
+    const int n = t1 - t < kChunk ? t1 - t : kChunk;
+    __syncthreads();
+    la_tile<T, kColStride>(pb + t * B_.s2, B_.s2, n, sB);
+    la_tile<T, kColStride>(pc + t * C_.s2, C_.s2, n, sC);
+    la_weights<REV>(lg, n, s_w);
+    __syncthreads();
+    la_update<kColStride>(sB, sC, s_w, la_power(lg, n), us, acc);
+  }
+  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave;
+  float* out = local + static_cast<int64_t>(blockIdx.x) * kState;
+#pragma unroll
+  for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) out[(16 * w + 4 * (l / 16) + r) * kHd + 16 * ct + l % 16] = acc[ct][r];
+}
+
+// Turns the segment sums in place into the state in front of each segment (reverse: the adjoint behind it); a thread
+// owns one element of one head's state.  first: the state that enters (NULL: zero), last: where the one that leaves
+// goes (NULL: nowhere).  Reverse with dot: the boundary terms of dlog_decay, per workgroup.
+constexpr int kScanWgs = kState / kLaThreads;
+constexpr int kScanAhead = 8;
+template <bool REV>
+__global__ __launch_bounds__(kLaThreads) void la_scan_kernel(float* __restrict__ local, const float* __restrict__ first,
+                                                             float* __restrict__ last, LaGeom gm,
+                                                             const float* __restrict__ states,
+                                                             const float* __restrict__ initial,
+                                                             const float* __restrict__ final, float* __restrict__ dot) {
+  __shared__ float s_red[kLaThreads / kWave];
+  const int bh = blockIdx.x / kScanWgs, e = blockIdx.x % kScanWgs * kLaThreads + threadIdx.x;
+  const int b = bh / gm.H, h = bh % gm.H;
+  const int len = la_length(gm, b), active = (len + gm.seg - 1) / gm.seg;
+  const float lg = la_log2_decay(gm, h);
+  const float full = la_power(lg, gm.seg), tail = active ? la_power(lg, len - (active - 1) * gm.seg) : 1.f;
+  float* x = local + static_cast<int64_t>(bh) * gm.segs * kState + e;
+  const float* st = states ? states + static_cast<int64_t>(bh) * gm.segs * kState + e : nullptr;
+  const int64_t at = static_cast<int64_t>(bh) * kState + e;
+  const float mid = 0.5f * static_cast<float>(gm.seg);
+  float m = first ? first[at] : 0.f, sum = 0.f;
+  if (REV && dot && final && active) sum = (static_cast<float>(len - (active - 1) * gm.seg) - mid) * m * final[at];
+  for (int s0 = 0; s0 < active; s0 += kScanAhead) {
+    float in[kScanAhead], sv[kScanAhead];
+    const int cnt = active - s0 < kScanAhead ? active - s0 : kScanAhead;
+#pragma unroll
+    for (int i = 0; i < kScanAhead; ++i) {
+      const int s = REV ? active - 1 - s0 - i : s0 + i;
+      in[i] = i < cnt ? x[static_cast<int64_t>(s) * kState] : 0.f;
+      sv[i] = REV && dot && i < cnt && s > 0 ? st[static_cast<int64_t>(s) * kState] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kScanAhead; ++i) {
+      if (i < cnt) {
+        const int s = REV ? active - 1 - s0 - i : s0 + i;
+        x[static_cast<int64_t>(s) * kState] = m;
+        m = fmaf(s == active - 1 ? tail : full, m, in[i]);
+        if (REV) sum = fmaf(static_cast<float>(gm.seg) * sv[i], m, sum);   // <S in front of s, G in front of s>
+      }
+    }
+  }
+  if (last) last[at] = m;
+  if (REV && dot) {
+    if (initial && active) sum = fmaf(mid * initial[at], m, sum);
+    sum = lanes_sum<kWave>(sum);
+    if (threadIdx.x % kWave == 0) s_red[threadIdx.x / kWave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) dot[blockIdx.x] = ((s_red[0] + s_red[1]) + s_red[2]) + s_red[3];
+  }
+}
+
+// out_i = intra sum_j W_ij (A_i.B_j) C_j + cs W_i A_i M over a segment's chunks, M updated behind each (in front, in
+// reverse).  enter: the state per segment [.. segs ..] or, with one segment, per head (NULL: zero); TRANS: read
+// transposed.  leave: with one segment, where the state that leaves goes.  dot: sum of tau <out_i, D_i>.
+template <typename T, typename TO, bool REV, bool TRANS>
+__global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRows A_, int ah, LaRows B_, int bh, LaRows C_, int ch,
+                                                             LaGeom gm, float intra, float cs, float us,
+                                                             const float* __restrict__ enter, TO* __restrict__ out,
+                                                             int64_t o0, int64_t o1, int64_t o2,
+                                                             float* __restrict__ leave, LaRows D_, int dh,
+                                                             float* __restrict__ dot) {
+  __shared__ __align__(16) float sB[kChunk * kRowStride];
+  __shared__ float sC[kChunk * kColStride], sM[kHd * kColStride], sP[kChunk * kColStride], s_w[kChunk];
+  __shared__ float s_red[kLaThreads / kWave];
+  const int seg = blockIdx.x % gm.segs, h = blockIdx.x / gm.segs % gm.H, b = blockIdx.x / gm.segs / gm.H;
+  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave, g = l / 16, c = l % 16;
+  const int len = la_length(gm, b), t0 = seg * gm.seg;
+  const int tend = t0 + gm.seg < gm.N ? t0 + gm.seg : gm.N;
+  const int t1 = tend < len ? tend : len;
+  TO* po = out + b * o0 + h * o1;
+  // rows behind the sequence are zero
+  for (int i = (t1 > t0 ? t1 : t0) * kHd + threadIdx.x; i < tend * kHd; i += kLaThreads)
+    po[static_cast<int64_t>(i / kHd) * o2 + i % kHd] = from_f32<TO>(0.f);
+  const float lg = la_log2_decay(gm, h);
+  const T* pa = static_cast<const T*>(A_.p) + b * A_.s0 + (h / (gm.H / ah)) * A_.s1;
+  const T* pb = static_cast<const T*>(B_.p) + b * B_.s0 + (h / (gm.H / bh)) * B_.s1;
+  const T* pc = static_cast<const T*>(C_.p) + b * C_.s0 + (h / (gm.H / ch)) * C_.s1;
+  const T* pd = D_.p ? static_cast<const T*>(D_.p) + b * D_.s0 + (h / (gm.H / dh)) * D_.s1 : nullptr;
+  f32x4 M[4];
+  const float* en = enter ? enter + static_cast<int64_t>(blockIdx.x) * kState : nullptr;
+#pragma unroll
+  for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * w + 4 * g + r, j = 16 * ct + c;
+      M[ct][r] = en ? en[TRANS ? j * kHd + i : i * kHd + j] : 0.f;
+    }
+  const float mid = 0.5f * static_cast<float>(gm.seg);
+  float total = 0.f;
+  const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
+  for (int i = 0; i < chunks; ++i) {
+    const int t = t0 + (REV ? chunks - 1 - i : i) * kChunk;
+    const int n = t1 - t < kChunk ? t1 - t : kChunk;
+    __syncthreads();
+    la_tile<T, kRowStride>(pb + t * B_.s2, B_.s2, n, sB);
+    la_tile<T, kColStride>(pc + t * C_.s2, C_.s2, n, sC);
+    la_weights<REV>(lg, n, s_w);
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sM[(16 * w + 4 * g + r) * kColStride + 16 * ct + c] = M[ct][r];
+    // row 16w + c of A, elements [16g, 16g + 16): the k index of step kk is 16g + kk in both operands
+    float a[16];
+    la_load16<T>(pa + (t + 16 * w + c) * A_.s2 + 16 * g, 16 * w + c < n, a);
+    __syncthreads();
+    f32x4 p[4];
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct) {
+      p[ct] = zero4();
+      const float* row = sB + (16 * ct + c) * kRowStride + 16 * g;
+#pragma unroll
+      for (int k4 = 0; k4 < 4; ++k4) {
+        const float4 x = *reinterpret_cast<const float4*>(row + 4 * k4);
+        p[ct] = mfma16_f32(a[4 * k4], x.x, p[ct]);
+        p[ct] = mfma16_f32(a[4 * k4 + 1], x.y, p[ct]);
+        p[ct] = mfma16_f32(a[4 * k4 + 2], x.z, p[ct]);
+        p[ct] = mfma16_f32(a[4 * k4 + 3], x.w, p[ct]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int ii = 16 * w + 4 * g + r, jj = 16 * ct + c, gap = REV ? jj - ii : ii - jj;
+        sP[ii * kColStride + jj] = gap >= 0 ? intra * p[ct][r] * la_power(lg, gap) : 0.f;
+      }
+    }
+    __syncthreads();
+    f32x4 o[4] = {zero4(), zero4(), zero4(), zero4()}, x[4] = {zero4(), zero4(), zero4(), zero4()};
+#pragma unroll
+    for (int kk = 0; kk < 16; ++kk) {
+      const float pk = sP[(16 * w + c) * kColStride + 16 * g + kk];
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        o[ct] = mfma16_f32(pk, sC[(16 * g + kk) * kColStride + 16 * ct + c], o[ct]);
+        x[ct] = mfma16_f32(a[kk], sM[(16 * g + kk) * kColStride + 16 * ct + c], x[ct]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int ii = 16 * w + 4 * g + r;
+      if (ii < n) {
+        const float carry = cs * la_power(lg, REV ? n - 1 - ii : ii + 1);
+        const float tau = static_cast<float>(t - t0 + ii + 1) - mid;
+        float s = 0.f;
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) {
+          const float v = fmaf(carry, x[ct][r], o[ct][r]);
+          po[(t + ii) * o2 + 16 * ct + c] = from_f32<TO>(v);
+          if (dot) s = fmaf(v, to_f32(pd[(t + ii) * D_.s2 + 16 * ct + c]), s);
+        }
+        total = fmaf(tau, s, total);
+      }
+    }
+    la_update<kRowStride>(sB, sC, s_w, la_power(lg, n), us, M);
+  }
+  if (leave) {
+    float* lv = leave + static_cast<int64_t>(blockIdx.x) * kState;
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) lv[(16 * w + 4 * g + r) * kHd + 16 * ct + c] = M[ct][r];
+  }
+  if (dot) {
+    total = lanes_sum<kWave>(total);
+    __syncthreads();
+    if (l == 0) s_red[w] = total;
+    __syncthreads();
+    if (threadIdx.x == 0) dot[blockIdx.x] = ((s_red[0] + s_red[1]) + s_red[2]) + s_red[3];
+  }
+}
+
+// dk or dv of a shared head: the query heads' parts in head order.
+template <typename T>
+__global__ __launch_bounds__(kLaThreads) void la_group_sum(const float* __restrict__ part, T* __restrict__ out, int64_t o0,
+                                                           int64_t o1, int64_t o2, LaGeom gm) {
+  const int group = gm.H / gm.Hkv;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kLaThreads + threadIdx.x;   // four elements of a row
+  const int d = static_cast<int>(i % (kHd / 4)) * 4;
+  const int64_t row = i / (kHd / 4);
+  if (row >= static_cast<int64_t>(gm.B) * gm.Hkv * gm.N) return;
+  const int64_t n = row % gm.N, kv = row / gm.N % gm.Hkv, b = row / gm.N / gm.Hkv;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int q = 0; q < group; ++q) {
+    const float4 x = *reinterpret_cast<const float4*>(part + ((b * gm.H + kv * group + q) * gm.N + n) * kHd + d);
+    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  }
+  const float v[4] = {s.x, s.y, s.z, s.w};
+  store_vec<T, 4>(out + b * o0 + kv * o1 + n * o2 + d, v);
+}
+
+// dlog_decay[h]: the segments' sums over the batch, then the boundary terms; a workgroup per head, fixed order.
+__global__ __launch_bounds__(kLaThreads) void la_dlog_kernel(const float* __restrict__ dq_dot,
+                                                             const float* __restrict__ dk_dot,
+                                                             const float* __restrict__ edge, LaGeom gm,
+                                                             float* __restrict__ dlog) {
+  __shared__ float s_red[kLaThreads / kWave];
+  const int h = blockIdx.x;
+  float t = 0.f;
+  if (dq_dot) {
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(gm.B) * gm.segs; i += kLaThreads) {
+      const int64_t b = i / gm.segs, s = i % gm.segs;
+      if (s * gm.seg < la_length(gm, static_cast<int>(b))) {
+        const int64_t at = (b * gm.H + h) * gm.segs + s;
+        t += dq_dot[at] - dk_dot[at];
+      }
+    }
+  }
+  if (edge)
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(gm.B) * kScanWgs; i += kLaThreads)
+      t += edge[(i / kScanWgs * gm.H + h) * kScanWgs + i % kScanWgs];
+  t = lanes_sum<kWave>(t);
+  if (threadIdx.x % kWave == 0) s_red[threadIdx.x / kWave] = t;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    dlog[h] = gm.log_decay[h] > 0.f ? 0.f : ((s_red[0] + s_red[1]) + s_red[2]) + s_red[3];
+}
+
+// One token of each row: a wave per (row, head) and column quarter... the state streams through once.
+constexpr int kStepThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kStepThreads) void la_step_kernel(dwarf_linear_attention_step_args a) {
+  __shared__ float s_o[kStepThreads / 16][kHd];
+  __shared__ int s_next;
+  const int h = blockIdx.x % a.H, row0 = blockIdx.x / a.H, kv = h / (a.H / a.H_kv);
+  const int c4 = threadIdx.x % 16 * 4, r0 = threadIdx.x / 16 * 4;   // four rows and four columns of the state
+  const int slot = a.slots ? a.slots[row0] : row0;
+  if (slot < 0 || slot >= a.pool) {
+    if (threadIdx.x < kHd)
+      static_cast<T*>(a.out)[row0 * a.out_stride[0] + h * a.out_stride[1] + threadIdx.x] = from_f32<T>(0.f);
+    return;
+  }
+  LaGeom gm;
+  gm.log_decay = a.log_decay;
+  const float decay = la_power(la_log2_decay(gm, h), 1);
+  // the first row of a slot takes the slot's later rows after it, in order
+  auto next_of = [&](int from) {
+    __syncthreads();
+    if (threadIdx.x == 0) s_next = a.S;
+    __syncthreads();
+    for (int i = from + static_cast<int>(threadIdx.x); i < a.S; i += kStepThreads)
+      if (a.slots[i] == slot) {
+        atomicMin(&s_next, i);
+        break;
+      }
+    __syncthreads();
+    return s_next;
+  };
+  if (a.slots && next_of(0) < row0) return;   // uniform
+  const int64_t at = slot * a.slot_stride + static_cast<int64_t>(h) * kState;
+  float4 st[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) st[i] = *reinterpret_cast<const float4*>(a.state + at + (r0 + i) * kHd + c4);
+  for (int row = row0; row < a.S; row = a.slots ? next_of(row + 1) : a.S) {
+    const T* q = static_cast<const T*>(a.q) + row * a.q_stride[0] + h * a.q_stride[1];
+    const T* k = static_cast<const T*>(a.k) + row * a.k_stride[0] + kv * a.k_stride[1];
+    const T* v = static_cast<const T*>(a.v) + row * a.v_stride[0] + kv * a.v_stride[1];
+    float qv[4], kx[4], vx[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+    load_vec<T, 4>(q + r0, qv);
+    load_vec<T, 4>(k + r0, kx);
+    load_vec<T, 4>(v + c4, vx);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      st[i].x = fmaf(decay, st[i].x, kx[i] * vx[0]);
+      st[i].y = fmaf(decay, st[i].y, kx[i] * vx[1]);
+      st[i].z = fmaf(decay, st[i].z, kx[i] * vx[2]);
+      st[i].w = fmaf(decay, st[i].w, kx[i] * vx[3]);
+      o[0] = fmaf(qv[i], st[i].x, o[0]);
+      o[1] = fmaf(qv[i], st[i].y, o[1]);
+      o[2] = fmaf(qv[i], st[i].z, o[2]);
+      o[3] = fmaf(qv[i], st[i].w, o[3]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_o[threadIdx.x / 16][c4 + i] = o[i];
+    __syncthreads();
+    if (threadIdx.x < kHd) {
+      float t = 0.f;
+#pragma unroll
+      for (int i = 0; i < kStepThreads / 16; ++i) t += s_o[i][threadIdx.x];
+      static_cast<T*>(a.out)[row * a.out_stride[0] + h * a.out_stride[1] + threadIdx.x] = from_f32<T>(a.scale * t);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(a.new_state + at + (r0 + i) * kHd + c4) = st[i];
+}
+
+int la_segment(int64_t B, int64_t H, int64_t N) {
+  for (int seg = 256; seg > kChunk; seg /= 2)
+    if (B * H * ((N + seg - 1) / seg) >= 512) return seg;
+  return kChunk;
+}
+
+LaGeom la_geom(const dwarf_linear_attention_fwd_args& a) {
+  LaGeom gm;
+  gm.B = a.B; gm.H = a.H; gm.Hkv = a.H_kv; gm.N = a.N;
+  gm.seg = la_segment(a.B, a.H, a.N);
+  gm.segs = (a.N + gm.seg - 1) / gm.seg;
+  gm.scale = a.scale;
+  gm.log_decay = a.log_decay;
+  gm.lengths = a.lengths;
+  return gm;
+}
+
+LaRows la_operand(const void* p, const int64_t* s) { return LaRows{p, s[0], s[1], s[2]}; }
+
+template <typename T>
+void la_fwd_typed(const dwarf_linear_attention_fwd_args& a, const LaGeom& gm, hipStream_t stream) {
+  const LaRows q = la_operand(a.q, a.q_stride), k = la_operand(a.k, a.k_stride), v = la_operand(a.v, a.v_stride);
+  const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * gm.segs), block(kLaThreads);
+  const float* enter = a.initial;
+  if (gm.segs > 1) {
+    hipLaunchKernelGGL((la_local_kernel<T, false>), grid, block, 0, stream, k, gm.Hkv, v, gm.Hkv, gm, 1.f, a.states);
+    enter = a.states;
+  }
+  if (gm.segs != 1)
+    hipLaunchKernelGGL((la_scan_kernel<false>), dim3(gm.B * gm.H * kScanWgs), block, 0, stream, a.states, a.initial,
+                       a.final, gm, nullptr, nullptr, nullptr, nullptr);
+  if (gm.segs == 0) return;
+  hipLaunchKernelGGL((la_rows_kernel<T, T, false, false>), grid, block, 0, stream, q, gm.H, k, gm.Hkv, v, gm.Hkv, gm,
+                     gm.scale, gm.scale, 1.f, enter, static_cast<T*>(a.out), a.out_stride[0], a.out_stride[1],
+                     a.out_stride[2], gm.segs == 1 ? a.final : nullptr, LaRows{}, 1, nullptr);
+}
+
+// Workspace of the backward, in floats: the adjoints per segment, the dlog_decay sums, the shared heads' parts.
+struct LaBwdSpace {
+  size_t adjoint, dq_dot, dk_dot, edge, dk_part, dv_part, total;
+};
+LaBwdSpace la_bwd_space(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm) {
+  const size_t wgs = static_cast<size_t>(gm.B) * gm.H * gm.segs, rows = static_cast<size_t>(gm.B) * gm.H * gm.N * kHd;
+  const bool shared = gm.H != gm.Hkv;
+  auto pad = [](size_t n) { return (n + 63) / 64 * 64; };
+  LaBwdSpace s;
+  size_t at = 0;
+  s.adjoint = at; at += wgs * kState;
+  s.dq_dot = at; at += a.dlog_decay ? pad(wgs) : 0;
+  s.dk_dot = at; at += a.dlog_decay ? pad(wgs) : 0;
+  s.edge = at; at += a.dlog_decay ? pad(static_cast<size_t>(gm.B) * gm.H * kScanWgs) : 0;
+  s.dk_part = at; at += shared ? rows : 0;
+  s.dv_part = at; at += shared ? rows : 0;
+  s.total = at;
+  return s;
+}
+
+template <typename T>
+void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hipStream_t stream) {
+  const dwarf_linear_attention_fwd_args& f = a.fwd;
+  const LaRows q = la_operand(f.q, f.q_stride), k = la_operand(f.k, f.k_stride), v = la_operand(f.v, f.v_stride);
+  const LaRows dout = la_operand(a.dout, a.dout_stride);
+  const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * gm.segs), block(kLaThreads);
+  const LaBwdSpace sp = la_bwd_space(a, gm);
+  float* ws = static_cast<float*>(a.workspace);
+  const bool dlog = a.dlog_decay != nullptr;
+  float *adj = ws + sp.adjoint, *dq_dot = dlog ? ws + sp.dq_dot : nullptr, *dk_dot = dlog ? ws + sp.dk_dot : nullptr;
+  float* edge = dlog ? ws + sp.edge : nullptr;
+  const bool joined = gm.segs != 1 || a.dinitial || dlog;
+  if (joined) {
+    if (gm.segs)
+      hipLaunchKernelGGL((la_local_kernel<T, true>), grid, block, 0, stream, q, gm.H, dout, gm.H, gm, gm.scale, adj);
+    hipLaunchKernelGGL((la_scan_kernel<true>), dim3(gm.B * gm.H * kScanWgs), block, 0, stream, adj, a.dfinal, a.dinitial,
+                       gm, f.states, f.initial, f.final, edge);
+  }
+  if (gm.segs) {
+    hipLaunchKernelGGL((la_rows_kernel<T, T, false, true>), grid, block, 0, stream, dout, gm.H, v, gm.Hkv, k, gm.Hkv, gm,
+                       gm.scale, gm.scale, 1.f, gm.segs > 1 ? f.states : f.initial, static_cast<T*>(a.dq),
+                       a.dq_stride[0], a.dq_stride[1], a.dq_stride[2], nullptr, q, gm.H, dq_dot);
+    const float* enter = joined ? adj : a.dfinal;
+    if (gm.H == gm.Hkv) {
+      hipLaunchKernelGGL((la_rows_kernel<T, T, true, false>), grid, block, 0, stream, k, gm.Hkv, q, gm.H, dout, gm.H, gm,
+                         gm.scale, 1.f, gm.scale, enter, static_cast<T*>(a.dv), a.dv_stride[0], a.dv_stride[1],
+                         a.dv_stride[2], nullptr, LaRows{}, 1, nullptr);
+      hipLaunchKernelGGL((la_rows_kernel<T, T, true, true>), grid, block, 0, stream, v, gm.Hkv, dout, gm.H, q, gm.H, gm,
+                         gm.scale, 1.f, gm.scale, enter, static_cast<T*>(a.dk), a.dk_stride[0], a.dk_stride[1],
+                         a.dk_stride[2], nullptr, k, gm.Hkv, dk_dot);
+    } else {
+      float *pk = ws + sp.dk_part, *pv = ws + sp.dv_part;
+      const int64_t s1 = static_cast<int64_t>(gm.N) * kHd, s0 = s1 * gm.H;
+      hipLaunchKernelGGL((la_rows_kernel<T, float, true, false>), grid, block, 0, stream, k, gm.Hkv, q, gm.H, dout, gm.H,
+                         gm, gm.scale, 1.f, gm.scale, enter, pv, s0, s1, kHd, nullptr, LaRows{}, 1, nullptr);
+      hipLaunchKernelGGL((la_rows_kernel<T, float, true, true>), grid, block, 0, stream, v, gm.Hkv, dout, gm.H, q, gm.H,
+                         gm, gm.scale, 1.f, gm.scale, enter, pk, s0, s1, kHd, nullptr, k, gm.Hkv, dk_dot);
+      const int64_t quads = static_cast<int64_t>(gm.B) * gm.Hkv * gm.N * (kHd / 4);
+      const dim3 sums(static_cast<unsigned>((quads + kLaThreads - 1) / kLaThreads));
+      hipLaunchKernelGGL((la_group_sum<T>), sums, block, 0, stream, pv, static_cast<T*>(a.dv), a.dv_stride[0],
+                         a.dv_stride[1], a.dv_stride[2], gm);
+      hipLaunchKernelGGL((la_group_sum<T>), sums, block, 0, stream, pk, static_cast<T*>(a.dk), a.dk_stride[0],
+                         a.dk_stride[1], a.dk_stride[2], gm);
+    }
+  }
+  if (dlog)
+    hipLaunchKernelGGL(la_dlog_kernel, dim3(gm.H), block, 0, stream, gm.segs ? dq_dot : nullptr, dk_dot, edge, gm,
+                       a.dlog_decay);
+}
+
+}  // namespace
+
+int linear_attention_segment(int B, int H, int N) { return la_segment(B, H, N); }
+
+size_t linear_attention_states_bytes(const dwarf_linear_attention_fwd_args& a) {
+  const LaGeom gm = la_geom(a);
+  return gm.segs > 1 ? static_cast<size_t>(gm.B) * gm.H * gm.segs * kState * sizeof(float) : 0;
+}
+
+size_t linear_attention_bwd_workspace(const dwarf_linear_attention_bwd_args& a) {
+  return la_bwd_space(a, la_geom(a.fwd)).total * sizeof(float);
+}
+
+hipError_t launch_linear_attention_fwd(const dwarf_linear_attention_fwd_args& a, hipStream_t stream) {
+  const LaGeom gm = la_geom(a);
+  if (a.dtype == DWARF_F32) la_fwd_typed<float>(a, gm, stream);
+  else if (a.dtype == DWARF_F16) la_fwd_typed<f16>(a, gm, stream);
+  else la_fwd_typed<bf16>(a, gm, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_linear_attention_bwd(const dwarf_linear_attention_bwd_args& a, hipStream_t stream) {
+  const LaGeom gm = la_geom(a.fwd);
+  if (a.fwd.dtype == DWARF_F32) la_bwd_typed<float>(a, gm, stream);
+  else if (a.fwd.dtype == DWARF_F16) la_bwd_typed<f16>(a, gm, stream);
+  else la_bwd_typed<bf16>(a, gm, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_linear_attention_step(const dwarf_linear_attention_step_args& a, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(a.S) * a.H), block(kStepThreads);
+  if (a.dtype == DWARF_F32) hipLaunchKernelGGL((la_step_kernel<float>), grid, block, 0, stream, a);
+  else if (a.dtype == DWARF_F16) hipLaunchKernelGGL((la_step_kernel<f16>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((la_step_kernel<bf16>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace dwarf

@@ -1,0 +1,259 @@
+"""Linear attention with a decay for each head, on MI355X: prompts, training and single tokens.
+
+With g = exp(log_decay[h]) <= 1 a head keeps one 64 x 64 state,
+
+    S_t = g S_{t-1} + k_t v_t^T,    o_t = scale q_t S_t,
+
+the matrix form of ``causal_ema_scan``'s recurrence, whose serving state does
+not grow with the context.  ``linear_attention`` runs whole sequences in chunks
+on the matrix cores (with gradients for q, k, v, log_decay and the state that
+enters); ``linear_attention_step`` runs one token of each running sequence
+against a pool of states.  States and sums are fp32; q, k, v are bf16, fp16 or
+fp32; head_dim is 64, the query heads a multiple of the K/V heads.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _launch, _lib
+from .dsqg import HEAD_DIM, _kernel_rows
+
+
+def segment_tokens(B: int, H: int, N: int) -> int:
+    """Tokens of a segment (dwarf_linear_attention_segment): shorter ones where long ones leave CUs idle."""
+    for seg in (256, 128):
+        if B * H * -(-N // seg) >= 512:
+            return seg
+    return 64
+
+
+def states_shape(B: int, H: int, N: int) -> tuple[int, ...]:
+    """Shape of the states the forward keeps for the backward: one per segment, none for a single segment."""
+    segs = -(-N // segment_tokens(B, H, N)) if B * H * N else 0
+    return (B, H, segs if segs > 1 else 0, HEAD_DIM, HEAD_DIM)
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _decay(log_decay: torch.Tensor) -> torch.Tensor:
+    return log_decay.detach().reshape(-1).float().contiguous()
+
+
+def _fill(a: _lib.LinearAttentionFwdArgs, q, k, v, log_decay, initial, lengths, scale: float, states) -> None:
+    B, H, N, hd = q.shape
+    a.B, a.H, a.H_kv, a.N, a.head_dim = B, H, k.shape[1], N, hd
+    a.dtype, a.scale = _launch.DTYPES[q.dtype], scale
+    a.q, a.q_stride = q.data_ptr(), q.stride()
+    a.k, a.k_stride = k.data_ptr(), k.stride()
+    a.v, a.v_stride = v.data_ptr(), v.stride()
+    a.log_decay, a.lengths, a.initial = log_decay.data_ptr(), _ptr(lengths), _ptr(initial)
+    a.states, a.states_bytes = states.data_ptr(), states.numel() * 4
+
+
+def _operands(q, k, v, log_decay, initial, lengths):
+    q, k, v = _kernel_rows(q), _kernel_rows(k), _kernel_rows(v)
+    return (q, k, v, _decay(log_decay), None if initial is None else initial.detach().contiguous(),
+            None if lengths is None else lengths.to(torch.int32).contiguous())
+
+
+def attention_forward(q, k, v, log_decay, initial, lengths, scale: float, want_state: bool
+                      ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor]:
+    """Raw launches: (out in token-major memory, the final state or None, the segments' states)."""
+    q, k, v, decay, initial, lengths = _operands(q, k, v, log_decay, initial, lengths)
+    B, H, N, hd = q.shape
+    out = _launch.token_major(B, H, N, hd, q)
+    state = torch.empty((B, H, hd, hd), device=q.device, dtype=torch.float32) if want_state else None
+    states = torch.empty(states_shape(B, H, N), device=q.device, dtype=torch.float32)
+    a = _lib.LinearAttentionFwdArgs()
+    _fill(a, q, k, v, decay, initial, lengths, scale, states)
+    a.out, a.out_stride, a.final = out.data_ptr(), out.stride(), _ptr(state)
+    _launch.launch("dwarf_linear_attention_fwd", a, q.device)
+    return out, state, states
+
+
+def attention_backward(dout, dstate, q, k, v, log_decay, initial, lengths, scale: float, states, state,
+                       need_decay: bool, need_initial: bool):
+    """Raw launches: (dq, dk, dv in token-major memory, dlog_decay [H] or None, dinitial or None)."""
+    q, k, v, decay, initial, lengths = _operands(q, k, v, log_decay, initial, lengths)
+    B, H, N, hd = q.shape
+    dout = _kernel_rows(dout.to(q.dtype))
+    dstate = None if dstate is None else dstate.float().contiguous()
+    a = _lib.LinearAttentionBwdArgs()
+    _fill(a.fwd, q, k, v, decay, initial, lengths, scale, states)
+    a.fwd.final = _ptr(state)
+    a.dout, a.dout_stride, a.dfinal = dout.data_ptr(), dout.stride(), _ptr(dstate)
+    dq = _launch.token_major(B, H, N, hd, q)
+    dk, dv = (_launch.token_major(B, k.shape[1], N, hd, q) for _ in range(2))
+    a.dq, a.dq_stride = dq.data_ptr(), dq.stride()
+    a.dk, a.dk_stride = dk.data_ptr(), dk.stride()
+    a.dv, a.dv_stride = dv.data_ptr(), dv.stride()
+    dlog = torch.empty(H, device=q.device, dtype=torch.float32) if need_decay else None
+    dinitial = torch.empty((B, H, hd, hd), device=q.device, dtype=torch.float32) if need_initial else None
+    a.dlog_decay, a.dinitial = _ptr(dlog), _ptr(dinitial)
+    ws = _launch.workspace("dwarf_linear_attention_bwd_workspace_bytes", a, q.device)
+    if ws is not None:
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _launch.launch("dwarf_linear_attention_bwd", a, q.device)
+    return dq, dk, dv, dlog, dinitial
+
+
+class _LinearAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, initial, lengths, scale: float, want_state: bool):
+        if torch.compiler.is_compiling():
+            out, state, states = torch.ops.dwarf.linear_attention_fwd(q, k, v, log_decay, initial, lengths, scale,
+                                                                      want_state)
+        else:
+            out, state, states = attention_forward(q, k, v, log_decay, initial, lengths, scale, want_state)
+        kept = state if want_state and log_decay.requires_grad else None   # for the decay's gradient
+        ctx.save_for_backward(q, k, v, log_decay, initial, lengths, states, kept)
+        ctx.scale, ctx.want_state = scale, want_state
+        ctx.set_materialize_grads(False)
+        return (out, state) if want_state else out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dstate=None):
+        q, k, v, log_decay, initial, lengths, states, state = ctx.saved_tensors
+        if dout is None and dstate is None:
+            return (None,) * 8
+        if dout is None:
+            dout = torch.zeros_like(q)
+        need = ctx.needs_input_grad
+        backward = torch.ops.dwarf.linear_attention_bwd if torch.compiler.is_compiling() else attention_backward
+        dq, dk, dv, dlog, dinitial = backward(dout, dstate, q, k, v, log_decay, initial, lengths, ctx.scale, states,
+                                              state, need[3], need[4])
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
+                dlog.view(log_decay.shape).to(log_decay.dtype) if need[3] else None,
+                dinitial if need[4] else None, None, None, None)
+
+
+def _check_scale(scale) -> float:
+    scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    return scale
+
+
+def _check_heads(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, dims: str) -> None:
+    H, Hkv = q.shape[1], k.shape[1]
+    if k.shape != v.shape or q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ValueError(f"k and v must share a shape and q's dtype {q.dtype}; got {tuple(k.shape)} {k.dtype}, "
+                         f"{tuple(v.shape)} {v.dtype}")
+    if q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+        raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)} ({dims})")
+    if Hkv < 1 or H < 1 or H % Hkv:
+        raise ValueError(f"num query heads H={H} must be divisible by KV heads H_kv={Hkv}")
+    if log_decay.numel() != H or not log_decay.is_floating_point():
+        raise ValueError(f"log_decay must hold one floating value per head ({H}), got {tuple(log_decay.shape)} {log_decay.dtype}")
+    _launch.check_dtype("q", q)
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, *,
+                     scale: float | None = None, initial_state: torch.Tensor | None = None,
+                     lengths: torch.Tensor | None = None, return_state: bool = False):
+    """Decayed linear attention over whole sequences: out [B,H,N,64] in q's dtype ([B,N,H,64] memory), and with
+    ``return_state`` the state [B,H,64,64] fp32 behind each sequence's last token.
+
+    q [B,H,N,64], k and v [B,H_kv,N,64]; log_decay [H], values above 0 count as 0 (their gradient is 0);
+    scale 1/8 by default; initial_state [B,H,64,64] fp32; lengths [B] integers, clamped to [0, N]: the tokens of
+    each sequence, behind which nothing is used and the output is zero."""
+    scale = _check_scale(scale)
+    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
+        raise ValueError(f"q, k and v must be [B,H,N,{HEAD_DIM}], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    _check_heads(q, k, v, log_decay, "[B,H,N,64]")
+    B, H, N, hd = q.shape
+    if initial_state is not None and (tuple(initial_state.shape) != (B, H, hd, hd) or initial_state.dtype != torch.float32):
+        raise ValueError(f"initial_state must be fp32 [{B},{H},{hd},{hd}], got {tuple(initial_state.shape)} "
+                         f"{initial_state.dtype}")
+    if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"lengths must be [{B}] int32 or int64, got {tuple(lengths.shape)} {lengths.dtype}")
+    _launch.check_device(q, k=k, v=v, log_decay=log_decay, initial_state=initial_state, lengths=lengths)
+    if hd != HEAD_DIM:
+        raise RuntimeError(f"linear attention is built for head_dim {HEAD_DIM}, got {hd}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
+        return _LinearAttentionFn.apply(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
+    forward = torch.ops.dwarf.linear_attention_fwd if torch.compiler.is_compiling() else attention_forward
+    out, state, _ = forward(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
+    return (out, state) if return_state else out
+
+
+def _pool_ok(t: torch.Tensor, H: int) -> bool:
+    return (t.ndim == 4 and t.dtype == torch.float32 and tuple(t.shape[1:]) == (H, HEAD_DIM, HEAD_DIM)
+            and (t.shape[0] == 1 or (t.stride(0) >= H * HEAD_DIM * HEAD_DIM and t.stride(0) % 4 == 0))
+            and t.stride()[1:] == (HEAD_DIM * HEAD_DIM, HEAD_DIM, 1) and t.data_ptr() % 16 == 0)
+
+
+def attention_step(q, k, v, log_decay, state, new_state, slots, scale: float, out=None) -> torch.Tensor:
+    """Raw launch of one step: out [S,H,64]; new_state None writes the pool itself."""
+    q, k, v = _kernel_rows(q), _kernel_rows(k), _kernel_rows(v)
+    decay = _decay(log_decay)
+    if slots is not None:
+        slots = slots.to(torch.int32).contiguous()
+    S, H, hd = q.shape
+    if out is None:
+        out = torch.empty((S, H, hd), device=q.device, dtype=q.dtype)
+    a = _lib.LinearAttentionStepArgs()
+    a.S, a.H, a.H_kv, a.pool, a.head_dim = S, H, k.shape[1], state.shape[0], hd
+    a.dtype, a.scale = _launch.DTYPES[q.dtype], scale
+    a.q, a.q_stride = q.data_ptr(), q.stride()
+    a.k, a.k_stride = k.data_ptr(), k.stride()
+    a.v, a.v_stride = v.data_ptr(), v.stride()
+    a.log_decay, a.slots = decay.data_ptr(), _ptr(slots)
+    a.state = state.data_ptr()
+    a.new_state = a.state if new_state is None else new_state.data_ptr()
+    a.slot_stride = state.stride(0) if state.shape[0] > 1 else H * hd * hd
+    a.out, a.out_stride = out.data_ptr(), out.stride()
+    _launch.launch("dwarf_linear_attention_step", a, q.device)
+    return out
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                          state: torch.Tensor, *, slots: torch.Tensor | None = None,
+                          new_state: torch.Tensor | None = None, scale: float | None = None,
+                          out: torch.Tensor | None = None) -> torch.Tensor:
+    """One token of each of S rows: q [S,H,64], k and v [S,H_kv,64]; returns out [S,H,64].
+
+    state [P,H,64,64] fp32 is a pool of sequences' states, each slot contiguous.  Row s works on slot slots[s]
+    (slot s where slots is None); its new state is written to the same slot of ``new_state``, or of ``state`` itself
+    where that is None.  Slots outside [0, P) mark rows that pad the batch: no state is touched, their output
+    is zero.  Rows that share a slot are consecutive tokens of its sequence, in row order.  ``out``: where to write
+    the result.  No gradients."""
+    scale = _check_scale(scale)
+    if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
+        raise ValueError(f"q, k and v must be [S,H,{HEAD_DIM}], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    _check_heads(q, k, v, log_decay, "[S,H,64]")
+    S, H, hd = q.shape
+    if hd != HEAD_DIM:
+        raise RuntimeError(f"linear attention is built for head_dim {HEAD_DIM}, got {hd}")
+    for name, t in (("state", state), ("new_state", new_state)):
+        if t is not None and not _pool_ok(t, H):
+            raise ValueError(f"{name} must be an fp32 [P,{H},{hd},{hd}] pool with contiguous, 16-byte aligned slots, got "
+                             f"{tuple(t.shape)} {t.dtype} strides {t.stride()}")
+    if new_state is not None and (new_state.shape != state.shape
+                                  or (state.shape[0] > 1 and new_state.stride() != state.stride())):
+        raise ValueError("new_state must have state's shape and strides")
+    if slots is None and state.shape[0] < S:
+        raise ValueError(f"a pool of {state.shape[0]} states does not hold the {S} rows")
+    if slots is not None and (tuple(slots.shape) != (S,) or slots.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"slots must be [{S}] int32 or int64, got {tuple(slots.shape)} {slots.dtype}")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or _kernel_rows(out) is not out):
+        raise ValueError(f"out must be [{S},{H},{hd}] {q.dtype} with 16-byte aligned rows")
+    _launch.check_device(q, k=k, v=v, log_decay=log_decay, state=state, new_state=new_state, slots=slots, out=out)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+        raise RuntimeError("linear_attention_step has no gradients: call it under torch.no_grad(), or linear_attention")
+    if S and not state.shape[0]:
+        raise ValueError("the pool is empty")
+    if torch.compiler.is_compiling():
+        if out is not None:
+            raise RuntimeError("out= is for eager calls and captured graphs, not for torch.compile")
+        if new_state is None:
+            return torch.ops.dwarf.linear_attention_step_(q, k, v, log_decay, state, slots, scale)
+        return torch.ops.dwarf.linear_attention_step(q, k, v, log_decay, state, new_state, slots, scale)
+    return attention_step(q, k, v, log_decay, state, new_state, slots, scale, out)

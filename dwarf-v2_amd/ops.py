@@ -6,9 +6,12 @@
 ``dwarf::npci_fwd``, ``dwarf::npci_bwd``, ``dwarf::packet_pool_fwd``,
 ``dwarf::packet_pool_bwd``, ``dwarf::packet_fwd``, ``dwarf::packet_bwd``,
 ``dwarf::normalize_probes``,
-``dwarf::linear_wgrad``, ``dwarf::dsqg_block_fwd`` and ``dwarf::dsqg_block_bwd`` are
+``dwarf::linear_wgrad``, ``dwarf::dsqg_block_fwd``, ``dwarf::dsqg_block_bwd``,
+``dwarf::layer_norm_fwd``, ``dwarf::layer_norm_bwd``, ``dwarf::rotary``,
+``dwarf::linear_attention_fwd``, ``dwarf::linear_attention_bwd``,
+``dwarf::linear_attention_step`` and ``dwarf::linear_attention_step_`` are
 custom ops with fake (shape-only) implementations, so ``torch.compile`` traces
-the DSQG, EMA, phase-probe, NPCI and InterferencePacket autograd Functions
+the DSQG, EMA, phase-probe, NPCI, InterferencePacket and mixer autograd Functions
 without graph breaks (the trainer
 compiles the model, train:1083).  The real
 implementations normalise layouts (unit head-dim stride, 16-byte rows,
@@ -28,9 +31,12 @@ import torch
 from . import block as _block
 from . import dsqg as _dsqg
 from . import ema as _ema
+from . import linattn as _linattn
+from . import norm as _norm
 from . import npci as _npci
 from . import packet as _packet
 from . import probe as _probe
+from . import rotary as _rotary
 
 Tensor = torch.Tensor
 
@@ -324,3 +330,114 @@ def packet_bwd(x: Tensor, alpha: Tensor, weight: Tensor, gate: Tensor, pooled: T
 def _packet_bwd_fake(x, alpha, weight, gate, pooled, state, ms, dpacket, floor, ceiling):
     return (x.new_empty(x.shape), x.new_empty((alpha.numel(),), dtype=torch.float32),
             x.new_empty((alpha.numel(),), dtype=torch.float32), x.new_empty(x.shape, dtype=gate.dtype))
+
+
+# ---- layer norm ------------------------------------------------------------------------------
+def _or_empty(t: Optional[Tensor], like: Tensor) -> Tensor:
+    return t if t is not None else like.new_empty((0,), dtype=torch.float32)
+
+
+@torch.library.custom_op("dwarf::layer_norm_fwd", mutates_args=())
+def layer_norm_fwd(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, eps: float) -> Tensor:
+    """y, contiguous, of x's dtype."""
+    return _norm.norm_forward(x, weight, bias, groups, eps)
+
+
+@layer_norm_fwd.register_fake
+def _layer_norm_fwd_fake(x, weight, bias, groups, eps):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("dwarf::layer_norm_bwd", mutates_args=())
+def layer_norm_bwd(dy: Tensor, x: Tensor, weight: Optional[Tensor], groups: int, eps: float, need_dx: bool,
+                   need_dw: bool, need_db: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """(dx of x's dtype, dweight, dbias fp32 [groups * D]); empty [0] where not needed."""
+    dx, dw, db = _norm.norm_backward(dy, x, weight, groups, eps, need_dx, need_dw, need_db)
+    return (dx if need_dx else x.new_empty((0,)), _or_empty(dw, x), _or_empty(db, x))
+
+
+@layer_norm_bwd.register_fake
+def _layer_norm_bwd_fake(dy, x, weight, groups, eps, need_dx, need_dw, need_db):
+    n, f32 = groups * x.shape[-1], torch.float32
+    return (x.new_empty(x.shape if need_dx else (0,)), x.new_empty((n if need_dw else 0,), dtype=f32),
+            x.new_empty((n if need_db else 0,), dtype=f32))
+
+
+# ---- rotary positions ------------------------------------------------------------------------
+def _token_major_fake(t, B, H, N, D):
+    return t.new_empty((B, N, H, D)).transpose(1, 2)
+
+
+@torch.library.custom_op("dwarf::rotary", mutates_args=())
+def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, turns: Tensor, interleaved: bool, inverse: bool,
+           magnitude: float) -> tuple[Tensor, Tensor]:
+    """(q, k) turned, in token-major memory; k empty [0] where there is none."""
+    q_out, k_out = _rotary.rotate(q, k, positions, turns, interleaved, inverse, magnitude)
+    return q_out, k_out if k_out is not None else q.new_empty((0,))
+
+
+@rotary.register_fake
+def _rotary_fake(q, k, positions, turns, interleaved, inverse, magnitude):
+    return _token_major_fake(q, *q.shape), _token_major_fake(k, *k.shape) if k is not None else q.new_empty((0,))
+
+
+# ---- decayed linear attention ----------------------------------------------------------------
+@torch.library.custom_op("dwarf::linear_attention_fwd", mutates_args=())
+def linear_attention_fwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, initial: Optional[Tensor],
+                         lengths: Optional[Tensor], scale: float, want_state: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """(out in token-major memory, the final state or empty [0], the segments' states for the backward)."""
+    out, state, states = _linattn.attention_forward(q, k, v, log_decay, initial, lengths, scale, want_state)
+    return out, _or_empty(state, q), states
+
+
+@linear_attention_fwd.register_fake
+def _linear_attention_fwd_fake(q, k, v, log_decay, initial, lengths, scale, want_state):
+    B, H, N, hd = q.shape
+    f32 = torch.float32
+    return (_token_major_fake(q, B, H, N, hd), q.new_empty((B, H, hd, hd) if want_state else (0,), dtype=f32),
+            q.new_empty(_linattn.states_shape(B, H, N), dtype=f32))
+
+
+@torch.library.custom_op("dwarf::linear_attention_bwd", mutates_args=())
+def linear_attention_bwd(dout: Tensor, dstate: Optional[Tensor], q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor,
+                         initial: Optional[Tensor], lengths: Optional[Tensor], scale: float, states: Tensor,
+                         state: Optional[Tensor], need_decay: bool, need_initial: bool
+                         ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(dq, dk, dv in token-major memory, dlog_decay [H] and dinitial fp32, each empty [0] where not needed)."""
+    dq, dk, dv, dlog, dinitial = _linattn.attention_backward(dout, dstate, q, k, v, log_decay, initial, lengths, scale,
+                                                             states, state, need_decay, need_initial)
+    return dq, dk, dv, _or_empty(dlog, q), _or_empty(dinitial, q)
+
+
+@linear_attention_bwd.register_fake
+def _linear_attention_bwd_fake(dout, dstate, q, k, v, log_decay, initial, lengths, scale, states, state, need_decay,
+                               need_initial):
+    B, H, N, hd = q.shape
+    f32 = torch.float32
+    return (_token_major_fake(q, B, H, N, hd), _token_major_fake(q, *k.shape), _token_major_fake(q, *k.shape),
+            q.new_empty((H if need_decay else 0,), dtype=f32),
+            q.new_empty((B, H, hd, hd) if need_initial else (0,), dtype=f32))
+
+
+@torch.library.custom_op("dwarf::linear_attention_step", mutates_args=("new_state",))
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, new_state: Tensor,
+                          slots: Optional[Tensor], scale: float) -> Tensor:
+    """One token of each row, the states going from one pool to another; out [S,H,64]."""
+    return _linattn.attention_step(q, k, v, log_decay, state, new_state, slots, scale)
+
+
+@linear_attention_step.register_fake
+def _linear_attention_step_fake(q, k, v, log_decay, state, new_state, slots, scale):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("dwarf::linear_attention_step_", mutates_args=("state",))
+def linear_attention_step_(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor,
+                           slots: Optional[Tensor], scale: float) -> Tensor:
+    """One token of each row, the pool updated in place; out [S,H,64]."""
+    return _linattn.attention_step(q, k, v, log_decay, state, None, slots, scale)
+
+
+@linear_attention_step_.register_fake
+def _linear_attention_step__fake(q, k, v, log_decay, state, slots, scale):
+    return q.new_empty(q.shape)

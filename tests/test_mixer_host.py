@@ -1,0 +1,285 @@
+"""Host side of the mixer's operators, without a GPU: the header's exports and layouts, refusals of bad calls, the
+plan of rotary positions, the segment rule, fake shapes."""
+
+import ctypes
+import math
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+from tests.conftest import ROOT
+
+HEADER = os.path.join(ROOT, "include", "dwarf_mixer.h")
+STRUCTS = {"dwarf_layer_norm_fwd_args": "LayerNormFwdArgs", "dwarf_layer_norm_bwd_args": "LayerNormBwdArgs",
+           "dwarf_rotary_args": "RotaryArgs", "dwarf_linear_attention_fwd_args": "LinearAttentionFwdArgs",
+           "dwarf_linear_attention_bwd_args": "LinearAttentionBwdArgs",
+           "dwarf_linear_attention_step_args": "LinearAttentionStepArgs"}
+
+
+@pytest.fixture(scope="module")
+def lib(pkg):
+    return pkg._lib.load()
+
+
+def test_header_exports_and_layout(pkg, lib, tmp_path):
+    names = sorted(set(re.findall(r"^(?:int|int32_t|size_t)\s+(dwarf_\w+)\s*\(", open(HEADER).read(), re.M)))
+    assert sorted(pkg._lib.MIXER_SYMBOLS) == names
+    assert all(hasattr(lib, n) for n in names)
+    if shutil.which("gcc") is None:
+        pytest.skip("gcc not available")
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "dwarf_mixer.h"', "int main(void) {",
+             'printf("f16 %d\\n", DWARF_F16);']
+    for cname, pyname in STRUCTS.items():
+        lines.append(f'printf("{cname} sizeof %zu\\n", sizeof({cname}));')
+        lines += [f'printf("{cname} {f} %zu\\n", offsetof({cname}, {f}));' for f, _ in getattr(pkg._lib, pyname)._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-I", os.path.dirname(HEADER), str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()
+    assert out[0] == f"f16 {pkg._lib.DWARF_F16}"
+    for line in out[1:]:
+        cname, field, value = line.split()
+        struct = getattr(pkg._lib, STRUCTS[cname])
+        assert (ctypes.sizeof(struct) if field == "sizeof" else getattr(struct, field).offset) == int(value), line
+
+
+P = 0x10000   # an aligned address that no refused call reads
+
+
+def test_layer_norm_entry_points_refuse(pkg, lib):
+    L = pkg._lib
+    bad = L.DWARF_ERR_INVALID_ARGUMENT
+    assert lib.dwarf_layer_norm_fwd(None, None) == bad and lib.dwarf_layer_norm_bwd(None, None) == bad
+    a = L.LayerNormBwdArgs()
+    f = a.fwd
+    f.rows, f.groups, f.D, f.dtype, f.eps = 6, 1, 64, L.DWARF_BF16, 1e-5
+    assert lib.dwarf_layer_norm_fwd(ctypes.byref(f), None) == bad           # x is NULL
+    f.x, f.x_stride = P, (64, 64)
+    assert lib.dwarf_layer_norm_fwd(ctypes.byref(f), None) == bad           # y is NULL
+    f.x = P + 1
+    assert lib.dwarf_layer_norm_fwd(ctypes.byref(f), None) == bad           # between elements
+    f.x = P
+    for name, value in (("D", 0), ("groups", 0), ("rows", -1), ("dtype", 7), ("eps", -1.0), ("eps", math.nan),
+                        ("eps", math.inf)):
+        keep = getattr(f, name)
+        setattr(f, name, value)
+        assert lib.dwarf_layer_norm_fwd(ctypes.byref(f), None) == bad, name
+        assert lib.dwarf_layer_norm_bwd_workspace_bytes(ctypes.byref(a)) == 0
+        setattr(f, name, keep)
+    f.groups = 65536
+    assert lib.dwarf_layer_norm_fwd(ctypes.byref(f), None) == L.DWARF_ERR_UNSUPPORTED
+    f.groups, f.D = 1, (1 << 24) + 1
+    assert lib.dwarf_layer_norm_fwd(ctypes.byref(f), None) == L.DWARF_ERR_UNSUPPORTED
+    f.D = 64
+    assert lib.dwarf_layer_norm_bwd(ctypes.byref(a), None) == bad           # dy is NULL
+    a.dy, a.dy_stride, a.dweight = P, (64, 64), P
+    need = lib.dwarf_layer_norm_bwd_workspace_bytes(ctypes.byref(a))
+    assert need > 0
+    assert lib.dwarf_layer_norm_bwd(ctypes.byref(a), None) == L.DWARF_ERR_WORKSPACE
+    a.workspace, a.workspace_bytes = P, need - 1
+    assert lib.dwarf_layer_norm_bwd(ctypes.byref(a), None) == L.DWARF_ERR_WORKSPACE
+    f.rows = 0
+    assert lib.dwarf_layer_norm_fwd(ctypes.byref(f), None) == L.DWARF_OK    # nothing to do
+
+
+def test_rotary_entry_point_refuses(pkg, lib):
+    L = pkg._lib
+    bad = L.DWARF_ERR_INVALID_ARGUMENT
+    assert lib.dwarf_rotary(None, None) == bad
+    a = L.RotaryArgs()
+    a.B, a.H, a.H_kv, a.N, a.D, a.pairs, a.position_bytes, a.magnitude = 1, 2, 2, 4, 64, 32, 8, 1.0
+    assert lib.dwarf_rotary(ctypes.byref(a), None) == bad                   # no positions
+    a.positions = a.turns = P
+    assert lib.dwarf_rotary(ctypes.byref(a), None) == bad                   # q is NULL
+    a.q = a.q_out = P
+    a.q_stride = a.q_out_stride = (512, 256, 64, 2)
+    assert lib.dwarf_rotary(ctypes.byref(a), None) == bad                   # strided elements
+    a.q_stride = (512, 256, 65, 1)
+    a.q_out_stride, a.interleaved = (512, 256, 64, 1), 1
+    assert lib.dwarf_rotary(ctypes.byref(a), None) == bad                   # odd strides, pairs side by side
+    assert b"even strides" in lib.dwarf_last_error()
+    a.q_stride = (512, 256, 64, 1)
+    for name, value in (("D", 63), ("D", 0), ("pairs", 0), ("pairs", 33), ("dtype", 3), ("position_bytes", 2),
+                        ("magnitude", math.nan), ("H", 0), ("N", -1)):
+        keep = getattr(a, name)
+        setattr(a, name, value)
+        assert lib.dwarf_rotary(ctypes.byref(a), None) == bad, name
+        setattr(a, name, keep)
+    a.k, a.H_kv = P, 0
+    assert lib.dwarf_rotary(ctypes.byref(a), None) == bad
+    a.H_kv, a.B, a.N = 2, 1 << 20, 1 << 20
+    assert lib.dwarf_rotary(ctypes.byref(a), None) == L.DWARF_ERR_UNSUPPORTED
+    a.N = 0
+    assert lib.dwarf_rotary(ctypes.byref(a), None) == L.DWARF_OK
+
+
+def test_linear_attention_entry_points_refuse(pkg, lib):
+    L = pkg._lib
+    bad = L.DWARF_ERR_INVALID_ARGUMENT
+    assert lib.dwarf_linear_attention_fwd(None, None) == bad and lib.dwarf_linear_attention_bwd(None, None) == bad
+    assert lib.dwarf_linear_attention_step(None, None) == bad
+    a = L.LinearAttentionBwdArgs()
+    f = a.fwd
+    f.B, f.H, f.H_kv, f.N, f.head_dim, f.scale = 2, 4, 2, 100, 64, 0.125
+    rows, kv = (100 * 256, 64, 256, 1), (100 * 128, 64, 128, 1)
+    assert lib.dwarf_linear_attention_fwd(ctypes.byref(f), None) == bad     # log_decay is NULL
+    f.log_decay = P
+    assert lib.dwarf_linear_attention_fwd(ctypes.byref(f), None) == bad     # q is NULL
+    f.q = f.k = f.v = f.out = P
+    f.q_stride = f.out_stride = rows
+    f.k_stride = f.v_stride = kv
+    need = lib.dwarf_linear_attention_states_bytes(ctypes.byref(f))
+    assert need == 2 * 4 * 2 * 64 * 64 * 4                                  # two segments of 64
+    assert lib.dwarf_linear_attention_fwd(ctypes.byref(f), None) == L.DWARF_ERR_WORKSPACE
+    f.states, f.states_bytes = P, need - 1
+    assert lib.dwarf_linear_attention_fwd(ctypes.byref(f), None) == L.DWARF_ERR_WORKSPACE
+    f.states_bytes = need
+    for name, value, want in (("H_kv", 3, bad), ("H_kv", 0, bad), ("head_dim", 128, L.DWARF_ERR_UNSUPPORTED),
+                              ("dtype", 9, bad), ("scale", math.inf, bad), ("N", -1, bad), ("B", -1, bad),
+                              ("N", (1 << 24) + 1, L.DWARF_ERR_UNSUPPORTED), ("q", P + 8, bad)):
+        keep = getattr(f, name)
+        setattr(f, name, value)
+        assert lib.dwarf_linear_attention_fwd(ctypes.byref(f), None) == want, name
+        assert lib.dwarf_linear_attention_bwd(ctypes.byref(a), None) == want, name
+        setattr(f, name, keep)
+    assert lib.dwarf_linear_attention_bwd(ctypes.byref(a), None) == bad     # dout is NULL
+    a.dout = a.dq = a.dk = a.dv = a.dlog_decay = a.dfinal = P
+    a.dout_stride = a.dq_stride = rows
+    a.dk_stride = a.dv_stride = kv
+    assert lib.dwarf_linear_attention_bwd(ctypes.byref(a), None) == bad     # the final state is needed
+    a.dfinal = None
+    assert lib.dwarf_linear_attention_bwd(ctypes.byref(a), None) == L.DWARF_ERR_WORKSPACE
+    s = L.LinearAttentionStepArgs()
+    s.S, s.H, s.H_kv, s.pool, s.head_dim, s.scale = 3, 4, 2, 5, 64, 0.125
+    s.q = s.k = s.v = s.out = s.log_decay = s.state = s.new_state = P
+    s.q_stride = s.out_stride = (256, 64, 1)
+    s.k_stride = s.v_stride = (128, 64, 1)
+    s.slot_stride = 4 * 4096
+    for name, value in (("slot_stride", 4 * 4096 - 4), ("slot_stride", 4 * 4096 + 2), ("pool", 2), ("pool", -1),
+                        ("state", P + 4), ("new_state", P + 16), ("new_state", None), ("q", None), ("H_kv", 3),
+                        ("scale", math.nan), ("S", -1)):
+        keep = getattr(s, name)
+        setattr(s, name, value)
+        assert lib.dwarf_linear_attention_step(ctypes.byref(s), None) == bad, name
+        setattr(s, name, keep)
+    s.S = 0
+    assert lib.dwarf_linear_attention_step(ctypes.byref(s), None) == L.DWARF_OK
+
+
+def test_segment_rule_is_the_librarys(pkg, lib):
+    for B in (1, 2, 3, 15, 20, 64):
+        for H in (1, 6, 8, 32):
+            for N in (1, 63, 64, 65, 777, 2048, 8192, 65536):
+                seg = pkg.linattn.segment_tokens(B, H, N)
+                assert seg == lib.dwarf_linear_attention_segment(B, H, N)
+                a = pkg._lib.LinearAttentionFwdArgs()
+                a.B, a.H, a.H_kv, a.N, a.head_dim = B, H, H, N, 64
+                want = pkg.linattn.states_shape(B, H, N)
+                assert lib.dwarf_linear_attention_states_bytes(ctypes.byref(a)) == 4 * math.prod(want)
+
+
+def _qkv(S=(2, 4, 5, 64), Hkv=2, dtype=torch.bfloat16):
+    kv = (S[0], Hkv, *S[2:])
+    return torch.zeros(S, dtype=dtype), torch.zeros(kv, dtype=dtype), torch.zeros(kv, dtype=dtype)
+
+
+def test_python_calls_refuse(pkg):
+    q, k, v = _qkv()
+    lg = torch.zeros(4)
+    with pytest.raises(RuntimeError, match="device tensors"):
+        pkg.linear_attention(q, k, v, lg)
+    for args, kw in (((q[0], k, v, lg), {}), ((q, k, v[:, :1], lg), {}), ((q, k.float(), v, lg), {}),
+                     ((q, k[:, :, :3], v[:, :, :3], lg), {}), ((q[:, :3], k, v, lg[:3]), {}), ((q, k, v, lg[:2]), {}),
+                     ((q, k, v, lg.int()), {}), ((q.double(), k.double(), v.double(), lg), {}),
+                     ((q, k, v, lg), dict(scale=math.inf)), ((q, k, v, lg), dict(initial_state=torch.zeros(2, 2, 64, 64))),
+                     ((q, k, v, lg), dict(initial_state=torch.zeros(2, 4, 64, 64).bfloat16())),
+                     ((q, k, v, lg), dict(lengths=torch.zeros(3, dtype=torch.int32))),
+                     ((q, k, v, lg), dict(lengths=torch.zeros(2)))):
+        with pytest.raises(ValueError):
+            pkg.linear_attention(*args, **kw)
+    q, k, v = (x[:, :, 0] for x in (q, k, v))
+    pool = torch.zeros(3, 4, 64, 64)
+    with pytest.raises(RuntimeError, match="device tensors"):
+        pkg.linear_attention_step(q, k, v, lg, pool)
+    for state, kw in ((pool.bfloat16(), {}), (pool[:, :2], {}), (pool[:1], {}), (pool.transpose(2, 3), {}),
+                      (pool, dict(new_state=torch.zeros(4, 4, 64, 64))), (pool, dict(slots=torch.zeros(2))),
+                      (pool, dict(slots=torch.zeros(3, dtype=torch.int32))), (pool, dict(scale=math.nan)),
+                      (pool, dict(out=torch.zeros(2, 4, 64)))):
+        with pytest.raises(ValueError):
+            pkg.linear_attention_step(q, k, v, lg, state, **kw)
+    x = torch.zeros(3, 4, 8)
+    with pytest.raises(RuntimeError, match="device tensors"):
+        pkg.layer_norm(x)
+    for args in ((x, torch.zeros(4)), (x, torch.zeros(3, 8)), (x, torch.zeros(8), torch.zeros(4, 8)),
+                 (x, torch.zeros(8, dtype=torch.int32)), (x, None, None, -1.0), (x, None, None, math.nan), (x.double(),),
+                 (x.long(),), (torch.zeros(()),), (torch.zeros(3, 0),), (x, torch.zeros(3, 4, 8))):
+        with pytest.raises(ValueError):
+            pkg.layer_norm(*args)
+    plan = pkg.rotary_plan(64, device="cpu")
+    q, k, _ = _qkv()
+    pos = torch.arange(5)
+    with pytest.raises(RuntimeError, match="device tensors"):
+        pkg.rotary_embed(q, k, pos, plan)
+    for args in ((q[0], k, pos, plan), (q, k[:, :, :3], pos, plan), (q, k.float(), pos, plan), (q, k, pos[:4], plan),
+                 (q, k, pos.float(), plan), (q, k, pos.expand(3, 5), plan), (q[..., :32], k[..., :32], pos, plan),
+                 (q.double(), None, pos, plan), (q[..., :63], None, pos, pkg.rotary_plan(32, device="cpu"))):
+        with pytest.raises(ValueError):
+            pkg.rotary_embed(*args)
+
+
+def test_rotary_plan_frequencies(pkg):
+    """Turns are the nearest 2^-64 fractions, and each scaling gives its formula's frequencies."""
+    plan = pkg.rotary_plan(64, device="cpu")
+    f = 10000.0 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64)
+    assert torch.equal(plan.inverse_frequencies, f)
+    got = torch.tensor([(t % 2 ** 64) / 2 ** 64 for t in plan.turns.tolist()], dtype=torch.float64) * 2 * math.pi
+    torch.testing.assert_close(got, f, rtol=4e-16, atol=1e-18)   # three float64 roundings
+    lin = pkg.rotary_plan(64, scaling="linear", factor=4.0, device="cpu")
+    assert torch.equal(lin.inverse_frequencies, f / 4)
+    ntk = pkg.rotary_plan(64, scaling="base", factor=8.0, device="cpu").inverse_frequencies
+    assert float(ntk[0]) == 1.0
+    assert abs(float(ntk[-1] * 8 / f[-1]) - 1) < 1e-12   # the slowest pair is stretched by the factor
+    bands = pkg.rotary_plan(64, scaling="bands", factor=16.0, original_length=2048, device="cpu").inverse_frequencies
+    turns = 2048 * f / (2 * math.pi)
+    assert torch.equal(bands[turns >= 32], f[turns >= 32])
+    slow = turns <= 1
+    assert slow.any() and torch.allclose(bands[slow], f[slow] / 16, rtol=1e-15)
+    assert bool((bands[1:] < bands[:-1]).all())
+    own = pkg.rotary_plan(6, inverse_frequencies=torch.tensor([1.0, -0.5, 0.0]), device="cpu")
+    assert own.turns.tolist()[2] == 0 and own.turns.tolist()[1] < 0
+    assert own.to("cpu").turns.tolist() == own.turns.tolist()
+    for args, kw in (((7,), {}), ((0,), {}), ((64,), dict(scaling="other")), ((64,), dict(factor=0.0)),
+                     ((64,), dict(base=-1.0)), ((64,), dict(scaling="bands", factor=2.0)),
+                     ((64,), dict(scaling="bands", original_length=2048, fast_turns=1.0, slow_turns=2.0)),
+                     ((2,), dict(scaling="base", factor=2.0)), ((64,), dict(magnitude=math.nan)),
+                     ((64,), dict(inverse_frequencies=torch.ones(3))),
+                     ((2,), dict(inverse_frequencies=torch.tensor([math.inf])))):
+        with pytest.raises(ValueError):
+            pkg.rotary_plan(*args, device="cpu", **kw)
+
+
+def test_fake_shapes(pkg):
+    m = torch.device("meta")
+    q, k = torch.empty(2, 4, 300, 64, device=m, dtype=torch.bfloat16), torch.empty(2, 2, 300, 64, device=m, dtype=torch.bfloat16)
+    lg = torch.empty(4, device=m)
+    out, state, states = torch.ops.dwarf.linear_attention_fwd(q, k, k, lg, None, None, 0.125, True)
+    assert out.shape == q.shape and out.transpose(1, 2).is_contiguous() and state.shape == (2, 4, 64, 64)
+    assert states.shape == pkg.linattn.states_shape(2, 4, 300) and states.dtype == torch.float32
+    g = torch.ops.dwarf.linear_attention_bwd(out, None, q, k, k, lg, state, None, 0.125, states, None, True, False)
+    assert [tuple(x.shape) for x in g] == [tuple(q.shape), tuple(k.shape), tuple(k.shape), (4,), (0,)]
+    a, b = torch.ops.dwarf.rotary(q, k, torch.empty(300, device=m, dtype=torch.int64),
+                                  torch.empty(32, device=m, dtype=torch.int64), False, False, 1.0)
+    assert a.shape == q.shape and b.shape == k.shape and b.transpose(1, 2).is_contiguous()
+    x = torch.empty(3, 4, 8, device=m, dtype=torch.float16)
+    w = torch.empty(4, 8, device=m)
+    y = torch.ops.dwarf.layer_norm_fwd(x, w, w, 4, 1e-5)
+    assert y.shape == x.shape and y.dtype == torch.float16
+    dx, dw, db = torch.ops.dwarf.layer_norm_bwd(y, x, w, 4, 1e-5, True, True, False)
+    assert dx.shape == x.shape and dw.shape == (32,) and db.shape == (0,)
+    pool = torch.empty(5, 4, 64, 64, device=m)
+    o = torch.ops.dwarf.linear_attention_step(q[:, :, 0], k[:, :, 0], k[:, :, 0], lg, pool, pool.clone(), None, 0.125)
+    assert o.shape == (2, 4, 64)
