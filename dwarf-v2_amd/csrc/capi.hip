@@ -945,6 +945,14 @@ static int check_heads(int B, int H, int H_kv, int hd, int dtype, float scale) {
   return DWARF_OK;
 }
 
+// A chunk's 64 rows are addressed with 32-bit byte offsets, and the rows behind a sequence's last one lie behind the
+// end of its memory: rows may not overlap.
+static int check_chunk_rows(const char* name, int N, int64_t row_stride) {
+  if (N > 1 && (row_stride < dwarf::kHeadDim || row_stride >= (int64_t(1) << 22)))
+    return fail(DWARF_ERR_UNSUPPORTED, "%s row stride %lld outside [64, 2^22) elements", name, static_cast<long long>(row_stride));
+  return DWARF_OK;
+}
+
 static int check_linear_attention(const dwarf_linear_attention_fwd_args& a) {
   int rc = check_heads(a.B, a.H, a.H_kv, a.head_dim, a.dtype, a.scale);
   if (rc) return rc;
@@ -957,6 +965,10 @@ static int check_linear_attention(const dwarf_linear_attention_fwd_args& a) {
   if ((rc = check_rows("q", a.q, a.q_stride, 3, a.dtype))) return rc;
   if ((rc = check_rows("k", a.k, a.k_stride, 3, a.dtype))) return rc;
   if ((rc = check_rows("v", a.v, a.v_stride, 3, a.dtype))) return rc;
+  if ((rc = check_chunk_rows("q", a.N, a.q_stride[2])) || (rc = check_chunk_rows("k", a.N, a.k_stride[2])) ||
+      (rc = check_chunk_rows("v", a.N, a.v_stride[2])))
+    return rc;
+  if (a.initial && !aligned16(a.initial)) return fail(DWARF_ERR_INVALID_ARGUMENT, "initial must be 16-byte aligned");
   const size_t need = dwarf::linear_attention_states_bytes(a);
   if (need && (!a.states || a.states_bytes < need || !aligned16(a.states)))
     return fail(DWARF_ERR_WORKSPACE, "states needs %zu bytes, 16-byte aligned, got %zu", need, a.states_bytes);
@@ -998,6 +1010,7 @@ int dwarf_linear_attention_bwd(const dwarf_linear_attention_bwd_args* args, dwar
     if ((rc = check_rows("dq", a.dq, a.dq_stride, 3, a.fwd.dtype))) return rc;
     if ((rc = check_rows("dk", a.dk, a.dk_stride, 3, a.fwd.dtype))) return rc;
     if ((rc = check_rows("dv", a.dv, a.dv_stride, 3, a.fwd.dtype))) return rc;
+    if ((rc = check_chunk_rows("dout", a.fwd.N, a.dout_stride[2]))) return rc;
   }
   if (a.dlog_decay && a.dfinal && !a.fwd.final)
     return fail(DWARF_ERR_INVALID_ARGUMENT, "dlog_decay with dfinal needs the final state");

@@ -18,8 +18,11 @@
 // scan joins them into the state in front of each segment (behind it, for G),
 // and la_rows walks a segment's chunks with the state in registers.  One
 // segment needs la_rows alone.
-#include "mixer.h"
+#include <type_traits>
+
+#include "gather.h"
 #include "mfma.h"
+#include "mixer.h"
 
 namespace dwarf {
 namespace {
@@ -30,7 +33,6 @@ constexpr int kLaThreads = 256;
 constexpr int kState = kHd * kHd;
 constexpr int kRowStride = 68;   // LDS rows read as 16-byte vectors
 constexpr int kColStride = 65;   // LDS rows read down the columns: rows 16 apart lie 16 banks apart
-constexpr float kLog2E = 1.4426950408889634f;
 
 struct LaRows {
   const void* p;
@@ -47,7 +49,7 @@ struct LaGeom {
 __device__ __forceinline__ float la_log2_decay(const LaGeom& gm, int h) {
   const float ld = gm.log_decay[h];
   const float x = ld > 0.f ? 0.f : ld;
-  return (x < -1e4f ? -1e4f : x) * kLog2E;
+  return (x < -1e4f ? -1e4f : x) * kLog2e;
 }
 __device__ __forceinline__ float la_power(float lg, int n) { return __builtin_amdgcn_exp2f(lg * static_cast<float>(n)); }
 
@@ -312,6 +314,516 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRows A_, int ah, 
   }
 }
 
+// ---- bf16 --------------------------------------------------------------------------------------
+// The same sums on v_mfma_f32_16x16x32_bf16.  Products of two inputs are exact in fp32; what the kernel forms itself
+// (weighted scores, the state, weighted keys) is split into bf16 parts before it meets the matrix cores, two parts
+// (2^-17 relative) where the result is rounded to bf16 anyway and three (2^-24, fp32 itself) where it goes into the
+// state, so that no intermediate rounding is coarser than the output's.  The sums are bound by memory, and the matrix
+// cores have the room: 64 instructions a wave and chunk at most, of which 40 are the split parts.
+//
+// LDS holds tiles as 64 rows of 128 bytes; 16-byte piece p of row r sits at piece p ^ tile_key(r), so that both the
+// row reads (16 rows, one piece each) and the transposed reads (8 rows, two pieces each) take every bank once.
+// Scores are formed transposed (rows: the other side's tokens): a lane then holds four consecutive tokens of one own
+// row, which is the next product's operand as it stands.  Its tokens are slots in the order 4 g + e, 16 + 4 g + e of
+// each 32 (g the lane's group of 16), and a transposed read of four rows gives the other operand in the same order.
+// Results come out transposed too: a lane holds four consecutive elements of one row.
+constexpr int kTileBytes = kChunk * kHd * 2;
+
+__device__ __forceinline__ int tile_key(int r) { return ((r >> 1) & 3) * 2 + ((r >> 3) & 1); }
+__device__ __forceinline__ int tile_at(int r, int byte) { return r * 128 + ((((byte >> 4) ^ tile_key(r)) << 4) | (byte & 15)); }
+
+// A chunk's rows on their way through registers: rows tid / 8 and tid / 8 + 32, piece tid % 8.
+struct TileRegs {
+  uint4 x[2];
+};
+__device__ __forceinline__ void tile_fetch(TileRegs& t, const bf16* base, int64_t stride, int n) {
+  const int ld = static_cast<int>(stride) * 2;
+  const __amdgpu_buffer_rsrc_t r = rows_rsrc(base, ld, n, 128);   // rows behind the n live ones read zeros
+  const uint32_t off = (threadIdx.x >> 3) * static_cast<uint32_t>(ld) + (threadIdx.x & 7) * 16;
+  t.x[0] = buf_load16(r, off);
+  t.x[1] = buf_load16(r, off + 32u * static_cast<uint32_t>(ld));
+}
+__device__ __forceinline__ void tile_put(const TileRegs& t, char* s) {
+  const int at = tile_at(threadIdx.x >> 3, (threadIdx.x & 7) * 16);   // rows 32 apart share a key
+  *reinterpret_cast<uint4*>(s + at) = t.x[0];
+  *reinterpret_cast<uint4*>(s + at + 32 * 128) = t.x[1];
+}
+// Row r, elements 32 ks + 8 g + [0, 8).
+__device__ __forceinline__ bf16x8 tile_row(const char* s, int r, int ks) {
+  return bf16x8_from_bits(*reinterpret_cast<const uint4*>(s + tile_at(r, 64 * ks + 16 * ((threadIdx.x % kWave) / 16))));
+}
+// Row r, elements in slot order: 32 ks + 4 g + [0, 4) and 32 ks + 16 + 4 g + [0, 4).
+__device__ __forceinline__ bf16x8 tile_row_slots(const char* s, int r, int ks) {
+  const int b = 64 * ks + 8 * ((threadIdx.x % kWave) / 16);
+  const uint2 lo = *reinterpret_cast<const uint2*>(s + tile_at(r, b)), hi = *reinterpret_cast<const uint2*>(s + tile_at(r, b + 32));
+  return bf16x8_from_bits(uint4{lo.x, lo.y, hi.x, hi.y});
+}
+// Column 16 ct + lane % 16 of the 32 rows from 32 ks, in slot order.
+__device__ __forceinline__ bf16x8 tile_column(const char* s, int ct, int ks) {
+  typedef short i16x8 __attribute__((ext_vector_type(8)));
+  const int l = threadIdx.x % kWave, r = 32 * ks + 4 * (l / 16) + (l % 16) / 4, byte = 32 * ct + 8 * (l % 4);
+  const i16x4 lo = lds_read_tr16(s + tile_at(r, byte)), hi = lds_read_tr16(s + tile_at(r + 16, byte));
+  const i16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+__device__ __forceinline__ void unpack8(bf16x8 v, float* x) {
+  const uint4 w = __builtin_bit_cast(uint4, v);
+  x[0] = bf16_lo(w.x); x[1] = bf16_hi(w.x); x[2] = bf16_lo(w.y); x[3] = bf16_hi(w.y);
+  x[4] = bf16_lo(w.z); x[5] = bf16_hi(w.z); x[6] = bf16_lo(w.w); x[7] = bf16_hi(w.w);
+}
+// Two values' bf16 parts: the pair's high parts, and what they leave in x.
+__device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
+  const uint32_t h = pack_bf16x2(a, b);
+  a -= bf16_lo(h);
+  b -= bf16_hi(h);
+  return h;
+}
+template <int PARTS>
+__device__ __forceinline__ void split8(float* x, bf16x8* parts) {
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    uint4 w;
+    if (p + 1 < PARTS) {
+      w.x = split_pair(x[0], x[1]); w.y = split_pair(x[2], x[3]);
+      w.z = split_pair(x[4], x[5]); w.w = split_pair(x[6], x[7]);
+    } else {
+      w = uint4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+    }
+    parts[p] = bf16x8_from_bits(w);
+  }
+}
+
+// The wave's 16 rows of the state (rows 16 w + 4 g + r, column 16 ct + c) into two LDS tiles of the transposed state:
+// its high parts, and behind them what those leave.
+__device__ __forceinline__ void state_put(const f32x4* M, char* s) {
+  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave, g = l / 16, c = l % 16;
+#pragma unroll
+  for (int ct = 0; ct < 4; ++ct) {
+    float x[4] = {M[ct][0], M[ct][1], M[ct][2], M[ct][3]};
+    const int at = tile_at(16 * ct + c, 2 * (16 * w + 4 * g));
+    *reinterpret_cast<uint2*>(s + at) = uint2{split_pair(x[0], x[1]), split_pair(x[2], x[3])};
+    *reinterpret_cast<uint2*>(s + kTileBytes + at) = uint2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+  }
+}
+
+// Weights of the slots' tokens in the state's sum: forward us g^{n-1-j}, reverse us g^{j+1}.
+template <bool REV>
+__device__ __forceinline__ void slot_weights(float lg, int n, float us, float* wt) {
+  const int g = (threadIdx.x % kWave) / 16;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int j = 32 * (i / 8) + (i & 4 ? 16 : 0) + 4 * g + (i & 3);
+    const int p = REV ? j + 1 : n - 1 - j;
+    wt[i] = us * la_power(lg, p < 0 ? 0 : p);   // tokens behind the last are zero rows
+  }
+}
+
+// M = shrink M + sum_j wt_j X_j Y_j^T for the wave's 16 columns of X and all of Y; y holds Y's columns.
+__device__ __forceinline__ void state_update(const char* sX, const bf16x8 (*y)[4], const float* wt, float shrink, f32x4* M) {
+  const int w = threadIdx.x / kWave;
+#pragma unroll
+  for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) M[ct][r] *= shrink;
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    float x[8];
+    unpack8(tile_column(sX, w, ks), x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= wt[8 * ks + e];
+    bf16x8 parts[3];
+    split8<3>(x, parts);
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) M[ct] = mfma16_bf16(parts[p], y[ks][ct], M[ct]);
+  }
+}
+
+__device__ __forceinline__ void state_load(const float* en, bool trans, f32x4* M) {
+  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave, g = l / 16, c = l % 16;
+#pragma unroll
+  for (int ct = 0; ct < 4; ++ct) {
+    const int i = 16 * w + 4 * g, j = 16 * ct + c;
+    if (!en) M[ct] = zero4();
+    else if (trans) M[ct] = *reinterpret_cast<const f32x4*>(en + j * kHd + i);
+    else
+#pragma unroll
+      for (int r = 0; r < 4; ++r) M[ct][r] = en[(i + r) * kHd + j];
+  }
+}
+__device__ __forceinline__ void state_store(const f32x4* M, float* out) {
+  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave, g = l / 16, c = l % 16;
+#pragma unroll
+  for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) out[(16 * w + 4 * g + r) * kHd + 16 * ct + c] = M[ct][r];
+}
+
+// Four consecutive elements of a row.
+__device__ __forceinline__ void put4(bf16* p, const float* v) {
+  *reinterpret_cast<uint2*>(p) = uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+}
+__device__ __forceinline__ void put4(float* p, const float* v) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// Work item of a workgroup: the query heads of a shared K/V head next to each other on one XCD, then the segments.
+struct LaItem {
+  int b, h, seg;
+  int64_t at;   // (b, h, seg) in the state arrays
+};
+__device__ __forceinline__ LaItem la_item(const LaGeom& gm) {
+  const int group = gm.H / gm.Hkv;
+  const int i = xcd_remap(blockIdx.x, gridDim.x);
+  LaItem it;
+  const int hq = i % group, rest = i / group;
+  it.seg = rest % gm.segs;
+  const int kv = rest / gm.segs % gm.Hkv;
+  it.b = rest / gm.segs / gm.Hkv;
+  it.h = kv * group + hq;
+  it.at = (static_cast<int64_t>(it.b) * gm.H + it.h) * gm.segs + it.seg;
+  return it;
+}
+__device__ __forceinline__ const bf16* la_rows_of(const LaRows& x, int heads, const LaGeom& gm, const LaItem& it) {
+  return static_cast<const bf16*>(x.p) + it.b * x.s0 + (it.h / (gm.H / heads)) * x.s1;
+}
+
+template <typename TO>
+__device__ __forceinline__ void la_zero_rows(TO* po, int64_t o2, int from, int to) {
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = from * (kHd / 4) + threadIdx.x; i < to * (kHd / 4); i += kLaThreads)
+    put4(po + static_cast<int64_t>(i / (kHd / 4)) * o2 + i % (kHd / 4) * 4, zero);
+}
+
+__device__ __forceinline__ float workgroup_sum(float x, float* s_red) {   // in thread 0
+  x = lanes_sum<kWave>(x);
+  __syncthreads();
+  if (threadIdx.x % kWave == 0) s_red[threadIdx.x / kWave] = x;
+  __syncthreads();
+  return ((s_red[0] + s_red[1]) + s_red[2]) + s_red[3];
+}
+
+// Segment sums (see la_local_kernel).
+template <bool REV>
+__global__ __launch_bounds__(kLaThreads) void la_local_bf16(LaRows X_, int xh, LaRows Y_, int yh, LaGeom gm, float us,
+                                                            float* __restrict__ local) {
+  __shared__ __align__(16) char smem[4 * kTileBytes];   // two chunks of X and Y
+  const LaItem it = la_item(gm);
+  const int len = la_length(gm, it.b), t0 = it.seg * gm.seg;
+  if (t0 >= len) return;
+  const int t1 = t0 + gm.seg < len ? t0 + gm.seg : len;
+  const float lg = la_log2_decay(gm, it.h), full = la_power(lg, kChunk);
+  const bf16 *px = la_rows_of(X_, xh, gm, it), *py = la_rows_of(Y_, yh, gm, it);
+  const int chunks = (t1 - t0 + kChunk - 1) / kChunk;
+  auto token = [&](int i) { return t0 + (REV ? chunks - 1 - i : i) * kChunk; };
+  auto fetch = [&](TileRegs& x, TileRegs& y, int i) {
+    const int t = token(i < chunks ? i : chunks - 1);
+    tile_fetch(x, px + t * X_.s2, X_.s2, t1 - t < kChunk ? t1 - t : kChunk);
+    tile_fetch(y, py + t * Y_.s2, Y_.s2, t1 - t < kChunk ? t1 - t : kChunk);
+  };
+  f32x4 M[4] = {zero4(), zero4(), zero4(), zero4()};
+  float wt[16];
+  slot_weights<REV>(lg, kChunk, us, wt);
+  TileRegs x, y;
+  fetch(x, y, 0);
+  for (int i = 0; i < chunks; ++i) {
+    char* s = smem + (i & 1) * 2 * kTileBytes;
+    tile_put(x, s);
+    tile_put(y, s + kTileBytes);
+    __syncthreads();   // also: every wave is done with the other buffer
+    fetch(x, y, i + 1);
+    const int t = token(i), n = t1 - t < kChunk ? t1 - t : kChunk;
+    if (n < kChunk) slot_weights<REV>(lg, n, us, wt);   // the last chunk: at the end, or first of all in reverse
+    bf16x8 yc[2][4];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) yc[ks][ct] = tile_column(s + kTileBytes, ct, ks);
+    state_update(s, yc, wt, n < kChunk ? la_power(lg, n) : full, M);
+  }
+  state_store(M, local + it.at * kState);
+}
+
+// The forward's rows, and with other operands dq (see la_rows_kernel): out_i = scale (sum_{j <= i} g^{i-j} (A_i.X_j) Y_j
+// + g^{i+1} A_i M).  LDS: two chunks of X and Y, the state's two parts.
+template <bool TRANS>
+__global__ __launch_bounds__(kLaThreads) void la_rows_bf16(LaRows A_, int ah, LaRows X_, int xh, LaRows Y_, int yh,
+                                                           LaGeom gm, const float* __restrict__ enter,
+                                                           bf16* __restrict__ out, int64_t o0, int64_t o1, int64_t o2,
+                                                           float* __restrict__ leave, LaRows D_, int dh,
+                                                           float* __restrict__ dot) {
+  __shared__ __align__(16) char smem[8 * kTileBytes];
+  __shared__ float s_red[kLaThreads / kWave];
+  const LaItem it = la_item(gm);
+  const int l = threadIdx.x % kWave, w = uniform(threadIdx.x / kWave), g = l / 16, c = l % 16;
+  const int len = la_length(gm, it.b), t0 = it.seg * gm.seg;
+  const int tend = t0 + gm.seg < gm.N ? t0 + gm.seg : gm.N;
+  const int t1 = tend < len ? tend : len;
+  bf16* po = out + it.b * o0 + it.h * o1;
+  la_zero_rows(po, o2, t1 > t0 ? t1 : t0, tend);
+  const float lg = la_log2_decay(gm, it.h), full = la_power(lg, kChunk);
+  const bf16 *pa = la_rows_of(A_, ah, gm, it), *px = la_rows_of(X_, xh, gm, it), *py = la_rows_of(Y_, yh, gm, it);
+  const bf16* pd = dot ? la_rows_of(D_, dh, gm, it) : nullptr;
+  f32x4 M[4];
+  state_load(enter ? enter + it.at * kState : nullptr, TRANS, M);
+  const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
+  TileRegs x, y;
+  bf16x8 a[2], a_next[2];
+  auto fetch = [&](int i) {
+    const int t = t0 + (i < chunks ? i : chunks - 1) * kChunk, n = t1 - t < kChunk ? t1 - t : kChunk;
+    tile_fetch(x, px + t * X_.s2, X_.s2, n);
+    tile_fetch(y, py + t * Y_.s2, Y_.s2, n);
+    const int ld = static_cast<int>(A_.s2) * 2;
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(pa + t * A_.s2, ld, n, 128);
+    const uint32_t off = static_cast<uint32_t>(16 * w + c) * static_cast<uint32_t>(ld) + 16 * g;
+    a_next[0] = bf16x8_from_bits(buf_load16(r, off));
+    a_next[1] = bf16x8_from_bits(buf_load16(r, off + 64));
+  };
+  // scores' weights, tokens 16 (w - jt) apart: on the diagonal, one tile before it (from 1 up), and whole tiles
+  float w0[4], w1[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int d = c - 4 * g - r;
+    w0[r] = d >= 0 ? gm.scale * la_power(lg, d) : 0.f;
+    w1[r] = gm.scale * la_power(lg, d + 16);
+  }
+  const float tile16 = la_power(lg, 16), carry = gm.scale * la_power(lg, 16 * w + c + 1);
+  float wt[16];
+  slot_weights<false>(lg, kChunk, 1.f, wt);
+  const float mid = 0.5f * static_cast<float>(gm.seg);
+  float total = 0.f;
+  if (chunks) fetch(0);
+  for (int i = 0; i < chunks; ++i) {
+    const int t = t0 + i * kChunk, n = t1 - t < kChunk ? t1 - t : kChunk;
+    char *sX = smem + (i & 1) * 4 * kTileBytes, *sY = sX + kTileBytes, *sM = sX + 2 * kTileBytes;
+    tile_put(x, sX);
+    tile_put(y, sY);
+    state_put(M, sM);
+    a[0] = a_next[0];
+    a[1] = a_next[1];
+    __syncthreads();   // also: every wave is done with the other buffer
+    fetch(i + 1);
+    bf16x8 yc[2][4];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) yc[ks][ct] = tile_column(sY, ct, ks);
+    f32x4 o[4] = {zero4(), zero4(), zero4(), zero4()}, z[4] = {zero4(), zero4(), zero4(), zero4()};
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      if (2 * ks <= w) {   // uniform: some of the 32 tokens are not behind the wave's rows
+        float p[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int jt = 2 * ks + half;
+          f32x4 s = zero4();
+          if (jt <= w) {
+            s = mfma16_bf16(tile_row(sX, 16 * jt + c, 0), a[0], s);
+            s = mfma16_bf16(tile_row(sX, 16 * jt + c, 1), a[1], s);
+          }
+          const float far = w - jt <= 1 ? 1.f : w - jt == 2 ? tile16 : tile16 * tile16;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[4 * half + r] = jt == w ? s[r] * w0[r] : s[r] * (w1[r] * far);
+        }
+        bf16x8 parts[2];
+        split8<2>(p, parts);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int ct = 0; ct < 4; ++ct) o[ct] = mfma16_bf16(yc[ks][ct], parts[q], o[ct]);
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        z[ct] = mfma16_bf16(tile_row(sM, 16 * ct + c, ks), a[ks], z[ct]);
+        z[ct] = mfma16_bf16(tile_row(sM + kTileBytes, 16 * ct + c, ks), a[ks], z[ct]);
+      }
+    const int row = 16 * w + c;
+    if (row < n) {
+      bf16* pr = po + (t + row) * o2;
+      float sum = 0.f;
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = fmaf(carry, z[ct][r], o[ct][r]);
+        put4(pr + 16 * ct + 4 * g, v);
+        if (pd) {
+          const uint2 dd = *reinterpret_cast<const uint2*>(pd + (t + row) * D_.s2 + 16 * ct + 4 * g);
+          sum = fmaf(v[0], bf16_lo(dd.x), fmaf(v[1], bf16_hi(dd.x), fmaf(v[2], bf16_lo(dd.y), fmaf(v[3], bf16_hi(dd.y), sum))));
+        }
+      }
+      total = fmaf(static_cast<float>(t - t0 + row + 1) - mid, sum, total);
+    }
+    if (n < kChunk) slot_weights<false>(lg, n, 1.f, wt);
+    state_update(sX, yc, wt, n < kChunk ? la_power(lg, n) : full, M);
+  }
+  if (leave) state_store(M, leave + it.at * kState);
+  if (dot) {
+    total = workgroup_sum(total, s_red);
+    if (threadIdx.x == 0) dot[it.at] = total;
+  }
+}
+
+// dk and dv of a segment, chunks from its end, G the adjoint of the state behind the chunk:
+//   dv_j = scale sum_{i >= j} g^{i-j} (k_j.q_i) do_i + g^{n-1-j} k_j G,  dk_j the same with v, do, q and G^T.
+// The q and do tiles serve as rows and as columns; G lies in LDS transposed, read by rows for dv and transposed for dk.
+template <typename TO>
+__global__ __launch_bounds__(kLaThreads, 2) void la_dkdv_bf16(LaRows Q_, LaRows O_, LaRows K_, LaRows V_, LaGeom gm,
+                                                              const float* __restrict__ enter, TO* __restrict__ dk,
+                                                              int64_t k0, int64_t k1, int64_t k2, TO* __restrict__ dv,
+                                                              int64_t v0, int64_t v1, int64_t v2, int outh,
+                                                              float* __restrict__ dot) {
+  __shared__ __align__(16) char smem[8 * kTileBytes];
+  __shared__ float s_red[kLaThreads / kWave];
+  const LaItem it = la_item(gm);
+  const int l = threadIdx.x % kWave, w = uniform(threadIdx.x / kWave), g = l / 16, c = l % 16;
+  const int len = la_length(gm, it.b), t0 = it.seg * gm.seg;
+  const int tend = t0 + gm.seg < gm.N ? t0 + gm.seg : gm.N;
+  const int t1 = tend < len ? tend : len;
+  const int oh = it.h / (gm.H / outh);
+  TO *pdk = dk + it.b * k0 + oh * k1, *pdv = dv + it.b * v0 + oh * v1;
+  la_zero_rows(pdk, k2, t1 > t0 ? t1 : t0, tend);
+  la_zero_rows(pdv, v2, t1 > t0 ? t1 : t0, tend);
+  const float lg = la_log2_decay(gm, it.h), full = la_power(lg, kChunk);
+  const bf16 *pq = la_rows_of(Q_, gm.H, gm, it), *pdo = la_rows_of(O_, gm.H, gm, it);
+  const bf16 *pk = la_rows_of(K_, gm.Hkv, gm, it), *pv = la_rows_of(V_, gm.Hkv, gm, it);
+  f32x4 G[4];
+  state_load(enter ? enter + it.at * kState : nullptr, false, G);
+  const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
+  TileRegs xq, xo;
+  uint4 kn[2];
+  uint2 vn[4];
+  auto fetch = [&](int i) {
+    const int t = t0 + (i < chunks ? chunks - 1 - i : 0) * kChunk, n = t1 - t < kChunk ? t1 - t : kChunk;
+    tile_fetch(xq, pq + t * Q_.s2, Q_.s2, n);
+    tile_fetch(xo, pdo + t * O_.s2, O_.s2, n);
+    const int lk = static_cast<int>(K_.s2) * 2, lv = static_cast<int>(V_.s2) * 2;
+    const __amdgpu_buffer_rsrc_t rk = rows_rsrc(pk + t * K_.s2, lk, n, 128), rv = rows_rsrc(pv + t * V_.s2, lv, n, 128);
+    const uint32_t ok = static_cast<uint32_t>(16 * w + c) * static_cast<uint32_t>(lk) + 16 * g;
+    const uint32_t ov = static_cast<uint32_t>(16 * w + c) * static_cast<uint32_t>(lv) + 8 * g;
+    kn[0] = buf_load16(rk, ok);
+    kn[1] = buf_load16(rk, ok + 64);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {   // slot order: elements 16 p + 4 g + [0, 4)
+      const auto x = __builtin_amdgcn_raw_buffer_load_b64(rv, ov + 32 * p, 0, 0);
+      vn[p] = uint2{x[0], x[1]};
+    }
+  };
+  // scores' weights, own tokens j before i = 16 it + 4 g + r: on the diagonal, one tile behind it, and whole tiles
+  float w0[4], w1[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int d = 4 * g + r - c;
+    w0[r] = d >= 0 ? gm.scale * la_power(lg, d) : 0.f;
+    w1[r] = gm.scale * la_power(lg, d + 16);
+  }
+  const float tile16 = la_power(lg, 16);
+  float wt[16];
+  slot_weights<true>(lg, kChunk, gm.scale, wt);
+  const float mid = 0.5f * static_cast<float>(gm.seg);
+  float total = 0.f;
+  if (chunks) fetch(0);
+  for (int i = 0; i < chunks; ++i) {
+    const int t = t0 + (chunks - 1 - i) * kChunk, n = t1 - t < kChunk ? t1 - t : kChunk;
+    char *sQ = smem + (i & 1) * 4 * kTileBytes, *sO = sQ + kTileBytes, *sG = sQ + 2 * kTileBytes;
+    tile_put(xq, sQ);
+    tile_put(xo, sO);
+    state_put(G, sG);
+    const bf16x8 ka[2] = {bf16x8_from_bits(kn[0]), bf16x8_from_bits(kn[1])};
+    const bf16x8 va[2] = {bf16x8_from_bits(uint4{vn[0].x, vn[0].y, vn[1].x, vn[1].y}),
+                          bf16x8_from_bits(uint4{vn[2].x, vn[2].y, vn[3].x, vn[3].y})};
+    __syncthreads();   // also: every wave is done with the other buffer
+    fetch(i + 1);
+    const int row = 16 * w + c;
+    const float carry = la_power(lg, n - 1 - row < 0 ? 0 : n - 1 - row);
+    bf16x8 oc[2][4];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) oc[ks][ct] = tile_column(sO, ct, ks);
+    f32x4 av[4] = {zero4(), zero4(), zero4(), zero4()}, ak[4] = {zero4(), zero4(), zero4(), zero4()};
+    // carried parts first, in the same accumulators: (g^{n-1-j} X G) / then the scores' parts on top
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        av[ct] = mfma16_bf16(tile_row(sG, 16 * ct + c, ks), ka[ks], av[ct]);
+        av[ct] = mfma16_bf16(tile_row(sG + kTileBytes, 16 * ct + c, ks), ka[ks], av[ct]);
+        ak[ct] = mfma16_bf16(tile_column(sG, ct, ks), va[ks], ak[ct]);
+        ak[ct] = mfma16_bf16(tile_column(sG + kTileBytes, ct, ks), va[ks], ak[ct]);
+      }
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        av[ct][r] *= carry;
+        ak[ct][r] *= carry;
+      }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      if (2 * ks + 1 >= w) {   // uniform: some of the 32 tokens are not before the wave's rows
+        float p1[8], p2[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int tt = 2 * ks + half;
+          f32x4 s1 = zero4(), s2 = zero4();
+          if (tt >= w) {
+            s1 = mfma16_bf16(tile_row(sQ, 16 * tt + c, 0), ka[0], s1);
+            s1 = mfma16_bf16(tile_row(sQ, 16 * tt + c, 1), ka[1], s1);
+            s2 = mfma16_bf16(tile_row_slots(sO, 16 * tt + c, 0), va[0], s2);
+            s2 = mfma16_bf16(tile_row_slots(sO, 16 * tt + c, 1), va[1], s2);
+          }
+          const float far = tt - w <= 1 ? 1.f : tt - w == 2 ? tile16 : tile16 * tile16;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float weight = tt == w ? w0[r] : w1[r] * far;
+            p1[4 * half + r] = s1[r] * weight;
+            p2[4 * half + r] = s2[r] * weight;
+          }
+        }
+        bf16x8 h1[2], h2[2];
+        split8<2>(p1, h1);
+        split8<2>(p2, h2);
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) {
+          const bf16x8 qc = tile_column(sQ, ct, ks);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            av[ct] = mfma16_bf16(oc[ks][ct], h1[q], av[ct]);
+            ak[ct] = mfma16_bf16(qc, h2[q], ak[ct]);
+          }
+        }
+      }
+    }
+    if (row < n) {
+      TO *rk = pdk + (t + row) * k2, *rv = pdv + (t + row) * v2;
+      float sum = 0.f;
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        const float vk[4] = {ak[ct][0], ak[ct][1], ak[ct][2], ak[ct][3]};
+        const float vv[4] = {av[ct][0], av[ct][1], av[ct][2], av[ct][3]};
+        put4(rk + 16 * ct + 4 * g, vk);
+        put4(rv + 16 * ct + 4 * g, vv);
+        if (dot) {
+          const uint2 dd = *reinterpret_cast<const uint2*>(pk + (t + row) * K_.s2 + 16 * ct + 4 * g);
+          sum = fmaf(vk[0], bf16_lo(dd.x), fmaf(vk[1], bf16_hi(dd.x), fmaf(vk[2], bf16_lo(dd.y), fmaf(vk[3], bf16_hi(dd.y), sum))));
+        }
+      }
+      total = fmaf(static_cast<float>(t - t0 + row + 1) - mid, sum, total);
+    }
+    state_update(sQ, oc, wt, n < kChunk ? la_power(lg, n) : full, G);
+  }
+  if (dot) {
+    total = workgroup_sum(total, s_red);
+    if (threadIdx.x == 0) dot[it.at] = total;
+  }
+}
+
 // dk or dv of a shared head: the query heads' parts in head order.
 template <typename T>
 __global__ __launch_bounds__(kLaThreads) void la_group_sum(const float* __restrict__ part, T* __restrict__ out, int64_t o0,
@@ -444,11 +956,29 @@ LaGeom la_geom(const dwarf_linear_attention_fwd_args& a) {
   return gm;
 }
 
-LaRows la_operand(const void* p, const int64_t* s) { return LaRows{p, s[0], s[1], s[2]}; }
+// A single row's stride is whatever the caller's view says: rows behind it must not fall on it.
+LaRows la_operand(const void* p, const int64_t* s, int N) { return LaRows{p, s[0], s[1], N > 1 ? s[2] : kHd}; }
+
+void la_fwd_bf16(const dwarf_linear_attention_fwd_args& a, const LaGeom& gm, hipStream_t stream) {
+  const LaRows q = la_operand(a.q, a.q_stride, gm.N), k = la_operand(a.k, a.k_stride, gm.N), v = la_operand(a.v, a.v_stride, gm.N);
+  const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * gm.segs), block(kLaThreads);
+  const float* enter = a.initial;
+  if (gm.segs > 1) {
+    hipLaunchKernelGGL((la_local_bf16<false>), grid, block, 0, stream, k, gm.Hkv, v, gm.Hkv, gm, 1.f, a.states);
+    enter = a.states;
+  }
+  if (gm.segs != 1)
+    hipLaunchKernelGGL((la_scan_kernel<false>), dim3(gm.B * gm.H * kScanWgs), block, 0, stream, a.states, a.initial,
+                       a.final, gm, nullptr, nullptr, nullptr, nullptr);
+  if (gm.segs == 0) return;
+  hipLaunchKernelGGL((la_rows_bf16<false>), grid, block, 0, stream, q, gm.H, k, gm.Hkv, v, gm.Hkv, gm, enter,
+                     static_cast<bf16*>(a.out), a.out_stride[0], a.out_stride[1], a.out_stride[2],
+                     gm.segs == 1 ? a.final : nullptr, LaRows{}, 1, nullptr);
+}
 
 template <typename T>
 void la_fwd_typed(const dwarf_linear_attention_fwd_args& a, const LaGeom& gm, hipStream_t stream) {
-  const LaRows q = la_operand(a.q, a.q_stride), k = la_operand(a.k, a.k_stride), v = la_operand(a.v, a.v_stride);
+  const LaRows q = la_operand(a.q, a.q_stride, gm.N), k = la_operand(a.k, a.k_stride, gm.N), v = la_operand(a.v, a.v_stride, gm.N);
   const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * gm.segs), block(kLaThreads);
   const float* enter = a.initial;
   if (gm.segs > 1) {
@@ -487,8 +1017,8 @@ LaBwdSpace la_bwd_space(const dwarf_linear_attention_bwd_args& a, const LaGeom& 
 template <typename T>
 void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hipStream_t stream) {
   const dwarf_linear_attention_fwd_args& f = a.fwd;
-  const LaRows q = la_operand(f.q, f.q_stride), k = la_operand(f.k, f.k_stride), v = la_operand(f.v, f.v_stride);
-  const LaRows dout = la_operand(a.dout, a.dout_stride);
+  const LaRows q = la_operand(f.q, f.q_stride, gm.N), k = la_operand(f.k, f.k_stride, gm.N), v = la_operand(f.v, f.v_stride, gm.N);
+  const LaRows dout = la_operand(a.dout, a.dout_stride, gm.N);
   const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * gm.segs), block(kLaThreads);
   const LaBwdSpace sp = la_bwd_space(a, gm);
   float* ws = static_cast<float*>(a.workspace);
@@ -496,31 +1026,50 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
   float *adj = ws + sp.adjoint, *dq_dot = dlog ? ws + sp.dq_dot : nullptr, *dk_dot = dlog ? ws + sp.dk_dot : nullptr;
   float* edge = dlog ? ws + sp.edge : nullptr;
   const bool joined = gm.segs != 1 || a.dinitial || dlog;
-  if (joined) {
-    if (gm.segs)
+  const float* enter = joined ? adj : a.dfinal;
+  const float* before = gm.segs > 1 ? f.states : f.initial;
+  const bool shared = gm.H != gm.Hkv;
+  float *pk = ws + sp.dk_part, *pv = ws + sp.dv_part;
+  const int64_t s1 = static_cast<int64_t>(gm.N) * kHd, s0 = s1 * gm.H;   // of the shared heads' parts
+  if (joined && gm.segs) {
+    if constexpr (std::is_same<T, bf16>::value)
+      hipLaunchKernelGGL((la_local_bf16<true>), grid, block, 0, stream, q, gm.H, dout, gm.H, gm, gm.scale, adj);
+    else
       hipLaunchKernelGGL((la_local_kernel<T, true>), grid, block, 0, stream, q, gm.H, dout, gm.H, gm, gm.scale, adj);
+  }
+  if (joined)
     hipLaunchKernelGGL((la_scan_kernel<true>), dim3(gm.B * gm.H * kScanWgs), block, 0, stream, adj, a.dfinal, a.dinitial,
                        gm, f.states, f.initial, f.final, edge);
-  }
   if (gm.segs) {
-    hipLaunchKernelGGL((la_rows_kernel<T, T, false, true>), grid, block, 0, stream, dout, gm.H, v, gm.Hkv, k, gm.Hkv, gm,
-                       gm.scale, gm.scale, 1.f, gm.segs > 1 ? f.states : f.initial, static_cast<T*>(a.dq),
-                       a.dq_stride[0], a.dq_stride[1], a.dq_stride[2], nullptr, q, gm.H, dq_dot);
-    const float* enter = joined ? adj : a.dfinal;
-    if (gm.H == gm.Hkv) {
-      hipLaunchKernelGGL((la_rows_kernel<T, T, true, false>), grid, block, 0, stream, k, gm.Hkv, q, gm.H, dout, gm.H, gm,
-                         gm.scale, 1.f, gm.scale, enter, static_cast<T*>(a.dv), a.dv_stride[0], a.dv_stride[1],
-                         a.dv_stride[2], nullptr, LaRows{}, 1, nullptr);
-      hipLaunchKernelGGL((la_rows_kernel<T, T, true, true>), grid, block, 0, stream, v, gm.Hkv, dout, gm.H, q, gm.H, gm,
-                         gm.scale, 1.f, gm.scale, enter, static_cast<T*>(a.dk), a.dk_stride[0], a.dk_stride[1],
-                         a.dk_stride[2], nullptr, k, gm.Hkv, dk_dot);
+    if constexpr (std::is_same<T, bf16>::value) {
+      hipLaunchKernelGGL((la_rows_bf16<true>), grid, block, 0, stream, dout, gm.H, v, gm.Hkv, k, gm.Hkv, gm, before,
+                         static_cast<bf16*>(a.dq), a.dq_stride[0], a.dq_stride[1], a.dq_stride[2], nullptr, q, gm.H, dq_dot);
+      if (shared)
+        hipLaunchKernelGGL((la_dkdv_bf16<float>), grid, block, 0, stream, q, dout, k, v, gm, enter, pk, s0, s1, kHd, pv,
+                           s0, s1, kHd, gm.H, dk_dot);
+      else
+        hipLaunchKernelGGL((la_dkdv_bf16<bf16>), grid, block, 0, stream, q, dout, k, v, gm, enter, static_cast<bf16*>(a.dk),
+                           a.dk_stride[0], a.dk_stride[1], a.dk_stride[2], static_cast<bf16*>(a.dv), a.dv_stride[0],
+                           a.dv_stride[1], a.dv_stride[2], gm.Hkv, dk_dot);
     } else {
-      float *pk = ws + sp.dk_part, *pv = ws + sp.dv_part;
-      const int64_t s1 = static_cast<int64_t>(gm.N) * kHd, s0 = s1 * gm.H;
-      hipLaunchKernelGGL((la_rows_kernel<T, float, true, false>), grid, block, 0, stream, k, gm.Hkv, q, gm.H, dout, gm.H,
-                         gm, gm.scale, 1.f, gm.scale, enter, pv, s0, s1, kHd, nullptr, LaRows{}, 1, nullptr);
-      hipLaunchKernelGGL((la_rows_kernel<T, float, true, true>), grid, block, 0, stream, v, gm.Hkv, dout, gm.H, q, gm.H,
-                         gm, gm.scale, 1.f, gm.scale, enter, pk, s0, s1, kHd, nullptr, k, gm.Hkv, dk_dot);
+      hipLaunchKernelGGL((la_rows_kernel<T, T, false, true>), grid, block, 0, stream, dout, gm.H, v, gm.Hkv, k, gm.Hkv, gm,
+                         gm.scale, gm.scale, 1.f, before, static_cast<T*>(a.dq), a.dq_stride[0], a.dq_stride[1],
+                         a.dq_stride[2], nullptr, q, gm.H, dq_dot);
+      if (shared) {
+        hipLaunchKernelGGL((la_rows_kernel<T, float, true, false>), grid, block, 0, stream, k, gm.Hkv, q, gm.H, dout, gm.H,
+                           gm, gm.scale, 1.f, gm.scale, enter, pv, s0, s1, kHd, nullptr, LaRows{}, 1, nullptr);
+        hipLaunchKernelGGL((la_rows_kernel<T, float, true, true>), grid, block, 0, stream, v, gm.Hkv, dout, gm.H, q, gm.H,
+                           gm, gm.scale, 1.f, gm.scale, enter, pk, s0, s1, kHd, nullptr, k, gm.Hkv, dk_dot);
+      } else {
+        hipLaunchKernelGGL((la_rows_kernel<T, T, true, false>), grid, block, 0, stream, k, gm.Hkv, q, gm.H, dout, gm.H, gm,
+                           gm.scale, 1.f, gm.scale, enter, static_cast<T*>(a.dv), a.dv_stride[0], a.dv_stride[1],
+                           a.dv_stride[2], nullptr, LaRows{}, 1, nullptr);
+        hipLaunchKernelGGL((la_rows_kernel<T, T, true, true>), grid, block, 0, stream, v, gm.Hkv, dout, gm.H, q, gm.H, gm,
+                           gm.scale, 1.f, gm.scale, enter, static_cast<T*>(a.dk), a.dk_stride[0], a.dk_stride[1],
+                           a.dk_stride[2], nullptr, k, gm.Hkv, dk_dot);
+      }
+    }
+    if (shared) {
       const int64_t quads = static_cast<int64_t>(gm.B) * gm.Hkv * gm.N * (kHd / 4);
       const dim3 sums(static_cast<unsigned>((quads + kLaThreads - 1) / kLaThreads));
       hipLaunchKernelGGL((la_group_sum<T>), sums, block, 0, stream, pv, static_cast<T*>(a.dv), a.dv_stride[0],
@@ -551,7 +1100,7 @@ hipError_t launch_linear_attention_fwd(const dwarf_linear_attention_fwd_args& a,
   const LaGeom gm = la_geom(a);
   if (a.dtype == DWARF_F32) la_fwd_typed<float>(a, gm, stream);
   else if (a.dtype == DWARF_F16) la_fwd_typed<f16>(a, gm, stream);
-  else la_fwd_typed<bf16>(a, gm, stream);
+  else la_fwd_bf16(a, gm, stream);
   return hipGetLastError();
 }
 

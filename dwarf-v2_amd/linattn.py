@@ -56,9 +56,21 @@ def _fill(a: _lib.LinearAttentionFwdArgs, q, k, v, log_decay, initial, lengths, 
     a.states, a.states_bytes = states.data_ptr(), states.numel() * 4
 
 
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[B,H,N,64] as the kernels read it: 16-byte aligned rows that do not overlap, less than 2^22 elements apart."""
+    if t.shape[2] > 1 and not HEAD_DIM <= t.stride(2) < 1 << 22:
+        return t.contiguous()
+    return _kernel_rows(t)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.detach().contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 def _operands(q, k, v, log_decay, initial, lengths):
-    q, k, v = _kernel_rows(q), _kernel_rows(k), _kernel_rows(v)
-    return (q, k, v, _decay(log_decay), None if initial is None else initial.detach().contiguous(),
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    return (q, k, v, _decay(log_decay), None if initial is None else _aligned(initial),
             None if lengths is None else lengths.to(torch.int32).contiguous())
 
 
@@ -82,7 +94,7 @@ def attention_backward(dout, dstate, q, k, v, log_decay, initial, lengths, scale
     """Raw launches: (dq, dk, dv in token-major memory, dlog_decay [H] or None, dinitial or None)."""
     q, k, v, decay, initial, lengths = _operands(q, k, v, log_decay, initial, lengths)
     B, H, N, hd = q.shape
-    dout = _kernel_rows(dout.to(q.dtype))
+    dout = _rows(dout.to(q.dtype))
     dstate = None if dstate is None else dstate.float().contiguous()
     a = _lib.LinearAttentionBwdArgs()
     _fill(a.fwd, q, k, v, decay, initial, lengths, scale, states)

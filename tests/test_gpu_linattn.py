@@ -234,6 +234,14 @@ def test_layouts_agree_bit_for_bit(pkg, device):
     fused = torch.cat([d[n].transpose(1, 2).reshape(2, 90, -1) for n in ("q", "k", "v")], -1)
     parts = [t.unflatten(-1, (-1, HD)).transpose(1, 2) for t in fused.split([256, 128, 128], -1)]
     assert torch.equal(forward(pkg, dict(d, **dict(zip("qkv", parts)))), want)
+    one = d["k"][:, :, :1].expand(-1, -1, 90, -1)          # one key for every token: rows a stride of 0 apart
+    assert torch.equal(forward(pkg, dict(d, k=one)), forward(pkg, dict(d, k=one.contiguous())))
+    over = torch.randn(90 * 8 + 64, device=device).bfloat16().as_strided((2, 4, 90, 64), (0, 0, 8, 1))   # overlapping rows
+    assert torch.equal(forward(pkg, dict(d, q=over)), forward(pkg, dict(d, q=over.contiguous())))
+    single = torch.randn(2, 4, 1, 64, device=device).bfloat16()
+    tight = single.as_strided((2, 4, 1, 64), (256, 64, 0, 1))
+    alone = dict(d, k=d["k"][:, :, :1], v=d["v"][:, :, :1], lengths=None)
+    assert torch.equal(forward(pkg, dict(alone, q=tight)), forward(pkg, dict(alone, q=single)))
     odd = torch.empty(2, 4, 90, 67, device=device, dtype=torch.bfloat16)[..., 1:65]
     odd.copy_(d["q"])
     assert torch.equal(forward(pkg, dict(d, q=odd)), want)

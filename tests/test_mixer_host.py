@@ -146,6 +146,13 @@ def test_linear_attention_entry_points_refuse(pkg, lib):
         assert lib.dwarf_linear_attention_fwd(ctypes.byref(f), None) == want, name
         assert lib.dwarf_linear_attention_bwd(ctypes.byref(a), None) == want, name
         setattr(f, name, keep)
+    for stride in (0, 56, 1 << 22):                                         # overlapping rows, rows too far apart
+        f.q_stride = (100 * 256, 64, stride, 1)
+        assert lib.dwarf_linear_attention_fwd(ctypes.byref(f), None) == L.DWARF_ERR_UNSUPPORTED, stride
+    f.q_stride = rows
+    f.initial = P + 4
+    assert lib.dwarf_linear_attention_fwd(ctypes.byref(f), None) == bad     # the state that enters is not aligned
+    f.initial = None
     assert lib.dwarf_linear_attention_bwd(ctypes.byref(a), None) == bad     # dout is NULL
     a.dout = a.dq = a.dk = a.dv = a.dlog_decay = a.dfinal = P
     a.dout_stride = a.dq_stride = rows
