@@ -19,8 +19,8 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _launch, _lib
-from .dsqg import HEAD_DIM, _kernel_rows
+from . import _launch
+from .dsqg import HEAD_DIM
 
 
 def segment_tokens(B: int, H: int, N: int) -> int:
@@ -37,113 +37,83 @@ def states_shape(B: int, H: int, N: int) -> tuple[int, ...]:
     return (B, H, segs if segs > 1 else 0, HEAD_DIM, HEAD_DIM)
 
 
-def _ptr(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
-
-
-def _decay(log_decay: torch.Tensor) -> torch.Tensor:
-    return log_decay.detach().reshape(-1).float().contiguous()
-
-
-def _fill(a: _lib.LinearAttentionFwdArgs, q, k, v, log_decay, initial, lengths, scale: float, states) -> None:
-    B, H, N, hd = q.shape
-    a.B, a.H, a.H_kv, a.N, a.head_dim = B, H, k.shape[1], N, hd
-    a.dtype, a.scale = _launch.DTYPES[q.dtype], scale
-    a.q, a.q_stride = q.data_ptr(), q.stride()
-    a.k, a.k_stride = k.data_ptr(), k.stride()
-    a.v, a.v_stride = v.data_ptr(), v.stride()
-    a.log_decay, a.lengths, a.initial = log_decay.data_ptr(), _ptr(lengths), _ptr(initial)
-    a.states, a.states_bytes = states.data_ptr(), states.numel() * 4
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """[B,H,N,64] as the kernels read it: 16-byte aligned rows that do not overlap, less than 2^22 elements apart."""
-    if t.shape[2] > 1 and not HEAD_DIM <= t.stride(2) < 1 << 22:
-        return t.contiguous()
-    return _kernel_rows(t)
-
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.detach().contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
-
-
-def _operands(q, k, v, log_decay, initial, lengths):
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    return (q, k, v, _decay(log_decay), None if initial is None else _aligned(initial),
-            None if lengths is None else lengths.to(torch.int32).contiguous())
-
-
 def attention_forward(q, k, v, log_decay, initial, lengths, scale: float, want_state: bool
                       ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor]:
     """Raw launches: (out in token-major memory, the final state or None, the segments' states)."""
-    q, k, v, decay, initial, lengths = _operands(q, k, v, log_decay, initial, lengths)
-    B, H, N, hd = q.shape
-    out = _launch.token_major(B, H, N, hd, q)
-    state = torch.empty((B, H, hd, hd), device=q.device, dtype=torch.float32) if want_state else None
-    states = torch.empty(states_shape(B, H, N), device=q.device, dtype=torch.float32)
-    a = _lib.LinearAttentionFwdArgs()
-    _fill(a, q, k, v, decay, initial, lengths, scale, states)
-    a.out, a.out_stride, a.final = out.data_ptr(), out.stride(), _ptr(state)
-    _launch.launch("dwarf_linear_attention_fwd", a, q.device)
-    return out, state, states
+    return _launch.native().attention_forward(q, k, v, log_decay, initial, lengths, scale, want_state)
 
 
 def attention_backward(dout, dstate, q, k, v, log_decay, initial, lengths, scale: float, states, state,
                        need_decay: bool, need_initial: bool):
     """Raw launches: (dq, dk, dv in token-major memory, dlog_decay [H] or None, dinitial or None)."""
-    q, k, v, decay, initial, lengths = _operands(q, k, v, log_decay, initial, lengths)
-    B, H, N, hd = q.shape
-    dout = _rows(dout.to(q.dtype))
-    dstate = None if dstate is None else dstate.float().contiguous()
-    a = _lib.LinearAttentionBwdArgs()
-    _fill(a.fwd, q, k, v, decay, initial, lengths, scale, states)
-    a.fwd.final = _ptr(state)
-    a.dout, a.dout_stride, a.dfinal = dout.data_ptr(), dout.stride(), _ptr(dstate)
-    dq = _launch.token_major(B, H, N, hd, q)
-    dk, dv = (_launch.token_major(B, k.shape[1], N, hd, q) for _ in range(2))
-    a.dq, a.dq_stride = dq.data_ptr(), dq.stride()
-    a.dk, a.dk_stride = dk.data_ptr(), dk.stride()
-    a.dv, a.dv_stride = dv.data_ptr(), dv.stride()
-    dlog = torch.empty(H, device=q.device, dtype=torch.float32) if need_decay else None
-    dinitial = torch.empty((B, H, hd, hd), device=q.device, dtype=torch.float32) if need_initial else None
-    a.dlog_decay, a.dinitial = _ptr(dlog), _ptr(dinitial)
-    ws = _launch.workspace("dwarf_linear_attention_bwd_workspace_bytes", a, q.device)
-    if ws is not None:
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    _launch.launch("dwarf_linear_attention_bwd", a, q.device)
-    return dq, dk, dv, dlog, dinitial
+    return _launch.native().attention_backward(dout, dstate, q, k, v, log_decay, initial, lengths, scale, states, state,
+                                               need_decay, need_initial)
+
+
+def attention_step(q, k, v, log_decay, state, new_state, slots, scale: float, out=None) -> torch.Tensor:
+    """Raw launch of one step: out [S,H,64]; new_state None writes the pool itself."""
+    return _launch.native().attention_step(q, k, v, log_decay, state, new_state, slots, scale, out)
 
 
 class _LinearAttentionFn(torch.autograd.Function):
+    """The autograd node of compiled calls; eager calls have theirs in C++."""
+
     @staticmethod
     def forward(ctx, q, k, v, log_decay, initial, lengths, scale: float, want_state: bool):
-        if torch.compiler.is_compiling():
-            out, state, states = torch.ops.dwarf.linear_attention_fwd(q, k, v, log_decay, initial, lengths, scale,
-                                                                      want_state)
-        else:
-            out, state, states = attention_forward(q, k, v, log_decay, initial, lengths, scale, want_state)
-        kept = state if want_state and log_decay.requires_grad else None   # for the decay's gradient
-        ctx.save_for_backward(q, k, v, log_decay, initial, lengths, states, kept)
-        ctx.scale, ctx.want_state = scale, want_state
-        ctx.set_materialize_grads(False)
+        out, state, states = torch.ops.dwarf.linear_attention_fwd(q, k, v, log_decay, initial, lengths, scale, want_state)
+        ctx.save_for_backward(q, k, v, log_decay, initial, lengths, states, state if want_state else None)
+        ctx.scale = scale
         return (out, state) if want_state else out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dstate=None):
         q, k, v, log_decay, initial, lengths, states, state = ctx.saved_tensors
-        if dout is None and dstate is None:
-            return (None,) * 8
-        if dout is None:
-            dout = torch.zeros_like(q)
         need = ctx.needs_input_grad
-        backward = torch.ops.dwarf.linear_attention_bwd if torch.compiler.is_compiling() else attention_backward
-        dq, dk, dv, dlog, dinitial = backward(dout, dstate, q, k, v, log_decay, initial, lengths, ctx.scale, states,
-                                              state, need[3], need[4])
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
-                dlog.view(log_decay.shape).to(log_decay.dtype) if need[3] else None,
+        dq, dk, dv, dlog, dinitial = torch.ops.dwarf.linear_attention_bwd(
+            dout, dstate, q, k, v, log_decay, initial, lengths, ctx.scale, states, state, need[3], need[4])
+        return (dq, dk, dv, dlog.view(log_decay.shape).to(log_decay.dtype) if need[3] else None,
                 dinitial if need[4] else None, None, None, None)
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, *,
+                     scale: float | None = None, initial_state: torch.Tensor | None = None,
+                     lengths: torch.Tensor | None = None, return_state: bool = False):
+    """Decayed linear attention over whole sequences: out [B,H,N,64] in q's dtype ([B,N,H,64] memory), and with
+    ``return_state`` the state [B,H,64,64] fp32 behind each sequence's last token.
+
+    q [B,H,N,64], k and v [B,H_kv,N,64]; log_decay [H], values above 0 count as 0 (their gradient is 0);
+    scale 1/8 by default; initial_state [B,H,64,64] fp32; lengths [B] integers, clamped to [0, N]: the tokens of
+    each sequence, behind which nothing is used and the output is zero.  Tokens are summed 64 at a time, so one
+    that is not finite spoils its sequence's outputs from the first of its 64 on."""
+    if not torch.compiler.is_compiling():
+        return _launch.native().linear_attention(q, k, v, log_decay, scale, initial_state, lengths, return_state)
+    scale = _check(q, k, v, log_decay, scale, initial_state, lengths)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
+        return _LinearAttentionFn.apply(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
+    out, state, _ = torch.ops.dwarf.linear_attention_fwd(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
+    return (out, state) if return_state else out
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                          state: torch.Tensor, *, slots: torch.Tensor | None = None,
+                          new_state: torch.Tensor | None = None, scale: float | None = None,
+                          out: torch.Tensor | None = None) -> torch.Tensor:
+    """One token of each of S rows: q [S,H,64], k and v [S,H_kv,64]; returns out [S,H,64].
+
+    state [P,H,64,64] fp32 is a pool of sequences' states, each slot contiguous.  Row s works on slot slots[s]
+    (slot s where slots is None); its new state is written to the same slot of ``new_state``, or of ``state`` itself
+    where that is None.  Slots outside [0, P) mark rows that pad the batch: no state is touched, their output
+    is zero.  Rows that share a slot are consecutive tokens of its sequence, in row order.  ``out``: where to write
+    the result (eager calls).  No gradients."""
+    if not torch.compiler.is_compiling():
+        return _launch.native().linear_attention_step(q, k, v, log_decay, state, slots, new_state, scale, out)
+    if out is not None:
+        raise RuntimeError("out= is for eager calls and captured graphs, not for torch.compile")
+    scale = _check_step(q, k, v, log_decay, state, slots, new_state, scale)
+    if new_state is None:
+        return torch.ops.dwarf.linear_attention_step_(q, k, v, log_decay, state, slots, scale)
+    return torch.ops.dwarf.linear_attention_step(q, k, v, log_decay, state, new_state, slots, scale)
 
 
 def _check_scale(scale) -> float:
@@ -167,15 +137,8 @@ def _check_heads(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: t
     _launch.check_dtype("q", q)
 
 
-def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, *,
-                     scale: float | None = None, initial_state: torch.Tensor | None = None,
-                     lengths: torch.Tensor | None = None, return_state: bool = False):
-    """Decayed linear attention over whole sequences: out [B,H,N,64] in q's dtype ([B,N,H,64] memory), and with
-    ``return_state`` the state [B,H,64,64] fp32 behind each sequence's last token.
-
-    q [B,H,N,64], k and v [B,H_kv,N,64]; log_decay [H], values above 0 count as 0 (their gradient is 0);
-    scale 1/8 by default; initial_state [B,H,64,64] fp32; lengths [B] integers, clamped to [0, N]: the tokens of
-    each sequence, behind which nothing is used and the output is zero."""
+def _check(q, k, v, log_decay, scale, initial_state, lengths) -> float:
+    """The native call's checks, for compiled calls; returns the scale."""
     scale = _check_scale(scale)
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError(f"q, k and v must be [B,H,N,{HEAD_DIM}], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -189,54 +152,11 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     _launch.check_device(q, k=k, v=v, log_decay=log_decay, initial_state=initial_state, lengths=lengths)
     if hd != HEAD_DIM:
         raise RuntimeError(f"linear attention is built for head_dim {HEAD_DIM}, got {hd}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
-        return _LinearAttentionFn.apply(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
-    forward = torch.ops.dwarf.linear_attention_fwd if torch.compiler.is_compiling() else attention_forward
-    out, state, _ = forward(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
-    return (out, state) if return_state else out
+    return scale
 
 
-def _pool_ok(t: torch.Tensor, H: int) -> bool:
-    return (t.ndim == 4 and t.dtype == torch.float32 and tuple(t.shape[1:]) == (H, HEAD_DIM, HEAD_DIM)
-            and (t.shape[0] == 1 or (t.stride(0) >= H * HEAD_DIM * HEAD_DIM and t.stride(0) % 4 == 0))
-            and t.stride()[1:] == (HEAD_DIM * HEAD_DIM, HEAD_DIM, 1) and t.data_ptr() % 16 == 0)
-
-
-def attention_step(q, k, v, log_decay, state, new_state, slots, scale: float, out=None) -> torch.Tensor:
-    """Raw launch of one step: out [S,H,64]; new_state None writes the pool itself."""
-    q, k, v = _kernel_rows(q), _kernel_rows(k), _kernel_rows(v)
-    decay = _decay(log_decay)
-    if slots is not None:
-        slots = slots.to(torch.int32).contiguous()
-    S, H, hd = q.shape
-    if out is None:
-        out = torch.empty((S, H, hd), device=q.device, dtype=q.dtype)
-    a = _lib.LinearAttentionStepArgs()
-    a.S, a.H, a.H_kv, a.pool, a.head_dim = S, H, k.shape[1], state.shape[0], hd
-    a.dtype, a.scale = _launch.DTYPES[q.dtype], scale
-    a.q, a.q_stride = q.data_ptr(), q.stride()
-    a.k, a.k_stride = k.data_ptr(), k.stride()
-    a.v, a.v_stride = v.data_ptr(), v.stride()
-    a.log_decay, a.slots = decay.data_ptr(), _ptr(slots)
-    a.state = state.data_ptr()
-    a.new_state = a.state if new_state is None else new_state.data_ptr()
-    a.slot_stride = state.stride(0) if state.shape[0] > 1 else H * hd * hd
-    a.out, a.out_stride = out.data_ptr(), out.stride()
-    _launch.launch("dwarf_linear_attention_step", a, q.device)
-    return out
-
-
-def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
-                          state: torch.Tensor, *, slots: torch.Tensor | None = None,
-                          new_state: torch.Tensor | None = None, scale: float | None = None,
-                          out: torch.Tensor | None = None) -> torch.Tensor:
-    """One token of each of S rows: q [S,H,64], k and v [S,H_kv,64]; returns out [S,H,64].
-
-    state [P,H,64,64] fp32 is a pool of sequences' states, each slot contiguous.  Row s works on slot slots[s]
-    (slot s where slots is None); its new state is written to the same slot of ``new_state``, or of ``state`` itself
-    where that is None.  Slots outside [0, P) mark rows that pad the batch: no state is touched, their output
-    is zero.  Rows that share a slot are consecutive tokens of its sequence, in row order.  ``out``: where to write
-    the result.  No gradients."""
+def _check_step(q, k, v, log_decay, state, slots, new_state, scale) -> float:
+    """The native call's checks but those of memory (strides and alignment, made at the launch), for compiled calls."""
     scale = _check_scale(scale)
     if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
         raise ValueError(f"q, k and v must be [S,H,{HEAD_DIM}], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -245,27 +165,15 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     if hd != HEAD_DIM:
         raise RuntimeError(f"linear attention is built for head_dim {HEAD_DIM}, got {hd}")
     for name, t in (("state", state), ("new_state", new_state)):
-        if t is not None and not _pool_ok(t, H):
-            raise ValueError(f"{name} must be an fp32 [P,{H},{hd},{hd}] pool with contiguous, 16-byte aligned slots, got "
-                             f"{tuple(t.shape)} {t.dtype} strides {t.stride()}")
-    if new_state is not None and (new_state.shape != state.shape
-                                  or (state.shape[0] > 1 and new_state.stride() != state.stride())):
+        if t is not None and (t.dtype != torch.float32 or t.ndim != 4 or tuple(t.shape[1:]) != (H, hd, hd)):
+            raise ValueError(f"{name} must be an fp32 [P,{H},{hd},{hd}] pool, got {tuple(t.shape)} {t.dtype}")
+    if new_state is not None and new_state.shape != state.shape:
         raise ValueError("new_state must have state's shape and strides")
     if slots is None and state.shape[0] < S:
         raise ValueError(f"a pool of {state.shape[0]} states does not hold the {S} rows")
     if slots is not None and (tuple(slots.shape) != (S,) or slots.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"slots must be [{S}] int32 or int64, got {tuple(slots.shape)} {slots.dtype}")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or _kernel_rows(out) is not out):
-        raise ValueError(f"out must be [{S},{H},{hd}] {q.dtype} with 16-byte aligned rows")
-    _launch.check_device(q, k=k, v=v, log_decay=log_decay, state=state, new_state=new_state, slots=slots, out=out)
+    _launch.check_device(q, k=k, v=v, log_decay=log_decay, state=state, new_state=new_state, slots=slots)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
         raise RuntimeError("linear_attention_step has no gradients: call it under torch.no_grad(), or linear_attention")
-    if S and not state.shape[0]:
-        raise ValueError("the pool is empty")
-    if torch.compiler.is_compiling():
-        if out is not None:
-            raise RuntimeError("out= is for eager calls and captured graphs, not for torch.compile")
-        if new_state is None:
-            return torch.ops.dwarf.linear_attention_step_(q, k, v, log_decay, state, slots, scale)
-        return torch.ops.dwarf.linear_attention_step(q, k, v, log_decay, state, new_state, slots, scale)
-    return attention_step(q, k, v, log_decay, state, new_state, slots, scale, out)
+    return scale

@@ -18,7 +18,7 @@ from fractions import Fraction
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _launch, _lib
+from . import _launch
 
 _TWO_PI = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
 SCALINGS = (None, "linear", "base", "bands")
@@ -90,72 +90,29 @@ def rotary_plan(rotary_dim: int, base: float = 10000.0, *, interleaved: bool = F
     return RotaryPlan(f, interleaved, magnitude, device)
 
 
-def _operand(x: torch.Tensor, interleaved: bool) -> torch.Tensor:
-    """Unit last stride; even strides and pair alignment where pairs lie side by side."""
-    ok = x.stride(-1) == 1
-    if ok and interleaved:
-        ok = x.data_ptr() % (2 * x.element_size()) == 0 and all(s % 2 == 0 for s in x.stride()[:-1])
-    return x if ok else x.contiguous()
-
-
 def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, turns: torch.Tensor, interleaved: bool,
            inverse: bool, magnitude: float) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Raw launch: the turned (q, k), in token-major memory."""
-    q = _operand(q, interleaved)
-    B, H, N, D = q.shape
-    a = _lib.RotaryArgs()
-    a.B, a.H, a.N, a.D, a.pairs = B, H, N, D, turns.numel()
-    a.dtype, a.interleaved, a.inverse = _launch.DTYPES[q.dtype], interleaved, inverse
-    a.magnitude = magnitude
-    q_out = _launch.token_major(B, H, N, D, q)
-    a.q, a.q_stride = q.data_ptr(), q.stride()
-    a.q_out, a.q_out_stride = q_out.data_ptr(), q_out.stride()
-    k_out = None
-    if k is not None:
-        k = _operand(k, interleaved)
-        k_out = _launch.token_major(B, k.shape[1], N, D, k)
-        a.H_kv = k.shape[1]
-        a.k, a.k_stride = k.data_ptr(), k.stride()
-        a.k_out, a.k_out_stride = k_out.data_ptr(), k_out.stride()
-    a.positions, a.position_bytes = positions.data_ptr(), positions.element_size()
-    a.position_stride = (positions.stride(0), positions.stride(1)) if positions.ndim == 2 else (0, positions.stride(0))
-    a.turns = turns.data_ptr()
-    _launch.launch("dwarf_rotary", a, q.device)
-    return q_out, k_out
+    return _launch.native().rotate(q, k, positions, turns, interleaved, inverse, magnitude)
 
 
 class _RotaryFn(torch.autograd.Function):
+    """The autograd node of compiled calls; eager calls have theirs in C++."""
+
     @staticmethod
     def forward(ctx, q, k, positions, turns, interleaved: bool, magnitude: float):
         ctx.save_for_backward(positions, turns)
-        ctx.how = (interleaved, magnitude)
-        ctx.set_materialize_grads(False)
-        ctx.shapes = (q.shape, None if k is None else k.shape, q.dtype, q.device)
-        if torch.compiler.is_compiling():
-            q_out, k_out = torch.ops.dwarf.rotary(q, k, positions, turns, interleaved, False, magnitude)
-            return (q_out, k_out) if k is not None else (q_out, None)
-        return rotate(q, k, positions, turns, interleaved, False, magnitude)
+        ctx.how = (interleaved, magnitude, k is not None)
+        q_out, k_out = torch.ops.dwarf.rotary(q, k, positions, turns, interleaved, False, magnitude)
+        return (q_out, k_out) if k is not None else (q_out, None)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq, dk):
         positions, turns = ctx.saved_tensors
-        interleaved, magnitude = ctx.how
-        q_shape, k_shape, dtype, device = ctx.shapes
-        if dq is None and dk is None:
-            return (None,) * 6
-        if dq is None:
-            dq = torch.zeros(q_shape, dtype=dtype, device=device)
-        if dk is None and k_shape is not None:
-            dk = torch.zeros(k_shape, dtype=dtype, device=device)
-        dq = dq.to(dtype)
-        dk = None if dk is None else dk.to(dtype)
-        if torch.compiler.is_compiling():
-            gq, gk = torch.ops.dwarf.rotary(dq, dk, positions, turns, interleaved, True, magnitude)
-        else:
-            gq, gk = rotate(dq, dk, positions, turns, interleaved, True, magnitude)
-        need = ctx.needs_input_grad
-        return gq if need[0] else None, gk if need[1] else None, None, None, None, None
+        interleaved, magnitude, has_k = ctx.how
+        gq, gk = torch.ops.dwarf.rotary(dq, dk if has_k else None, positions, turns, interleaved, True, magnitude)
+        return gq, gk if has_k else None, None, None, None, None
 
 
 def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
@@ -164,6 +121,17 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
 
     bf16, fp16 or fp32, any strides with a unit last one; D even, at least the plan's rotary_dim.  The results
     have q's and k's shapes in [B,N,H,D] memory."""
+    if not torch.compiler.is_compiling():
+        return _launch.native().rotary_embed(q, k, positions, plan.turns, plan.interleaved, plan.magnitude)
+    _check(q, k, positions, plan)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryFn.apply(q, k, positions, plan.turns, plan.interleaved, plan.magnitude)
+    q_out, k_out = torch.ops.dwarf.rotary(q, k, positions, plan.turns, plan.interleaved, False, plan.magnitude)
+    return q_out, (k_out if k is not None else None)
+
+
+def _check(q, k, positions, plan) -> None:
+    """The native call's checks, for compiled calls."""
     if q.ndim != 4:
         raise ValueError(f"q must be [B,H,N,D], got {tuple(q.shape)}")
     B, H, N, D = q.shape
@@ -179,9 +147,3 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         raise ValueError(f"positions must be [{N}] or [{B},{N}], got {tuple(positions.shape)}")
     _launch.check_dtype("q", q)
     _launch.check_device(q, k=k, positions=positions, plan=plan.turns)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryFn.apply(q, k, positions, plan.turns, plan.interleaved, plan.magnitude)
-    if torch.compiler.is_compiling():
-        q_out, k_out = torch.ops.dwarf.rotary(q, k, positions, plan.turns, plan.interleaved, False, plan.magnitude)
-        return q_out, (k_out if k is not None else None)
-    return rotate(q, k, positions, plan.turns, plan.interleaved, False, plan.magnitude)
