@@ -343,26 +343,48 @@ __device__ __forceinline__ void tile_fetch(TileRegs& t, const bf16* base, int64_
   t.x[0] = buf_load16(r, off);
   t.x[1] = buf_load16(r, off + 32u * static_cast<uint32_t>(ld));
 }
-__device__ __forceinline__ void tile_put(const TileRegs& t, char* s) {
-  const int at = tile_at(threadIdx.x >> 3, (threadIdx.x & 7) * 16);   // rows 32 apart share a key
-  *reinterpret_cast<uint4*>(s + at) = t.x[0];
-  *reinterpret_cast<uint4*>(s + at + 32 * 128) = t.x[1];
+// Where a lane (group g, place c in it) reads and writes in a tile.  A tile_key takes bits 1 to 3 of a row, so steps of
+// 16 rows are plain offsets and steps along a row are exclusive ors: everything else is fixed once per launch.
+struct TileMap {
+  int row;      // row c, elements 8 g + [0, 8)                    (^ 64: 32 elements on, + 2048: 16 rows on)
+  int slots;    // row c, elements 4 g + [0, 4)                    (^ 32: 16 elements on, ^ 64: 32)
+  int column;   // rows 4 g + [0, 4), column c of the first 16     (^ 32 ct: column 16 ct + c, + 2048: 16 rows on)
+  int state;    // row c, elements 16 w + 4 g + [0, 4)             (+ 2048: 16 rows on)
+  int put;      // row threadIdx.x / 8, piece threadIdx.x % 8      (+ 4096: 32 rows on)
+  __device__ __forceinline__ TileMap() {
+    const int l = threadIdx.x % kWave, w = threadIdx.x / kWave % 4, g = l / 16, c = l % 16;
+    row = tile_at(c, 16 * g);
+    slots = tile_at(c, 8 * g);
+    column = tile_at(4 * g + c / 4, 8 * (c % 4));
+    state = tile_at(c, 32 * w + 8 * g);
+    put = tile_at(threadIdx.x >> 3, (threadIdx.x & 7) * 16);
+  }
+};
+__device__ __forceinline__ void tile_put(const TileRegs& t, char* s, const TileMap& m) {
+  *reinterpret_cast<uint4*>(s + m.put) = t.x[0];
+  *reinterpret_cast<uint4*>(s + m.put + 4096) = t.x[1];
 }
-// Row r, elements 32 ks + 8 g + [0, 8).
-__device__ __forceinline__ bf16x8 tile_row(const char* s, int r, int ks) {
-  return bf16x8_from_bits(*reinterpret_cast<const uint4*>(s + tile_at(r, 64 * ks + 16 * ((threadIdx.x % kWave) / 16))));
+// The same for a workgroup of 512 threads: row tid / 8, piece tid % 8.
+__device__ __forceinline__ uint4 tile_fetch_wide(const bf16* base, int64_t stride, int n) {
+  const int ld = static_cast<int>(stride) * 2;
+  return buf_load16(rows_rsrc(base, ld, n, 128), (threadIdx.x >> 3) * static_cast<uint32_t>(ld) + (threadIdx.x & 7) * 16);
 }
-// Row r, elements in slot order: 32 ks + 4 g + [0, 4) and 32 ks + 16 + 4 g + [0, 4).
-__device__ __forceinline__ bf16x8 tile_row_slots(const char* s, int r, int ks) {
-  const int b = 64 * ks + 8 * ((threadIdx.x % kWave) / 16);
-  const uint2 lo = *reinterpret_cast<const uint2*>(s + tile_at(r, b)), hi = *reinterpret_cast<const uint2*>(s + tile_at(r, b + 32));
+__device__ __forceinline__ void tile_put_wide(uint4 x, char* s, const TileMap& m) { *reinterpret_cast<uint4*>(s + m.put) = x; }
+// Row 16 rt + c, elements 32 ks + 8 g + [0, 8).
+__device__ __forceinline__ bf16x8 tile_row(const char* s, const TileMap& m, int rt, int ks) {
+  return bf16x8_from_bits(*reinterpret_cast<const uint4*>(s + (m.row ^ 64 * ks) + 2048 * rt));
+}
+// Row 16 rt + c, elements in slot order: 32 ks + 4 g + [0, 4) and 32 ks + 16 + 4 g + [0, 4).
+__device__ __forceinline__ bf16x8 tile_row_slots(const char* s, const TileMap& m, int rt, int ks) {
+  const uint2 lo = *reinterpret_cast<const uint2*>(s + (m.slots ^ 64 * ks) + 2048 * rt);
+  const uint2 hi = *reinterpret_cast<const uint2*>(s + (m.slots ^ 64 * ks ^ 32) + 2048 * rt);
   return bf16x8_from_bits(uint4{lo.x, lo.y, hi.x, hi.y});
 }
-// Column 16 ct + lane % 16 of the 32 rows from 32 ks, in slot order.
-__device__ __forceinline__ bf16x8 tile_column(const char* s, int ct, int ks) {
+// Column 16 ct + c of the 32 rows from 32 ks, in slot order.
+__device__ __forceinline__ bf16x8 tile_column(const char* s, const TileMap& m, int ct, int ks) {
   typedef short i16x8 __attribute__((ext_vector_type(8)));
-  const int l = threadIdx.x % kWave, r = 32 * ks + 4 * (l / 16) + (l % 16) / 4, byte = 32 * ct + 8 * (l % 4);
-  const i16x4 lo = lds_read_tr16(s + tile_at(r, byte)), hi = lds_read_tr16(s + tile_at(r + 16, byte));
+  const char* p = s + (m.column ^ 32 * ct) + 4096 * ks;
+  const i16x4 lo = lds_read_tr16(p), hi = lds_read_tr16(p + 2048);
   const i16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   return __builtin_bit_cast(bf16x8, v);
 }
@@ -394,58 +416,94 @@ __device__ __forceinline__ void split8(float* x, bf16x8* parts) {
   }
 }
 
-// The wave's 16 rows of the state (rows 16 w + 4 g + r, column 16 ct + c) into two LDS tiles of the transposed state:
-// its high parts, and behind them what those leave.
-__device__ __forceinline__ void state_put(const f32x4* M, char* s) {
-  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave, g = l / 16, c = l % 16;
+// The wave's rows of the state (rows 16 w + 4 g + r, CT column tiles from ct0, column 16 ct + c) into two LDS tiles of
+// the transposed state: its high parts, and behind them what those leave.
+template <int CT>
+__device__ __forceinline__ void state_put(const f32x4* M, char* s, const TileMap& m, int ct0) {
 #pragma unroll
-  for (int ct = 0; ct < 4; ++ct) {
+  for (int ct = 0; ct < CT; ++ct) {
     float x[4] = {M[ct][0], M[ct][1], M[ct][2], M[ct][3]};
-    const int at = tile_at(16 * ct + c, 2 * (16 * w + 4 * g));
-    *reinterpret_cast<uint2*>(s + at) = uint2{split_pair(x[0], x[1]), split_pair(x[2], x[3])};
-    *reinterpret_cast<uint2*>(s + kTileBytes + at) = uint2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+    char* at = s + m.state + 2048 * (ct0 + ct);
+    *reinterpret_cast<uint2*>(at) = uint2{split_pair(x[0], x[1]), split_pair(x[2], x[3])};
+    *reinterpret_cast<uint2*>(at + kTileBytes) = uint2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
   }
 }
 
-// Weights of the slots' tokens in the state's sum: forward us g^{n-1-j}, reverse us g^{j+1}.
-template <bool REV>
-__device__ __forceinline__ void slot_weights(float lg, int n, float us, float* wt) {
-  const int g = (threadIdx.x % kWave) / 16;
+// A chunk's weights in the adjoint's sum, us g^{j+1}, in factors: token 32 ks + 16 h + 4 g + r has base[r] tile[2 ks + h],
+// the second uniform.
+struct AdjointWeights {
+  float base[4], tile[4];
+  __device__ __forceinline__ AdjointWeights(float lg, float us) {
+    const int g = (threadIdx.x % kWave) / 16;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int j = 32 * (i / 8) + (i & 4 ? 16 : 0) + 4 * g + (i & 3);
-    const int p = REV ? j + 1 : n - 1 - j;
-    wt[i] = us * la_power(lg, p < 0 ? 0 : p);   // tokens behind the last are zero rows
+    for (int r = 0; r < 4; ++r) {
+      base[r] = us * la_power(lg, 4 * g + r + 1);
+      tile[r] = __uint_as_float(uniform(__float_as_uint(la_power(lg, 16 * r))));
+    }
+  }
+  __device__ __forceinline__ void apply(int ks, float factor, float* x) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= base[e & 3] * (tile[2 * ks + (e >> 2)] * factor);
+  }
+};
+// In the state's sum, g^{n-1-j}, from LDS tables: of a whole chunk, and of the last chunk of n tokens behind it (its dead
+// rows are zero, their weight only has to be finite).
+constexpr int kTableBytes = 2 * kChunk * 4;
+__device__ __forceinline__ void state_weights_put(float lg, int n_last, float* s) {
+  const int j = threadIdx.x;
+  if (j < 2 * kChunk) {
+    const int n = j < kChunk ? kChunk : n_last, p = n - 1 - (j & (kChunk - 1));
+    s[j] = la_power(lg, p < 0 ? 0 : p);
   }
 }
+struct StateWeights {
+  const float* s;   // the chunk's table
+  __device__ __forceinline__ StateWeights(const float* tables, int n) : s(tables + (n < kChunk ? kChunk : 0)) {}
+  __device__ __forceinline__ void apply(int ks, float, float* x) const {
+    const float* p = s + 32 * ks + 4 * ((threadIdx.x % kWave) / 16);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 w = *reinterpret_cast<const float4*>(p + 16 * h);
+      x[4 * h] *= w.x; x[4 * h + 1] *= w.y; x[4 * h + 2] *= w.z; x[4 * h + 3] *= w.w;
+    }
+  }
+};
 
-// M = shrink M + sum_j wt_j X_j Y_j^T for the wave's 16 columns of X and all of Y; y holds Y's columns.
-__device__ __forceinline__ void state_update(const char* sX, const bf16x8 (*y)[4], const float* wt, float shrink, f32x4* M) {
-  const int w = threadIdx.x / kWave;
-#pragma unroll
-  for (int ct = 0; ct < 4; ++ct)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) M[ct][r] *= shrink;
+// M += factor sum_j weight_j X_j Y_j^T for the wave's 16 columns of X and CT tiles of Y's columns from ct0.  PARTS: of
+// the weighted X, three where the sum itself is a result, two where it only goes into rows that are rounded to bf16.
+template <int CT, int PARTS, typename W>
+__device__ __forceinline__ void state_add(const char* sX, const char* sY, const TileMap& m, int w, int ct0, const W& weights,
+                                          float factor, f32x4* M) {
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
+    bf16x8 y[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) y[ct] = tile_column(sY, m, ct0 + ct, ks);
     float x[8];
-    unpack8(tile_column(sX, w, ks), x);
+    unpack8(tile_column(sX, m, w, ks), x);
+    weights.apply(ks, factor, x);
+    bf16x8 parts[PARTS];
+    split8<PARTS>(x, parts);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= wt[8 * ks + e];
-    bf16x8 parts[3];
-    split8<3>(x, parts);
+    for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-    for (int p = 0; p < 3; ++p)
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct) M[ct] = mfma16_bf16(parts[p], y[ks][ct], M[ct]);
+      for (int ct = 0; ct < CT; ++ct) M[ct] = mfma16_bf16(parts[p], y[ct], M[ct]);
   }
 }
-
-__device__ __forceinline__ void state_load(const float* en, bool trans, f32x4* M) {
-  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave, g = l / 16, c = l % 16;
+template <int CT>
+__device__ __forceinline__ void state_shrink(f32x4* M, float shrink) {
 #pragma unroll
-  for (int ct = 0; ct < 4; ++ct) {
-    const int i = 16 * w + 4 * g, j = 16 * ct + c;
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) M[ct][r] *= shrink;
+}
+
+template <int CT>
+__device__ __forceinline__ void state_load(const float* en, bool trans, int ct0, f32x4* M) {
+  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave % 4, g = l / 16, c = l % 16;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int i = 16 * w + 4 * g, j = 16 * (ct0 + ct) + c;
     if (!en) M[ct] = zero4();
     else if (trans) M[ct] = *reinterpret_cast<const f32x4*>(en + j * kHd + i);
     else
@@ -454,7 +512,7 @@ __device__ __forceinline__ void state_load(const float* en, bool trans, f32x4* M
   }
 }
 __device__ __forceinline__ void state_store(const f32x4* M, float* out) {
-  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave, g = l / 16, c = l % 16;
+  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave % 4, g = l / 16, c = l % 16;
 #pragma unroll
   for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
@@ -469,20 +527,18 @@ __device__ __forceinline__ void put4(float* p, const float* v) {
   *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
 
-// Work item of a workgroup: the query heads of a shared K/V head next to each other on one XCD, then the segments.
+// Work item of a workgroup: the heads of one segment next to each other on one XCD (token-major rows of the heads lie
+// side by side in memory, and query heads share their K/V head's rows), then the segments.
 struct LaItem {
   int b, h, seg;
   int64_t at;   // (b, h, seg) in the state arrays
 };
 __device__ __forceinline__ LaItem la_item(const LaGeom& gm) {
-  const int group = gm.H / gm.Hkv;
   const int i = xcd_remap(blockIdx.x, gridDim.x);
   LaItem it;
-  const int hq = i % group, rest = i / group;
-  it.seg = rest % gm.segs;
-  const int kv = rest / gm.segs % gm.Hkv;
-  it.b = rest / gm.segs / gm.Hkv;
-  it.h = kv * group + hq;
+  it.h = i % gm.H;
+  it.seg = i / gm.H % gm.segs;
+  it.b = i / gm.H / gm.segs;
   it.at = (static_cast<int64_t>(it.b) * gm.H + it.h) * gm.segs + it.seg;
   return it;
 }
@@ -493,124 +549,169 @@ __device__ __forceinline__ const bf16* la_rows_of(const LaRows& x, int heads, co
 template <typename TO>
 __device__ __forceinline__ void la_zero_rows(TO* po, int64_t o2, int from, int to) {
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = from * (kHd / 4) + threadIdx.x; i < to * (kHd / 4); i += kLaThreads)
+  for (int i = from * (kHd / 4) + threadIdx.x; i < to * (kHd / 4); i += blockDim.x)
     put4(po + static_cast<int64_t>(i / (kHd / 4)) * o2 + i % (kHd / 4) * 4, zero);
 }
 
+template <int WAVES>
 __device__ __forceinline__ float workgroup_sum(float x, float* s_red) {   // in thread 0
   x = lanes_sum<kWave>(x);
   __syncthreads();
   if (threadIdx.x % kWave == 0) s_red[threadIdx.x / kWave] = x;
   __syncthreads();
-  return ((s_red[0] + s_red[1]) + s_red[2]) + s_red[3];
+  float t = s_red[0];
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i) t += s_red[i];
+  return t;
 }
 
-// Segment sums (see la_local_kernel).
-template <bool REV>
-__global__ __launch_bounds__(kLaThreads) void la_local_bf16(LaRows X_, int xh, LaRows Y_, int yh, LaGeom gm, float us,
-                                                            float* __restrict__ local) {
-  __shared__ __align__(16) char smem[4 * kTileBytes];   // two chunks of X and Y
+// Segment sums of the forward (see la_local_kernel).  The loads of two chunks are issued at once.
+constexpr int kLocalAhead = 2;
+__global__ __launch_bounds__(kLaThreads, 4) void la_local_bf16(LaRows X_, int xh, LaRows Y_, int yh, LaGeom gm,
+                                                               float* __restrict__ local) {
+  __shared__ __align__(16) char smem[4 * kTileBytes + kTableBytes];   // two chunks of X and Y
   const LaItem it = la_item(gm);
   const int len = la_length(gm, it.b), t0 = it.seg * gm.seg;
   if (t0 >= len) return;
   const int t1 = t0 + gm.seg < len ? t0 + gm.seg : len;
   const float lg = la_log2_decay(gm, it.h), full = la_power(lg, kChunk);
   const bf16 *px = la_rows_of(X_, xh, gm, it), *py = la_rows_of(Y_, yh, gm, it);
-  const int chunks = (t1 - t0 + kChunk - 1) / kChunk;
-  auto token = [&](int i) { return t0 + (REV ? chunks - 1 - i : i) * kChunk; };
-  auto fetch = [&](TileRegs& x, TileRegs& y, int i) {
-    const int t = token(i < chunks ? i : chunks - 1);
-    tile_fetch(x, px + t * X_.s2, X_.s2, t1 - t < kChunk ? t1 - t : kChunk);
-    tile_fetch(y, py + t * Y_.s2, Y_.s2, t1 - t < kChunk ? t1 - t : kChunk);
-  };
+  const int chunks = (t1 - t0 + kChunk - 1) / kChunk, w = uniform(threadIdx.x / kWave);
+  const TileMap m;
   f32x4 M[4] = {zero4(), zero4(), zero4(), zero4()};
-  float wt[16];
-  slot_weights<REV>(lg, kChunk, us, wt);
-  TileRegs x, y;
-  fetch(x, y, 0);
-  for (int i = 0; i < chunks; ++i) {
-    char* s = smem + (i & 1) * 2 * kTileBytes;
-    tile_put(x, s);
-    tile_put(y, s + kTileBytes);
-    __syncthreads();   // also: every wave is done with the other buffer
-    fetch(x, y, i + 1);
-    const int t = token(i), n = t1 - t < kChunk ? t1 - t : kChunk;
-    if (n < kChunk) slot_weights<REV>(lg, n, us, wt);   // the last chunk: at the end, or first of all in reverse
-    bf16x8 yc[2][4];
+  const float* tables = reinterpret_cast<const float*>(smem + 4 * kTileBytes);   // written before the first barrier
+  state_weights_put(lg, t1 - t0 - (chunks - 1) * kChunk, reinterpret_cast<float*>(smem + 4 * kTileBytes));
+  for (int i0 = 0; i0 < chunks; i0 += kLocalAhead) {
+    TileRegs x[kLocalAhead], y[kLocalAhead];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
+    for (int u = 0; u < kLocalAhead; ++u) {
+      const int t = t0 + (i0 + u) * kChunk;
+      const int n = i0 + u < chunks ? (t1 - t < kChunk ? t1 - t : kChunk) : 0;   // 0: reads nothing
+      tile_fetch(x[u], px + t * X_.s2, X_.s2, n);
+      tile_fetch(y[u], py + t * Y_.s2, Y_.s2, n);
+    }
 #pragma unroll
-      for (int ct = 0; ct < 4; ++ct) yc[ks][ct] = tile_column(s + kTileBytes, ct, ks);
-    state_update(s, yc, wt, n < kChunk ? la_power(lg, n) : full, M);
+    for (int u = 0; u < kLocalAhead; ++u) {
+      if (i0 + u < chunks) {   // uniform
+        char* s = smem + (u & 1) * 2 * kTileBytes;
+        tile_put(x[u], s, m);
+        tile_put(y[u], s + kTileBytes, m);
+        __syncthreads();   // also: every wave is done with the other buffer
+        const int t = t0 + (i0 + u) * kChunk, n = t1 - t < kChunk ? t1 - t : kChunk;
+        state_shrink<4>(M, n < kChunk ? la_power(lg, n) : full);
+        state_add<4, 3>(s, s + kTileBytes, m, w, 0, StateWeights(tables, n), 1.f, M);
+      }
+    }
   }
   state_store(M, local + it.at * kState);
 }
 
-// The forward's rows, and with other operands dq (see la_rows_kernel): out_i = scale (sum_{j <= i} g^{i-j} (A_i.X_j) Y_j
-// + g^{i+1} A_i M).  LDS: two chunks of X and Y, the state's two parts.
-template <bool TRANS>
-__global__ __launch_bounds__(kLaThreads) void la_rows_bf16(LaRows A_, int ah, LaRows X_, int xh, LaRows Y_, int yh,
-                                                           LaGeom gm, const float* __restrict__ enter,
-                                                           bf16* __restrict__ out, int64_t o0, int64_t o1, int64_t o2,
-                                                           float* __restrict__ leave, LaRows D_, int dh,
-                                                           float* __restrict__ dot) {
-  __shared__ __align__(16) char smem[8 * kTileBytes];
-  __shared__ float s_red[kLaThreads / kWave];
+// Scores' weights of a lane: rows 4 g + r of a tile of the other side's tokens against its own token c.  near: one
+// tile away (gap 1 and up), diagonal: the same tile, 0 where the other token lies on the wrong side.
+struct ScoreWeights {
+  float diagonal[4], near[4], tile;   // tile: 16 tokens' decay
+  __device__ __forceinline__ ScoreWeights(float lg, float scale, bool other_behind) {
+    const int l = threadIdx.x % kWave, g = l / 16, c = l % 16;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = other_behind ? 4 * g + r - c : c - 4 * g - r;
+      diagonal[r] = d >= 0 ? scale * la_power(lg, d) : 0.f;
+      near[r] = scale * la_power(lg, d + 16);
+    }
+    tile = la_power(lg, 16);
+  }
+  // scores against a tile `away` tiles off (uniform), weighted; away < 0: none of it counts
+  __device__ __forceinline__ void apply(f32x4 s, int away, float* p) const {
+    const float far = away <= 1 ? 1.f : away == 2 ? tile : tile * tile;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[r] = away == 0 ? s[r] * diagonal[r] : s[r] * (near[r] * far);
+  }
+};
+
+// The workgroups that form rows have eight waves: four with 16 rows each, and four that keep the state (forward, dq)
+// or form the other gradient (dk beside dv), so that neither part's registers keep a CU from holding sixteen waves.
+constexpr int kWideThreads = 512;
+
+// out_i = scale (sum_{j <= i} g^{i-j} (q_i.k_j) v_j + g^{i+1} q_i S) over a segment's chunks.  LDS: two chunks of k and v
+// and the two parts of the state in front of each.  enter: the state in front of each segment or, with one segment, of
+// each head (NULL: zero); leave: with one segment, where the last state goes.
+__global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRows K_, LaRows V_, LaGeom gm,
+                                                                const float* __restrict__ enter, bf16* __restrict__ out,
+                                                                int64_t o0, int64_t o1, int64_t o2,
+                                                                float* __restrict__ leave) {
+  __shared__ __align__(16) char smem[8 * kTileBytes + kTableBytes];
   const LaItem it = la_item(gm);
-  const int l = threadIdx.x % kWave, w = uniform(threadIdx.x / kWave), g = l / 16, c = l % 16;
+  const int l = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), w = wave % 4, g = l / 16, c = l % 16;
+  const bool keeps = wave >= 4;   // this wave keeps the state
   const int len = la_length(gm, it.b), t0 = it.seg * gm.seg;
   const int tend = t0 + gm.seg < gm.N ? t0 + gm.seg : gm.N;
   const int t1 = tend < len ? tend : len;
   bf16* po = out + it.b * o0 + it.h * o1;
   la_zero_rows(po, o2, t1 > t0 ? t1 : t0, tend);
-  const float lg = la_log2_decay(gm, it.h), full = la_power(lg, kChunk);
-  const bf16 *pa = la_rows_of(A_, ah, gm, it), *px = la_rows_of(X_, xh, gm, it), *py = la_rows_of(Y_, yh, gm, it);
-  const bf16* pd = dot ? la_rows_of(D_, dh, gm, it) : nullptr;
-  f32x4 M[4];
-  state_load(enter ? enter + it.at * kState : nullptr, TRANS, M);
+  const float lg = la_log2_decay(gm, it.h);
+  const bf16 *pq = la_rows_of(Q_, gm.H, gm, it), *pk = la_rows_of(K_, gm.Hkv, gm, it), *pv = la_rows_of(V_, gm.Hkv, gm, it);
+  const TileMap m;
   const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
-  TileRegs x, y;
-  bf16x8 a[2], a_next[2];
-  auto fetch = [&](int i) {
-    const int t = t0 + (i < chunks ? i : chunks - 1) * kChunk, n = t1 - t < kChunk ? t1 - t : kChunk;
-    tile_fetch(x, px + t * X_.s2, X_.s2, n);
-    tile_fetch(y, py + t * Y_.s2, Y_.s2, n);
-    const int ld = static_cast<int>(A_.s2) * 2;
-    const __amdgpu_buffer_rsrc_t r = rows_rsrc(pa + t * A_.s2, ld, n, 128);
-    const uint32_t off = static_cast<uint32_t>(16 * w + c) * static_cast<uint32_t>(ld) + 16 * g;
-    a_next[0] = bf16x8_from_bits(buf_load16(r, off));
-    a_next[1] = bf16x8_from_bits(buf_load16(r, off + 64));
+  auto live = [&](int i) { return i < chunks ? (t1 - t0 - i * kChunk < kChunk ? t1 - t0 - i * kChunk : kChunk) : 0; };
+  uint4 x, y;
+  auto fetch = [&](int i) {   // behind the last chunk: reads nothing
+    const int64_t t = t0 + static_cast<int64_t>(i) * kChunk;
+    x = tile_fetch_wide(pk + t * K_.s2, K_.s2, live(i));
+    y = tile_fetch_wide(pv + t * V_.s2, V_.s2, live(i));
   };
-  // scores' weights, tokens 16 (w - jt) apart: on the diagonal, one tile before it (from 1 up), and whole tiles
-  float w0[4], w1[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int d = c - 4 * g - r;
-    w0[r] = d >= 0 ? gm.scale * la_power(lg, d) : 0.f;
-    w1[r] = gm.scale * la_power(lg, d + 16);
+  const float* tables = reinterpret_cast<const float*>(smem + 8 * kTileBytes);   // written before the first barrier
+  state_weights_put(lg, live(chunks - 1), reinterpret_cast<float*>(smem + 8 * kTileBytes));
+  fetch(0);
+  if (keeps) {
+    f32x4 M[4];
+    state_load<4>(enter ? enter + it.at * kState : nullptr, false, 0, M);
+    state_put<4>(M, smem + 2 * kTileBytes, m, 0);
+    const float full = la_power(lg, kChunk);
+    for (int i = 0; i < chunks; ++i) {
+      char *s = smem + (i & 1) * 4 * kTileBytes, *other = smem + (~i & 1) * 4 * kTileBytes;
+      tile_put_wide(x, s, m);
+      tile_put_wide(y, s + kTileBytes, m);
+      __syncthreads();   // also: every wave is done with the other buffer
+      fetch(i + 1);
+      const int n = live(i);
+      state_shrink<4>(M, n < kChunk ? la_power(lg, n) : full);
+      const StateWeights wt(tables, n);
+      if (leave) state_add<4, 3>(s, s + kTileBytes, m, w, 0, wt, 1.f, M);   // uniform
+      else state_add<4, 2>(s, s + kTileBytes, m, w, 0, wt, 1.f, M);
+      state_put<4>(M, other + 2 * kTileBytes, m, 0);
+    }
+    if (leave) state_store(M, leave + it.at * kState);
+    return;
   }
-  const float tile16 = la_power(lg, 16), carry = gm.scale * la_power(lg, 16 * w + c + 1);
-  float wt[16];
-  slot_weights<false>(lg, kChunk, 1.f, wt);
-  const float mid = 0.5f * static_cast<float>(gm.seg);
-  float total = 0.f;
-  if (chunks) fetch(0);
+  const ScoreWeights sw(lg, gm.scale, false);
+  const float carry = gm.scale * la_power(lg, 16 * w + c + 1);
+  uint4 qn[2];
+  auto fetch_q = [&](int i) {
+    const int ld = static_cast<int>(Q_.s2) * 2;
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(pq + (t0 + static_cast<int64_t>(i) * kChunk) * Q_.s2, ld, live(i), 128);
+    const uint32_t off = static_cast<uint32_t>(16 * w + c) * static_cast<uint32_t>(ld) + 16 * g;
+    qn[0] = buf_load16(r, off);
+    qn[1] = buf_load16(r, off + 64);
+  };
+  fetch_q(0);
   for (int i = 0; i < chunks; ++i) {
-    const int t = t0 + i * kChunk, n = t1 - t < kChunk ? t1 - t : kChunk;
-    char *sX = smem + (i & 1) * 4 * kTileBytes, *sY = sX + kTileBytes, *sM = sX + 2 * kTileBytes;
-    tile_put(x, sX);
-    tile_put(y, sY);
-    state_put(M, sM);
-    a[0] = a_next[0];
-    a[1] = a_next[1];
-    __syncthreads();   // also: every wave is done with the other buffer
+    char* s = smem + (i & 1) * 4 * kTileBytes;
+    tile_put_wide(x, s, m);
+    tile_put_wide(y, s + kTileBytes, m);
+    const bf16x8 a[2] = {bf16x8_from_bits(qn[0]), bf16x8_from_bits(qn[1])};
+    __syncthreads();
     fetch(i + 1);
-    bf16x8 yc[2][4];
+    fetch_q(i + 1);
+    const char *sK = s, *sV = s + kTileBytes, *sM = s + 2 * kTileBytes;
+    f32x4 o[4] = {zero4(), zero4(), zero4(), zero4()};
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
+    for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
-      for (int ct = 0; ct < 4; ++ct) yc[ks][ct] = tile_column(sY, ct, ks);
-    f32x4 o[4] = {zero4(), zero4(), zero4(), zero4()}, z[4] = {zero4(), zero4(), zero4(), zero4()};
+      for (int ks = 0; ks < 2; ++ks) {
+        o[ct] = mfma16_bf16(tile_row(sM, m, ct, ks), a[ks], o[ct]);
+        o[ct] = mfma16_bf16(tile_row(sM + kTileBytes, m, ct, ks), a[ks], o[ct]);
+      }
+    state_shrink<4>(o, carry);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       if (2 * ks <= w) {   // uniform: some of the 32 tokens are not behind the wave's rows
@@ -618,70 +719,284 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_bf16(LaRows A_, int ah, La
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int jt = 2 * ks + half;
-          f32x4 s = zero4();
+          f32x4 z = zero4();
           if (jt <= w) {
-            s = mfma16_bf16(tile_row(sX, 16 * jt + c, 0), a[0], s);
-            s = mfma16_bf16(tile_row(sX, 16 * jt + c, 1), a[1], s);
+            z = mfma16_bf16(tile_row(sK, m, jt, 0), a[0], z);
+            z = mfma16_bf16(tile_row(sK, m, jt, 1), a[1], z);
           }
-          const float far = w - jt <= 1 ? 1.f : w - jt == 2 ? tile16 : tile16 * tile16;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) p[4 * half + r] = jt == w ? s[r] * w0[r] : s[r] * (w1[r] * far);
+          sw.apply(z, w - jt, p + 4 * half);
         }
         bf16x8 parts[2];
         split8<2>(p, parts);
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-          for (int ct = 0; ct < 4; ++ct) o[ct] = mfma16_bf16(yc[ks][ct], parts[q], o[ct]);
-      }
-    }
-#pragma unroll
-    for (int ct = 0; ct < 4; ++ct)
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        z[ct] = mfma16_bf16(tile_row(sM, 16 * ct + c, ks), a[ks], z[ct]);
-        z[ct] = mfma16_bf16(tile_row(sM + kTileBytes, 16 * ct + c, ks), a[ks], z[ct]);
-      }
-    const int row = 16 * w + c;
-    if (row < n) {
-      bf16* pr = po + (t + row) * o2;
-      float sum = 0.f;
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct) {
-        float v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = fmaf(carry, z[ct][r], o[ct][r]);
-        put4(pr + 16 * ct + 4 * g, v);
-        if (pd) {
-          const uint2 dd = *reinterpret_cast<const uint2*>(pd + (t + row) * D_.s2 + 16 * ct + 4 * g);
-          sum = fmaf(v[0], bf16_lo(dd.x), fmaf(v[1], bf16_hi(dd.x), fmaf(v[2], bf16_lo(dd.y), fmaf(v[3], bf16_hi(dd.y), sum))));
+        for (int ct = 0; ct < 4; ++ct) {
+          const bf16x8 v = tile_column(sV, m, ct, ks);
+          o[ct] = mfma16_bf16(v, parts[0], o[ct]);
+          o[ct] = mfma16_bf16(v, parts[1], o[ct]);
         }
       }
-      total = fmaf(static_cast<float>(t - t0 + row + 1) - mid, sum, total);
     }
-    if (n < kChunk) slot_weights<false>(lg, n, 1.f, wt);
-    state_update(sX, yc, wt, n < kChunk ? la_power(lg, n) : full, M);
+    if (16 * w + c < live(i)) {
+      bf16* pr = po + (t0 + static_cast<int64_t>(i) * kChunk + 16 * w + c) * o2;
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        const float v[4] = {o[ct][0], o[ct][1], o[ct][2], o[ct][3]};
+        put4(pr + 16 * ct + 4 * g, v);
+      }
+    }
   }
-  if (leave) state_store(M, leave + it.at * kState);
+}
+
+// dq_i = scale (sum_{j <= i} g^{i-j} (do_i.v_j) k_j + g^{i+1} do_i S^T), and from the same tiles the segment's own sum
+// of the adjoint, local = sum_i scale g^{i+1} q_i do_i^T (NULL: not wanted): one pass over q and do instead of two.  The
+// four state waves keep both.  LDS: one chunk of v, k, q and do, and the two parts of S^T in front of this and the next.
+__global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows O_, LaRows K_, LaRows V_, LaGeom gm,
+                                                              const float* __restrict__ enter, bf16* __restrict__ dq,
+                                                              int64_t o0, int64_t o1, int64_t o2,
+                                                              float* __restrict__ local, float* __restrict__ dot) {
+  __shared__ __align__(16) char smem[8 * kTileBytes + kTableBytes];
+  const LaItem it = la_item(gm);
+  const int l = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), w = wave % 4, g = l / 16, c = l % 16;
+  const bool keeps = wave >= 4;
+  const int len = la_length(gm, it.b), t0 = it.seg * gm.seg;
+  const int tend = t0 + gm.seg < gm.N ? t0 + gm.seg : gm.N;
+  const int t1 = tend < len ? tend : len;
+  bf16* po = dq + it.b * o0 + it.h * o1;
+  la_zero_rows(po, o2, t1 > t0 ? t1 : t0, tend);
+  const float lg = la_log2_decay(gm, it.h);
+  const bf16 *pq = la_rows_of(Q_, gm.H, gm, it), *pdo = la_rows_of(O_, gm.H, gm, it);
+  const bf16 *pk = la_rows_of(K_, gm.Hkv, gm, it), *pv = la_rows_of(V_, gm.Hkv, gm, it);
+  const TileMap m;
+  const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
+  auto live = [&](int i) { return i < chunks ? (t1 - t0 - i * kChunk < kChunk ? t1 - t0 - i * kChunk : kChunk) : 0; };
+  char *sV = smem, *sK = smem + kTileBytes, *sQ = smem + 2 * kTileBytes, *sO = smem + 3 * kTileBytes;
+  uint4 x[4];
+  auto fetch = [&](int i) {
+    const int64_t t = t0 + static_cast<int64_t>(i) * kChunk;
+    x[0] = tile_fetch_wide(pv + t * V_.s2, V_.s2, live(i));
+    x[1] = tile_fetch_wide(pk + t * K_.s2, K_.s2, live(i));
+    x[2] = tile_fetch_wide(pq + t * Q_.s2, Q_.s2, live(i));
+    x[3] = tile_fetch_wide(pdo + t * O_.s2, O_.s2, live(i));
+  };
+  auto put = [&]() {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) tile_put_wide(x[u], smem + u * kTileBytes, m);
+  };
+  const float* tables = reinterpret_cast<const float*>(smem + 8 * kTileBytes);   // written before the first barrier
+  state_weights_put(lg, live(chunks - 1), reinterpret_cast<float*>(smem + 8 * kTileBytes));
+  fetch(0);
+  float total = 0.f;
+  if (keeps) {
+    f32x4 M[4], L[4] = {zero4(), zero4(), zero4(), zero4()};
+    state_load<4>(enter ? enter + it.at * kState : nullptr, true, 0, M);
+    state_put<4>(M, smem + 4 * kTileBytes, m, 0);
+    const float full = la_power(lg, kChunk);
+    const AdjointWeights wl(lg, gm.scale);
+    float past = 1.f;
+    for (int i = 0; i < chunks; ++i) {
+      put();
+      __syncthreads();
+      fetch(i + 1);
+      const int n = live(i);
+      state_shrink<4>(M, n < kChunk ? la_power(lg, n) : full);
+      state_add<4, 2>(sV, sK, m, w, 0, StateWeights(tables, n), 1.f, M);
+      if (local) {
+        state_add<4, 3>(sQ, sO, m, w, 0, wl, past, L);
+        past *= full;
+      }
+      state_put<4>(M, smem + (i & 1 ? 4 : 6) * kTileBytes, m, 0);
+      __syncthreads();   // every wave is done with the tiles
+    }
+    if (local && chunks) state_store(L, local + it.at * kState);
+  } else {
+    const ScoreWeights sw(lg, gm.scale, false);
+    const float carry = gm.scale * la_power(lg, 16 * w + c + 1), mid = 0.5f * static_cast<float>(gm.seg);
+    for (int i = 0; i < chunks; ++i) {
+      put();
+      __syncthreads();
+      fetch(i + 1);
+      const char* sM = smem + (i & 1 ? 6 : 4) * kTileBytes;
+      const bf16x8 a[2] = {tile_row(sO, m, w, 0), tile_row(sO, m, w, 1)};
+      f32x4 o[4] = {zero4(), zero4(), zero4(), zero4()};
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          o[ct] = mfma16_bf16(tile_row(sM, m, ct, ks), a[ks], o[ct]);
+          o[ct] = mfma16_bf16(tile_row(sM + kTileBytes, m, ct, ks), a[ks], o[ct]);
+        }
+      state_shrink<4>(o, carry);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (2 * ks <= w) {
+          float p[8];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int jt = 2 * ks + half;
+            f32x4 z = zero4();
+            if (jt <= w) {
+              z = mfma16_bf16(tile_row(sV, m, jt, 0), a[0], z);
+              z = mfma16_bf16(tile_row(sV, m, jt, 1), a[1], z);
+            }
+            sw.apply(z, w - jt, p + 4 * half);
+          }
+          bf16x8 parts[2];
+          split8<2>(p, parts);
+#pragma unroll
+          for (int ct = 0; ct < 4; ++ct) {
+            const bf16x8 k = tile_column(sK, m, ct, ks);
+            o[ct] = mfma16_bf16(k, parts[0], o[ct]);
+            o[ct] = mfma16_bf16(k, parts[1], o[ct]);
+          }
+        }
+      }
+      const int row = 16 * w + c;
+      if (row < live(i)) {
+        bf16* pr = po + (t0 + static_cast<int64_t>(i) * kChunk + row) * o2;
+        float sum = 0.f;
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) {
+          const float v[4] = {o[ct][0], o[ct][1], o[ct][2], o[ct][3]};
+          put4(pr + 16 * ct + 4 * g, v);
+          if (dot) {
+            const uint2 q = *reinterpret_cast<const uint2*>(sQ + (m.slots ^ 32 * ct) + 2048 * w);
+            sum = fmaf(v[0], bf16_lo(q.x), fmaf(v[1], bf16_hi(q.x), fmaf(v[2], bf16_lo(q.y), fmaf(v[3], bf16_hi(q.y), sum))));
+          }
+        }
+        total = fmaf(static_cast<float>(i * kChunk + row + 1) - mid, sum, total);
+      }
+      __syncthreads();   // every wave is done with the tiles
+    }
+  }
   if (dot) {
-    total = workgroup_sum(total, s_red);
+    total = workgroup_sum<kWideThreads / kWave>(total, reinterpret_cast<float*>(smem));
     if (threadIdx.x == 0) dot[it.at] = total;
   }
 }
 
+// One gradient of la_dkdv_bf16: dv, with its rows of k from LDS, or (KEYS) dk, with its rows of v in registers.
+template <bool KEYS, typename TO>
+__device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, const LaRows& O_, const LaRows& K_, const LaRows& V_,
+                                              const LaGeom& gm, const LaItem& it, int t0, int t1,
+                                              const float* __restrict__ enter, TO* __restrict__ pr, int64_t stride, bool dot) {
+  const int l = threadIdx.x % kWave, w = uniform(threadIdx.x / kWave) % 4, g = l / 16, c = l % 16;
+  const float lg = la_log2_decay(gm, it.h), full = la_power(lg, kChunk);
+  const bf16 *pq = la_rows_of(Q_, gm.H, gm, it), *pdo = la_rows_of(O_, gm.H, gm, it);
+  const bf16 *pv = la_rows_of(V_, gm.Hkv, gm, it), *pk = la_rows_of(K_, gm.Hkv, gm, it);
+  const TileMap m;
+  f32x4 G[4];
+  if constexpr (!KEYS) state_load<4>(enter ? enter + it.at * kState : nullptr, false, 0, G);
+  const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
+  // chunk i counts from the end; behind the first one nothing is live
+  auto live = [&](int i) { return i >= chunks ? 0 : i > 0 ? kChunk : t1 - t0 - (chunks - 1) * kChunk; };
+  auto token = [&](int i) { return t0 + static_cast<int64_t>(i < chunks ? chunks - 1 - i : 0) * kChunk; };
+  uint4 xq, xo, xk, own[2];
+  auto fetch = [&](int i) {
+    const int64_t t = token(i);
+    xq = tile_fetch_wide(pq + t * Q_.s2, Q_.s2, live(i));
+    xo = tile_fetch_wide(pdo + t * O_.s2, O_.s2, live(i));
+    xk = tile_fetch_wide(pk + t * K_.s2, K_.s2, live(i));
+    if constexpr (KEYS) {   // v in slot order: elements 32 p + 4 g + [0, 4) and 16 on
+      const int ld = static_cast<int>(V_.s2) * 2;
+      const __amdgpu_buffer_rsrc_t r = rows_rsrc(pv + t * V_.s2, ld, live(i), 128);
+      const uint32_t row = static_cast<uint32_t>(16 * w + c) * static_cast<uint32_t>(ld) + 8 * g;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const auto a = __builtin_amdgcn_raw_buffer_load_b64(r, row + 64 * p, 0, 0);
+        const auto b = __builtin_amdgcn_raw_buffer_load_b64(r, row + 64 * p + 32, 0, 0);
+        own[p] = uint4{a[0], a[1], b[0], b[1]};
+      }
+    }
+  };
+  const ScoreWeights sw(lg, gm.scale, true);
+  const AdjointWeights wt(lg, gm.scale);
+  const float mid = 0.5f * static_cast<float>(gm.seg);
+  float total = 0.f;
+  fetch(0);
+  for (int i = 0; i < chunks; ++i) {
+    const int n = live(i);
+    char *sQ = smem + (i & 1) * 5 * kTileBytes, *sO = sQ + kTileBytes, *sK = sQ + 2 * kTileBytes, *sG = sQ + 3 * kTileBytes;
+    tile_put_wide(xq, sQ, m);
+    tile_put_wide(xo, sO, m);
+    tile_put_wide(xk, sK, m);
+    if constexpr (!KEYS) state_put<4>(G, sG, m, 0);
+    bf16x8 a[2] = {bf16x8_from_bits(own[0]), bf16x8_from_bits(own[1])};
+    __syncthreads();   // also: every wave is done with the other buffer
+    fetch(i + 1);
+    if constexpr (!KEYS) {
+      a[0] = tile_row(sK, m, w, 0);
+      a[1] = tile_row(sK, m, w, 1);
+    }
+    const int row = 16 * w + c;
+    f32x4 acc[4] = {zero4(), zero4(), zero4(), zero4()};
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          const char* s = sG + part * kTileBytes;
+          acc[ct] = mfma16_bf16(KEYS ? tile_column(s, m, ct, ks) : tile_row(s, m, ct, ks), a[ks], acc[ct]);
+        }
+    state_shrink<4>(acc, la_power(lg, n - 1 - row < 0 ? 0 : n - 1 - row));
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      if (2 * ks + 1 >= w) {   // uniform: some of the 32 tokens are not before the wave's rows
+        float p[8];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int tt = 2 * ks + hf;
+          f32x4 z = zero4();
+          if (tt >= w) {
+            z = mfma16_bf16(KEYS ? tile_row_slots(sO, m, tt, 0) : tile_row(sQ, m, tt, 0), a[0], z);
+            z = mfma16_bf16(KEYS ? tile_row_slots(sO, m, tt, 1) : tile_row(sQ, m, tt, 1), a[1], z);
+          }
+          sw.apply(z, tt - w, p + 4 * hf);
+        }
+        bf16x8 parts[2];
+        split8<2>(p, parts);
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) {
+          const bf16x8 v = tile_column(KEYS ? sQ : sO, m, ct, ks);
+          acc[ct] = mfma16_bf16(v, parts[0], acc[ct]);
+          acc[ct] = mfma16_bf16(v, parts[1], acc[ct]);
+        }
+      }
+    }
+    if (row < n) {
+      const int64_t t = token(i) + row;
+      float sum = 0.f;
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        const float v[4] = {acc[ct][0], acc[ct][1], acc[ct][2], acc[ct][3]};
+        put4(pr + t * stride + 16 * ct + 4 * g, v);
+        if (KEYS && dot) {
+          const uint2 k = *reinterpret_cast<const uint2*>(sK + (m.slots ^ 32 * ct) + 2048 * w);
+          sum = fmaf(v[0], bf16_lo(k.x), fmaf(v[1], bf16_hi(k.x), fmaf(v[2], bf16_lo(k.y), fmaf(v[3], bf16_hi(k.y), sum))));
+        }
+      }
+      total = fmaf(static_cast<float>(t - t0 + 1) - mid, sum, total);
+    }
+    if constexpr (!KEYS) {
+      state_shrink<4>(G, n < kChunk ? la_power(lg, n) : full);
+      state_add<4, 2>(sQ, sO, m, w, 0, wt, 1.f, G);
+    }
+  }
+  return total;
+}
+
 // dk and dv of a segment, chunks from its end, G the adjoint of the state behind the chunk:
 //   dv_j = scale sum_{i >= j} g^{i-j} (k_j.q_i) do_i + g^{n-1-j} k_j G,  dk_j the same with v, do, q and G^T.
-// The q and do tiles serve as rows and as columns; G lies in LDS transposed, read by rows for dv and transposed for dk.
+// Four waves form dv and keep G, and four form dk.  The q and do tiles serve as rows and
+// as columns; G lies in LDS transposed, read by rows for dv and transposed for dk.  Both roles pass the same barriers.
 template <typename TO>
-__global__ __launch_bounds__(kLaThreads, 2) void la_dkdv_bf16(LaRows Q_, LaRows O_, LaRows K_, LaRows V_, LaGeom gm,
-                                                              const float* __restrict__ enter, TO* __restrict__ dk,
-                                                              int64_t k0, int64_t k1, int64_t k2, TO* __restrict__ dv,
-                                                              int64_t v0, int64_t v1, int64_t v2, int outh,
-                                                              float* __restrict__ dot) {
-  __shared__ __align__(16) char smem[8 * kTileBytes];
-  __shared__ float s_red[kLaThreads / kWave];
+__global__ __launch_bounds__(kWideThreads, 4) void la_dkdv_bf16(LaRows Q_, LaRows O_, LaRows K_, LaRows V_, LaGeom gm,
+                                                                const float* __restrict__ enter, TO* __restrict__ dk,
+                                                                int64_t k0, int64_t k1, int64_t k2, TO* __restrict__ dv,
+                                                                int64_t v0, int64_t v1, int64_t v2, int outh,
+                                                                float* __restrict__ dot) {
+  __shared__ __align__(16) char smem[10 * kTileBytes];   // two chunks of q, do and k, and G's two parts for each
   const LaItem it = la_item(gm);
-  const int l = threadIdx.x % kWave, w = uniform(threadIdx.x / kWave), g = l / 16, c = l % 16;
   const int len = la_length(gm, it.b), t0 = it.seg * gm.seg;
   const int tend = t0 + gm.seg < gm.N ? t0 + gm.seg : gm.N;
   const int t1 = tend < len ? tend : len;
@@ -689,137 +1004,11 @@ __global__ __launch_bounds__(kLaThreads, 2) void la_dkdv_bf16(LaRows Q_, LaRows 
   TO *pdk = dk + it.b * k0 + oh * k1, *pdv = dv + it.b * v0 + oh * v1;
   la_zero_rows(pdk, k2, t1 > t0 ? t1 : t0, tend);
   la_zero_rows(pdv, v2, t1 > t0 ? t1 : t0, tend);
-  const float lg = la_log2_decay(gm, it.h), full = la_power(lg, kChunk);
-  const bf16 *pq = la_rows_of(Q_, gm.H, gm, it), *pdo = la_rows_of(O_, gm.H, gm, it);
-  const bf16 *pk = la_rows_of(K_, gm.Hkv, gm, it), *pv = la_rows_of(V_, gm.Hkv, gm, it);
-  f32x4 G[4];
-  state_load(enter ? enter + it.at * kState : nullptr, false, G);
-  const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
-  TileRegs xq, xo;
-  uint4 kn[2];
-  uint2 vn[4];
-  auto fetch = [&](int i) {
-    const int t = t0 + (i < chunks ? chunks - 1 - i : 0) * kChunk, n = t1 - t < kChunk ? t1 - t : kChunk;
-    tile_fetch(xq, pq + t * Q_.s2, Q_.s2, n);
-    tile_fetch(xo, pdo + t * O_.s2, O_.s2, n);
-    const int lk = static_cast<int>(K_.s2) * 2, lv = static_cast<int>(V_.s2) * 2;
-    const __amdgpu_buffer_rsrc_t rk = rows_rsrc(pk + t * K_.s2, lk, n, 128), rv = rows_rsrc(pv + t * V_.s2, lv, n, 128);
-    const uint32_t ok = static_cast<uint32_t>(16 * w + c) * static_cast<uint32_t>(lk) + 16 * g;
-    const uint32_t ov = static_cast<uint32_t>(16 * w + c) * static_cast<uint32_t>(lv) + 8 * g;
-    kn[0] = buf_load16(rk, ok);
-    kn[1] = buf_load16(rk, ok + 64);
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {   // slot order: elements 16 p + 4 g + [0, 4)
-      const auto x = __builtin_amdgcn_raw_buffer_load_b64(rv, ov + 32 * p, 0, 0);
-      vn[p] = uint2{x[0], x[1]};
-    }
-  };
-  // scores' weights, own tokens j before i = 16 it + 4 g + r: on the diagonal, one tile behind it, and whole tiles
-  float w0[4], w1[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int d = 4 * g + r - c;
-    w0[r] = d >= 0 ? gm.scale * la_power(lg, d) : 0.f;
-    w1[r] = gm.scale * la_power(lg, d + 16);
-  }
-  const float tile16 = la_power(lg, 16);
-  float wt[16];
-  slot_weights<true>(lg, kChunk, gm.scale, wt);
-  const float mid = 0.5f * static_cast<float>(gm.seg);
-  float total = 0.f;
-  if (chunks) fetch(0);
-  for (int i = 0; i < chunks; ++i) {
-    const int t = t0 + (chunks - 1 - i) * kChunk, n = t1 - t < kChunk ? t1 - t : kChunk;
-    char *sQ = smem + (i & 1) * 4 * kTileBytes, *sO = sQ + kTileBytes, *sG = sQ + 2 * kTileBytes;
-    tile_put(xq, sQ);
-    tile_put(xo, sO);
-    state_put(G, sG);
-    const bf16x8 ka[2] = {bf16x8_from_bits(kn[0]), bf16x8_from_bits(kn[1])};
-    const bf16x8 va[2] = {bf16x8_from_bits(uint4{vn[0].x, vn[0].y, vn[1].x, vn[1].y}),
-                          bf16x8_from_bits(uint4{vn[2].x, vn[2].y, vn[3].x, vn[3].y})};
-    __syncthreads();   // also: every wave is done with the other buffer
-    fetch(i + 1);
-    const int row = 16 * w + c;
-    const float carry = la_power(lg, n - 1 - row < 0 ? 0 : n - 1 - row);
-    bf16x8 oc[2][4];
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct) oc[ks][ct] = tile_column(sO, ct, ks);
-    f32x4 av[4] = {zero4(), zero4(), zero4(), zero4()}, ak[4] = {zero4(), zero4(), zero4(), zero4()};
-    // carried parts first, in the same accumulators: (g^{n-1-j} X G) / then the scores' parts on top
-#pragma unroll
-    for (int ct = 0; ct < 4; ++ct)
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        av[ct] = mfma16_bf16(tile_row(sG, 16 * ct + c, ks), ka[ks], av[ct]);
-        av[ct] = mfma16_bf16(tile_row(sG + kTileBytes, 16 * ct + c, ks), ka[ks], av[ct]);
-        ak[ct] = mfma16_bf16(tile_column(sG, ct, ks), va[ks], ak[ct]);
-        ak[ct] = mfma16_bf16(tile_column(sG + kTileBytes, ct, ks), va[ks], ak[ct]);
-      }
-#pragma unroll
-    for (int ct = 0; ct < 4; ++ct)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        av[ct][r] *= carry;
-        ak[ct][r] *= carry;
-      }
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if (2 * ks + 1 >= w) {   // uniform: some of the 32 tokens are not before the wave's rows
-        float p1[8], p2[8];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int tt = 2 * ks + half;
-          f32x4 s1 = zero4(), s2 = zero4();
-          if (tt >= w) {
-            s1 = mfma16_bf16(tile_row(sQ, 16 * tt + c, 0), ka[0], s1);
-            s1 = mfma16_bf16(tile_row(sQ, 16 * tt + c, 1), ka[1], s1);
-            s2 = mfma16_bf16(tile_row_slots(sO, 16 * tt + c, 0), va[0], s2);
-            s2 = mfma16_bf16(tile_row_slots(sO, 16 * tt + c, 1), va[1], s2);
-          }
-          const float far = tt - w <= 1 ? 1.f : tt - w == 2 ? tile16 : tile16 * tile16;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float weight = tt == w ? w0[r] : w1[r] * far;
-            p1[4 * half + r] = s1[r] * weight;
-            p2[4 * half + r] = s2[r] * weight;
-          }
-        }
-        bf16x8 h1[2], h2[2];
-        split8<2>(p1, h1);
-        split8<2>(p2, h2);
-#pragma unroll
-        for (int ct = 0; ct < 4; ++ct) {
-          const bf16x8 qc = tile_column(sQ, ct, ks);
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            av[ct] = mfma16_bf16(oc[ks][ct], h1[q], av[ct]);
-            ak[ct] = mfma16_bf16(qc, h2[q], ak[ct]);
-          }
-        }
-      }
-    }
-    if (row < n) {
-      TO *rk = pdk + (t + row) * k2, *rv = pdv + (t + row) * v2;
-      float sum = 0.f;
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct) {
-        const float vk[4] = {ak[ct][0], ak[ct][1], ak[ct][2], ak[ct][3]};
-        const float vv[4] = {av[ct][0], av[ct][1], av[ct][2], av[ct][3]};
-        put4(rk + 16 * ct + 4 * g, vk);
-        put4(rv + 16 * ct + 4 * g, vv);
-        if (dot) {
-          const uint2 dd = *reinterpret_cast<const uint2*>(pk + (t + row) * K_.s2 + 16 * ct + 4 * g);
-          sum = fmaf(vk[0], bf16_lo(dd.x), fmaf(vk[1], bf16_hi(dd.x), fmaf(vk[2], bf16_lo(dd.y), fmaf(vk[3], bf16_hi(dd.y), sum))));
-        }
-      }
-      total = fmaf(static_cast<float>(t - t0 + row + 1) - mid, sum, total);
-    }
-    state_update(sQ, oc, wt, n < kChunk ? la_power(lg, n) : full, G);
-  }
+  float total;
+  if (uniform(threadIdx.x / kWave) >= 4) total = la_dkdv_role<true>(smem, Q_, O_, K_, V_, gm, it, t0, t1, enter, pdk, k2, dot != nullptr);
+  else total = la_dkdv_role<false>(smem, Q_, O_, K_, V_, gm, it, t0, t1, enter, pdv, v2, false);
   if (dot) {
-    total = workgroup_sum(total, s_red);
+    total = workgroup_sum<kWideThreads / kWave>(total, reinterpret_cast<float*>(smem));
     if (threadIdx.x == 0) dot[it.at] = total;
   }
 }
@@ -940,8 +1129,8 @@ __global__ __launch_bounds__(kStepThreads) void la_step_kernel(dwarf_linear_atte
 }
 
 int la_segment(int64_t B, int64_t H, int64_t N) {
-  for (int seg = 256; seg > kChunk; seg /= 2)
-    if (B * H * ((N + seg - 1) / seg) >= 512) return seg;
+  for (int seg = 512; seg > kChunk; seg /= 2)
+    if (B * H * ((N + seg - 1) / seg) >= 448) return seg;
   return kChunk;
 }
 
@@ -964,16 +1153,15 @@ void la_fwd_bf16(const dwarf_linear_attention_fwd_args& a, const LaGeom& gm, hip
   const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * gm.segs), block(kLaThreads);
   const float* enter = a.initial;
   if (gm.segs > 1) {
-    hipLaunchKernelGGL((la_local_bf16<false>), grid, block, 0, stream, k, gm.Hkv, v, gm.Hkv, gm, 1.f, a.states);
+    hipLaunchKernelGGL(la_local_bf16, grid, block, 0, stream, k, gm.Hkv, v, gm.Hkv, gm, a.states);
     enter = a.states;
   }
   if (gm.segs != 1)
     hipLaunchKernelGGL((la_scan_kernel<false>), dim3(gm.B * gm.H * kScanWgs), block, 0, stream, a.states, a.initial,
                        a.final, gm, nullptr, nullptr, nullptr, nullptr);
   if (gm.segs == 0) return;
-  hipLaunchKernelGGL((la_rows_bf16<false>), grid, block, 0, stream, q, gm.H, k, gm.Hkv, v, gm.Hkv, gm, enter,
-                     static_cast<bf16*>(a.out), a.out_stride[0], a.out_stride[1], a.out_stride[2],
-                     gm.segs == 1 ? a.final : nullptr, LaRows{}, 1, nullptr);
+  hipLaunchKernelGGL(la_rows_bf16, grid, dim3(kWideThreads), 0, stream, q, k, v, gm, enter, static_cast<bf16*>(a.out),
+                     a.out_stride[0], a.out_stride[1], a.out_stride[2], gm.segs == 1 ? a.final : nullptr);
 }
 
 template <typename T>
@@ -1031,24 +1219,24 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
   const bool shared = gm.H != gm.Hkv;
   float *pk = ws + sp.dk_part, *pv = ws + sp.dv_part;
   const int64_t s1 = static_cast<int64_t>(gm.N) * kHd, s0 = s1 * gm.H;   // of the shared heads' parts
-  if (joined && gm.segs) {
-    if constexpr (std::is_same<T, bf16>::value)
-      hipLaunchKernelGGL((la_local_bf16<true>), grid, block, 0, stream, q, gm.H, dout, gm.H, gm, gm.scale, adj);
-    else
-      hipLaunchKernelGGL((la_local_kernel<T, true>), grid, block, 0, stream, q, gm.H, dout, gm.H, gm, gm.scale, adj);
+  const dim3 wide(kWideThreads);
+  if constexpr (std::is_same<T, bf16>::value) {
+    if (gm.segs)
+      hipLaunchKernelGGL(la_dq_bf16, grid, wide, 0, stream, q, dout, k, v, gm, before, static_cast<bf16*>(a.dq),
+                         a.dq_stride[0], a.dq_stride[1], a.dq_stride[2], joined ? adj : nullptr, dq_dot);
+  } else if (joined && gm.segs) {
+    hipLaunchKernelGGL((la_local_kernel<T, true>), grid, block, 0, stream, q, gm.H, dout, gm.H, gm, gm.scale, adj);
   }
   if (joined)
     hipLaunchKernelGGL((la_scan_kernel<true>), dim3(gm.B * gm.H * kScanWgs), block, 0, stream, adj, a.dfinal, a.dinitial,
                        gm, f.states, f.initial, f.final, edge);
   if (gm.segs) {
     if constexpr (std::is_same<T, bf16>::value) {
-      hipLaunchKernelGGL((la_rows_bf16<true>), grid, block, 0, stream, dout, gm.H, v, gm.Hkv, k, gm.Hkv, gm, before,
-                         static_cast<bf16*>(a.dq), a.dq_stride[0], a.dq_stride[1], a.dq_stride[2], nullptr, q, gm.H, dq_dot);
       if (shared)
-        hipLaunchKernelGGL((la_dkdv_bf16<float>), grid, block, 0, stream, q, dout, k, v, gm, enter, pk, s0, s1, kHd, pv,
+        hipLaunchKernelGGL((la_dkdv_bf16<float>), grid, wide, 0, stream, q, dout, k, v, gm, enter, pk, s0, s1, kHd, pv,
                            s0, s1, kHd, gm.H, dk_dot);
       else
-        hipLaunchKernelGGL((la_dkdv_bf16<bf16>), grid, block, 0, stream, q, dout, k, v, gm, enter, static_cast<bf16*>(a.dk),
+        hipLaunchKernelGGL((la_dkdv_bf16<bf16>), grid, wide, 0, stream, q, dout, k, v, gm, enter, static_cast<bf16*>(a.dk),
                            a.dk_stride[0], a.dk_stride[1], a.dk_stride[2], static_cast<bf16*>(a.dv), a.dv_stride[0],
                            a.dv_stride[1], a.dv_stride[2], gm.Hkv, dk_dot);
     } else {
