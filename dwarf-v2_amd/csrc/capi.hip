@@ -961,6 +961,8 @@ static int check_linear_attention(const dwarf_linear_attention_fwd_args& a) {
     return fail(DWARF_ERR_UNSUPPORTED, "N up to 2^24 and B * H * N / 64 below 2^31");
   if (a.B == 0) return DWARF_OK;
   if (!a.log_decay) return fail(DWARF_ERR_INVALID_ARGUMENT, "log_decay is NULL");
+  if ((a.initial && !aligned16(a.initial)) || (a.final && !aligned16(a.final)))
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "initial and final must be 16-byte aligned");
   if (a.N == 0) return DWARF_OK;
   if ((rc = check_rows("q", a.q, a.q_stride, 3, a.dtype))) return rc;
   if ((rc = check_rows("k", a.k, a.k_stride, 3, a.dtype))) return rc;
@@ -968,7 +970,6 @@ static int check_linear_attention(const dwarf_linear_attention_fwd_args& a) {
   if ((rc = check_chunk_rows("q", a.N, a.q_stride[2])) || (rc = check_chunk_rows("k", a.N, a.k_stride[2])) ||
       (rc = check_chunk_rows("v", a.N, a.v_stride[2])))
     return rc;
-  if (a.initial && !aligned16(a.initial)) return fail(DWARF_ERR_INVALID_ARGUMENT, "initial must be 16-byte aligned");
   const size_t need = dwarf::linear_attention_states_bytes(a);
   if (need && (!a.states || a.states_bytes < need || !aligned16(a.states)))
     return fail(DWARF_ERR_WORKSPACE, "states needs %zu bytes, 16-byte aligned, got %zu", need, a.states_bytes);
@@ -1012,6 +1013,8 @@ int dwarf_linear_attention_bwd(const dwarf_linear_attention_bwd_args* args, dwar
     if ((rc = check_rows("dv", a.dv, a.dv_stride, 3, a.fwd.dtype))) return rc;
     if ((rc = check_chunk_rows("dout", a.fwd.N, a.dout_stride[2]))) return rc;
   }
+  if ((a.dfinal && !aligned16(a.dfinal)) || (a.dinitial && !aligned16(a.dinitial)))
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "dfinal and dinitial must be 16-byte aligned");
   if (a.dlog_decay && a.dfinal && !a.fwd.final)
     return fail(DWARF_ERR_INVALID_ARGUMENT, "dlog_decay with dfinal needs the final state");
   const size_t need = dwarf::linear_attention_bwd_workspace(a);

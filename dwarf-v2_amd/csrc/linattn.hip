@@ -144,56 +144,116 @@ __global__ __launch_bounds__(kLaThreads) void la_local_kernel(LaRows B_, int bh,
     for (int r = 0; r < 4; ++r) out[(16 * w + 4 * (l / 16) + r) * kHd + 16 * ct + l % 16] = acc[ct][r];
 }
 
-// Turns the segment sums in place into the state in front of each segment (reverse: the adjoint behind it); a thread
-// owns one element of one head's state.  first: the state that enters (NULL: zero), last: where the one that leaves
-// goes (NULL: nowhere).  Reverse with dot: the boundary terms of dlog_decay, per workgroup.
-constexpr int kScanWgs = kState / kLaThreads;
-constexpr int kScanAhead = 8;
-template <bool REV>
+// Turns the segment sums in place into the state in front of each segment (reverse: the adjoint behind it).  first: the
+// state that enters (NULL: zero), last: where the one that leaves goes (NULL: nowhere).  Reverse with dot: the boundary
+// terms of dlog_decay, per workgroup.
+//
+// A thread owns four neighbouring elements of one head's state and up to kScanRun segments in a row, all loaded at once;
+// GROUPS threads share the elements, each with a run of its own, and join their runs through LDS.  GROUPS is 1 up to
+// kScanRun segments, and 16 above: a long sequence's segments would otherwise be read one memory latency after another.
+constexpr int kScanRun = 8;
+template <int GROUPS>
+constexpr int kScanWgs = kState / 4 * GROUPS / kLaThreads;   // workgroups per head
+int scan_wgs(const LaGeom& gm) { return gm.segs > kScanRun ? kScanWgs<16> : kScanWgs<1>; }
+
+template <bool REV, int GROUPS>
 __global__ __launch_bounds__(kLaThreads) void la_scan_kernel(float* __restrict__ local, const float* __restrict__ first,
                                                              float* __restrict__ last, LaGeom gm,
                                                              const float* __restrict__ states,
                                                              const float* __restrict__ initial,
                                                              const float* __restrict__ final, float* __restrict__ dot) {
+  constexpr int kOwners = kLaThreads / GROUPS;   // threads of a group
+  __shared__ f32x4 s_run[GROUPS][kOwners];
   __shared__ float s_red[kLaThreads / kWave];
-  const int bh = blockIdx.x / kScanWgs, e = blockIdx.x % kScanWgs * kLaThreads + threadIdx.x;
+  const int bh = blockIdx.x / kScanWgs<GROUPS>, owner = threadIdx.x % kOwners, group = threadIdx.x / kOwners;
+  const int e = 4 * (blockIdx.x % kScanWgs<GROUPS> * kOwners + owner);
   const int b = bh / gm.H, h = bh % gm.H;
   const int len = la_length(gm, b), active = (len + gm.seg - 1) / gm.seg;
   const float lg = la_log2_decay(gm, h);
-  const float full = la_power(lg, gm.seg), tail = active ? la_power(lg, len - (active - 1) * gm.seg) : 1.f;
+  const int n_last = active ? len - (active - 1) * gm.seg : 0;
+  const float full = la_power(lg, gm.seg), tail = la_power(lg, n_last), run_full = la_power(lg, gm.seg * kScanRun);
   float* x = local + static_cast<int64_t>(bh) * gm.segs * kState + e;
   const float* st = states ? states + static_cast<int64_t>(bh) * gm.segs * kState + e : nullptr;
   const int64_t at = static_cast<int64_t>(bh) * kState + e;
+  auto load = [](const float* p) { return *reinterpret_cast<const f32x4*>(p); };
   const float mid = 0.5f * static_cast<float>(gm.seg);
-  float m = first ? first[at] : 0.f, sum = 0.f;
-  if (REV && dot && final && active) sum = (static_cast<float>(len - (active - 1) * gm.seg) - mid) * m * final[at];
-  for (int s0 = 0; s0 < active; s0 += kScanAhead) {
-    float in[kScanAhead], sv[kScanAhead];
-    const int cnt = active - s0 < kScanAhead ? active - s0 : kScanAhead;
+  f32x4 m = first ? load(first + at) : zero4();
+  float sum = 0.f;
+  auto add_dot = [&](float weight, f32x4 a, f32x4 c) {
+    sum = fmaf(weight, fmaf(a[0], c[0], fmaf(a[1], c[1], fmaf(a[2], c[2], a[3] * c[3]))), sum);
+  };
+  if (REV && dot && final && active && group == 0) add_dot(static_cast<float>(n_last) - mid, m, load(final + at));
+  // a pass takes GROUPS runs; position p counts segments in the direction of the scan
+  for (int p0 = 0; p0 < active; p0 += GROUPS * kScanRun) {
+    const int base = p0 + group * kScanRun;
+    const int cnt = active - base < kScanRun ? (active - base < 0 ? 0 : active - base) : kScanRun;
+    auto segment = [&](int i) { return static_cast<int64_t>(REV ? active - 1 - base - i : base + i); };
+    f32x4 in[kScanRun], sv[kScanRun];
 #pragma unroll
-    for (int i = 0; i < kScanAhead; ++i) {
-      const int s = REV ? active - 1 - s0 - i : s0 + i;
-      in[i] = i < cnt ? x[static_cast<int64_t>(s) * kState] : 0.f;
-      sv[i] = REV && dot && i < cnt && s > 0 ? st[static_cast<int64_t>(s) * kState] : 0.f;
+    for (int i = 0; i < kScanRun; ++i) {
+      in[i] = i < cnt ? load(x + segment(i) * kState) : zero4();
+      sv[i] = REV && dot && i < cnt && segment(i) > 0 ? load(st + segment(i) * kState) : zero4();
     }
+    auto shrink = [&](int i) { return segment(i) == active - 1 ? tail : full; };
+    f32x4 enter = m;
+    if constexpr (GROUPS > 1) {
+      f32x4 r = zero4();   // the run's own sum
 #pragma unroll
-    for (int i = 0; i < kScanAhead; ++i) {
-      if (i < cnt) {
-        const int s = REV ? active - 1 - s0 - i : s0 + i;
-        x[static_cast<int64_t>(s) * kState] = m;
-        m = fmaf(s == active - 1 ? tail : full, m, in[i]);
-        if (REV) sum = fmaf(static_cast<float>(gm.seg) * sv[i], m, sum);   // <S in front of s, G in front of s>
+      for (int i = 0; i < kScanRun; ++i)
+        if (i < cnt) r = r * shrink(i) + in[i];
+      __syncthreads();   // the pass before has been read
+      s_run[group][owner] = r;
+      __syncthreads();
+      for (int q = 0; q < GROUPS; ++q) {   // the runs in front are whole but for the sequence's last segment
+        if (q == group) enter = m;
+        const int behind = active - (p0 + q * kScanRun);   // segments from run q on
+        if (behind <= 0) break;
+        const bool whole = behind >= kScanRun;
+        // decay over run q: in the forward direction its last segment may be the tail, in reverse its first one is
+        float over = whole ? run_full : 1.f;
+        if (!whole)
+          for (int i = 0; i < behind; ++i) over *= full;
+        const bool has_tail = REV ? p0 + q * kScanRun == 0 : behind <= kScanRun;
+        if (has_tail) {
+          over = 1.f;
+          const int n = behind < kScanRun ? behind : kScanRun;
+          for (int i = 0; i + 1 < n; ++i) over *= full;
+          over *= tail;
+        }
+        m = m * over + s_run[q][owner];
       }
     }
+    f32x4 v = enter;
+#pragma unroll
+    for (int i = 0; i < kScanRun; ++i) {
+      if (i < cnt) {
+        *reinterpret_cast<f32x4*>(x + segment(i) * kState) = v;
+        v = v * shrink(i) + in[i];
+        if (REV && dot) add_dot(static_cast<float>(gm.seg), sv[i], v);   // <S in front of it, G in front of it>
+      }
+    }
+    if constexpr (GROUPS == 1) m = v;
   }
-  if (last) last[at] = m;
+  if (last && group == 0) *reinterpret_cast<f32x4*>(last + at) = m;
   if (REV && dot) {
-    if (initial && active) sum = fmaf(mid * initial[at], m, sum);
+    if (initial && active && group == 0) add_dot(mid, load(initial + at), m);
     sum = lanes_sum<kWave>(sum);
     if (threadIdx.x % kWave == 0) s_red[threadIdx.x / kWave] = sum;
     __syncthreads();
     if (threadIdx.x == 0) dot[blockIdx.x] = ((s_red[0] + s_red[1]) + s_red[2]) + s_red[3];
   }
+}
+
+template <bool REV>
+void la_scan(float* local, const float* first, float* last, const LaGeom& gm, const float* states, const float* initial,
+             const float* final, float* dot, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * scan_wgs(gm));
+  if (gm.segs > kScanRun)
+    hipLaunchKernelGGL((la_scan_kernel<REV, 16>), grid, dim3(kLaThreads), 0, stream, local, first, last, gm, states, initial,
+                       final, dot);
+  else
+    hipLaunchKernelGGL((la_scan_kernel<REV, 1>), grid, dim3(kLaThreads), 0, stream, local, first, last, gm, states, initial,
+                       final, dot);
 }
 
 // out_i = intra sum_j W_ij (A_i.B_j) C_j + cs W_i A_i M over a segment's chunks, M updated behind each (in front, in
@@ -336,10 +396,10 @@ __device__ __forceinline__ int tile_at(int r, int byte) { return r * 128 + ((((b
 struct TileRegs {
   uint4 x[2];
 };
-__device__ __forceinline__ void tile_fetch(TileRegs& t, const bf16* base, int64_t stride, int n) {
+__device__ __forceinline__ void tile_fetch(TileRegs& t, const bf16* base, int64_t stride, int n, int tid) {
   const int ld = static_cast<int>(stride) * 2;
   const __amdgpu_buffer_rsrc_t r = rows_rsrc(base, ld, n, 128);   // rows behind the n live ones read zeros
-  const uint32_t off = (threadIdx.x >> 3) * static_cast<uint32_t>(ld) + (threadIdx.x & 7) * 16;
+  const uint32_t off = (tid >> 3) * static_cast<uint32_t>(ld) + (tid & 7) * 16;
   t.x[0] = buf_load16(r, off);
   t.x[1] = buf_load16(r, off + 32u * static_cast<uint32_t>(ld));
 }
@@ -350,14 +410,14 @@ struct TileMap {
   int slots;    // row c, elements 4 g + [0, 4)                    (^ 32: 16 elements on, ^ 64: 32)
   int column;   // rows 4 g + [0, 4), column c of the first 16     (^ 32 ct: column 16 ct + c, + 2048: 16 rows on)
   int state;    // row c, elements 16 w + 4 g + [0, 4)             (+ 2048: 16 rows on)
-  int put;      // row threadIdx.x / 8, piece threadIdx.x % 8      (+ 4096: 32 rows on)
-  __device__ __forceinline__ TileMap() {
+  int put;      // row tid / 8, piece tid % 8                       (+ 4096: 32 rows on)
+  __device__ __forceinline__ explicit TileMap(int tid) {
     const int l = threadIdx.x % kWave, w = threadIdx.x / kWave % 4, g = l / 16, c = l % 16;
     row = tile_at(c, 16 * g);
     slots = tile_at(c, 8 * g);
     column = tile_at(4 * g + c / 4, 8 * (c % 4));
     state = tile_at(c, 32 * w + 8 * g);
-    put = tile_at(threadIdx.x >> 3, (threadIdx.x & 7) * 16);
+    put = tile_at(tid >> 3, (tid & 7) * 16);
   }
 };
 __device__ __forceinline__ void tile_put(const TileRegs& t, char* s, const TileMap& m) {
@@ -570,14 +630,14 @@ constexpr int kLocalAhead = 2;
 __global__ __launch_bounds__(kLaThreads, 4) void la_local_bf16(LaRows X_, int xh, LaRows Y_, int yh, LaGeom gm,
                                                                float* __restrict__ local) {
   __shared__ __align__(16) char smem[4 * kTileBytes + kTableBytes];   // two chunks of X and Y
-  const LaItem it = la_item(gm);
+  const LaItem it = la_item(gm);   // the rows' launch has the same items on the same XCDs and finds k and v in their L2
   const int len = la_length(gm, it.b), t0 = it.seg * gm.seg;
   if (t0 >= len) return;
   const int t1 = t0 + gm.seg < len ? t0 + gm.seg : len;
   const float lg = la_log2_decay(gm, it.h), full = la_power(lg, kChunk);
   const bf16 *px = la_rows_of(X_, xh, gm, it), *py = la_rows_of(Y_, yh, gm, it);
   const int chunks = (t1 - t0 + kChunk - 1) / kChunk, w = uniform(threadIdx.x / kWave);
-  const TileMap m;
+  const TileMap m(threadIdx.x);
   f32x4 M[4] = {zero4(), zero4(), zero4(), zero4()};
   const float* tables = reinterpret_cast<const float*>(smem + 4 * kTileBytes);   // written before the first barrier
   state_weights_put(lg, t1 - t0 - (chunks - 1) * kChunk, reinterpret_cast<float*>(smem + 4 * kTileBytes));
@@ -585,10 +645,10 @@ __global__ __launch_bounds__(kLaThreads, 4) void la_local_bf16(LaRows X_, int xh
     TileRegs x[kLocalAhead], y[kLocalAhead];
 #pragma unroll
     for (int u = 0; u < kLocalAhead; ++u) {
-      const int t = t0 + (i0 + u) * kChunk;
-      const int n = i0 + u < chunks ? (t1 - t < kChunk ? t1 - t : kChunk) : 0;   // 0: reads nothing
-      tile_fetch(x[u], px + t * X_.s2, X_.s2, n);
-      tile_fetch(y[u], py + t * Y_.s2, Y_.s2, n);
+      const int64_t t = t0 + static_cast<int64_t>(i0 + u) * kChunk;
+      const int n = i0 + u < chunks ? (t1 - t < kChunk ? static_cast<int>(t1 - t) : kChunk) : 0;   // 0: reads nothing
+      tile_fetch(x[u], px + t * X_.s2, X_.s2, n, threadIdx.x);
+      tile_fetch(y[u], py + t * Y_.s2, Y_.s2, n, threadIdx.x);
     }
 #pragma unroll
     for (int u = 0; u < kLocalAhead; ++u) {
@@ -634,7 +694,7 @@ constexpr int kWideThreads = 512;
 
 // out_i = scale (sum_{j <= i} g^{i-j} (q_i.k_j) v_j + g^{i+1} q_i S) over a segment's chunks.  LDS: two chunks of k and v
 // and the two parts of the state in front of each.  enter: the state in front of each segment or, with one segment, of
-// each head (NULL: zero); leave: with one segment, where the last state goes.
+// each head (NULL: zero); leave: with one segment, where the state behind it goes.
 __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRows K_, LaRows V_, LaGeom gm,
                                                                 const float* __restrict__ enter, bf16* __restrict__ out,
                                                                 int64_t o0, int64_t o1, int64_t o2,
@@ -650,7 +710,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
   la_zero_rows(po, o2, t1 > t0 ? t1 : t0, tend);
   const float lg = la_log2_decay(gm, it.h);
   const bf16 *pq = la_rows_of(Q_, gm.H, gm, it), *pk = la_rows_of(K_, gm.Hkv, gm, it), *pv = la_rows_of(V_, gm.Hkv, gm, it);
-  const TileMap m;
+  const TileMap m(threadIdx.x);
   const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
   auto live = [&](int i) { return i < chunks ? (t1 - t0 - i * kChunk < kChunk ? t1 - t0 - i * kChunk : kChunk) : 0; };
   uint4 x, y;
@@ -676,8 +736,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
       const int n = live(i);
       state_shrink<4>(M, n < kChunk ? la_power(lg, n) : full);
       const StateWeights wt(tables, n);
-      if (leave) state_add<4, 3>(s, s + kTileBytes, m, w, 0, wt, 1.f, M);   // uniform
-      else state_add<4, 2>(s, s + kTileBytes, m, w, 0, wt, 1.f, M);
+      state_add<4, 3>(s, s + kTileBytes, m, w, 0, wt, 1.f, M);   // (two parts would do where nothing leaves: no faster)
       state_put<4>(M, other + 2 * kTileBytes, m, 0);
     }
     if (leave) state_store(M, leave + it.at * kState);
@@ -766,7 +825,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
   const float lg = la_log2_decay(gm, it.h);
   const bf16 *pq = la_rows_of(Q_, gm.H, gm, it), *pdo = la_rows_of(O_, gm.H, gm, it);
   const bf16 *pk = la_rows_of(K_, gm.Hkv, gm, it), *pv = la_rows_of(V_, gm.Hkv, gm, it);
-  const TileMap m;
+  const TileMap m(threadIdx.x);
   const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
   auto live = [&](int i) { return i < chunks ? (t1 - t0 - i * kChunk < kChunk ? t1 - t0 - i * kChunk : kChunk) : 0; };
   char *sV = smem, *sK = smem + kTileBytes, *sQ = smem + 2 * kTileBytes, *sO = smem + 3 * kTileBytes;
@@ -883,7 +942,7 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
   const float lg = la_log2_decay(gm, it.h), full = la_power(lg, kChunk);
   const bf16 *pq = la_rows_of(Q_, gm.H, gm, it), *pdo = la_rows_of(O_, gm.H, gm, it);
   const bf16 *pv = la_rows_of(V_, gm.Hkv, gm, it), *pk = la_rows_of(K_, gm.Hkv, gm, it);
-  const TileMap m;
+  const TileMap m(threadIdx.x);
   f32x4 G[4];
   if constexpr (!KEYS) state_load<4>(enter ? enter + it.at * kState : nullptr, false, 0, G);
   const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
@@ -1035,7 +1094,7 @@ __global__ __launch_bounds__(kLaThreads) void la_group_sum(const float* __restri
 // dlog_decay[h]: the segments' sums over the batch, then the boundary terms; a workgroup per head, fixed order.
 __global__ __launch_bounds__(kLaThreads) void la_dlog_kernel(const float* __restrict__ dq_dot,
                                                              const float* __restrict__ dk_dot,
-                                                             const float* __restrict__ edge, LaGeom gm,
+                                                             const float* __restrict__ edge, int edges, LaGeom gm,
                                                              float* __restrict__ dlog) {
   __shared__ float s_red[kLaThreads / kWave];
   const int h = blockIdx.x;
@@ -1050,8 +1109,8 @@ __global__ __launch_bounds__(kLaThreads) void la_dlog_kernel(const float* __rest
     }
   }
   if (edge)
-    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(gm.B) * kScanWgs; i += kLaThreads)
-      t += edge[(i / kScanWgs * gm.H + h) * kScanWgs + i % kScanWgs];
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(gm.B) * edges; i += kLaThreads)
+      t += edge[(i / edges * gm.H + h) * edges + i % edges];
   t = lanes_sum<kWave>(t);
   if (threadIdx.x % kWave == 0) s_red[threadIdx.x / kWave] = t;
   __syncthreads();
@@ -1150,15 +1209,14 @@ LaRows la_operand(const void* p, const int64_t* s, int N) { return LaRows{p, s[0
 
 void la_fwd_bf16(const dwarf_linear_attention_fwd_args& a, const LaGeom& gm, hipStream_t stream) {
   const LaRows q = la_operand(a.q, a.q_stride, gm.N), k = la_operand(a.k, a.k_stride, gm.N), v = la_operand(a.v, a.v_stride, gm.N);
-  const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * gm.segs), block(kLaThreads);
+  const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * gm.segs);
   const float* enter = a.initial;
   if (gm.segs > 1) {
-    hipLaunchKernelGGL(la_local_bf16, grid, block, 0, stream, k, gm.Hkv, v, gm.Hkv, gm, a.states);
+    hipLaunchKernelGGL(la_local_bf16, grid, dim3(kLaThreads), 0, stream, k, gm.Hkv, v, gm.Hkv, gm, a.states);
     enter = a.states;
   }
   if (gm.segs != 1)
-    hipLaunchKernelGGL((la_scan_kernel<false>), dim3(gm.B * gm.H * kScanWgs), block, 0, stream, a.states, a.initial,
-                       a.final, gm, nullptr, nullptr, nullptr, nullptr);
+    la_scan<false>(a.states, a.initial, a.final, gm, nullptr, nullptr, nullptr, nullptr, stream);
   if (gm.segs == 0) return;
   hipLaunchKernelGGL(la_rows_bf16, grid, dim3(kWideThreads), 0, stream, q, k, v, gm, enter, static_cast<bf16*>(a.out),
                      a.out_stride[0], a.out_stride[1], a.out_stride[2], gm.segs == 1 ? a.final : nullptr);
@@ -1174,8 +1232,7 @@ void la_fwd_typed(const dwarf_linear_attention_fwd_args& a, const LaGeom& gm, hi
     enter = a.states;
   }
   if (gm.segs != 1)
-    hipLaunchKernelGGL((la_scan_kernel<false>), dim3(gm.B * gm.H * kScanWgs), block, 0, stream, a.states, a.initial,
-                       a.final, gm, nullptr, nullptr, nullptr, nullptr);
+    la_scan<false>(a.states, a.initial, a.final, gm, nullptr, nullptr, nullptr, nullptr, stream);
   if (gm.segs == 0) return;
   hipLaunchKernelGGL((la_rows_kernel<T, T, false, false>), grid, block, 0, stream, q, gm.H, k, gm.Hkv, v, gm.Hkv, gm,
                      gm.scale, gm.scale, 1.f, enter, static_cast<T*>(a.out), a.out_stride[0], a.out_stride[1],
@@ -1195,7 +1252,7 @@ LaBwdSpace la_bwd_space(const dwarf_linear_attention_bwd_args& a, const LaGeom& 
   s.adjoint = at; at += wgs * kState;
   s.dq_dot = at; at += a.dlog_decay ? pad(wgs) : 0;
   s.dk_dot = at; at += a.dlog_decay ? pad(wgs) : 0;
-  s.edge = at; at += a.dlog_decay ? pad(static_cast<size_t>(gm.B) * gm.H * kScanWgs) : 0;
+  s.edge = at; at += a.dlog_decay ? pad(static_cast<size_t>(gm.B) * gm.H * scan_wgs(gm)) : 0;
   s.dk_part = at; at += shared ? rows : 0;
   s.dv_part = at; at += shared ? rows : 0;
   s.total = at;
@@ -1228,8 +1285,7 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
     hipLaunchKernelGGL((la_local_kernel<T, true>), grid, block, 0, stream, q, gm.H, dout, gm.H, gm, gm.scale, adj);
   }
   if (joined)
-    hipLaunchKernelGGL((la_scan_kernel<true>), dim3(gm.B * gm.H * kScanWgs), block, 0, stream, adj, a.dfinal, a.dinitial,
-                       gm, f.states, f.initial, f.final, edge);
+    la_scan<true>(adj, a.dfinal, a.dinitial, gm, f.states, f.initial, f.final, edge, stream);
   if (gm.segs) {
     if constexpr (std::is_same<T, bf16>::value) {
       if (shared)
@@ -1267,8 +1323,8 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
     }
   }
   if (dlog)
-    hipLaunchKernelGGL(la_dlog_kernel, dim3(gm.H), block, 0, stream, gm.segs ? dq_dot : nullptr, dk_dot, edge, gm,
-                       a.dlog_decay);
+    hipLaunchKernelGGL(la_dlog_kernel, dim3(gm.H), block, 0, stream, gm.segs ? dq_dot : nullptr, dk_dot, edge,
+                       scan_wgs(gm), gm, a.dlog_decay);
 }
 
 }  // namespace

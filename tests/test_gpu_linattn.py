@@ -124,6 +124,34 @@ def test_gradients(pkg, device, B, H, Hkv, N, initial, lengths, dtype):
     within(got["log_decay"], want["log_decay"], 3 * 256 * flow, torch.float32, slack(dtype))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("B,H,Hkv,N,lengths", [(2, 2, 1, 700, [700, 577]), (3, 1, 1, 512, [512, 65, 513]),
+                                               (1, 1, 1, 9001, None), (2, 1, 1, 8300, [8193, 1100])])
+def test_many_segments(pkg, device, B, H, Hkv, N, lengths, dtype):
+    """More segments than one thread of the scan takes, and more than one pass of it: forward and gradients."""
+    x = make(B, H, Hkv, N, dtype, seed=N, initial=True, lengths=lengths, decays=[-0.002] * H)
+    d = put(x, device)
+    names = ("q", "k", "v", "log_decay", "initial")
+    for n in names:
+        d[n].requires_grad_(True)
+    out, state = forward(pkg, d, return_state=True)
+    segments = -(-N // 64)
+    # one more product and sum for each segment that a state has passed, on top of the module's bound
+    more = segments * 2 * 2.0 ** -24
+    want, wstate = oracle(x)
+    terms, tstate = oracle(absolute(x))
+    within(out, want, terms, dtype, slack(dtype) + more)
+    within(state, wstate, tstate, torch.float32, FP32 + more)
+    got = dict(zip(names, torch.autograd.grad((out, state), [d[n] for n in names], (d["dout"], d["dstate"]))))
+    want, terms = dict(zip(names, oracle_grads(x))), dict(zip(names, oracle_grads(absolute(x))))
+    for n in ("q", "k", "v"):
+        within(got[n], want[n], terms[n], dtype, slack(dtype) + more)
+    within(got["initial"], want["initial"], terms["initial"], torch.float32, FP32 + more)
+    a = absolute(x)
+    flow = (a["q"].double() * terms["q"]).sum((0, 2, 3)) + (oracle(a)[1] * a["dstate"].double()).sum((0, 2, 3))
+    within(got["log_decay"], want["log_decay"], 3 * 512 * flow, torch.float32, slack(dtype) + more)
+
+
 def test_gradients_with_parts_left_out(pkg, device):
     """Without dstate, without log_decay's or the initial state's gradient, and through the state alone."""
     x = make(2, 4, 2, 150, torch.float32, seed=5, initial=True)

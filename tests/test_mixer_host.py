@@ -158,7 +158,13 @@ def test_linear_attention_entry_points_refuse(pkg, lib):
     a.dout_stride = a.dq_stride = rows
     a.dk_stride = a.dv_stride = kv
     assert lib.dwarf_linear_attention_bwd(ctypes.byref(a), None) == bad     # the final state is needed
-    a.dfinal = None
+    for name in ("dfinal", "dinitial"):
+        setattr(a, name, P + 8)
+        assert lib.dwarf_linear_attention_bwd(ctypes.byref(a), None) == bad, name
+        setattr(a, name, None)
+    f.final = P + 8
+    assert lib.dwarf_linear_attention_fwd(ctypes.byref(f), None) == bad
+    f.final = None
     assert lib.dwarf_linear_attention_bwd(ctypes.byref(a), None) == L.DWARF_ERR_WORKSPACE
     s = L.LinearAttentionStepArgs()
     s.S, s.H, s.H_kv, s.pool, s.head_dim, s.scale = 3, 4, 2, 5, 64, 0.125
