@@ -1188,7 +1188,7 @@ __global__ __launch_bounds__(kStepThreads) void la_step_kernel(dwarf_linear_atte
 }
 
 int la_segment(int64_t B, int64_t H, int64_t N) {
-  for (int seg = 512; seg > kChunk; seg /= 2)
+  for (int seg = 1024; seg > kChunk; seg /= 2)
     if (B * H * ((N + seg - 1) / seg) >= 448) return seg;
   return kChunk;
 }

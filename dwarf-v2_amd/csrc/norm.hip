@@ -55,6 +55,26 @@ __device__ __forceinline__ float row_sum(float x, float* s_red) {
   }
 }
 
+// A row's vectors of one thread, as they are in memory; vectors behind the row's end are the row's first one again (no
+// branch stands around a load) and are zeroed when they are widened.
+template <typename T, int VEC, int TPR, int K>
+struct NormRaw {
+  Vec<T, VEC> v[K];
+  __device__ __forceinline__ void load(const T* row, int sub, int D) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int d = (k * TPR + sub) * VEC;
+      v[k] = *reinterpret_cast<const Vec<T, VEC>*>(row + (d < D ? d : 0));
+    }
+  }
+  __device__ __forceinline__ void widen(int sub, int D, float* x) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[k * VEC + e] = (k * TPR + sub) * VEC < D ? to_f32(v[k].e[e]) : 0.f;
+  }
+};
+
 template <typename T, int VEC, int TPR, int K>
 __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const T* __restrict__ x, int64_t xs0, int64_t xs1,
                                                                 const float* __restrict__ weight,
@@ -65,7 +85,10 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const T* __restr
   const int sub = threadIdx.x % TPR;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;   // a multiple of the groups
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
+  if (first >= gm.rows) return;   // a row's threads together
   const float fd = static_cast<float>(gm.D);   // sums are divided, so that a row of one value has it as its mean
+  NormRaw<T, VEC, TPR, K> next;
+  next.load(x + norm_at(first, gm.groups, xs0, xs1), sub, gm.D);
   const float* wg = weight + (first % gm.groups) * gm.D;
   const float* bg = bias + (first % gm.groups) * gm.D;
   float w[K * VEC], b[K * VEC];
@@ -79,19 +102,11 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const T* __restr
     }
   }
   for (int64_t r = first; r < gm.rows; r += step) {
-    const T* xr = x + norm_at(r, gm.groups, xs0, xs1);
     float v[K * VEC];
+    next.widen(sub, gm.D, v);
+    // the next row's loads are under way while this one is summed (behind the last row: this one again)
+    next.load(x + norm_at(r + step < gm.rows ? r + step : r, gm.groups, xs0, xs1), sub, gm.D);
     float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int d = (k * TPR + sub) * VEC;
-      if (d < gm.D) {
-        load_vec<T, VEC>(xr + d, v + k * VEC);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[k * VEC + e] = 0.f;
-      }
-    }
 #pragma unroll
     for (int i = 0; i < K * VEC; ++i) s += v[i];
     const float mu = row_sum<TPR, kNormThreads>(s, s_red) / fd;
@@ -144,22 +159,19 @@ __global__ __launch_bounds__(kNormBwdThreads) void norm_bwd_kernel(
       dw[k * VEC + e] = db[k * VEC + e] = 0.f;
     }
   }
+  NormRaw<T, VEC, TPR, K> nx, ng;
+  auto fetch = [&](int64_t r) {   // behind the last row: that one again
+    if (r >= gm.rows) r = gm.rows - 1;
+    nx.load(x + norm_at(r, gm.groups, xs0, xs1), sub, gm.D);
+    ng.load(dy + norm_at(r, gm.groups, gs0, gs1), sub, gm.D);
+  };
+  fetch(first);
   for (int64_t r = first; r < gm.rows; r += step) {
-    const T* xr = x + norm_at(r, gm.groups, xs0, xs1);
-    const T* gr = dy + norm_at(r, gm.groups, gs0, gs1);
     float v[K * VEC], g[K * VEC];
     float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int d = (k * TPR + sub) * VEC;
-      if (d < gm.D) {
-        load_vec<T, VEC>(xr + d, v + k * VEC);
-        load_vec<T, VEC>(gr + d, g + k * VEC);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[k * VEC + e] = g[k * VEC + e] = 0.f;
-      }
-    }
+    nx.widen(sub, gm.D, v);
+    ng.widen(sub, gm.D, g);
+    fetch(r + step);
 #pragma unroll
     for (int i = 0; i < K * VEC; ++i) s += v[i];
     const float mu = row_sum<TPR, kNormBwdThreads>(s, s_red) / fd;
@@ -330,39 +342,42 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_columns(const T* __rest
   if (part_b) part_b[at] = b;
 }
 
-// dw (blockIdx.y 0) and db from the partials: 64 columns of one group per workgroup, sixteen waves share the partial
-// rows of the group and are added in wave order.  Partial row i of workgroup b belongs to group (b block_rows + i) %
-// groups: one row of each workgroup where its rows hold every group, one of some workgroups where they do not.
-constexpr int kNormSumWaves = 16;
-__global__ __launch_bounds__(kWave * kNormSumWaves) void norm_sum_kernel(const float* __restrict__ part_w,
-                                                                        const float* __restrict__ part_b, int blocks,
-                                                                        int block_rows, int groups, int D,
-                                                                        float* __restrict__ dweight,
-                                                                        float* __restrict__ dbias) {
-  __shared__ float s_part[kNormSumWaves][kWave];
+// dw (blockIdx.y 0) and db from the partials: 16 columns of one group per workgroup, 64 threads to a column, which add
+// every 64th partial row in order and are then added in order themselves.  Partial row i of workgroup b belongs to group
+// (b block_rows + i) % groups: one row of each workgroup where its rows hold every group, of some where they do not.
+constexpr int kNormSumCols = 16, kNormSumRows = 64;
+__global__ __launch_bounds__(kNormSumCols * kNormSumRows) void norm_sum_kernel(const float* __restrict__ part_w,
+                                                                              const float* __restrict__ part_b, int blocks,
+                                                                              int block_rows, int groups, int D,
+                                                                              float* __restrict__ dweight,
+                                                                              float* __restrict__ dbias) {
+  __shared__ float s_part[kNormSumRows][kNormSumCols + 1];
   const float* part = blockIdx.y ? part_b : part_w;
   float* out = blockIdx.y ? dbias : dweight;
   if (!out) return;   // uniform
-  const int col_blocks = (D + kWave - 1) / kWave;
-  const int group = blockIdx.x / col_blocks, d = blockIdx.x % col_blocks * kWave + threadIdx.x % kWave;
-  const int wave = threadIdx.x / kWave;
+  const int col_blocks = (D + kNormSumCols - 1) / kNormSumCols;
+  const int group = blockIdx.x / col_blocks, col = threadIdx.x % kNormSumCols, row = threadIdx.x / kNormSumCols;
+  const int d = blockIdx.x % col_blocks * kNormSumCols + col;
   const int parts = norm_parts(groups, block_rows);
   float t = 0.f;
   if (d < D) {
-#pragma unroll 4
-    for (int b = wave; b < blocks; b += kNormSumWaves) {
+#pragma unroll 8
+    for (int b = row; b < blocks; b += kNormSumRows) {
       const uint32_t behind = static_cast<uint32_t>(b) * static_cast<uint32_t>(block_rows) % static_cast<uint32_t>(groups);
       const int i = group >= static_cast<int>(behind) ? group - static_cast<int>(behind) : group + groups - static_cast<int>(behind);
-      if (i < parts) t += part[(static_cast<int64_t>(b) * parts + i) * D + d];
+      const float v = part[(static_cast<int64_t>(b) * parts + (i < parts ? i : 0)) * D + d];
+      t += i < parts ? v : 0.f;
     }
   }
-  s_part[wave][threadIdx.x % kWave] = t;
+  s_part[row][col] = t;
   __syncthreads();
-  if (wave == 0 && d < D) {
+  if (row < 4) {   // 16 rows each, then the four
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kNormSumWaves; ++w) s += s_part[w][threadIdx.x];
-    out[static_cast<int64_t>(group) * D + d] = s;
+    for (int r = 0; r < kNormSumRows / 4; ++r) s += s_part[row * (kNormSumRows / 4) + r][col];
+    s += __shfl_down(s, 2 * kNormSumCols);
+    s += __shfl_down(s, kNormSumCols);
+    if (row == 0 && d < D) out[static_cast<int64_t>(group) * D + d] = s;
   }
 }
 
@@ -412,7 +427,7 @@ NormPlan norm_plan(const dwarf_layer_norm_fwd_args& f, bool vec, int threads) {
   else p.tpr = 0;
   p.block_rows = p.tpr ? threads / p.tpr : 1;
   const int64_t rows = f.rows * f.groups;
-  p.blocks = static_cast<int>(norm_blocks(rows, f.groups, p.block_rows, 2048));
+  p.blocks = static_cast<int>(norm_blocks(rows, f.groups, p.block_rows, 768));
   p.columns_y = 0;
   return p;
 }
@@ -479,7 +494,7 @@ void norm_bwd_typed(const dwarf_layer_norm_bwd_args& a, const NormPlan& p, const
     hipLaunchKernelGGL((norm_bwd_columns<T>), dim3((f.D + kNormThreads - 1) / kNormThreads, p.columns_y, f.groups),
                        dim3(kNormThreads), 0, stream, x, f.x_stride[0], f.x_stride[1], dy, a.dy_stride[0],
                        a.dy_stride[1], stats, pw, pb, gm);
-    hipLaunchKernelGGL(norm_sum_kernel, dim3((f.D + kWave - 1) / kWave * f.groups, 2), dim3(kWave * kNormSumWaves), 0,
+    hipLaunchKernelGGL(norm_sum_kernel, dim3((f.D + kNormSumCols - 1) / kNormSumCols * f.groups, 2), dim3(kNormSumCols * kNormSumRows), 0,
                        stream, pw, pb, p.columns_y, f.groups, f.groups, f.D, a.dweight, a.dbias);
     return;
   }
@@ -494,7 +509,7 @@ void norm_bwd_typed(const dwarf_layer_norm_bwd_args& a, const NormPlan& p, const
   DWARF_NORM_SHAPES(DWARF_NORM_LAUNCH)
 #undef DWARF_NORM_LAUNCH
   if (sums)
-    hipLaunchKernelGGL(norm_sum_kernel, dim3((f.D + kWave - 1) / kWave * f.groups, 2), dim3(kWave * kNormSumWaves), 0,
+    hipLaunchKernelGGL(norm_sum_kernel, dim3((f.D + kNormSumCols - 1) / kNormSumCols * f.groups, 2), dim3(kNormSumCols * kNormSumRows), 0,
                        stream, pw, pb, p.blocks, p.block_rows, f.groups, f.D, a.dweight, a.dbias);
 }
 
