@@ -476,16 +476,18 @@ __device__ __forceinline__ void split8(float* x, bf16x8* parts) {
   }
 }
 
-// The wave's rows of the state (rows 16 w + 4 g + r, CT column tiles from ct0, column 16 ct + c) into two LDS tiles of
-// the transposed state: its high parts, and behind them what those leave.
-template <int CT>
-__device__ __forceinline__ void state_put(const f32x4* M, char* s, const TileMap& m, int ct0) {
+// The wave's 16 rows of the state (rows 16 w + 4 g + r, column 16 ct + c) into PARTS LDS tiles of the transposed state: its
+// high parts, behind them what those leave, and so on.
+template <int PARTS>
+__device__ __forceinline__ void state_put(const f32x4* M, char* s, const TileMap& m) {
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
+  for (int ct = 0; ct < 4; ++ct) {
     float x[4] = {M[ct][0], M[ct][1], M[ct][2], M[ct][3]};
-    char* at = s + m.state + 2048 * (ct0 + ct);
-    *reinterpret_cast<uint2*>(at) = uint2{split_pair(x[0], x[1]), split_pair(x[2], x[3])};
-    *reinterpret_cast<uint2*>(at + kTileBytes) = uint2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+    char* at = s + m.state + 2048 * ct;
+#pragma unroll
+    for (int p = 0; p + 1 < PARTS; ++p)
+      *reinterpret_cast<uint2*>(at + p * kTileBytes) = uint2{split_pair(x[0], x[1]), split_pair(x[2], x[3])};
+    *reinterpret_cast<uint2*>(at + (PARTS - 1) * kTileBytes) = uint2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
   }
 }
 
@@ -529,16 +531,16 @@ struct StateWeights {
   }
 };
 
-// M += factor sum_j weight_j X_j Y_j^T for the wave's 16 columns of X and CT tiles of Y's columns from ct0.  PARTS: of
-// the weighted X, three where the sum itself is a result, two where it only goes into rows that are rounded to bf16.
-template <int CT, int PARTS, typename W>
-__device__ __forceinline__ void state_add(const char* sX, const char* sY, const TileMap& m, int w, int ct0, const W& weights,
+// M += factor sum_j weight_j X_j Y_j^T for the wave's 16 columns of X and all of Y.  PARTS: of the weighted X, three where
+// the sum goes into an fp32 result, two where it only goes into rows that are rounded to bf16.
+template <int PARTS, typename W>
+__device__ __forceinline__ void state_add(const char* sX, const char* sY, const TileMap& m, int w, const W& weights,
                                           float factor, f32x4* M) {
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
-    bf16x8 y[CT];
+    bf16x8 y[4];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) y[ct] = tile_column(sY, m, ct0 + ct, ks);
+    for (int ct = 0; ct < 4; ++ct) y[ct] = tile_column(sY, m, ct, ks);
     float x[8];
     unpack8(tile_column(sX, m, w, ks), x);
     weights.apply(ks, factor, x);
@@ -547,23 +549,21 @@ __device__ __forceinline__ void state_add(const char* sX, const char* sY, const 
 #pragma unroll
     for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) M[ct] = mfma16_bf16(parts[p], y[ct], M[ct]);
+      for (int ct = 0; ct < 4; ++ct) M[ct] = mfma16_bf16(parts[p], y[ct], M[ct]);
   }
 }
-template <int CT>
 __device__ __forceinline__ void state_shrink(f32x4* M, float shrink) {
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct)
+  for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
     for (int r = 0; r < 4; ++r) M[ct][r] *= shrink;
 }
 
-template <int CT>
-__device__ __forceinline__ void state_load(const float* en, bool trans, int ct0, f32x4* M) {
+__device__ __forceinline__ void state_load(const float* en, bool trans, f32x4* M) {
   const int l = threadIdx.x % kWave, w = threadIdx.x / kWave % 4, g = l / 16, c = l % 16;
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int i = 16 * w + 4 * g, j = 16 * (ct0 + ct) + c;
+  for (int ct = 0; ct < 4; ++ct) {
+    const int i = 16 * w + 4 * g, j = 16 * ct + c;
     if (!en) M[ct] = zero4();
     else if (trans) M[ct] = *reinterpret_cast<const f32x4*>(en + j * kHd + i);
     else
@@ -658,8 +658,8 @@ __global__ __launch_bounds__(kLaThreads, 4) void la_local_bf16(LaRows X_, int xh
         tile_put(y[u], s + kTileBytes, m);
         __syncthreads();   // also: every wave is done with the other buffer
         const int t = t0 + (i0 + u) * kChunk, n = t1 - t < kChunk ? t1 - t : kChunk;
-        state_shrink<4>(M, n < kChunk ? la_power(lg, n) : full);
-        state_add<4, 3>(s, s + kTileBytes, m, w, 0, StateWeights(tables, n), 1.f, M);
+        state_shrink(M, n < kChunk ? la_power(lg, n) : full);
+        state_add<3>(s, s + kTileBytes, m, w, StateWeights(tables, n), 1.f, M);
       }
     }
   }
@@ -724,8 +724,8 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
   fetch(0);
   if (keeps) {
     f32x4 M[4];
-    state_load<4>(enter ? enter + it.at * kState : nullptr, false, 0, M);
-    state_put<4>(M, smem + 2 * kTileBytes, m, 0);
+    state_load(enter ? enter + it.at * kState : nullptr, false, M);
+    state_put<2>(M, smem + 2 * kTileBytes, m);
     const float full = la_power(lg, kChunk);
     for (int i = 0; i < chunks; ++i) {
       char *s = smem + (i & 1) * 4 * kTileBytes, *other = smem + (~i & 1) * 4 * kTileBytes;
@@ -734,10 +734,10 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
       __syncthreads();   // also: every wave is done with the other buffer
       fetch(i + 1);
       const int n = live(i);
-      state_shrink<4>(M, n < kChunk ? la_power(lg, n) : full);
+      state_shrink(M, n < kChunk ? la_power(lg, n) : full);
       const StateWeights wt(tables, n);
-      state_add<4, 3>(s, s + kTileBytes, m, w, 0, wt, 1.f, M);   // (two parts would do where nothing leaves: no faster)
-      state_put<4>(M, other + 2 * kTileBytes, m, 0);
+      state_add<3>(s, s + kTileBytes, m, w, wt, 1.f, M);   // (two parts would do where nothing leaves: no faster)
+      state_put<2>(M, other + 2 * kTileBytes, m);
     }
     if (leave) state_store(M, leave + it.at * kState);
     return;
@@ -770,7 +770,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
         o[ct] = mfma16_bf16(tile_row(sM, m, ct, ks), a[ks], o[ct]);
         o[ct] = mfma16_bf16(tile_row(sM + kTileBytes, m, ct, ks), a[ks], o[ct]);
       }
-    state_shrink<4>(o, carry);
+    state_shrink(o, carry);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       if (2 * ks <= w) {   // uniform: some of the 32 tokens are not behind the wave's rows
@@ -808,12 +808,18 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
 
 // dq_i = scale (sum_{j <= i} g^{i-j} (do_i.v_j) k_j + g^{i+1} do_i S^T), and from the same tiles the segment's own sum
 // of the adjoint, local = sum_i scale g^{i+1} q_i do_i^T (NULL: not wanted): one pass over q and do instead of two.  The
-// four state waves keep both.  LDS: one chunk of v, k, q and do, and the two parts of S^T in front of this and the next.
+// four state waves keep both.  LDS: one chunk of v, k, q and do, and the parts of S^T in front of it.
+//
+// DECAY: the rows' side of dlog_decay, sum tau q_i.(the share of dq_i that comes from in front of i's chunk), with the
+// state in three parts: it nearly cancels against the keys' side, so that two parts' 2^-17 would show.  Pairs within a
+// chunk are the keys' side's (la_dkdv_role).
+template <bool DECAY>
 __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows O_, LaRows K_, LaRows V_, LaGeom gm,
                                                               const float* __restrict__ enter, bf16* __restrict__ dq,
                                                               int64_t o0, int64_t o1, int64_t o2,
                                                               float* __restrict__ local, float* __restrict__ dot) {
-  __shared__ __align__(16) char smem[8 * kTileBytes + kTableBytes];
+  constexpr int kParts = DECAY ? 3 : 2;
+  __shared__ __align__(16) char smem[(4 + kParts) * kTileBytes + kTableBytes];
   const LaItem it = la_item(gm);
   const int l = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), w = wave % 4, g = l / 16, c = l % 16;
   const bool keeps = wave >= 4;
@@ -828,7 +834,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
   const TileMap m(threadIdx.x);
   const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
   auto live = [&](int i) { return i < chunks ? (t1 - t0 - i * kChunk < kChunk ? t1 - t0 - i * kChunk : kChunk) : 0; };
-  char *sV = smem, *sK = smem + kTileBytes, *sQ = smem + 2 * kTileBytes, *sO = smem + 3 * kTileBytes;
+  char *sV = smem, *sK = smem + kTileBytes, *sQ = smem + 2 * kTileBytes, *sO = smem + 3 * kTileBytes, *sM = smem + 4 * kTileBytes;
   uint4 x[4];
   auto fetch = [&](int i) {
     const int64_t t = t0 + static_cast<int64_t>(i) * kChunk;
@@ -841,29 +847,28 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
 #pragma unroll
     for (int u = 0; u < 4; ++u) tile_put_wide(x[u], smem + u * kTileBytes, m);
   };
-  const float* tables = reinterpret_cast<const float*>(smem + 8 * kTileBytes);   // written before the first barrier
-  state_weights_put(lg, live(chunks - 1), reinterpret_cast<float*>(smem + 8 * kTileBytes));
+  const float* tables = reinterpret_cast<const float*>(smem + (4 + kParts) * kTileBytes);   // written before the first barrier
+  state_weights_put(lg, live(chunks - 1), reinterpret_cast<float*>(smem + (4 + kParts) * kTileBytes));
   fetch(0);
   float total = 0.f;
   if (keeps) {
     f32x4 M[4], L[4] = {zero4(), zero4(), zero4(), zero4()};
-    state_load<4>(enter ? enter + it.at * kState : nullptr, true, 0, M);
-    state_put<4>(M, smem + 4 * kTileBytes, m, 0);
+    state_load(enter ? enter + it.at * kState : nullptr, true, M);
     const float full = la_power(lg, kChunk);
     const AdjointWeights wl(lg, gm.scale);
     float past = 1.f;
     for (int i = 0; i < chunks; ++i) {
       put();
+      state_put<kParts>(M, sM, m);
       __syncthreads();
       fetch(i + 1);
       const int n = live(i);
-      state_shrink<4>(M, n < kChunk ? la_power(lg, n) : full);
-      state_add<4, 2>(sV, sK, m, w, 0, StateWeights(tables, n), 1.f, M);
+      state_shrink(M, n < kChunk ? la_power(lg, n) : full);
+      state_add<kParts>(sV, sK, m, w, StateWeights(tables, n), 1.f, M);
       if (local) {
-        state_add<4, 3>(sQ, sO, m, w, 0, wl, past, L);
+        state_add<3>(sQ, sO, m, w, wl, past, L);
         past *= full;
       }
-      state_put<4>(M, smem + (i & 1 ? 4 : 6) * kTileBytes, m, 0);
       __syncthreads();   // every wave is done with the tiles
     }
     if (local && chunks) state_store(L, local + it.at * kState);
@@ -874,17 +879,25 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
       put();
       __syncthreads();
       fetch(i + 1);
-      const char* sM = smem + (i & 1 ? 6 : 4) * kTileBytes;
+      const int row = 16 * w + c;
       const bf16x8 a[2] = {tile_row(sO, m, w, 0), tile_row(sO, m, w, 1)};
       f32x4 o[4] = {zero4(), zero4(), zero4(), zero4()};
 #pragma unroll
       for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          o[ct] = mfma16_bf16(tile_row(sM, m, ct, ks), a[ks], o[ct]);
-          o[ct] = mfma16_bf16(tile_row(sM + kTileBytes, m, ct, ks), a[ks], o[ct]);
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int p = 0; p < kParts; ++p) o[ct] = mfma16_bf16(tile_row(sM + p * kTileBytes, m, ct, ks), a[ks], o[ct]);
+      state_shrink(o, carry);
+      if constexpr (DECAY) {
+        float sum = 0.f;
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) {
+          const uint2 x2 = *reinterpret_cast<const uint2*>(sQ + (m.slots ^ 32 * ct) + 2048 * w);
+          sum = fmaf(o[ct][0], bf16_lo(x2.x), fmaf(o[ct][1], bf16_hi(x2.x), fmaf(o[ct][2], bf16_lo(x2.y), fmaf(o[ct][3], bf16_hi(x2.y), sum))));
         }
-      state_shrink<4>(o, carry);
+        total = fmaf(static_cast<float>(i * kChunk + row + 1) - mid, sum, total);   // dead rows of q are zero
+      }
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         if (2 * ks <= w) {
@@ -909,42 +922,39 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
           }
         }
       }
-      const int row = 16 * w + c;
       if (row < live(i)) {
         bf16* pr = po + (t0 + static_cast<int64_t>(i) * kChunk + row) * o2;
-        float sum = 0.f;
 #pragma unroll
         for (int ct = 0; ct < 4; ++ct) {
           const float v[4] = {o[ct][0], o[ct][1], o[ct][2], o[ct][3]};
           put4(pr + 16 * ct + 4 * g, v);
-          if (dot) {
-            const uint2 q = *reinterpret_cast<const uint2*>(sQ + (m.slots ^ 32 * ct) + 2048 * w);
-            sum = fmaf(v[0], bf16_lo(q.x), fmaf(v[1], bf16_hi(q.x), fmaf(v[2], bf16_lo(q.y), fmaf(v[3], bf16_hi(q.y), sum))));
-          }
         }
-        total = fmaf(static_cast<float>(i * kChunk + row + 1) - mid, sum, total);
       }
       __syncthreads();   // every wave is done with the tiles
     }
   }
-  if (dot) {
+  if constexpr (DECAY) {
     total = workgroup_sum<kWideThreads / kWave>(total, reinterpret_cast<float*>(smem));
     if (threadIdx.x == 0) dot[it.at] = total;
   }
 }
 
-// One gradient of la_dkdv_bf16: dv, with its rows of k from LDS, or (KEYS) dk, with its rows of v in registers.
-template <bool KEYS, typename TO>
+// One gradient of la_dkdv_bf16: dv, with its rows of k from LDS, or (KEYS) dk, with its rows of v in registers.  DECAY: the
+// keys' side of dlog_decay (see la_dq_bf16), returned by the dk waves.  Without it a chunk's tiles and G's two parts have
+// two LDS buffers each; with it G has three parts, and all have one buffer and a second barrier.
+template <bool KEYS, bool DECAY, typename TO>
 __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, const LaRows& O_, const LaRows& K_, const LaRows& V_,
                                               const LaGeom& gm, const LaItem& it, int t0, int t1,
-                                              const float* __restrict__ enter, TO* __restrict__ pr, int64_t stride, bool dot) {
+                                              const float* __restrict__ enter, TO* __restrict__ pr, int64_t stride) {
+  constexpr int kParts = DECAY ? 3 : 2;        // of G in LDS
+  constexpr int kRead = KEYS ? kParts : 2;     // that this wave's rows take
   const int l = threadIdx.x % kWave, w = uniform(threadIdx.x / kWave) % 4, g = l / 16, c = l % 16;
   const float lg = la_log2_decay(gm, it.h), full = la_power(lg, kChunk);
   const bf16 *pq = la_rows_of(Q_, gm.H, gm, it), *pdo = la_rows_of(O_, gm.H, gm, it);
   const bf16 *pv = la_rows_of(V_, gm.Hkv, gm, it), *pk = la_rows_of(K_, gm.Hkv, gm, it);
   const TileMap m(threadIdx.x);
   f32x4 G[4];
-  if constexpr (!KEYS) state_load<4>(enter ? enter + it.at * kState : nullptr, false, 0, G);
+  if constexpr (!KEYS) state_load(enter ? enter + it.at * kState : nullptr, false, G);
   const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
   // chunk i counts from the end; behind the first one nothing is live
   auto live = [&](int i) { return i >= chunks ? 0 : i > 0 ? kChunk : t1 - t0 - (chunks - 1) * kChunk; };
@@ -974,13 +984,13 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
   fetch(0);
   for (int i = 0; i < chunks; ++i) {
     const int n = live(i);
-    char *sQ = smem + (i & 1) * 5 * kTileBytes, *sO = sQ + kTileBytes, *sK = sQ + 2 * kTileBytes, *sG = sQ + 3 * kTileBytes;
+    char *sQ = smem + (DECAY ? 0 : (i & 1) * 5 * kTileBytes), *sO = sQ + kTileBytes, *sK = sQ + 2 * kTileBytes, *sG = sQ + 3 * kTileBytes;
     tile_put_wide(xq, sQ, m);
     tile_put_wide(xo, sO, m);
     tile_put_wide(xk, sK, m);
-    if constexpr (!KEYS) state_put<4>(G, sG, m, 0);
+    if constexpr (!KEYS) state_put<kParts>(G, sG, m);
     bf16x8 a[2] = {bf16x8_from_bits(own[0]), bf16x8_from_bits(own[1])};
-    __syncthreads();   // also: every wave is done with the other buffer
+    __syncthreads();   // without DECAY also: every wave is done with the other buffer
     fetch(i + 1);
     if constexpr (!KEYS) {
       a[0] = tile_row(sK, m, w, 0);
@@ -993,11 +1003,20 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
+        for (int part = 0; part < kRead; ++part) {
           const char* s = sG + part * kTileBytes;
           acc[ct] = mfma16_bf16(KEYS ? tile_column(s, m, ct, ks) : tile_row(s, m, ct, ks), a[ks], acc[ct]);
         }
-    state_shrink<4>(acc, la_power(lg, n - 1 - row < 0 ? 0 : n - 1 - row));
+    state_shrink(acc, la_power(lg, n - 1 - row < 0 ? 0 : n - 1 - row));
+    if constexpr (KEYS && DECAY) {
+      float sum = 0.f;
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        const uint2 k = *reinterpret_cast<const uint2*>(sK + (m.slots ^ 32 * ct) + 2048 * w);
+        sum = fmaf(acc[ct][0], bf16_lo(k.x), fmaf(acc[ct][1], bf16_hi(k.x), fmaf(acc[ct][2], bf16_lo(k.y), fmaf(acc[ct][3], bf16_hi(k.y), sum))));
+      }
+      total = fmaf(static_cast<float>(token(i) + row - t0 + 1) - mid, sum, total);   // dead rows of k are zero
+    }
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       if (2 * ks + 1 >= w) {   // uniform: some of the 32 tokens are not before the wave's rows
@@ -1011,6 +1030,16 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
             z = mfma16_bf16(KEYS ? tile_row_slots(sO, m, tt, 1) : tile_row(sQ, m, tt, 1), a[1], z);
           }
           sw.apply(z, tt - w, p + 4 * hf);
+          if constexpr (KEYS && DECAY) {
+            if (tt >= w) {
+              f32x4 y = zero4();
+              y = mfma16_bf16(tile_row(sQ, m, tt, 0), tile_row(sK, m, w, 0), y);
+              y = mfma16_bf16(tile_row(sQ, m, tt, 1), tile_row(sK, m, w, 1), y);
+              const float gap = static_cast<float>(16 * (tt - w) + 4 * g - c);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) total = fmaf(-(gap + static_cast<float>(r)) * p[4 * hf + r], y[r], total);
+            }
+          }
         }
         bf16x8 parts[2];
         split8<2>(p, parts);
@@ -1023,38 +1052,33 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
       }
     }
     if (row < n) {
-      const int64_t t = token(i) + row;
-      float sum = 0.f;
+      TO* at = pr + (token(i) + row) * stride + 4 * g;
 #pragma unroll
       for (int ct = 0; ct < 4; ++ct) {
         const float v[4] = {acc[ct][0], acc[ct][1], acc[ct][2], acc[ct][3]};
-        put4(pr + t * stride + 16 * ct + 4 * g, v);
-        if (KEYS && dot) {
-          const uint2 k = *reinterpret_cast<const uint2*>(sK + (m.slots ^ 32 * ct) + 2048 * w);
-          sum = fmaf(v[0], bf16_lo(k.x), fmaf(v[1], bf16_hi(k.x), fmaf(v[2], bf16_lo(k.y), fmaf(v[3], bf16_hi(k.y), sum))));
-        }
+        put4(at + 16 * ct, v);
       }
-      total = fmaf(static_cast<float>(t - t0 + 1) - mid, sum, total);
     }
     if constexpr (!KEYS) {
-      state_shrink<4>(G, n < kChunk ? la_power(lg, n) : full);
-      state_add<4, 2>(sQ, sO, m, w, 0, wt, 1.f, G);
+      state_shrink(G, n < kChunk ? la_power(lg, n) : full);
+      state_add<kParts>(sQ, sO, m, w, wt, 1.f, G);
     }
+    if constexpr (DECAY) __syncthreads();   // every wave is done with the tiles
   }
   return total;
 }
 
 // dk and dv of a segment, chunks from its end, G the adjoint of the state behind the chunk:
 //   dv_j = scale sum_{i >= j} g^{i-j} (k_j.q_i) do_i + g^{n-1-j} k_j G,  dk_j the same with v, do, q and G^T.
-// Four waves form dv and keep G, and four form dk.  The q and do tiles serve as rows and
-// as columns; G lies in LDS transposed, read by rows for dv and transposed for dk.  Both roles pass the same barriers.
-template <typename TO>
+// Four waves form dv and keep G, and four form dk.  The q and do tiles serve as rows and as columns; G lies in LDS
+// transposed, read by rows for dv and transposed for dk.  Both roles pass the same barriers.
+template <bool DECAY, typename TO>
 __global__ __launch_bounds__(kWideThreads, 4) void la_dkdv_bf16(LaRows Q_, LaRows O_, LaRows K_, LaRows V_, LaGeom gm,
                                                                 const float* __restrict__ enter, TO* __restrict__ dk,
                                                                 int64_t k0, int64_t k1, int64_t k2, TO* __restrict__ dv,
                                                                 int64_t v0, int64_t v1, int64_t v2, int outh,
                                                                 float* __restrict__ dot) {
-  __shared__ __align__(16) char smem[10 * kTileBytes];   // two chunks of q, do and k, and G's two parts for each
+  __shared__ __align__(16) char smem[(DECAY ? 6 : 10) * kTileBytes];   // q, do, k and G's parts
   const LaItem it = la_item(gm);
   const int len = la_length(gm, it.b), t0 = it.seg * gm.seg;
   const int tend = t0 + gm.seg < gm.N ? t0 + gm.seg : gm.N;
@@ -1064,9 +1088,9 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dkdv_bf16(LaRows Q_, LaRow
   la_zero_rows(pdk, k2, t1 > t0 ? t1 : t0, tend);
   la_zero_rows(pdv, v2, t1 > t0 ? t1 : t0, tend);
   float total;
-  if (uniform(threadIdx.x / kWave) >= 4) total = la_dkdv_role<true>(smem, Q_, O_, K_, V_, gm, it, t0, t1, enter, pdk, k2, dot != nullptr);
-  else total = la_dkdv_role<false>(smem, Q_, O_, K_, V_, gm, it, t0, t1, enter, pdv, v2, false);
-  if (dot) {
+  if (uniform(threadIdx.x / kWave) >= 4) total = la_dkdv_role<true, DECAY>(smem, Q_, O_, K_, V_, gm, it, t0, t1, enter, pdk, k2);
+  else total = la_dkdv_role<false, DECAY>(smem, Q_, O_, K_, V_, gm, it, t0, t1, enter, pdv, v2);
+  if constexpr (DECAY) {
     total = workgroup_sum<kWideThreads / kWave>(total, reinterpret_cast<float*>(smem));
     if (threadIdx.x == 0) dot[it.at] = total;
   }
@@ -1278,9 +1302,11 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
   const int64_t s1 = static_cast<int64_t>(gm.N) * kHd, s0 = s1 * gm.H;   // of the shared heads' parts
   const dim3 wide(kWideThreads);
   if constexpr (std::is_same<T, bf16>::value) {
-    if (gm.segs)
-      hipLaunchKernelGGL(la_dq_bf16, grid, wide, 0, stream, q, dout, k, v, gm, before, static_cast<bf16*>(a.dq),
-                         a.dq_stride[0], a.dq_stride[1], a.dq_stride[2], joined ? adj : nullptr, dq_dot);
+    if (gm.segs) {
+      auto kernel = dlog ? la_dq_bf16<true> : la_dq_bf16<false>;
+      hipLaunchKernelGGL(kernel, grid, wide, 0, stream, q, dout, k, v, gm, before, static_cast<bf16*>(a.dq), a.dq_stride[0],
+                         a.dq_stride[1], a.dq_stride[2], joined ? adj : nullptr, dq_dot);
+    }
   } else if (joined && gm.segs) {
     hipLaunchKernelGGL((la_local_kernel<T, true>), grid, block, 0, stream, q, gm.H, dout, gm.H, gm, gm.scale, adj);
   }
@@ -1288,13 +1314,16 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
     la_scan<true>(adj, a.dfinal, a.dinitial, gm, f.states, f.initial, f.final, edge, stream);
   if (gm.segs) {
     if constexpr (std::is_same<T, bf16>::value) {
-      if (shared)
-        hipLaunchKernelGGL((la_dkdv_bf16<float>), grid, wide, 0, stream, q, dout, k, v, gm, enter, pk, s0, s1, kHd, pv,
-                           s0, s1, kHd, gm.H, dk_dot);
-      else
-        hipLaunchKernelGGL((la_dkdv_bf16<bf16>), grid, wide, 0, stream, q, dout, k, v, gm, enter, static_cast<bf16*>(a.dk),
-                           a.dk_stride[0], a.dk_stride[1], a.dk_stride[2], static_cast<bf16*>(a.dv), a.dv_stride[0],
-                           a.dv_stride[1], a.dv_stride[2], gm.Hkv, dk_dot);
+      if (shared) {
+        auto kernel = dlog ? la_dkdv_bf16<true, float> : la_dkdv_bf16<false, float>;
+        hipLaunchKernelGGL(kernel, grid, wide, 0, stream, q, dout, k, v, gm, enter, pk, s0, s1, int64_t(kHd), pv, s0, s1,
+                           int64_t(kHd), gm.H, dk_dot);
+      } else {
+        auto kernel = dlog ? la_dkdv_bf16<true, bf16> : la_dkdv_bf16<false, bf16>;
+        hipLaunchKernelGGL(kernel, grid, wide, 0, stream, q, dout, k, v, gm, enter, static_cast<bf16*>(a.dk), a.dk_stride[0],
+                           a.dk_stride[1], a.dk_stride[2], static_cast<bf16*>(a.dv), a.dv_stride[0], a.dv_stride[1],
+                           a.dv_stride[2], gm.Hkv, dk_dot);
+      }
     } else {
       hipLaunchKernelGGL((la_rows_kernel<T, T, false, true>), grid, block, 0, stream, dout, gm.H, v, gm.Hkv, k, gm.Hkv, gm,
                          gm.scale, gm.scale, 1.f, before, static_cast<T*>(a.dq), a.dq_stride[0], a.dq_stride[1],
