@@ -53,6 +53,24 @@ __device__ __forceinline__ float la_log2_decay(const LaGeom& gm, int h) {
 }
 __device__ __forceinline__ float la_power(float lg, int n) { return __builtin_amdgcn_exp2f(lg * static_cast<float>(n)); }
 
+// The terms of dlog_decay nearly cancel: their sums over threads, segments and sequences are kept in 64 bits.
+__device__ __forceinline__ double wave_sum_f64(double x) {
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) x += __shfl_xor(x, o);
+  return x;
+}
+template <int WAVES>
+__device__ __forceinline__ double workgroup_sum_f64(double x, double* s_red) {
+  x = wave_sum_f64(x);
+  __syncthreads();
+  if (threadIdx.x % kWave == 0) s_red[threadIdx.x / kWave] = x;
+  __syncthreads();
+  double t = s_red[0];
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i) t += s_red[i];
+  return t;
+}
+
 __device__ __forceinline__ int la_length(const LaGeom& gm, int b) {
   if (!gm.lengths) return gm.N;
   const int n = gm.lengths[b];
@@ -161,10 +179,10 @@ __global__ __launch_bounds__(kLaThreads) void la_scan_kernel(float* __restrict__
                                                              float* __restrict__ last, LaGeom gm,
                                                              const float* __restrict__ states,
                                                              const float* __restrict__ initial,
-                                                             const float* __restrict__ final, float* __restrict__ dot) {
+                                                             const float* __restrict__ final, double* __restrict__ dot) {
   constexpr int kOwners = kLaThreads / GROUPS;   // threads of a group
   __shared__ f32x4 s_run[GROUPS][kOwners];
-  __shared__ float s_red[kLaThreads / kWave];
+  __shared__ double s_red[kLaThreads / kWave];
   const int bh = blockIdx.x / kScanWgs<GROUPS>, owner = threadIdx.x % kOwners, group = threadIdx.x / kOwners;
   const int e = 4 * (blockIdx.x % kScanWgs<GROUPS> * kOwners + owner);
   const int b = bh / gm.H, h = bh % gm.H;
@@ -178,9 +196,10 @@ __global__ __launch_bounds__(kLaThreads) void la_scan_kernel(float* __restrict__
   auto load = [](const float* p) { return *reinterpret_cast<const f32x4*>(p); };
   const float mid = 0.5f * static_cast<float>(gm.seg);
   f32x4 m = first ? load(first + at) : zero4();
-  float sum = 0.f;
+  double sum = 0.;
   auto add_dot = [&](float weight, f32x4 a, f32x4 c) {
-    sum = fmaf(weight, fmaf(a[0], c[0], fmaf(a[1], c[1], fmaf(a[2], c[2], a[3] * c[3]))), sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum = fma(static_cast<double>(weight) * a[i], static_cast<double>(c[i]), sum);
   };
   if (REV && dot && final && active && group == 0) add_dot(static_cast<float>(n_last) - mid, m, load(final + at));
   // a pass takes GROUPS runs; position p counts segments in the direction of the scan
@@ -237,16 +256,14 @@ __global__ __launch_bounds__(kLaThreads) void la_scan_kernel(float* __restrict__
   if (last && group == 0) *reinterpret_cast<f32x4*>(last + at) = m;
   if (REV && dot) {
     if (initial && active && group == 0) add_dot(mid, load(initial + at), m);
-    sum = lanes_sum<kWave>(sum);
-    if (threadIdx.x % kWave == 0) s_red[threadIdx.x / kWave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) dot[blockIdx.x] = ((s_red[0] + s_red[1]) + s_red[2]) + s_red[3];
+    sum = workgroup_sum_f64<kLaThreads / kWave>(sum, s_red);
+    if (threadIdx.x == 0) dot[blockIdx.x] = sum;
   }
 }
 
 template <bool REV>
 void la_scan(float* local, const float* first, float* last, const LaGeom& gm, const float* states, const float* initial,
-             const float* final, float* dot, hipStream_t stream) {
+             const float* final, double* dot, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * scan_wgs(gm));
   if (gm.segs > kScanRun)
     hipLaunchKernelGGL((la_scan_kernel<REV, 16>), grid, dim3(kLaThreads), 0, stream, local, first, last, gm, states, initial,
@@ -256,44 +273,57 @@ void la_scan(float* local, const float* first, float* last, const LaGeom& gm, co
                        final, dot);
 }
 
+// One call of la_rows_kernel: rows of A against rows of B and C, the state that enters per segment [.. segs ..] or, with
+// one segment, per head (NULL: zero; trans: read transposed), the result, and with dot the decay's gradient's rows D.
+template <typename TO>
+struct LaRowsCall {
+  LaRows A, B, C, D;
+  int ah, bh, ch, dh;    // heads of each
+  const float* enter;
+  bool trans;
+  TO* out;
+  int64_t o0, o1, o2;
+  double* dot;
+};
+
 // out_i = intra sum_j W_ij (A_i.B_j) C_j + cs W_i A_i M over a segment's chunks, M updated behind each (in front, in
-// reverse).  enter: the state per segment [.. segs ..] or, with one segment, per head (NULL: zero); TRANS: read
-// transposed.  leave: with one segment, where the state that leaves goes.  dot: sum of tau <out_i, D_i>.
-template <typename T, typename TO, bool REV, bool TRANS>
-__global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRows A_, int ah, LaRows B_, int bh, LaRows C_, int ch,
-                                                             LaGeom gm, float intra, float cs, float us,
-                                                             const float* __restrict__ enter, TO* __restrict__ out,
-                                                             int64_t o0, int64_t o1, int64_t o2,
-                                                             float* __restrict__ leave, LaRows D_, int dh,
-                                                             float* __restrict__ dot) {
+// reverse); in fp32 throughout, for fp32 and fp16 rows.  leave: with one segment, where the state that leaves goes.
+// dot, forward: sum tau D_i.(out_i's part that comes from M); in reverse the same less (i - j) times each pair's share
+// within a chunk, W_ij (A_i.B_j) (D_i.C_j).  blockIdx.y picks the call (dv and dk go in one launch).
+template <typename T, typename TO, bool REV>
+__global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRowsCall<TO> call0, LaRowsCall<TO> call1, LaGeom gm,
+                                                             float intra, float cs, float us, float* __restrict__ leave) {
   __shared__ __align__(16) float sB[kChunk * kRowStride];
   __shared__ float sC[kChunk * kColStride], sM[kHd * kColStride], sP[kChunk * kColStride], s_w[kChunk];
-  __shared__ float s_red[kLaThreads / kWave];
+  __shared__ double s_red[kLaThreads / kWave];
+  const LaRowsCall<TO>& call = blockIdx.y ? call1 : call0;
+  const LaRows A_ = call.A, B_ = call.B, C_ = call.C, D_ = call.D;
+  const int64_t o2 = call.o2;
   const int seg = blockIdx.x % gm.segs, h = blockIdx.x / gm.segs % gm.H, b = blockIdx.x / gm.segs / gm.H;
   const int l = threadIdx.x % kWave, w = threadIdx.x / kWave, g = l / 16, c = l % 16;
   const int len = la_length(gm, b), t0 = seg * gm.seg;
   const int tend = t0 + gm.seg < gm.N ? t0 + gm.seg : gm.N;
   const int t1 = tend < len ? tend : len;
-  TO* po = out + b * o0 + h * o1;
+  TO* po = call.out + b * call.o0 + h * call.o1;
   // rows behind the sequence are zero
   for (int i = (t1 > t0 ? t1 : t0) * kHd + threadIdx.x; i < tend * kHd; i += kLaThreads)
     po[static_cast<int64_t>(i / kHd) * o2 + i % kHd] = from_f32<TO>(0.f);
   const float lg = la_log2_decay(gm, h);
-  const T* pa = static_cast<const T*>(A_.p) + b * A_.s0 + (h / (gm.H / ah)) * A_.s1;
-  const T* pb = static_cast<const T*>(B_.p) + b * B_.s0 + (h / (gm.H / bh)) * B_.s1;
-  const T* pc = static_cast<const T*>(C_.p) + b * C_.s0 + (h / (gm.H / ch)) * C_.s1;
-  const T* pd = D_.p ? static_cast<const T*>(D_.p) + b * D_.s0 + (h / (gm.H / dh)) * D_.s1 : nullptr;
+  const T* pa = static_cast<const T*>(A_.p) + b * A_.s0 + (h / (gm.H / call.ah)) * A_.s1;
+  const T* pb = static_cast<const T*>(B_.p) + b * B_.s0 + (h / (gm.H / call.bh)) * B_.s1;
+  const T* pc = static_cast<const T*>(C_.p) + b * C_.s0 + (h / (gm.H / call.ch)) * C_.s1;
+  const T* pd = call.dot ? static_cast<const T*>(D_.p) + b * D_.s0 + (h / (gm.H / call.dh)) * D_.s1 : nullptr;
   f32x4 M[4];
-  const float* en = enter ? enter + static_cast<int64_t>(blockIdx.x) * kState : nullptr;
+  const float* en = call.enter ? call.enter + static_cast<int64_t>(blockIdx.x) * kState : nullptr;
 #pragma unroll
   for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * w + 4 * g + r, j = 16 * ct + c;
-      M[ct][r] = en ? en[TRANS ? j * kHd + i : i * kHd + j] : 0.f;
+      M[ct][r] = en ? en[call.trans ? j * kHd + i : i * kHd + j] : 0.f;
     }
   const float mid = 0.5f * static_cast<float>(gm.seg);
-  float total = 0.f;
+  double total = 0.;
   const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
   for (int i = 0; i < chunks; ++i) {
     const int t = t0 + (REV ? chunks - 1 - i : i) * kChunk;
@@ -326,8 +356,26 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRows A_, int ah, 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int ii = 16 * w + 4 * g + r, jj = 16 * ct + c, gap = REV ? jj - ii : ii - jj;
-        sP[ii * kColStride + jj] = gap >= 0 ? intra * p[ct][r] * la_power(lg, gap) : 0.f;
+        p[ct][r] = gap >= 0 ? intra * p[ct][r] * la_power(lg, gap) : 0.f;
+        sP[ii * kColStride + jj] = p[ct][r];
       }
+    }
+    if (REV && call.dot) {   // uniform
+      float d[16];
+      la_load16<T>(pd + (t + 16 * w + c) * D_.s2 + 16 * g, 16 * w + c < n, d);
+      float pairs = 0.f;
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        f32x4 y = zero4();
+#pragma unroll
+        for (int kk = 0; kk < 16; ++kk) y = mfma16_f32(d[kk], sC[(16 * ct + c) * kColStride + 16 * g + kk], y);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int gap = 16 * ct + c - (16 * w + 4 * g + r);
+          pairs = fmaf(static_cast<float>(gap) * p[ct][r], y[r], pairs);   // p is 0 where the gap is negative
+        }
+      }
+      total -= pairs;
     }
     __syncthreads();
     f32x4 o[4] = {zero4(), zero4(), zero4(), zero4()}, x[4] = {zero4(), zero4(), zero4(), zero4()};
@@ -349,11 +397,11 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRows A_, int ah, 
         float s = 0.f;
 #pragma unroll
         for (int ct = 0; ct < 4; ++ct) {
-          const float v = fmaf(carry, x[ct][r], o[ct][r]);
-          po[(t + ii) * o2 + 16 * ct + c] = from_f32<TO>(v);
-          if (dot) s = fmaf(v, to_f32(pd[(t + ii) * D_.s2 + 16 * ct + c]), s);
+          const float v = carry * x[ct][r];
+          po[(t + ii) * o2 + 16 * ct + c] = from_f32<TO>(v + o[ct][r]);
+          if (call.dot) s = fmaf(v, to_f32(pd[(t + ii) * D_.s2 + 16 * ct + c]), s);
         }
-        total = fmaf(tau, s, total);
+        total += tau * s;
       }
     }
     la_update<kRowStride>(sB, sC, s_w, la_power(lg, n), us, M);
@@ -365,12 +413,9 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRows A_, int ah, 
 #pragma unroll
       for (int r = 0; r < 4; ++r) lv[(16 * w + 4 * g + r) * kHd + 16 * ct + c] = M[ct][r];
   }
-  if (dot) {
-    total = lanes_sum<kWave>(total);
-    __syncthreads();
-    if (l == 0) s_red[w] = total;
-    __syncthreads();
-    if (threadIdx.x == 0) dot[blockIdx.x] = ((s_red[0] + s_red[1]) + s_red[2]) + s_red[3];
+  if (call.dot) {
+    total = workgroup_sum_f64<kLaThreads / kWave>(total, s_red);
+    if (threadIdx.x == 0) call.dot[blockIdx.x] = total;
   }
 }
 
@@ -613,18 +658,6 @@ __device__ __forceinline__ void la_zero_rows(TO* po, int64_t o2, int from, int t
     put4(po + static_cast<int64_t>(i / (kHd / 4)) * o2 + i % (kHd / 4) * 4, zero);
 }
 
-template <int WAVES>
-__device__ __forceinline__ float workgroup_sum(float x, float* s_red) {   // in thread 0
-  x = lanes_sum<kWave>(x);
-  __syncthreads();
-  if (threadIdx.x % kWave == 0) s_red[threadIdx.x / kWave] = x;
-  __syncthreads();
-  float t = s_red[0];
-#pragma unroll
-  for (int i = 1; i < WAVES; ++i) t += s_red[i];
-  return t;
-}
-
 // Segment sums of the forward (see la_local_kernel).  The loads of two chunks are issued at once.
 constexpr int kLocalAhead = 2;
 __global__ __launch_bounds__(kLaThreads, 4) void la_local_bf16(LaRows X_, int xh, LaRows Y_, int yh, LaGeom gm,
@@ -817,7 +850,7 @@ template <bool DECAY>
 __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows O_, LaRows K_, LaRows V_, LaGeom gm,
                                                               const float* __restrict__ enter, bf16* __restrict__ dq,
                                                               int64_t o0, int64_t o1, int64_t o2,
-                                                              float* __restrict__ local, float* __restrict__ dot) {
+                                                              float* __restrict__ local, double* __restrict__ dot) {
   constexpr int kParts = DECAY ? 3 : 2;
   __shared__ __align__(16) char smem[(4 + kParts) * kTileBytes + kTableBytes];
   const LaItem it = la_item(gm);
@@ -934,8 +967,8 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
     }
   }
   if constexpr (DECAY) {
-    total = workgroup_sum<kWideThreads / kWave>(total, reinterpret_cast<float*>(smem));
-    if (threadIdx.x == 0) dot[it.at] = total;
+    const double sum = workgroup_sum_f64<kWideThreads / kWave>(total, reinterpret_cast<double*>(smem));
+    if (threadIdx.x == 0) dot[it.at] = sum;
   }
 }
 
@@ -1077,7 +1110,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dkdv_bf16(LaRows Q_, LaRow
                                                                 const float* __restrict__ enter, TO* __restrict__ dk,
                                                                 int64_t k0, int64_t k1, int64_t k2, TO* __restrict__ dv,
                                                                 int64_t v0, int64_t v1, int64_t v2, int outh,
-                                                                float* __restrict__ dot) {
+                                                                double* __restrict__ dot) {
   __shared__ __align__(16) char smem[(DECAY ? 6 : 10) * kTileBytes];   // q, do, k and G's parts
   const LaItem it = la_item(gm);
   const int len = la_length(gm, it.b), t0 = it.seg * gm.seg;
@@ -1091,15 +1124,21 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dkdv_bf16(LaRows Q_, LaRow
   if (uniform(threadIdx.x / kWave) >= 4) total = la_dkdv_role<true, DECAY>(smem, Q_, O_, K_, V_, gm, it, t0, t1, enter, pdk, k2);
   else total = la_dkdv_role<false, DECAY>(smem, Q_, O_, K_, V_, gm, it, t0, t1, enter, pdv, v2);
   if constexpr (DECAY) {
-    total = workgroup_sum<kWideThreads / kWave>(total, reinterpret_cast<float*>(smem));
-    if (threadIdx.x == 0) dot[it.at] = total;
+    const double sum = workgroup_sum_f64<kWideThreads / kWave>(total, reinterpret_cast<double*>(smem));
+    if (threadIdx.x == 0) dot[it.at] = sum;
   }
 }
 
-// dk or dv of a shared head: the query heads' parts in head order.
+// dk (blockIdx.y 0) and dv of a shared head: the query heads' parts in head order.
 template <typename T>
-__global__ __launch_bounds__(kLaThreads) void la_group_sum(const float* __restrict__ part, T* __restrict__ out, int64_t o0,
-                                                           int64_t o1, int64_t o2, LaGeom gm) {
+struct LaShared {
+  const float* part;
+  T* out;
+  int64_t o0, o1, o2;
+};
+template <typename T>
+__global__ __launch_bounds__(kLaThreads) void la_group_sum(LaShared<T> dk, LaShared<T> dv, LaGeom gm) {
+  const LaShared<T>& x = blockIdx.y ? dv : dk;
   const int group = gm.H / gm.Hkv;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kLaThreads + threadIdx.x;   // four elements of a row
   const int d = static_cast<int>(i % (kHd / 4)) * 4;
@@ -1108,21 +1147,21 @@ __global__ __launch_bounds__(kLaThreads) void la_group_sum(const float* __restri
   const int64_t n = row % gm.N, kv = row / gm.N % gm.Hkv, b = row / gm.N / gm.Hkv;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int q = 0; q < group; ++q) {
-    const float4 x = *reinterpret_cast<const float4*>(part + ((b * gm.H + kv * group + q) * gm.N + n) * kHd + d);
-    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    const float4 v = *reinterpret_cast<const float4*>(x.part + ((b * gm.H + kv * group + q) * gm.N + n) * kHd + d);
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
   }
   const float v[4] = {s.x, s.y, s.z, s.w};
-  store_vec<T, 4>(out + b * o0 + kv * o1 + n * o2 + d, v);
+  store_vec<T, 4>(x.out + b * x.o0 + kv * x.o1 + n * x.o2 + d, v);
 }
 
 // dlog_decay[h]: the segments' sums over the batch, then the boundary terms; a workgroup per head, fixed order.
-__global__ __launch_bounds__(kLaThreads) void la_dlog_kernel(const float* __restrict__ dq_dot,
-                                                             const float* __restrict__ dk_dot,
-                                                             const float* __restrict__ edge, int edges, LaGeom gm,
+__global__ __launch_bounds__(kLaThreads) void la_dlog_kernel(const double* __restrict__ dq_dot,
+                                                             const double* __restrict__ dk_dot,
+                                                             const double* __restrict__ edge, int edges, LaGeom gm,
                                                              float* __restrict__ dlog) {
-  __shared__ float s_red[kLaThreads / kWave];
+  __shared__ double s_red[kLaThreads / kWave];
   const int h = blockIdx.x;
-  float t = 0.f;
+  double t = 0.;
   if (dq_dot) {
     for (int64_t i = threadIdx.x; i < static_cast<int64_t>(gm.B) * gm.segs; i += kLaThreads) {
       const int64_t b = i / gm.segs, s = i % gm.segs;
@@ -1135,11 +1174,8 @@ __global__ __launch_bounds__(kLaThreads) void la_dlog_kernel(const float* __rest
   if (edge)
     for (int64_t i = threadIdx.x; i < static_cast<int64_t>(gm.B) * edges; i += kLaThreads)
       t += edge[(i / edges * gm.H + h) * edges + i % edges];
-  t = lanes_sum<kWave>(t);
-  if (threadIdx.x % kWave == 0) s_red[threadIdx.x / kWave] = t;
-  __syncthreads();
-  if (threadIdx.x == 0)
-    dlog[h] = gm.log_decay[h] > 0.f ? 0.f : ((s_red[0] + s_red[1]) + s_red[2]) + s_red[3];
+  t = workgroup_sum_f64<kLaThreads / kWave>(t, s_red);
+  if (threadIdx.x == 0) dlog[h] = gm.log_decay[h] > 0.f ? 0.f : static_cast<float>(t);
 }
 
 // One token of each row: a wave per (row, head) and column quarter... the state streams through once.
@@ -1258,9 +1294,10 @@ void la_fwd_typed(const dwarf_linear_attention_fwd_args& a, const LaGeom& gm, hi
   if (gm.segs != 1)
     la_scan<false>(a.states, a.initial, a.final, gm, nullptr, nullptr, nullptr, nullptr, stream);
   if (gm.segs == 0) return;
-  hipLaunchKernelGGL((la_rows_kernel<T, T, false, false>), grid, block, 0, stream, q, gm.H, k, gm.Hkv, v, gm.Hkv, gm,
-                     gm.scale, gm.scale, 1.f, enter, static_cast<T*>(a.out), a.out_stride[0], a.out_stride[1],
-                     a.out_stride[2], gm.segs == 1 ? a.final : nullptr, LaRows{}, 1, nullptr);
+  const LaRowsCall<T> call{q, k, v, LaRows{}, gm.H, gm.Hkv, gm.Hkv, 1, enter, false, static_cast<T*>(a.out), a.out_stride[0],
+                           a.out_stride[1], a.out_stride[2], nullptr};
+  hipLaunchKernelGGL((la_rows_kernel<T, T, false>), grid, block, 0, stream, call, call, gm, gm.scale, gm.scale, 1.f,
+                     gm.segs == 1 ? a.final : nullptr);
 }
 
 // Workspace of the backward, in floats: the adjoints per segment, the dlog_decay sums, the shared heads' parts.
@@ -1274,9 +1311,9 @@ LaBwdSpace la_bwd_space(const dwarf_linear_attention_bwd_args& a, const LaGeom& 
   LaBwdSpace s;
   size_t at = 0;
   s.adjoint = at; at += wgs * kState;
-  s.dq_dot = at; at += a.dlog_decay ? pad(wgs) : 0;
-  s.dk_dot = at; at += a.dlog_decay ? pad(wgs) : 0;
-  s.edge = at; at += a.dlog_decay ? pad(static_cast<size_t>(gm.B) * gm.H * scan_wgs(gm)) : 0;
+  s.dq_dot = at; at += a.dlog_decay ? pad(2 * wgs) : 0;   // 64 bits each
+  s.dk_dot = at; at += a.dlog_decay ? pad(2 * wgs) : 0;
+  s.edge = at; at += a.dlog_decay ? pad(2 * static_cast<size_t>(gm.B) * gm.H * scan_wgs(gm)) : 0;
   s.dk_part = at; at += shared ? rows : 0;
   s.dv_part = at; at += shared ? rows : 0;
   s.total = at;
@@ -1292,8 +1329,10 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
   const LaBwdSpace sp = la_bwd_space(a, gm);
   float* ws = static_cast<float*>(a.workspace);
   const bool dlog = a.dlog_decay != nullptr;
-  float *adj = ws + sp.adjoint, *dq_dot = dlog ? ws + sp.dq_dot : nullptr, *dk_dot = dlog ? ws + sp.dk_dot : nullptr;
-  float* edge = dlog ? ws + sp.edge : nullptr;
+  float* adj = ws + sp.adjoint;
+  double* dq_dot = dlog ? reinterpret_cast<double*>(ws + sp.dq_dot) : nullptr;
+  double* dk_dot = dlog ? reinterpret_cast<double*>(ws + sp.dk_dot) : nullptr;
+  double* edge = dlog ? reinterpret_cast<double*>(ws + sp.edge) : nullptr;
   const bool joined = gm.segs != 1 || a.dinitial || dlog;
   const float* enter = joined ? adj : a.dfinal;
   const float* before = gm.segs > 1 ? f.states : f.initial;
@@ -1325,30 +1364,30 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
                            a.dv_stride[2], gm.Hkv, dk_dot);
       }
     } else {
-      hipLaunchKernelGGL((la_rows_kernel<T, T, false, true>), grid, block, 0, stream, dout, gm.H, v, gm.Hkv, k, gm.Hkv, gm,
-                         gm.scale, gm.scale, 1.f, before, static_cast<T*>(a.dq), a.dq_stride[0], a.dq_stride[1],
-                         a.dq_stride[2], nullptr, q, gm.H, dq_dot);
+      const LaRowsCall<T> rows{dout, v, k, q, gm.H, gm.Hkv, gm.Hkv, gm.H, before, true, static_cast<T*>(a.dq), a.dq_stride[0],
+                               a.dq_stride[1], a.dq_stride[2], dq_dot};
+      hipLaunchKernelGGL((la_rows_kernel<T, T, false>), grid, block, 0, stream, rows, rows, gm, gm.scale, gm.scale, 1.f,
+                         nullptr);
+      const dim3 both(grid.x, 2);
       if (shared) {
-        hipLaunchKernelGGL((la_rows_kernel<T, float, true, false>), grid, block, 0, stream, k, gm.Hkv, q, gm.H, dout, gm.H,
-                           gm, gm.scale, 1.f, gm.scale, enter, pv, s0, s1, kHd, nullptr, LaRows{}, 1, nullptr);
-        hipLaunchKernelGGL((la_rows_kernel<T, float, true, true>), grid, block, 0, stream, v, gm.Hkv, dout, gm.H, q, gm.H,
-                           gm, gm.scale, 1.f, gm.scale, enter, pk, s0, s1, kHd, nullptr, k, gm.Hkv, dk_dot);
+        const LaRowsCall<float> cv{k, q, dout, LaRows{}, gm.Hkv, gm.H, gm.H, 1, enter, false, pv, s0, s1, kHd, nullptr};
+        const LaRowsCall<float> ck{v, dout, q, k, gm.Hkv, gm.H, gm.H, gm.Hkv, enter, true, pk, s0, s1, kHd, dk_dot};
+        hipLaunchKernelGGL((la_rows_kernel<T, float, true>), both, block, 0, stream, cv, ck, gm, gm.scale, 1.f, gm.scale,
+                           nullptr);
       } else {
-        hipLaunchKernelGGL((la_rows_kernel<T, T, true, false>), grid, block, 0, stream, k, gm.Hkv, q, gm.H, dout, gm.H, gm,
-                           gm.scale, 1.f, gm.scale, enter, static_cast<T*>(a.dv), a.dv_stride[0], a.dv_stride[1],
-                           a.dv_stride[2], nullptr, LaRows{}, 1, nullptr);
-        hipLaunchKernelGGL((la_rows_kernel<T, T, true, true>), grid, block, 0, stream, v, gm.Hkv, dout, gm.H, q, gm.H, gm,
-                           gm.scale, 1.f, gm.scale, enter, static_cast<T*>(a.dk), a.dk_stride[0], a.dk_stride[1],
-                           a.dk_stride[2], nullptr, k, gm.Hkv, dk_dot);
+        const LaRowsCall<T> cv{k, q, dout, LaRows{}, gm.Hkv, gm.H, gm.H, 1, enter, false, static_cast<T*>(a.dv),
+                               a.dv_stride[0], a.dv_stride[1], a.dv_stride[2], nullptr};
+        const LaRowsCall<T> ck{v, dout, q, k, gm.Hkv, gm.H, gm.H, gm.Hkv, enter, true, static_cast<T*>(a.dk),
+                               a.dk_stride[0], a.dk_stride[1], a.dk_stride[2], dk_dot};
+        hipLaunchKernelGGL((la_rows_kernel<T, T, true>), both, block, 0, stream, cv, ck, gm, gm.scale, 1.f, gm.scale, nullptr);
       }
     }
     if (shared) {
       const int64_t quads = static_cast<int64_t>(gm.B) * gm.Hkv * gm.N * (kHd / 4);
-      const dim3 sums(static_cast<unsigned>((quads + kLaThreads - 1) / kLaThreads));
-      hipLaunchKernelGGL((la_group_sum<T>), sums, block, 0, stream, pv, static_cast<T*>(a.dv), a.dv_stride[0],
-                         a.dv_stride[1], a.dv_stride[2], gm);
-      hipLaunchKernelGGL((la_group_sum<T>), sums, block, 0, stream, pk, static_cast<T*>(a.dk), a.dk_stride[0],
-                         a.dk_stride[1], a.dk_stride[2], gm);
+      const LaShared<T> sk{pk, static_cast<T*>(a.dk), a.dk_stride[0], a.dk_stride[1], a.dk_stride[2]};
+      const LaShared<T> sv{pv, static_cast<T*>(a.dv), a.dv_stride[0], a.dv_stride[1], a.dv_stride[2]};
+      hipLaunchKernelGGL((la_group_sum<T>), dim3(static_cast<unsigned>((quads + kLaThreads - 1) / kLaThreads), 2), block, 0,
+                         stream, sk, sv, gm);
     }
   }
   if (dlog)
