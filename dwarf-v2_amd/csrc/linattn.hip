@@ -576,28 +576,35 @@ struct StateWeights {
   }
 };
 
-// M += factor sum_j weight_j X_j Y_j^T for the wave's 16 columns of X and all of Y.  PARTS: of the weighted X, three where
-// the sum goes into an fp32 result, two where it only goes into rows that are rounded to bf16.
+// M = shrink M + factor sum_j weight_j X_j Y_j^T for the wave's 16 columns of X and all of Y.  PARTS: of the weighted X,
+// three where the sum goes into an fp32 result, two where it only goes into rows that are rounded to bf16.  The chunk's sum
+// is formed from zero and then joins M by rounded arithmetic: the matrix instructions round each addition towards zero, and
+// over a state's many chunks that would be a bias.
 template <int PARTS, typename W>
-__device__ __forceinline__ void state_add(const char* sX, const char* sY, const TileMap& m, int w, const W& weights,
-                                          float factor, f32x4* M) {
+__device__ __forceinline__ void state_update(const char* sX, const char* sY, const TileMap& m, int w, const W& weights,
+                                             float factor, float shrink, f32x4* M) {
+  bf16x8 parts[2][PARTS];
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
-    bf16x8 y[4];
-#pragma unroll
-    for (int ct = 0; ct < 4; ++ct) y[ct] = tile_column(sY, m, ct, ks);
     float x[8];
     unpack8(tile_column(sX, m, w, ks), x);
     weights.apply(ks, factor, x);
-    bf16x8 parts[PARTS];
-    split8<PARTS>(x, parts);
+    split8<PARTS>(x, parts[ks]);
+  }
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p)
+  for (int ct = 0; ct < 4; ++ct) {   // one tile of M at a time: all four at once spill (dq 61 us for 47 at B8 N2048 H8)
+    f32x4 add = zero4();
 #pragma unroll
-      for (int ct = 0; ct < 4; ++ct) M[ct] = mfma16_bf16(parts[p], y[ct], M[ct]);
+    for (int ks = 0; ks < 2; ++ks) {
+      const bf16x8 y = tile_column(sY, m, ct, ks);
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) add = mfma16_bf16(parts[ks][p], y, add);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) M[ct][r] = fmaf(M[ct][r], shrink, add[r]);
   }
 }
-__device__ __forceinline__ void state_shrink(f32x4* M, float shrink) {
+__device__ __forceinline__ void rows_scale(f32x4* M, float shrink) {
 #pragma unroll
   for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
@@ -691,8 +698,7 @@ __global__ __launch_bounds__(kLaThreads, 4) void la_local_bf16(LaRows X_, int xh
         tile_put(y[u], s + kTileBytes, m);
         __syncthreads();   // also: every wave is done with the other buffer
         const int t = t0 + (i0 + u) * kChunk, n = t1 - t < kChunk ? t1 - t : kChunk;
-        state_shrink(M, n < kChunk ? la_power(lg, n) : full);
-        state_add<3>(s, s + kTileBytes, m, w, StateWeights(tables, n), 1.f, M);
+        state_update<3>(s, s + kTileBytes, m, w, StateWeights(tables, n), 1.f, n < kChunk ? la_power(lg, n) : full, M);
       }
     }
   }
@@ -767,9 +773,8 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
       __syncthreads();   // also: every wave is done with the other buffer
       fetch(i + 1);
       const int n = live(i);
-      state_shrink(M, n < kChunk ? la_power(lg, n) : full);
       const StateWeights wt(tables, n);
-      state_add<3>(s, s + kTileBytes, m, w, wt, 1.f, M);   // (two parts would do where nothing leaves: no faster)
+      state_update<3>(s, s + kTileBytes, m, w, wt, 1.f, n < kChunk ? la_power(lg, n) : full, M);   // (two parts would do where nothing leaves: no faster)
       state_put<2>(M, other + 2 * kTileBytes, m);
     }
     if (leave) state_store(M, leave + it.at * kState);
@@ -803,7 +808,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
         o[ct] = mfma16_bf16(tile_row(sM, m, ct, ks), a[ks], o[ct]);
         o[ct] = mfma16_bf16(tile_row(sM + kTileBytes, m, ct, ks), a[ks], o[ct]);
       }
-    state_shrink(o, carry);
+    rows_scale(o, carry);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       if (2 * ks <= w) {   // uniform: some of the 32 tokens are not behind the wave's rows
@@ -896,10 +901,9 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
       __syncthreads();
       fetch(i + 1);
       const int n = live(i);
-      state_shrink(M, n < kChunk ? la_power(lg, n) : full);
-      state_add<kParts>(sV, sK, m, w, StateWeights(tables, n), 1.f, M);
+      state_update<kParts>(sV, sK, m, w, StateWeights(tables, n), 1.f, n < kChunk ? la_power(lg, n) : full, M);
       if (local) {
-        state_add<3>(sQ, sO, m, w, wl, past, L);
+        state_update<3>(sQ, sO, m, w, wl, past, 1.f, L);
         past *= full;
       }
       __syncthreads();   // every wave is done with the tiles
@@ -921,7 +925,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
           for (int p = 0; p < kParts; ++p) o[ct] = mfma16_bf16(tile_row(sM + p * kTileBytes, m, ct, ks), a[ks], o[ct]);
-      state_shrink(o, carry);
+      rows_scale(o, carry);
       if constexpr (DECAY) {
         float sum = 0.f;
 #pragma unroll
@@ -1040,7 +1044,7 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
           const char* s = sG + part * kTileBytes;
           acc[ct] = mfma16_bf16(KEYS ? tile_column(s, m, ct, ks) : tile_row(s, m, ct, ks), a[ks], acc[ct]);
         }
-    state_shrink(acc, la_power(lg, n - 1 - row < 0 ? 0 : n - 1 - row));
+    rows_scale(acc, la_power(lg, n - 1 - row < 0 ? 0 : n - 1 - row));
     if constexpr (KEYS && DECAY) {
       float sum = 0.f;
 #pragma unroll
@@ -1093,8 +1097,7 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
       }
     }
     if constexpr (!KEYS) {
-      state_shrink(G, n < kChunk ? la_power(lg, n) : full);
-      state_add<kParts>(sQ, sO, m, w, wt, 1.f, G);
+      state_update<kParts>(sQ, sO, m, w, wt, 1.f, n < kChunk ? la_power(lg, n) : full, G);
     }
     if constexpr (DECAY) __syncthreads();   // every wave is done with the tiles
   }
