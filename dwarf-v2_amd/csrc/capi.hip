@@ -867,9 +867,9 @@ static int check_norm(const dwarf_layer_norm_fwd_args& a) {
     return fail(DWARF_ERR_INVALID_ARGUMENT, "bad sizes rows=%lld groups=%d D=%d", static_cast<long long>(a.rows), a.groups, a.D);
   if (!mixer_dtype(a.dtype)) return fail(DWARF_ERR_INVALID_ARGUMENT, "dtype=%d", a.dtype);
   if (!(a.eps >= 0.f) || !finite_f32(a.eps)) return fail(DWARF_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
-  if (a.groups > 65535 || a.D > (1 << 24) || static_cast<int64_t>(a.groups) * a.D >= (int64_t(1) << 30) ||
+  if (a.groups > 65535 || a.D > (1 << 24) || static_cast<int64_t>(a.groups) * a.D >= (int64_t(1) << 25) ||
       a.rows >= (int64_t(1) << 40))
-    return fail(DWARF_ERR_UNSUPPORTED, "groups up to 65535, D up to 2^24 and groups * D below 2^30");
+    return fail(DWARF_ERR_UNSUPPORTED, "groups up to 65535, D up to 2^24 and groups * D below 2^25");
   return a.rows ? check_elements("x", a.x, a.dtype) : DWARF_OK;
 }
 
@@ -957,8 +957,12 @@ static int check_linear_attention(const dwarf_linear_attention_fwd_args& a) {
   int rc = check_heads(a.B, a.H, a.H_kv, a.head_dim, a.dtype, a.scale);
   if (rc) return rc;
   if (a.N < 0) return fail(DWARF_ERR_INVALID_ARGUMENT, "N=%d", a.N);
-  if (a.N > (1 << 24) || static_cast<double>(a.B) * a.H * (a.N / 64 + 16) >= 0x1p31)
-    return fail(DWARF_ERR_UNSUPPORTED, "N up to 2^24 and B * H * N / 64 below 2^31");
+  if (a.N > (1 << 24)) return fail(DWARF_ERR_UNSUPPORTED, "N up to 2^24 (got %d)", a.N);
+  // a launch counts its threads in 32 bits: 512 for each segment of a head, and in the scan at most 2^14 for each head
+  const int64_t heads = static_cast<int64_t>(a.B) * a.H, seg = dwarf::linear_attention_segment(a.B, a.H, a.N);
+  const int64_t segs = (a.N + seg - 1) / seg;
+  if (heads * (segs > 2 ? segs : 2) >= (int64_t(1) << 23) || (segs > 8 && heads >= (int64_t(1) << 18)))
+    return fail(DWARF_ERR_UNSUPPORTED, "B * H * segments must stay below 2^23");
   if (a.B == 0) return DWARF_OK;
   if (!a.log_decay) return fail(DWARF_ERR_INVALID_ARGUMENT, "log_decay is NULL");
   if ((a.initial && !aligned16(a.initial)) || (a.final && !aligned16(a.final)))
@@ -1004,6 +1008,8 @@ int dwarf_linear_attention_bwd(const dwarf_linear_attention_bwd_args* args, dwar
   const dwarf_linear_attention_bwd_args& a = *args;
   int rc = check_linear_attention(a.fwd);
   if (rc) return rc;
+  if (a.fwd.H != a.fwd.H_kv && static_cast<double>(a.fwd.B) * a.fwd.H_kv * a.fwd.N >= 0x1p28)   // threads of the groups' sums
+    return fail(DWARF_ERR_UNSUPPORTED, "gradients of shared heads: B * H_kv * N must stay below 2^28");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (a.fwd.B == 0) return zero_floats(a.dlog_decay, a.fwd.H, s, "dwarf_linear_attention_bwd");
   if (a.fwd.N) {
@@ -1028,7 +1034,7 @@ int dwarf_linear_attention_step(const dwarf_linear_attention_step_args* args, dw
   const dwarf_linear_attention_step_args& a = *args;
   int rc = check_heads(a.S, a.H, a.H_kv, a.head_dim, a.dtype, a.scale);
   if (rc) return rc;
-  if (static_cast<int64_t>(a.S) * a.H >= (int64_t(1) << 30)) return fail(DWARF_ERR_UNSUPPORTED, "S * H must stay below 2^30");
+  if (static_cast<int64_t>(a.S) * a.H >= (int64_t(1) << 24)) return fail(DWARF_ERR_UNSUPPORTED, "S * H must stay below 2^24");
   if (a.S == 0) return ok();
   if (!a.log_decay) return fail(DWARF_ERR_INVALID_ARGUMENT, "log_decay is NULL");
   if ((rc = check_rows("q", a.q, a.q_stride, 2, a.dtype))) return rc;

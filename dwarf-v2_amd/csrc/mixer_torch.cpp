@@ -13,6 +13,7 @@
 #include <pybind11/stl.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -58,6 +59,12 @@ int dtype_of(const Tensor& x, const char* what) {
   }
 }
 
+// A size as the C ABI takes it.
+int32_t size32(int64_t n) {
+  TORCH_CHECK(n <= INT32_MAX, "dimensions must stay below 2^31, got ", n);
+  return static_cast<int32_t>(n);
+}
+
 void check_cuda(const Tensor& x) { TORCH_CHECK(x.is_cuda(), "the mixer's HIP kernels require device tensors"); }
 void check_beside(const char* name, const Tensor& t, const Tensor& x) {
   TORCH_CHECK_VALUE(t.device() == x.device(), name, " is on ", t.device(), ", expected ", x.device());
@@ -96,7 +103,9 @@ bool rows_ok(const Tensor& t) {
     if (s[i] % per16) return false;
   return true;
 }
-Tensor kernel_rows(const Tensor& t) { return rows_ok(t) ? t : t.contiguous(); }
+// A contiguous copy: contiguous() alone gives a dense tensor back as it is, at whatever address it begins.
+Tensor dense_copy(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
+Tensor kernel_rows(const Tensor& t) { return rows_ok(t) ? t : dense_copy(t); }
 
 // Gradients whose own derivative raises: the backward nodes are first order.
 variable_list first_order(variable_list grads, const char* what) {
@@ -156,8 +165,8 @@ float* f32_out(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nul
 void norm_fill(dwarf_layer_norm_fwd_args& a, const NormRows& r, int64_t groups, const Tensor& w, double eps) {
   const int64_t D = r.x.size(-1);
   a.rows = r.x.numel() / (groups * D);
-  a.groups = static_cast<int32_t>(groups);
-  a.D = static_cast<int32_t>(D);
+  a.groups = size32(groups);
+  a.D = size32(D);
   a.dtype = dtype_of(r.x, "x");
   a.eps = static_cast<float>(eps);
   a.x = r.x.const_data_ptr();
@@ -267,18 +276,18 @@ Tensor pair_rows(const Tensor& x, bool interleaved) {
   const auto s = x.strides();
   bool ok = s[3] == 1;
   if (interleaved) ok = ok && aligned(x, 2 * x.element_size()) && s[0] % 2 == 0 && s[1] % 2 == 0 && s[2] % 2 == 0;
-  return ok ? x : x.contiguous();
+  return ok ? x : dense_copy(x);
 }
 
 std::tuple<Tensor, Tensor> rotate(const Tensor& q_, const OptTensor& k_, const Tensor& positions, const Tensor& turns,
                                   bool interleaved, bool inverse, double magnitude) {
   const Tensor q = pair_rows(q_.detach(), interleaved);
   dwarf_rotary_args a{};
-  a.B = static_cast<int32_t>(q.size(0));
-  a.H = static_cast<int32_t>(q.size(1));
-  a.N = static_cast<int32_t>(q.size(2));
-  a.D = static_cast<int32_t>(q.size(3));
-  a.pairs = static_cast<int32_t>(turns.numel());
+  a.B = size32(q.size(0));
+  a.H = size32(q.size(1));
+  a.N = size32(q.size(2));
+  a.D = size32(q.size(3));
+  a.pairs = size32(turns.numel());
   a.dtype = dtype_of(q, "q");
   a.interleaved = interleaved;
   a.inverse = inverse;
@@ -291,7 +300,7 @@ std::tuple<Tensor, Tensor> rotate(const Tensor& q_, const OptTensor& k_, const T
   Tensor k, k_out;
   if (k_) {
     k = pair_rows(k_->detach(), interleaved);
-    a.H_kv = static_cast<int32_t>(k.size(1));
+    a.H_kv = size32(k.size(1));
     k_out = token_major(a.B, a.H_kv, a.N, a.D, k);
     a.k = k.const_data_ptr();
     put_strides(a.k_stride, k);
@@ -370,20 +379,22 @@ std::tuple<Tensor, OptTensor> rotary_embed(const Tensor& q, const OptTensor& k, 
 // ---- decayed linear attention ------------------------------------------------------------------
 // [B,H,N,64] as the kernels read it: 16-byte aligned rows that do not overlap, less than 2^22 elements apart.
 Tensor token_rows(const Tensor& t) {
-  if (t.size(2) > 1 && (t.stride(2) < kHd || t.stride(2) >= (int64_t(1) << 22))) return t.contiguous();
+  if (t.size(2) > 1 && (t.stride(2) < kHd || t.stride(2) >= (int64_t(1) << 22))) return dense_copy(t);
   return kernel_rows(t);
 }
 Tensor aligned_f32(const Tensor& t) {
   const Tensor c = t.detach().to(at::kFloat).contiguous();
-  return aligned(c, 16) ? c : c.clone();
+  return aligned(c, 16) ? c : dense_copy(c);
 }
 Tensor decay_table(const Tensor& log_decay) {
   const Tensor d = log_decay.detach();
   return d.scalar_type() == at::kFloat && d.is_contiguous() ? d : d.to(at::kFloat).contiguous();
 }
+// 64-bit values beyond 32 bits stay what they mean, below every slot and length or above them all.
 Tensor index_table(const OptTensor& t) {
   if (!t) return Tensor();
-  return t->scalar_type() == at::kInt && t->is_contiguous() ? *t : t->to(at::kInt).contiguous();
+  if (t->scalar_type() != at::kInt) return t->clamp(-1, INT32_MAX).to(at::kInt).contiguous();
+  return t->contiguous();
 }
 const int32_t* i32_ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
 
@@ -395,11 +406,11 @@ struct Operands {
       : q(token_rows(q_.detach())), k(token_rows(k_.detach())), v(token_rows(v_.detach())), decay(decay_table(log_decay)),
         initial(initial_ ? aligned_f32(*initial_) : Tensor()), lengths(index_table(lengths_)) {}
   void fill(dwarf_linear_attention_fwd_args& a, double scale) const {
-    a.B = static_cast<int32_t>(q.size(0));
-    a.H = static_cast<int32_t>(q.size(1));
-    a.H_kv = static_cast<int32_t>(k.size(1));
-    a.N = static_cast<int32_t>(q.size(2));
-    a.head_dim = static_cast<int32_t>(q.size(3));
+    a.B = size32(q.size(0));
+    a.H = size32(q.size(1));
+    a.H_kv = size32(k.size(1));
+    a.N = size32(q.size(2));
+    a.head_dim = size32(q.size(3));
     a.dtype = dtype_of(q, "q");
     a.scale = static_cast<float>(scale);
     a.q = q.const_data_ptr();
@@ -585,11 +596,11 @@ Tensor attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, cons
   const Tensor decay = decay_table(log_decay), slots = index_table(slots_);
   const Tensor out = out_ ? *out_ : at::empty(q.sizes(), q.options());
   dwarf_linear_attention_step_args a{};
-  a.S = static_cast<int32_t>(q.size(0));
-  a.H = static_cast<int32_t>(q.size(1));
-  a.H_kv = static_cast<int32_t>(k.size(1));
-  a.pool = static_cast<int32_t>(state.size(0));
-  a.head_dim = static_cast<int32_t>(q.size(2));
+  a.S = size32(q.size(0));
+  a.H = size32(q.size(1));
+  a.H_kv = size32(k.size(1));
+  a.pool = size32(state.size(0));
+  a.head_dim = size32(q.size(2));
   a.dtype = dtype_of(q, "q");
   a.scale = static_cast<float>(scale);
   a.q = q.const_data_ptr();
@@ -629,6 +640,14 @@ Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, 
   if (out)
     TORCH_CHECK_VALUE(out->sizes() == q.sizes() && out->scalar_type() == q.scalar_type() && rows_ok(*out), "out must be [", S,
                       ",", H, ",64] ", q.scalar_type(), " with 16-byte aligned rows");
+  if (out)
+    for (const auto& [name, t] : {std::make_pair("out", &*out), std::make_pair("q", &q), std::make_pair("k", &k),
+                                  std::make_pair("v", &v), std::make_pair("state", &state)}) {
+      const bool shared = t == &*out ? at::has_internal_overlap(*t) == at::MemOverlap::Yes
+                                     : at::get_overlap_status(*out, *t) != at::MemOverlapStatus::No &&
+                                           at::get_overlap_status(*out, *t) != at::MemOverlapStatus::TooHard;
+      TORCH_CHECK_VALUE(!shared, "out shares memory with ", name);
+    }
   check_cuda(q);
   check_beside("k", k, q);
   check_beside("v", v, q);
@@ -638,7 +657,8 @@ Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, 
   check_beside("new_state", new_state, q);
   check_beside("out", out, q);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() ||
-                                               log_decay.requires_grad() || state.requires_grad()),
+                                               log_decay.requires_grad() || state.requires_grad() ||
+                                               (new_state && new_state->requires_grad()) || (out && out->requires_grad())),
               "linear_attention_step has no gradients: call it under torch.no_grad(), or linear_attention");
   TORCH_CHECK_VALUE(!S || state.size(0), "the pool is empty");
   return attention_step(q, k, v, log_decay, state, new_state, slots, scale, out);

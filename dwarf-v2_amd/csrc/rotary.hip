@@ -58,7 +58,7 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotTensor q, RotTen
                                                              int64_t p0, int64_t p1, int narrow, int inverse,
                                                              const uint64_t* __restrict__ turns, RotGeom gm) {
   constexpr int kPairs = INTERLEAVED ? VEC / 2 : VEC;   // pairs of a unit
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kRotThreads + threadIdx.x;
+  const int64_t id = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * kRotThreads + threadIdx.x;
   const uint32_t per_token = static_cast<uint32_t>(gm.units) * static_cast<uint32_t>(gm.slices);
   int64_t token, b;
   if (gm.small) {   // uniform: the whole grid counts in 32 bits
@@ -150,10 +150,12 @@ void rot_launch(const dwarf_rotary_args& a, hipStream_t stream) {
   gm.slices = each * four >= 256 * 1024 ? four : gm.heads;
   const int64_t threads = each * gm.slices;
   gm.small = threads < (int64_t(1) << 31);
-  hipLaunchKernelGGL((rotary_kernel<T, VEC, INTERLEAVED>), dim3(static_cast<unsigned>((threads + kRotThreads - 1) / kRotThreads)),
-                     dim3(kRotThreads), 0, stream, rot_tensor(a.q, a.q_stride, a.q_out, a.q_out_stride),
-                     rot_tensor(a.k, a.k_stride, a.k_out, a.k_out_stride), a.positions, a.position_stride[0],
-                     a.position_stride[1], a.position_bytes == 4, a.inverse, a.turns, gm);
+  // a grid's dimension counts its threads in 32 bits
+  const int64_t blocks = (threads + kRotThreads - 1) / kRotThreads, most = 1 << 22, wide = blocks < most ? blocks : most;
+  const dim3 grid(static_cast<unsigned>(wide), static_cast<unsigned>((blocks + wide - 1) / wide));
+  hipLaunchKernelGGL((rotary_kernel<T, VEC, INTERLEAVED>), grid, dim3(kRotThreads), 0, stream,
+                     rot_tensor(a.q, a.q_stride, a.q_out, a.q_out_stride), rot_tensor(a.k, a.k_stride, a.k_out, a.k_out_stride),
+                     a.positions, a.position_stride[0], a.position_stride[1], a.position_bytes == 4, a.inverse, a.turns, gm);
 }
 
 template <typename T>

@@ -183,6 +183,33 @@ def test_linear_attention_entry_points_refuse(pkg, lib):
     assert lib.dwarf_linear_attention_step(ctypes.byref(s), None) == L.DWARF_OK
 
 
+def test_sizes_that_no_launch_holds_are_refused(pkg, lib):
+    """Before anything is read or launched: more threads than 32 bits count."""
+    L = pkg._lib
+    a = L.LinearAttentionBwdArgs()
+    f = a.fwd
+    f.H, f.H_kv, f.head_dim, f.scale = 4, 2, 64, 0.125
+    for B, N in ((1 << 21, 1), (1 << 20, 1025), (1 << 13, 1 << 18), (1 << 20, 0)):
+        f.B, f.N = B, N
+        assert lib.dwarf_linear_attention_fwd(ctypes.byref(f), None) == L.DWARF_ERR_UNSUPPORTED, (B, N)
+        assert lib.dwarf_linear_attention_bwd(ctypes.byref(a), None) == L.DWARF_ERR_UNSUPPORTED, (B, N)
+    s = L.LinearAttentionStepArgs()
+    s.S, s.H, s.H_kv, s.head_dim, s.scale = 1 << 22, 4, 2, 64, 0.125
+    assert lib.dwarf_linear_attention_step(ctypes.byref(s), None) == L.DWARF_ERR_UNSUPPORTED
+    n = L.LayerNormFwdArgs()
+    n.rows, n.groups, n.D, n.dtype, n.eps = 1, 1 << 9, 1 << 16, L.DWARF_BF16, 1e-5
+    assert lib.dwarf_layer_norm_fwd(ctypes.byref(n), None) == L.DWARF_ERR_UNSUPPORTED
+
+
+def test_step_refuses_out_in_its_inputs_memory(pkg):
+    q, k, v = (torch.zeros(3, 4, 64) for _ in range(3))
+    pool = torch.zeros(3, 4, 64, 64)
+    for out in (q, v, pool[0, :3], torch.zeros(1, 4, 64).expand(3, 4, 64)):
+        out = out if out.shape == q.shape else out.reshape(-1)[:768].view(3, 4, 64)
+        with pytest.raises(ValueError, match="memory|aligned"):
+            pkg.linear_attention_step(q, k, v, torch.zeros(4), pool, out=out)
+
+
 def test_segment_rule_is_the_librarys(pkg, lib):
     for B in (1, 2, 3, 15, 20, 64):
         for H in (1, 6, 8, 32):
