@@ -13,7 +13,9 @@
 //
 // The grid's stride over the rows is a multiple of the groups, so a thread
 // keeps one group: its weights and its part of dw and db stay in registers
-// over all its rows.  A workgroup adds its threads' parts in LDS and writes
+// over all its rows, and its place moves by one step (with a division by the
+// groups for each row and weights read one by one, B15 T2048 D512 took 19.4 us
+// forward and 23.5 backward where it takes 12.6 and 21.9).  A workgroup adds its threads' parts in LDS and writes
 // one partial row per group that it holds; a second launch adds those in a
 // fixed order.
 #include "mixer.h"
@@ -23,6 +25,8 @@ namespace {
 
 constexpr int kNormThreads = 256;
 constexpr int kNormBwdThreads = 512;
+constexpr int kNormBlocks = 2048;   // 768: 14.4 us for B15 T2048 D512 in bf16, 1,536: 13.1, 2,048: 12.6 (63 MB: 5.0 TB/s)
+constexpr int kNormBwdBlocks = 512;   // with the sums' launch behind it, 256: 27.6 us there, 512: 25.9, 768: 27.5, 1,024: 29.0
 
 struct NormGeom {
   int64_t rows;   // rows * groups of the call
@@ -75,6 +79,35 @@ struct NormRaw {
   }
 };
 
+// The rows of a thread in the register kernels: row `first` and every row a grid's stride behind it, all of one group, so
+// that its place moves by one fixed step and no row is divided by the groups.
+struct NormWalk {
+  uint32_t first, group;   // both kernels' grids hold fewer than 2^32 rows
+  int64_t outer, by;       // first / groups, and the stride over the outer rows
+  __device__ __forceinline__ NormWalk(int block_rows, int row, int groups) {
+    first = blockIdx.x * static_cast<uint32_t>(block_rows) + static_cast<uint32_t>(row);
+    const uint32_t o = first / static_cast<uint32_t>(groups);
+    group = first - o * static_cast<uint32_t>(groups);
+    outer = o;
+    by = gridDim.x * static_cast<uint32_t>(block_rows) / static_cast<uint32_t>(groups);   // a whole number
+  }
+  template <typename T>
+  __device__ __forceinline__ T* at(T* p, int64_t s0, int64_t s1) const { return p + outer * s0 + group * s1; }
+};
+
+// A thread's part of a group's weights (or biases), `none` where there are none; aligned to their elements only.
+template <int VEC, int TPR, int K>
+__device__ __forceinline__ void norm_table(const float* t, uint32_t group, int sub, int D, float none, float* w) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int d = (k * TPR + sub) * VEC;
+    if (t) __builtin_memcpy(w + k * VEC, t + static_cast<int64_t>(group) * D + (d < D ? d : 0), VEC * sizeof(float));
+    else
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[k * VEC + e] = none;
+  }
+}
+
 template <typename T, int VEC, int TPR, int K>
 __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const T* __restrict__ x, int64_t xs0, int64_t xs1,
                                                                 const float* __restrict__ weight,
@@ -84,28 +117,22 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const T* __restr
   __shared__ float s_red[kNormThreads / kWave];
   const int sub = threadIdx.x % TPR;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;   // a multiple of the groups
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
-  if (first >= gm.rows) return;   // a row's threads together
+  const NormWalk walk(kRows, threadIdx.x / TPR, gm.groups);
+  if (walk.first >= gm.rows) return;   // a row's threads together
   const float fd = static_cast<float>(gm.D);   // sums are divided, so that a row of one value has it as its mean
+  const T* px = walk.at(x, xs0, xs1);
+  T* yr = walk.at(y, ys0, ys1);
   NormRaw<T, VEC, TPR, K> next;
-  next.load(x + norm_at(first, gm.groups, xs0, xs1), sub, gm.D);
-  const float* wg = weight + (first % gm.groups) * gm.D;
-  const float* bg = bias + (first % gm.groups) * gm.D;
+  next.load(px, sub, gm.D);
   float w[K * VEC], b[K * VEC];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int d = (k * TPR + sub) * VEC;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[k * VEC + e] = weight && d < gm.D ? wg[d + e] : 1.f;
-      b[k * VEC + e] = bias && d < gm.D ? bg[d + e] : 0.f;
-    }
-  }
-  for (int64_t r = first; r < gm.rows; r += step) {
+  norm_table<VEC, TPR, K>(weight, walk.group, sub, gm.D, 1.f, w);
+  norm_table<VEC, TPR, K>(bias, walk.group, sub, gm.D, 0.f, b);
+  for (int64_t r = walk.first; r < gm.rows; r += step, yr += walk.by * ys0) {
     float v[K * VEC];
     next.widen(sub, gm.D, v);
     // the next row's loads are under way while this one is summed (behind the last row: this one again)
-    next.load(x + norm_at(r + step < gm.rows ? r + step : r, gm.groups, xs0, xs1), sub, gm.D);
+    if (r + step < gm.rows) px += walk.by * xs0;
+    next.load(px, sub, gm.D);
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < K * VEC; ++i) s += v[i];
@@ -121,7 +148,6 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const T* __restr
       }
     }
     const float rs = 1.f / sqrtf(row_sum<TPR, kNormThreads>(q, s_red) / fd + gm.eps);
-    T* yr = y + norm_at(r, gm.groups, ys0, ys1);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int d = (k * TPR + sub) * VEC;
@@ -146,32 +172,30 @@ __global__ __launch_bounds__(kNormBwdThreads) void norm_bwd_kernel(
   __shared__ float s_red[kNormBwdThreads / kWave];
   const int sub = threadIdx.x % TPR, row = threadIdx.x / TPR;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;   // a multiple of the groups
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows + row;
+  const NormWalk walk(kRows, row, gm.groups);
   const float fd = static_cast<float>(gm.D);   // sums are divided, so that a row of one value has it as its mean
-  const float* wg = weight + (first % gm.groups) * gm.D;
-  float w[K * VEC], dw[K * VEC], db[K * VEC];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int d = (k * TPR + sub) * VEC;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[k * VEC + e] = weight && d < gm.D ? wg[d + e] : 1.f;
-      dw[k * VEC + e] = db[k * VEC + e] = 0.f;
-    }
-  }
+  const bool any = walk.first < gm.rows;   // threads without a row read the first one and add nothing
+  const T* px = any ? walk.at(x, xs0, xs1) : x;
+  const T* pg = any ? walk.at(dy, gs0, gs1) : dy;
+  T* dr = walk.at(dx, ds0, ds1);
   NormRaw<T, VEC, TPR, K> nx, ng;
-  auto fetch = [&](int64_t r) {   // behind the last row: that one again
-    if (r >= gm.rows) r = gm.rows - 1;
-    nx.load(x + norm_at(r, gm.groups, xs0, xs1), sub, gm.D);
-    ng.load(dy + norm_at(r, gm.groups, gs0, gs1), sub, gm.D);
-  };
-  fetch(first);
-  for (int64_t r = first; r < gm.rows; r += step) {
+  nx.load(px, sub, gm.D);
+  ng.load(pg, sub, gm.D);
+  float w[K * VEC], dw[K * VEC], db[K * VEC];
+  norm_table<VEC, TPR, K>(weight, walk.group, sub, gm.D, 1.f, w);
+#pragma unroll
+  for (int i = 0; i < K * VEC; ++i) dw[i] = db[i] = 0.f;
+  for (int64_t r = walk.first; r < gm.rows; r += step, dr += walk.by * ds0) {
     float v[K * VEC], g[K * VEC];
     float s = 0.f;
     nx.widen(sub, gm.D, v);
     ng.widen(sub, gm.D, g);
-    fetch(r + step);
+    if (r + step < gm.rows) {   // behind the last row: this one again
+      px += walk.by * xs0;
+      pg += walk.by * gs0;
+    }
+    nx.load(px, sub, gm.D);
+    ng.load(pg, sub, gm.D);
 #pragma unroll
     for (int i = 0; i < K * VEC; ++i) s += v[i];
     const float mu = row_sum<TPR, kNormBwdThreads>(s, s_red) / fd;
@@ -194,7 +218,6 @@ __global__ __launch_bounds__(kNormBwdThreads) void norm_bwd_kernel(
     sgv = row_sum<TPR, kNormBwdThreads>(sgv, s_red);
     const float rs = 1.f / sqrtf(q / fd + gm.eps);
     const float m1 = sg / fd, m2 = sgv / fd * rs * rs;   // mean(gw), mean(gw h) r
-    T* dr = dx + norm_at(r, gm.groups, ds0, ds1);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int d = (k * TPR + sub) * VEC;
@@ -427,7 +450,7 @@ NormPlan norm_plan(const dwarf_layer_norm_fwd_args& f, bool vec, int threads) {
   else p.tpr = 0;
   p.block_rows = p.tpr ? threads / p.tpr : 1;
   const int64_t rows = f.rows * f.groups;
-  p.blocks = static_cast<int>(norm_blocks(rows, f.groups, p.block_rows, 768));
+  p.blocks = static_cast<int>(norm_blocks(rows, f.groups, p.block_rows, kNormBlocks));
   p.columns_y = 0;
   return p;
 }
@@ -439,7 +462,7 @@ NormPlan norm_bwd_plan(const dwarf_layer_norm_bwd_args& a) {
   if (a.dx) vec = vec && norm_vec_ok(a.dx, a.dx_stride, es);
   NormPlan p = norm_plan(a.fwd, vec, kNormBwdThreads);
   const int64_t rows = a.fwd.rows * a.fwd.groups;
-  p.blocks = static_cast<int>(norm_blocks(rows, a.fwd.groups, p.block_rows, 512));
+  p.blocks = static_cast<int>(norm_blocks(rows, a.fwd.groups, p.block_rows, kNormBwdBlocks));
   if (!p.tpr) {
     p.blocks = static_cast<int>(rows < 2048 ? rows : 2048);
     p.columns_y = static_cast<int>(a.fwd.rows < 64 ? a.fwd.rows : 64);
