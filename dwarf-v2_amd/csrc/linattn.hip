@@ -643,6 +643,33 @@ __device__ __forceinline__ void put4(float* p, const float* v) {
   *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
 
+// Rows as the lanes hold them (row c, elements 16 ct + 4 g + [0, 4) of the wave's 16) to memory, `at` the row's start.
+// bf16: the lanes of a row trade halves, so that each holds eight consecutive elements and a store covers 64 bytes of each
+// row, not 32: every lane of the wave takes part.
+__device__ __forceinline__ void put_rows(bf16* at, bool live, const f32x4* o) {
+  const int g = (threadIdx.x % kWave) / 16;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    uint32_t a[2], b[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      a[i] = pack_bf16x2(o[2 * s][2 * i], o[2 * s][2 * i + 1]);
+      b[i] = pack_bf16x2(o[2 * s + 1][2 * i], o[2 * s + 1][2 * i + 1]);
+      const auto x = __builtin_amdgcn_permlane32_swap(a[i], b[i], false, false);   // trades ct's low bit for g's high one
+      const auto y = __builtin_amdgcn_permlane16_swap(x[0], x[1], false, false);   // and that one for g's low one
+      a[i] = y[0];
+      b[i] = y[1];
+    }
+    if (live) *reinterpret_cast<uint4*>(at + 32 * s + 8 * g) = uint4{a[0], a[1], b[0], b[1]};
+  }
+}
+__device__ __forceinline__ void put_rows(float* at, bool live, const f32x4* o) {
+  const int g = (threadIdx.x % kWave) / 16;
+  if (live)
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct) *reinterpret_cast<f32x4*>(at + 16 * ct + 4 * g) = o[ct];
+}
+
 // Work item of a workgroup: the heads of one segment next to each other on one XCD (token-major rows of the heads lie
 // side by side in memory, and query heads share their K/V head's rows), then the segments.
 struct LaItem {
@@ -837,14 +864,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
         }
       }
     }
-    if (16 * w + c < live(i)) {
-      bf16* pr = po + (t0 + static_cast<int64_t>(i) * kChunk + 16 * w + c) * o2;
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct) {
-        const float v[4] = {o[ct][0], o[ct][1], o[ct][2], o[ct][3]};
-        put4(pr + 16 * ct + 4 * g, v);
-      }
-    }
+    put_rows(po + (t0 + static_cast<int64_t>(i) * kChunk + 16 * w + c) * o2, 16 * w + c < live(i), o);
   }
 }
 
@@ -863,7 +883,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
   constexpr int kParts = DECAY ? 3 : 2;
   __shared__ __align__(16) char smem[(4 + kParts) * kTileBytes + kTableBytes];
   const LaItem it = la_item(gm);
-  const int l = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), w = wave % 4, g = l / 16, c = l % 16;
+  const int l = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), w = wave % 4, c = l % 16;
   const bool keeps = wave >= 4;
   const int len = la_length(gm, it.b), t0 = it.seg * gm.seg;
   const int tend = t0 + gm.seg < gm.N ? t0 + gm.seg : gm.N;
@@ -963,14 +983,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
           }
         }
       }
-      if (row < live(i)) {
-        bf16* pr = po + (t0 + static_cast<int64_t>(i) * kChunk + row) * o2;
-#pragma unroll
-        for (int ct = 0; ct < 4; ++ct) {
-          const float v[4] = {o[ct][0], o[ct][1], o[ct][2], o[ct][3]};
-          put4(pr + 16 * ct + 4 * g, v);
-        }
-      }
+      put_rows(po + (t0 + static_cast<int64_t>(i) * kChunk + row) * o2, row < live(i), o);
       __syncthreads();   // every wave is done with the tiles
     }
   }
@@ -1092,14 +1105,7 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
         }
       }
     }
-    if (row < n) {
-      TO* at = pr + (token(i) + row) * stride + 4 * g;
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct) {
-        const float v[4] = {acc[ct][0], acc[ct][1], acc[ct][2], acc[ct][3]};
-        put4(at + 16 * ct, v);
-      }
-    }
+    put_rows(pr + (token(i) + row) * stride, row < n, acc);
     if constexpr (!KEYS) {
       state_update<kParts>(sQ, sO, m, w, wt, 1.f, n < kChunk ? la_power(lg, n) : full, G);
     }
