@@ -181,6 +181,7 @@ __global__ __launch_bounds__(kLaThreads) void la_scan_kernel(float* __restrict__
                                                              const float* __restrict__ initial,
                                                              const float* __restrict__ final, double* __restrict__ dot) {
   constexpr int kOwners = kLaThreads / GROUPS;   // threads of a group
+  constexpr int kSums = GROUPS == 1;             // states: the segments' own sums (LaEnter), not the states in front
   __shared__ f32x4 s_run[GROUPS][kOwners];
   __shared__ double s_red[kLaThreads / kWave];
   const int bh = blockIdx.x / kScanWgs<GROUPS>, owner = threadIdx.x % kOwners, group = threadIdx.x / kOwners;
@@ -211,9 +212,15 @@ __global__ __launch_bounds__(kLaThreads) void la_scan_kernel(float* __restrict__
 #pragma unroll
     for (int i = 0; i < kScanRun; ++i) {
       in[i] = i < cnt ? load(x + segment(i) * kState) : zero4();
-      sv[i] = REV && dot && i < cnt && segment(i) > 0 ? load(st + segment(i) * kState) : zero4();
+      sv[i] = REV && dot && i < cnt && segment(i) > 0 ? load(st + (segment(i) - kSums) * kState) : zero4();
     }
     auto shrink = [&](int i) { return segment(i) == active - 1 ? tail : full; };
+    if constexpr (REV && kSums) {   // all of the head's segments are here: the sums become the states in front
+      f32x4 u = dot && initial ? load(initial + at) : zero4();
+#pragma unroll
+      for (int i = kScanRun - 1; i >= 0; --i)
+        if (i < cnt && segment(i) > 0) u = sv[i] = u * full + sv[i];
+    }
     f32x4 enter = m;
     if constexpr (GROUPS > 1) {
       f32x4 r = zero4();   // the run's own sum
@@ -273,13 +280,19 @@ void la_scan(float* local, const float* first, float* last, const LaGeom& gm, co
                        final, dot);
 }
 
-// One call of la_rows_kernel: rows of A against rows of B and C, the state that enters per segment [.. segs ..] or, with
-// one segment, per head (NULL: zero; trans: read transposed), the result, and with dot the decay's gradient's rows D.
+// Where the state in front of a segment comes from: the scan's array (or, for the adjoint of one segment, dfinal), or,
+// up to kScanRun segments, the head's first state (NULL: zero) and the sums of the segments in front (NULL: none are),
+// joined by the workgroup itself: a few more reads of 16 KB in place of a launch between the sums and the rows.
+struct LaEnter {
+  const float *scanned, *first, *sums;
+};
+
+// One call of la_rows_kernel: rows of A against rows of B and C, the state that enters (trans: read transposed), the result, and with dot the decay's gradient's rows D.
 template <typename TO>
 struct LaRowsCall {
   LaRows A, B, C, D;
   int ah, bh, ch, dh;    // heads of each
-  const float* enter;
+  LaEnter enter;
   bool trans;
   TO* out;
   int64_t o0, o1, o2;
@@ -287,7 +300,8 @@ struct LaRowsCall {
 };
 
 // out_i = intra sum_j W_ij (A_i.B_j) C_j + cs W_i A_i M over a segment's chunks, M updated behind each (in front, in
-// reverse); in fp32 throughout, for fp32 and fp16 rows.  leave: with one segment, where the state that leaves goes.
+// reverse); in fp32 throughout, for fp32 and fp16 rows.  leave: where the state behind the last token goes (NULL: nowhere, or the
+// scan has written it).
 // dot, forward: sum tau D_i.(out_i's part that comes from M); in reverse the same less (i - j) times each pair's share
 // within a chunk, W_ij (A_i.B_j) (D_i.C_j).  blockIdx.y picks the call (dv and dk go in one launch).
 template <typename T, typename TO, bool REV>
@@ -313,15 +327,25 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRowsCall<TO> call
   const T* pb = static_cast<const T*>(B_.p) + b * B_.s0 + (h / (gm.H / call.bh)) * B_.s1;
   const T* pc = static_cast<const T*>(C_.p) + b * C_.s0 + (h / (gm.H / call.ch)) * C_.s1;
   const T* pd = call.dot ? static_cast<const T*>(D_.p) + b * D_.s0 + (h / (gm.H / call.dh)) * D_.s1 : nullptr;
-  f32x4 M[4];
-  const float* en = call.enter ? call.enter + static_cast<int64_t>(blockIdx.x) * kState : nullptr;
+  const int64_t head = static_cast<int64_t>(b) * gm.H + h;
+  const bool leaves = leave && (len ? t0 < len && len <= t0 + gm.seg : seg == 0);
+  f32x4 M[4] = {zero4(), zero4(), zero4(), zero4()};
+  auto join = [&](const float* en, float shrink) {
 #pragma unroll
-  for (int ct = 0; ct < 4; ++ct)
+    for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = 16 * w + 4 * g + r, j = 16 * ct + c;
-      M[ct][r] = en ? en[call.trans ? j * kHd + i : i * kHd + j] : 0.f;
-    }
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * w + 4 * g + r, j = 16 * ct + c;
+        M[ct][r] = fmaf(M[ct][r], shrink, en[call.trans ? j * kHd + i : i * kHd + j]);
+      }
+  };
+  if (t1 > t0 || leaves) {
+    const LaEnter& e = call.enter;
+    if (e.scanned) join(e.scanned + static_cast<int64_t>(blockIdx.x) * kState, 0.f);
+    if (e.first) join(e.first + head * kState, 0.f);
+    if (e.sums)
+      for (int p = 0; p < seg; ++p) join(e.sums + (head * gm.segs + p) * kState, la_power(lg, gm.seg));
+  }
   const float mid = 0.5f * static_cast<float>(gm.seg);
   double total = 0.;
   const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
@@ -406,8 +430,8 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRowsCall<TO> call
     }
     la_update<kRowStride>(sB, sC, s_w, la_power(lg, n), us, M);
   }
-  if (leave) {
-    float* lv = leave + static_cast<int64_t>(blockIdx.x) * kState;
+  if (leaves) {
+    float* lv = leave + head * kState;
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
@@ -615,6 +639,22 @@ __device__ __forceinline__ void rows_scale(f32x4* M, float shrink) {
     for (int r = 0; r < 4; ++r) M[ct][r] *= shrink;
 }
 
+// Work item of a workgroup: the heads of one segment next to each other on one XCD (token-major rows of the heads lie
+// side by side in memory, and query heads share their K/V head's rows), then the segments.
+struct LaItem {
+  int b, h, seg;
+  int64_t at;   // (b, h, seg) in the state arrays
+};
+__device__ __forceinline__ LaItem la_item(const LaGeom& gm) {
+  const int i = xcd_remap(blockIdx.x, gridDim.x);
+  LaItem it;
+  it.h = i % gm.H;
+  it.seg = i / gm.H % gm.segs;
+  it.b = i / gm.H / gm.segs;
+  it.at = (static_cast<int64_t>(it.b) * gm.H + it.h) * gm.segs + it.seg;
+  return it;
+}
+
 __device__ __forceinline__ void state_load(const float* en, bool trans, f32x4* M) {
   const int l = threadIdx.x % kWave, w = threadIdx.x / kWave % 4, g = l / 16, c = l % 16;
 #pragma unroll
@@ -625,6 +665,22 @@ __device__ __forceinline__ void state_load(const float* en, bool trans, f32x4* M
     else
 #pragma unroll
       for (int r = 0; r < 4; ++r) M[ct][r] = en[(i + r) * kHd + j];
+  }
+}
+__device__ __forceinline__ void state_enter(const LaEnter& e, bool trans, const LaGeom& gm, const LaItem& it, float lg,
+                                            f32x4* M) {
+  const int64_t head = it.b * static_cast<int64_t>(gm.H) + it.h;
+  state_load(e.scanned ? e.scanned + it.at * kState : e.first ? e.first + head * kState : nullptr, trans, M);
+  if (!e.sums) return;
+  const float full = la_power(lg, gm.seg);
+#pragma unroll 1
+  for (int p = 0; p < it.seg; ++p) {
+    f32x4 L[4];
+    state_load(e.sums + (head * gm.segs + p) * kState, trans, L);
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) M[ct][r] = fmaf(M[ct][r], full, L[ct][r]);
   }
 }
 __device__ __forceinline__ void state_store(const f32x4* M, float* out) {
@@ -670,21 +726,6 @@ __device__ __forceinline__ void put_rows(float* at, bool live, const f32x4* o) {
     for (int ct = 0; ct < 4; ++ct) *reinterpret_cast<f32x4*>(at + 16 * ct + 4 * g) = o[ct];
 }
 
-// Work item of a workgroup: the heads of one segment next to each other on one XCD (token-major rows of the heads lie
-// side by side in memory, and query heads share their K/V head's rows), then the segments.
-struct LaItem {
-  int b, h, seg;
-  int64_t at;   // (b, h, seg) in the state arrays
-};
-__device__ __forceinline__ LaItem la_item(const LaGeom& gm) {
-  const int i = xcd_remap(blockIdx.x, gridDim.x);
-  LaItem it;
-  it.h = i % gm.H;
-  it.seg = i / gm.H % gm.segs;
-  it.b = i / gm.H / gm.segs;
-  it.at = (static_cast<int64_t>(it.b) * gm.H + it.h) * gm.segs + it.seg;
-  return it;
-}
 __device__ __forceinline__ const bf16* la_rows_of(const LaRows& x, int heads, const LaGeom& gm, const LaItem& it) {
   return static_cast<const bf16*>(x.p) + it.b * x.s0 + (it.h / (gm.H / heads)) * x.s1;
 }
@@ -763,10 +804,9 @@ struct ScoreWeights {
 constexpr int kWideThreads = 512;
 
 // out_i = scale (sum_{j <= i} g^{i-j} (q_i.k_j) v_j + g^{i+1} q_i S) over a segment's chunks.  LDS: two chunks of k and v
-// and the two parts of the state in front of each.  enter: the state in front of each segment or, with one segment, of
-// each head (NULL: zero); leave: with one segment, where the state behind it goes.
+// and the two parts of the state in front of each.  leave: see la_rows_kernel.
 __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRows K_, LaRows V_, LaGeom gm,
-                                                                const float* __restrict__ enter, bf16* __restrict__ out,
+                                                                LaEnter enter, bf16* __restrict__ out,
                                                                 int64_t o0, int64_t o1, int64_t o2,
                                                                 float* __restrict__ leave) {
   __shared__ __align__(16) char smem[8 * kTileBytes + kTableBytes];
@@ -793,8 +833,10 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
   state_weights_put(lg, live(chunks - 1), reinterpret_cast<float*>(smem + 8 * kTileBytes));
   fetch(0);
   if (keeps) {
+    const bool leaves = leave && (len ? t0 < len && len <= t0 + gm.seg : it.seg == 0);
+    if (!chunks && !leaves) return;
     f32x4 M[4];
-    state_load(enter ? enter + it.at * kState : nullptr, false, M);
+    state_enter(enter, false, gm, it, lg, M);
     state_put<2>(M, smem + 2 * kTileBytes, m);
     const float full = la_power(lg, kChunk);
     for (int i = 0; i < chunks; ++i) {
@@ -808,7 +850,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
       state_update<3>(s, s + kTileBytes, m, w, wt, 1.f, n < kChunk ? la_power(lg, n) : full, M);   // (two parts would do where nothing leaves: no faster)
       state_put<2>(M, other + 2 * kTileBytes, m);
     }
-    if (leave) state_store(M, leave + it.at * kState);
+    if (leaves) state_store(M, leave + (static_cast<int64_t>(it.b) * gm.H + it.h) * kState);
     return;
   }
   const ScoreWeights sw(lg, gm.scale, false);
@@ -877,7 +919,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_rows_bf16(LaRows Q_, LaRow
 // chunk are the keys' side's (la_dkdv_role).
 template <bool DECAY>
 __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows O_, LaRows K_, LaRows V_, LaGeom gm,
-                                                              const float* __restrict__ enter, bf16* __restrict__ dq,
+                                                              LaEnter enter, bf16* __restrict__ dq,
                                                               int64_t o0, int64_t o1, int64_t o2,
                                                               float* __restrict__ local, double* __restrict__ dot) {
   constexpr int kParts = DECAY ? 3 : 2;
@@ -911,11 +953,13 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
   };
   const float* tables = reinterpret_cast<const float*>(smem + (4 + kParts) * kTileBytes);   // written before the first barrier
   state_weights_put(lg, live(chunks - 1), reinterpret_cast<float*>(smem + (4 + kParts) * kTileBytes));
-  fetch(0);
   float total = 0.f;
   if (keeps) {
-    f32x4 M[4], L[4] = {zero4(), zero4(), zero4(), zero4()};
-    state_load(enter ? enter + it.at * kState : nullptr, true, M);
+    f32x4 M[4], L[4];
+    state_enter(enter, true, gm, it, lg, M);
+    fetch(0);
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct) L[ct] = zero4();
     const float full = la_power(lg, kChunk);
     const AdjointWeights wl(lg, gm.scale);
     float past = 1.f;
@@ -934,6 +978,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
     }
     if (local && chunks) state_store(L, local + it.at * kState);
   } else {
+    fetch(0);
     const ScoreWeights sw(lg, gm.scale, false);
     const float carry = gm.scale * la_power(lg, 16 * w + c + 1), mid = 0.5f * static_cast<float>(gm.seg);
     for (int i = 0; i < chunks; ++i) {
@@ -1277,40 +1322,41 @@ LaGeom la_geom(const dwarf_linear_attention_fwd_args& a) {
   return gm;
 }
 
+// The forward's segments are joined by a launch of the scan (also where there are none: the state that enters leaves).
+bool la_scanned(const LaGeom& gm) { return gm.segs == 0 || gm.segs > kScanRun; }
+LaEnter la_enter(const dwarf_linear_attention_fwd_args& a, const LaGeom& gm) {
+  if (la_scanned(gm)) return LaEnter{a.states, nullptr, nullptr};
+  return LaEnter{nullptr, a.initial, gm.segs > 1 ? a.states : nullptr};
+}
+
 // A single row's stride is whatever the caller's view says: rows behind it must not fall on it.
 LaRows la_operand(const void* p, const int64_t* s, int N) { return LaRows{p, s[0], s[1], N > 1 ? s[2] : kHd}; }
 
 void la_fwd_bf16(const dwarf_linear_attention_fwd_args& a, const LaGeom& gm, hipStream_t stream) {
   const LaRows q = la_operand(a.q, a.q_stride, gm.N), k = la_operand(a.k, a.k_stride, gm.N), v = la_operand(a.v, a.v_stride, gm.N);
   const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * gm.segs);
-  const float* enter = a.initial;
-  if (gm.segs > 1) {
+  const bool scanned = la_scanned(gm);
+  if (gm.segs > 1)
     hipLaunchKernelGGL(la_local_bf16, grid, dim3(kLaThreads), 0, stream, k, gm.Hkv, v, gm.Hkv, gm, a.states);
-    enter = a.states;
-  }
-  if (gm.segs != 1)
-    la_scan<false>(a.states, a.initial, a.final, gm, nullptr, nullptr, nullptr, nullptr, stream);
+  if (scanned) la_scan<false>(a.states, a.initial, a.final, gm, nullptr, nullptr, nullptr, nullptr, stream);
   if (gm.segs == 0) return;
-  hipLaunchKernelGGL(la_rows_bf16, grid, dim3(kWideThreads), 0, stream, q, k, v, gm, enter, static_cast<bf16*>(a.out),
-                     a.out_stride[0], a.out_stride[1], a.out_stride[2], gm.segs == 1 ? a.final : nullptr);
+  hipLaunchKernelGGL(la_rows_bf16, grid, dim3(kWideThreads), 0, stream, q, k, v, gm, la_enter(a, gm),
+                     static_cast<bf16*>(a.out), a.out_stride[0], a.out_stride[1], a.out_stride[2], scanned ? nullptr : a.final);
 }
 
 template <typename T>
 void la_fwd_typed(const dwarf_linear_attention_fwd_args& a, const LaGeom& gm, hipStream_t stream) {
   const LaRows q = la_operand(a.q, a.q_stride, gm.N), k = la_operand(a.k, a.k_stride, gm.N), v = la_operand(a.v, a.v_stride, gm.N);
   const dim3 grid(static_cast<unsigned>(gm.B) * gm.H * gm.segs), block(kLaThreads);
-  const float* enter = a.initial;
-  if (gm.segs > 1) {
+  const bool scanned = la_scanned(gm);
+  if (gm.segs > 1)
     hipLaunchKernelGGL((la_local_kernel<T, false>), grid, block, 0, stream, k, gm.Hkv, v, gm.Hkv, gm, 1.f, a.states);
-    enter = a.states;
-  }
-  if (gm.segs != 1)
-    la_scan<false>(a.states, a.initial, a.final, gm, nullptr, nullptr, nullptr, nullptr, stream);
+  if (scanned) la_scan<false>(a.states, a.initial, a.final, gm, nullptr, nullptr, nullptr, nullptr, stream);
   if (gm.segs == 0) return;
-  const LaRowsCall<T> call{q, k, v, LaRows{}, gm.H, gm.Hkv, gm.Hkv, 1, enter, false, static_cast<T*>(a.out), a.out_stride[0],
+  const LaRowsCall<T> call{q, k, v, LaRows{}, gm.H, gm.Hkv, gm.Hkv, 1, la_enter(a, gm), false, static_cast<T*>(a.out), a.out_stride[0],
                            a.out_stride[1], a.out_stride[2], nullptr};
   hipLaunchKernelGGL((la_rows_kernel<T, T, false>), grid, block, 0, stream, call, call, gm, gm.scale, gm.scale, 1.f,
-                     gm.segs == 1 ? a.final : nullptr);
+                     scanned ? nullptr : a.final);
 }
 
 // Workspace of the backward, in floats: the adjoints per segment, the dlog_decay sums, the shared heads' parts.
@@ -1348,7 +1394,7 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
   double* edge = dlog ? reinterpret_cast<double*>(ws + sp.edge) : nullptr;
   const bool joined = gm.segs != 1 || a.dinitial || dlog;
   const float* enter = joined ? adj : a.dfinal;
-  const float* before = gm.segs > 1 ? f.states : f.initial;
+  const LaEnter before = la_enter(f, gm), behind = joined ? LaEnter{adj, nullptr, nullptr} : LaEnter{nullptr, a.dfinal, nullptr};
   const bool shared = gm.H != gm.Hkv;
   float *pk = ws + sp.dk_part, *pv = ws + sp.dv_part;
   const int64_t s1 = static_cast<int64_t>(gm.N) * kHd, s0 = s1 * gm.H;   // of the shared heads' parts
@@ -1383,14 +1429,14 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
                          nullptr);
       const dim3 both(grid.x, 2);
       if (shared) {
-        const LaRowsCall<float> cv{k, q, dout, LaRows{}, gm.Hkv, gm.H, gm.H, 1, enter, false, pv, s0, s1, kHd, nullptr};
-        const LaRowsCall<float> ck{v, dout, q, k, gm.Hkv, gm.H, gm.H, gm.Hkv, enter, true, pk, s0, s1, kHd, dk_dot};
+        const LaRowsCall<float> cv{k, q, dout, LaRows{}, gm.Hkv, gm.H, gm.H, 1, behind, false, pv, s0, s1, kHd, nullptr};
+        const LaRowsCall<float> ck{v, dout, q, k, gm.Hkv, gm.H, gm.H, gm.Hkv, behind, true, pk, s0, s1, kHd, dk_dot};
         hipLaunchKernelGGL((la_rows_kernel<T, float, true>), both, block, 0, stream, cv, ck, gm, gm.scale, 1.f, gm.scale,
                            nullptr);
       } else {
-        const LaRowsCall<T> cv{k, q, dout, LaRows{}, gm.Hkv, gm.H, gm.H, 1, enter, false, static_cast<T*>(a.dv),
+        const LaRowsCall<T> cv{k, q, dout, LaRows{}, gm.Hkv, gm.H, gm.H, 1, behind, false, static_cast<T*>(a.dv),
                                a.dv_stride[0], a.dv_stride[1], a.dv_stride[2], nullptr};
-        const LaRowsCall<T> ck{v, dout, q, k, gm.Hkv, gm.H, gm.H, gm.Hkv, enter, true, static_cast<T*>(a.dk),
+        const LaRowsCall<T> ck{v, dout, q, k, gm.Hkv, gm.H, gm.H, gm.Hkv, behind, true, static_cast<T*>(a.dk),
                                a.dk_stride[0], a.dk_stride[1], a.dk_stride[2], dk_dot};
         hipLaunchKernelGGL((la_rows_kernel<T, T, true>), both, block, 0, stream, cv, ck, gm, gm.scale, 1.f, gm.scale, nullptr);
       }
