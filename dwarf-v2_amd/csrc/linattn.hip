@@ -14,10 +14,22 @@
 // where tau is taken from the segment's middle, so that the two sums, which
 // nearly cancel, stay small.
 //
-// A sequence is cut into segments.  la_local forms each segment's own sum, the
-// scan joins them into the state in front of each segment (behind it, for G),
-// and la_rows walks a segment's chunks with the state in registers.  One
-// segment needs la_rows alone.
+// A sequence is cut into segments.  The local launch forms each segment's own
+// sum; up to eight segments the rows' launch joins the sums in front of its
+// own, above that a scan launch does; the rows' launch walks a segment's chunks
+// with the state in registers.  One segment needs the rows alone.  The backward
+// is the same in reverse: dq together with the adjoint's segment sums (they
+// read the same rows), a scan (also for the boundary terms), dk and dv, and the
+// sums of dlog_decay.
+//
+// Least traffic is one read of q, k, v and one write of o (backward: q, k, v,
+// do read, dq, dk, dv written); two passes read k and v twice.  Measured in
+// bf16: B1 N65536 H8, 268 MB at least and 403 MB here, 102 us of launches (rows
+// 57, local 38, scan 6.5: 3.9 TB/s); training at B15 N2048 H8 (346 MB at least,
+// 566 MB here), 151 us: local 23.5, rows 28.6, dq 43.4, scan 6.5, dk and dv 44.5,
+// dlog_decay 4.  The rows, dq and dk/dv are bound by a CU's issue slots as much
+// as by memory: with k and v from the L2 and nothing stored, the rows of the
+// long prompt still take 41 us.
 #include <type_traits>
 
 #include "gather.h"
@@ -448,7 +460,7 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRowsCall<TO> call
 // (weighted scores, the state, weighted keys) is split into bf16 parts before it meets the matrix cores, two parts
 // (2^-17 relative) where the result is rounded to bf16 anyway and three (2^-24, fp32 itself) where it goes into the
 // state, so that no intermediate rounding is coarser than the output's.  The sums are bound by memory, and the matrix
-// cores have the room: 64 instructions a wave and chunk at most, of which 40 are the split parts.
+// cores have the room: at most 28 instructions a wave and chunk on average, busy a third of the time.
 //
 // LDS holds tiles as 64 rows of 128 bytes; 16-byte piece p of row r sits at piece p ^ tile_key(r).  Of the 4,096 keys that
 // are linear in a row's four low bits this is one of those without bank conflicts in all five accesses: whole pieces read
@@ -1236,7 +1248,11 @@ __global__ __launch_bounds__(kLaThreads) void la_dlog_kernel(const double* __res
   if (threadIdx.x == 0) dlog[h] = gm.log_decay[h] > 0.f ? 0.f : static_cast<float>(t);
 }
 
-// One token of each row: a wave per (row, head) and column quarter... the state streams through once.
+// One token of each row, S' = g S + k v^T, o = scale q S': a workgroup for each (row, head), whose threads hold four by four
+// elements of the state, all of it in flight at once; the rows of the result are added through LDS.  The state is read and
+// written once and is all there is: bound by memory.  256 rows of H8 (67 MB): 12.9 us, 5.2 TB/s; one row 4.2 us, a launch's
+// own time.  A slot that several rows share is worked by the first one's workgroups, row after row, and the others leave:
+// each looks the slots through once, 256 at a time.
 constexpr int kStepThreads = 256;
 template <typename T>
 __global__ __launch_bounds__(kStepThreads) void la_step_kernel(dwarf_linear_attention_step_args a) {
@@ -1305,9 +1321,14 @@ __global__ __launch_bounds__(kStepThreads) void la_step_kernel(dwarf_linear_atte
   for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(a.new_state + at + (r0 + i) * kHd + c4) = st[i];
 }
 
+// Tokens of a segment: the longest whose workgroups fill the card.  Long ones (512 and 1,024 tokens) have to leave two for
+// each CU, since their rows are bound by what a CU computes: B15 N2048 H8, bf16 forward 45.5 us with 480 workgroups of 512
+// tokens, 54.8 with 240 of 1,024.  Short ones one: B4 N2048 H8 20.2 us forward and 42.3 backward with 256 of 256 tokens,
+// 24.5 and 45.5 with 512 of 128 (more sums to join).  More of them than that only adds states: B1 N65536 H8 97.7 us with
+// 512 of 1,024 tokens, 106 with 1,024 of 512.
 int la_segment(int64_t B, int64_t H, int64_t N) {
   for (int seg = 1024; seg > kChunk; seg /= 2)
-    if (B * H * ((N + seg - 1) / seg) >= 448) return seg;
+    if (B * H * ((N + seg - 1) / seg) >= (seg >= 512 ? 448 : 224)) return seg;
   return kChunk;
 }
 

@@ -26,7 +26,7 @@ from .dsqg import HEAD_DIM
 def segment_tokens(B: int, H: int, N: int) -> int:
     """Tokens of a segment (dwarf_linear_attention_segment): shorter ones where long ones leave CUs idle."""
     for seg in (1024, 512, 256, 128):
-        if B * H * -(-N // seg) >= 448:
+        if B * H * -(-N // seg) >= (448 if seg >= 512 else 224):
             return seg
     return 64
 
