@@ -156,8 +156,7 @@ NormRows norm_rows(const Tensor& x, int64_t groups) {
 
 Tensor table(const OptTensor& t) {
   if (!t) return Tensor();
-  const Tensor d = t->detach();
-  return d.scalar_type() == at::kFloat && d.is_contiguous() ? d : d.to(at::kFloat).contiguous();
+  return t->scalar_type() == at::kFloat && t->is_contiguous() ? *t : t->to(at::kFloat).contiguous();
 }
 const float* f32_ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
 float* f32_out(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
@@ -176,7 +175,7 @@ void norm_fill(dwarf_layer_norm_fwd_args& a, const NormRows& r, int64_t groups, 
 }
 
 Tensor norm_forward(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps) {
-  const NormRows r = norm_rows(x.detach(), groups);
+  const NormRows r = norm_rows(x, groups);
   const Tensor w = table(weight), b = table(bias);
   const Tensor y = at::empty(x.sizes(), x.options());
   dwarf_layer_norm_fwd_args a{};
@@ -191,7 +190,7 @@ Tensor norm_forward(const Tensor& x, const OptTensor& weight, const OptTensor& b
 
 std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& dy, const Tensor& x, const OptTensor& weight, int64_t groups,
                                                  double eps, bool need_dx, bool need_dw, bool need_db) {
-  const NormRows r = norm_rows(x.detach(), groups), g = norm_rows(dy.detach().to(x.scalar_type()), groups);
+  const NormRows r = norm_rows(x, groups), g = norm_rows(dy.to(x.scalar_type()), groups);
   const Tensor w = table(weight);
   Tensor dx, dw, db;
   dwarf_layer_norm_bwd_args a{};
@@ -281,7 +280,7 @@ Tensor pair_rows(const Tensor& x, bool interleaved) {
 
 std::tuple<Tensor, Tensor> rotate(const Tensor& q_, const OptTensor& k_, const Tensor& positions, const Tensor& turns,
                                   bool interleaved, bool inverse, double magnitude) {
-  const Tensor q = pair_rows(q_.detach(), interleaved);
+  const Tensor q = pair_rows(q_, interleaved);
   dwarf_rotary_args a{};
   a.B = size32(q.size(0));
   a.H = size32(q.size(1));
@@ -299,7 +298,7 @@ std::tuple<Tensor, Tensor> rotate(const Tensor& q_, const OptTensor& k_, const T
   put_strides(a.q_out_stride, q_out);
   Tensor k, k_out;
   if (k_) {
-    k = pair_rows(k_->detach(), interleaved);
+    k = pair_rows(*k_, interleaved);
     a.H_kv = size32(k.size(1));
     k_out = token_major(a.B, a.H_kv, a.N, a.D, k);
     a.k = k.const_data_ptr();
@@ -383,12 +382,11 @@ Tensor token_rows(const Tensor& t) {
   return kernel_rows(t);
 }
 Tensor aligned_f32(const Tensor& t) {
-  const Tensor c = t.detach().to(at::kFloat).contiguous();
+  const Tensor c = t.to(at::kFloat).contiguous();
   return aligned(c, 16) ? c : dense_copy(c);
 }
 Tensor decay_table(const Tensor& log_decay) {
-  const Tensor d = log_decay.detach();
-  return d.scalar_type() == at::kFloat && d.is_contiguous() ? d : d.to(at::kFloat).contiguous();
+  return log_decay.scalar_type() == at::kFloat && log_decay.is_contiguous() ? log_decay : log_decay.to(at::kFloat).contiguous();
 }
 // 64-bit values beyond 32 bits stay what they mean, below every slot and length or above them all.
 Tensor index_table(const OptTensor& t) {
@@ -403,7 +401,7 @@ struct Operands {
   Tensor q, k, v, decay, initial, lengths;
   Operands(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& log_decay, const OptTensor& initial_,
            const OptTensor& lengths_)
-      : q(token_rows(q_.detach())), k(token_rows(k_.detach())), v(token_rows(v_.detach())), decay(decay_table(log_decay)),
+      : q(token_rows(q_)), k(token_rows(k_)), v(token_rows(v_)), decay(decay_table(log_decay)),
         initial(initial_ ? aligned_f32(*initial_) : Tensor()), lengths(index_table(lengths_)) {}
   void fill(dwarf_linear_attention_fwd_args& a, double scale) const {
     a.B = size32(q.size(0));
@@ -425,10 +423,11 @@ struct Operands {
   }
 };
 
-// (out, the final state or undefined, the segments' states)
+// (out, the final state or undefined, the segments' states: undefined where there are none, unless `shaped`)
 std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor& q, const Tensor& k, const Tensor& v,
                                                      const Tensor& log_decay, const OptTensor& initial,
-                                                     const OptTensor& lengths, double scale, bool want_state) {
+                                                     const OptTensor& lengths, double scale, bool want_state,
+                                                     bool shaped) {
   const Operands in(q, k, v, log_decay, initial, lengths);
   dwarf_linear_attention_fwd_args a{};
   in.fill(a, scale);
@@ -436,11 +435,12 @@ std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor& q, const Tens
   const Tensor state = want_state ? empty_f32({a.B, a.H, kHd, kHd}, q) : Tensor();
   a.states_bytes = dwarf_linear_attention_states_bytes(&a);
   const int64_t per = static_cast<int64_t>(a.B) * a.H * kHd * kHd;
-  const Tensor states = empty_f32({a.B, a.H, per ? static_cast<int64_t>(a.states_bytes / sizeof(float)) / per : 0, kHd, kHd}, q);
+  const int64_t segs = per ? static_cast<int64_t>(a.states_bytes / sizeof(float)) / per : 0;
+  const Tensor states = segs || shaped ? empty_f32({a.B, a.H, segs, kHd, kHd}, q) : Tensor();
   a.out = out.data_ptr();
   put_strides(a.out_stride, out);
   a.final = f32_out(state);
-  a.states = states.data_ptr<float>();
+  a.states = f32_out(states);
   launch(dwarf_linear_attention_fwd, a, q, "dwarf_linear_attention_fwd");
   return {out, state, states};
 }
@@ -451,13 +451,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(
     const Tensor& log_decay, const OptTensor& initial, const OptTensor& lengths, double scale, const Tensor& states,
     const OptTensor& state, bool need_decay, bool need_initial) {
   const Operands in(q, k, v, log_decay, initial, lengths);
-  const Tensor dout = token_rows(dout_.detach().to(q.scalar_type()));
+  const Tensor dout = token_rows(dout_.to(q.scalar_type()));
   const Tensor dstate = dstate_ ? aligned_f32(*dstate_) : Tensor();
   dwarf_linear_attention_bwd_args a{};
   in.fill(a.fwd, scale);
   const int64_t B = a.fwd.B, H = a.fwd.H, Hkv = a.fwd.H_kv, N = a.fwd.N;
-  a.fwd.states = const_cast<float*>(states.const_data_ptr<float>());
-  a.fwd.states_bytes = static_cast<size_t>(states.numel()) * sizeof(float);
+  a.fwd.states = const_cast<float*>(f32_ptr(states));
+  a.fwd.states_bytes = states.defined() ? static_cast<size_t>(states.numel()) * sizeof(float) : 0;
   a.fwd.final = state ? const_cast<float*>(state->const_data_ptr<float>()) : nullptr;
   a.dout = dout.const_data_ptr();
   put_strides(a.dout_stride, dout);
@@ -486,7 +486,7 @@ struct LinearAttentionFn : torch::autograd::Function<LinearAttentionFn> {
                                bool want_state) {
     at::AutoDispatchBelowADInplaceOrView below;
     ctx->set_materialize_grads(false);
-    auto [out, state, states] = attention_forward(q, k, v, log_decay, initial, lengths, scale, want_state);
+    auto [out, state, states] = attention_forward(q, k, v, log_decay, initial, lengths, scale, want_state, false);
     // the final state serves the decay's gradient
     const Tensor kept = want_state && log_decay.requires_grad() ? state : Tensor();
     ctx->save_for_backward({q, k, v, log_decay, initial.value_or(Tensor()), lengths.value_or(Tensor()), states, kept});
@@ -565,7 +565,7 @@ py::object linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, c
       if (return_state) state = r[1];
     } else {
       Tensor states;
-      std::tie(out, state, states) = attention_forward(q, k, v, log_decay, initial, lengths, scale, return_state);
+      std::tie(out, state, states) = attention_forward(q, k, v, log_decay, initial, lengths, scale, return_state, false);
     }
   }
   return return_state ? py::object(py::make_tuple(out, state)) : py::cast(out);
@@ -592,7 +592,7 @@ void check_pools(const Tensor& state, const OptTensor& new_state, int64_t H) {
 Tensor attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& log_decay, const Tensor& state,
                       const OptTensor& new_state, const OptTensor& slots_, double scale, const OptTensor& out_) {
   check_pools(state, new_state, q_.size(1));
-  const Tensor q = kernel_rows(q_.detach()), k = kernel_rows(k_.detach()), v = kernel_rows(v_.detach());
+  const Tensor q = kernel_rows(q_), k = kernel_rows(k_), v = kernel_rows(v_);
   const Tensor decay = decay_table(log_decay), slots = index_table(slots_);
   const Tensor out = out_ ? *out_ : at::empty(q.sizes(), q.options());
   dwarf_linear_attention_step_args a{};
@@ -689,7 +689,10 @@ PYBIND11_MODULE(_mixer, m) {
   m.def("rotary_embed", &rotary_embed, no_gil);
   m.def("rotate", &rotate, no_gil);
   m.def("linear_attention", &linear_attention);
-  m.def("attention_forward", &attention_forward, no_gil);
+  m.def("attention_forward", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
+                                const OptTensor& initial, const OptTensor& lengths, double scale, bool want_state) {
+    return attention_forward(q, k, v, log_decay, initial, lengths, scale, want_state, true);
+  }, no_gil);
   m.def("attention_backward", &attention_backward, no_gil);
   m.def("linear_attention_step", &linear_attention_step, no_gil);
   m.def("attention_step", &attention_step, no_gil);
