@@ -8,8 +8,8 @@
 // (mean, then the variance of the centred values, then the result), and the
 // backward forms the statistics again from the row it reads anyway instead of
 // reading saved ones.  TPR adjacent threads share a row, K vectors each; rows
-// too long for the registers take the streaming kernels, one workgroup per
-// row, whose second and third pass read the caches.
+// too long for the registers (16,384 elements of 16 bits) take the streaming
+// kernels, one workgroup per row, whose second and third pass read the caches.
 //
 // The grid's stride over the rows is a multiple of the groups, so a thread
 // keeps one group: its weights and its part of dw and db stay in registers
@@ -108,13 +108,14 @@ __device__ __forceinline__ void norm_table(const float* t, uint32_t group, int s
   }
 }
 
+constexpr int norm_fwd_threads(int tpr) { return tpr > kNormThreads ? tpr : kNormThreads; }
+
 template <typename T, int VEC, int TPR, int K>
-__global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const T* __restrict__ x, int64_t xs0, int64_t xs1,
-                                                                const float* __restrict__ weight,
-                                                                const float* __restrict__ bias, T* __restrict__ y,
-                                                                int64_t ys0, int64_t ys1, NormGeom gm) {
-  constexpr int kRows = kNormThreads / TPR;
-  __shared__ float s_red[kNormThreads / kWave];
+__global__ __launch_bounds__(norm_fwd_threads(TPR)) void norm_fwd_kernel(
+    const T* __restrict__ x, int64_t xs0, int64_t xs1, const float* __restrict__ weight, const float* __restrict__ bias,
+    T* __restrict__ y, int64_t ys0, int64_t ys1, NormGeom gm) {
+  constexpr int kThreads = norm_fwd_threads(TPR), kRows = kThreads / TPR;
+  __shared__ float s_red[kThreads / kWave];
   const int sub = threadIdx.x % TPR;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;   // a multiple of the groups
   const NormWalk walk(kRows, threadIdx.x / TPR, gm.groups);
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const T* __restr
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < K * VEC; ++i) s += v[i];
-    const float mu = row_sum<TPR, kNormThreads>(s, s_red) / fd;
+    const float mu = row_sum<TPR, kThreads>(s, s_red) / fd;
     float q = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const T* __restr
         q = fmaf(v[k * VEC + e], v[k * VEC + e], q);
       }
     }
-    const float rs = 1.f / sqrtf(row_sum<TPR, kNormThreads>(q, s_red) / fd + gm.eps);
+    const float rs = 1.f / sqrtf(row_sum<TPR, kThreads>(q, s_red) / fd + gm.eps);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int d = (k * TPR + sub) * VEC;
@@ -434,6 +435,10 @@ int64_t norm_blocks(int64_t rows, int groups, int block_rows, int most) {
   return (want + unit - 1) / unit * unit;
 }
 
+// A row goes to as many threads as take one vector each, up to the wave, then to a wave with up to four each, then to the
+// workgroup: its sums need barriers, which a row of a wave does not (33.5 MB in bf16, forward and backward with the sums:
+// 16,384 rows of 1,024 by waves 12.2 and 25.6 us, by workgroups 18.6 and 70; 8,192 of 2,048 13.2 and 28.5 against 12.9 and
+// 42).  Longer rows are read three times: 1,024 of 16,384 19.6 us forward in the registers of 512 threads, 66 streamed.
 NormPlan norm_plan(const dwarf_layer_norm_fwd_args& f, bool vec, int threads) {
   NormPlan p;
   const int per = f.dtype == DWARF_F32 ? 4 : 8;
@@ -447,22 +452,27 @@ NormPlan norm_plan(const dwarf_layer_norm_fwd_args& f, bool vec, int threads) {
   else if (units <= 128) p.tpr = 64, p.k = 2;
   else if (units <= 256) p.tpr = 64, p.k = 4;
   else if (units <= 4 * threads) p.tpr = threads, p.k = units <= threads ? 1 : units <= 2 * threads ? 2 : 4;
+  else if (units <= 4 * kNormBwdThreads) p.tpr = kNormBwdThreads, p.k = 4;   // forward: a larger workgroup
   else p.tpr = 0;
-  p.block_rows = p.tpr ? threads / p.tpr : 1;
+  p.block_rows = p.tpr && p.tpr < threads ? threads / p.tpr : 1;
   const int64_t rows = f.rows * f.groups;
   p.blocks = static_cast<int>(norm_blocks(rows, f.groups, p.block_rows, kNormBlocks));
   p.columns_y = 0;
   return p;
 }
 
-// The backward's grid: two workgroups per CU, which leave at most 512 partial rows per group to the sum.
+// The backward's grid: up to two workgroups per CU, which leave at most 512 partial rows per group to the sum.
 NormPlan norm_bwd_plan(const dwarf_layer_norm_bwd_args& a) {
   const int es = a.fwd.dtype == DWARF_F32 ? 4 : 2;
   bool vec = norm_vec_ok(a.fwd.x, a.fwd.x_stride, es) && norm_vec_ok(a.dy, a.dy_stride, es);
   if (a.dx) vec = vec && norm_vec_ok(a.dx, a.dx_stride, es);
   NormPlan p = norm_plan(a.fwd, vec, kNormBwdThreads);
   const int64_t rows = a.fwd.rows * a.fwd.groups;
-  p.blocks = static_cast<int>(norm_blocks(rows, a.fwd.groups, p.block_rows, kNormBwdBlocks));
+  // Threads with several vectors of a row have enough loads in flight with one workgroup on their CU, and each workgroup
+  // leaves a partial row.  33.5 MB in bf16, with 256 and with 512 workgroups: rows of 1,024 25.6 and 30.7 us, of 2,048 28.5
+  // and 38.4, of 8,192 39.6 and 52.8; with one vector to a thread, rows of 4,096 37.0 and 35.2.
+  const int most = p.k >= 2 ? kNormBwdBlocks / 2 : kNormBwdBlocks;
+  p.blocks = static_cast<int>(norm_blocks(rows, a.fwd.groups, p.block_rows, most));
   if (!p.tpr) {
     p.blocks = static_cast<int>(rows < 2048 ? rows : 2048);
     p.columns_y = static_cast<int>(a.fwd.rows < 64 ? a.fwd.rows : 64);
@@ -490,9 +500,10 @@ void norm_fwd_typed(const dwarf_layer_norm_fwd_args& f, const NormPlan& p, const
                        f.x_stride[0], f.x_stride[1], f.weight, f.bias, y, f.y_stride[0], f.y_stride[1], gm);
     return;
   }
-#define DWARF_NORM_LAUNCH(TPR, K)                                                                                \
-  hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, TPR, K>), dim3(p.blocks), dim3(kThr), 0, stream, x, f.x_stride[0], \
-                     f.x_stride[1], f.weight, f.bias, y, f.y_stride[0], f.y_stride[1], gm)
+#define DWARF_NORM_LAUNCH(TPR, K)                                                                               \
+  hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, TPR, K>), dim3(p.blocks), dim3(norm_fwd_threads(TPR)), 0, stream, \
+                     x, f.x_stride[0], f.x_stride[1], f.weight, f.bias, y, f.y_stride[0], f.y_stride[1], gm)
+  if (p.tpr == kNormBwdThreads) { DWARF_NORM_LAUNCH(kNormBwdThreads, 4); return; }
   DWARF_NORM_SHAPES(DWARF_NORM_LAUNCH)
 #undef DWARF_NORM_LAUNCH
 }
