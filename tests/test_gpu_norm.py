@@ -65,6 +65,13 @@ def check(pkg, device, x, w, b, dy, eps=1e-5, place=lambda t: t):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("D", [2051, 8184, 16384, 16392, 20001])
+def test_longest_rows(pkg, device, dtype, D):
+    """The last widths that registers hold, with and without vectors, and rows that are streamed."""
+    check(pkg, device, *make((3, 5, D), dtype, seed=D))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("D", [1, 2, 7, 8, 63, 64, 65, 100, 256, 512, 513, 1024, 1031, 1536, 2056, 4096, 8200])
 def test_widths(pkg, device, dtype, D):
     check(pkg, device, *make((5, 7, D), dtype, seed=D))
