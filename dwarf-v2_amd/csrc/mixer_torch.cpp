@@ -642,7 +642,8 @@ Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, 
                       ",", H, ",64] ", q.scalar_type(), " with 16-byte aligned rows");
   if (out)
     for (const auto& [name, t] : {std::make_pair("out", &*out), std::make_pair("q", &q), std::make_pair("k", &k),
-                                  std::make_pair("v", &v), std::make_pair("state", &state)}) {
+                                  std::make_pair("v", &v), std::make_pair("state", &state),
+                                  std::make_pair("new_state", new_state ? &*new_state : &state)}) {
       const bool shared = t == &*out ? at::has_internal_overlap(*t) == at::MemOverlap::Yes
                                      : at::get_overlap_status(*out, *t) != at::MemOverlapStatus::No &&
                                            at::get_overlap_status(*out, *t) != at::MemOverlapStatus::TooHard;

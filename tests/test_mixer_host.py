@@ -208,6 +208,9 @@ def test_step_refuses_out_in_its_inputs_memory(pkg):
         out = out if out.shape == q.shape else out.reshape(-1)[:768].view(3, 4, 64)
         with pytest.raises(ValueError, match="memory|aligned"):
             pkg.linear_attention_step(q, k, v, torch.zeros(4), pool, out=out)
+    other = torch.zeros(3, 4, 64, 64)
+    with pytest.raises(ValueError, match="new_state"):
+        pkg.linear_attention_step(q, k, v, torch.zeros(4), pool, new_state=other, out=other.reshape(-1)[:768].view(3, 4, 64))
 
 
 def test_segment_rule_is_the_librarys(pkg, lib):
