@@ -104,14 +104,33 @@ __device__ __forceinline__ void la_load16(const T* row, bool live, float* x) {
   }
 }
 
-// A 64-row tile into LDS rows of STRIDE floats.
-template <typename T, int STRIDE>
-__device__ __forceinline__ void la_tile(const T* base, int64_t stride, int n, float* s) {
-  const int r = threadIdx.x / 4, c = 16 * (threadIdx.x % 4);
-  float x[16];
-  la_load16<T>(base + r * stride + c, r < n, x);
+// The same on its way: as it is in memory until it is needed, so that a chunk's loads are under way while the one in front
+// of it is worked on.
+template <typename T>
+struct LaRaw16 {
+  static constexpr int kPer = 16 / sizeof(T);
+  Vec<T, kPer> v[16 / kPer];
+  __device__ __forceinline__ void load(const T* row, bool live) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s[r * STRIDE + c + i] = x[i];
+    for (int i = 0; i < 16 / kPer; ++i) v[i] = live ? *reinterpret_cast<const Vec<T, kPer>*>(row + i * kPer) : Vec<T, kPer>{};
+  }
+  __device__ __forceinline__ void widen(float* x) const {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = to_f32(v[i / kPer].e[i % kPer]);
+  }
+};
+// A thread's part of a 64-row tile, row tid / 4 from column 16 (tid % 4), and the tile into LDS rows of STRIDE floats.
+template <typename T>
+__device__ __forceinline__ void la_tile_fetch(LaRaw16<T>& x, const T* base, int64_t stride, int n) {
+  const int r = threadIdx.x / 4;
+  x.load(base + r * stride + 16 * (threadIdx.x % 4), r < n);
+}
+template <typename T, int STRIDE>
+__device__ __forceinline__ void la_tile_put(const LaRaw16<T>& t, float* s) {
+  float x[16];
+  t.widen(x);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[threadIdx.x / 4 * STRIDE + 16 * (threadIdx.x % 4) + i] = x[i];
 }
 
 // The chunk's weights in the state's sum, in LDS: forward g^{n-1-j}, reverse g^{j+1}.
@@ -156,14 +175,23 @@ __global__ __launch_bounds__(kLaThreads) void la_local_kernel(LaRows B_, int bh,
   const T* pc = static_cast<const T*>(C_.p) + b * C_.s0 + (h / (gm.H / ch)) * C_.s1;
   f32x4 acc[4] = {zero4(), zero4(), zero4(), zero4()};
   const int chunks = (t1 - t0 + kChunk - 1) / kChunk;
+  LaRaw16<T> xb, xc;
+  auto token = [&](int i) { return t0 + (REV ? chunks - 1 - i : i) * kChunk; };
+  auto live = [&](int i) { return i < chunks ? (t1 - token(i) < kChunk ? t1 - token(i) : kChunk) : 0; };
+  auto fetch = [&](int i) {   // behind the last chunk: reads nothing
+    const int64_t t = i < chunks ? token(i) : t0;
+    la_tile_fetch(xb, pb + t * B_.s2, B_.s2, live(i));
+    la_tile_fetch(xc, pc + t * C_.s2, C_.s2, live(i));
+  };
+  fetch(0);
   for (int i = 0; i < chunks; ++i) {
-    const int t = t0 + (REV ? chunks - 1 - i : i) * kChunk;
-    const int n = t1 - t < kChunk ? t1 - t : kChunk;
+    const int n = live(i);
     __syncthreads();
-    la_tile<T, kColStride>(pb + t * B_.s2, B_.s2, n, sB);
-    la_tile<T, kColStride>(pc + t * C_.s2, C_.s2, n, sC);
+    la_tile_put<T, kColStride>(xb, sB);
+    la_tile_put<T, kColStride>(xc, sC);
     la_weights<REV>(lg, n, s_w);
     __syncthreads();
+    fetch(i + 1);
     la_update<kColStride>(sB, sC, s_w, la_power(lg, n), us, acc);
   }
   const int l = threadIdx.x % kWave, w = threadIdx.x / kWave;
@@ -326,7 +354,7 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRowsCall<TO> call
   const LaRows A_ = call.A, B_ = call.B, C_ = call.C, D_ = call.D;
   const int64_t o2 = call.o2;
   const int seg = blockIdx.x % gm.segs, h = blockIdx.x / gm.segs % gm.H, b = blockIdx.x / gm.segs / gm.H;
-  const int l = threadIdx.x % kWave, w = threadIdx.x / kWave, g = l / 16, c = l % 16;
+  const int l = threadIdx.x % kWave, w = uniform(threadIdx.x / kWave), g = l / 16, c = l % 16;
   const int len = la_length(gm, b), t0 = seg * gm.seg;
   const int tend = t0 + gm.seg < gm.N ? t0 + gm.seg : gm.N;
   const int t1 = tend < len ? tend : len;
@@ -361,33 +389,46 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRowsCall<TO> call
   const float mid = 0.5f * static_cast<float>(gm.seg);
   double total = 0.;
   const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
+  LaRaw16<T> xa, xb, xc;
+  auto token = [&](int i) { return t0 + (REV ? chunks - 1 - i : i) * kChunk; };
+  auto live = [&](int i) { return i < chunks ? (t1 - token(i) < kChunk ? t1 - token(i) : kChunk) : 0; };
+  auto fetch = [&](int i) {   // behind the last chunk: reads nothing
+    const int64_t t = i < chunks ? token(i) : t0;
+    const int n = live(i);
+    la_tile_fetch(xb, pb + t * B_.s2, B_.s2, n);
+    la_tile_fetch(xc, pc + t * C_.s2, C_.s2, n);
+    // row 16w + c of A, elements [16g, 16g + 16): the k index of step kk is 16g + kk in both operands
+    xa.load(pa + (t + 16 * w + c) * A_.s2 + 16 * g, 16 * w + c < n);
+  };
+  fetch(0);
   for (int i = 0; i < chunks; ++i) {
-    const int t = t0 + (REV ? chunks - 1 - i : i) * kChunk;
-    const int n = t1 - t < kChunk ? t1 - t : kChunk;
+    const int t = token(i), n = live(i);
     __syncthreads();
-    la_tile<T, kRowStride>(pb + t * B_.s2, B_.s2, n, sB);
-    la_tile<T, kColStride>(pc + t * C_.s2, C_.s2, n, sC);
+    la_tile_put<T, kRowStride>(xb, sB);
+    la_tile_put<T, kColStride>(xc, sC);
     la_weights<REV>(lg, n, s_w);
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
       for (int r = 0; r < 4; ++r) sM[(16 * w + 4 * g + r) * kColStride + 16 * ct + c] = M[ct][r];
-    // row 16w + c of A, elements [16g, 16g + 16): the k index of step kk is 16g + kk in both operands
     float a[16];
-    la_load16<T>(pa + (t + 16 * w + c) * A_.s2 + 16 * g, 16 * w + c < n, a);
+    xa.widen(a);
     __syncthreads();
+    fetch(i + 1);
     f32x4 p[4];
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct) {
       p[ct] = zero4();
       const float* row = sB + (16 * ct + c) * kRowStride + 16 * g;
+      if (REV ? ct >= w : ct <= w) {   // uniform: the others lie on the wrong side of the wave's rows
 #pragma unroll
-      for (int k4 = 0; k4 < 4; ++k4) {
-        const float4 x = *reinterpret_cast<const float4*>(row + 4 * k4);
-        p[ct] = mfma16_f32(a[4 * k4], x.x, p[ct]);
-        p[ct] = mfma16_f32(a[4 * k4 + 1], x.y, p[ct]);
-        p[ct] = mfma16_f32(a[4 * k4 + 2], x.z, p[ct]);
-        p[ct] = mfma16_f32(a[4 * k4 + 3], x.w, p[ct]);
+        for (int k4 = 0; k4 < 4; ++k4) {
+          const float4 x = *reinterpret_cast<const float4*>(row + 4 * k4);
+          p[ct] = mfma16_f32(a[4 * k4], x.x, p[ct]);
+          p[ct] = mfma16_f32(a[4 * k4 + 1], x.y, p[ct]);
+          p[ct] = mfma16_f32(a[4 * k4 + 2], x.z, p[ct]);
+          p[ct] = mfma16_f32(a[4 * k4 + 3], x.w, p[ct]);
+        }
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -402,6 +443,7 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRowsCall<TO> call
       float pairs = 0.f;
 #pragma unroll
       for (int ct = 0; ct < 4; ++ct) {
+        if (ct < w) continue;
         f32x4 y = zero4();
 #pragma unroll
         for (int kk = 0; kk < 16; ++kk) y = mfma16_f32(d[kk], sC[(16 * ct + c) * kColStride + 16 * g + kk], y);
