@@ -340,7 +340,10 @@ struct LaRowsCall {
 };
 
 // out_i = intra sum_j W_ij (A_i.B_j) C_j + cs W_i A_i M over a segment's chunks, M updated behind each (in front, in
-// reverse); in fp32 throughout, for fp32 and fp16 rows.  leave: where the state behind the last token goes (NULL: nowhere, or the
+// reverse); in fp32 throughout, for fp32 and fp16 rows (fp16 parts of a state would overflow,
+// and bf16 parts of fp16 rows would double the tiles and the products; B15 N2048 H8 in fp16: forward 124 us, backward 351).
+// Bound by the fp32 matrix rate, of which it reaches half: 232 instructions of 32 cycles a wave and chunk, 46 of 92 us.
+//  leave: where the state behind the last token goes (NULL: nowhere, or the
 // scan has written it).
 // dot, forward: sum tau D_i.(out_i's part that comes from M); in reverse the same less (i - j) times each pair's share
 // within a chunk, W_ij (A_i.B_j) (D_i.C_j).  blockIdx.y picks the call (dv and dk go in one launch).
