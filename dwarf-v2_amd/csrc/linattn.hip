@@ -340,11 +340,10 @@ struct LaRowsCall {
 };
 
 // out_i = intra sum_j W_ij (A_i.B_j) C_j + cs W_i A_i M over a segment's chunks, M updated behind each (in front, in
-// reverse); in fp32 throughout, for fp32 and fp16 rows (fp16 parts of a state would overflow,
-// and bf16 parts of fp16 rows would double the tiles and the products; B15 N2048 H8 in fp16: forward 124 us, backward 351).
-// Bound by the fp32 matrix rate, of which it reaches half: 232 instructions of 32 cycles a wave and chunk, 46 of 92 us.
-//  leave: where the state behind the last token goes (NULL: nowhere, or the
-// scan has written it).
+// reverse); in fp32 throughout, for fp32 and fp16 rows (fp16 parts of a state would overflow, and bf16 parts of fp16 rows
+// would double the tiles and the products; B15 N2048 H8 in fp16: forward 124 us, backward 351).  Bound by the fp32 matrix
+// rate, of which it reaches half: 232 instructions of 32 cycles a wave and chunk, 46 of 92 us.
+// leave: where the state behind the last token goes (NULL: nowhere, or the scan has written it).
 // dot, forward: sum tau D_i.(out_i's part that comes from M); in reverse the same less (i - j) times each pair's share
 // within a chunk, W_ij (A_i.B_j) (D_i.C_j).  blockIdx.y picks the call (dv and dk go in one launch).
 template <typename T, typename TO, bool REV>
@@ -1295,7 +1294,7 @@ __global__ __launch_bounds__(kLaThreads) void la_dlog_kernel(const double* __res
 
 // One token of each row, S' = g S + k v^T, o = scale q S': a workgroup for each (row, head), whose threads hold four by four
 // elements of the state, all of it in flight at once; the rows of the result are added through LDS.  The state is read and
-// written once and is all there is: bound by memory.  256 rows of H8 (67 MB): 12.9 us, 5.2 TB/s; one row 4.2 us, a launch's
+// written once and is all there is: bound by memory.  256 rows of H8 (67 MB): 12.6 us, 5.3 TB/s; one row 3.9 us, a launch's
 // own time.  A slot that several rows share is worked by the first one's workgroups, row after row, and the others leave:
 // each looks the slots through once, 256 at a time.
 constexpr int kStepThreads = 256;
@@ -1327,19 +1326,20 @@ __global__ __launch_bounds__(kStepThreads) void la_step_kernel(dwarf_linear_atte
     __syncthreads();
     return s_next;
   };
-  if (a.slots && next_of(0) < row0) return;   // uniform
   const int64_t at = slot * a.slot_stride + static_cast<int64_t>(h) * kState;
-  float4 st[4];
+  float4 st[4];   // under way while the slots are looked through
 #pragma unroll
   for (int i = 0; i < 4; ++i) st[i] = *reinterpret_cast<const float4*>(a.state + at + (r0 + i) * kHd + c4);
-  for (int row = row0; row < a.S; row = a.slots ? next_of(row + 1) : a.S) {
-    const T* q = static_cast<const T*>(a.q) + row * a.q_stride[0] + h * a.q_stride[1];
-    const T* k = static_cast<const T*>(a.k) + row * a.k_stride[0] + kv * a.k_stride[1];
-    const T* v = static_cast<const T*>(a.v) + row * a.v_stride[0] + kv * a.v_stride[1];
-    float qv[4], kx[4], vx[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-    load_vec<T, 4>(q + r0, qv);
-    load_vec<T, 4>(k + r0, kx);
-    load_vec<T, 4>(v + c4, vx);
+  float qv[4], kx[4], vx[4];
+  auto fetch = [&](int row) {
+    load_vec<T, 4>(static_cast<const T*>(a.q) + row * a.q_stride[0] + h * a.q_stride[1] + r0, qv);
+    load_vec<T, 4>(static_cast<const T*>(a.k) + row * a.k_stride[0] + kv * a.k_stride[1] + r0, kx);
+    load_vec<T, 4>(static_cast<const T*>(a.v) + row * a.v_stride[0] + kv * a.v_stride[1] + c4, vx);
+  };
+  fetch(row0);
+  if (row0 > 0 && a.slots && next_of(0) < row0) return;   // uniform
+  for (int row = row0; row < a.S;) {
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       st[i].x = fmaf(decay, st[i].x, kx[i] * vx[0]);
@@ -1361,6 +1361,8 @@ __global__ __launch_bounds__(kStepThreads) void la_step_kernel(dwarf_linear_atte
       for (int i = 0; i < kStepThreads / 16; ++i) t += s_o[i][threadIdx.x];
       static_cast<T*>(a.out)[row * a.out_stride[0] + h * a.out_stride[1] + threadIdx.x] = from_f32<T>(a.scale * t);
     }
+    row = a.slots && row + 1 < a.S ? next_of(row + 1) : a.S;
+    if (row < a.S) fetch(row);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(a.new_state + at + (r0 + i) * kHd + c4) = st[i];
