@@ -175,6 +175,22 @@ void norm_fill(dwarf_layer_norm_fwd_args& a, const NormRows& r, int64_t groups, 
   a.weight = f32_ptr(w);
 }
 
+// What the launches take for granted, for callers that come without layer_norm's own checks (the custom ops).
+void check_norm_launch(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must have a last dimension to normalise, got ", x.sizes());
+  TORCH_CHECK_VALUE(groups == 1 || (groups > 1 && x.dim() >= 2 && x.size(-2) == groups), "groups=", groups, " does not fit x ",
+                    x.sizes());
+  for (const auto& [name, t] : {std::make_pair("weight", &weight), std::make_pair("bias", &bias)}) {
+    if (!*t) continue;
+    TORCH_CHECK_VALUE((*t)->is_floating_point() && (*t)->numel() == groups * x.size(-1), name, " must hold ", groups, " x ",
+                      x.size(-1), " floating values, got ", (*t)->sizes(), " ", (*t)->scalar_type());
+  }
+  dtype_of(x, "x");
+  check_cuda(x);
+  check_beside("weight", weight, x);
+  check_beside("bias", bias, x);
+}
+
 Tensor norm_forward(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps) {
   const NormRows r = norm_rows(x, groups);
   const Tensor w = table(weight), b = table(bias);
@@ -350,8 +366,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
   }
 };
 
-std::tuple<Tensor, OptTensor> rotary_embed(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns,
-                                           bool interleaved, double magnitude) {
+void check_rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns) {
   TORCH_CHECK_VALUE(q.dim() == 4, "q must be [B,H,N,D], got ", q.sizes());
   const int64_t B = q.size(0), N = q.size(2), D = q.size(3);
   if (k)
@@ -363,11 +378,18 @@ std::tuple<Tensor, OptTensor> rotary_embed(const Tensor& q, const OptTensor& k, 
   TORCH_CHECK_VALUE((positions.dim() == 1 && positions.size(0) == N) ||
                         (positions.dim() == 2 && positions.size(0) == B && positions.size(1) == N),
                     "positions must be [", N, "] or [", B, ",", N, "], got ", positions.sizes());
+  TORCH_CHECK_VALUE(turns.scalar_type() == at::kLong && turns.is_contiguous(), "the plan's turns must be contiguous int64, got ",
+                    turns.scalar_type(), " strides ", turns.strides());
   dtype_of(q, "q");
   check_cuda(q);
   check_beside("k", k, q);
   check_beside("positions", positions, q);
   check_beside("plan", turns, q);
+}
+
+std::tuple<Tensor, OptTensor> rotary_embed(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns,
+                                           bool interleaved, double magnitude) {
+  check_rotary(q, k, positions, turns);
   if (at::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()))) {
     const variable_list r = RotaryFn::apply(q, k, positions, turns, interleaved, magnitude);
     return {r[0], k ? OptTensor(r[1]) : std::nullopt};
@@ -535,17 +557,21 @@ void check_heads(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   dtype_of(q, "q");
 }
 
-py::object linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
-                            const std::optional<double>& scale_, const OptTensor& initial, const OptTensor& lengths,
-                            bool return_state) {
-  const double scale = scale_or_default(scale_);
+void check_state(const char* name, const OptTensor& t, const Tensor& q) {
+  if (!t) return;
+  TORCH_CHECK_VALUE(q.dim() == 4, "q must be [B,H,N,64], got ", q.sizes());
+  const int64_t B = q.size(0), H = q.size(1), hd = q.size(3);
+  TORCH_CHECK_VALUE(t->sizes() == at::IntArrayRef({B, H, hd, hd}) && t->scalar_type() == at::kFloat, name, " must be fp32 [", B,
+                    ",", H, ",", hd, ",", hd, "], got ", t->sizes(), " ", t->scalar_type());
+}
+
+void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const OptTensor& initial,
+                     const OptTensor& lengths) {
   TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q, k and v must be [B,H,N,64], got ", q.sizes(), ", ",
                     k.sizes(), ", ", v.sizes());
   check_heads(q, k, v, log_decay, "[B,H,N,64]");
-  const int64_t B = q.size(0), H = q.size(1), hd = q.size(3);
-  if (initial)
-    TORCH_CHECK_VALUE(initial->sizes() == at::IntArrayRef({B, H, hd, hd}) && initial->scalar_type() == at::kFloat,
-                      "initial_state must be fp32 [", B, ",", H, ",", hd, ",", hd, "], got ", initial->sizes(), " ", initial->scalar_type());
+  const int64_t B = q.size(0), hd = q.size(3);
+  check_state("initial_state", initial, q);
   if (lengths)
     TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == B && is_index(*lengths), "lengths must be [", B,
                       "] int32 or int64, got ", lengths->sizes(), " ", lengths->scalar_type());
@@ -556,6 +582,13 @@ py::object linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, c
   check_beside("initial_state", initial, q);
   check_beside("lengths", lengths, q);
   TORCH_CHECK(hd == kHd, "linear attention is built for head_dim 64, got ", hd);
+}
+
+py::object linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
+                            const std::optional<double>& scale_, const OptTensor& initial, const OptTensor& lengths,
+                            bool return_state) {
+  const double scale = scale_or_default(scale_);
+  check_attention(q, k, v, log_decay, initial, lengths);
   Tensor out, state;
   {
     const py::gil_scoped_release release;
@@ -592,7 +625,6 @@ void check_pools(const Tensor& state, const OptTensor& new_state, int64_t H) {
 
 Tensor attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& log_decay, const Tensor& state,
                       const OptTensor& new_state, const OptTensor& slots_, double scale, const OptTensor& out_) {
-  check_pools(state, new_state, q_.size(1));
   const Tensor q = kernel_rows(q_), k = kernel_rows(k_), v = kernel_rows(v_);
   const Tensor decay = decay_table(log_decay), slots = index_table(slots_);
   const Tensor out = out_ ? *out_ : at::empty(q.sizes(), q.options());
@@ -624,10 +656,8 @@ Tensor attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, cons
   return out;
 }
 
-Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
-                             const OptTensor& slots, const OptTensor& new_state, const std::optional<double>& scale_,
-                             const OptTensor& out) {
-  const double scale = scale_or_default(scale_);
+void check_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
+                const OptTensor& slots, const OptTensor& new_state, const OptTensor& out) {
   TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "q, k and v must be [S,H,64], got ", q.sizes(), ", ",
                     k.sizes(), ", ", v.sizes());
   check_heads(q, k, v, log_decay, "[S,H,64]");
@@ -658,11 +688,18 @@ Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, 
   check_beside("slots", slots, q);
   check_beside("new_state", new_state, q);
   check_beside("out", out, q);
+  TORCH_CHECK_VALUE(!S || state.size(0), "the pool is empty");
+}
+
+Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
+                             const OptTensor& slots, const OptTensor& new_state, const std::optional<double>& scale_,
+                             const OptTensor& out) {
+  const double scale = scale_or_default(scale_);
+  check_step(q, k, v, log_decay, state, slots, new_state, out);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                log_decay.requires_grad() || state.requires_grad() ||
                                                (new_state && new_state->requires_grad()) || (out && out->requires_grad())),
               "linear_attention_step has no gradients: call it under torch.no_grad(), or linear_attention");
-  TORCH_CHECK_VALUE(!S || state.size(0), "the pool is empty");
   return attention_step(q, k, v, log_decay, state, new_state, slots, scale, out);
 }
 
@@ -686,16 +723,49 @@ PYBIND11_MODULE(_mixer, m) {
   });
   const auto no_gil = py::call_guard<py::gil_scoped_release>();
   m.def("layer_norm", &layer_norm, no_gil);
-  m.def("norm_forward", &norm_forward, no_gil);
-  m.def("norm_backward", &norm_backward, no_gil);
   m.def("rotary_embed", &rotary_embed, no_gil);
-  m.def("rotate", &rotate, no_gil);
   m.def("linear_attention", &linear_attention);
+  m.def("linear_attention_step", &linear_attention_step, no_gil);
+  // the custom ops' launches: the same, checked here
+  m.def("norm_forward", [](const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps) {
+    check_norm_launch(x, weight, bias, groups);
+    return norm_forward(x, weight, bias, groups, eps);
+  }, no_gil);
+  m.def("norm_backward", [](const Tensor& dy, const Tensor& x, const OptTensor& weight, int64_t groups, double eps, bool need_dx,
+                            bool need_dw, bool need_db) {
+    TORCH_CHECK_VALUE(dy.sizes() == x.sizes(), "dy must have x's shape ", x.sizes(), ", got ", dy.sizes());
+    check_norm_launch(x, weight, std::nullopt, groups);
+    check_beside("dy", dy, x);
+    return norm_backward(dy, x, weight, groups, eps, need_dx, need_dw, need_db);
+  }, no_gil);
+  m.def("rotate", [](const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns, bool interleaved,
+                     bool inverse, double magnitude) {
+    check_rotary(q, k, positions, turns);
+    return rotate(q, k, positions, turns, interleaved, inverse, magnitude);
+  }, no_gil);
   m.def("attention_forward", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
                                 const OptTensor& initial, const OptTensor& lengths, double scale, bool want_state) {
+    check_attention(q, k, v, log_decay, initial, lengths);
     return attention_forward(q, k, v, log_decay, initial, lengths, scale, want_state, true);
   }, no_gil);
-  m.def("attention_backward", &attention_backward, no_gil);
-  m.def("linear_attention_step", &linear_attention_step, no_gil);
-  m.def("attention_step", &attention_step, no_gil);
+  m.def("attention_backward", [](const Tensor& dout, const OptTensor& dstate, const Tensor& q, const Tensor& k, const Tensor& v,
+                                 const Tensor& log_decay, const OptTensor& initial, const OptTensor& lengths, double scale,
+                                 const Tensor& states, const OptTensor& state, bool need_decay, bool need_initial) {
+    TORCH_CHECK_VALUE(dout.sizes() == q.sizes(), "dout must have q's shape ", q.sizes(), ", got ", dout.sizes());
+    check_state("dstate", dstate, q);
+    check_state("state", state, q);
+    TORCH_CHECK_VALUE(!state || (state->is_contiguous() && aligned(*state, 16)), "state must be contiguous and 16-byte aligned");
+    TORCH_CHECK_VALUE(states.scalar_type() == at::kFloat && states.is_contiguous(), "states must be the forward's");
+    check_attention(q, k, v, log_decay, initial, lengths);
+    check_beside("dout", dout, q);
+    check_beside("dstate", dstate, q);
+    check_beside("state", state, q);
+    check_beside("states", states, q);
+    return attention_backward(dout, dstate, q, k, v, log_decay, initial, lengths, scale, states, state, need_decay, need_initial);
+  }, no_gil);
+  m.def("attention_step", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
+                             const OptTensor& new_state, const OptTensor& slots, double scale, const OptTensor& out) {
+    check_step(q, k, v, log_decay, state, slots, new_state, out);
+    return attention_step(q, k, v, log_decay, state, new_state, slots, scale, out);
+  }, no_gil);
 }

@@ -274,6 +274,44 @@ def test_python_calls_refuse(pkg):
             pkg.rotary_embed(*args)
 
 
+def test_custom_ops_refuse(pkg):
+    """The custom ops are called without the Python checks of compiled calls too: their launches check for themselves."""
+    ops = torch.ops.dwarf
+    x, w = torch.zeros(3, 4, 8), torch.zeros(4, 8)
+    for args in ((x, None, None, 0, 1e-5), (x, None, None, 3, 1e-5), (x, w, None, 1, 1e-5), (x, None, w[:2], 4, 1e-5),
+                 (x, w.int(), None, 4, 1e-5), (torch.zeros(3, 0), None, None, 1, 1e-5), (x.double(), None, None, 1, 1e-5)):
+        with pytest.raises(ValueError):
+            ops.layer_norm_fwd(*args)
+    for args in ((x[:2], x, None, 1), (x, x, w, 1), (x, x, None, 0)):
+        with pytest.raises(ValueError):
+            ops.layer_norm_bwd(*args, 1e-5, True, True, True)
+    q, k, v = _qkv()
+    pos, turns = torch.arange(5), torch.zeros(32, dtype=torch.int64)
+    for args in ((q, k[:, :, :3], pos, turns), (q, k, pos[:4], turns), (q, k, pos, turns.int()), (q, k, pos, turns.repeat(2)),
+                 (q, k, pos, torch.zeros(64, dtype=torch.int64)[::2])):
+        with pytest.raises(ValueError):
+            ops.rotary(*args, False, False, 1.0)
+    lg, state, states = torch.zeros(4), torch.zeros(2, 4, 64, 64), torch.zeros(0)
+    for args in ((q, k[:, :, :3], v[:, :, :3], lg, None, None), (q, k, v, lg[:2], None, None), (q, k, v, lg, state[:1], None),
+                 (q, k, v, lg, None, torch.zeros(3, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            ops.linear_attention_fwd(*args, 0.125, True)
+        with pytest.raises(ValueError):
+            ops.linear_attention_bwd(q, None, *args, 0.125, states, None, True, True)
+    for dout, dstate, st, kept in ((q[:, :, :3], None, states, None), (q, state[:1], states, None), (q, None, states.int(), None),
+                                   (q, None, states, state[:, :2]), (q, None, states, state.transpose(2, 3))):
+        with pytest.raises(ValueError):
+            ops.linear_attention_bwd(dout, dstate, q, k, v, lg, None, None, 0.125, st, kept, True, True)
+    q, k, v = (x[:, :, 0] for x in (q, k, v))
+    for pool, slots in ((state[:1], None), (state.bfloat16(), None), (state, torch.zeros(3, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            ops.linear_attention_step_(q, k, v, lg, pool, slots, 0.125)
+        with pytest.raises(ValueError):
+            ops.linear_attention_step(q, k, v, lg, pool, pool.clone(), slots, 0.125)
+    with pytest.raises(RuntimeError, match="device tensors"):
+        ops.linear_attention_step_(q, k, v, lg, state, None, 0.125)
+
+
 def test_rotary_plan_frequencies(pkg):
     """Turns are the nearest 2^-64 fractions, and each scaling gives its formula's frequencies."""
     plan = pkg.rotary_plan(64, device="cpu")
