@@ -9,10 +9,14 @@
 //   dv_j = scale sum_{i >= j} g^{i-j} (k_j.q_i) do_i + g^{n-1-j} k_j G
 //   dk_j = scale sum_{i >= j} g^{i-j} (v_j.do_i) q_i + g^{n-1-j} v_j G^T
 //   G_in = g^n G + scale sum_i g^{i+1} q_i do_i^T
-// and, with tau the token's place in its segment counted from 1,
-//   dlog_decay = sum_segments [ sum_t tau (q.dq - k.dk) + n <S_out, G_out> ],
-// where tau is taken from the segment's middle, so that the two sums, which
-// nearly cancel, stay small.
+// and, with tau the token's place in its segment counted from 1, R and K the
+// shares of q.dq and k.dk that come from other chunks, and D the pairs within a
+// chunk, weighted with their gap,
+//   dlog_decay = sum_segments [ D + sum_t tau (R - K) + n <S_out, G_out> ].
+// A segment of one chunk takes each part by its own distance instead,
+//   D + sum_t tau R + sum_t (n - tau) K + n g^n <S_in, G_out>,
+// where nothing cancels (one token alone has exactly 0); longer ones count tau
+// from their middle, so that the two sums, which nearly cancel, stay small.
 //
 // A sequence is cut into segments.  The local launch forms each segment's own
 // sum; up to eight segments the rows' launch joins the sums in front of its
@@ -81,6 +85,15 @@ __device__ __forceinline__ double workgroup_sum_f64(double x, double* s_red) {
 #pragma unroll
   for (int i = 1; i < WAVES; ++i) t += s_red[i];
   return t;
+}
+
+// Where the weights of dlog_decay's two sides count from in a segment of n tokens.
+struct LaMid {
+  float rows, keys;
+};
+__device__ __forceinline__ LaMid la_mid(int n) {
+  const float f = static_cast<float>(n);
+  return n <= kChunk ? LaMid{0.f, f} : LaMid{0.5f * f, 0.5f * f};
 }
 
 __device__ __forceinline__ int la_length(const LaGeom& gm, int b) {
@@ -235,14 +248,16 @@ __global__ __launch_bounds__(kLaThreads) void la_scan_kernel(float* __restrict__
   const float* st = states ? states + static_cast<int64_t>(bh) * gm.segs * kState + e : nullptr;
   const int64_t at = static_cast<int64_t>(bh) * kState + e;
   auto load = [](const float* p) { return *reinterpret_cast<const f32x4*>(p); };
-  const float mid = 0.5f * static_cast<float>(gm.seg);
+  const bool one_chunk = n_last <= kChunk;   // the last segment, and with gm.seg one chunk every one
+  const float mid = gm.seg > kChunk ? 0.5f * static_cast<float>(gm.seg) : 0.f;
+  const float mid_last = one_chunk ? 0.f : 0.5f * static_cast<float>(n_last);
   f32x4 m = first ? load(first + at) : zero4();
   double sum = 0.;
   auto add_dot = [&](float weight, f32x4 a, f32x4 c) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum = fma(static_cast<double>(weight) * a[i], static_cast<double>(c[i]), sum);
   };
-  if (REV && dot && final && active && group == 0) add_dot(static_cast<float>(n_last) - mid, m, load(final + at));
+  if (REV && dot && final && active && !one_chunk && group == 0) add_dot(mid_last, m, load(final + at));
   // a pass takes GROUPS runs; position p counts segments in the direction of the scan
   for (int p0 = 0; p0 < active; p0 += GROUPS * kScanRun) {
     const int base = p0 + group * kScanRun;
@@ -252,11 +267,14 @@ __global__ __launch_bounds__(kLaThreads) void la_scan_kernel(float* __restrict__
 #pragma unroll
     for (int i = 0; i < kScanRun; ++i) {
       in[i] = i < cnt ? load(x + segment(i) * kState) : zero4();
-      sv[i] = REV && dot && i < cnt && segment(i) > 0 ? load(st + (segment(i) - kSums) * kState) : zero4();
+      sv[i] = !(REV && dot && i < cnt) ? zero4()
+              : segment(i) > 0         ? load(st + (segment(i) - kSums) * kState)
+              : initial                ? load(initial + at)
+                                       : zero4();
     }
     auto shrink = [&](int i) { return segment(i) == active - 1 ? tail : full; };
     if constexpr (REV && kSums) {   // all of the head's segments are here: the sums become the states in front
-      f32x4 u = dot && initial ? load(initial + at) : zero4();
+      f32x4 u = dot && initial ? load(initial + at) : zero4();   // and sv of segment 0
 #pragma unroll
       for (int i = kScanRun - 1; i >= 0; --i)
         if (i < cnt && segment(i) > 0) u = sv[i] = u * full + sv[i];
@@ -294,15 +312,18 @@ __global__ __launch_bounds__(kLaThreads) void la_scan_kernel(float* __restrict__
     for (int i = 0; i < kScanRun; ++i) {
       if (i < cnt) {
         *reinterpret_cast<f32x4*>(x + segment(i) * kState) = v;
+        const bool tail_segment = segment(i) == active - 1;
+        if (REV && dot && (gm.seg <= kChunk || (tail_segment && one_chunk)))   // uniform
+          add_dot(static_cast<float>(tail_segment ? n_last : gm.seg) * shrink(i), sv[i], v);   // <S in front of it, G behind it>
         v = v * shrink(i) + in[i];
-        if (REV && dot) add_dot(static_cast<float>(gm.seg), sv[i], v);   // <S in front of it, G in front of it>
+        // <S in front of it, G in front of it>, with its own part and that of the segment in front
+        if (REV && dot) add_dot((tail_segment ? mid_last : mid) + (segment(i) > 0 ? mid : 0.f), sv[i], v);
       }
     }
     if constexpr (GROUPS == 1) m = v;
   }
   if (last && group == 0) *reinterpret_cast<f32x4*>(last + at) = m;
   if (REV && dot) {
-    if (initial && active && group == 0) add_dot(mid, load(initial + at), m);
     sum = workgroup_sum_f64<kLaThreads / kWave>(sum, s_red);
     if (threadIdx.x == 0) dot[blockIdx.x] = sum;
   }
@@ -388,7 +409,7 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRowsCall<TO> call
     if (e.sums)
       for (int p = 0; p < seg; ++p) join(e.sums + (head * gm.segs + p) * kState, la_power(lg, gm.seg));
   }
-  const float mid = 0.5f * static_cast<float>(gm.seg);
+  const float mid = REV ? la_mid(t1 - t0).keys : la_mid(t1 - t0).rows;
   double total = 0.;
   const int chunks = t1 > t0 ? (t1 - t0 + kChunk - 1) / kChunk : 0;
   LaRaw16<T> xa, xb, xc;
@@ -1036,7 +1057,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
   } else {
     fetch(0);
     const ScoreWeights sw(lg, gm.scale, false);
-    const float carry = gm.scale * la_power(lg, 16 * w + c + 1), mid = 0.5f * static_cast<float>(gm.seg);
+    const float carry = gm.scale * la_power(lg, 16 * w + c + 1), mid = la_mid(t1 - t0).rows;
     for (int i = 0; i < chunks; ++i) {
       put();
       __syncthreads();
@@ -1134,7 +1155,7 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
   };
   const ScoreWeights sw(lg, gm.scale, true);
   const AdjointWeights wt(lg, gm.scale);
-  const float mid = 0.5f * static_cast<float>(gm.seg);
+  const float mid = la_mid(t1 - t0).keys;
   float total = 0.f;
   fetch(0);
   for (int i = 0; i < chunks; ++i) {

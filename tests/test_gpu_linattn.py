@@ -124,6 +124,31 @@ def test_gradients(pkg, device, B, H, Hkv, N, initial, lengths, dtype):
     within(got["log_decay"], want["log_decay"], 3 * 256 * flow, torch.float32, slack(dtype))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("B,H,N,lengths", [(13, 1, 1, None), (64, 8, 1, None), (3, 2, 200, [1, 0, 1]), (70, 8, 70, [1] * 70)])
+def test_one_token_has_no_decay_gradient(pkg, device, B, H, N, lengths, dtype):
+    """A sequence's first token onto an empty state: no decay stands in its output or its state, so the gradient is 0
+    itself, in short segments and in long ones."""
+    d = put(make(B, H, H, N, dtype, seed=B + N, lengths=lengths), device)
+    d["log_decay"].requires_grad_(True)
+    out, state = forward(pkg, d, return_state=True)
+    g, = torch.autograd.grad((out, state), d["log_decay"], (d["dout"], d["dstate"]))
+    assert torch.equal(g, torch.zeros_like(g))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("B,H,Hkv,N,initial,lengths", [(1, 4, 2, 655, False, None), (2, 3, 3, 257, True, [257, 64]),
+                                                       (1, 2, 1, 31, True, None), (16, 32, 32, 40, True, None)])
+def test_decay_gradient_where_nothing_cancels(pkg, device, B, H, Hkv, N, initial, lengths, dtype):
+    """Segments of one chunk add positive multiples of each share: the fp32 bound over the terms themselves."""
+    x = make(B, H, Hkv, N, dtype, seed=N, initial=initial, lengths=lengths)
+    d = put(x, device)
+    d["log_decay"].requires_grad_(True)
+    out, state = forward(pkg, d, return_state=True)
+    g, = torch.autograd.grad((out, state), d["log_decay"], (d["dout"], d["dstate"]))
+    within(g, oracle_grads(x)[3], oracle_grads(absolute(x))[3], torch.float32, FP32)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
 @pytest.mark.parametrize("B,H,Hkv,N,lengths", [(2, 2, 1, 700, [700, 577]), (3, 1, 1, 512, [512, 65, 513]),
                                                (1, 1, 1, 9001, None), (2, 1, 1, 8300, [8193, 1100])])
