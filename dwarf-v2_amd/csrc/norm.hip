@@ -41,6 +41,13 @@ __device__ __forceinline__ int64_t norm_at(int64_t r, int groups, int64_t s0, in
   return o * s0 + (r - o * groups) * s1;
 }
 
+// g w, rounded the same in the row's mean and in what the mean is taken from: a row of one value then has a gradient of
+// exactly 0, where a fused product would leave the rounding's residue times r.
+__device__ __forceinline__ float norm_weighted(float g, float w) {
+#pragma clang fp contract(off)
+  return g * w;
+}
+
 // Sum over the TPR threads of a row.  TPR above the wave: the whole workgroup of THREADS is one row's.
 template <int TPR, int THREADS>
 __device__ __forceinline__ float row_sum(float x, float* s_red) {
@@ -209,7 +216,7 @@ __global__ __launch_bounds__(kNormBwdThreads) void norm_bwd_kernel(
         const int i = k * VEC + e;
         v[i] = in ? v[i] - mu : 0.f;
         q = fmaf(v[i], v[i], q);
-        const float gw = g[i] * w[i];
+        const float gw = norm_weighted(g[i], w[i]);
         sg += gw;
         sgv = fmaf(gw, v[i], sgv);
       }
@@ -226,7 +233,7 @@ __global__ __launch_bounds__(kNormBwdThreads) void norm_bwd_kernel(
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const int i = k * VEC + e;
-        o[e] = rs * (fmaf(g[i], w[i], -m1) - v[i] * m2);
+        o[e] = rs * (norm_weighted(g[i], w[i]) - m1 - v[i] * m2);
         dw[i] = fmaf(g[i], v[i] * rs, dw[i]);
         db[i] += g[i];
       }
@@ -317,7 +324,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_stream(const T* __restr
       load_vec<T, VEC>(gr + d, g);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float c = v[e] - mu, gw = g[e] * (weight ? wg[d + e] : 1.f);
+        const float c = v[e] - mu, gw = norm_weighted(g[e], weight ? wg[d + e] : 1.f);
         q = fmaf(c, c, q);
         sg += gw;
         sgv = fmaf(gw, c, sgv);
@@ -338,7 +345,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_stream(const T* __restr
       load_vec<T, VEC>(xr + d, v);
       load_vec<T, VEC>(gr + d, g);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = rs * (fmaf(g[e], weight ? wg[d + e] : 1.f, -m1) - (v[e] - mu) * m2);
+      for (int e = 0; e < VEC; ++e) v[e] = rs * (norm_weighted(g[e], weight ? wg[d + e] : 1.f) - m1 - (v[e] - mu) * m2);
       store_vec<T, VEC>(dr + d, v);
     }
   }

@@ -134,6 +134,19 @@ def test_rows_far_off_centre(pkg, device):
     assert float((y - mixer_ref.layer_norm(x)).abs().max()) <= 16 * 2.0 ** -24 * 1000 * 4
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_rows_of_one_value_have_no_gradient(pkg, device, dtype):
+    """y is the bias whatever x holds: dx and dw are 0 themselves."""
+    g = torch.Generator().manual_seed(5)
+    x, dy = (torch.randn(1000, 1, generator=g).to(dtype).to(device) for _ in range(2))
+    w, b = (torch.randn(1, generator=g).to(device) for _ in range(2))
+    for t in (x, w, b):
+        t.requires_grad_(True)
+    y = pkg.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert torch.equal(y, b.to(dtype).expand_as(y)) and not dx.any() and not dw.any() and db.any()
+
+
 def test_constant_rows_and_values_that_are_not_numbers(pkg, device):
     """A constant row gives the bias; a NaN or infinity spoils its own row alone."""
     x = torch.full((6, 130), 3.0)
