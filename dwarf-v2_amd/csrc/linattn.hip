@@ -1448,6 +1448,15 @@ void la_fwd_typed(const dwarf_linear_attention_fwd_args& a, const LaGeom& gm, hi
                      scanned ? nullptr : a.final);
 }
 
+// Whether the backward needs the adjoint's scan: several segments, the gradient of the state that enters, or boundary terms
+// of dlog_decay.  A single segment has those only where a state enters or its adjoint does; one chunk only where both do.
+// Without it a training call of one segment has a launch less (of four), and dq forms no sums.
+bool la_joined(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm) {
+  if (gm.segs != 1 || a.dinitial) return true;
+  if (!a.dlog_decay) return false;
+  return gm.N <= kChunk ? a.fwd.initial && a.dfinal : a.fwd.initial || a.dfinal;
+}
+
 // Workspace of the backward, in floats: the adjoints per segment, the dlog_decay sums, the shared heads' parts.
 struct LaBwdSpace {
   size_t adjoint, dq_dot, dk_dot, edge, dk_part, dv_part, total;
@@ -1481,7 +1490,7 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
   double* dq_dot = dlog ? reinterpret_cast<double*>(ws + sp.dq_dot) : nullptr;
   double* dk_dot = dlog ? reinterpret_cast<double*>(ws + sp.dk_dot) : nullptr;
   double* edge = dlog ? reinterpret_cast<double*>(ws + sp.edge) : nullptr;
-  const bool joined = gm.segs != 1 || a.dinitial || dlog;
+  const bool joined = la_joined(a, gm);
   const float* enter = joined ? adj : a.dfinal;
   const LaEnter before = la_enter(f, gm), behind = joined ? LaEnter{adj, nullptr, nullptr} : LaEnter{nullptr, a.dfinal, nullptr};
   const bool shared = gm.H != gm.Hkv;
@@ -1539,7 +1548,7 @@ void la_bwd_typed(const dwarf_linear_attention_bwd_args& a, const LaGeom& gm, hi
     }
   }
   if (dlog)
-    hipLaunchKernelGGL(la_dlog_kernel, dim3(gm.H), block, 0, stream, gm.segs ? dq_dot : nullptr, dk_dot, edge,
+    hipLaunchKernelGGL(la_dlog_kernel, dim3(gm.H), block, 0, stream, gm.segs ? dq_dot : nullptr, dk_dot, joined ? edge : nullptr,
                        scan_wgs(gm), gm, a.dlog_decay);
 }
 

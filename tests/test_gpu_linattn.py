@@ -202,6 +202,29 @@ def test_gradients_with_parts_left_out(pkg, device):
     within(dlg, want[3], 3 * 256 * flow, torch.float32, FP32)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("initial", [False, True])
+@pytest.mark.parametrize("state", [False, True])
+@pytest.mark.parametrize("B,H,Hkv,N,lengths", [(2, 2, 1, 40, [40, 9]), (14, 32, 32, 100, [100, 64, 65, 0] + [77] * 10)])
+def test_decay_gradient_of_a_single_segment(pkg, device, B, H, Hkv, N, lengths, state, initial, dtype):
+    """One segment of one chunk and of two, with and without a state that enters (and needs no gradient) or leaves."""
+    x = make(B, H, Hkv, N, dtype, seed=N + state, initial=initial, lengths=lengths)
+    d = put(x, device)
+    names = ("q", "k", "v", "log_decay")
+    for n in names:
+        d[n].requires_grad_(True)
+    out, left = forward(pkg, d, return_state=True)
+    outs, ups = ((out, left), (d["dout"], d["dstate"])) if state else ((out,), (d["dout"],))
+    got = torch.autograd.grad(outs, [d[n] for n in names], ups)
+    a = absolute(x)
+    want, terms = oracle_grads(x, state=state), oracle_grads(a, state=state)
+    for i in range(3):
+        within(got[i], want[i], terms[i], dtype, slack(dtype))
+    # as in test_gradients
+    flow = (a["q"].double() * terms[0]).sum((0, 2, 3)) + (oracle(a)[1] * a["dstate"].double()).sum((0, 2, 3))
+    within(got[3], want[3], 3 * 256 * flow, torch.float32, slack(dtype))
+
+
 def test_gradients_match_differences(pkg, device):
     """The output is linear in q, in k and in v and the state enters linearly: a central difference of any step is
     exact up to rounding.  log_decay takes a step that stays below 0; what its difference leaves out is the float64
