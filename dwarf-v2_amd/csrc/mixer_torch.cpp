@@ -51,6 +51,14 @@ void launch(F fn, const A& args, const Tensor& on, const char* what) {
   check_status(fn(&args, reinterpret_cast<dwarf_stream_t>(c10::hip::getCurrentHIPStream(on.device().index()).stream())), what);
 }
 
+// Derivatives in forward mode: there are none, and a result without a tangent would count as a constant.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
+template <typename... T>
+void refuse_tangents(const char* what, const T&... t) {
+  TORCH_CHECK(!(has_tangent(t) || ...), what, " has no derivative in forward mode: differentiate it backward");
+}
+
 int dtype_of(const Tensor& x, const char* what) {
   switch (x.scalar_type()) {
     case at::kBFloat16: return DWARF_BF16;
@@ -254,6 +262,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     {
       const at::NoGradGuard no_grad;
       const OptTensor weight = has_w ? OptTensor(saved[1]) : std::nullopt;
+      refuse_tangents("layer_norm", grads[0], saved[0], weight);
       auto [dx, dw, db] = norm_backward(grads[0], saved[0], weight, ctx->saved_data["groups"].toInt(),
                                         ctx->saved_data["eps"].toDouble(), ctx->needs_input_grad(0), need_w, need_b);
       out[0] = dx;
@@ -265,6 +274,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
 };
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  refuse_tangents("layer_norm", x, weight, bias);
   TORCH_CHECK_VALUE(std::isfinite(eps) && eps >= 0, "eps must be finite and not negative");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must have a last dimension to normalise, got ", x.sizes());
   int64_t groups = 1;
@@ -353,6 +363,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
     if (!dq.defined() && !dk.defined()) return out;
     {
       const at::NoGradGuard no_grad;
+      refuse_tangents("rotary_embed", dq, dk);
       const bool interleaved = ctx->saved_data["interleaved"].toBool();
       const double magnitude = ctx->saved_data["magnitude"].toDouble();
       // a single one is turned alone: its heads take q's place
@@ -389,6 +400,7 @@ void check_rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, 
 
 std::tuple<Tensor, OptTensor> rotary_embed(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns,
                                            bool interleaved, double magnitude) {
+  refuse_tangents("rotary_embed", q, k);
   check_rotary(q, k, positions, turns);
   if (at::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()))) {
     const variable_list r = RotaryFn::apply(q, k, positions, turns, interleaved, magnitude);
@@ -524,6 +536,7 @@ struct LinearAttentionFn : torch::autograd::Function<LinearAttentionFn> {
     if (!dout.defined() && !dstate.defined()) return result;
     {
       const at::NoGradGuard no_grad;
+      refuse_tangents("linear_attention", dout, dstate, s[0], s[1], s[2], s[3], s[4]);
       if (!dout.defined()) dout = at::zeros_like(s[0]);
       auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
       auto [dq, dk, dv, dlog, dinitial] =
@@ -587,6 +600,7 @@ void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Te
 py::object linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
                             const std::optional<double>& scale_, const OptTensor& initial, const OptTensor& lengths,
                             bool return_state) {
+  refuse_tangents("linear_attention", q, k, v, log_decay, initial);
   const double scale = scale_or_default(scale_);
   check_attention(q, k, v, log_decay, initial, lengths);
   Tensor out, state;
@@ -694,6 +708,7 @@ void check_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
 Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
                              const OptTensor& slots, const OptTensor& new_state, const std::optional<double>& scale_,
                              const OptTensor& out) {
+  refuse_tangents("linear_attention_step", q, k, v, log_decay, state, new_state, out);
   const double scale = scale_or_default(scale_);
   check_step(q, k, v, log_decay, state, slots, new_state, out);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() ||
@@ -728,11 +743,13 @@ PYBIND11_MODULE(_mixer, m) {
   m.def("linear_attention_step", &linear_attention_step, no_gil);
   // the custom ops' launches: the same, checked here
   m.def("norm_forward", [](const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps) {
+    refuse_tangents("layer_norm", x, weight, bias);
     check_norm_launch(x, weight, bias, groups);
     return norm_forward(x, weight, bias, groups, eps);
   }, no_gil);
   m.def("norm_backward", [](const Tensor& dy, const Tensor& x, const OptTensor& weight, int64_t groups, double eps, bool need_dx,
                             bool need_dw, bool need_db) {
+    refuse_tangents("layer_norm", dy, x, weight);
     TORCH_CHECK_VALUE(dy.sizes() == x.sizes(), "dy must have x's shape ", x.sizes(), ", got ", dy.sizes());
     check_norm_launch(x, weight, std::nullopt, groups);
     check_beside("dy", dy, x);
@@ -740,17 +757,20 @@ PYBIND11_MODULE(_mixer, m) {
   }, no_gil);
   m.def("rotate", [](const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns, bool interleaved,
                      bool inverse, double magnitude) {
+    refuse_tangents("rotary_embed", q, k);
     check_rotary(q, k, positions, turns);
     return rotate(q, k, positions, turns, interleaved, inverse, magnitude);
   }, no_gil);
   m.def("attention_forward", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
                                 const OptTensor& initial, const OptTensor& lengths, double scale, bool want_state) {
+    refuse_tangents("linear_attention", q, k, v, log_decay, initial);
     check_attention(q, k, v, log_decay, initial, lengths);
     return attention_forward(q, k, v, log_decay, initial, lengths, scale, want_state, true);
   }, no_gil);
   m.def("attention_backward", [](const Tensor& dout, const OptTensor& dstate, const Tensor& q, const Tensor& k, const Tensor& v,
                                  const Tensor& log_decay, const OptTensor& initial, const OptTensor& lengths, double scale,
                                  const Tensor& states, const OptTensor& state, bool need_decay, bool need_initial) {
+    refuse_tangents("linear_attention", dout, dstate, q, k, v, log_decay, initial);
     TORCH_CHECK_VALUE(dout.sizes() == q.sizes(), "dout must have q's shape ", q.sizes(), ", got ", dout.sizes());
     check_state("dstate", dstate, q);
     check_state("state", state, q);
@@ -765,6 +785,7 @@ PYBIND11_MODULE(_mixer, m) {
   }, no_gil);
   m.def("attention_step", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
                              const OptTensor& new_state, const OptTensor& slots, double scale, const OptTensor& out) {
+    refuse_tangents("linear_attention_step", q, k, v, log_decay, state, new_state, out);
     check_step(q, k, v, log_decay, state, slots, new_state, out);
     return attention_step(q, k, v, log_decay, state, new_state, slots, scale, out);
   }, no_gil);

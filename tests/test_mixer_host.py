@@ -312,6 +312,49 @@ def test_custom_ops_refuse(pkg):
         ops.linear_attention_step_(q, k, v, lg, state, None, 0.125)
 
 
+def _tangent_calls(pkg, tensors):
+    """(name, call) for each floating tensor of each operator, the tensor taken from ``tensors`` (name -> tensor)."""
+    t = tensors
+    args = (t["q"], t["k"], t["v"], t["log_decay"])
+    rows = tuple(t[n][:, :, 0] for n in ("q", "k", "v"))
+    return (("layer_norm", lambda: pkg.layer_norm(t["x"], t["weight"], t["bias"]), ("x", "weight", "bias")),
+            ("rotary_embed", lambda: pkg.rotary_embed(t["q"], t["k"], t["positions"], t["plan"]), ("q", "k")),
+            ("linear_attention", lambda: pkg.linear_attention(*args, initial_state=t["initial"]),
+             ("q", "k", "v", "log_decay", "initial")),
+            ("linear_attention_step", lambda: pkg.linear_attention_step(*rows, t["log_decay"], t["pool"]),
+             ("q", "k", "v", "log_decay", "pool")),
+            ("layer_norm", lambda: torch.ops.dwarf.layer_norm_fwd(t["x"], t["weight"], t["bias"], 1, 1e-5), ("x", "weight", "bias")),
+            ("layer_norm", lambda: torch.ops.dwarf.layer_norm_bwd(t["x"], t["x"], t["weight"], 1, 1e-5, True, True, True),
+             ("x", "weight")),
+            ("rotary_embed", lambda: torch.ops.dwarf.rotary(t["q"], t["k"], t["positions"], t["plan"].turns, False, False, 1.0),
+             ("q", "k")),
+            ("linear_attention", lambda: torch.ops.dwarf.linear_attention_fwd(*args, t["initial"], None, 0.125, True),
+             ("q", "k", "v", "log_decay", "initial")),
+            ("linear_attention", lambda: torch.ops.dwarf.linear_attention_bwd(
+                t["q"], t["initial"], *args, None, None, 0.125, t["states"], None, True, False), ("q", "k", "v", "log_decay", "initial")),
+            ("linear_attention_step", lambda: torch.ops.dwarf.linear_attention_step_(*rows, t["log_decay"], t["pool"], None, 0.125),
+             ("q", "k", "v", "log_decay", "pool")))
+
+
+def test_forward_mode_derivatives_are_refused(pkg):
+    """A tangent of any input, which the results would drop, is an error (before the device is asked for)."""
+    import torch.autograd.forward_ad as fw
+    q, k, v = _qkv(dtype=torch.float32)
+    base = dict(q=q, k=k, v=v, log_decay=torch.zeros(4), initial=torch.zeros(2, 4, 64, 64), pool=torch.zeros(3, 4, 64, 64),
+                x=torch.zeros(3, 8), weight=torch.ones(8), bias=torch.zeros(8), states=torch.zeros(0), positions=torch.arange(5),
+                plan=pkg.rotary_plan(64, device="cpu"))
+    count = len(_tangent_calls(pkg, base))
+    for i in range(count):
+        for name in _tangent_calls(pkg, base)[i][2]:
+            with fw.dual_level():
+                dual = dict(base, **{name: fw.make_dual(base[name], torch.ones_like(base[name]))})
+                what, call, _ = _tangent_calls(pkg, dual)[i]
+                with pytest.raises(RuntimeError, match=f"{what} has no derivative in forward mode"):
+                    call()
+    with pytest.raises(RuntimeError, match="has no derivative in forward mode"):
+        torch.func.jvp(pkg.layer_norm, (base["x"],), (base["x"],))
+
+
 def test_rotary_plan_frequencies(pkg):
     """Turns are the nearest 2^-64 fractions, and each scaling gives its formula's frequencies."""
     plan = pkg.rotary_plan(64, device="cpu")
