@@ -1,5 +1,5 @@
 """Host-side pieces of the mixer's operators (norm.py, rotary.py, linattn.py): the native module, and the argument
-checks of compiled calls."""
+checks of compiled and traced calls."""
 
 from __future__ import annotations
 

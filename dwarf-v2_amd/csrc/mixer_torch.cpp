@@ -15,7 +15,9 @@
 
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -49,6 +51,36 @@ template <typename F, typename A>
 void launch(F fn, const A& args, const Tensor& on, const char* what) {
   const c10::DeviceGuard guard(on.device());
   check_status(fn(&args, reinterpret_cast<dwarf_stream_t>(c10::hip::getCurrentHIPStream(on.device().index()).stream())), what);
+}
+
+// What a launch on raw pointers would go past: tensors without memory of their own (fake, batched, wrapped by a transform),
+// those that stand for other values than their memory holds (negated, zero tensors), and whatever watches the dispatcher
+// (modes, traces).  An eager call or backward node that meets any of them goes through the custom ops, which the dispatcher
+// knows.
+constexpr c10::DispatchKeySet kWatched{
+    c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot, c10::DispatchKey::PythonDispatcher,
+    c10::DispatchKey::PreDispatch, c10::DispatchKey::Functionalize, c10::DispatchKey::Tracer, c10::DispatchKey::Batched,
+    c10::DispatchKey::VmapMode, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchVmapMode,
+    c10::DispatchKey::FuncTorchBatchedDecomposition, c10::DispatchKey::FuncTorchGradWrapper,
+    c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchDynamicLayerBackMode,
+    c10::DispatchKey::Negative, c10::DispatchKey::Conjugate, c10::DispatchKey::ZeroTensor};
+
+c10::DispatchKeySet keys_of(const Tensor& t) { return t.defined() ? t.key_set() : c10::DispatchKeySet(); }
+c10::DispatchKeySet keys_of(const OptTensor& t) { return t ? keys_of(*t) : c10::DispatchKeySet(); }
+template <typename... T>
+bool watched(const T&... t) {
+  const c10::impl::LocalDispatchKeySet local = c10::impl::tls_local_dispatch_key_set();
+  return (((keys_of(t) | ...) | local.included_) - local.excluded_).has_any(kWatched);
+}
+
+// The custom op `name` through the dispatcher.
+template <typename... T>
+std::vector<Tensor> dispatched(const char* name, const T&... args) {
+  torch::jit::Stack stack{c10::IValue(args)...};
+  c10::Dispatcher::singleton().findSchemaOrThrow(name, "").callBoxed(&stack);
+  std::vector<Tensor> out;
+  for (const c10::IValue& v : stack) out.push_back(v.toTensor());
+  return out;
 }
 
 // Derivatives in forward mode: there are none, and a result without a tangent would count as a constant.
@@ -262,10 +294,18 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     {
       const at::NoGradGuard no_grad;
       const OptTensor weight = has_w ? OptTensor(saved[1]) : std::nullopt;
+      const int64_t groups = ctx->saved_data["groups"].toInt();
+      const double eps = ctx->saved_data["eps"].toDouble();
+      const bool need_x = ctx->needs_input_grad(0);
+      Tensor dx, dw, db;
       refuse_tangents("layer_norm", grads[0], saved[0], weight);
-      auto [dx, dw, db] = norm_backward(grads[0], saved[0], weight, ctx->saved_data["groups"].toInt(),
-                                        ctx->saved_data["eps"].toDouble(), ctx->needs_input_grad(0), need_w, need_b);
-      out[0] = dx;
+      if (watched(grads[0], saved[0], weight)) {
+        const auto r = dispatched("dwarf::layer_norm_bwd", grads[0], saved[0], weight, groups, eps, need_x, need_w, need_b);
+        dx = r[0], dw = r[1], db = r[2];
+      } else {
+        std::tie(dx, dw, db) = norm_backward(grads[0], saved[0], weight, groups, eps, need_x, need_w, need_b);
+      }
+      if (need_x) out[0] = dx;
       if (need_w) out[1] = dw.view(saved[1].sizes()).to(saved[1].scalar_type());
       if (need_b) out[2] = db.view(ctx->saved_data["bias_shape"].toIntVector()).to(ctx->saved_data["bias_dtype"].toScalarType());
     }
@@ -273,8 +313,10 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   }
 };
 
-Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+// Nothing: the call goes through the custom ops (see kWatched).
+OptTensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
   refuse_tangents("layer_norm", x, weight, bias);
+  if (watched(x, weight, bias)) return std::nullopt;
   TORCH_CHECK_VALUE(std::isfinite(eps) && eps >= 0, "eps must be finite and not negative");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must have a last dimension to normalise, got ", x.sizes());
   int64_t groups = 1;
@@ -368,8 +410,14 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
       const double magnitude = ctx->saved_data["magnitude"].toDouble();
       // a single one is turned alone: its heads take q's place
       const Tensor& first = dq.defined() ? dq : dk;
-      auto [a, b] = rotate(first, dq.defined() && dk.defined() ? OptTensor(dk) : std::nullopt, saved[0], saved[1],
-                           interleaved, true, magnitude);
+      const OptTensor second = dq.defined() && dk.defined() ? OptTensor(dk) : std::nullopt;
+      Tensor a, b;
+      if (watched(dq, dk, saved[0], saved[1])) {
+        const auto r = dispatched("dwarf::rotary", first, second, saved[0], saved[1], interleaved, true, magnitude);
+        a = r[0], b = r[1];
+      } else {
+        std::tie(a, b) = rotate(first, second, saved[0], saved[1], interleaved, true, magnitude);
+      }
       if (dq.defined()) out[0] = a;
       if (dk.defined()) out[1] = dq.defined() ? b : a;
     }
@@ -398,16 +446,19 @@ void check_rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, 
   check_beside("plan", turns, q);
 }
 
-std::tuple<Tensor, OptTensor> rotary_embed(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns,
-                                           bool interleaved, double magnitude) {
+// Nothing: the call goes through the custom ops (see kWatched).
+std::optional<std::tuple<Tensor, OptTensor>> rotary_embed(const Tensor& q, const OptTensor& k, const Tensor& positions,
+                                                          const Tensor& turns, bool interleaved, double magnitude) {
+  using Result = std::tuple<Tensor, OptTensor>;
   refuse_tangents("rotary_embed", q, k);
+  if (watched(q, k, positions, turns)) return std::nullopt;
   check_rotary(q, k, positions, turns);
   if (at::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()))) {
     const variable_list r = RotaryFn::apply(q, k, positions, turns, interleaved, magnitude);
-    return {r[0], k ? OptTensor(r[1]) : std::nullopt};
+    return Result{r[0], k ? OptTensor(r[1]) : std::nullopt};
   }
   auto [q_out, k_out] = rotate(q, k, positions, turns, interleaved, false, magnitude);
-  return {q_out, k ? OptTensor(k_out) : std::nullopt};
+  return Result{q_out, k ? OptTensor(k_out) : std::nullopt};
 }
 
 // ---- decayed linear attention ------------------------------------------------------------------
@@ -539,9 +590,20 @@ struct LinearAttentionFn : torch::autograd::Function<LinearAttentionFn> {
       refuse_tangents("linear_attention", dout, dstate, s[0], s[1], s[2], s[3], s[4]);
       if (!dout.defined()) dout = at::zeros_like(s[0]);
       auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
-      auto [dq, dk, dv, dlog, dinitial] =
-          attention_backward(dout, opt(dstate), s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), ctx->saved_data["scale"].toDouble(),
-                             s[6], opt(s[7]), ctx->needs_input_grad(3), s[4].defined() && ctx->needs_input_grad(4));
+      const double scale = ctx->saved_data["scale"].toDouble();
+      const bool need_decay = ctx->needs_input_grad(3), need_initial = s[4].defined() && ctx->needs_input_grad(4);
+      Tensor dq, dk, dv, dlog, dinitial;
+      if (watched(dout, dstate, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7])) {
+        const Tensor states = s[6].defined() ? s[6] : empty_f32({0}, s[0]);
+        const auto r = dispatched("dwarf::linear_attention_bwd", dout, opt(dstate), s[0], s[1], s[2], s[3], opt(s[4]),
+                                  opt(s[5]), scale, states, opt(s[7]), need_decay, need_initial);
+        dq = r[0], dk = r[1], dv = r[2];
+        if (need_decay) dlog = r[3];
+        if (need_initial) dinitial = r[4];
+      } else {
+        std::tie(dq, dk, dv, dlog, dinitial) = attention_backward(dout, opt(dstate), s[0], s[1], s[2], s[3], opt(s[4]),
+                                                                  opt(s[5]), scale, s[6], opt(s[7]), need_decay, need_initial);
+      }
       if (ctx->needs_input_grad(0)) result[0] = dq;
       if (ctx->needs_input_grad(1)) result[1] = dk;
       if (ctx->needs_input_grad(2)) result[2] = dv;
@@ -597,10 +659,12 @@ void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   TORCH_CHECK(hd == kHd, "linear attention is built for head_dim 64, got ", hd);
 }
 
+// None: the call goes through the custom ops (see kWatched).
 py::object linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
                             const std::optional<double>& scale_, const OptTensor& initial, const OptTensor& lengths,
                             bool return_state) {
   refuse_tangents("linear_attention", q, k, v, log_decay, initial);
+  if (watched(q, k, v, log_decay, initial, lengths)) return py::none();
   const double scale = scale_or_default(scale_);
   check_attention(q, k, v, log_decay, initial, lengths);
   Tensor out, state;
@@ -705,10 +769,12 @@ void check_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
   TORCH_CHECK_VALUE(!S || state.size(0), "the pool is empty");
 }
 
-Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
-                             const OptTensor& slots, const OptTensor& new_state, const std::optional<double>& scale_,
-                             const OptTensor& out) {
+// Nothing: the call goes through the custom ops (see kWatched).
+OptTensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
+                                const OptTensor& slots, const OptTensor& new_state, const std::optional<double>& scale_,
+                                const OptTensor& out) {
   refuse_tangents("linear_attention_step", q, k, v, log_decay, state, new_state, out);
+  if (watched(q, k, v, log_decay, state, slots, new_state, out)) return std::nullopt;
   const double scale = scale_or_default(scale_);
   check_step(q, k, v, log_decay, state, slots, new_state, out);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() ||

@@ -56,7 +56,7 @@ def attention_step(q, k, v, log_decay, state, new_state, slots, scale: float, ou
 
 
 class _LinearAttentionFn(torch.autograd.Function):
-    """The autograd node of compiled calls; eager calls have theirs in C++."""
+    """The autograd node of compiled and traced calls; eager calls have theirs in C++."""
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, initial, lengths, scale: float, want_state: bool):
@@ -87,7 +87,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     each sequence, behind which nothing is used and the output is zero.  Tokens are summed 64 at a time, so one
     that is not finite spoils its sequence's outputs from the first of its 64 on."""
     if not torch.compiler.is_compiling():
-        return _launch.native().linear_attention(q, k, v, log_decay, scale, initial_state, lengths, return_state)
+        done = _launch.native().linear_attention(q, k, v, log_decay, scale, initial_state, lengths, return_state)
+        if done is not None:   # None: fake or wrapped tensors, a mode or a trace
+            return done
     scale = _check(q, k, v, log_decay, scale, initial_state, lengths)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
         return _LinearAttentionFn.apply(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
@@ -107,13 +109,17 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     is zero.  Rows that share a slot are consecutive tokens of its sequence, in row order.  ``out``: where to write
     the result (eager calls).  No gradients."""
     if not torch.compiler.is_compiling():
-        return _launch.native().linear_attention_step(q, k, v, log_decay, state, slots, new_state, scale, out)
-    if out is not None:
+        done = _launch.native().linear_attention_step(q, k, v, log_decay, state, slots, new_state, scale, out)
+        if done is not None:   # None: fake or wrapped tensors, a mode or a trace
+            return done
+    elif out is not None:
         raise RuntimeError("out= is for eager calls and captured graphs, not for torch.compile")
-    scale = _check_step(q, k, v, log_decay, state, slots, new_state, scale)
+    scale = _check_step(q, k, v, log_decay, state, slots, new_state, scale, out)
     if new_state is None:
-        return torch.ops.dwarf.linear_attention_step_(q, k, v, log_decay, state, slots, scale)
-    return torch.ops.dwarf.linear_attention_step(q, k, v, log_decay, state, new_state, slots, scale)
+        result = torch.ops.dwarf.linear_attention_step_(q, k, v, log_decay, state, slots, scale)
+    else:
+        result = torch.ops.dwarf.linear_attention_step(q, k, v, log_decay, state, new_state, slots, scale)
+    return result if out is None else out.copy_(result)
 
 
 def _check_scale(scale) -> float:
@@ -138,7 +144,7 @@ def _check_heads(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: t
 
 
 def _check(q, k, v, log_decay, scale, initial_state, lengths) -> float:
-    """The native call's checks, for compiled calls; returns the scale."""
+    """The native call's checks, for compiled and traced calls; returns the scale."""
     scale = _check_scale(scale)
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError(f"q, k and v must be [B,H,N,{HEAD_DIM}], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -155,8 +161,9 @@ def _check(q, k, v, log_decay, scale, initial_state, lengths) -> float:
     return scale
 
 
-def _check_step(q, k, v, log_decay, state, slots, new_state, scale) -> float:
-    """The native call's checks but those of memory (strides and alignment, made at the launch), for compiled calls."""
+def _check_step(q, k, v, log_decay, state, slots, new_state, scale, out) -> float:
+    """The native call's checks but those of memory (strides and alignment, made at the launch), for compiled and traced
+    calls."""
     scale = _check_scale(scale)
     if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
         raise ValueError(f"q, k and v must be [S,H,{HEAD_DIM}], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -173,7 +180,10 @@ def _check_step(q, k, v, log_decay, state, slots, new_state, scale) -> float:
         raise ValueError(f"a pool of {state.shape[0]} states does not hold the {S} rows")
     if slots is not None and (tuple(slots.shape) != (S,) or slots.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"slots must be [{S}] int32 or int64, got {tuple(slots.shape)} {slots.dtype}")
-    _launch.check_device(q, k=k, v=v, log_decay=log_decay, state=state, new_state=new_state, slots=slots)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
+        raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}, got {tuple(out.shape)} {out.dtype}")
+    _launch.check_device(q, k=k, v=v, log_decay=log_decay, state=state, new_state=new_state, slots=slots, out=out)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (q, k, v, log_decay, state, new_state, out)):
         raise RuntimeError("linear_attention_step has no gradients: call it under torch.no_grad(), or linear_attention")
     return scale

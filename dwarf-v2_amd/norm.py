@@ -33,7 +33,7 @@ def norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None
 
 
 class _LayerNormFn(torch.autograd.Function):
-    """The autograd node of compiled calls; eager calls have theirs in C++."""
+    """The autograd node of compiled and traced calls; eager calls have theirs in C++."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups: int, eps: float):
@@ -58,7 +58,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                eps: float = 1e-5) -> torch.Tensor:
     """Layer norm of the last dimension; weight and bias [D], or [G, D] over the last two dimensions, or None."""
     if not torch.compiler.is_compiling():
-        return _launch.native().layer_norm(x, weight, bias, eps)
+        y = _launch.native().layer_norm(x, weight, bias, eps)
+        if y is not None:   # None: fake or wrapped tensors, a mode or a trace
+            return y
     groups = _check(x, weight, bias, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNormFn.apply(x, weight, bias, groups, float(eps))
@@ -66,7 +68,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 
 
 def _check(x, weight, bias, eps) -> int:
-    """The native call's checks, for compiled calls; returns the groups."""
+    """The native call's checks, for compiled and traced calls; returns the groups."""
     if not (math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be finite and not negative")
     if x.ndim < 1 or x.shape[-1] < 1:

@@ -97,7 +97,7 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, tur
 
 
 class _RotaryFn(torch.autograd.Function):
-    """The autograd node of compiled calls; eager calls have theirs in C++."""
+    """The autograd node of compiled and traced calls; eager calls have theirs in C++."""
 
     @staticmethod
     def forward(ctx, q, k, positions, turns, interleaved: bool, magnitude: float):
@@ -122,7 +122,9 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     bf16, fp16 or fp32, any strides with a unit last one; D even, at least the plan's rotary_dim.  The results
     have q's and k's shapes in [B,N,H,D] memory."""
     if not torch.compiler.is_compiling():
-        return _launch.native().rotary_embed(q, k, positions, plan.turns, plan.interleaved, plan.magnitude)
+        turned = _launch.native().rotary_embed(q, k, positions, plan.turns, plan.interleaved, plan.magnitude)
+        if turned is not None:   # None: fake or wrapped tensors, a mode or a trace
+            return turned
     _check(q, k, positions, plan)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryFn.apply(q, k, positions, plan.turns, plan.interleaved, plan.magnitude)
@@ -131,7 +133,7 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
 
 
 def _check(q, k, positions, plan) -> None:
-    """The native call's checks, for compiled calls."""
+    """The native call's checks, for compiled and traced calls."""
     if q.ndim != 4:
         raise ValueError(f"q must be [B,H,N,D], got {tuple(q.shape)}")
     B, H, N, D = q.shape

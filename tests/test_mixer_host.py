@@ -355,6 +355,65 @@ def test_forward_mode_derivatives_are_refused(pkg):
         torch.func.jvp(pkg.layer_norm, (base["x"],), (base["x"],))
 
 
+def test_fake_tensors_give_shapes(pkg):
+    """Tensors without memory, with and without gradients: the custom ops' shapes, as the other operators of the package
+    give them, and no launch."""
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    plan = pkg.rotary_plan(64, device="cpu")
+    with FakeTensorMode():
+        make = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device="cuda")   # noqa: E731
+        for grad in (False, True):
+            q, k = make(2, 4, 70, 64, dtype=torch.bfloat16), make(2, 2, 70, 64, dtype=torch.bfloat16)
+            x, w, lg = make(3, 4, 8, dtype=torch.float16), make(4, 8), make(4)
+            for t in (q, k, x, w, lg):
+                t.requires_grad_(grad)
+            plan.turns = make(32, dtype=torch.int64)
+            qr, kr = pkg.rotary_embed(q, k, torch.arange(70, device="cuda"), plan)
+            alone, none = pkg.rotary_embed(q, None, torch.arange(70, device="cuda"), plan)
+            o, state = pkg.linear_attention(qr, kr, kr, lg, return_state=True)
+            y = pkg.layer_norm(x, w, w)
+            assert none is None and alone.shape == q.shape
+            assert qr.shape == q.shape and kr.shape == k.shape and o.shape == q.shape and y.shape == x.shape
+            assert state.shape == (2, 4, 64, 64) and state.dtype == torch.float32
+            assert o.transpose(1, 2).is_contiguous() and qr.transpose(1, 2).is_contiguous()
+            assert all(isinstance(t, FakeTensor) and t.requires_grad == grad for t in (qr, kr, o, state, y))
+        pool, rows = make(5, 4, 64, 64), make(3, 4, 64, dtype=torch.bfloat16)
+        out = make(3, 4, 64, dtype=torch.bfloat16)
+        with torch.no_grad():
+            one = pkg.linear_attention_step(rows, rows, rows, lg, pool, slots=make(3, dtype=torch.int64))
+            assert one.shape == (3, 4, 64) and one.dtype == torch.bfloat16
+            assert pkg.linear_attention_step(rows, rows, rows, lg, pool, new_state=make(5, 4, 64, 64), out=out) is out
+            for bad in (make(3, 4, 64), make(2, 4, 64, dtype=torch.bfloat16)):
+                with pytest.raises(ValueError, match="out must be"):
+                    pkg.linear_attention_step(rows, rows, rows, lg, pool, out=bad)
+        with pytest.raises(ValueError, match="floating"):
+            pkg.layer_norm(x, make(8, dtype=torch.int32))
+
+
+def test_traces_hold_the_operators(pkg):
+    """make_fx records the custom ops, not an allocation that nothing writes."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def layer(x, w, lg):
+        y = pkg.layer_norm(x, w)
+        q, k = pkg.rotary_embed(y.transpose(1, 2), None, positions, plan)[0], y.transpose(1, 2)
+        o, state = pkg.linear_attention(q, k, k, lg, return_state=True)
+        with torch.no_grad():
+            one = pkg.linear_attention_step(q[:, :, 0], k[:, :, 0], k[:, :, 0], lg, state.clone())
+        return [o, one]
+
+    plan = pkg.rotary_plan(64, device="cpu")
+    with FakeTensorMode():
+        plan.turns, positions = torch.empty(32, dtype=torch.int64, device="cuda"), torch.arange(70, device="cuda")
+        args = (torch.empty(2, 70, 4, 64, device="cuda", dtype=torch.bfloat16), torch.empty(4, 64, device="cuda"),
+                torch.empty(4, device="cuda"))
+        graph = make_fx(layer)(*args)
+    seen = [str(n.target) for n in graph.graph.nodes]
+    for name in ("layer_norm_fwd", "rotary", "linear_attention_fwd", "linear_attention_step_"):
+        assert seen.count(f"dwarf.{name}.default") == 1, (name, seen)
+
+
 def test_rotary_plan_frequencies(pkg):
     """Turns are the nearest 2^-64 fractions, and each scaling gives its formula's frequencies."""
     plan = pkg.rotary_plan(64, device="cpu")
