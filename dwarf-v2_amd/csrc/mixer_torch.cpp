@@ -14,12 +14,12 @@
 #include <pybind11/stl.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "dwarf_mixer.h"
@@ -734,6 +734,63 @@ Tensor attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, cons
   return out;
 }
 
+// The step's tensors in memory, in bytes: n0 rows of n1 runs of `run` bytes ([S,H,64], or a pool whose slots are whole).
+struct Runs {
+  int64_t at, n0, s0, n1, s1, run;
+  explicit Runs(const Tensor& t) {
+    const bool pool = t.dim() == 4;
+    const int64_t es = static_cast<int64_t>(t.element_size());
+    at = static_cast<int64_t>(reinterpret_cast<intptr_t>(t.const_data_ptr()));
+    n0 = t.size(0), s0 = t.stride(0) * es;
+    n1 = pool ? 1 : t.size(1), s1 = pool ? 0 : t.stride(1) * es;
+    run = (pool ? t.size(1) * kHd * kHd : kHd) * es;
+  }
+  int64_t end() const { return at + (n0 - 1) * s0 + (n1 - 1) * s1 + run; }
+};
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b != 0 && a < 0); }
+
+// Whether some n in [low, high] has n step + e inside (-behind, ahead).
+bool steps_into(int64_t low, int64_t high, int64_t step, int64_t e, int64_t behind, int64_t ahead) {
+  if (step == 0) return -behind < e && e < ahead;
+  low = std::max(low, -floor_div(e + behind - 1, step));
+  high = std::min(high, floor_div(ahead - 1 - e, step));
+  return low <= high;
+}
+
+// Whether a byte belongs to both.  Rows of one stride, which slices of a fused buffer have, need no loop over them.
+bool meet(Runs a, Runs b) {
+  if (a.end() <= b.at || b.end() <= a.at) return false;
+  if (a.s0 == 0) a.n0 = 1;   // expanded: one row, one head
+  if (b.s0 == 0) b.n0 = 1;
+  if (a.s1 == 0) a.n1 = 1;
+  if (b.s1 == 0) b.n1 = 1;
+  if (a.n0 > 1 && b.n0 > 1 && a.s0 != b.s0) {
+    Runs row = a;
+    row.n0 = 1;
+    for (int64_t i = 0; i < a.n0; ++i, row.at += a.s0)
+      if (meet(row, b)) return true;
+    return false;
+  }
+  const int64_t s0 = b.n0 > 1 ? b.s0 : a.s0, d = b.at - a.at;
+  auto heads = [&](int64_t e) { return steps_into(1 - a.n0, b.n0 - 1, s0, e, b.run, a.run); };
+  if (a.s1 == b.s1 || a.n1 == 1 || b.n1 == 1) {
+    const int64_t s1 = b.n1 > 1 ? b.s1 : a.s1;
+    for (int64_t m = 1 - a.n1; m < b.n1; ++m)
+      if (heads(d + m * s1)) return true;
+    return false;
+  }
+  for (int64_t i = 0; i < a.n1; ++i)
+    for (int64_t j = 0; j < b.n1; ++j)
+      if (heads(d + j * b.s1 - i * a.s1)) return true;
+  return false;
+}
+bool meets_itself(const Runs& a) {
+  if ((a.n0 > 1 && a.s0 < a.run) || (a.n1 > 1 && a.s1 < a.run)) return true;
+  for (int64_t m = 1; m < a.n1; ++m)   // the other sign is the same pair
+    if (steps_into(1 - a.n0, a.n0 - 1, a.s0, m * a.s1, a.run, a.run)) return true;
+  return false;
+}
+
 void check_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
                 const OptTensor& slots, const OptTensor& new_state, const OptTensor& out) {
   TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "q, k and v must be [S,H,64], got ", q.sizes(), ", ",
@@ -753,10 +810,8 @@ void check_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
     for (const auto& [name, t] : {std::make_pair("out", &*out), std::make_pair("q", &q), std::make_pair("k", &k),
                                   std::make_pair("v", &v), std::make_pair("state", &state),
                                   std::make_pair("new_state", new_state ? &*new_state : &state)}) {
-      const bool shared = t == &*out ? at::has_internal_overlap(*t) == at::MemOverlap::Yes
-                                     : at::get_overlap_status(*out, *t) != at::MemOverlapStatus::No &&
-                                           at::get_overlap_status(*out, *t) != at::MemOverlapStatus::TooHard;
-      TORCH_CHECK_VALUE(!shared, "out shares memory with ", name);
+      if (!out->numel() || !t->numel()) continue;
+      TORCH_CHECK_VALUE(!(t == &*out ? meets_itself(Runs(*t)) : meet(Runs(*out), Runs(*t))), "out shares memory with ", name);
     }
   check_cuda(q);
   check_beside("k", k, q);

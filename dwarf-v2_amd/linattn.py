@@ -107,7 +107,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     (slot s where slots is None); its new state is written to the same slot of ``new_state``, or of ``state`` itself
     where that is None.  Slots outside [0, P) mark rows that pad the batch: no state is touched, their output
     is zero.  Rows that share a slot are consecutive tokens of its sequence, in row order.  ``out``: where to write
-    the result (eager calls).  No gradients."""
+    the result (eager calls), in memory of its own: it may lie between the rows of the others, but not on them.  No
+    gradients."""
     if not torch.compiler.is_compiling():
         done = _launch.native().linear_attention_step(q, k, v, log_decay, state, slots, new_state, scale, out)
         if done is not None:   # None: fake or wrapped tensors, a mode or a trace

@@ -127,7 +127,8 @@ int dwarf_linear_attention_bwd(const dwarf_linear_attention_bwd_args* args, dwar
  * contiguous): row s takes slot slots[s] (s itself where slots is NULL), S' = g S + k v^T, out = scale q S'.  The
  * new state goes to new_state (the pool itself, or another one of the same slot stride).  A slot outside
  * [0, pool) marks a row that pads the batch: no state is touched and its output is zero.  Rows of one slot are
- * consecutive tokens of its sequence, in row order.  q, out [S,H,64], k, v [S,H_kv,64].
+ * consecutive tokens of its sequence, in row order.  q, out [S,H,64], k, v [S,H_kv,64]; out shares no memory with
+ * the others.
  */
 typedef struct {
   int32_t S, H, H_kv, pool, head_dim;

@@ -213,6 +213,50 @@ def test_step_refuses_out_in_its_inputs_memory(pkg):
         pkg.linear_attention_step(q, k, v, torch.zeros(4), pool, new_state=other, out=other.reshape(-1)[:768].view(3, 4, 64))
 
 
+def test_step_refuses_out_among_rows_that_are_read(pkg):
+    """Strided slices of one buffer: out is refused where it holds an element of another tensor, or one of its own twice,
+    and accepted between them.  The truth is the set of the elements."""
+    import random
+    rng = random.Random(3)
+    buf, pool, lg = torch.zeros(1 << 15), torch.zeros(2, 4, 64, 64), torch.zeros(4)
+    at = (buf.data_ptr() // 4) % 4   # keeps every view 16-byte aligned
+
+    def view(H, S=3):
+        s1 = rng.choice([64, 64, 128, 192, 256, 72, 0, 20])
+        s0 = rng.choice([64 * 12, 64 * 12, 64 * 12, 64 * 4, 64, 1024, 0, 200])
+        return buf.as_strided((S, H, 64), (s0, s1, 1), (4 - at) % 4 + 4 * rng.randint(0, 256))
+
+    def elements(t):
+        S, H, _ = t.shape
+        return [t.storage_offset() + s * t.stride(0) + h * t.stride(1) + d for s in range(S) for h in range(H) for d in range(64)]
+
+    seen = set()
+    for _ in range(600):
+        S = rng.choice([1, 2, 3])
+        tensors = dict(out=view(4, S), q=view(4, S), k=view(2, S), v=view(2, S))
+        own = elements(tensors["out"])
+        if len(set(own)) < len(own):
+            want = "out"
+        else:
+            want = next((n for n in "qkv" if not set(own).isdisjoint(elements(tensors[n]))), None)
+        seen.add(want)
+        with pytest.raises((ValueError, RuntimeError)) as e:
+            pkg.linear_attention_step(tensors["q"], tensors["k"], tensors["v"], lg, pool, slots=torch.zeros(S, dtype=torch.int32),
+                                      out=tensors["out"])
+        text = str(e.value)
+        assert (f"shares memory with {want}" if want else "device tensors") in text, (want, text, tensors)
+    assert seen == {"out", "q", "k", "v", None}
+    fused = torch.zeros(3, 10, 64)   # out, q, k and v side by side in each row: allowed
+    with pytest.raises(RuntimeError, match="device tensors"):
+        pkg.linear_attention_step(fused[:, 4:8], fused[:, 8:9], fused[:, 9:], lg, torch.zeros(3, 4, 64, 64), out=fused[:, :4])
+    layers = torch.zeros(3, 2, 4, 64, 64)   # out in a slot of the pool, and between the pool's slots
+    rows = torch.zeros(3, 4, 64)
+    for layer, want in ((0, "shares memory with state"), (1, "device tensors")):
+        out = layers[:, layer, 0, :4]
+        with pytest.raises((ValueError, RuntimeError), match=want):
+            pkg.linear_attention_step(rows, rows, rows, lg, layers[:, 0], out=out)
+
+
 def test_segment_rule_is_the_librarys(pkg, lib):
     for B in (1, 2, 3, 15, 20, 64):
         for H in (1, 6, 8, 32):
