@@ -69,7 +69,8 @@ __device__ __forceinline__ float la_log2_decay(const LaGeom& gm, int h) {
 }
 __device__ __forceinline__ float la_power(float lg, int n) { return __builtin_amdgcn_exp2f(lg * static_cast<float>(n)); }
 
-// The terms of dlog_decay nearly cancel: their sums over threads, segments and sequences are kept in 64 bits.
+// The terms of dlog_decay nearly cancel.  A lane's share of one chunk is formed in fp32; its weight and every sum behind it
+// (over a lane's chunks, lanes, segments and sequences) are kept in 64 bits: two instructions a chunk and lane.
 __device__ __forceinline__ double wave_sum_f64(double x) {
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) x += __shfl_xor(x, o);
@@ -502,7 +503,7 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRowsCall<TO> call
           po[(t + ii) * o2 + 16 * ct + c] = from_f32<TO>(v + o[ct][r]);
           if (call.dot) s = fmaf(v, to_f32(pd[(t + ii) * D_.s2 + 16 * ct + c]), s);
         }
-        total += tau * s;
+        total = fma(static_cast<double>(tau), static_cast<double>(s), total);
       }
     }
     la_update<kRowStride>(sB, sC, s_w, la_power(lg, n), us, M);
@@ -1030,7 +1031,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
   };
   const float* tables = reinterpret_cast<const float*>(smem + (4 + kParts) * kTileBytes);   // written before the first barrier
   state_weights_put(lg, live(chunks - 1), reinterpret_cast<float*>(smem + (4 + kParts) * kTileBytes));
-  float total = 0.f;
+  double total = 0.;
   if (keeps) {
     f32x4 M[4], L[4];
     state_enter(enter, true, gm, it, lg, M);
@@ -1079,7 +1080,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
           const uint2 x2 = *reinterpret_cast<const uint2*>(sQ + (m.slots ^ 32 * ct) + 2048 * w);
           sum = fmaf(o[ct][0], bf16_lo(x2.x), fmaf(o[ct][1], bf16_hi(x2.x), fmaf(o[ct][2], bf16_lo(x2.y), fmaf(o[ct][3], bf16_hi(x2.y), sum))));
         }
-        total = fmaf(static_cast<float>(i * kChunk + row + 1) - mid, sum, total);   // dead rows of q are zero
+        total = fma(static_cast<double>(static_cast<float>(i * kChunk + row + 1) - mid), static_cast<double>(sum), total);   // dead rows of q are zero
       }
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -1119,7 +1120,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dq_bf16(LaRows Q_, LaRows 
 // keys' side of dlog_decay (see la_dq_bf16), returned by the dk waves.  Without it a chunk's tiles and G's two parts have
 // two LDS buffers each; with it G has three parts, and all have one buffer and a second barrier.
 template <bool KEYS, bool DECAY, typename TO>
-__device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, const LaRows& O_, const LaRows& K_, const LaRows& V_,
+__device__ __forceinline__ double la_dkdv_role(char* smem, const LaRows& Q_, const LaRows& O_, const LaRows& K_, const LaRows& V_,
                                               const LaGeom& gm, const LaItem& it, int t0, int t1,
                                               const float* __restrict__ enter, TO* __restrict__ pr, int64_t stride) {
   constexpr int kParts = DECAY ? 3 : 2;        // of G in LDS
@@ -1156,7 +1157,7 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
   const ScoreWeights sw(lg, gm.scale, true);
   const AdjointWeights wt(lg, gm.scale);
   const float mid = la_mid(t1 - t0).keys;
-  float total = 0.f;
+  double total = 0.;
   fetch(0);
   for (int i = 0; i < chunks; ++i) {
     const int n = live(i);
@@ -1191,7 +1192,7 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
         const uint2 k = *reinterpret_cast<const uint2*>(sK + (m.slots ^ 32 * ct) + 2048 * w);
         sum = fmaf(acc[ct][0], bf16_lo(k.x), fmaf(acc[ct][1], bf16_hi(k.x), fmaf(acc[ct][2], bf16_lo(k.y), fmaf(acc[ct][3], bf16_hi(k.y), sum))));
       }
-      total = fmaf(static_cast<float>(token(i) + row - t0 + 1) - mid, sum, total);   // dead rows of k are zero
+      total = fma(static_cast<double>(static_cast<float>(token(i) + row - t0 + 1) - mid), static_cast<double>(sum), total);   // dead rows of k are zero
     }
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -1212,8 +1213,10 @@ __device__ __forceinline__ float la_dkdv_role(char* smem, const LaRows& Q_, cons
               y = mfma16_bf16(tile_row(sQ, m, tt, 0), tile_row(sK, m, w, 0), y);
               y = mfma16_bf16(tile_row(sQ, m, tt, 1), tile_row(sK, m, w, 1), y);
               const float gap = static_cast<float>(16 * (tt - w) + 4 * g - c);
+              float pairs = 0.f;
 #pragma unroll
-              for (int r = 0; r < 4; ++r) total = fmaf(-(gap + static_cast<float>(r)) * p[4 * hf + r], y[r], total);
+              for (int r = 0; r < 4; ++r) pairs = fmaf((gap + static_cast<float>(r)) * p[4 * hf + r], y[r], pairs);
+              total -= pairs;
             }
           }
         }
@@ -1255,7 +1258,7 @@ __global__ __launch_bounds__(kWideThreads, 4) void la_dkdv_bf16(LaRows Q_, LaRow
   TO *pdk = dk + it.b * k0 + oh * k1, *pdv = dv + it.b * v0 + oh * v1;
   la_zero_rows(pdk, k2, t1 > t0 ? t1 : t0, tend);
   la_zero_rows(pdv, v2, t1 > t0 ? t1 : t0, tend);
-  float total;
+  double total;
   if (uniform(threadIdx.x / kWave) >= 4) total = la_dkdv_role<true, DECAY>(smem, Q_, O_, K_, V_, gm, it, t0, t1, enter, pdk, k2);
   else total = la_dkdv_role<false, DECAY>(smem, Q_, O_, K_, V_, gm, it, t0, t1, enter, pdv, v2);
   if constexpr (DECAY) {
