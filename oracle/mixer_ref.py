@@ -2,6 +2,7 @@
 
 ``linear_attention``: the recurrence S_t = g S_{t-1} + k_t v_t^T, o_t = scale q_t S_t token by token, with
 g = exp(min(log_decay, 0)); ``linear_attention_backward``: its adjoint recurrence, token by token.
+``linear_attention_chunked``: the same in blocks of tokens, for long sequences, its gradients by autograd.
 ``rotary``: each pair as a complex number times exp(i position f).  ``layer_norm`` and its gradients from the formula.
 """
 
@@ -57,6 +58,44 @@ def linear_attention_backward(q, k, v, log_decay, scale, dout, initial=None, len
     dlog = torch.where(log_decay.double() > 0, torch.zeros((), dtype=torch.float64), dlog)
     shared = lambda x: x.reshape(B, Hkv, group, N, D).sum(2)   # noqa: E731
     return dq, shared(dk), shared(dv), dlog, dinitial
+
+
+def linear_attention_chunked(q, k, v, log_decay, scale, dout, initial=None, lengths=None, dstate=None, block=64):
+    """(out, state, (dq, dk, dv, dlog_decay, dinitial), crossing): crossing[b] holds <S, G> per head, the state behind
+    every ``block`` tokens of sequence b (the first one: what enters) times its adjoint."""
+    B, H, N, D = q.shape
+    group = H // k.shape[1]
+    leaves = [x.double().clone().requires_grad_(True) for x in (q, k, v, log_decay)]
+    S0 = (torch.zeros(B, H, D, D, dtype=torch.float64) if initial is None else initial.double().clone()).requires_grad_(True)
+    ql, kl, vl, lgl = leaves
+    lg = lgl.clamp(max=0)[:, None, None]
+    outs, ends, passed = [], [], []
+    for b in range(B):
+        n = N if lengths is None else min(max(int(lengths[b]), 0), N)
+        S, rows, kept = S0[b], [], []
+        for t in range(0, n, block):
+            m = min(block, n - t)
+            S = S * 1.0   # a value of its own, whose gradient is the adjoint here
+            kept.append(S)
+            i = torch.arange(m, dtype=torch.float64)
+            gap = i[:, None] - i[None, :]
+            near = torch.where(gap >= 0, torch.exp(lg * gap.clamp(min=0)), torch.zeros((), dtype=torch.float64))
+            qb, kb, vb = ql[b, :, t:t + m], *(x[b, :, t:t + m].repeat_interleave(group, 0) for x in (kl, vl))
+            rows.append(scale * ((qb @ kb.transpose(1, 2) * near) @ vb + torch.exp(lg * (i[:, None] + 1)) * (qb @ S)))
+            S = torch.exp(lg * m) * S + (kb * torch.exp(lg * (m - 1 - i)[:, None])).transpose(1, 2) @ vb
+        outs.append(torch.cat([*rows, torch.zeros(H, N - n, D, dtype=torch.float64)], 1))
+        ends.append(S)
+        passed.append(kept)
+    out, state = torch.stack(outs), torch.stack(ends)
+    loss = (out * dout.double()).sum() + (0 if dstate is None else (state * dstate.double()).sum())
+    flat = [S for kept in passed for S in kept]
+    grads = torch.autograd.grad(loss, [*leaves, S0, *flat], allow_unused=True)
+    given = [torch.zeros_like(x) if g is None else g for x, g in zip([*leaves, S0], grads)]
+    at, crossing = 5, []
+    for kept in passed:
+        crossing.append([(S.detach() * g).sum((1, 2)) for S, g in zip(kept, grads[at:at + len(kept)])])
+        at += len(kept)
+    return out.detach(), state.detach(), tuple(given), crossing
 
 
 def rotary(x, positions, frequencies, interleaved, magnitude=1.0, inverse=False):

@@ -1,16 +1,86 @@
 """GPU tests of linear_attention over several long segments (256 to 1,024 tokens, up to eight of them and more), which the
-training microbatch, padded prompts and long prompts take.
+training microbatch, padded prompts and long prompts take, against the float64 oracle in blocks.
 
-The segment rule goes by B, H and N alone, so a few live sequences in a batch of empty ones reach every length.
+The segment rule goes by B, H and N alone, so a few live sequences in a batch of empty ones reach every length.  Inputs are
+positive: nothing cancels, every result is as large as its terms, and a wrong weight in any part of dlog_decay shows.
+Bounds: those of test_gpu_linattn.py; dlog_decay adds at most three weights of a segment's tokens times |q.dq|, |k.dk| and
+<S, G> at the segments' borders (exact in float64 here), each term formed in fp32: 400 half steps, two more for each
+segment that a state has passed.  The results are at least 20 bounds large, so that zeros or half weights cannot pass.
 """
+
+import math
 
 import pytest
 import torch
 
-from tests.mixer_cases import DTYPES
-from tests.test_gpu_linattn import HD
+from oracle import mixer_ref
+from tests.mixer_cases import DTYPES, within
+from tests.test_gpu_linattn import FP32, HD, put, slack
 
 pytestmark = pytest.mark.gpu
+
+CASES = [
+    # B, H, Hkv, N, segment, lengths of the live sequences (the others are empty)
+    (16, 8, 8, 1600, 512, [1600, 1537, 1090]),          # four segments; tails of 64, 1 and 66 tokens
+    (15, 8, 2, 2048, 512, [2048, 1500]),                 # the training microbatch's, shared heads
+    (32, 8, 4, 1100, 1024, [1100, 1025]),                # two segments of 1,024, the second with 76 and 1 tokens
+    (56, 8, 8, 1088, 1024, [1088, 1030, 1024]),          # two segments of 1,024; tails of 64, 6 and none
+    (3, 8, 8, 1300, 128, [1300, 1217]),                  # eleven segments: the scan in groups
+    (3, 8, 4, 2600, 256, [2600, 2497, 300]),
+    (6, 8, 8, 5200, 512, [5184, 3333]),
+    (7, 8, 2, 9300, 1024, [9280, 9000]),                 # ten segments of 1,024, a tail of 64
+]
+
+
+def positive(B, H, Hkv, N, dtype, lengths, seed):
+    g = torch.Generator().manual_seed(seed)
+    live = len(lengths)
+
+    def heads(n):
+        x = torch.zeros(B, N, n, HD, dtype=dtype)
+        x[:live] = (torch.rand(live, N, n, HD, generator=g) * 0.9 + 0.1).to(dtype)
+        return x.transpose(1, 2)
+
+    x = dict(q=heads(H), k=heads(Hkv), v=heads(Hkv), dout=heads(H))
+    x["log_decay"] = torch.log1p(-torch.exp(-torch.linspace(math.log(8.0), math.log(512.0), H)))
+    x["initial"], x["dstate"] = torch.rand(B, H, HD, HD, generator=g), torch.rand(B, H, HD, HD, generator=g)
+    x["lengths"] = torch.tensor([*lengths] + [0] * (B - live), dtype=torch.int32)
+    return x
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("B,H,Hkv,N,seg,lengths", CASES)
+def test_long_segments(pkg, device, B, H, Hkv, N, seg, lengths, dtype):
+    assert pkg.linattn.segment_tokens(B, H, N) == seg
+    x = positive(B, H, Hkv, N, dtype, lengths, seed=N)
+    d = put(x, device)
+    names = ("q", "k", "v", "log_decay", "initial")
+    for n in names:
+        d[n].requires_grad_(True)
+    out, state = pkg.linear_attention(d["q"], d["k"], d["v"], d["log_decay"], initial_state=d["initial"], lengths=d["lengths"],
+                                      return_state=True)
+    got = dict(zip(names, torch.autograd.grad((out, state), [d[n] for n in names], (d["dout"], d["dstate"]))))
+    live = len(lengths)
+    rows = {n: x[n][:live] for n in ("q", "k", "v", "dout", "initial", "dstate")}
+    want, wstate, grads, crossing = mixer_ref.linear_attention_chunked(
+        rows["q"], rows["k"], rows["v"], x["log_decay"], 0.125, rows["dout"], rows["initial"], lengths, rows["dstate"])
+    grads = dict(zip(names, grads))
+    more = -(-N // seg) * 2 * 2.0 ** -24
+    # positive inputs: the results are their terms
+    within(out[:live], want, want, dtype, slack(dtype) + more)
+    within(state[:live], wstate, wstate, torch.float32, FP32 + more)
+    for n in ("q", "k", "v"):
+        within(got[n][:live], grads[n], grads[n], dtype, slack(dtype) + more)
+    within(got["initial"][:live], grads["initial"], grads["initial"], torch.float32, FP32 + more)
+    # the empty sequences: nothing but the state that goes through
+    assert not any(bool(t[live:].any()) for t in (out, got["q"], got["k"], got["v"]))
+    assert torch.equal(state[live:], d["initial"][live:]) and torch.equal(got["initial"][live:], d["dstate"][live:])
+    flow = (rows["q"].double() * grads["q"]).sum((0, 2, 3)) + (
+        rows["k"].double() * grads["k"]).sum((0, 2, 3)).repeat_interleave(H // Hkv) + sum(
+            c for kept in crossing for c in kept[::seg // 64])
+    terms = seg * flow
+    assert bool((20 * (FP32 + more) * terms < grads["log_decay"]).all())
+    within(got["log_decay"], grads["log_decay"], terms, torch.float32, FP32 + more)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)

@@ -2,6 +2,7 @@
 
 import math
 
+import pytest
 import torch
 
 from oracle import mixer_ref
@@ -85,3 +86,25 @@ def test_layer_norm_gradients_match_autograd():
         for a, want in zip(mixer_ref.layer_norm_backward(dy, x.detach(), w.detach(), 1e-3),
                            torch.autograd.grad(y, (x, w, b), dy)):
             torch.testing.assert_close(a, want)
+
+
+@pytest.mark.parametrize("lengths,state", [(None, True), ([150, 64, 0], True), ([65, 1, 149], False)])
+def test_chunked_attention_is_the_recurrence(lengths, state):
+    """Outputs, states and gradients in blocks of tokens, and the terms that cross a block's border."""
+    g = torch.Generator().manual_seed(5)
+    B, H, Hkv, N, D = 3, 4, 2, 150, 8
+    q, dout = (torch.randn(B, H, N, D, generator=g) for _ in range(2))
+    k, v = (torch.randn(B, Hkv, N, D, generator=g) for _ in range(2))
+    lg = torch.tensor([-0.5, -0.01, 0.0, 0.3])
+    S0, dS = (torch.randn(B, H, D, D, generator=g) for _ in range(2))
+    dS = dS if state else None
+    out, end, grads, crossing = mixer_ref.linear_attention_chunked(q, k, v, lg, 0.3, dout, S0, lengths, dS)
+    want = mixer_ref.linear_attention(q, k, v, lg, 0.3, S0, lengths)
+    wgrads = mixer_ref.linear_attention_backward(q, k, v, lg, 0.3, dout, S0, lengths, dS)
+    for a, b in zip((out, end, *grads), (*want, *wgrads)):
+        torch.testing.assert_close(a, b, rtol=1e-11, atol=1e-11)
+    for b in range(B):
+        n = N if lengths is None else lengths[b]
+        assert len(crossing[b]) == -(-n // 64)
+        if n:   # what enters times its adjoint
+            torch.testing.assert_close(crossing[b][0], (S0[b].double() * grads[4][b]).sum((1, 2)), rtol=1e-11, atol=1e-11)
