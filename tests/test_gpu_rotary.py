@@ -174,3 +174,37 @@ def test_graph_and_compile(pkg, device):
         got = [t.clone() for t in outs]
         assert all(torch.equal(a, b) for a, b in zip(got, pkg.rotary_embed(q, k, pos, plan))), rep
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_angles_near_quarter_turns(pkg, device, dtype, interleaved):
+    """Sines and cosines that are nearly 0, of angles around every quarter turn: in fp32 as exact as around angle 0.
+
+    Exact: the plan's integer turns, the nearest quarter taken off in integers.  Bound in fp32: 2^-32 of a turn is cut off,
+    and relative to the value half a step for the angle, 4 for sine and cosine, 2 for the products; 16-bit results add the
+    hardware's 2^-20 and their own rounding."""
+    import math
+    from fractions import Fraction
+    g = torch.Generator().manual_seed(9)
+    near = torch.tensor([q / 4 + s * d for q in range(-3, 5) for s in (1, -1) for d in (3.0e-7, 2.87e-6, 1.3e-4, 0.011, 0.1249)])
+    f = 2 * math.pi * (near.double() + 1e-9 * torch.rand(near.numel(), generator=g, dtype=torch.float64))
+    plan = pkg.rotary_plan(2 * f.numel(), inverse_frequencies=f, interleaved=interleaved, device=device)
+    n = f.numel()
+    x = torch.zeros(1, 1, 3, 2 * n)
+    (x[..., 0::2] if interleaved else x[..., :n]).fill_(1.0)   # pairs (1, 0): the results are the cosine and the sine
+    positions = torch.tensor([0, 1, 1023])
+    y = pkg.rotary_embed(x.to(device=device, dtype=dtype), None, positions.to(device), plan)[0].cpu().double()
+    c, s = (y[0, 0, :, 0::2], y[0, 0, :, 1::2]) if interleaved else (y[0, 0, :, :n], y[0, 0, :, n:])
+    step = {torch.float32: 8 * 2.0 ** -24, torch.bfloat16: 2.0 ** -8 + 8 * 2.0 ** -24, torch.float16: 2.0 ** -11 + 8 * 2.0 ** -24}[dtype]
+    floor = 2 * math.pi * 2.0 ** -32 + (0 if dtype == torch.float32 else 2.0 ** -20 + (2.0 ** -25 if dtype == torch.float16 else 0))
+    for i, p in enumerate(positions.tolist()):
+        for j, t in enumerate(plan.turns.tolist()):
+            at = Fraction(p * t % 2 ** 64, 2 ** 64)
+            quarter = round(4 * at)
+            rest = float(at - Fraction(quarter, 4)) * 2 * math.pi
+            sn, cs = math.sin(rest), math.cos(rest)
+            for _ in range(quarter % 4):
+                sn, cs = cs, -sn
+            for got, want in ((float(s[i, j]), sn), (float(c[i, j]), cs)):
+                assert abs(got - want) <= floor + step * abs(want), (p, float(at), got, want)
