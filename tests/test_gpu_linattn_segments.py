@@ -29,6 +29,8 @@ CASES = [
     (3, 8, 4, 2600, 256, [2600, 2497, 300]),
     (6, 8, 8, 5200, 512, [5184, 3333]),
     (7, 8, 2, 9300, 1024, [9280, 9000]),                 # ten segments of 1,024, a tail of 64
+    (1, 2, 1, 9001, 64, [9001]),                         # 141 segments of one chunk: the scan in two passes
+    (1, 2, 2, 16600, 128, [16600]),                      # 130 of two chunks
 ]
 
 
