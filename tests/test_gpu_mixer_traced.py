@@ -196,3 +196,31 @@ def test_forward_mode_derivatives_are_refused(pkg, device, x):
             with pytest.raises(RuntimeError, match="forward mode"):
                 torch.autograd.grad(outs[i], [t[n] for n in (LEAVES[:5] if i < 4 else LEAVES[5:])],
                                     fw.make_dual(up, up.clone()), retain_graph=True)
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=str)
+def test_compiled_step_matches_eager(pkg, device, x, index):
+    """linear_attention_step in a compiled call: the pool in place, and from one pool into another."""
+    rows = [x[n][:, :, 5] for n in ("q", "k", "v")]
+    slots = torch.tensor([3, -1], dtype=index, device=device)
+    start = torch.randn(5, H, HD, HD, generator=torch.Generator().manual_seed(3)).to(device)
+
+    def in_place(q, k, v, lg, pool, slots):
+        out = pkg.linear_attention_step(q, k, v, lg, pool, slots=slots)
+        return out * 2, pool.sum()
+
+    def across(q, k, v, lg, pool, new, slots):
+        return pkg.linear_attention_step(q, k, v, lg, pool, slots=slots, new_state=new, scale=0.5)
+
+    compile_ = lambda f: torch.compile(f, backend="aot_eager", fullgraph=True)   # noqa: E731
+    results = []
+    for f, g in ((in_place, across), (compile_(in_place), compile_(across))):
+        pool, old, new = start.clone(), start.clone(), torch.zeros_like(start)
+        for _ in range(2):
+            a, total = f(*rows, x["log_decay"], pool, slots)
+        b = g(*rows, x["log_decay"], old, new, slots)
+        results.append([a, total, pool, b, old, new])
+    same(*results)
+    assert torch.equal(results[0][4], start) and not torch.equal(results[0][2], start)
+    with pytest.raises(Exception, match="torch.compile"):
+        compile_(lambda o: pkg.linear_attention_step(*rows, x["log_decay"], start, slots=slots, out=o))(torch.empty_like(rows[0]))
