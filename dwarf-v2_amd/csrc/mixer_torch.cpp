@@ -119,9 +119,10 @@ Tensor empty_like_dtype(at::IntArrayRef shape, const Tensor& like, at::ScalarTyp
   return at::empty(shape, like.options().dtype(dtype));
 }
 Tensor empty_f32(at::IntArrayRef shape, const Tensor& like) { return empty_like_dtype(shape, like, at::kFloat); }
-// An empty [B,H,N,D] tensor in [B,N,H,D] memory.
+// An empty [B,H,N,D] tensor in [B,N,H,D] memory; no view, which made without gradients could not be changed in place with them.
 Tensor token_major(int64_t B, int64_t H, int64_t N, int64_t D, const Tensor& like) {
-  return at::empty({B, N, H, D}, like.options()).transpose(1, 2);
+  const int64_t row = std::max<int64_t>(H, 1) * D;
+  return at::empty_strided({B, H, N, D}, {std::max<int64_t>(N, 1) * row, D, row, 1}, like.options());
 }
 Tensor workspace(size_t nbytes, const Tensor& like) {
   return nbytes ? empty_like_dtype({static_cast<int64_t>(nbytes)}, like, at::kByte) : Tensor();

@@ -224,3 +224,15 @@ def test_compiled_step_matches_eager(pkg, device, x, index):
     assert torch.equal(results[0][4], start) and not torch.equal(results[0][2], start)
     with pytest.raises(Exception, match="torch.compile"):
         compile_(lambda o: pkg.linear_attention_step(*rows, x["log_decay"], start, slots=slots, out=o))(torch.empty_like(rows[0]))
+
+
+def test_results_of_calls_without_gradients_are_tensors_of_their_own(pkg, device, x):
+    """What a call under no_grad returns may be changed in place with gradients on, as any operator's result may."""
+    with torch.no_grad():
+        results = calls(pkg, x)
+    gate = torch.full((), 0.5, device=device, requires_grad=True)
+    for t in results:
+        assert not t._is_view()
+        half = t * 0.5
+        t.mul_(gate)
+        assert t.requires_grad and torch.equal(t.detach(), half)
