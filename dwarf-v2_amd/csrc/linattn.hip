@@ -28,10 +28,10 @@
 //
 // Least traffic is one read of q, k, v and one write of o (backward: q, k, v,
 // do read, dq, dk, dv written); two passes read k and v twice.  Measured in
-// bf16: B1 N65536 H8, 268 MB at least and 403 MB here, 102 us of launches (rows
-// 57, local 38, scan 6.5: 3.9 TB/s); training at B15 N2048 H8 (346 MB at least,
-// 566 MB here), 151 us: local 23.5, rows 28.6, dq 43.4, scan 6.5, dk and dv 44.5,
-// dlog_decay 4.  The rows, dq and dk/dv are bound by a CU's issue slots as much
+// bf16: B1 N65536 H8, 268 MB at least and 403 MB here, 101 us of launches (rows
+// 55, local 39, scan 6.6: 4.0 TB/s); training at B15 N2048 H8 (346 MB at least,
+// 566 MB here), 148 us: local 23.9, rows 28.7, dq 41.8, scan 6.5, dk and dv 43.4,
+// dlog_decay 3.9.  The rows, dq and dk/dv are bound by a CU's issue slots as much
 // as by memory: with k and v from the L2 and nothing stored, the rows of the
 // long prompt still take 41 us.
 #include <type_traits>
@@ -362,9 +362,11 @@ struct LaRowsCall {
 };
 
 // out_i = intra sum_j W_ij (A_i.B_j) C_j + cs W_i A_i M over a segment's chunks, M updated behind each (in front, in
-// reverse); in fp32 throughout, for fp32 and fp16 rows (fp16 parts of a state would overflow, and bf16 parts of fp16 rows
-// would double the tiles and the products; B15 N2048 H8 in fp16: forward 124 us, backward 351).  Bound by the fp32 matrix
-// rate, of which it reaches half: 232 instructions of 32 cycles a wave and chunk, 46 of 92 us.
+// reverse); in fp32 throughout, for fp32 and fp16 rows (the fp16 matrix instructions would multiply fp16 rows exactly, but
+// what is formed here, scores and states, fits fp16's range only after a power of two for each tile; that is not built, and
+// bf16 parts of fp16 rows would double the tiles and the products).  B15 N2048 H8, forward and backward: 124 and 343 us in
+// fp16, 133 and 396 in fp32.  Bound by the fp32 matrix rate, of which the forward's rows reach half: 232 instructions of 32
+// cycles a wave and chunk, 46 of 92 us.
 // leave: where the state behind the last token goes (NULL: nowhere, or the scan has written it).
 // dot, forward: sum tau D_i.(out_i's part that comes from M); in reverse the same less (i - j) times each pair's share
 // within a chunk, W_ij (A_i.B_j) (D_i.C_j).  blockIdx.y picks the call (dv and dk go in one launch).
@@ -526,14 +528,16 @@ __global__ __launch_bounds__(kLaThreads) void la_rows_kernel(LaRowsCall<TO> call
 // (weighted scores, the state, weighted keys) is split into bf16 parts before it meets the matrix cores, two parts
 // (2^-17 relative) where the result is rounded to bf16 anyway and three (2^-24, fp32 itself) where it goes into the
 // state, so that no intermediate rounding is coarser than the output's.  The sums are bound by memory, and the matrix
-// cores have the room: at most 28 instructions a wave and chunk on average, busy a third of the time.
+// cores have the room, busy a third of the time: instructions of a wave and chunk, on average over the waves, 28 in the
+// forward's rows, 37 in dq and 41 in dk and dv, with dlog_decay 44 and 52.
 //
 // LDS holds tiles as 64 rows of 128 bytes; 16-byte piece p of row r sits at piece p ^ tile_key(r).  Of the 4,096 keys that
-// are linear in a row's four low bits this is one of those without bank conflicts in all five accesses: whole pieces read
-// down 16 rows, and written along a row, 8-byte halves read and written down 16 rows, and the transposed reads of four
-// rows.  (The lanes that one cycle of a 16-byte read serves are not consecutive ones; measured cycles for 1,024
-// instructions of a workgroup, without and with the usual two-way conflicts: 4,160 and 8,252 for whole pieces read, 8,324
-// and 16,472 for halves written.)
+// are linear in a row's four low bits this is one of the best: no bank conflicts in whole pieces read down 16 rows and
+// written along a row, in 8-byte halves read down 16 rows and in the transposed reads of four rows; the state's 8-byte
+// halves written down 16 rows (state_put) take 8 cycles for the 4 of consecutive addresses, which is all of the conflicts
+// that SQ_LDS_BANK_CONFLICT shows, 10 to 13% of the LDS's busy cycles.  (The lanes that one cycle of a 16-byte read serves
+// are not consecutive ones; measured cycles for 1,024 instructions of a workgroup, with this key and with twice the
+// conflicts: 4,160 and 8,252 for whole pieces read, 8,324 and 16,472 for halves written.)
 // Scores are formed transposed (rows: the other side's tokens): a lane then holds four consecutive tokens of one own
 // row, which is the next product's operand as it stands.  Its tokens are slots in the order 4 g + e, 16 + 4 g + e of
 // each 32 (g the lane's group of 16), and a transposed read of four rows gives the other operand in the same order.
