@@ -50,39 +50,64 @@ def positive(B, H, Hkv, N, dtype, lengths, seed):
     return x
 
 
-@pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("B,H,Hkv,N,seg,lengths", CASES)
-def test_long_segments(pkg, device, B, H, Hkv, N, seg, lengths, dtype):
+def check(pkg, device, B, H, Hkv, N, seg, lengths, dtype, enters, leaves, dinitial=True):
+    """Forward and gradients of positive inputs; enters, leaves: with a state in front and a gradient of the one behind;
+    dinitial: with the gradient of the state that enters."""
     assert pkg.linattn.segment_tokens(B, H, N) == seg
     x = positive(B, H, Hkv, N, dtype, lengths, seed=N)
+    if not enters:
+        x["initial"] = None
     d = put(x, device)
-    names = ("q", "k", "v", "log_decay", "initial")
+    names = ["q", "k", "v", "log_decay"] + (["initial"] if enters and dinitial else [])
     for n in names:
         d[n].requires_grad_(True)
     out, state = pkg.linear_attention(d["q"], d["k"], d["v"], d["log_decay"], initial_state=d["initial"], lengths=d["lengths"],
                                       return_state=True)
-    got = dict(zip(names, torch.autograd.grad((out, state), [d[n] for n in names], (d["dout"], d["dstate"]))))
+    outs, ups = ((out, state), (d["dout"], d["dstate"])) if leaves else ((out,), (d["dout"],))
+    got = dict(zip(names, torch.autograd.grad(outs, [d[n] for n in names], ups)))
     live = len(lengths)
-    rows = {n: x[n][:live] for n in ("q", "k", "v", "dout", "initial", "dstate")}
+    rows = {n: None if x[n] is None else x[n][:live] for n in ("q", "k", "v", "dout", "initial", "dstate")}
     want, wstate, grads, crossing = mixer_ref.linear_attention_chunked(
-        rows["q"], rows["k"], rows["v"], x["log_decay"], 0.125, rows["dout"], rows["initial"], lengths, rows["dstate"])
-    grads = dict(zip(names, grads))
+        rows["q"], rows["k"], rows["v"], x["log_decay"], 0.125, rows["dout"], rows["initial"], lengths,
+        rows["dstate"] if leaves else None)
+    grads = dict(zip(("q", "k", "v", "log_decay", "initial"), grads))
     more = -(-N // seg) * 2 * 2.0 ** -24
     # positive inputs: the results are their terms
     within(out[:live], want, want, dtype, slack(dtype) + more)
     within(state[:live], wstate, wstate, torch.float32, FP32 + more)
     for n in ("q", "k", "v"):
         within(got[n][:live], grads[n], grads[n], dtype, slack(dtype) + more)
-    within(got["initial"][:live], grads["initial"], grads["initial"], torch.float32, FP32 + more)
+    if "initial" in got:
+        within(got["initial"][:live], grads["initial"], grads["initial"], torch.float32, FP32 + more)
     # the empty sequences: nothing but the state that goes through
     assert not any(bool(t[live:].any()) for t in (out, got["q"], got["k"], got["v"]))
-    assert torch.equal(state[live:], d["initial"][live:]) and torch.equal(got["initial"][live:], d["dstate"][live:])
+    assert torch.equal(state[live:], d["initial"][live:]) if enters else not bool(state[live:].any())
+    if "initial" in got:
+        assert torch.equal(got["initial"][live:], d["dstate"][live:]) if leaves else not bool(got["initial"][live:].any())
     flow = (rows["q"].double() * grads["q"]).sum((0, 2, 3)) + (
         rows["k"].double() * grads["k"]).sum((0, 2, 3)).repeat_interleave(H // Hkv) + sum(
             c for kept in crossing for c in kept[::seg // 64])
     terms = seg * flow
     assert bool((20 * (FP32 + more) * terms < grads["log_decay"]).all())
     within(got["log_decay"], grads["log_decay"], terms, torch.float32, FP32 + more)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("B,H,Hkv,N,seg,lengths", CASES)
+def test_long_segments(pkg, device, B, H, Hkv, N, seg, lengths, dtype):
+    check(pkg, device, B, H, Hkv, N, seg, lengths, dtype, True, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("enters,leaves", [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize("B,H,Hkv,N,seg,lengths", [
+    (57, 8, 8, 1000, 1024, [1000, 70, 64, 1]),           # one segment: with no state on either side there is no scan
+    (28, 8, 4, 100, 256, [100, 65, 64]),
+    (15, 8, 2, 2048, 512, [2048, 1601, 30]),
+    (6, 8, 8, 5200, 512, [5184, 3333])])
+def test_segments_with_parts_left_out(pkg, device, B, H, Hkv, N, seg, lengths, dtype, enters, leaves):
+    """Without a state that enters, without a gradient of the one that leaves; the entering one needs no gradient."""
+    check(pkg, device, B, H, Hkv, N, seg, lengths, dtype, enters, leaves, dinitial=False)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
