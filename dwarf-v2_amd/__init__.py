@@ -20,20 +20,25 @@ Public surface (reference names, Lanerra/dwarf-v2):
   q6: pack_kv, unpack_kv, q6_prefill, q6_decode      (no reference counterpart)
   layer_norm; rotary_plan, RotaryPlan, rotary_embed;
   linear_attention, linear_attention_step            (no reference counterpart)
+  rms_norm, rms_norm_fp8; causal_conv,
+  causal_conv_step; selective_scan,
+  selective_scan_step                                (no reference counterpart)
 """
 
-from . import _lib, block, lattice, linattn, norm, npci, ops, packet, planner, probe, q6, rotary
+from . import _lib, block, conv, lattice, linattn, norm, npci, ops, packet, planner, probe, q6, rotary, selscan
 from .block import dsqg_block_forward
+from .conv import causal_conv, causal_conv_step
 from .dsqg import (_DSQGProbedFn, _DSQGV18GroupedFn, dsqg_attention_v18_grouped, dsqg_attention_with_probes,
                    dsqg_backward, dsqg_forward)
 from .ema import bounded_ema_factor, causal_ema_scan, inverse_bounded_ema_factor
 from .linattn import linear_attention, linear_attention_step
-from .norm import layer_norm
+from .norm import layer_norm, rms_norm, rms_norm_fp8
 from .npci import npci_rotate
 from .packet import _InterferencePacketFn, _InterferencePoolFn, interference_packet, interference_packet_forward, interference_pool
 from .planner import _normalize_grouping_args, _plan_sparse_groups, _verify_sparse_plan
 from .probe import _PhaseProbeFn, phase_probe_features
 from .rotary import RotaryPlan, rotary_embed, rotary_plan
+from .selscan import selective_scan, selective_scan_step
 from .lattice import (
     ALL_OFFSETS,
     GROUPED_MODE_IDS,
@@ -64,6 +69,8 @@ __all__ = [
     "_verify_sparse_plan",
     "bounded_ema_factor",
     "build_offset_groups",
+    "causal_conv",
+    "causal_conv_step",
     "causal_ema_scan",
     "dsqg_attention_v18_grouped",
     "dsqg_attention_with_probes",
@@ -80,8 +87,12 @@ __all__ = [
     "npci_rotate",
     "phase_probe_features",
     "q6",
+    "rms_norm",
+    "rms_norm_fp8",
     "rotary_embed",
     "rotary_plan",
+    "selective_scan",
+    "selective_scan_step",
 ]
 
 

@@ -13,7 +13,7 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t
 
 LIB_NAME = "libdwarf_dsqg.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 DWARF_OK = 0
 DWARF_ERR_INVALID_ARGUMENT = 1
@@ -23,7 +23,7 @@ DWARF_ERR_WORKSPACE = 4
 
 DWARF_BF16 = 0
 DWARF_F32 = 1
-DWARF_F16 = 2   # the entry points of dwarf_mixer.h only
+DWARF_F16 = 2   # the entry points of dwarf_mixer.h and dwarf_selective.h only
 
 EXPORTED_SYMBOLS = (
     "dwarf_abi_version",
@@ -402,6 +402,121 @@ class LinearAttentionStepArgs(ctypes.Structure):
     ]
 
 
+# ---- include/dwarf_selective.h ----
+SELECTIVE_SYMBOLS = ("dwarf_rms_norm_fwd", "dwarf_rms_norm_bwd_workspace_bytes", "dwarf_rms_norm_bwd",
+                     "dwarf_causal_conv_fwd", "dwarf_causal_conv_bwd_workspace_bytes", "dwarf_causal_conv_bwd",
+                     "dwarf_causal_conv_step", "dwarf_selective_scan_checkpoint_bytes",
+                     "dwarf_selective_scan_fwd_workspace_bytes", "dwarf_selective_scan_fwd",
+                     "dwarf_selective_scan_bwd_workspace_bytes", "dwarf_selective_scan_bwd", "dwarf_selective_scan_step")
+
+
+class RmsNormFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("groups", c_int32), ("D", c_int32),
+        ("dtype", c_int32), ("residual_dtype", c_int32), ("eps", c_float),
+        ("x", c_void_p), ("x_stride", _i64(2)),
+        ("residual", c_void_p), ("residual_stride", _i64(2)),
+        ("weight", c_void_p),
+        ("sum", c_void_p), ("sum_stride", _i64(2)),
+        ("y", c_void_p), ("y_stride", _i64(2)),
+        ("scale", c_void_p),
+    ]
+
+
+class RmsNormBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("groups", c_int32), ("D", c_int32),
+        ("dtype", c_int32), ("stream_dtype", c_int32), ("eps", c_float),
+        ("stream", c_void_p), ("stream_stride", _i64(2)),
+        ("weight", c_void_p),
+        ("dy", c_void_p), ("dy_stride", _i64(2)),
+        ("dsum", c_void_p), ("dsum_stride", _i64(2)),
+        ("dx", c_void_p), ("dx_stride", _i64(2)),
+        ("dresidual", c_void_p), ("dresidual_stride", _i64(2)),
+        ("dweight", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class CausalConvFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", c_int32), ("N", c_int32), ("D", c_int32), ("W", c_int32),
+        ("dtype", c_int32), ("silu", c_int32),
+        ("x", c_void_p), ("x_stride", _i64(2)),
+        ("weight", c_void_p), ("bias", c_void_p), ("lengths", c_void_p), ("initial", c_void_p),
+        ("y", c_void_p), ("y_stride", _i64(2)),
+        ("final", c_void_p),
+    ]
+
+
+class CausalConvBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", CausalConvFwdArgs),
+        ("dy", c_void_p), ("dy_stride", _i64(2)),
+        ("dfinal", c_void_p),
+        ("dx", c_void_p), ("dx_stride", _i64(2)),
+        ("dweight", c_void_p), ("dbias", c_void_p), ("dinitial", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class CausalConvStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("R", c_int32), ("D", c_int32), ("W", c_int32), ("pool", c_int32),
+        ("dtype", c_int32), ("silu", c_int32),
+        ("x", c_void_p), ("x_stride", c_int64),
+        ("weight", c_void_p), ("bias", c_void_p), ("slots", c_void_p),
+        ("state", c_void_p), ("new_state", c_void_p), ("slot_stride", c_int64),
+        ("out", c_void_p), ("out_stride", c_int64),
+    ]
+
+
+class SelectiveScanFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", c_int32), ("N", c_int32), ("D", c_int32), ("G", c_int32), ("S", c_int32),
+        ("dtype", c_int32), ("softplus", c_int32),
+        ("x", c_void_p), ("x_stride", _i64(2)),
+        ("delta", c_void_p), ("delta_stride", _i64(2)),
+        ("gate", c_void_p), ("gate_stride", _i64(2)),
+        ("Bm", c_void_p), ("B_stride", _i64(3)),
+        ("Cm", c_void_p), ("C_stride", _i64(3)),
+        ("A", c_void_p), ("skip", c_void_p), ("delta_bias", c_void_p), ("lengths", c_void_p), ("initial", c_void_p),
+        ("y", c_void_p), ("y_stride", _i64(2)),
+        ("final", c_void_p),
+        ("checkpoints", c_void_p), ("checkpoint_bytes", c_size_t),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class SelectiveScanBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", SelectiveScanFwdArgs),
+        ("dy", c_void_p), ("dy_stride", _i64(2)),
+        ("dfinal", c_void_p),
+        ("dx", c_void_p), ("dx_stride", _i64(2)),
+        ("ddelta", c_void_p), ("ddelta_stride", _i64(2)),
+        ("dgate", c_void_p), ("dgate_stride", _i64(2)),
+        ("dB", c_void_p), ("dC", c_void_p),
+        ("dA", c_void_p), ("dskip", c_void_p), ("ddelta_bias", c_void_p), ("dinitial", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class SelectiveScanStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("R", c_int32), ("D", c_int32), ("G", c_int32), ("S", c_int32), ("pool", c_int32),
+        ("dtype", c_int32), ("softplus", c_int32),
+        ("x", c_void_p), ("x_stride", c_int64),
+        ("delta", c_void_p), ("delta_stride", c_int64),
+        ("gate", c_void_p), ("gate_stride", c_int64),
+        ("Bm", c_void_p), ("B_stride", _i64(2)),
+        ("Cm", c_void_p), ("C_stride", _i64(2)),
+        ("A", c_void_p), ("skip", c_void_p), ("delta_bias", c_void_p), ("slots", c_void_p),
+        ("state", c_void_p), ("new_state", c_void_p), ("slot_stride", c_int64),
+        ("out", c_void_p), ("out_stride", c_int64),
+    ]
+
+
 class NativeLibraryError(RuntimeError):
     """The HIP library is missing, stale or failed a call."""
 
@@ -528,6 +643,20 @@ def load() -> ctypes.CDLL:
     lib.dwarf_linear_attention_bwd.argtypes = [POINTER(LinearAttentionBwdArgs), c_void_p]
     lib.dwarf_linear_attention_step.restype = c_int
     lib.dwarf_linear_attention_step.argtypes = [POINTER(LinearAttentionStepArgs), c_void_p]
+    for name, args in (("dwarf_rms_norm_fwd", RmsNormFwdArgs), ("dwarf_rms_norm_bwd", RmsNormBwdArgs),
+                       ("dwarf_causal_conv_fwd", CausalConvFwdArgs), ("dwarf_causal_conv_bwd", CausalConvBwdArgs),
+                       ("dwarf_causal_conv_step", CausalConvStepArgs), ("dwarf_selective_scan_fwd", SelectiveScanFwdArgs),
+                       ("dwarf_selective_scan_bwd", SelectiveScanBwdArgs),
+                       ("dwarf_selective_scan_step", SelectiveScanStepArgs)):
+        getattr(lib, name).restype = c_int
+        getattr(lib, name).argtypes = [POINTER(args), c_void_p]
+    for name, args in (("dwarf_rms_norm_bwd_workspace_bytes", RmsNormBwdArgs),
+                       ("dwarf_causal_conv_bwd_workspace_bytes", CausalConvBwdArgs),
+                       ("dwarf_selective_scan_checkpoint_bytes", SelectiveScanFwdArgs),
+                       ("dwarf_selective_scan_fwd_workspace_bytes", SelectiveScanFwdArgs),
+                       ("dwarf_selective_scan_bwd_workspace_bytes", SelectiveScanBwdArgs)):
+        getattr(lib, name).restype = c_size_t
+        getattr(lib, name).argtypes = [POINTER(args)]
     _LIB = lib
     return lib
 

@@ -11,6 +11,8 @@
 #include "dwarf_block.h"
 #include "dwarf_dsqg.h"
 #include "dwarf_mixer.h"
+#include "dwarf_selective.h"
+#include "selective.h"
 
 namespace dwarf {
 size_t ema_fwd_workspace(int B, int N, int D);
@@ -1056,6 +1058,255 @@ int dwarf_linear_attention_step(const dwarf_linear_attention_step_args* args, dw
     return fail(DWARF_ERR_INVALID_ARGUMENT, "state and new_state overlap: give one pool twice, or two apart");
   return hip_status(dwarf::launch_linear_attention_step(a, reinterpret_cast<hipStream_t>(stream)),
                     "dwarf_linear_attention_step");
+}
+
+// ---- RMS norm, short causal convolution, selective scan (dwarf_selective.h) ----
+static int check_stream_rows(int64_t rows, int groups, int D, int dtype, int stream_dtype, float eps) {
+  if (rows < 0 || groups < 1 || D < 1)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "bad sizes rows=%lld groups=%d D=%d", static_cast<long long>(rows), groups, D);
+  if (!mixer_dtype(dtype)) return fail(DWARF_ERR_INVALID_ARGUMENT, "dtype=%d", dtype);
+  if (stream_dtype != dtype && stream_dtype != DWARF_F32)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "the residual stream has dtype=%d (the rows' or fp32)", stream_dtype);
+  if (!(eps >= 0.f) || !finite_f32(eps)) return fail(DWARF_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+  if (groups > 65535 || D > (1 << 24) || static_cast<int64_t>(groups) * D >= (int64_t(1) << 25) || rows >= (int64_t(1) << 40))
+    return fail(DWARF_ERR_UNSUPPORTED, "groups up to 65535, D up to 2^24 and groups * D below 2^25");
+  return DWARF_OK;
+}
+
+int dwarf_rms_norm_fwd(const dwarf_rms_norm_fwd_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_rms_norm_fwd_args& a = *args;
+  int rc = check_stream_rows(a.rows, a.groups, a.D, a.dtype, a.residual ? a.residual_dtype : a.dtype, a.eps);
+  if (rc || a.rows == 0) return rc ? rc : ok();
+  if ((rc = check_elements("x", a.x, a.dtype))) return rc;
+  if (a.residual && ((rc = check_elements("residual", a.residual, a.residual_dtype)) ||
+                     (rc = check_elements("sum", a.sum, a.residual_dtype))))
+    return rc;
+  if (a.scale ? !a.y : (rc = check_elements("y", a.y, a.dtype)) != DWARF_OK)
+    return a.scale ? fail(DWARF_ERR_INVALID_ARGUMENT, "y is NULL") : rc;
+  return hip_status(dwarf::launch_rms_norm_fwd(a, reinterpret_cast<hipStream_t>(stream)), "dwarf_rms_norm_fwd");
+}
+
+size_t dwarf_rms_norm_bwd_workspace_bytes(const dwarf_rms_norm_bwd_args* a) {
+  return a && check_stream_rows(a->rows, a->groups, a->D, a->dtype, a->stream_dtype, a->eps) == DWARF_OK && a->rows
+             ? dwarf::rms_norm_bwd_workspace(*a) : 0;
+}
+
+int dwarf_rms_norm_bwd(const dwarf_rms_norm_bwd_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_rms_norm_bwd_args& a = *args;
+  int rc = check_stream_rows(a.rows, a.groups, a.D, a.dtype, a.stream_dtype, a.eps);
+  if (rc) return rc;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (a.rows == 0)   // the weight's gradient is a sum over nothing
+    return zero_floats(a.dweight, static_cast<int64_t>(a.groups) * a.D, s, "dwarf_rms_norm_bwd");
+  if ((rc = check_elements("stream", a.stream, a.stream_dtype)) || (rc = check_elements("dy", a.dy, a.dtype))) return rc;
+  if (a.dsum && (rc = check_elements("dsum", a.dsum, a.stream_dtype))) return rc;
+  if (a.dx && (rc = check_elements("dx", a.dx, a.dtype))) return rc;
+  if (a.dresidual && (rc = check_elements("dresidual", a.dresidual, a.stream_dtype))) return rc;
+  if (!a.dx && !a.dresidual && !a.dweight) return ok();
+  const size_t need = dwarf::rms_norm_bwd_workspace(a);
+  if (need && (!a.workspace || a.workspace_bytes < need || !aligned16(a.workspace)))
+    return fail(DWARF_ERR_WORKSPACE, "workspace needs %zu bytes, 16-byte aligned, got %zu", need, a.workspace_bytes);
+  return hip_status(dwarf::launch_rms_norm_bwd(a, s), "dwarf_rms_norm_bwd");
+}
+
+// [.., tokens, D] rows: unit stride on D is implied; rows lie apart or, with a stride of 0, are one row.
+static int check_conv(const dwarf_causal_conv_fwd_args& a) {
+  if (a.B < 0 || a.N < 0 || a.D < 1 || a.W < 1)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "bad sizes B=%d N=%d D=%d W=%d", a.B, a.N, a.D, a.W);
+  if (!mixer_dtype(a.dtype)) return fail(DWARF_ERR_INVALID_ARGUMENT, "dtype=%d", a.dtype);
+  if (a.W > 8) return fail(DWARF_ERR_UNSUPPORTED, "the convolution is built for W up to 8 (got %d)", a.W);
+  if (a.N > (1 << 24) || a.D > (1 << 24)) return fail(DWARF_ERR_UNSUPPORTED, "N and D up to 2^24 (got %d, %d)", a.N, a.D);
+  if (a.B == 0) return DWARF_OK;
+  if (dwarf::causal_conv_workgroups(a) >= (int64_t(1) << 23))   // a launch counts its threads in 32 bits
+    return fail(DWARF_ERR_UNSUPPORTED, "B * N * D is too large for one launch");
+  if (!a.weight) return fail(DWARF_ERR_INVALID_ARGUMENT, "weight is NULL");
+  int rc;
+  if (a.N && (rc = check_elements("x", a.x, a.dtype))) return rc;
+  if (a.initial && (rc = check_elements("initial", a.initial, a.dtype))) return rc;
+  return DWARF_OK;
+}
+
+int dwarf_causal_conv_fwd(const dwarf_causal_conv_fwd_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_causal_conv_fwd_args& a = *args;
+  int rc = check_conv(a);
+  if (rc || a.B == 0) return rc ? rc : ok();
+  if (a.N && (rc = check_elements("y", a.y, a.dtype))) return rc;
+  if (a.final && (rc = check_elements("final", a.final, a.dtype))) return rc;
+  if (a.N == 0 && !a.final) return ok();
+  return hip_status(dwarf::launch_causal_conv_fwd(a, reinterpret_cast<hipStream_t>(stream)), "dwarf_causal_conv_fwd");
+}
+
+size_t dwarf_causal_conv_bwd_workspace_bytes(const dwarf_causal_conv_bwd_args* a) {
+  return a && a->fwd.B > 0 && a->fwd.N >= 0 && a->fwd.D > 0 && a->fwd.W > 0 && mixer_dtype(a->fwd.dtype)
+             ? dwarf::causal_conv_bwd_workspace(*a) : 0;
+}
+
+int dwarf_causal_conv_bwd(const dwarf_causal_conv_bwd_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_causal_conv_bwd_args& a = *args;
+  int rc = check_conv(a.fwd);
+  if (rc) return rc;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (a.fwd.B == 0) {   // sums over nothing
+    rc = zero_floats(a.dweight, static_cast<int64_t>(a.fwd.D) * a.fwd.W, s, "dwarf_causal_conv_bwd");
+    return rc ? rc : zero_floats(a.dbias, a.fwd.D, s, "dwarf_causal_conv_bwd");
+  }
+  if (a.fwd.N && ((rc = check_elements("dy", a.dy, a.fwd.dtype)) || (rc = check_elements("dx", a.dx, a.fwd.dtype)))) return rc;
+  if (a.dfinal && (rc = check_elements("dfinal", a.dfinal, a.fwd.dtype))) return rc;
+  if (a.dinitial && (rc = check_elements("dinitial", a.dinitial, a.fwd.dtype))) return rc;
+  const size_t need = dwarf::causal_conv_bwd_workspace(a);
+  if (need && (!a.workspace || a.workspace_bytes < need || !aligned16(a.workspace)))
+    return fail(DWARF_ERR_WORKSPACE, "workspace needs %zu bytes, 16-byte aligned, got %zu", need, a.workspace_bytes);
+  return hip_status(dwarf::launch_causal_conv_bwd(a, s), "dwarf_causal_conv_bwd");
+}
+
+// A pool of `each` contiguous elements a slot, and the one the new states go to: the same, or one apart.
+static int check_pool(const void* state, const void* new_state, int pool, int rows, const int32_t* slots, int64_t slot_stride,
+                      int64_t each, int dtype) {
+  if (pool < 0 || (!slots && pool < rows))
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "pool=%d holds fewer states than the %d rows", pool, rows);
+  if (pool == 0) return fail(DWARF_ERR_INVALID_ARGUMENT, "the pool is empty");
+  if (each == 0) return DWARF_OK;
+  int rc;
+  if ((rc = check_elements("state", state, dtype)) || (rc = check_elements("new_state", new_state, dtype))) return rc;
+  if (slot_stride < each)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "slot_stride=%lld must be at least %lld", static_cast<long long>(slot_stride),
+                static_cast<long long>(each));
+  const uintptr_t x = reinterpret_cast<uintptr_t>(state), y = reinterpret_cast<uintptr_t>(new_state);
+  const uintptr_t span = (static_cast<uintptr_t>(pool - 1) * slot_stride + each) * elem_size(dtype);
+  if (x != y && x < y + span && y < x + span)
+    return fail(DWARF_ERR_INVALID_ARGUMENT, "state and new_state overlap: give one pool twice, or two apart");
+  return DWARF_OK;
+}
+
+int dwarf_causal_conv_step(const dwarf_causal_conv_step_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_causal_conv_step_args& a = *args;
+  if (a.R < 0 || a.D < 1 || a.W < 1) return fail(DWARF_ERR_INVALID_ARGUMENT, "bad sizes R=%d D=%d W=%d", a.R, a.D, a.W);
+  if (!mixer_dtype(a.dtype)) return fail(DWARF_ERR_INVALID_ARGUMENT, "dtype=%d", a.dtype);
+  if (a.W > 8) return fail(DWARF_ERR_UNSUPPORTED, "the convolution is built for W up to 8 (got %d)", a.W);
+  // a launch counts its threads in 32 bits: 256 for each 256 vectors, or channels, of a row
+  if (a.D > (1 << 24) || static_cast<int64_t>(a.R) * ((a.D + 255) / 256) >= (int64_t(1) << 23))
+    return fail(DWARF_ERR_UNSUPPORTED, "D up to 2^24 and R * D / 256 below 2^23");
+  if (a.R == 0) return ok();
+  if (!a.weight) return fail(DWARF_ERR_INVALID_ARGUMENT, "weight is NULL");
+  int rc;
+  if ((rc = check_elements("x", a.x, a.dtype)) || (rc = check_elements("out", a.out, a.dtype))) return rc;
+  if ((rc = check_pool(a.state, a.new_state, a.pool, a.R, a.slots, a.slot_stride, static_cast<int64_t>(a.W - 1) * a.D, a.dtype)))
+    return rc;
+  return hip_status(dwarf::launch_causal_conv_step(a, reinterpret_cast<hipStream_t>(stream)), "dwarf_causal_conv_step");
+}
+
+static int check_scan_sizes(int D, int G, int S, int dtype) {
+  if (D < 1 || G < 1 || S < 1) return fail(DWARF_ERR_INVALID_ARGUMENT, "bad sizes D=%d G=%d S=%d", D, G, S);
+  if (D % G) return fail(DWARF_ERR_INVALID_ARGUMENT, "D=%d channels must be divisible by G=%d groups", D, G);
+  if (!mixer_dtype(dtype)) return fail(DWARF_ERR_INVALID_ARGUMENT, "dtype=%d", dtype);
+  if (S > 64) return fail(DWARF_ERR_UNSUPPORTED, "the scan is built for up to 64 states (got %d)", S);
+  if (D > (1 << 24)) return fail(DWARF_ERR_UNSUPPORTED, "D up to 2^24 (got %d)", D);
+  return DWARF_OK;
+}
+
+static int check_scan(const dwarf_selective_scan_fwd_args& a) {
+  if (a.B < 0 || a.N < 0) return fail(DWARF_ERR_INVALID_ARGUMENT, "bad sizes B=%d N=%d", a.B, a.N);
+  int rc = check_scan_sizes(a.D, a.G, a.S, a.dtype);
+  if (rc) return rc;
+  if (a.N > (1 << 24)) return fail(DWARF_ERR_UNSUPPORTED, "N up to 2^24 (got %d)", a.N);
+  if (a.B == 0) return DWARF_OK;
+  if (dwarf::selective_scan_workgroups(a) >= (int64_t(1) << 23))   // a launch counts its threads in 32 bits
+    return fail(DWARF_ERR_UNSUPPORTED, "B * D * segments is too large for one launch");
+  if (!a.A) return fail(DWARF_ERR_INVALID_ARGUMENT, "A is NULL");
+  if (a.N == 0) return DWARF_OK;
+  if ((rc = check_elements("x", a.x, a.dtype)) || (rc = check_elements("delta", a.delta, a.dtype)) ||
+      (rc = check_elements("B", a.Bm, a.dtype)) || (rc = check_elements("C", a.Cm, a.dtype)))
+    return rc;
+  return a.gate ? check_elements("gate", a.gate, a.dtype) : DWARF_OK;
+}
+
+static bool scan_sized(const dwarf_selective_scan_fwd_args* a) {
+  return a && a->B > 0 && a->N >= 0 && check_scan_sizes(a->D, a->G, a->S, a->dtype) == DWARF_OK;
+}
+size_t dwarf_selective_scan_checkpoint_bytes(const dwarf_selective_scan_fwd_args* a) {
+  return scan_sized(a) ? dwarf::selective_scan_checkpoints(*a) : 0;
+}
+size_t dwarf_selective_scan_fwd_workspace_bytes(const dwarf_selective_scan_fwd_args* a) {
+  return scan_sized(a) ? dwarf::selective_scan_fwd_workspace(*a) : 0;
+}
+
+static int check_checkpoints(const dwarf_selective_scan_fwd_args& a) {
+  const size_t need = dwarf::selective_scan_checkpoints(a);
+  if (need && (!a.checkpoints || a.checkpoint_bytes < need || !aligned16(a.checkpoints)))
+    return fail(DWARF_ERR_WORKSPACE, "checkpoints need %zu bytes, 16-byte aligned, got %zu", need, a.checkpoint_bytes);
+  return DWARF_OK;
+}
+
+int dwarf_selective_scan_fwd(const dwarf_selective_scan_fwd_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_selective_scan_fwd_args& a = *args;
+  int rc = check_scan(a);
+  if (rc || a.B == 0) return rc ? rc : ok();
+  if (a.N && (rc = check_elements("y", a.y, a.dtype))) return rc;
+  if (a.checkpoints && (rc = check_checkpoints(a))) return rc;
+  if (a.N == 0 && !a.final) return ok();
+  const size_t need = dwarf::selective_scan_fwd_workspace(a);
+  if (need && (!a.workspace || a.workspace_bytes < need || !aligned16(a.workspace)))
+    return fail(DWARF_ERR_WORKSPACE, "workspace needs %zu bytes, 16-byte aligned, got %zu", need, a.workspace_bytes);
+  return hip_status(dwarf::launch_selective_scan_fwd(a, reinterpret_cast<hipStream_t>(stream)), "dwarf_selective_scan_fwd");
+}
+
+size_t dwarf_selective_scan_bwd_workspace_bytes(const dwarf_selective_scan_bwd_args* a) {
+  return a && scan_sized(&a->fwd) ? dwarf::selective_scan_bwd_workspace(*a) : 0;
+}
+
+int dwarf_selective_scan_bwd(const dwarf_selective_scan_bwd_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_selective_scan_bwd_args& a = *args;
+  int rc = check_scan(a.fwd);
+  if (rc) return rc;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (a.fwd.B == 0) {   // sums over nothing
+    rc = zero_floats(a.dA, static_cast<int64_t>(a.fwd.D) * a.fwd.S, s, "dwarf_selective_scan_bwd");
+    if (!rc) rc = zero_floats(a.dskip, a.fwd.D, s, "dwarf_selective_scan_bwd");
+    return rc ? rc : zero_floats(a.ddelta_bias, a.fwd.D, s, "dwarf_selective_scan_bwd");
+  }
+  // the threads that add the channel tiles' rows
+  if (static_cast<double>(a.fwd.B) * a.fwd.N * a.fwd.G * 128. >= 0x1p31)
+    return fail(DWARF_ERR_UNSUPPORTED, "gradients: B * N * G must stay below 2^24");
+  if (a.fwd.N) {
+    if ((rc = check_elements("dy", a.dy, a.fwd.dtype)) || (rc = check_elements("dx", a.dx, a.fwd.dtype)) ||
+        (rc = check_elements("ddelta", a.ddelta, a.fwd.dtype)) || (rc = check_elements("dB", a.dB, a.fwd.dtype)) ||
+        (rc = check_elements("dC", a.dC, a.fwd.dtype)))
+      return rc;
+    if (a.fwd.gate && (rc = check_elements("dgate", a.dgate, a.fwd.dtype))) return rc;
+    if ((rc = check_checkpoints(a.fwd))) return rc;
+  }
+  const size_t need = dwarf::selective_scan_bwd_workspace(a);
+  if (need && (!a.workspace || a.workspace_bytes < need || !aligned16(a.workspace)))
+    return fail(DWARF_ERR_WORKSPACE, "workspace needs %zu bytes, 16-byte aligned, got %zu", need, a.workspace_bytes);
+  return hip_status(dwarf::launch_selective_scan_bwd(a, s), "dwarf_selective_scan_bwd");
+}
+
+int dwarf_selective_scan_step(const dwarf_selective_scan_step_args* args, dwarf_stream_t stream) {
+  if (!args) return fail(DWARF_ERR_INVALID_ARGUMENT, "args is NULL");
+  const dwarf_selective_scan_step_args& a = *args;
+  if (a.R < 0) return fail(DWARF_ERR_INVALID_ARGUMENT, "R=%d", a.R);
+  int rc = check_scan_sizes(a.D, a.G, a.S, a.dtype);
+  if (rc) return rc;
+  // a launch counts its threads in 32 bits: 256 for each 32 channels of a group at least
+  if (static_cast<int64_t>(a.R) * a.G * ((a.D / a.G + 31) / 32) >= (int64_t(1) << 23))
+    return fail(DWARF_ERR_UNSUPPORTED, "R * D / 32 must stay below 2^23");
+  if (a.R == 0) return ok();
+  if (!a.A) return fail(DWARF_ERR_INVALID_ARGUMENT, "A is NULL");
+  if ((rc = check_elements("x", a.x, a.dtype)) || (rc = check_elements("delta", a.delta, a.dtype)) ||
+      (rc = check_elements("B", a.Bm, a.dtype)) || (rc = check_elements("C", a.Cm, a.dtype)) ||
+      (rc = check_elements("out", a.out, a.dtype)))
+    return rc;
+  if (a.gate && (rc = check_elements("gate", a.gate, a.dtype))) return rc;
+  if ((rc = check_pool(a.state, a.new_state, a.pool, a.R, a.slots, a.slot_stride, static_cast<int64_t>(a.D) * a.S, DWARF_F32)))
+    return rc;
+  return hip_status(dwarf::launch_selective_scan_step(a, reinterpret_cast<hipStream_t>(stream)), "dwarf_selective_scan_step");
 }
 
 }  // extern "C"

@@ -1,0 +1,446 @@
+// A short causal convolution of each channel, forward, backward and for single
+// tokens:
+//   p_t = bias + sum_j w_j x_{t-W+1+j},   y_t = p_t or silu(p_t)
+//   dp = dy silu'(p),  dx_t = sum_j w_j dp_{t+W-1-j},  dw_j = sum dp_t x_{t-W+1+j},  dbias = sum dp
+//
+// Bound by memory.  A thread takes VEC adjacent channels (16 bytes) and walks a
+// strip of tokens with the last W - 1 inputs in registers: each input is loaded
+// once but for the W - 1 rows in front of a strip, which another strip's thread
+// loads at about the same time.  Rows need no alignment but their elements':
+// gfx950 loads 16 bytes from any address, and a width that VEC does not divide
+// has its last vector moved back to the row's end, where two threads then store
+// the same values.  The backward forms p again from x, which it needs for dw
+// anyway, instead of reading a saved one; a strip goes W - 1 tokens further to
+// have the dp that its own dx need.  dw and dbias: a thread's sums over its
+// strip in registers, a workgroup's over its strips in LDS, then one partial
+// row for each workgroup and a last launch that adds those in order, in 64
+// bits.
+#include "selective.h"
+
+namespace dwarf {
+namespace {
+
+constexpr int kConvThreads = 256;
+constexpr int kConvCols = 32;                              // vectors of channels in a workgroup
+constexpr int kConvStrips = kConvThreads / kConvCols;      // strips of tokens in a workgroup
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_any(const T* p, float* x) {
+  T v[VEC];
+  __builtin_memcpy(v, p, sizeof(v));
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) x[e] = to_f32(v[e]);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_any(T* p, const float* x) {
+  T v[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) v[e] = from_f32<T>(x[e]);
+  __builtin_memcpy(p, v, sizeof(v));
+}
+
+struct ConvGeom {
+  int cols;        // vectors of channels of a row
+  int col_blocks;  // workgroups over them
+  int strip;       // tokens of a strip
+  int strips;      // strips of a sequence
+};
+
+__device__ __forceinline__ int conv_length(const dwarf_causal_conv_fwd_args& a, int b) {
+  if (!a.lengths) return a.N;
+  const int n = a.lengths[b];
+  return n < 0 ? 0 : n > a.N ? a.N : n;
+}
+
+// Where a thread stands: its vector's first channel (the last vector lies at the row's end), its sequence and strip.
+template <int VEC>
+struct ConvAt {
+  int d, b, strip, col;
+  bool in;
+  __device__ __forceinline__ ConvAt(int D, const ConvGeom& gm, int B) {
+    col = blockIdx.x % static_cast<uint32_t>(gm.col_blocks) * kConvCols + threadIdx.x % kConvCols;
+    const int64_t s = static_cast<int64_t>(blockIdx.x / static_cast<uint32_t>(gm.col_blocks)) * kConvStrips + threadIdx.x / kConvCols;
+    in = col < gm.cols && s < static_cast<int64_t>(B) * gm.strips;
+    b = in ? static_cast<int>(s / gm.strips) : 0;
+    strip = in ? static_cast<int>(s - static_cast<int64_t>(b) * gm.strips) : 0;
+    d = col * VEC;
+    if (d > D - VEC) d = D - VEC;   // D >= VEC
+    if (!in) d = 0;
+  }
+};
+
+template <int VEC, int W>
+__device__ __forceinline__ void conv_weights(const float* weight, const float* bias, int d, float (*w)[VEC], float* c) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j][e] = weight[static_cast<int64_t>(d + e) * W + j];
+    c[e] = bias ? bias[d + e] : 0.f;
+  }
+}
+
+// Input row t of a sequence, t >= -(W - 1): the state's in front of the first token.
+template <typename T, int VEC, int W>
+__device__ __forceinline__ void conv_input(const dwarf_causal_conv_fwd_args& a, const T* x, int b, int d, int t, float* v) {
+  if (t >= 0) {
+    load_any<T, VEC>(x + t * a.x_stride[1], v);
+  } else if (a.initial) {
+    load_any<T, VEC>(static_cast<const T*>(a.initial) + (static_cast<int64_t>(b) * (W - 1) + (t + W - 1)) * a.D + d, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = 0.f;
+  }
+}
+
+template <typename T, int VEC, int W>
+__global__ __launch_bounds__(kConvThreads) void conv_fwd_kernel(dwarf_causal_conv_fwd_args a, ConvGeom gm) {
+  const ConvAt<VEC> at(a.D, gm, a.B);
+  if (!at.in) return;
+  const int d = at.d, n = conv_length(a, at.b);
+  const int t0 = at.strip * gm.strip, t1 = min(a.N, t0 + gm.strip), end = min(t1, n);
+  const T* x = static_cast<const T*>(a.x) + at.b * a.x_stride[0] + d;
+  T* y = static_cast<T*>(a.y) + at.b * a.y_stride[0] + d;
+  if (t0 < end) {
+    float w[W][VEC], c[VEC], win[W][VEC];   // win[j]: input t - W + 1 + j
+    conv_weights<VEC, W>(a.weight, a.bias, d, w, c);
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) conv_input<T, VEC, W>(a, x, at.b, d, t0 - W + 1 + j, win[j + 1]);
+#pragma unroll 4
+    for (int t = t0; t < end; ++t) {
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) win[j][e] = win[j + 1][e];
+      load_any<T, VEC>(x + t * a.x_stride[1], win[W - 1]);
+      float p[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        p[e] = c[e];
+#pragma unroll
+        for (int j = 0; j < W; ++j) p[e] = fmaf(w[j][e], win[j][e], p[e]);
+        if (a.silu) p[e] *= sigmoid_f32(p[e]);
+      }
+      store_any<T, VEC>(y + t * a.y_stride[1], p);
+    }
+  }
+  float z[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) z[e] = 0.f;
+  for (int t = max(t0, end); t < t1; ++t) store_any<T, VEC>(y + t * a.y_stride[1], z);
+  // the last W - 1 inputs, by the sequence's last strip
+  if (a.final && at.strip == gm.strips - 1) {
+    T* f = static_cast<T*>(a.final) + static_cast<int64_t>(at.b) * (W - 1) * a.D + d;
+    for (int j = 0; j < W - 1; ++j) {
+      float v[VEC];
+      conv_input<T, VEC, W>(a, x, at.b, d, n - (W - 1) + j, v);
+      store_any<T, VEC>(f + static_cast<int64_t>(j) * a.D, v);
+    }
+  }
+}
+
+__device__ __forceinline__ float silu_slope(float p) {
+  const float e = sigmoid_f32(p);
+  return e * fmaf(p, 1.f - e, 1.f);
+}
+
+template <typename T, int VEC, int W>
+__global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(dwarf_causal_conv_bwd_args w_, ConvGeom gm, float* __restrict__ part) {
+  __shared__ float s_red[kConvStrips][kConvCols * VEC];
+  const dwarf_causal_conv_fwd_args& a = w_.fwd;
+  const ConvAt<VEC> at(a.D, gm, a.B);
+  const int d = at.d;
+  float dw[W + 1][VEC];   // dbias last
+#pragma unroll
+  for (int j = 0; j <= W; ++j)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) dw[j][e] = 0.f;
+  if (at.in) {
+    const int n = conv_length(a, at.b);
+    const int t0 = at.strip * gm.strip, t1 = min(a.N, t0 + gm.strip), end = min(t1, n);
+    const T* x = static_cast<const T*>(a.x) + at.b * a.x_stride[0] + d;
+    const T* dy = static_cast<const T*>(w_.dy) + at.b * w_.dy_stride[0] + d;
+    T* dx = static_cast<T*>(w_.dx) + at.b * w_.dx_stride[0] + d;
+    const T* df = w_.dfinal ? static_cast<const T*>(w_.dfinal) + static_cast<int64_t>(at.b) * (W - 1) * a.D + d : nullptr;
+    T* di = w_.dinitial ? static_cast<T*>(w_.dinitial) + static_cast<int64_t>(at.b) * (W - 1) * a.D + d : nullptr;
+    float w[W][VEC], c[VEC], win[W][VEC], dp[W][VEC];   // dp[i]: token t - i
+    conv_weights<VEC, W>(a.weight, a.bias, d, w, c);
+    // the state's rows get their gradient from the first strip
+    const int from = at.strip == 0 && di ? -(W - 1) : t0;
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) dp[j][e] = 0.f;
+    if (t0 < end || from < 0) {
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) conv_input<T, VEC, W>(a, x, at.b, d, t0 - W + 1 + j, win[j + 1]);
+      // tokens up to W - 1 behind the strip, whose dp its last tokens' dx need; none behind the sequence's end
+      for (int t = t0; t < end + W - 1; ++t) {
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) win[j][e] = win[j + 1][e];
+#pragma unroll
+        for (int j = W - 1; j > 0; --j)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) dp[j][e] = dp[j - 1][e];
+        if (t < n) {
+          load_any<T, VEC>(x + t * a.x_stride[1], win[W - 1]);
+          load_any<T, VEC>(dy + t * w_.dy_stride[1], dp[0]);
+          if (a.silu) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              float p = c[e];
+#pragma unroll
+              for (int j = 0; j < W; ++j) p = fmaf(w[j][e], win[j][e], p);
+              dp[0][e] *= silu_slope(p);
+            }
+          }
+          if (t < end) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+#pragma unroll
+              for (int j = 0; j < W; ++j) dw[j][e] = fmaf(dp[0][e], win[j][e], dw[j][e]);
+              dw[W][e] += dp[0][e];
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) dp[0][e] = 0.f;
+        }
+        const int to = t - (W - 1);   // dx_to = sum_j w_j dp_{to + W - 1 - j} = sum_j w_j dp[j]
+        if (to >= t0 ? to < end : to >= from) {
+          float v[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            v[e] = 0.f;
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[e] = fmaf(w[j][e], dp[j][e], v[e]);
+          }
+          // the state that leaves holds inputs n - W + 1 .. n - 1
+          if (df && to >= n - (W - 1)) {
+            float f[VEC];
+            load_any<T, VEC>(df + static_cast<int64_t>(to - (n - (W - 1))) * a.D, f);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] += f[e];
+          }
+          if (to >= 0) store_any<T, VEC>(dx + to * w_.dx_stride[1], v);
+          else store_any<T, VEC>(di + static_cast<int64_t>(to + W - 1) * a.D, v);
+        }
+      }
+    }
+    float z[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) z[e] = 0.f;
+    for (int t = max(t0, end); t < t1; ++t) store_any<T, VEC>(dx + t * w_.dx_stride[1], z);
+  }
+  if (!part) return;   // uniform
+  // the workgroup's strips in order; of channels that two vectors hold the first one's threads write
+  const int row = threadIdx.x / kConvCols, col = threadIdx.x % kConvCols;
+  const int64_t group = blockIdx.x / static_cast<uint32_t>(gm.col_blocks);
+#pragma unroll 1
+  for (int j = 0; j <= W; ++j) {
+    __syncthreads();
+#pragma unroll
+    for (int jj = 0; jj <= W; ++jj)
+      if (jj == j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s_red[row][col * VEC + e] = dw[jj][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kConvCols * VEC; i += kConvThreads) {
+      const int cc = static_cast<int>(at.col - col) + i / VEC;   // the vector, of all
+      if (cc >= gm.cols) continue;
+      int ch = cc * VEC;
+      const bool moved = ch > a.D - VEC;
+      if (moved) ch = a.D - VEC;
+      ch += i % VEC;
+      if (moved && ch < cc * VEC) continue;   // the vector in front has it
+      float t = 0.f;
+#pragma unroll
+      for (int r = 0; r < kConvStrips; ++r) t += s_red[r][i];
+      part[(group * (W + 1) + j) * a.D + ch] = t;
+    }
+  }
+}
+
+// dweight [D][W] and dbias [D]: 16 channels of one j in a workgroup, 64 threads to a channel, each every 64th partial row
+// in order.
+constexpr int kConvSumCols = 16, kConvSumRows = 64;
+__global__ __launch_bounds__(kConvSumCols * kConvSumRows) void conv_sum_kernel(const float* __restrict__ part, int64_t parts,
+                                                                              int D, int W, float* __restrict__ dweight,
+                                                                              float* __restrict__ dbias) {
+  __shared__ double s_part[kConvSumRows][kConvSumCols + 1];
+  const int j = blockIdx.y, col = threadIdx.x % kConvSumCols, row = threadIdx.x / kConvSumCols;
+  const int d = blockIdx.x * kConvSumCols + col;
+  float* out = j < W ? dweight : dbias;
+  if (!out) return;   // uniform
+  double t = 0.;
+  if (d < D)
+#pragma unroll 4
+    for (int64_t p = row; p < parts; p += kConvSumRows) t += part[(p * (W + 1) + j) * D + d];
+  s_part[row][col] = t;
+  __syncthreads();
+  if (row == 0 && d < D) {
+    double s = 0.;
+#pragma unroll 8
+    for (int r = 0; r < kConvSumRows; ++r) s += s_part[r][col];
+    if (j < W) dweight[static_cast<int64_t>(d) * W + j] = static_cast<float>(s);
+    else dbias[d] = static_cast<float>(s);
+  }
+}
+
+// One token of each row.  The first row of a slot takes the slot's later rows after it, in order.
+template <typename T, int VEC, int W>
+__global__ __launch_bounds__(kConvThreads) void conv_step_kernel(dwarf_causal_conv_step_args a, int col_blocks) {
+  __shared__ int s_next;
+  const int row0 = blockIdx.x / col_blocks, col = blockIdx.x % col_blocks * kConvThreads + threadIdx.x;
+  const bool in = col < (a.D + VEC - 1) / VEC;
+  int d = in ? col * VEC : 0;
+  // where the last vector lies at the row's end, channels that two vectors hold are the first one's to store: the states may
+  // be updated in place, and what the second then reads of those channels it does not use
+  int skip = 0;
+  if (d > a.D - VEC) skip = d - (a.D - VEC), d = a.D - VEC;
+  const int slot = a.slots ? a.slots[row0] : row0;
+  T* out = static_cast<T*>(a.out) + d;
+  float v[W][VEC], w[W][VEC], c[VEC];
+  auto put = [&](T* p, const float* x) {
+    if (!skip) store_any<T, VEC>(p, x);
+    else
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (e >= skip) p[e] = from_f32<T>(x[e]);
+  };
+  if (slot < 0 || slot >= a.pool) {   // uniform
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) c[e] = 0.f;
+    if (in) put(out + row0 * a.out_stride, c);
+    return;
+  }
+  const T* st = static_cast<const T*>(a.state) + slot * a.slot_stride + d;
+  T* ns = static_cast<T*>(a.new_state) + slot * a.slot_stride + d;
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) load_any<T, VEC>(st + static_cast<int64_t>(j) * a.D, v[j]);
+  load_any<T, VEC>(static_cast<const T*>(a.x) + row0 * a.x_stride + d, v[W - 1]);
+  conv_weights<VEC, W>(a.weight, a.bias, d, w, c);
+  if (row0 > 0 && a.slots && next_row_of<kConvThreads>(a.slots, slot, 0, a.R, &s_next) < row0) return;   // uniform
+  for (int row = row0; row < a.R;) {
+    float p[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      p[e] = c[e];
+#pragma unroll
+      for (int j = 0; j < W; ++j) p[e] = fmaf(w[j][e], v[j][e], p[e]);
+      if (a.silu) p[e] *= sigmoid_f32(p[e]);
+    }
+    if (in) put(out + row * a.out_stride, p);
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[j][e] = v[j + 1][e];
+    row = a.slots && row + 1 < a.R ? next_row_of<kConvThreads>(a.slots, slot, row + 1, a.R, &s_next) : a.R;
+    if (row < a.R) load_any<T, VEC>(static_cast<const T*>(a.x) + row * a.x_stride + d, v[W - 1]);
+  }
+  if (in)
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) put(ns + static_cast<int64_t>(j) * a.D, v[j]);
+}
+
+int conv_vec(int dtype, int D) {
+  const int per = dtype == DWARF_F32 ? 4 : 8;
+  return D >= per ? per : 1;
+}
+
+ConvGeom conv_geom(const dwarf_causal_conv_fwd_args& a, int least) {
+  ConvGeom gm;
+  const int vec = conv_vec(a.dtype, a.D);
+  gm.cols = (a.D + vec - 1) / vec;
+  gm.col_blocks = (gm.cols + kConvCols - 1) / kConvCols;
+  // strips as long as leave 1,024 workgroups (and partial rows within reason), `least` to 64 tokens
+  gm.strip = least;
+  while (gm.strip < 64 && static_cast<int64_t>(a.B) * a.N / (2 * gm.strip) / kConvStrips * gm.col_blocks >= 1024) gm.strip *= 2;
+  gm.strips = a.N > 0 ? (a.N + gm.strip - 1) / gm.strip : 1;
+  return gm;
+}
+int64_t conv_groups(const dwarf_causal_conv_fwd_args& a, const ConvGeom& gm) {
+  return (static_cast<int64_t>(a.B) * gm.strips + kConvStrips - 1) / kConvStrips;
+}
+constexpr int kConvFwdStrip = 8, kConvBwdStrip = 16;
+
+template <typename T, int VEC, int W>
+void conv_fwd_typed(const dwarf_causal_conv_fwd_args& a, hipStream_t stream) {
+  const ConvGeom gm = conv_geom(a, kConvFwdStrip);
+  hipLaunchKernelGGL((conv_fwd_kernel<T, VEC, W>), dim3(static_cast<unsigned>(conv_groups(a, gm) * gm.col_blocks)),
+                     dim3(kConvThreads), 0, stream, a, gm);
+}
+template <typename T, int VEC, int W>
+void conv_bwd_typed(const dwarf_causal_conv_bwd_args& a, hipStream_t stream) {
+  const ConvGeom gm = conv_geom(a.fwd, kConvBwdStrip);
+  const int64_t groups = conv_groups(a.fwd, gm);
+  float* part = a.dweight || a.dbias ? static_cast<float*>(a.workspace) : nullptr;
+  hipLaunchKernelGGL((conv_bwd_kernel<T, VEC, W>), dim3(static_cast<unsigned>(groups * gm.col_blocks)), dim3(kConvThreads), 0,
+                     stream, a, gm, part);
+  if (part)
+    hipLaunchKernelGGL(conv_sum_kernel, dim3((a.fwd.D + kConvSumCols - 1) / kConvSumCols, W + 1),
+                       dim3(kConvSumCols * kConvSumRows), 0, stream, part, groups, a.fwd.D, W, a.dweight, a.dbias);
+}
+template <typename T, int VEC, int W>
+void conv_step_typed(const dwarf_causal_conv_step_args& a, hipStream_t stream) {
+  const int cols = (a.D + VEC - 1) / VEC, col_blocks = (cols + kConvThreads - 1) / kConvThreads;
+  hipLaunchKernelGGL((conv_step_kernel<T, VEC, W>), dim3(static_cast<unsigned>(a.R) * col_blocks), dim3(kConvThreads), 0, stream,
+                     a, col_blocks);
+}
+
+#define DWARF_CONV_WIDTHS(T, VEC, W, CALL)    \
+  switch (W) {                                \
+    case 1: CALL(T, VEC, 1); break;           \
+    case 2: CALL(T, VEC, 2); break;           \
+    case 3: CALL(T, VEC, 3); break;           \
+    case 4: CALL(T, VEC, 4); break;           \
+    case 5: CALL(T, VEC, 5); break;           \
+    case 6: CALL(T, VEC, 6); break;           \
+    case 7: CALL(T, VEC, 7); break;           \
+    default: CALL(T, VEC, 8); break;          \
+  }
+#define DWARF_CONV_TYPES(dtype, D, W, CALL)                                                    \
+  const bool wide = conv_vec(dtype, D) > 1;                                                    \
+  if ((dtype) == DWARF_F32) {                                                                  \
+    if (wide) { DWARF_CONV_WIDTHS(float, 4, W, CALL) } else { DWARF_CONV_WIDTHS(float, 1, W, CALL) } \
+  } else if ((dtype) == DWARF_F16) {                                                           \
+    if (wide) { DWARF_CONV_WIDTHS(f16, 8, W, CALL) } else { DWARF_CONV_WIDTHS(f16, 1, W, CALL) }     \
+  } else {                                                                                     \
+    if (wide) { DWARF_CONV_WIDTHS(bf16, 8, W, CALL) } else { DWARF_CONV_WIDTHS(bf16, 1, W, CALL) }   \
+  }
+
+}  // namespace
+
+int64_t causal_conv_workgroups(const dwarf_causal_conv_fwd_args& a) {
+  const ConvGeom gm = conv_geom(a, kConvFwdStrip);   // the shorter strips
+  return conv_groups(a, gm) * gm.col_blocks;
+}
+
+size_t causal_conv_bwd_workspace(const dwarf_causal_conv_bwd_args& a) {
+  if (!a.dweight && !a.dbias) return 0;
+  return static_cast<size_t>(conv_groups(a.fwd, conv_geom(a.fwd, kConvBwdStrip))) * (a.fwd.W + 1) * a.fwd.D * sizeof(float);
+}
+
+hipError_t launch_causal_conv_fwd(const dwarf_causal_conv_fwd_args& a, hipStream_t stream) {
+#define DWARF_CONV_CALL(T, VEC, W) conv_fwd_typed<T, VEC, W>(a, stream)
+  DWARF_CONV_TYPES(a.dtype, a.D, a.W, DWARF_CONV_CALL)
+#undef DWARF_CONV_CALL
+  return hipGetLastError();
+}
+
+hipError_t launch_causal_conv_bwd(const dwarf_causal_conv_bwd_args& a, hipStream_t stream) {
+#define DWARF_CONV_CALL(T, VEC, W) conv_bwd_typed<T, VEC, W>(a, stream)
+  DWARF_CONV_TYPES(a.fwd.dtype, a.fwd.D, a.fwd.W, DWARF_CONV_CALL)
+#undef DWARF_CONV_CALL
+  return hipGetLastError();
+}
+
+hipError_t launch_causal_conv_step(const dwarf_causal_conv_step_args& a, hipStream_t stream) {
+#define DWARF_CONV_CALL(T, VEC, W) conv_step_typed<T, VEC, W>(a, stream)
+  DWARF_CONV_TYPES(a.dtype, a.D, a.W, DWARF_CONV_CALL)
+#undef DWARF_CONV_CALL
+  return hipGetLastError();
+}
+
+}  // namespace dwarf

@@ -29,6 +29,7 @@ from typing import Optional
 import torch
 
 from . import block as _block
+from . import conv as _conv
 from . import dsqg as _dsqg
 from . import ema as _ema
 from . import linattn as _linattn
@@ -37,6 +38,7 @@ from . import npci as _npci
 from . import packet as _packet
 from . import probe as _probe
 from . import rotary as _rotary
+from . import selscan as _selscan
 
 Tensor = torch.Tensor
 
@@ -441,3 +443,177 @@ def linear_attention_step_(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s
 @linear_attention_step_.register_fake
 def _linear_attention_step__fake(q, k, v, log_decay, state, slots, scale):
     return q.new_empty(q.shape)
+
+
+# ---- RMS norm --------------------------------------------------------------------------------
+def _or_none(t: Optional[Tensor], like: Tensor) -> Tensor:
+    return t if t is not None else like.new_empty((0,))
+
+
+@torch.library.custom_op("dwarf::rms_norm_fwd", mutates_args=())
+def rms_norm_fwd(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], groups: int, eps: float
+                 ) -> tuple[Tensor, Tensor]:
+    """(y of x's dtype, the sum of residual's or empty [0]), contiguous."""
+    y, total, _ = _norm.rms_forward(x, weight, residual, groups, eps, False)
+    return y, _or_none(total, x)
+
+
+@rms_norm_fwd.register_fake
+def _rms_norm_fwd_fake(x, weight, residual, groups, eps):
+    return x.new_empty(x.shape), x.new_empty((0,)) if residual is None else residual.new_empty(x.shape)
+
+
+@torch.library.custom_op("dwarf::rms_norm_fp8", mutates_args=())
+def rms_norm_fp8(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], groups: int, eps: float
+                 ) -> tuple[Tensor, Tensor, Tensor]:
+    """(q in e4m3, scales fp32 [..., 1], the sum of residual's dtype or empty [0])."""
+    q, total, scale = _norm.rms_forward(x, weight, residual, groups, eps, True)
+    return q, scale, _or_none(total, x)
+
+
+@rms_norm_fp8.register_fake
+def _rms_norm_fp8_fake(x, weight, residual, groups, eps):
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty((*x.shape[:-1], 1), dtype=torch.float32),
+            x.new_empty((0,)) if residual is None else residual.new_empty(x.shape))
+
+
+@torch.library.custom_op("dwarf::rms_norm_bwd", mutates_args=())
+def rms_norm_bwd(dy: Tensor, dsum: Optional[Tensor], stream: Tensor, weight: Optional[Tensor], groups: int, eps: float,
+                 need_dx: bool, need_dr: bool, need_dw: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """(dx of dy's dtype, dresidual of the stream's, dweight fp32 [groups * D]); empty [0] where not needed."""
+    dx, dr, dw = _norm.rms_backward(dy, dsum, stream, weight, groups, eps, need_dx, need_dr, need_dw)
+    if dx is not None and dr is not None and dr.data_ptr() == dx.data_ptr():
+        dr = dr.clone()   # the results of a custom op share no memory
+    return _or_none(dx, dy), _or_none(dr, stream), _or_empty(dw, stream)
+
+
+@rms_norm_bwd.register_fake
+def _rms_norm_bwd_fake(dy, dsum, stream, weight, groups, eps, need_dx, need_dr, need_dw):
+    return (dy.new_empty(dy.shape if need_dx else (0,)), stream.new_empty(stream.shape if need_dr else (0,)),
+            stream.new_empty((groups * stream.shape[-1] if need_dw else 0,), dtype=torch.float32))
+
+
+# ---- short causal convolution ----------------------------------------------------------------
+@torch.library.custom_op("dwarf::causal_conv_fwd", mutates_args=())
+def causal_conv_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], initial: Optional[Tensor],
+                    lengths: Optional[Tensor], silu: bool, want_state: bool) -> tuple[Tensor, Tensor]:
+    """(y, the final state or empty [0])."""
+    y, state = _conv.conv_forward(x, weight, bias, initial, lengths, silu, want_state)
+    return y, _or_none(state, x)
+
+
+@causal_conv_fwd.register_fake
+def _causal_conv_fwd_fake(x, weight, bias, initial, lengths, silu, want_state):
+    state = (x.shape[0], weight.shape[1] - 1, x.shape[2]) if want_state else (0,)
+    return x.new_empty(x.shape), x.new_empty(state)
+
+
+@torch.library.custom_op("dwarf::causal_conv_bwd", mutates_args=())
+def causal_conv_bwd(dy: Tensor, dstate: Optional[Tensor], x: Tensor, weight: Tensor, bias: Optional[Tensor],
+                    initial: Optional[Tensor], lengths: Optional[Tensor], silu: bool, need_w: bool, need_b: bool,
+                    need_initial: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(dx, dweight [D,W] and dbias [D] fp32, dinitial); empty [0] where not needed."""
+    dx, dw, db, di = _conv.conv_backward(dy, dstate, x, weight, bias, initial, lengths, silu, need_w, need_b, need_initial)
+    return dx, _or_empty(dw, x), _or_empty(db, x), _or_none(di, x)
+
+
+@causal_conv_bwd.register_fake
+def _causal_conv_bwd_fake(dy, dstate, x, weight, bias, initial, lengths, silu, need_w, need_b, need_initial):
+    f32 = torch.float32
+    return (x.new_empty(x.shape), x.new_empty(weight.shape if need_w else (0,), dtype=f32),
+            x.new_empty((x.shape[2] if need_b else 0,), dtype=f32),
+            x.new_empty((x.shape[0], weight.shape[1] - 1, x.shape[2]) if need_initial else (0,)))
+
+
+@torch.library.custom_op("dwarf::causal_conv_step", mutates_args=("new_state",))
+def causal_conv_step(x: Tensor, weight: Tensor, bias: Optional[Tensor], state: Tensor, new_state: Tensor,
+                     slots: Optional[Tensor], silu: bool) -> Tensor:
+    """One token of each row, the states going from one pool to another; out [rows,D]."""
+    return _conv.conv_step(x, weight, bias, state, new_state, slots, silu)
+
+
+@causal_conv_step.register_fake
+def _causal_conv_step_fake(x, weight, bias, state, new_state, slots, silu):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("dwarf::causal_conv_step_", mutates_args=("state",))
+def causal_conv_step_(x: Tensor, weight: Tensor, bias: Optional[Tensor], state: Tensor, slots: Optional[Tensor],
+                      silu: bool) -> Tensor:
+    """One token of each row, the pool updated in place; out [rows,D]."""
+    return _conv.conv_step(x, weight, bias, state, None, slots, silu)
+
+
+@causal_conv_step_.register_fake
+def _causal_conv_step__fake(x, weight, bias, state, slots, silu):
+    return x.new_empty(x.shape)
+
+
+# ---- selective scan --------------------------------------------------------------------------
+@torch.library.custom_op("dwarf::selective_scan_fwd", mutates_args=())
+def selective_scan_fwd(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, skip: Optional[Tensor],
+                       gate: Optional[Tensor], delta_bias: Optional[Tensor], initial: Optional[Tensor],
+                       lengths: Optional[Tensor], softplus: bool, want_state: bool, want_checkpoints: bool
+                       ) -> tuple[Tensor, Tensor, Tensor]:
+    """(y, the final state or empty [0], the backward's checkpoints or empty [0])."""
+    y, state, checkpoints = _selscan.scan_forward(x, delta, A, B, C, skip, gate, delta_bias, initial, lengths, softplus,
+                                                  want_state, want_checkpoints)
+    return y, _or_empty(state, x), _or_empty(checkpoints, x)
+
+
+@selective_scan_fwd.register_fake
+def _selective_scan_fwd_fake(x, delta, A, B, C, skip, gate, delta_bias, initial, lengths, softplus, want_state,
+                             want_checkpoints):
+    (b, n, d), s, f32 = x.shape, A.shape[1], torch.float32
+    return (x.new_empty(x.shape), x.new_empty((b, d, s) if want_state else (0,), dtype=f32),
+            x.new_empty((_selscan.checkpoint_elements(b, n, d, s) if want_checkpoints else 0,), dtype=f32))
+
+
+@torch.library.custom_op("dwarf::selective_scan_bwd", mutates_args=())
+def selective_scan_bwd(dy: Tensor, dstate: Optional[Tensor], x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor,
+                       skip: Optional[Tensor], gate: Optional[Tensor], delta_bias: Optional[Tensor],
+                       initial: Optional[Tensor], lengths: Optional[Tensor], checkpoints: Tensor, softplus: bool,
+                       need_A: bool, need_skip: bool, need_bias: bool, need_initial: bool
+                       ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(dx, ddelta, dA, dB, dC, dskip, dgate, ddelta_bias, dinitial); empty [0] where there is none."""
+    dx, dd, dA, dB, dC, dskip, dgate, dbias, dinitial = _selscan.scan_backward(
+        dy, dstate, x, delta, A, B, C, skip, gate, delta_bias, initial, lengths, checkpoints, softplus, need_A, need_skip,
+        need_bias, need_initial)
+    return (dx, dd, _or_empty(dA, x), dB, dC, _or_empty(dskip, x), _or_none(dgate, x), _or_empty(dbias, x),
+            _or_empty(dinitial, x))
+
+
+@selective_scan_bwd.register_fake
+def _selective_scan_bwd_fake(dy, dstate, x, delta, A, B, C, skip, gate, delta_bias, initial, lengths, checkpoints, softplus,
+                             need_A, need_skip, need_bias, need_initial):
+    (b, _, d), s, f32 = x.shape, A.shape[1], torch.float32
+    return (x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty((d, s) if need_A else (0,), dtype=f32),
+            x.new_empty(B.shape), x.new_empty(C.shape), x.new_empty((d if need_skip else 0,), dtype=f32),
+            x.new_empty(x.shape if gate is not None else (0,)), x.new_empty((d if need_bias else 0,), dtype=f32),
+            x.new_empty((b, d, s) if need_initial else (0,), dtype=f32))
+
+
+@torch.library.custom_op("dwarf::selective_scan_step", mutates_args=("new_state",))
+def selective_scan_step(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, state: Tensor, new_state: Tensor,
+                        skip: Optional[Tensor], gate: Optional[Tensor], delta_bias: Optional[Tensor],
+                        slots: Optional[Tensor], softplus: bool) -> Tensor:
+    """One token of each row, the states going from one pool to another; out [rows,D]."""
+    return _selscan.scan_step(x, delta, A, B, C, state, new_state, skip, gate, delta_bias, slots, softplus)
+
+
+@selective_scan_step.register_fake
+def _selective_scan_step_fake(x, delta, A, B, C, state, new_state, skip, gate, delta_bias, slots, softplus):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("dwarf::selective_scan_step_", mutates_args=("state",))
+def selective_scan_step_(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, state: Tensor, skip: Optional[Tensor],
+                         gate: Optional[Tensor], delta_bias: Optional[Tensor], slots: Optional[Tensor], softplus: bool
+                         ) -> Tensor:
+    """One token of each row, the pool updated in place; out [rows,D]."""
+    return _selscan.scan_step(x, delta, A, B, C, state, None, skip, gate, delta_bias, slots, softplus)
+
+
+@selective_scan_step_.register_fake
+def _selective_scan_step__fake(x, delta, A, B, C, state, skip, gate, delta_bias, slots, softplus):
+    return x.new_empty(x.shape)

@@ -14,7 +14,7 @@
 extern "C" {
 #endif
 
-/* fp16 elements: a dtype of this header's entry points only (with DWARF_BF16 and DWARF_F32). */
+/* fp16 elements: a dtype of this header's entry points and dwarf_selective.h's only (with DWARF_BF16 and DWARF_F32). */
 #define DWARF_F16 2
 
 /*
