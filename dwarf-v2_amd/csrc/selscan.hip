@@ -73,8 +73,32 @@ __device__ __forceinline__ float quad_sums(float p0, float p1, float p2, float p
   return (high ? b : a) + dpp_f<0x4E>(high ? a : b);
 }
 
-__device__ __forceinline__ float step_of(float raw, int softplus) {
-  return !softplus ? raw : raw > 20.f ? raw : log1pf(expf(raw));
+// e^x with the argument's rounding to base 2 made up for: 2^-23 off at most (plus the instruction's own last bit).
+__device__ __forceinline__ float exp_f32(float x) {
+  const float h = x * kLog2e;
+  const float lo = fmaf(x, 1.92596299e-8f, fmaf(x, kLog2e, -h));   // log2(e) - kLog2e
+  return __builtin_amdgcn_exp2f(h) * fmaf(lo, 0.693147181f, 1.f);
+}
+
+// log(1 + e^x) without a branch.  log(w) / (w - 1) changes slowly around the rounded w = 1 + e (and is 1 where w is next to
+// 1), so that times the exact e it is right however small e is: 3.5e-7 off at most over [-30, 21], 8e-8 on average.  Above 20
+// it is x.  (The library's calls, with their branches, took half of the forward's instructions.)
+__device__ __forceinline__ float softplus_f32(float x) {
+  const float low = x > 20.f ? 20.f : x;
+  const float e = exp_f32(low), w = fmaxf(1.f + e, 1.00000012f);
+  return fmaf(__builtin_amdgcn_logf(w) * 0.693147181f, e * __builtin_amdgcn_rcpf(w - 1.f), x - low);
+}
+// Chosen, not branched to: a branch for each quad of tokens keeps the compiler from working on several of them at once.
+__device__ __forceinline__ float step_of(float raw, bool softplus) {
+  const float s = softplus_f32(raw);
+  return softplus ? s : raw;
+}
+// What step_of makes a step of 0 of.
+__device__ __forceinline__ float no_step(bool softplus) { return softplus ? -1e4f : 0.f; }
+// silu(z), or 1 without a gate.
+__device__ __forceinline__ float act_of(float z, bool gated) {
+  const float s = z * sigmoid_f32(z);
+  return gated ? s : 1.f;
 }
 
 // Where a lane stands.
@@ -106,27 +130,70 @@ __device__ __forceinline__ int scan_length(const dwarf_selective_scan_fwd_args& 
   return n < 0 ? 0 : n > a.N ? a.N : n;
 }
 
-// B or C rows of TOK tokens from t on, as the workgroup's threads carry them into LDS: raw in registers between.
+// Rows are addressed by a base that all threads share, which walks with the tiles, and 32-bit byte offsets of the threads
+// (the host keeps token strides below 2^22 elements).  Tokens behind the live ones read the last live one again: an offset is
+// at most `limit`, one instruction, where a second path for a sequence's last tile would make the compiler wait for its loads
+// where the paths meet.
+constexpr uint32_t kNoLimit = 0xffffffffu;
+
+// B or C rows of TOK tokens, as the workgroup's threads carry them into LDS: raw in registers between.
 template <typename T, int SP, int TOK>
 struct BcRows {
-  static constexpr int kEach = (TOK * SP + kScanThreads - 1) / kScanThreads;
+  static_assert(TOK * SP % kScanThreads == 0 && kScanThreads % SP == 0, "whole rows, each thread one state");
+  static constexpr int kEach = TOK * SP / kScanThreads, kRows = kScanThreads / SP;
+  const char* base;   // the tile's first row
+  uint32_t stride, state, off;   // bytes: of a token, of the thread's state, of its first row and state
   T v[kEach];
-  __device__ __forceinline__ void load(const T* p, int64_t stride, int t, int end, int S) {
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = e * kScanThreads + threadIdx.x, s = i % SP;
-      int tt = t + i / SP;
-      if (tt >= end) tt = end - 1;
-      v[e] = p[tt * stride + (s < S ? s : 0)];
-    }
+  __device__ __forceinline__ BcRows(const T* p, int64_t stride_, int t, int S)
+      : base(reinterpret_cast<const char*>(p + t * stride_)), stride(static_cast<uint32_t>(stride_) * sizeof(T)) {
+    const uint32_t s = threadIdx.x % SP;
+    state = (s < static_cast<uint32_t>(S) ? s : 0) * sizeof(T);
+    off = threadIdx.x / SP * stride + state;
   }
-  // rows from `end` on and states from S on are zero
-  __device__ __forceinline__ void store(float* to, int t, int end, int S) const {
+  __device__ __forceinline__ void move(int tiles) { base += tiles * (TOK * static_cast<int64_t>(stride)); }
+  __device__ __forceinline__ void load(int live) {   // of the tile's rows
+    const uint32_t limit = live < TOK ? (live - 1) * stride + state : kNoLimit;
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = e * kScanThreads + threadIdx.x, s = i % SP;
-      if (TOK * SP % kScanThreads == 0 || i < TOK * SP) to[i] = s < S && t + i / SP < end ? to_f32(v[e]) : 0.f;
-    }
+    for (int e = 0; e < kEach; ++e) v[e] = *reinterpret_cast<const T*>(base + min(off + e * (kRows * stride), limit));
+  }
+  // rows from `live` on and states from S on are zero
+  __device__ __forceinline__ void store(float* to, int live, int S) const {
+    const bool in = static_cast<int>(threadIdx.x % SP) < S;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      to[e * kScanThreads + threadIdx.x] = in && static_cast<int>(threadIdx.x / SP) + e * kRows < live ? to_f32(v[e]) : 0.f;
+  }
+};
+
+// A lane's tokens of a channel, one of each quad of a tile of 4 QUADS.
+template <typename T, int QUADS>
+struct QuadRows {
+  char* base;   // the tile's first token
+  uint32_t stride, channel, off;   // bytes: of a token, of the channel, of the lane's first token and channel
+  __device__ __forceinline__ QuadRows(const void* p, int64_t sequence, int64_t stride_, int64_t d, int t, int quad)
+      : base(reinterpret_cast<char*>(static_cast<T*>(const_cast<void*>(p)) + sequence + t * stride_)),
+        stride(static_cast<uint32_t>(stride_) * sizeof(T)), channel(static_cast<uint32_t>(d) * sizeof(T)) {
+    off = quad * stride + channel;
+  }
+  __device__ __forceinline__ void move(int tiles) { base += tiles * (4 * QUADS * static_cast<int64_t>(stride)); }
+  __device__ __forceinline__ void load(T* v, int live) const {   // of the tile's tokens
+    const uint32_t limit = live < 4 * QUADS ? (live - 1) * stride + channel : kNoLimit;
+#pragma unroll
+    for (int k = 0; k < QUADS; ++k) v[k] = *reinterpret_cast<const T*>(base + min(off + k * (4 * stride), limit));
+  }
+  __device__ __forceinline__ void store(const float* x) const {
+#pragma unroll
+    for (int k = 0; k < QUADS; ++k) *reinterpret_cast<T*>(base + (off + k * (4 * stride))) = from_f32<T>(x[k]);
+  }
+  __device__ __forceinline__ void store(const float* x, int quad, int live) const {
+#pragma unroll
+    for (int k = 0; k < QUADS; ++k)
+      if (4 * k + quad < live) *reinterpret_cast<T*>(base + (off + k * (4 * stride))) = from_f32<T>(x[k]);
+  }
+  // zeros from the sequence's token `from` to `to`; `t` is the tile's first
+  __device__ __forceinline__ void clear(int t, int quad, int from, int to) const {
+    for (int i = from + quad; i < to; i += 4)
+      *reinterpret_cast<T*>(base + static_cast<int64_t>(i - t) * stride + channel) = from_f32<T>(0.f);
   }
 };
 
@@ -176,7 +243,7 @@ __device__ __forceinline__ void load_rates(const float* A, int64_t d, int s0, in
 
 // LOCAL: what a segment adds from zero and its sum of steps, for all segments but the last; otherwise the rows.
 template <typename T, int SPL, int LPC, bool LOCAL>
-__global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(dwarf_selective_scan_fwd_args a, ScanGeom gm) {
+__global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void scan_fwd_kernel(dwarf_selective_scan_fwd_args a, ScanGeom gm) {
   constexpr int SP = SPL * LPC, kQuads = kTile / 4, kK = scan_chunk(SPL);
   __shared__ __align__(16) float s_b[2][kTile * SP];
   __shared__ __align__(16) float s_c[LOCAL ? 1 : 2][LOCAL ? 4 : kTile * SP];
@@ -201,82 +268,100 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(dwarf_selective_
       for (int s = 0; s < SPL; ++s) h[s] = fmaf(__builtin_amdgcn_exp2f(sum * rate[s]), h[s], add[s]);
     }
   }
-  const T* px = static_cast<const T*>(a.x) + at.b * a.x_stride[0] + d;
-  const T* pd = static_cast<const T*>(a.delta) + at.b * a.delta_stride[0] + d;
-  const T* pz = static_cast<const T*>(a.gate) + at.b * a.gate_stride[0] + d;
-  const T* pB = static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2];
-  const T* pC = static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
-  T* py = static_cast<T*>(a.y) + at.b * a.y_stride[0] + d;
-  const bool gated = !LOCAL && a.gate, writes = at.in && at.sq < 4;
+  const bool gated = !LOCAL && a.gate, softplus = a.softplus, writes = at.in && at.sq < 4;
+  const float none = no_step(softplus);
+  using Rows = QuadRows<T, kQuads>;
+  Rows px(a.x, at.b * a.x_stride[0], a.x_stride[1], d, t0, quad);
+  Rows pd(a.delta, at.b * a.delta_stride[0], a.delta_stride[1], d, t0, quad);
+  Rows pz(a.gate, at.b * a.gate_stride[0], a.gate_stride[1], d, t0, quad);
+  Rows py(a.y, at.b * a.y_stride[0], a.y_stride[1], d, t0, quad);
+  BcRows<T, SP, kTile> rb(static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2], a.B_stride[1], t0, a.S);
+  BcRows<T, SP, kTile> rc(static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2], a.C_stride[1], t0, a.S);
   float* ck = !LOCAL && a.checkpoints && at.in
-                  ? a.checkpoints + (static_cast<int64_t>(at.b) * ((a.N + kK - 1) / kK) * a.D + d) * SP + s0 : nullptr;
-  float total = 0.f;
+                  ? a.checkpoints + ((static_cast<int64_t>(at.b) * ((a.N + kK - 1) / kK) + t0 / kK) * a.D + d) * SP + s0 : nullptr;
+  const int64_t ck_step = static_cast<int64_t>(a.D) * SP;
+  float total = 0.f, u[kQuads], raw[kQuads], z[kQuads];
   T rx[kQuads], rd[kQuads], rz[kQuads];
-  BcRows<T, SP, kTile> rb, rc;
-  // a tile's loads: tokens behind the live ones read the last live one again
-  auto fetch = [&](int t) {
-    rb.load(pB, a.B_stride[1], t, end, a.S);
-    if constexpr (!LOCAL) rc.load(pC, a.C_stride[1], t, end, a.S);
+  auto fetch = [&](int live) {   // the tile's first `live` tokens are live
+    rb.load(live);
+    if constexpr (!LOCAL) rc.load(live);
+    px.load(rx, live);
+    pd.load(rd, live);
+    if (gated) pz.load(rz, live);
+  };
+  auto take = [&](int to, int live) {
+    rb.store(s_b[to], live, a.S);
+    if constexpr (!LOCAL) rc.store(s_c[to], live, a.S);
 #pragma unroll
     for (int k = 0; k < kQuads; ++k) {
-      const int64_t tt = min(t + 4 * k + quad, end - 1);
-      rx[k] = px[tt * a.x_stride[1]];
-      rd[k] = pd[tt * a.delta_stride[1]];
-      if (gated) rz[k] = pz[tt * a.gate_stride[1]];
+      const bool in = 4 * k + quad < live;
+      const float vx = to_f32(rx[k]), vd = to_f32(rd[k]) + bias, vz = to_f32(rz[k]);
+      u[k] = in ? vx : 0.f;
+      raw[k] = in ? vd : none;
+      z[k] = gated ? vz : 0.f;
     }
   };
   int buf = 0;
-  if (t0 < end) {
-    fetch(t0);
-    rb.store(s_b[0], t0, end, a.S);
-    if constexpr (!LOCAL) rc.store(s_c[0], t0, end, a.S);
+  if (t0 < end) {   // around the loop too: one that might not run would wait inside for what is loaded in front of it
+    fetch(end - t0);
+    take(0, end - t0);
     __syncthreads();
-  }
-  for (int t = t0; t < end; t += kTile, buf ^= 1) {
-    float u[kQuads], dl[kQuads], z[kQuads];
+    for (int t = t0; t < end; t += kTile, buf ^= 1) {
+      const bool more = t + kTile < end;
+      if (more) {   // under way while this tile is worked on
+        rb.move(1);
+        rc.move(1);
+        px.move(1);
+        pd.move(1);
+        pz.move(1);
+        fetch(end - t - kTile);
+      }
+      // A quad at a time; the next one's rows and steps are formed meanwhile, which the compiler does not do by itself.
+      float o[kQuads], B[2][4 * SPL], C[2][4 * SPL], st[2], su[2];
+      auto begin = [&](int k) {
 #pragma unroll
-    for (int k = 0; k < kQuads; ++k) {
-      u[k] = to_f32(rx[k]);
-      dl[k] = to_f32(rd[k]);
-      z[k] = gated ? to_f32(rz[k]) : 0.f;
-    }
-    const bool more = t + kTile < end;
-    if (more) fetch(t + kTile);   // under way while this tile is worked on
-#pragma unroll
-    for (int k = 0; k < kQuads; ++k) {
-      if (!LOCAL && 4 * k % kK == 0 && ck && t + 4 * k < end)
-        store_states<SPL>(ck + static_cast<int64_t>((t + 4 * k) / kK) * a.D * SP, h);
-      const int tk = t + 4 * k + quad;
-      const bool live = tk < end;
-      const float st = live ? step_of(dl[k] + bias, a.softplus) : 0.f;
-      const float su = live ? st * u[k] : 0.f;
-      if constexpr (LOCAL) total += st;
-      const float stj[4] = {quad_lane<0>(st), quad_lane<1>(st), quad_lane<2>(st), quad_lane<3>(st)};
-      const float suj[4] = {quad_lane<0>(su), quad_lane<1>(su), quad_lane<2>(su), quad_lane<3>(su)};
-      float p[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float B[SPL], C[SPL];
-        load_states<SPL>(s_b[buf] + (4 * k + j) * SP + s0, B);
-        if constexpr (!LOCAL) load_states<SPL>(s_c[buf] + (4 * k + j) * SP + s0, C);
-        p[j] = 0.f;
-#pragma unroll
-        for (int s = 0; s < SPL; ++s) {
-          h[s] = fmaf(__builtin_amdgcn_exp2f(stj[j] * rate[s]), h[s], suj[j] * B[s]);
-          if constexpr (!LOCAL) p[j] = fmaf(h[s], C[s], p[j]);
+        for (int j = 0; j < 4; ++j) {
+          load_states<SPL>(s_b[buf] + (4 * k + j) * SP + s0, B[k & 1] + j * SPL);
+          if constexpr (!LOCAL) load_states<SPL>(s_c[buf] + (4 * k + j) * SP + s0, C[k & 1] + j * SPL);
         }
+        st[k & 1] = step_of(raw[k], softplus);
+        su[k & 1] = st[k & 1] * u[k];
+        if constexpr (LOCAL) total += st[k & 1];
+      };
+      begin(0);
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) {
+        if (!LOCAL && 4 * k % kK == 0) {
+          if (ck && t + 4 * k < end) store_states<SPL>(ck, h);
+          ck += ck ? ck_step : 0;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (k + 1 < kQuads) begin(k + 1);
+        const float stj[4] = {quad_lane<0>(st[k & 1]), quad_lane<1>(st[k & 1]), quad_lane<2>(st[k & 1]), quad_lane<3>(st[k & 1])};
+        const float suj[4] = {quad_lane<0>(su[k & 1]), quad_lane<1>(su[k & 1]), quad_lane<2>(su[k & 1]), quad_lane<3>(su[k & 1])};
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          p[j] = 0.f;
+#pragma unroll
+          for (int s = 0; s < SPL; ++s) {
+            h[s] = fmaf(__builtin_amdgcn_exp2f(stj[j] * rate[s]), h[s], suj[j] * B[k & 1][j * SPL + s]);
+            if constexpr (!LOCAL) p[j] = fmaf(h[s], C[k & 1][j * SPL + s], p[j]);
+          }
+        }
+        if constexpr (!LOCAL)
+          o[k] = fmaf(skip, u[k], quad_sums<LPC>(p[0], p[1], p[2], p[3], at.lane)) * act_of(z[k], gated);
       }
-      if constexpr (!LOCAL) {
-        float o = fmaf(skip, u[k], quad_sums<LPC>(p[0], p[1], p[2], p[3], at.lane));
-        if (gated) o *= z[k] * sigmoid_f32(z[k]);
-        if (live && writes) py[tk * a.y_stride[1]] = from_f32<T>(o);
+      // The next tile's values are waited for in front of this one's stores: loads and stores are counted together, and waiting
+      // behind them would wait for the stores too (an eighth of the time).
+      if (more) take(buf ^ 1, end - t - kTile);
+      if (!LOCAL && writes) {
+        if (t + kTile <= end) py.store(o);
+        else py.store(o, quad, end - t);
       }
+      py.move(1);
+      __syncthreads();
     }
-    if (more) {
-      rb.store(s_b[buf ^ 1], t + kTile, end, a.S);
-      if constexpr (!LOCAL) rc.store(s_c[buf ^ 1], t + kTile, end, a.S);
-    }
-    __syncthreads();
   }
   if constexpr (LOCAL) {
     total = group_sum<4>(total);   // each quad has all tokens
@@ -286,8 +371,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(dwarf_selective_
       if (at.sq == 0) gm.steps[row] = total;
     }
   } else {
-    if (writes)
-      for (int t = max(t0, end) + quad; t < t1; t += 4) py[t * a.y_stride[1]] = from_f32<T>(0.f);
+    if (writes) Rows(a.y, at.b * a.y_stride[0], a.y_stride[1], d, t0, quad).clear(t0, quad, max(t0, end), t1);
     if (a.final && at.seg == gm.segs - 1 && at.in)
       store_user_states<SPL>(a.final + (static_cast<int64_t>(at.b) * a.D + d) * a.S, s0, a.S, h);
   }
@@ -296,7 +380,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(dwarf_selective_
 // The adjoint that leaves a segment through its front for none that enters at its end, and the sum of its steps; for all
 // segments but the first.
 template <typename T, int SPL, int LPC>
-__global__ __launch_bounds__(kScanThreads) void scan_adjoint_kernel(dwarf_selective_scan_bwd_args w, ScanGeom gm) {
+__global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void scan_adjoint_kernel(dwarf_selective_scan_bwd_args w, ScanGeom gm) {
   constexpr int SP = SPL * LPC, kQuads = kTile / 4;
   __shared__ __align__(16) float s_c[2][kTile * SP];
   const dwarf_selective_scan_fwd_args& a = w.fwd;
@@ -310,60 +394,67 @@ __global__ __launch_bounds__(kScanThreads) void scan_adjoint_kernel(dwarf_select
   const float bias = a.delta_bias ? a.delta_bias[d] : 0.f;
 #pragma unroll
   for (int s = 0; s < SPL; ++s) ga[s] = 0.f;
-  const T* pd = static_cast<const T*>(a.delta) + at.b * a.delta_stride[0] + d;
-  const T* pz = static_cast<const T*>(a.gate) + at.b * a.gate_stride[0] + d;
-  const T* pg = static_cast<const T*>(w.dy) + at.b * w.dy_stride[0] + d;
-  const T* pC = static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
-  const bool gated = a.gate != nullptr;
-  float total = 0.f;
+  const bool gated = a.gate != nullptr, softplus = a.softplus;
+  const float none = no_step(softplus);
+  const int tiles = end > t0 ? (end - t0 + kTile - 1) / kTile : 0, last = t0 + (tiles - 1) * kTile;
+  using Rows = QuadRows<T, kQuads>;
+  Rows pd(a.delta, at.b * a.delta_stride[0], a.delta_stride[1], d, last, quad);
+  Rows pz(a.gate, at.b * a.gate_stride[0], a.gate_stride[1], d, last, quad);
+  Rows pg(w.dy, at.b * w.dy_stride[0], w.dy_stride[1], d, last, quad);
+  BcRows<T, SP, kTile> rc(static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2], a.C_stride[1], last, a.S);
+  float total = 0.f, raw[kQuads], go[kQuads];
   T rg[kQuads], rd[kQuads], rz[kQuads];
-  BcRows<T, SP, kTile> rc;
-  auto fetch = [&](int t) {
-    rc.load(pC, a.C_stride[1], t, end, a.S);
+  auto take = [&](int to, int live) {
+    rc.store(s_c[to], live, a.S);
 #pragma unroll
     for (int k = 0; k < kQuads; ++k) {
-      const int64_t tt = min(t + 4 * k + quad, end - 1);
-      rg[k] = pg[tt * w.dy_stride[1]];
-      rd[k] = pd[tt * a.delta_stride[1]];
-      if (gated) rz[k] = pz[tt * a.gate_stride[1]];
+      const bool in = 4 * k + quad < live;
+      const float vd = to_f32(rd[k]) + bias, vg = to_f32(rg[k]), vz = to_f32(rz[k]);
+      raw[k] = in ? vd : none;
+      go[k] = (in ? vg : 0.f) * act_of(in && gated ? vz : 0.f, gated);
     }
   };
-  const int tiles = end > t0 ? (end - t0 + kTile - 1) / kTile : 0;
   int buf = 0;
   if (tiles) {
-    fetch(t0 + (tiles - 1) * kTile);
-    rc.store(s_c[0], t0 + (tiles - 1) * kTile, end, a.S);
+    rc.load(end - last);
+    pd.load(rd, end - last);
+    pg.load(rg, end - last);
+    if (gated) pz.load(rz, end - last);
+    take(0, end - last);
     __syncthreads();
-  }
-  for (int i = tiles - 1; i >= 0; --i, buf ^= 1) {
-    const int t = t0 + i * kTile;
-    float dy[kQuads], dl[kQuads], z[kQuads];
-#pragma unroll
-    for (int k = 0; k < kQuads; ++k) {
-      dy[k] = to_f32(rg[k]);
-      dl[k] = to_f32(rd[k]);
-      z[k] = gated ? to_f32(rz[k]) : 0.f;
-    }
-    if (i) fetch(t - kTile);
-#pragma unroll
-    for (int k = kQuads - 1; k >= 0; --k) {
-      const bool live = t + 4 * k + quad < end;
-      const float st = live ? step_of(dl[k] + bias, a.softplus) : 0.f;
-      const float act = gated ? z[k] * sigmoid_f32(z[k]) : 1.f;
-      const float go = live ? dy[k] * act : 0.f;
-      total += st;
-      const float stj[4] = {quad_lane<0>(st), quad_lane<1>(st), quad_lane<2>(st), quad_lane<3>(st)};
-      const float goj[4] = {quad_lane<0>(go), quad_lane<1>(go), quad_lane<2>(go), quad_lane<3>(go)};
-#pragma unroll
-      for (int j = 3; j >= 0; --j) {
-        float C[SPL];
-        load_states<SPL>(s_c[buf] + (4 * k + j) * SP + s0, C);
-#pragma unroll
-        for (int s = 0; s < SPL; ++s) ga[s] = __builtin_amdgcn_exp2f(stj[j] * rate[s]) * fmaf(C[s], goj[j], ga[s]);
+    for (int i = tiles - 1; i >= 0; --i, buf ^= 1) {
+      if (i) {   // all tiles in front of the last are whole
+        rc.move(-1);
+        pd.move(-1);
+        pg.move(-1);
+        pz.move(-1);
+        rc.load(kTile);
+        pd.load(rd, kTile);
+        pg.load(rg, kTile);
+        if (gated) pz.load(rz, kTile);
       }
+      float C[2][4 * SPL], st[2];
+      auto begin = [&](int k) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) load_states<SPL>(s_c[buf] + (4 * k + j) * SP + s0, C[k & 1] + j * SPL);
+        st[k & 1] = step_of(raw[k], softplus);
+        total += st[k & 1];
+      };
+      begin(kQuads - 1);
+#pragma unroll
+      for (int k = kQuads - 1; k >= 0; --k) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (k) begin(k - 1);
+        const float stj[4] = {quad_lane<0>(st[k & 1]), quad_lane<1>(st[k & 1]), quad_lane<2>(st[k & 1]), quad_lane<3>(st[k & 1])};
+        const float goj[4] = {quad_lane<0>(go[k]), quad_lane<1>(go[k]), quad_lane<2>(go[k]), quad_lane<3>(go[k])};
+#pragma unroll
+        for (int j = 3; j >= 0; --j)
+#pragma unroll
+          for (int s = 0; s < SPL; ++s) ga[s] = __builtin_amdgcn_exp2f(stj[j] * rate[s]) * fmaf(C[k & 1][j * SPL + s], goj[j], ga[s]);
+      }
+      if (i) take(buf ^ 1, kTile);
+      __syncthreads();
     }
-    if (i) rc.store(s_c[buf ^ 1], t - kTile, end, a.S);
-    __syncthreads();
   }
   total = group_sum<4>(total);
   const int64_t row = (static_cast<int64_t>(at.b) * gm.segs + at.seg) * a.D + d;
@@ -373,7 +464,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_adjoint_kernel(dwarf_select
   }
 }
 
-// Sums v[0 .. M-1] over the wave's channels (the lane bits above LPC's); lane l keeps value `which(l)` of them.
+// Sums v[0 .. M-1] over the wave's channels (the lane bits above LPC's); lane l gets values which(l) .. which(l) + kLeft - 1.
 template <int LPC, int M>
 struct ChannelSums {
   static constexpr int kLeft = M >= 8 ? M / 8 : 1;   // values a lane ends with
@@ -403,24 +494,20 @@ struct ChannelSums {
     }
     if constexpr (LPC == 4) {
 #pragma unroll
-      for (int i = 0; i < kLeft; ++i) out[i] += dpp_f<0x104>(out[i]);   // row_shl:4, for the lanes that write
+      for (int i = 0; i < kLeft; ++i) out[i] += dpp_f<0x1B>(dpp_f<0x141>(out[i]));   // lane ^ 7, then ^ 3: the other quad
     }
   }
   static __device__ __forceinline__ int which(int lane) {
     return (lane >> 5 & 1) * (M / 2) + (lane >> 4 & 1) * (M / 4) + (M >= 8 ? (lane >> 3 & 1) * (M / 8) : 0);
   }
-  // whether the lane is the one that writes its values
-  static __device__ __forceinline__ bool writes(int lane) {
-    return (LPC == 8 || !(lane & 4)) && (M >= 8 || !(lane & 8));
-  }
 };
 
 template <typename T, int SPL, int LPC>
-__global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(dwarf_selective_scan_bwd_args w, ScanGeom gm) {
+__global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void scan_bwd_kernel(dwarf_selective_scan_bwd_args w, ScanGeom gm) {
   constexpr int SP = SPL * LPC, kK = scan_chunk(SPL), kQuads = kK / 4;
   using Sums = ChannelSums<LPC, 2 * SPL>;
   __shared__ __align__(16) float s_b[2][kK * SP], s_c[2][kK * SP];
-  __shared__ float s_sum[kScanWaves][kK][2 * SP];
+  __shared__ float s_sum[2][kScanWaves][kK][2 * SP];
   const dwarf_selective_scan_fwd_args& a = w.fwd;
   const ScanLane<LPC> at(a, gm, gm.segs);
   const int s0 = at.sq * SPL, quad = at.lane & 3;
@@ -441,169 +528,195 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(dwarf_selective_
   if (!at.in)
 #pragma unroll
     for (int s = 0; s < SPL; ++s) ga[s] = 0.f;
-  const T* px = static_cast<const T*>(a.x) + at.b * a.x_stride[0] + d;
-  const T* pd = static_cast<const T*>(a.delta) + at.b * a.delta_stride[0] + d;
-  const T* pz = static_cast<const T*>(a.gate) + at.b * a.gate_stride[0] + d;
-  const T* pg = static_cast<const T*>(w.dy) + at.b * w.dy_stride[0] + d;
-  const T* pB = static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2];
-  const T* pC = static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2];
-  T* ox = static_cast<T*>(w.dx) + at.b * w.dx_stride[0] + d;
-  T* od = static_cast<T*>(w.ddelta) + at.b * w.ddelta_stride[0] + d;
-  T* oz = static_cast<T*>(w.dgate) + at.b * w.dgate_stride[0] + d;
-  const float* ck = a.checkpoints + (static_cast<int64_t>(at.b) * ((a.N + kK - 1) / kK) * a.D + d) * SP + s0;
+  const bool gated = a.gate != nullptr, softplus = a.softplus, writes = at.in && at.sq < 4;
+  const float none = no_step(softplus);
+  const int chunks = end > t0 ? (end - t0 + kK - 1) / kK : 0, last = t0 + (chunks - 1) * kK;
+  using Rows = QuadRows<T, kQuads>;
+  Rows px(a.x, at.b * a.x_stride[0], a.x_stride[1], d, last, quad);
+  Rows pd(a.delta, at.b * a.delta_stride[0], a.delta_stride[1], d, last, quad);
+  Rows pz(a.gate, at.b * a.gate_stride[0], a.gate_stride[1], d, last, quad);
+  Rows pg(w.dy, at.b * w.dy_stride[0], w.dy_stride[1], d, last, quad);
+  Rows ox(w.dx, at.b * w.dx_stride[0], w.dx_stride[1], d, last, quad);
+  Rows od(w.ddelta, at.b * w.ddelta_stride[0], w.ddelta_stride[1], d, last, quad);
+  Rows oz(w.dgate, at.b * w.dgate_stride[0], w.dgate_stride[1], d, last, quad);
+  BcRows<T, SP, kK> rb(static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2], a.B_stride[1], last, a.S);
+  BcRows<T, SP, kK> rc(static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2], a.C_stride[1], last, a.S);
+  const float* ck = a.checkpoints + ((static_cast<int64_t>(at.b) * ((a.N + kK - 1) / kK) + last / kK) * a.D + d) * SP + s0;
   const int64_t ck_step = static_cast<int64_t>(a.D) * SP;
-  const bool gated = a.gate != nullptr, writes = at.in && at.sq < 4;
   float* part = gm.part + ((static_cast<int64_t>(at.tile % gm.tiles_of_group) * a.B + at.b) * a.N * a.G + at.g) * (2 * SP);
+  const int64_t part_step = static_cast<int64_t>(a.G) * (2 * SP);   // from token to token
   double dA[SPL], dskip = 0., dbias = 0.;
 #pragma unroll
   for (int s = 0; s < SPL; ++s) dA[s] = 0.;
   // behind the live tokens everything is zero
-  if (writes)
-    for (int t = max(t0, end) + quad; t < t1; t += 4) {
-      ox[t * w.dx_stride[1]] = from_f32<T>(0.f);
-      od[t * w.ddelta_stride[1]] = from_f32<T>(0.f);
-      if (gated) oz[t * w.dgate_stride[1]] = from_f32<T>(0.f);
-    }
-  for (int64_t i = threadIdx.x + static_cast<int64_t>(max(t0, end)) * (2 * SP); i < static_cast<int64_t>(t1) * (2 * SP); i += kScanThreads)
-    part[i / (2 * SP) * a.G * (2 * SP) + i % (2 * SP)] = 0.f;
+  if (writes) {
+    ox.clear(last, quad, max(t0, end), t1);
+    od.clear(last, quad, max(t0, end), t1);
+    if (gated) oz.clear(last, quad, max(t0, end), t1);
+  }
+  for (int i = threadIdx.x / (2 * SP) + max(t0, end); i < t1; i += kScanThreads / (2 * SP))
+    part[i * part_step + threadIdx.x % (2 * SP)] = 0.f;
 
   T rx[kQuads], rd[kQuads], rz[kQuads], rg[kQuads];
-  float hn[SPL];
-  BcRows<T, SP, kK> rb, rc;
-  auto fetch = [&](int t) {
-    rb.load(pB, a.B_stride[1], t, end, a.S);
-    rc.load(pC, a.C_stride[1], t, end, a.S);
-    load_states<SPL>(ck + t / kK * ck_step, hn);
+  float hn[SPL], u[kQuads], raw[kQuads], z[kQuads], dy[kQuads];
+  // a chunk's values, its B and C to LDS
+  auto take = [&](int to, int live) {
+    rb.store(s_b[to], live, a.S);
+    rc.store(s_c[to], live, a.S);
 #pragma unroll
     for (int k = 0; k < kQuads; ++k) {
-      const int64_t tt = min(t + 4 * k + quad, end - 1);
-      rx[k] = px[tt * a.x_stride[1]];
-      rd[k] = pd[tt * a.delta_stride[1]];
-      rg[k] = pg[tt * w.dy_stride[1]];
-      if (gated) rz[k] = pz[tt * a.gate_stride[1]];
+      const bool in = 4 * k + quad < live && at.in;
+      const float vx = to_f32(rx[k]), vd = to_f32(rd[k]) + bias, vg = to_f32(rg[k]), vz = to_f32(rz[k]);
+      u[k] = in ? vx : 0.f;
+      raw[k] = in ? vd : none;
+      dy[k] = in ? vg : 0.f;
+      z[k] = in && gated ? vz : 0.f;
     }
   };
-  const int chunks = end > t0 ? (end - t0 + kK - 1) / kK : 0;
+  const int place = Sums::which(at.lane) / SPL * SP + s0 + Sums::which(at.lane) % SPL;   // lanes with the same sum write it alike
   int buf = 0;
   if (chunks) {
-    fetch(t0 + (chunks - 1) * kK);
-    rb.store(s_b[0], t0 + (chunks - 1) * kK, end, a.S);
-    rc.store(s_c[0], t0 + (chunks - 1) * kK, end, a.S);
+    const int live = end - last;
+    load_states<SPL>(ck, hn);
+    rb.load(live);
+    rc.load(live);
+    px.load(rx, live);
+    pd.load(rd, live);
+    pg.load(rg, live);
+    if (gated) pz.load(rz, live);
+    take(0, live);
     __syncthreads();
-  }
-  for (int i = chunks - 1; i >= 0; --i, buf ^= 1) {
-    const int t = t0 + i * kK;
-    float h0[SPL], u[kQuads], raw[kQuads], z[kQuads], dy[kQuads], st[kQuads], su[kQuads], go[kQuads];
+    for (int i = chunks - 1; i >= 0; --i, buf ^= 1) {
+      const int t = t0 + i * kK;
+      const bool whole = t + kK <= end;   // all chunks but the last
+      float h0[SPL], st[kQuads], su[kQuads], go[kQuads];
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) h0[s] = hn[s];
-#pragma unroll
-    for (int k = 0; k < kQuads; ++k) {
-      const bool live = t + 4 * k + quad < end && at.in;
-      u[k] = live ? to_f32(rx[k]) : 0.f;
-      raw[k] = to_f32(rd[k]) + bias;
-      dy[k] = live ? to_f32(rg[k]) : 0.f;
-      z[k] = gated ? to_f32(rz[k]) : 0.f;
-    }
-    if (i) fetch(t - kK);
-    // the chunk's states again
-    float dec[kK][SPL], hs[kK][SPL];
-#pragma unroll
-    for (int k = 0; k < kQuads; ++k) {
-      const bool live = t + 4 * k + quad < end && at.in;
-      st[k] = live ? step_of(raw[k], a.softplus) : 0.f;
-      su[k] = live ? st[k] * u[k] : 0.f;
-      go[k] = gated ? (live ? dy[k] * (z[k] * sigmoid_f32(z[k])) : 0.f) : dy[k];
-      const float stj[4] = {quad_lane<0>(st[k]), quad_lane<1>(st[k]), quad_lane<2>(st[k]), quad_lane<3>(st[k])};
-      const float suj[4] = {quad_lane<0>(su[k]), quad_lane<1>(su[k]), quad_lane<2>(su[k]), quad_lane<3>(su[k])};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = 4 * k + j;
-        float B[SPL];
-        load_states<SPL>(s_b[buf] + n * SP + s0, B);
-#pragma unroll
-        for (int s = 0; s < SPL; ++s) {
-          dec[n][s] = __builtin_amdgcn_exp2f(stj[j] * rate[s]);
-          hs[n][s] = fmaf(dec[n][s], n ? hs[n ? n - 1 : 0][s] : h0[s], suj[j] * B[s]);
-        }
+      for (int s = 0; s < SPL; ++s) h0[s] = hn[s];
+      if (i) {   // under way while this chunk is worked on
+        ck -= ck_step;
+        rb.move(-1);
+        rc.move(-1);
+        px.move(-1);
+        pd.move(-1);
+        pg.move(-1);
+        pz.move(-1);
+        load_states<SPL>(ck, hn);
+        rb.load(kK);
+        rc.load(kK);
+        px.load(rx, kK);
+        pd.load(rd, kK);
+        pg.load(rg, kK);
+        if (gated) pz.load(rz, kK);
       }
-    }
-    // and back through them
-    float cA[SPL], cskip = 0.f, cbias = 0.f;
+      // the chunk's states again
+      float dec[kK][SPL], hs[kK][SPL];
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) cA[s] = 0.f;
+      for (int k = 0; k < kQuads; ++k) {
+        st[k] = step_of(raw[k], softplus);
+        su[k] = st[k] * u[k];
+        go[k] = dy[k] * act_of(z[k], gated);
+        const float stj[4] = {quad_lane<0>(st[k]), quad_lane<1>(st[k]), quad_lane<2>(st[k]), quad_lane<3>(st[k])};
+        const float suj[4] = {quad_lane<0>(su[k]), quad_lane<1>(su[k]), quad_lane<2>(su[k]), quad_lane<3>(su[k])};
 #pragma unroll
-    for (int k = kQuads - 1; k >= 0; --k) {
-      const float stj[4] = {quad_lane<0>(st[k]), quad_lane<1>(st[k]), quad_lane<2>(st[k]), quad_lane<3>(st[k])};
-      const float suj[4] = {quad_lane<0>(su[k]), quad_lane<1>(su[k]), quad_lane<2>(su[k]), quad_lane<3>(su[k])};
-      const float goj[4] = {quad_lane<0>(go[k]), quad_lane<1>(go[k]), quad_lane<2>(go[k]), quad_lane<3>(go[k])};
-      float into[4], mA[4], o[4];
+        for (int j = 0; j < 4; ++j) {
+          const int n = 4 * k + j;
+          float B[SPL];
+          load_states<SPL>(s_b[buf] + n * SP + s0, B);
 #pragma unroll
-      for (int j = 3; j >= 0; --j) {
-        const int n = 4 * k + j;
-        float B[SPL], C[SPL], v[2 * SPL], left[Sums::kLeft];
-        load_states<SPL>(s_b[buf] + n * SP + s0, B);
-        load_states<SPL>(s_c[buf] + n * SP + s0, C);
-        into[j] = mA[j] = o[j] = 0.f;
-#pragma unroll
-        for (int s = 0; s < SPL; ++s) {
-          const float g = fmaf(C[s], goj[j], ga[s]);
-          v[s] = g * suj[j];
-          v[SPL + s] = goj[j] * hs[n][s];
-          into[j] = fmaf(g, B[s], into[j]);
-          ga[s] = g * dec[n][s];
-          const float m = ga[s] * (n ? hs[n ? n - 1 : 0][s] : h0[s]);
-          cA[s] = fmaf(m, stj[j], cA[s]);
-          mA[j] = fmaf(m, rate[s], mA[j]);
-          if (gated) o[j] = fmaf(hs[n][s], C[s], o[j]);
-        }
-        Sums::sum(v, left, at.lane);
-        if (Sums::writes(at.lane)) {
-#pragma unroll
-          for (int e = 0; e < Sums::kLeft; ++e) {
-            const int q = Sums::which(at.lane) + e;   // dB's states, then dC's
-            s_sum[at.wave][n][q / SPL * SP + s0 + q % SPL] = left[e];
+          for (int s = 0; s < SPL; ++s) {
+            dec[n][s] = __builtin_amdgcn_exp2f(stj[j] * rate[s]);
+            hs[n][s] = fmaf(dec[n][s], n ? hs[n ? n - 1 : 0][s] : h0[s], suj[j] * B[s]);
           }
         }
       }
-      const float gB = quad_sums<LPC>(into[0], into[1], into[2], into[3], at.lane);
-      const float gA = quad_sums<LPC>(mA[0], mA[1], mA[2], mA[3], at.lane) * (1.f / kLog2e);
-      const int tk = t + 4 * k + quad;
-      float dd = tk < end ? fmaf(u[k], gB, gA) : 0.f;   // the adjoint goes on through tokens behind the end, unchanged
-      if (a.softplus) dd *= sigmoid_f32(raw[k]);
-      cskip = fmaf(go[k], u[k], cskip);
-      cbias += dd;
-      float dz = 0.f;
-      if (gated) {
+      // and back through them; the rows of the two tokens in front are read meanwhile
+      float cA[SPL], cskip = 0.f, cbias = 0.f, gx[kQuads], gd[kQuads], gz[kQuads], B[2][2 * SPL], C[2][2 * SPL];
+#pragma unroll
+      for (int s = 0; s < SPL; ++s) cA[s] = 0.f;
+      auto rows = [&](int pair) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          load_states<SPL>(s_b[buf] + (2 * pair + j) * SP + s0, B[pair & 1] + j * SPL);
+          load_states<SPL>(s_c[buf] + (2 * pair + j) * SP + s0, C[pair & 1] + j * SPL);
+        }
+      };
+      rows(kK / 2 - 1);
+#pragma unroll
+      for (int k = kQuads - 1; k >= 0; --k) {
+        const float stj[4] = {quad_lane<0>(st[k]), quad_lane<1>(st[k]), quad_lane<2>(st[k]), quad_lane<3>(st[k])};
+        const float suj[4] = {quad_lane<0>(su[k]), quad_lane<1>(su[k]), quad_lane<2>(su[k]), quad_lane<3>(su[k])};
+        const float goj[4] = {quad_lane<0>(go[k]), quad_lane<1>(go[k]), quad_lane<2>(go[k]), quad_lane<3>(go[k])};
+        float into[4], mA[4], o[4];
+#pragma unroll
+        for (int j = 3; j >= 0; --j) {
+          const int n = 4 * k + j, pair = n / 2;
+          if (n % 2) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (pair) rows(pair - 1);
+          }
+          const float* Bn = B[pair & 1] + n % 2 * SPL;
+          const float* Cn = C[pair & 1] + n % 2 * SPL;
+          float v[2 * SPL], left[Sums::kLeft];
+          into[j] = mA[j] = o[j] = 0.f;
+#pragma unroll
+          for (int s = 0; s < SPL; ++s) {
+            const float g = fmaf(Cn[s], goj[j], ga[s]);
+            v[s] = g * suj[j];
+            v[SPL + s] = goj[j] * hs[n][s];
+            into[j] = fmaf(g, Bn[s], into[j]);
+            ga[s] = g * dec[n][s];
+            const float m = ga[s] * (n ? hs[n ? n - 1 : 0][s] : h0[s]);
+            cA[s] = fmaf(m, stj[j], cA[s]);
+            mA[j] = fmaf(m, rate[s], mA[j]);
+            o[j] = fmaf(hs[n][s], Cn[s], o[j]);
+          }
+          Sums::sum(v, left, at.lane);
+#pragma unroll
+          for (int e = 0; e < Sums::kLeft; ++e) s_sum[buf][at.wave][n][place + e] = left[e];   // dB's states, then dC's
+        }
+        const float gB = quad_sums<LPC>(into[0], into[1], into[2], into[3], at.lane);
+        const float gA = quad_sums<LPC>(mA[0], mA[1], mA[2], mA[3], at.lane) * (1.f / kLog2e);
         const float out = fmaf(skip, u[k], quad_sums<LPC>(o[0], o[1], o[2], o[3], at.lane)), e = sigmoid_f32(z[k]);
-        dz = dy[k] * out * (e * fmaf(z[k], 1.f - e, 1.f));
+        const float slope = sigmoid_f32(raw[k]), all = fmaf(u[k], gB, gA);
+        // the adjoint goes on through tokens behind the end, unchanged
+        gd[k] = t + 4 * k + quad < end ? softplus ? all * slope : all : 0.f;
+        cskip = fmaf(go[k], u[k], cskip);
+        cbias += gd[k];
+        gx[k] = fmaf(st[k], gB, skip * go[k]);
+        gz[k] = dy[k] * out * (e * fmaf(z[k], 1.f - e, 1.f));
       }
-      if (writes && tk < end) {
-        ox[tk * w.dx_stride[1]] = from_f32<T>(fmaf(st[k], gB, skip * go[k]));
-        od[tk * w.ddelta_stride[1]] = from_f32<T>(dd);
-        if (gated) oz[tk * w.dgate_stride[1]] = from_f32<T>(dz);
+      // the next chunk's values are waited for in front of this one's stores, as forward
+      if (i) take(buf ^ 1, kK);
+      if (writes) {
+        if (whole) {
+          ox.store(gx);
+          od.store(gd);
+          if (gated) oz.store(gz);
+        } else {
+          ox.store(gx, quad, end - t);
+          od.store(gd, quad, end - t);
+          if (gated) oz.store(gz, quad, end - t);
+        }
       }
-    }
+      ox.move(-1);
+      od.move(-1);
+      oz.move(-1);
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) dA[s] += cA[s];
-    if (at.in) {   // lanes behind the group's end have computed its last channel's steps
-      dskip += cskip;
-      dbias += cbias;
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < kK * 2 * SP; e += kScanThreads) {
-      const int n = e / (2 * SP), q = e % (2 * SP);
-      if (t + n < end) {
-        float x = s_sum[0][n][q];
+      for (int s = 0; s < SPL; ++s) dA[s] += cA[s];
+      if (at.in) {   // lanes behind the group's end have computed its last channel's steps
+        dskip += cskip;
+        dbias += cbias;
+      }
+      __syncthreads();   // one barrier a chunk: what it lets through writes the other buffers
 #pragma unroll
-        for (int v = 1; v < kScanWaves; ++v) x += s_sum[v][n][q];
-        part[static_cast<int64_t>(t + n) * a.G * (2 * SP) + q] = x;
+      for (int e = threadIdx.x; e < kK * 2 * SP; e += kScanThreads) {
+        const int n = e / (2 * SP), q = e % (2 * SP);
+        float x = s_sum[buf][0][n][q];
+#pragma unroll
+        for (int v = 1; v < kScanWaves; ++v) x += s_sum[buf][v][n][q];
+        if (t + n < end) part[(t + n) * part_step + q] = x;
       }
     }
-    if (i) {
-      rb.store(s_b[buf ^ 1], t - kK, end, a.S);
-      rc.store(s_c[buf ^ 1], t - kK, end, a.S);
-    }
-    __syncthreads();
   }
   if (!at.in) return;
   const int64_t row = static_cast<int64_t>(at.b) * gm.segs + at.seg;
@@ -709,15 +822,15 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(dwarf_selective
 int scan_tile_channels(int S) { return kScanWaves * (kWave / scan_lpc(S)); }
 int scan_padded(int S) { return scan_spl(S) * scan_lpc(S); }
 
-ScanGeom scan_geom(const dwarf_selective_scan_fwd_args& a) {
+ScanGeom scan_geom(const dwarf_selective_scan_fwd_args& a, bool backward) {
   ScanGeom gm{};
   const int per = a.D / a.G, ch = scan_tile_channels(a.S);
   gm.tiles_of_group = (per + ch - 1) / ch;
   gm.tiles = gm.tiles_of_group * a.G;
   const int64_t groups = static_cast<int64_t>(a.B) * gm.tiles;
-  // One segment where the workgroups (four waves, one for each vector unit of a CU) leave at most a quarter of the 256 CUs
-  // without any; otherwise segments for two workgroups a CU, of at least two units.
-  int64_t segs = groups >= 192 ? 1 : (512 + groups - 1) / groups;
+  // Segments for two workgroups a CU (four waves each, one for each vector unit), of two units at least.  Forward, where a
+  // segment costs most of its work a second time, one segment from three quarters of a workgroup a CU on.
+  int64_t segs = groups >= 192 ? 1 : 512 / groups;
   const int64_t most = a.N / (2 * kSegmentUnit);
   if (segs > most) segs = most;
   if (segs > kMaxSegments) segs = kMaxSegments;
@@ -780,7 +893,7 @@ void scan_step_typed(const dwarf_selective_scan_step_args& a, hipStream_t stream
 }  // namespace
 
 int64_t selective_scan_workgroups(const dwarf_selective_scan_fwd_args& a) {
-  const ScanGeom gm = scan_geom(a);
+  const ScanGeom gm = scan_geom(a, true);   // never fewer segments than forward
   return static_cast<int64_t>(a.B) * gm.tiles * gm.segs;
 }
 
@@ -790,12 +903,12 @@ size_t selective_scan_checkpoints(const dwarf_selective_scan_fwd_args& a) {
 }
 
 size_t selective_scan_fwd_workspace(const dwarf_selective_scan_fwd_args& a) {
-  const ScanGeom gm = scan_geom(a);
+  const ScanGeom gm = scan_geom(a, false);
   return (local_floats(a, gm) + step_floats(a, gm)) * sizeof(float);
 }
 
 hipError_t launch_selective_scan_fwd(const dwarf_selective_scan_fwd_args& a, hipStream_t stream) {
-  ScanGeom gm = scan_geom(a);
+  ScanGeom gm = scan_geom(a, false);
   gm.local = static_cast<float*>(a.workspace);
   gm.steps = gm.local + local_floats(a, gm);
 #define DWARF_SCAN_CALL(T, SPL, LPC) scan_fwd_typed<T, SPL, LPC>(a, gm, stream)
@@ -806,7 +919,7 @@ hipError_t launch_selective_scan_fwd(const dwarf_selective_scan_fwd_args& a, hip
 
 size_t selective_scan_bwd_workspace(const dwarf_selective_scan_bwd_args& w) {
   const dwarf_selective_scan_fwd_args& a = w.fwd;
-  const ScanGeom gm = scan_geom(a);
+  const ScanGeom gm = scan_geom(a, true);
   const size_t SP = scan_padded(a.S), parts = static_cast<size_t>(a.B) * gm.segs;
   return (local_floats(a, gm) + step_floats(a, gm) + static_cast<size_t>(gm.tiles_of_group) * a.B * a.N * a.G * 2 * SP +
           parts * a.D * SP + parts * 2 * a.D) * sizeof(float);
@@ -814,7 +927,7 @@ size_t selective_scan_bwd_workspace(const dwarf_selective_scan_bwd_args& w) {
 
 hipError_t launch_selective_scan_bwd(const dwarf_selective_scan_bwd_args& w, hipStream_t stream) {
   const dwarf_selective_scan_fwd_args& a = w.fwd;
-  ScanGeom gm = scan_geom(a);
+  ScanGeom gm = scan_geom(a, true);
   const size_t SP = scan_padded(a.S), parts = static_cast<size_t>(a.B) * gm.segs;
   gm.local = static_cast<float*>(w.workspace);
   gm.steps = gm.local + local_floats(a, gm);
