@@ -29,6 +29,8 @@
 // LDS, over workgroups by partial rows that a last launch adds in order.
 // Nothing is atomic: the same bits every time.  dA, dskip and the bias's
 // gradient, sums over all tokens, run in 64 bits from a chunk on.
+#include <utility>
+
 #include "selective.h"
 
 namespace dwarf {
@@ -107,6 +109,7 @@ struct ScanLane {
   static constexpr int kCh = kWave / LPC;              // channels of a wave
   static constexpr int kTileCh = kScanWaves * kCh;     // of a workgroup
   int lane, wave, sq, b, seg, tile, g, d;
+  int local, first, behind;   // the lane's channel in the tile; the tile's first channel, and the one behind its group
   bool in;   // the lane's channel is one of the group's; otherwise d is the group's last
   __device__ __forceinline__ ScanLane(const dwarf_selective_scan_fwd_args& a, const ScanGeom& gm, int segs) {
     lane = threadIdx.x % kWave;
@@ -118,9 +121,12 @@ struct ScanLane {
     seg = i % static_cast<uint32_t>(segs);
     b = i / static_cast<uint32_t>(segs);
     g = tile / gm.tiles_of_group;
-    const int per = a.D / a.G, c = tile % gm.tiles_of_group * kTileCh + wave * kCh + lane / LPC;
-    in = c < per;
-    d = g * per + (in ? c : per - 1);
+    const int per = a.D / a.G, c = tile % gm.tiles_of_group * kTileCh;
+    local = wave * kCh + lane / LPC;
+    first = g * per + c;
+    behind = g * per + per;
+    in = first + local < behind;
+    d = in ? first + local : behind - 1;
   }
 };
 
@@ -190,10 +196,183 @@ struct QuadRows {
     for (int k = 0; k < QUADS; ++k)
       if (4 * k + quad < live) *reinterpret_cast<T*>(base + (off + k * (4 * stride))) = from_f32<T>(x[k]);
   }
-  // zeros from the sequence's token `from` to `to`; `t` is the tile's first
-  __device__ __forceinline__ void clear(int t, int quad, int from, int to) const {
-    for (int i = from + quad; i < to; i += 4)
-      *reinterpret_cast<T*>(base + static_cast<int64_t>(i - t) * stride + channel) = from_f32<T>(0.f);
+};
+
+// Zeros in a channel's tokens `from` to `to`.
+template <typename T>
+__device__ __forceinline__ void clear_rows(const void* p, int64_t at, int64_t stride, int quad, int from, int to) {
+  T* q = static_cast<T*>(const_cast<void*>(p)) + at;
+  for (int t = from + quad; t < to; t += 4) q[t * stride] = from_f32<T>(0.f);
+}
+
+// A workgroup's tiles [TOK][kCh] of NS inputs, and of NS outputs.
+//
+// WIDE: the workgroup's threads carry whole rows of the tile between memory and LDS, 16 bytes a thread and access; a lane
+// then takes its channel's element from LDS.  A lane's own accesses, where rows are not aligned to 16 bytes, are 2 bytes
+// from four rows to a quad, sixteen places a wave's access, which kept the CU's address unit busy for a fifth of the time
+// (forward; B15 N2048, 1,024 channels in bf16).  In LDS the vectors of a row are turned by the row, so that the four rows that
+// a wave reads together lie in different banks.
+template <typename T, int LPC>
+struct ScanTile {
+  static constexpr int kCh = ScanLane<LPC>::kTileCh, kVe = 16 / sizeof(T), kNv = kCh / kVe;
+  static constexpr int kApart = 256 / (kCh * static_cast<int>(sizeof(T)));   // rows until a bank comes again
+  static constexpr int kWaveVecs = kCh / kScanWaves / kVe;
+  static __device__ __forceinline__ int turned(int row, int vec) {
+    return kApart >= 4 ? vec : vec ^ ((row & 3) / (kApart < 4 ? kApart : 4) * kWaveVecs);
+  }
+  // a lane's element of its first row
+  static __device__ __forceinline__ int spot(int quad, int local) {
+    return quad * kCh + turned(quad, local / kVe) * kVe + local % kVe;
+  }
+};
+
+typedef uint32_t Chunk __attribute__((ext_vector_type(4)));   // 16 bytes of a row
+
+struct ScanRows {   // of one input or output
+  const void* p;   // nullptr: none
+  int64_t sequence, stride;
+};
+
+template <typename T, int TOK, int LPC, int NS>
+struct WideRows {
+  using Tile = ScanTile<T, LPC>;
+  static constexpr int kVecs = TOK * Tile::kNv, kAll = NS * kVecs, kEach = (kAll + kScanThreads - 1) / kScanThreads;
+  char* at[kEach];       // the thread's vectors of the tile
+  int64_t stride[kEach]; // bytes of a token
+  int row[kEach], spot[kEach];
+  bool ok[kEach];        // the vector is one of the tile's and its group's
+  __device__ __forceinline__ WideRows(const ScanRows (&rows)[NS], const ScanLane<LPC>& lane, int D, int t) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = e * kScanThreads + threadIdx.x, which = min(i / kVecs, NS - 1), vec = i % Tile::kNv;
+      row[e] = i % kVecs / Tile::kNv;
+      spot[e] = which * (TOK * Tile::kCh) + row[e] * Tile::kCh + Tile::turned(row[e], vec) * Tile::kVe;
+      const int c = lane.first + vec * Tile::kVe;
+      const void* p = nullptr;
+      int64_t sequence = 0, step = 0;
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+        if (which == n) p = rows[n].p, sequence = rows[n].sequence, step = rows[n].stride;
+      ok[e] = i < kAll && p && c < lane.behind;
+      if (!p) p = rows[0].p, sequence = rows[0].sequence, step = rows[0].stride;   // loads have to go somewhere
+      stride[e] = step * static_cast<int64_t>(sizeof(T));
+      at[e] = reinterpret_cast<char*>(static_cast<T*>(const_cast<void*>(p)) + sequence + (t + row[e]) * step + min(c, D - Tile::kVe));
+    }
+  }
+  __device__ __forceinline__ void move(int tiles) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) at[e] += tiles * (TOK * stride[e]);
+  }
+};
+
+template <typename T, int TOK, int LPC, int NS, bool WIDE>
+struct ScanIn {   // WIDE
+  WideRows<T, TOK, LPC, NS> rows;
+  Chunk v[WideRows<T, TOK, LPC, NS>::kEach];
+  T* lds;
+  int mine;
+  static constexpr int kSpan = NS * TOK * ScanTile<T, LPC>::kCh;   // of one of the two buffers
+  __device__ __forceinline__ ScanIn(const ScanRows (&in)[NS], const ScanLane<LPC>& lane, int D, int t, T* lds_)
+      : rows(in, lane, D, t), lds(lds_), mine(ScanTile<T, LPC>::spot(lane.lane & 3, lane.local)) {}
+  __device__ __forceinline__ void move(int tiles) { rows.move(tiles); }
+  __device__ __forceinline__ void fetch(int live) {
+#pragma unroll
+    for (int e = 0; e < rows.kEach; ++e) {
+      const int over = rows.row[e] - live + 1;   // rows behind the live ones
+      v[e] = *reinterpret_cast<const Chunk*>(rows.at[e] - (over > 0 ? over : 0) * rows.stride[e]);
+    }
+  }
+  __device__ __forceinline__ void put(int buf) const {
+#pragma unroll
+    for (int e = 0; e < rows.kEach; ++e)
+      if (rows.kAll % kScanThreads == 0 || e * kScanThreads + static_cast<int>(threadIdx.x) < rows.kAll)
+        *reinterpret_cast<Chunk*>(lds + buf * kSpan + rows.spot[e]) = v[e];
+  }
+  __device__ __forceinline__ float get(int which, int buf, int k) const {
+    return to_f32(lds[buf * kSpan + which * (TOK * ScanTile<T, LPC>::kCh) + 4 * k * ScanTile<T, LPC>::kCh + mine]);
+  }
+};
+
+template <typename T, int TOK, int LPC, int NS>
+struct ScanIn<T, TOK, LPC, NS, false> {
+  static constexpr int kSpan = 8;   // no LDS
+  QuadRows<T, TOK / 4> q[NS];
+  bool given[NS];
+  T r[NS][TOK / 4];
+  float v[NS][TOK / 4];
+  template <int... I>
+  __device__ __forceinline__ ScanIn(const ScanRows (&in)[NS], const ScanLane<LPC>& lane, int t, std::integer_sequence<int, I...>)
+      : q{QuadRows<T, TOK / 4>(in[I].p, in[I].sequence, in[I].stride, lane.d, t, lane.lane & 3)...}, given{in[I].p != nullptr...} {}
+  __device__ __forceinline__ ScanIn(const ScanRows (&in)[NS], const ScanLane<LPC>& lane, int, int t, T*)
+      : ScanIn(in, lane, t, std::make_integer_sequence<int, NS>()) {}
+  __device__ __forceinline__ void move(int tiles) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) q[n].move(tiles);
+  }
+  __device__ __forceinline__ void fetch(int live) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+      if (given[n]) q[n].load(r[n], live);   // uniform
+  }
+  __device__ __forceinline__ void put(int) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int k = 0; k < TOK / 4; ++k) v[n][k] = to_f32(r[n][k]);
+  }
+  __device__ __forceinline__ float get(int which, int, int k) const { return v[which][k]; }
+};
+
+template <typename T, int TOK, int LPC, int NS, bool WIDE>
+struct ScanOut {   // WIDE
+  WideRows<T, TOK, LPC, NS> rows;
+  T* lds;
+  int mine;
+  static constexpr int kSpan = NS * TOK * ScanTile<T, LPC>::kCh;
+  __device__ __forceinline__ ScanOut(const ScanRows (&out)[NS], const ScanLane<LPC>& lane, int D, int t, T* lds_)
+      : rows(out, lane, D, t), lds(lds_), mine(ScanTile<T, LPC>::spot(lane.lane & 3, lane.local)) {}
+  __device__ __forceinline__ void move(int tiles) { rows.move(tiles); }
+  __device__ __forceinline__ void put(int which, int buf, int k, float x) {
+    lds[buf * kSpan + which * (TOK * ScanTile<T, LPC>::kCh) + 4 * k * ScanTile<T, LPC>::kCh + mine] = from_f32<T>(x);
+  }
+  // Behind a barrier: the tile's live rows, in two parts, so that other work lies between.
+  Chunk held[WideRows<T, TOK, LPC, NS>::kEach];
+  __device__ __forceinline__ void collect(int buf) {
+#pragma unroll
+    for (int e = 0; e < rows.kEach; ++e)
+      if (rows.kAll % kScanThreads == 0 || rows.ok[e]) held[e] = *reinterpret_cast<const Chunk*>(lds + buf * kSpan + rows.spot[e]);
+  }
+  __device__ __forceinline__ void send(int live) const {
+#pragma unroll
+    for (int e = 0; e < rows.kEach; ++e)
+      if (rows.ok[e] && rows.row[e] < live) *reinterpret_cast<Chunk*>(rows.at[e]) = held[e];
+  }
+};
+
+template <typename T, int TOK, int LPC, int NS>
+struct ScanOut<T, TOK, LPC, NS, false> {
+  static constexpr int kSpan = 8;
+  QuadRows<T, TOK / 4> q[NS];
+  bool given[NS];
+  float v[NS][TOK / 4];
+  template <int... I>
+  __device__ __forceinline__ ScanOut(const ScanRows (&out)[NS], const ScanLane<LPC>& lane, int t, std::integer_sequence<int, I...>)
+      : q{QuadRows<T, TOK / 4>(out[I].p, out[I].sequence, out[I].stride, lane.d, t, lane.lane & 3)...}, given{out[I].p != nullptr...} {}
+  __device__ __forceinline__ ScanOut(const ScanRows (&out)[NS], const ScanLane<LPC>& lane, int, int t, T*)
+      : ScanOut(out, lane, t, std::make_integer_sequence<int, NS>()) {}
+  __device__ __forceinline__ void move(int tiles) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) q[n].move(tiles);
+  }
+  __device__ __forceinline__ void put(int which, int, int k, float x) { v[which][k] = x; }
+  __device__ __forceinline__ void flush(int live, const ScanLane<LPC>& lane) const {
+    if (!lane.in || lane.sq >= 4) return;   // the channel's first quad stores
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      if (!given[n]) continue;
+      if (live >= TOK) q[n].store(v[n]);
+      else q[n].store(v[n], lane.lane & 3, live);
+    }
   }
 };
 
@@ -242,11 +421,14 @@ __device__ __forceinline__ void load_rates(const float* A, int64_t d, int s0, in
 }
 
 // LOCAL: what a segment adds from zero and its sum of steps, for all segments but the last; otherwise the rows.
-template <typename T, int SPL, int LPC, bool LOCAL>
+template <typename T, int SPL, int LPC, bool WIDE, bool LOCAL>
 __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void scan_fwd_kernel(dwarf_selective_scan_fwd_args a, ScanGeom gm) {
   constexpr int SP = SPL * LPC, kQuads = kTile / 4, kK = scan_chunk(SPL);
   __shared__ __align__(16) float s_b[2][kTile * SP];
   __shared__ __align__(16) float s_c[LOCAL ? 1 : 2][LOCAL ? 4 : kTile * SP];
+  constexpr int kIns = LOCAL ? 2 : 3;
+  __shared__ __align__(16) T s_in[2 * ScanIn<T, kTile, LPC, kIns, WIDE>::kSpan];
+  __shared__ __align__(16) T s_out[LOCAL ? 8 : 2 * ScanOut<T, kTile, LPC, 1, WIDE>::kSpan];
   const ScanLane<LPC> at(a, gm, LOCAL ? gm.segs - 1 : gm.segs);
   const int s0 = at.sq * SPL, quad = at.lane & 3;
   const int64_t d = at.d;
@@ -270,36 +452,26 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
   }
   const bool gated = !LOCAL && a.gate, softplus = a.softplus, writes = at.in && at.sq < 4;
   const float none = no_step(softplus);
-  using Rows = QuadRows<T, kQuads>;
-  Rows px(a.x, at.b * a.x_stride[0], a.x_stride[1], d, t0, quad);
-  Rows pd(a.delta, at.b * a.delta_stride[0], a.delta_stride[1], d, t0, quad);
-  Rows pz(a.gate, at.b * a.gate_stride[0], a.gate_stride[1], d, t0, quad);
-  Rows py(a.y, at.b * a.y_stride[0], a.y_stride[1], d, t0, quad);
+  const ScanRows ins[3] = {{a.x, at.b * a.x_stride[0], a.x_stride[1]}, {a.delta, at.b * a.delta_stride[0], a.delta_stride[1]},
+                           {gated ? a.gate : nullptr, at.b * a.gate_stride[0], a.gate_stride[1]}};
+  const ScanRows outs[1] = {{a.y, at.b * a.y_stride[0], a.y_stride[1]}};
+  ScanIn<T, kTile, LPC, kIns, WIDE> in(reinterpret_cast<const ScanRows(&)[kIns]>(ins), at, a.D, t0, s_in);
+  ScanOut<T, kTile, LPC, 1, WIDE> out(outs, at, a.D, t0, s_out);
   BcRows<T, SP, kTile> rb(static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2], a.B_stride[1], t0, a.S);
   BcRows<T, SP, kTile> rc(static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2], a.C_stride[1], t0, a.S);
   float* ck = !LOCAL && a.checkpoints && at.in
                   ? a.checkpoints + ((static_cast<int64_t>(at.b) * ((a.N + kK - 1) / kK) + t0 / kK) * a.D + d) * SP + s0 : nullptr;
   const int64_t ck_step = static_cast<int64_t>(a.D) * SP;
-  float total = 0.f, u[kQuads], raw[kQuads], z[kQuads];
-  T rx[kQuads], rd[kQuads], rz[kQuads];
+  float total = 0.f;
   auto fetch = [&](int live) {   // the tile's first `live` tokens are live
     rb.load(live);
     if constexpr (!LOCAL) rc.load(live);
-    px.load(rx, live);
-    pd.load(rd, live);
-    if (gated) pz.load(rz, live);
+    in.fetch(live);
   };
   auto take = [&](int to, int live) {
     rb.store(s_b[to], live, a.S);
     if constexpr (!LOCAL) rc.store(s_c[to], live, a.S);
-#pragma unroll
-    for (int k = 0; k < kQuads; ++k) {
-      const bool in = 4 * k + quad < live;
-      const float vx = to_f32(rx[k]), vd = to_f32(rd[k]) + bias, vz = to_f32(rz[k]);
-      u[k] = in ? vx : 0.f;
-      raw[k] = in ? vd : none;
-      z[k] = gated ? vz : 0.f;
-    }
+    in.put(to);
   };
   int buf = 0;
   if (t0 < end) {   // around the loop too: one that might not run would wait inside for what is loaded in front of it
@@ -311,24 +483,36 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
       if (more) {   // under way while this tile is worked on
         rb.move(1);
         rc.move(1);
-        px.move(1);
-        pd.move(1);
-        pz.move(1);
+        in.move(1);
         fetch(end - t - kTile);
       }
-      // A quad at a time; the next one's rows and steps are formed meanwhile, which the compiler does not do by itself.
-      float o[kQuads], B[2][4 * SPL], C[2][4 * SPL], st[2], su[2];
+      // A quad at a time; the next one's rows and steps are formed meanwhile, from values read one quad earlier yet: the compiler
+      // waits where it reads.
+      float B[2][4 * SPL], C[2][4 * SPL], st[2], su[2], u[2], act[2], vx[2], vd[2], vz[2];
+      auto look = [&](int k) {
+        const int i = k & 1;
+        vx[i] = in.get(0, buf, k), vd[i] = in.get(1, buf, k);
+        if constexpr (!LOCAL) vz[i] = in.get(2, buf, k);
+      };
       auto begin = [&](int k) {
+        const int i = k & 1;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          load_states<SPL>(s_b[buf] + (4 * k + j) * SP + s0, B[k & 1] + j * SPL);
-          if constexpr (!LOCAL) load_states<SPL>(s_c[buf] + (4 * k + j) * SP + s0, C[k & 1] + j * SPL);
+          load_states<SPL>(s_b[buf] + (4 * k + j) * SP + s0, B[i] + j * SPL);
+          if constexpr (!LOCAL) load_states<SPL>(s_c[buf] + (4 * k + j) * SP + s0, C[i] + j * SPL);
         }
-        st[k & 1] = step_of(raw[k], softplus);
-        su[k & 1] = st[k & 1] * u[k];
-        if constexpr (LOCAL) total += st[k & 1];
+        const bool live = t + 4 * k + quad < end;
+        u[i] = live ? vx[i] : 0.f;
+        st[i] = step_of(live ? vd[i] + bias : none, softplus);
+        su[i] = st[i] * u[i];
+        if constexpr (LOCAL) total += st[i];
+        else act[i] = act_of(vz[i], gated);
       };
+      look(0);
+      if constexpr (WIDE && !LOCAL)
+        if (t > t0) out.collect(buf ^ 1);   // the tile in front, which was whole
       begin(0);
+      look(1);
 #pragma unroll
       for (int k = 0; k < kQuads; ++k) {
         if (!LOCAL && 4 * k % kK == 0) {
@@ -337,30 +521,40 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
         }
         __builtin_amdgcn_sched_barrier(0);
         if (k + 1 < kQuads) begin(k + 1);
-        const float stj[4] = {quad_lane<0>(st[k & 1]), quad_lane<1>(st[k & 1]), quad_lane<2>(st[k & 1]), quad_lane<3>(st[k & 1])};
-        const float suj[4] = {quad_lane<0>(su[k & 1]), quad_lane<1>(su[k & 1]), quad_lane<2>(su[k & 1]), quad_lane<3>(su[k & 1])};
+        if (k + 2 < kQuads) look(k + 2);
+        const int i = k & 1;
+        const float stj[4] = {quad_lane<0>(st[i]), quad_lane<1>(st[i]), quad_lane<2>(st[i]), quad_lane<3>(st[i])};
+        const float suj[4] = {quad_lane<0>(su[i]), quad_lane<1>(su[i]), quad_lane<2>(su[i]), quad_lane<3>(su[i])};
         float p[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           p[j] = 0.f;
 #pragma unroll
           for (int s = 0; s < SPL; ++s) {
-            h[s] = fmaf(__builtin_amdgcn_exp2f(stj[j] * rate[s]), h[s], suj[j] * B[k & 1][j * SPL + s]);
-            if constexpr (!LOCAL) p[j] = fmaf(h[s], C[k & 1][j * SPL + s], p[j]);
+            h[s] = fmaf(__builtin_amdgcn_exp2f(stj[j] * rate[s]), h[s], suj[j] * B[i][j * SPL + s]);
+            if constexpr (!LOCAL) p[j] = fmaf(h[s], C[i][j * SPL + s], p[j]);
           }
         }
         if constexpr (!LOCAL)
-          o[k] = fmaf(skip, u[k], quad_sums<LPC>(p[0], p[1], p[2], p[3], at.lane)) * act_of(z[k], gated);
+          out.put(0, buf, k, fmaf(skip, u[i], quad_sums<LPC>(p[0], p[1], p[2], p[3], at.lane)) * act[i]);
       }
-      // The next tile's values are waited for in front of this one's stores: loads and stores are counted together, and waiting
-      // behind them would wait for the stores too (an eighth of the time).
+      if constexpr (WIDE && !LOCAL)
+        if (t > t0) {
+          out.send(kTile);
+          out.move(1);
+        }
+      // The next tile's values are waited for in front of this one's stores: loads and stores are counted together, and
+      // waiting behind them would wait for the stores too (an eighth of the time).
       if (more) take(buf ^ 1, end - t - kTile);
-      if (!LOCAL && writes) {
-        if (t + kTile <= end) py.store(o);
-        else py.store(o, quad, end - t);
+      __syncthreads();   // one barrier a tile: what it lets through writes the other buffers
+      if constexpr (!WIDE && !LOCAL) {
+        out.flush(end - t, at);
+        out.move(1);
       }
-      py.move(1);
-      __syncthreads();
+    }
+    if constexpr (WIDE && !LOCAL) {
+      out.collect(buf ^ 1);
+      out.send(end - t0 - (end - t0 - 1) / kTile * kTile);
     }
   }
   if constexpr (LOCAL) {
@@ -371,7 +565,7 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
       if (at.sq == 0) gm.steps[row] = total;
     }
   } else {
-    if (writes) Rows(a.y, at.b * a.y_stride[0], a.y_stride[1], d, t0, quad).clear(t0, quad, max(t0, end), t1);
+    if (writes) clear_rows<T>(a.y, at.b * a.y_stride[0] + d, a.y_stride[1], quad, max(t0, end), t1);
     if (a.final && at.seg == gm.segs - 1 && at.in)
       store_user_states<SPL>(a.final + (static_cast<int64_t>(at.b) * a.D + d) * a.S, s0, a.S, h);
   }
@@ -379,10 +573,11 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
 
 // The adjoint that leaves a segment through its front for none that enters at its end, and the sum of its steps; for all
 // segments but the first.
-template <typename T, int SPL, int LPC>
+template <typename T, int SPL, int LPC, bool WIDE>
 __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void scan_adjoint_kernel(dwarf_selective_scan_bwd_args w, ScanGeom gm) {
   constexpr int SP = SPL * LPC, kQuads = kTile / 4;
   __shared__ __align__(16) float s_c[2][kTile * SP];
+  __shared__ __align__(16) T s_in[2 * ScanIn<T, kTile, LPC, 3, WIDE>::kSpan];
   const dwarf_selective_scan_fwd_args& a = w.fwd;
   ScanLane<LPC> at(a, gm, gm.segs - 1);
   at.seg += 1;
@@ -397,62 +592,60 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
   const bool gated = a.gate != nullptr, softplus = a.softplus;
   const float none = no_step(softplus);
   const int tiles = end > t0 ? (end - t0 + kTile - 1) / kTile : 0, last = t0 + (tiles - 1) * kTile;
-  using Rows = QuadRows<T, kQuads>;
-  Rows pd(a.delta, at.b * a.delta_stride[0], a.delta_stride[1], d, last, quad);
-  Rows pz(a.gate, at.b * a.gate_stride[0], a.gate_stride[1], d, last, quad);
-  Rows pg(w.dy, at.b * w.dy_stride[0], w.dy_stride[1], d, last, quad);
+  const ScanRows ins[3] = {{w.dy, at.b * w.dy_stride[0], w.dy_stride[1]}, {a.delta, at.b * a.delta_stride[0], a.delta_stride[1]},
+                           {a.gate, at.b * a.gate_stride[0], a.gate_stride[1]}};
+  ScanIn<T, kTile, LPC, 3, WIDE> in(ins, at, a.D, last, s_in);
   BcRows<T, SP, kTile> rc(static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2], a.C_stride[1], last, a.S);
-  float total = 0.f, raw[kQuads], go[kQuads];
-  T rg[kQuads], rd[kQuads], rz[kQuads];
-  auto take = [&](int to, int live) {
-    rc.store(s_c[to], live, a.S);
-#pragma unroll
-    for (int k = 0; k < kQuads; ++k) {
-      const bool in = 4 * k + quad < live;
-      const float vd = to_f32(rd[k]) + bias, vg = to_f32(rg[k]), vz = to_f32(rz[k]);
-      raw[k] = in ? vd : none;
-      go[k] = (in ? vg : 0.f) * act_of(in && gated ? vz : 0.f, gated);
-    }
-  };
+  float total = 0.f;
   int buf = 0;
   if (tiles) {
     rc.load(end - last);
-    pd.load(rd, end - last);
-    pg.load(rg, end - last);
-    if (gated) pz.load(rz, end - last);
-    take(0, end - last);
+    in.fetch(end - last);
+    rc.store(s_c[0], end - last, a.S);
+    in.put(0);
     __syncthreads();
     for (int i = tiles - 1; i >= 0; --i, buf ^= 1) {
+      const int t = t0 + i * kTile;
       if (i) {   // all tiles in front of the last are whole
         rc.move(-1);
-        pd.move(-1);
-        pg.move(-1);
-        pz.move(-1);
+        in.move(-1);
         rc.load(kTile);
-        pd.load(rd, kTile);
-        pg.load(rg, kTile);
-        if (gated) pz.load(rz, kTile);
+        in.fetch(kTile);
       }
-      float C[2][4 * SPL], st[2];
-      auto begin = [&](int k) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) load_states<SPL>(s_c[buf] + (4 * k + j) * SP + s0, C[k & 1] + j * SPL);
-        st[k & 1] = step_of(raw[k], softplus);
-        total += st[k & 1];
+      float C[2][4 * SPL], st[2], go[2], vg[2], vd[2], vz[2];
+      auto look = [&](int k) {
+        const int m = k & 1;
+        vg[m] = in.get(0, buf, k), vd[m] = in.get(1, buf, k), vz[m] = in.get(2, buf, k);
       };
+      auto begin = [&](int k) {
+        const int m = k & 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) load_states<SPL>(s_c[buf] + (4 * k + j) * SP + s0, C[m] + j * SPL);
+        const bool live = t + 4 * k + quad < end;
+        st[m] = step_of(live ? vd[m] + bias : none, softplus);
+        go[m] = (live ? vg[m] : 0.f) * act_of(live && gated ? vz[m] : 0.f, gated);
+        total += st[m];
+      };
+      look(kQuads - 1);
       begin(kQuads - 1);
+      look(kQuads - 2);
 #pragma unroll
       for (int k = kQuads - 1; k >= 0; --k) {
         __builtin_amdgcn_sched_barrier(0);
         if (k) begin(k - 1);
-        const float stj[4] = {quad_lane<0>(st[k & 1]), quad_lane<1>(st[k & 1]), quad_lane<2>(st[k & 1]), quad_lane<3>(st[k & 1])};
-        const float goj[4] = {quad_lane<0>(go[k]), quad_lane<1>(go[k]), quad_lane<2>(go[k]), quad_lane<3>(go[k])};
+        if (k > 1) look(k - 2);
+        const int m = k & 1;
+        const float stj[4] = {quad_lane<0>(st[m]), quad_lane<1>(st[m]), quad_lane<2>(st[m]), quad_lane<3>(st[m])};
+        const float goj[4] = {quad_lane<0>(go[m]), quad_lane<1>(go[m]), quad_lane<2>(go[m]), quad_lane<3>(go[m])};
 #pragma unroll
         for (int j = 3; j >= 0; --j)
 #pragma unroll
-          for (int s = 0; s < SPL; ++s) ga[s] = __builtin_amdgcn_exp2f(stj[j] * rate[s]) * fmaf(C[k & 1][j * SPL + s], goj[j], ga[s]);
+          for (int s = 0; s < SPL; ++s) ga[s] = __builtin_amdgcn_exp2f(stj[j] * rate[s]) * fmaf(C[m][j * SPL + s], goj[j], ga[s]);
       }
-      if (i) take(buf ^ 1, kTile);
+      if (i) {
+        rc.store(s_c[buf ^ 1], kTile, a.S);
+        in.put(buf ^ 1);
+      }
       __syncthreads();
     }
   }
@@ -502,12 +695,14 @@ struct ChannelSums {
   }
 };
 
-template <typename T, int SPL, int LPC>
+template <typename T, int SPL, int LPC, bool WIDE>
 __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void scan_bwd_kernel(dwarf_selective_scan_bwd_args w, ScanGeom gm) {
   constexpr int SP = SPL * LPC, kK = scan_chunk(SPL), kQuads = kK / 4;
   using Sums = ChannelSums<LPC, 2 * SPL>;
   __shared__ __align__(16) float s_b[2][kK * SP], s_c[2][kK * SP];
   __shared__ float s_sum[2][kScanWaves][kK][2 * SP];
+  __shared__ __align__(16) T s_in[2 * ScanIn<T, kK, LPC, 4, WIDE>::kSpan];
+  __shared__ __align__(16) T s_out[2 * ScanOut<T, kK, LPC, 3, WIDE>::kSpan];
   const dwarf_selective_scan_fwd_args& a = w.fwd;
   const ScanLane<LPC> at(a, gm, gm.segs);
   const int s0 = at.sq * SPL, quad = at.lane & 3;
@@ -531,14 +726,12 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
   const bool gated = a.gate != nullptr, softplus = a.softplus, writes = at.in && at.sq < 4;
   const float none = no_step(softplus);
   const int chunks = end > t0 ? (end - t0 + kK - 1) / kK : 0, last = t0 + (chunks - 1) * kK;
-  using Rows = QuadRows<T, kQuads>;
-  Rows px(a.x, at.b * a.x_stride[0], a.x_stride[1], d, last, quad);
-  Rows pd(a.delta, at.b * a.delta_stride[0], a.delta_stride[1], d, last, quad);
-  Rows pz(a.gate, at.b * a.gate_stride[0], a.gate_stride[1], d, last, quad);
-  Rows pg(w.dy, at.b * w.dy_stride[0], w.dy_stride[1], d, last, quad);
-  Rows ox(w.dx, at.b * w.dx_stride[0], w.dx_stride[1], d, last, quad);
-  Rows od(w.ddelta, at.b * w.ddelta_stride[0], w.ddelta_stride[1], d, last, quad);
-  Rows oz(w.dgate, at.b * w.dgate_stride[0], w.dgate_stride[1], d, last, quad);
+  const ScanRows ins[4] = {{a.x, at.b * a.x_stride[0], a.x_stride[1]}, {a.delta, at.b * a.delta_stride[0], a.delta_stride[1]},
+                           {w.dy, at.b * w.dy_stride[0], w.dy_stride[1]}, {a.gate, at.b * a.gate_stride[0], a.gate_stride[1]}};
+  const ScanRows outs[3] = {{w.dx, at.b * w.dx_stride[0], w.dx_stride[1]}, {w.ddelta, at.b * w.ddelta_stride[0], w.ddelta_stride[1]},
+                            {gated ? w.dgate : nullptr, at.b * w.dgate_stride[0], w.dgate_stride[1]}};
+  ScanIn<T, kK, LPC, 4, WIDE> in(ins, at, a.D, last, s_in);
+  ScanOut<T, kK, LPC, 3, WIDE> out(outs, at, a.D, last, s_out);
   BcRows<T, SP, kK> rb(static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2], a.B_stride[1], last, a.S);
   BcRows<T, SP, kK> rc(static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2], a.C_stride[1], last, a.S);
   const float* ck = a.checkpoints + ((static_cast<int64_t>(at.b) * ((a.N + kK - 1) / kK) + last / kK) * a.D + d) * SP + s0;
@@ -550,87 +743,104 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
   for (int s = 0; s < SPL; ++s) dA[s] = 0.;
   // behind the live tokens everything is zero
   if (writes) {
-    ox.clear(last, quad, max(t0, end), t1);
-    od.clear(last, quad, max(t0, end), t1);
-    if (gated) oz.clear(last, quad, max(t0, end), t1);
+    clear_rows<T>(w.dx, outs[0].sequence + d, outs[0].stride, quad, max(t0, end), t1);
+    clear_rows<T>(w.ddelta, outs[1].sequence + d, outs[1].stride, quad, max(t0, end), t1);
+    if (gated) clear_rows<T>(w.dgate, outs[2].sequence + d, outs[2].stride, quad, max(t0, end), t1);
   }
   for (int i = threadIdx.x / (2 * SP) + max(t0, end); i < t1; i += kScanThreads / (2 * SP))
     part[i * part_step + threadIdx.x % (2 * SP)] = 0.f;
 
-  T rx[kQuads], rd[kQuads], rz[kQuads], rg[kQuads];
-  float hn[SPL], u[kQuads], raw[kQuads], z[kQuads], dy[kQuads];
-  // a chunk's values, its B and C to LDS
-  auto take = [&](int to, int live) {
-    rb.store(s_b[to], live, a.S);
-    rc.store(s_c[to], live, a.S);
+  float hn[SPL];
+  const int place = Sums::which(at.lane) / SPL * SP + s0 + Sums::which(at.lane) % SPL;   // lanes with the same sum write it alike
+  // A chunk's results go to memory while the next one is worked on: read from LDS behind the barrier, stored later.
+  constexpr int kSums = kK * 2 * SP / kScanThreads;
+  float sums[kSums][kScanWaves];
+  auto collect = [&](int from) {
 #pragma unroll
-    for (int k = 0; k < kQuads; ++k) {
-      const bool in = 4 * k + quad < live && at.in;
-      const float vx = to_f32(rx[k]), vd = to_f32(rd[k]) + bias, vg = to_f32(rg[k]), vz = to_f32(rz[k]);
-      u[k] = in ? vx : 0.f;
-      raw[k] = in ? vd : none;
-      dy[k] = in ? vg : 0.f;
-      z[k] = in && gated ? vz : 0.f;
+    for (int e = 0; e < kSums; ++e)
+#pragma unroll
+      for (int v = 0; v < kScanWaves; ++v)
+        sums[e][v] = (&s_sum[from][v][0][0])[e * kScanThreads + threadIdx.x];
+    if constexpr (WIDE) out.collect(from);
+  };
+  auto send = [&](int t, int live) {
+#pragma unroll
+    for (int e = 0; e < kSums; ++e) {
+      const int at_ = e * kScanThreads + threadIdx.x, n = at_ / (2 * SP);
+      float x = sums[e][0];
+#pragma unroll
+      for (int v = 1; v < kScanWaves; ++v) x += sums[e][v];
+      if (n < live) part[(t + n) * part_step + at_ % (2 * SP)] = x;
+    }
+    if constexpr (WIDE) {
+      out.send(live);
+      out.move(-1);
     }
   };
-  const int place = Sums::which(at.lane) / SPL * SP + s0 + Sums::which(at.lane) % SPL;   // lanes with the same sum write it alike
   int buf = 0;
   if (chunks) {
-    const int live = end - last;
     load_states<SPL>(ck, hn);
-    rb.load(live);
-    rc.load(live);
-    px.load(rx, live);
-    pd.load(rd, live);
-    pg.load(rg, live);
-    if (gated) pz.load(rz, live);
-    take(0, live);
+    rb.load(end - last);
+    rc.load(end - last);
+    in.fetch(end - last);
+    rb.store(s_b[0], end - last, a.S);
+    rc.store(s_c[0], end - last, a.S);
+    in.put(0);
     __syncthreads();
     for (int i = chunks - 1; i >= 0; --i, buf ^= 1) {
       const int t = t0 + i * kK;
-      const bool whole = t + kK <= end;   // all chunks but the last
-      float h0[SPL], st[kQuads], su[kQuads], go[kQuads];
+      float h0[SPL], u[kQuads], raw[kQuads], z[kQuads], dy[kQuads], st[kQuads], su[kQuads], go[kQuads];
 #pragma unroll
       for (int s = 0; s < SPL; ++s) h0[s] = hn[s];
-      if (i) {   // under way while this chunk is worked on
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) {
+        const bool live = t + 4 * k + quad < end && at.in;
+        const float vx = in.get(0, buf, k), vd = in.get(1, buf, k) + bias, vg = in.get(2, buf, k), vz = in.get(3, buf, k);
+        u[k] = live ? vx : 0.f;
+        raw[k] = live ? vd : none;
+        dy[k] = live ? vg : 0.f;
+        z[k] = live && gated ? vz : 0.f;
+      }
+      if (i) {   // under way while this chunk is worked on; all chunks in front of the last are whole
         ck -= ck_step;
         rb.move(-1);
         rc.move(-1);
-        px.move(-1);
-        pd.move(-1);
-        pg.move(-1);
-        pz.move(-1);
+        in.move(-1);
         load_states<SPL>(ck, hn);
         rb.load(kK);
         rc.load(kK);
-        px.load(rx, kK);
-        pd.load(rd, kK);
-        pg.load(rg, kK);
-        if (gated) pz.load(rz, kK);
+        in.fetch(kK);
       }
-      // the chunk's states again
-      float dec[kK][SPL], hs[kK][SPL];
+      if (i + 1 < chunks) collect(buf ^ 1);   // the chunk behind
+      // the chunk's states again; the next quad's rows are read meanwhile
+      float dec[kK][SPL], hs[kK][SPL], R[2][4 * SPL];
+      auto begin = [&](int k) {
 #pragma unroll
-      for (int k = 0; k < kQuads; ++k) {
+        for (int j = 0; j < 4; ++j) load_states<SPL>(s_b[buf] + (4 * k + j) * SP + s0, R[k & 1] + j * SPL);
         st[k] = step_of(raw[k], softplus);
         su[k] = st[k] * u[k];
         go[k] = dy[k] * act_of(z[k], gated);
+      };
+      begin(0);
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (k + 1 < kQuads) begin(k + 1);
         const float stj[4] = {quad_lane<0>(st[k]), quad_lane<1>(st[k]), quad_lane<2>(st[k]), quad_lane<3>(st[k])};
         const float suj[4] = {quad_lane<0>(su[k]), quad_lane<1>(su[k]), quad_lane<2>(su[k]), quad_lane<3>(su[k])};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int n = 4 * k + j;
-          float B[SPL];
-          load_states<SPL>(s_b[buf] + n * SP + s0, B);
 #pragma unroll
           for (int s = 0; s < SPL; ++s) {
             dec[n][s] = __builtin_amdgcn_exp2f(stj[j] * rate[s]);
-            hs[n][s] = fmaf(dec[n][s], n ? hs[n ? n - 1 : 0][s] : h0[s], suj[j] * B[s]);
+            hs[n][s] = fmaf(dec[n][s], n ? hs[n ? n - 1 : 0][s] : h0[s], suj[j] * R[k & 1][j * SPL + s]);
           }
         }
       }
+      if (i + 1 < chunks) send(t + kK, min(kK, end - t - kK));
       // and back through them; the rows of the two tokens in front are read meanwhile
-      float cA[SPL], cskip = 0.f, cbias = 0.f, gx[kQuads], gd[kQuads], gz[kQuads], B[2][2 * SPL], C[2][2 * SPL];
+      float cA[SPL], cskip = 0.f, cbias = 0.f, B[2][2 * SPL], C[2][2 * SPL];
 #pragma unroll
       for (int s = 0; s < SPL; ++s) cA[s] = 0.f;
       auto rows = [&](int pair) {
@@ -676,31 +886,22 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
         }
         const float gB = quad_sums<LPC>(into[0], into[1], into[2], into[3], at.lane);
         const float gA = quad_sums<LPC>(mA[0], mA[1], mA[2], mA[3], at.lane) * (1.f / kLog2e);
-        const float out = fmaf(skip, u[k], quad_sums<LPC>(o[0], o[1], o[2], o[3], at.lane)), e = sigmoid_f32(z[k]);
+        const float scanned = fmaf(skip, u[k], quad_sums<LPC>(o[0], o[1], o[2], o[3], at.lane)), e = sigmoid_f32(z[k]);
         const float slope = sigmoid_f32(raw[k]), all = fmaf(u[k], gB, gA);
         // the adjoint goes on through tokens behind the end, unchanged
-        gd[k] = t + 4 * k + quad < end ? softplus ? all * slope : all : 0.f;
+        const float dd = t + 4 * k + quad < end ? softplus ? all * slope : all : 0.f;
         cskip = fmaf(go[k], u[k], cskip);
-        cbias += gd[k];
-        gx[k] = fmaf(st[k], gB, skip * go[k]);
-        gz[k] = dy[k] * out * (e * fmaf(z[k], 1.f - e, 1.f));
+        cbias += dd;
+        out.put(0, buf, k, fmaf(st[k], gB, skip * go[k]));
+        out.put(1, buf, k, dd);
+        out.put(2, buf, k, dy[k] * scanned * (e * fmaf(z[k], 1.f - e, 1.f)));
       }
       // the next chunk's values are waited for in front of this one's stores, as forward
-      if (i) take(buf ^ 1, kK);
-      if (writes) {
-        if (whole) {
-          ox.store(gx);
-          od.store(gd);
-          if (gated) oz.store(gz);
-        } else {
-          ox.store(gx, quad, end - t);
-          od.store(gd, quad, end - t);
-          if (gated) oz.store(gz, quad, end - t);
-        }
+      if (i) {
+        rb.store(s_b[buf ^ 1], kK, a.S);
+        rc.store(s_c[buf ^ 1], kK, a.S);
+        in.put(buf ^ 1);
       }
-      ox.move(-1);
-      od.move(-1);
-      oz.move(-1);
 #pragma unroll
       for (int s = 0; s < SPL; ++s) dA[s] += cA[s];
       if (at.in) {   // lanes behind the group's end have computed its last channel's steps
@@ -708,15 +909,13 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
         dbias += cbias;
       }
       __syncthreads();   // one barrier a chunk: what it lets through writes the other buffers
-#pragma unroll
-      for (int e = threadIdx.x; e < kK * 2 * SP; e += kScanThreads) {
-        const int n = e / (2 * SP), q = e % (2 * SP);
-        float x = s_sum[buf][0][n][q];
-#pragma unroll
-        for (int v = 1; v < kScanWaves; ++v) x += s_sum[buf][v][n][q];
-        if (t + n < end) part[(t + n) * part_step + q] = x;
+      if constexpr (!WIDE) {
+        out.flush(end - t, at);
+        out.move(-1);
       }
     }
+    collect(buf ^ 1);
+    send(t0, min(kK, end - t0));
   }
   if (!at.in) return;
   const int64_t row = static_cast<int64_t>(at.b) * gm.segs + at.seg;
@@ -848,22 +1047,45 @@ size_t step_floats(const dwarf_selective_scan_fwd_args& a, const ScanGeom& gm) {
   return gm.segs > 1 ? (static_cast<size_t>(a.B) * gm.segs * a.D + 3) / 4 * 4 : 0;
 }
 
-template <typename T, int SPL, int LPC>
-void scan_fwd_typed(const dwarf_selective_scan_fwd_args& a, const ScanGeom& gm, hipStream_t stream) {
-  const unsigned each = static_cast<unsigned>(a.B) * gm.tiles;
-  if (gm.segs > 1)
-    hipLaunchKernelGGL((scan_fwd_kernel<T, SPL, LPC, true>), dim3(each * (gm.segs - 1)), dim3(kScanThreads), 0, stream, a, gm);
-  hipLaunchKernelGGL((scan_fwd_kernel<T, SPL, LPC, false>), dim3(each * gm.segs), dim3(kScanThreads), 0, stream, a, gm);
+// Whether rows can be taken 16 bytes at a time: all of them aligned, the groups' channels whole vectors.
+bool wide_rows(const void* p, const int64_t (&stride)[2], int es) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride[0] * es % 16 == 0 && stride[1] * es % 16 == 0;
+}
+bool scan_wide(const dwarf_selective_scan_fwd_args& a) {
+  const int es = a.dtype == DWARF_F32 ? 4 : 2;
+  return (a.D / a.G) % (16 / es) == 0 && wide_rows(a.x, a.x_stride, es) && wide_rows(a.delta, a.delta_stride, es) &&
+         (!a.gate || wide_rows(a.gate, a.gate_stride, es));
 }
 
+template <typename T, int SPL, int LPC, bool WIDE>
+void scan_fwd_laid(const dwarf_selective_scan_fwd_args& a, const ScanGeom& gm, hipStream_t stream) {
+  const unsigned each = static_cast<unsigned>(a.B) * gm.tiles;
+  if (gm.segs > 1)
+    hipLaunchKernelGGL((scan_fwd_kernel<T, SPL, LPC, WIDE, true>), dim3(each * (gm.segs - 1)), dim3(kScanThreads), 0, stream, a, gm);
+  hipLaunchKernelGGL((scan_fwd_kernel<T, SPL, LPC, WIDE, false>), dim3(each * gm.segs), dim3(kScanThreads), 0, stream, a, gm);
+}
+template <typename T, int SPL, int LPC>
+void scan_fwd_typed(const dwarf_selective_scan_fwd_args& a, const ScanGeom& gm, hipStream_t stream) {
+  if (scan_wide(a) && wide_rows(a.y, a.y_stride, sizeof(T))) scan_fwd_laid<T, SPL, LPC, true>(a, gm, stream);
+  else scan_fwd_laid<T, SPL, LPC, false>(a, gm, stream);
+}
+
+template <typename T, int SPL, int LPC, bool WIDE>
+void scan_bwd_laid(const dwarf_selective_scan_bwd_args& w, const ScanGeom& gm, hipStream_t stream) {
+  const unsigned each = static_cast<unsigned>(w.fwd.B) * gm.tiles;
+  if (gm.segs > 1)
+    hipLaunchKernelGGL((scan_adjoint_kernel<T, SPL, LPC, WIDE>), dim3(each * (gm.segs - 1)), dim3(kScanThreads), 0, stream, w, gm);
+  hipLaunchKernelGGL((scan_bwd_kernel<T, SPL, LPC, WIDE>), dim3(each * gm.segs), dim3(kScanThreads), 0, stream, w, gm);
+}
 template <typename T, int SPL, int LPC>
 void scan_bwd_typed(const dwarf_selective_scan_bwd_args& w, const ScanGeom& gm, hipStream_t stream) {
   const dwarf_selective_scan_fwd_args& a = w.fwd;
-  const unsigned each = static_cast<unsigned>(a.B) * gm.tiles;
-  constexpr int SP = SPL * LPC;
-  if (gm.segs > 1)
-    hipLaunchKernelGGL((scan_adjoint_kernel<T, SPL, LPC>), dim3(each * (gm.segs - 1)), dim3(kScanThreads), 0, stream, w, gm);
-  hipLaunchKernelGGL((scan_bwd_kernel<T, SPL, LPC>), dim3(each * gm.segs), dim3(kScanThreads), 0, stream, w, gm);
+  constexpr int SP = SPL * LPC, es = sizeof(T);
+  if (scan_wide(a) && wide_rows(w.dy, w.dy_stride, es) && wide_rows(w.dx, w.dx_stride, es) && wide_rows(w.ddelta, w.ddelta_stride, es) &&
+      (!a.gate || wide_rows(w.dgate, w.dgate_stride, es)))
+    scan_bwd_laid<T, SPL, LPC, true>(w, gm, stream);
+  else
+    scan_bwd_laid<T, SPL, LPC, false>(w, gm, stream);
   const int64_t rows = static_cast<int64_t>(a.B) * a.N * a.G;
   if (rows)
     hipLaunchKernelGGL((scan_sum_rows<T>), dim3(static_cast<unsigned>((rows * 2 * SP + 255) / 256)), dim3(256), 0, stream,
