@@ -3,10 +3,12 @@
 //   p_t = bias + sum_j w_j x_{t-W+1+j},   y_t = p_t or silu(p_t)
 //   dp = dy silu'(p),  dx_t = sum_j w_j dp_{t+W-1-j},  dw_j = sum dp_t x_{t-W+1+j},  dbias = sum dp
 //
-// Bound by memory.  A thread takes VEC adjacent channels (16 bytes) and walks a
-// strip of tokens with the last W - 1 inputs in registers: each input is loaded
-// once but for the W - 1 rows in front of a strip, which another strip's thread
-// loads at about the same time.  Rows need no alignment but their elements':
+// Bound by memory.  A thread takes VEC adjacent channels (forward 16 bytes of
+// them, backward four: with eight, 148 registers left too few waves, 86 us
+// where four take 54) and walks a strip of tokens with the last W - 1 inputs in
+// registers, four rows on their way: each input is loaded once but for the
+// W - 1 rows in front of a strip, which another strip's thread loads at about
+// the same time.  Rows need no alignment but their elements':
 // gfx950 loads 16 bytes from any address, and a width that VEC does not divide
 // has its last vector moved back to the row's end, where two threads then store
 // the same values.  The backward forms p again from x, which it needs for dw
@@ -23,6 +25,7 @@ namespace {
 constexpr int kConvThreads = 256;
 constexpr int kConvCols = 32;                              // vectors of channels in a workgroup
 constexpr int kConvStrips = kConvThreads / kConvCols;      // strips of tokens in a workgroup
+constexpr int kConvAhead = 4;                              // rows of a thread on their way
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_any(const T* p, float* x) {
@@ -105,22 +108,31 @@ __global__ __launch_bounds__(kConvThreads) void conv_fwd_kernel(dwarf_causal_con
     conv_weights<VEC, W>(a.weight, a.bias, d, w, c);
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) conv_input<T, VEC, W>(a, x, at.b, d, t0 - W + 1 + j, win[j + 1]);
-#pragma unroll 4
-    for (int t = t0; t < end; ++t) {
+    T raw[kConvAhead][VEC];   // rows on the way; behind the sequence's end its last one again
+    auto fetch = [&](int t, int i) { __builtin_memcpy(raw[i], x + min(t, end - 1) * a.x_stride[1], sizeof(raw[i])); };
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j)
+    for (int i = 0; i < kConvAhead; ++i) fetch(t0 + i, i);
+    for (int t = t0; t < end; t += kConvAhead) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) win[j][e] = win[j + 1][e];
-      load_any<T, VEC>(x + t * a.x_stride[1], win[W - 1]);
-      float p[VEC];
+      for (int i = 0; i < kConvAhead; ++i) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        p[e] = c[e];
+        for (int j = 0; j < W - 1; ++j)
 #pragma unroll
-        for (int j = 0; j < W; ++j) p[e] = fmaf(w[j][e], win[j][e], p[e]);
-        if (a.silu) p[e] *= sigmoid_f32(p[e]);
+          for (int e = 0; e < VEC; ++e) win[j][e] = win[j + 1][e];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) win[W - 1][e] = to_f32(raw[i][e]);
+        fetch(t + i + kConvAhead, i);
+        float p[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          p[e] = c[e];
+#pragma unroll
+          for (int j = 0; j < W; ++j) p[e] = fmaf(w[j][e], win[j][e], p[e]);
+          const float s = p[e] * sigmoid_f32(p[e]);
+          p[e] = a.silu ? s : p[e];
+        }
+        if (t + i < end) store_any<T, VEC>(y + (t + i) * a.y_stride[1], p);
       }
-      store_any<T, VEC>(y + t * a.y_stride[1], p);
     }
   }
   float z[VEC];
@@ -174,57 +186,63 @@ __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(dwarf_causal_con
 #pragma unroll
       for (int j = 0; j < W - 1; ++j) conv_input<T, VEC, W>(a, x, at.b, d, t0 - W + 1 + j, win[j + 1]);
       // tokens up to W - 1 behind the strip, whose dp its last tokens' dx need; none behind the sequence's end
-      for (int t = t0; t < end + W - 1; ++t) {
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) win[j][e] = win[j + 1][e];
-#pragma unroll
-        for (int j = W - 1; j > 0; --j)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) dp[j][e] = dp[j - 1][e];
-        if (t < n) {
-          load_any<T, VEC>(x + t * a.x_stride[1], win[W - 1]);
-          load_any<T, VEC>(dy + t * w_.dy_stride[1], dp[0]);
-          if (a.silu) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              float p = c[e];
-#pragma unroll
-              for (int j = 0; j < W; ++j) p = fmaf(w[j][e], win[j][e], p);
-              dp[0][e] *= silu_slope(p);
-            }
-          }
-          if (t < end) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-#pragma unroll
-              for (int j = 0; j < W; ++j) dw[j][e] = fmaf(dp[0][e], win[j][e], dw[j][e]);
-              dw[W][e] += dp[0][e];
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) dp[0][e] = 0.f;
+      const int stop = end + W - 1;
+      T rx[kConvAhead][VEC], rg[kConvAhead][VEC];
+      auto fetch = [&](int t, int i) {   // behind the sequence's last token: that again
+        const int64_t tt = min(t, max(n, 1) - 1);
+        if (n > 0) {
+          __builtin_memcpy(rx[i], x + tt * a.x_stride[1], sizeof(rx[i]));
+          __builtin_memcpy(rg[i], dy + tt * w_.dy_stride[1], sizeof(rg[i]));
         }
-        const int to = t - (W - 1);   // dx_to = sum_j w_j dp_{to + W - 1 - j} = sum_j w_j dp[j]
-        if (to >= t0 ? to < end : to >= from) {
-          float v[VEC];
+      };
+#pragma unroll
+      for (int i = 0; i < kConvAhead; ++i) fetch(t0 + i, i);
+      for (int tb = t0; tb < stop; tb += kConvAhead) {
+#pragma unroll
+        for (int i = 0; i < kConvAhead; ++i) {
+          const int t = tb + i;
+#pragma unroll
+          for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) win[j][e] = win[j + 1][e];
+#pragma unroll
+          for (int j = W - 1; j > 0; --j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) dp[j][e] = dp[j - 1][e];
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            v[e] = 0.f;
+            win[W - 1][e] = to_f32(rx[i][e]);
+            const float g = to_f32(rg[i][e]);
+            float p = c[e];
 #pragma unroll
-            for (int j = 0; j < W; ++j) v[e] = fmaf(w[j][e], dp[j][e], v[e]);
-          }
-          // the state that leaves holds inputs n - W + 1 .. n - 1
-          if (df && to >= n - (W - 1)) {
-            float f[VEC];
-            load_any<T, VEC>(df + static_cast<int64_t>(to - (n - (W - 1))) * a.D, f);
+            for (int j = 0; j < W; ++j) p = fmaf(w[j][e], win[j][e], p);
+            const float s = g * silu_slope(p), v = a.silu ? s : g;
+            dp[0][e] = t < n ? v : 0.f;   // n is also the first token without a dy
+            const float own = t < end ? v : 0.f;   // the strip's own tokens
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] += f[e];
+            for (int j = 0; j < W; ++j) dw[j][e] = fmaf(own, win[j][e], dw[j][e]);
+            dw[W][e] += own;
           }
-          if (to >= 0) store_any<T, VEC>(dx + to * w_.dx_stride[1], v);
-          else store_any<T, VEC>(di + static_cast<int64_t>(to + W - 1) * a.D, v);
+          fetch(t + kConvAhead, i);
+          const int to = t - (W - 1);   // dx_to = sum_j w_j dp_{to + W - 1 - j} = sum_j w_j dp[j]
+          if (to >= t0 ? to < end : to >= from) {
+            float v[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              v[e] = 0.f;
+#pragma unroll
+              for (int j = 0; j < W; ++j) v[e] = fmaf(w[j][e], dp[j][e], v[e]);
+            }
+            // the state that leaves holds inputs n - W + 1 .. n - 1
+            if (df && to >= n - (W - 1)) {
+              float f[VEC];
+              load_any<T, VEC>(df + static_cast<int64_t>(to - (n - (W - 1))) * a.D, f);
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) v[e] += f[e];
+            }
+            if (to >= 0) store_any<T, VEC>(dx + to * w_.dx_stride[1], v);
+            else store_any<T, VEC>(di + static_cast<int64_t>(to + W - 1) * a.D, v);
+          }
         }
       }
     }
@@ -291,7 +309,7 @@ __global__ __launch_bounds__(kConvSumCols * kConvSumRows) void conv_sum_kernel(c
 // One token of each row.  The first row of a slot takes the slot's later rows after it, in order.
 template <typename T, int VEC, int W>
 __global__ __launch_bounds__(kConvThreads) void conv_step_kernel(dwarf_causal_conv_step_args a, int col_blocks) {
-  __shared__ int s_next;
+  __shared__ int s_found[2];
   const int row0 = blockIdx.x / col_blocks, col = blockIdx.x % col_blocks * kConvThreads + threadIdx.x;
   const bool in = col < (a.D + VEC - 1) / VEC;
   int d = in ? col * VEC : 0;
@@ -321,7 +339,9 @@ __global__ __launch_bounds__(kConvThreads) void conv_step_kernel(dwarf_causal_co
   for (int j = 0; j < W - 1; ++j) load_any<T, VEC>(st + static_cast<int64_t>(j) * a.D, v[j]);
   load_any<T, VEC>(static_cast<const T*>(a.x) + row0 * a.x_stride + d, v[W - 1]);
   conv_weights<VEC, W>(a.weight, a.bias, d, w, c);
-  if (row0 > 0 && a.slots && next_row_of<kConvThreads>(a.slots, slot, 0, a.R, &s_next) < row0) return;   // uniform
+  SameSlot same{false, a.R};
+  if (a.slots) same = same_slot<kConvThreads>(a.slots, slot, row0, a.R, s_found);
+  if (same.before) return;   // uniform
   for (int row = row0; row < a.R;) {
     float p[VEC];
 #pragma unroll
@@ -336,7 +356,8 @@ __global__ __launch_bounds__(kConvThreads) void conv_step_kernel(dwarf_causal_co
     for (int j = 0; j < W - 1; ++j)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[j][e] = v[j + 1][e];
-    row = a.slots && row + 1 < a.R ? next_row_of<kConvThreads>(a.slots, slot, row + 1, a.R, &s_next) : a.R;
+    row = same.next;
+    if (row < a.R) same = same_slot<kConvThreads>(a.slots, slot, row, a.R, s_found);
     if (row < a.R) load_any<T, VEC>(static_cast<const T*>(a.x) + row * a.x_stride + d, v[W - 1]);
   }
   if (in)
@@ -348,32 +369,33 @@ int conv_vec(int dtype, int D) {
   const int per = dtype == DWARF_F32 ? 4 : 8;
   return D >= per ? per : 1;
 }
+int conv_bwd_vec(int D) { return D >= 4 ? 4 : 1; }
 
-ConvGeom conv_geom(const dwarf_causal_conv_fwd_args& a, int least) {
+ConvGeom conv_geom(const dwarf_causal_conv_fwd_args& a, int vec) {
   ConvGeom gm;
-  const int vec = conv_vec(a.dtype, a.D);
   gm.cols = (a.D + vec - 1) / vec;
   gm.col_blocks = (gm.cols + kConvCols - 1) / kConvCols;
-  // strips as long as leave 1,024 workgroups (and partial rows within reason), `least` to 64 tokens
-  gm.strip = least;
-  while (gm.strip < 64 && static_cast<int64_t>(a.B) * a.N / (2 * gm.strip) / kConvStrips * gm.col_blocks >= 1024) gm.strip *= 2;
+  // Strips of 16 to 64 tokens, as long as leave seven workgroups for each four CUs: a thread reads W - 1 rows in front of its
+  // strip and its weights once more for each (B15 N2048, 1,024 channels in bf16: strips of 16 tokens 29.5 us forward and
+  // 55 backward, of 32 27.0 and 51).
+  gm.strip = 16;
+  while (gm.strip < 64 && static_cast<int64_t>(a.B) * a.N / (2 * gm.strip) / kConvStrips * gm.col_blocks >= 448) gm.strip *= 2;
   gm.strips = a.N > 0 ? (a.N + gm.strip - 1) / gm.strip : 1;
   return gm;
 }
 int64_t conv_groups(const dwarf_causal_conv_fwd_args& a, const ConvGeom& gm) {
   return (static_cast<int64_t>(a.B) * gm.strips + kConvStrips - 1) / kConvStrips;
 }
-constexpr int kConvFwdStrip = 8, kConvBwdStrip = 16;
 
 template <typename T, int VEC, int W>
 void conv_fwd_typed(const dwarf_causal_conv_fwd_args& a, hipStream_t stream) {
-  const ConvGeom gm = conv_geom(a, kConvFwdStrip);
+  const ConvGeom gm = conv_geom(a, VEC);
   hipLaunchKernelGGL((conv_fwd_kernel<T, VEC, W>), dim3(static_cast<unsigned>(conv_groups(a, gm) * gm.col_blocks)),
                      dim3(kConvThreads), 0, stream, a, gm);
 }
 template <typename T, int VEC, int W>
 void conv_bwd_typed(const dwarf_causal_conv_bwd_args& a, hipStream_t stream) {
-  const ConvGeom gm = conv_geom(a.fwd, kConvBwdStrip);
+  const ConvGeom gm = conv_geom(a.fwd, VEC);
   const int64_t groups = conv_groups(a.fwd, gm);
   float* part = a.dweight || a.dbias ? static_cast<float*>(a.workspace) : nullptr;
   hipLaunchKernelGGL((conv_bwd_kernel<T, VEC, W>), dim3(static_cast<unsigned>(groups * gm.col_blocks)), dim3(kConvThreads), 0,
@@ -400,45 +422,42 @@ void conv_step_typed(const dwarf_causal_conv_step_args& a, hipStream_t stream) {
     case 7: CALL(T, VEC, 7); break;           \
     default: CALL(T, VEC, 8); break;          \
   }
-#define DWARF_CONV_TYPES(dtype, D, W, CALL)                                                    \
-  const bool wide = conv_vec(dtype, D) > 1;                                                    \
-  if ((dtype) == DWARF_F32) {                                                                  \
-    if (wide) { DWARF_CONV_WIDTHS(float, 4, W, CALL) } else { DWARF_CONV_WIDTHS(float, 1, W, CALL) } \
-  } else if ((dtype) == DWARF_F16) {                                                           \
-    if (wide) { DWARF_CONV_WIDTHS(f16, 8, W, CALL) } else { DWARF_CONV_WIDTHS(f16, 1, W, CALL) }     \
-  } else {                                                                                     \
-    if (wide) { DWARF_CONV_WIDTHS(bf16, 8, W, CALL) } else { DWARF_CONV_WIDTHS(bf16, 1, W, CALL) }   \
-  }
+#define DWARF_CONV_VECTORS(T, VEC, wide, W, CALL) \
+  if (wide) { DWARF_CONV_WIDTHS(T, VEC, W, CALL) } else { DWARF_CONV_WIDTHS(T, 1, W, CALL) }
+#define DWARF_CONV_TYPES(dtype, wide, W, VEC16, CALL)                                             \
+  if ((dtype) == DWARF_F32) { DWARF_CONV_VECTORS(float, 4, wide, W, CALL) }                       \
+  else if ((dtype) == DWARF_F16) { DWARF_CONV_VECTORS(f16, VEC16, wide, W, CALL) }                \
+  else { DWARF_CONV_VECTORS(bf16, VEC16, wide, W, CALL) }
 
 }  // namespace
 
 int64_t causal_conv_workgroups(const dwarf_causal_conv_fwd_args& a) {
-  const ConvGeom gm = conv_geom(a, kConvFwdStrip);   // the shorter strips
+  const ConvGeom gm = conv_geom(a, conv_bwd_vec(a.D));   // the backward's: its vectors are the shorter ones
   return conv_groups(a, gm) * gm.col_blocks;
 }
 
 size_t causal_conv_bwd_workspace(const dwarf_causal_conv_bwd_args& a) {
   if (!a.dweight && !a.dbias) return 0;
-  return static_cast<size_t>(conv_groups(a.fwd, conv_geom(a.fwd, kConvBwdStrip))) * (a.fwd.W + 1) * a.fwd.D * sizeof(float);
+  return static_cast<size_t>(conv_groups(a.fwd, conv_geom(a.fwd, conv_bwd_vec(a.fwd.D)))) * (a.fwd.W + 1) * a.fwd.D * sizeof(float);
 }
 
 hipError_t launch_causal_conv_fwd(const dwarf_causal_conv_fwd_args& a, hipStream_t stream) {
 #define DWARF_CONV_CALL(T, VEC, W) conv_fwd_typed<T, VEC, W>(a, stream)
-  DWARF_CONV_TYPES(a.dtype, a.D, a.W, DWARF_CONV_CALL)
+  DWARF_CONV_TYPES(a.dtype, conv_vec(a.dtype, a.D) > 1, a.W, 8, DWARF_CONV_CALL)
 #undef DWARF_CONV_CALL
   return hipGetLastError();
 }
 
 hipError_t launch_causal_conv_bwd(const dwarf_causal_conv_bwd_args& a, hipStream_t stream) {
 #define DWARF_CONV_CALL(T, VEC, W) conv_bwd_typed<T, VEC, W>(a, stream)
-  DWARF_CONV_TYPES(a.fwd.dtype, a.fwd.D, a.fwd.W, DWARF_CONV_CALL)
+  DWARF_CONV_TYPES(a.fwd.dtype, conv_bwd_vec(a.fwd.D) > 1, a.fwd.W, 4, DWARF_CONV_CALL)
 #undef DWARF_CONV_CALL
   return hipGetLastError();
 }
 
 hipError_t launch_causal_conv_step(const dwarf_causal_conv_step_args& a, hipStream_t stream) {
 #define DWARF_CONV_CALL(T, VEC, W) conv_step_typed<T, VEC, W>(a, stream)
-  DWARF_CONV_TYPES(a.dtype, a.D, a.W, DWARF_CONV_CALL)
+  DWARF_CONV_TYPES(a.dtype, conv_vec(a.dtype, a.D) > 1, a.W, 8, DWARF_CONV_CALL)
 #undef DWARF_CONV_CALL
   return hipGetLastError();
 }

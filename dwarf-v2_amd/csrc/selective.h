@@ -33,20 +33,25 @@ __device__ __forceinline__ float sigmoid_f32(float x) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-x * kLog2e));
 }
 
-// The last W - 1 inputs, states and slots hold rows of one sequence at a time: the first of `rows` rows that share
-// `slot` behind row `from`, or `rows`.  Every thread of the workgroup calls it; s_next is the workgroup's own.
+// The rows of a step that share `slot`: whether one lies in front of row `row`, and the next one behind it (`rows` if there
+// is none).  Every thread of the workgroup calls it; s_found is the workgroup's own.
+struct SameSlot {
+  bool before;
+  int next;
+};
 template <int THREADS>
-__device__ __forceinline__ int next_row_of(const int32_t* slots, int slot, int from, int rows, int* s_next) {
+__device__ __forceinline__ SameSlot same_slot(const int32_t* slots, int slot, int row, int rows, int* s_found) {
+  if (threadIdx.x == 0) s_found[0] = 0, s_found[1] = rows;
   __syncthreads();
-  if (threadIdx.x == 0) *s_next = rows;
-  __syncthreads();
-  for (int i = from + static_cast<int>(threadIdx.x); i < rows; i += THREADS)
-    if (slots[i] == slot) {
-      atomicMin(s_next, i);
-      break;
+  for (int i = threadIdx.x; i < rows; i += THREADS)
+    if (i != row && slots[i] == slot) {
+      if (i < row) s_found[0] = 1;
+      else atomicMin(&s_found[1], i);
     }
   __syncthreads();
-  return *s_next;
+  const SameSlot r{s_found[0] != 0, s_found[1]};
+  __syncthreads();   // read before it is written again
+  return r;
 }
 
 }  // namespace dwarf

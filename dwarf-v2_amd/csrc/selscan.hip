@@ -39,7 +39,7 @@ namespace {
 constexpr int kScanWaves = 4, kScanThreads = kScanWaves * kWave;
 constexpr int kTile = 32;           // tokens of B and C in LDS at a time, forward
 constexpr int kMaxSegments = 64;
-constexpr int kSegmentUnit = 64;    // tokens a segment is a multiple of
+constexpr int kSegmentUnit = 32, kSegmentLeast = 64;   // tokens a segment is a multiple of, and has at least
 
 // States per lane and lanes per channel for S states.
 constexpr int scan_spl(int S) { return S <= 8 ? 2 : S <= 16 ? 4 : 8; }
@@ -956,6 +956,7 @@ __global__ __launch_bounds__(256) void scan_sum_channels(const float* __restrict
   if (i < nA) {
     const int s = static_cast<int>(i % SP);
     if (!dA || s >= S) return;
+#pragma unroll 8
     for (int k = 0; k < parts; ++k) x += part_A[k * nA + i];
     dA[i / SP * S + s] = static_cast<float>(x);
   } else if (i < nA + 2 * D) {
@@ -967,10 +968,12 @@ __global__ __launch_bounds__(256) void scan_sum_channels(const float* __restrict
   }
 }
 
-// One token of each row.  The first row of a slot takes the slot's later rows after it, in order.
-template <typename T, int SPL, int LPC>
+// One token of each row, bound by the pool's memory: a lane reads and writes its SPL states of a channel as 16-byte vectors
+// where the pool allows them (WHOLE: S states to a channel fill the lanes, slots are aligned), B and C likewise.  The first
+// row of a slot takes the slot's later rows after it, in order.
+template <typename T, int SPL, int LPC, bool WHOLE>
 __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(dwarf_selective_scan_step_args a, int tiles_of_group) {
-  __shared__ int s_next;
+  __shared__ int s_found[2];
   constexpr int kCh = kWave / LPC;
   const int lane = threadIdx.x % kWave, sq = lane % LPC, s0 = sq * SPL, per = a.D / a.G;
   const int tiles = tiles_of_group * a.G, tile = blockIdx.x % tiles, row0 = blockIdx.x / tiles, g = tile / tiles_of_group;
@@ -984,23 +987,40 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(dwarf_selective
   }
   const int64_t at = slot * a.slot_stride + d * a.S;
   float h[SPL], rate[SPL], B[SPL], C[SPL], x, raw, z = 0.f;
-  load_user_states<SPL>(a.state + at, s0, a.S, h);   // under way while the slots are looked through
+  if constexpr (WHOLE) load_states<SPL>(a.state + at + s0, h);   // under way while the slots are looked through
+  else load_user_states<SPL>(a.state + at, s0, a.S, h);
   auto fetch = [&](int row) {
     x = to_f32(static_cast<const T*>(a.x)[row * a.x_stride + d]);
     raw = to_f32(static_cast<const T*>(a.delta)[row * a.delta_stride + d]);
     if (a.gate) z = to_f32(static_cast<const T*>(a.gate)[row * a.gate_stride + d]);
-    const T* pB = static_cast<const T*>(a.Bm) + row * a.B_stride[0] + g * a.B_stride[1];
-    const T* pC = static_cast<const T*>(a.Cm) + row * a.C_stride[0] + g * a.C_stride[1];
+    const T* pB = static_cast<const T*>(a.Bm) + row * a.B_stride[0] + g * a.B_stride[1] + s0;
+    const T* pC = static_cast<const T*>(a.Cm) + row * a.C_stride[0] + g * a.C_stride[1] + s0;
+    if constexpr (WHOLE) {
+      T vB[SPL], vC[SPL];
+      __builtin_memcpy(vB, pB, sizeof(vB));   // gfx950 loads vectors from any address
+      __builtin_memcpy(vC, pC, sizeof(vC));
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) {
-      B[s] = s0 + s < a.S ? to_f32(pB[s0 + s]) : 0.f;
-      C[s] = s0 + s < a.S ? to_f32(pC[s0 + s]) : 0.f;
+      for (int s = 0; s < SPL; ++s) B[s] = to_f32(vB[s]), C[s] = to_f32(vC[s]);
+    } else {
+#pragma unroll
+      for (int s = 0; s < SPL; ++s) {
+        B[s] = s0 + s < a.S ? to_f32(pB[s]) : 0.f;
+        C[s] = s0 + s < a.S ? to_f32(pC[s]) : 0.f;
+      }
     }
   };
   fetch(row0);
-  load_rates<SPL>(a.A, d, s0, a.S, rate);
+  if constexpr (WHOLE) {
+    __builtin_memcpy(rate, a.A + d * a.S + s0, sizeof(rate));
+#pragma unroll
+    for (int s = 0; s < SPL; ++s) rate[s] *= kLog2e;
+  } else {
+    load_rates<SPL>(a.A, d, s0, a.S, rate);
+  }
   const float bias = a.delta_bias ? a.delta_bias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
-  if (row0 > 0 && a.slots && next_row_of<kScanThreads>(a.slots, slot, 0, a.R, &s_next) < row0) return;   // uniform
+  SameSlot same{false, a.R};
+  if (a.slots) same = same_slot<kScanThreads>(a.slots, slot, row0, a.R, s_found);
+  if (same.before) return;   // uniform
   for (int row = row0; row < a.R;) {
     const float st = step_of(raw + bias, a.softplus), su = st * x;
     float p = 0.f;
@@ -1009,33 +1029,34 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(dwarf_selective
       h[s] = fmaf(__builtin_amdgcn_exp2f(st * rate[s]), h[s], su * B[s]);
       p = fmaf(h[s], C[s], p);
     }
-    float o = fmaf(skip, x, lanes_sum<LPC>(p));
-    if (a.gate) o *= z * sigmoid_f32(z);
+    const float o = fmaf(skip, x, lanes_sum<LPC>(p)) * act_of(z, a.gate != nullptr);
     if (in && sq == 0) static_cast<T*>(a.out)[row * a.out_stride + d] = from_f32<T>(o);
-    row = a.slots && row + 1 < a.R ? next_row_of<kScanThreads>(a.slots, slot, row + 1, a.R, &s_next) : a.R;
-    if (row < a.R) fetch(row);
+    row = same.next;
+    if (row < a.R) {
+      same = same_slot<kScanThreads>(a.slots, slot, row, a.R, s_found);
+      fetch(row);
+    }
   }
-  if (in) store_user_states<SPL>(a.new_state + at, s0, a.S, h);
+  if (!in) return;
+  if constexpr (WHOLE) store_states<SPL>(a.new_state + at + s0, h);
+  else store_user_states<SPL>(a.new_state + at, s0, a.S, h);
 }
 
 int scan_tile_channels(int S) { return kScanWaves * (kWave / scan_lpc(S)); }
 int scan_padded(int S) { return scan_spl(S) * scan_lpc(S); }
 
-ScanGeom scan_geom(const dwarf_selective_scan_fwd_args& a, bool backward) {
+ScanGeom scan_geom(const dwarf_selective_scan_fwd_args& a) {
   ScanGeom gm{};
   const int per = a.D / a.G, ch = scan_tile_channels(a.S);
   gm.tiles_of_group = (per + ch - 1) / ch;
   gm.tiles = gm.tiles_of_group * a.G;
   const int64_t groups = static_cast<int64_t>(a.B) * gm.tiles;
-  // Segments for two workgroups a CU (four waves each, one for each vector unit), of two units at least.  Forward, where a
-  // segment costs most of its work a second time, one segment from three quarters of a workgroup a CU on.
+  // One segment from three quarters of a workgroup (four waves, one for each vector unit) a CU on: more cost most of the
+  // forward's work a second time.  Below that, segments for two workgroups a CU.
   int64_t segs = groups >= 192 ? 1 : 512 / groups;
-  const int64_t most = a.N / (2 * kSegmentUnit);
-  if (segs > most) segs = most;
   if (segs > kMaxSegments) segs = kMaxSegments;
-  if (segs < 1) segs = 1;
-  gm.seg = static_cast<int>(((a.N + segs - 1) / segs + kSegmentUnit - 1) / kSegmentUnit * kSegmentUnit);
-  if (gm.seg < kSegmentUnit) gm.seg = kSegmentUnit;
+  gm.seg = static_cast<int>((a.N + segs - 1) / segs + kSegmentUnit - 1) / kSegmentUnit * kSegmentUnit;
+  if (gm.seg < kSegmentLeast) gm.seg = kSegmentLeast;
   gm.segs = a.N > 0 ? (a.N + gm.seg - 1) / gm.seg : 1;
   return gm;
 }
@@ -1098,8 +1119,11 @@ void scan_bwd_typed(const dwarf_selective_scan_bwd_args& w, const ScanGeom& gm, 
 template <typename T, int SPL, int LPC>
 void scan_step_typed(const dwarf_selective_scan_step_args& a, hipStream_t stream) {
   const int per = a.D / a.G, ch = scan_tile_channels(a.S), tiles = (per + ch - 1) / ch;
-  hipLaunchKernelGGL((scan_step_kernel<T, SPL, LPC>), dim3(static_cast<unsigned>(a.R) * tiles * a.G), dim3(kScanThreads), 0,
-                     stream, a, tiles);
+  const dim3 grid(static_cast<unsigned>(a.R) * tiles * a.G), block(kScanThreads);
+  const bool whole = a.S == SPL * LPC && a.slot_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.state) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(a.new_state) % 16 == 0;
+  if (whole) hipLaunchKernelGGL((scan_step_kernel<T, SPL, LPC, true>), grid, block, 0, stream, a, tiles);
+  else hipLaunchKernelGGL((scan_step_kernel<T, SPL, LPC, false>), grid, block, 0, stream, a, tiles);
 }
 
 #define DWARF_SCAN_SHAPES(T, S, CALL)   \
@@ -1115,7 +1139,7 @@ void scan_step_typed(const dwarf_selective_scan_step_args& a, hipStream_t stream
 }  // namespace
 
 int64_t selective_scan_workgroups(const dwarf_selective_scan_fwd_args& a) {
-  const ScanGeom gm = scan_geom(a, true);   // never fewer segments than forward
+  const ScanGeom gm = scan_geom(a);
   return static_cast<int64_t>(a.B) * gm.tiles * gm.segs;
 }
 
@@ -1125,12 +1149,12 @@ size_t selective_scan_checkpoints(const dwarf_selective_scan_fwd_args& a) {
 }
 
 size_t selective_scan_fwd_workspace(const dwarf_selective_scan_fwd_args& a) {
-  const ScanGeom gm = scan_geom(a, false);
+  const ScanGeom gm = scan_geom(a);
   return (local_floats(a, gm) + step_floats(a, gm)) * sizeof(float);
 }
 
 hipError_t launch_selective_scan_fwd(const dwarf_selective_scan_fwd_args& a, hipStream_t stream) {
-  ScanGeom gm = scan_geom(a, false);
+  ScanGeom gm = scan_geom(a);
   gm.local = static_cast<float*>(a.workspace);
   gm.steps = gm.local + local_floats(a, gm);
 #define DWARF_SCAN_CALL(T, SPL, LPC) scan_fwd_typed<T, SPL, LPC>(a, gm, stream)
@@ -1141,7 +1165,7 @@ hipError_t launch_selective_scan_fwd(const dwarf_selective_scan_fwd_args& a, hip
 
 size_t selective_scan_bwd_workspace(const dwarf_selective_scan_bwd_args& w) {
   const dwarf_selective_scan_fwd_args& a = w.fwd;
-  const ScanGeom gm = scan_geom(a, true);
+  const ScanGeom gm = scan_geom(a);
   const size_t SP = scan_padded(a.S), parts = static_cast<size_t>(a.B) * gm.segs;
   return (local_floats(a, gm) + step_floats(a, gm) + static_cast<size_t>(gm.tiles_of_group) * a.B * a.N * a.G * 2 * SP +
           parts * a.D * SP + parts * 2 * a.D) * sizeof(float);
@@ -1149,7 +1173,7 @@ size_t selective_scan_bwd_workspace(const dwarf_selective_scan_bwd_args& w) {
 
 hipError_t launch_selective_scan_bwd(const dwarf_selective_scan_bwd_args& w, hipStream_t stream) {
   const dwarf_selective_scan_fwd_args& a = w.fwd;
-  ScanGeom gm = scan_geom(a, true);
+  ScanGeom gm = scan_geom(a);
   const size_t SP = scan_padded(a.S), parts = static_cast<size_t>(a.B) * gm.segs;
   gm.local = static_cast<float*>(w.workspace);
   gm.steps = gm.local + local_floats(a, gm);
