@@ -1205,7 +1205,14 @@ static int check_scan_sizes(int D, int G, int S, int dtype) {
   if (D % G) return fail(DWARF_ERR_INVALID_ARGUMENT, "D=%d channels must be divisible by G=%d groups", D, G);
   if (!mixer_dtype(dtype)) return fail(DWARF_ERR_INVALID_ARGUMENT, "dtype=%d", dtype);
   if (S > 64) return fail(DWARF_ERR_UNSUPPORTED, "the scan is built for up to 64 states (got %d)", S);
-  if (D > (1 << 24)) return fail(DWARF_ERR_UNSUPPORTED, "D up to 2^24 (got %d)", D);
+  if (D >= (1 << 22)) return fail(DWARF_ERR_UNSUPPORTED, "D below 2^22 (got %d)", D);
+  return DWARF_OK;
+}
+
+// The scan's kernels reach a tile's rows by 32-bit offsets.
+static int check_token_stride(const char* name, int64_t stride) {
+  if (stride < 0 || stride >= (1 << 22))
+    return fail(DWARF_ERR_UNSUPPORTED, "%s token stride %lld outside [0, 2^22) elements", name, static_cast<long long>(stride));
   return DWARF_OK;
 }
 
@@ -1220,9 +1227,14 @@ static int check_scan(const dwarf_selective_scan_fwd_args& a) {
   if (!a.A) return fail(DWARF_ERR_INVALID_ARGUMENT, "A is NULL");
   if (a.N == 0) return DWARF_OK;
   if ((rc = check_elements("x", a.x, a.dtype)) || (rc = check_elements("delta", a.delta, a.dtype)) ||
-      (rc = check_elements("B", a.Bm, a.dtype)) || (rc = check_elements("C", a.Cm, a.dtype)))
+      (rc = check_elements("B", a.Bm, a.dtype)) || (rc = check_elements("C", a.Cm, a.dtype)) ||
+      (a.gate && (rc = check_elements("gate", a.gate, a.dtype))))
     return rc;
-  return a.gate ? check_elements("gate", a.gate, a.dtype) : DWARF_OK;
+  if ((rc = check_token_stride("x", a.x_stride[1])) || (rc = check_token_stride("delta", a.delta_stride[1])) ||
+      (rc = check_token_stride("B", a.B_stride[1])) || (rc = check_token_stride("C", a.C_stride[1])) ||
+      (a.gate && (rc = check_token_stride("gate", a.gate_stride[1]))))
+    return rc;
+  return DWARF_OK;
 }
 
 static bool scan_sized(const dwarf_selective_scan_fwd_args* a) {
@@ -1247,7 +1259,7 @@ int dwarf_selective_scan_fwd(const dwarf_selective_scan_fwd_args* args, dwarf_st
   const dwarf_selective_scan_fwd_args& a = *args;
   int rc = check_scan(a);
   if (rc || a.B == 0) return rc ? rc : ok();
-  if (a.N && (rc = check_elements("y", a.y, a.dtype))) return rc;
+  if (a.N && ((rc = check_elements("y", a.y, a.dtype)) || (rc = check_token_stride("y", a.y_stride[1])))) return rc;
   if (a.checkpoints && (rc = check_checkpoints(a))) return rc;
   if (a.N == 0 && !a.final) return ok();
   const size_t need = dwarf::selective_scan_fwd_workspace(a);
@@ -1277,9 +1289,11 @@ int dwarf_selective_scan_bwd(const dwarf_selective_scan_bwd_args* args, dwarf_st
   if (a.fwd.N) {
     if ((rc = check_elements("dy", a.dy, a.fwd.dtype)) || (rc = check_elements("dx", a.dx, a.fwd.dtype)) ||
         (rc = check_elements("ddelta", a.ddelta, a.fwd.dtype)) || (rc = check_elements("dB", a.dB, a.fwd.dtype)) ||
-        (rc = check_elements("dC", a.dC, a.fwd.dtype)))
+        (rc = check_elements("dC", a.dC, a.fwd.dtype)) || (rc = check_token_stride("dy", a.dy_stride[1])) ||
+        (rc = check_token_stride("dx", a.dx_stride[1])) || (rc = check_token_stride("ddelta", a.ddelta_stride[1])))
       return rc;
-    if (a.fwd.gate && (rc = check_elements("dgate", a.dgate, a.fwd.dtype))) return rc;
+    if (a.fwd.gate && ((rc = check_elements("dgate", a.dgate, a.fwd.dtype)) || (rc = check_token_stride("dgate", a.dgate_stride[1]))))
+      return rc;
     if ((rc = check_checkpoints(a.fwd))) return rc;
   }
   const size_t need = dwarf::selective_scan_bwd_workspace(a);

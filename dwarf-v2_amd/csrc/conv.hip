@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(dwarf_causal_con
       for (int j = 0; j < W - 1; ++j) conv_input<T, VEC, W>(a, x, at.b, d, t0 - W + 1 + j, win[j + 1]);
       // tokens up to W - 1 behind the strip, whose dp its last tokens' dx need; none behind the sequence's end
       const int stop = end + W - 1;
-      T rx[kConvAhead][VEC], rg[kConvAhead][VEC];
+      T rx[kConvAhead][VEC] = {}, rg[kConvAhead][VEC] = {};   // zeros where no token is live
       auto fetch = [&](int t, int i) {   // behind the sequence's last token: that again
         const int64_t tt = min(t, max(n, 1) - 1);
         if (n > 0) {

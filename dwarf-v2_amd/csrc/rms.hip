@@ -357,7 +357,13 @@ int elem_bytes(int dtype) { return dtype == DWARF_F32 ? 4 : 2; }
 
 NormPlan rms_fwd_plan(const dwarf_rms_norm_fwd_args& a) {
   const int es = elem_bytes(a.dtype);
-  bool vec = norm_vec_ok(a.x, a.x_stride, es) && norm_vec_ok(a.y, a.y_stride, a.scale ? 1 : es);
+  bool vec = norm_vec_ok(a.x, a.x_stride, es);
+  if (a.scale) {   // as many bytes as x's vectors have elements
+    const int per = 16 / es;
+    vec = vec && reinterpret_cast<uintptr_t>(a.y) % per == 0 && a.y_stride[0] % per == 0 && a.y_stride[1] % per == 0;
+  } else {
+    vec = vec && norm_vec_ok(a.y, a.y_stride, es);
+  }
   if (a.residual) {
     const int rs = elem_bytes(a.residual_dtype);
     vec = vec && norm_vec_ok(a.residual, a.residual_stride, rs) && norm_vec_ok(a.sum, a.sum_stride, rs);

@@ -512,12 +512,19 @@ OptTensor causal_conv_step(const Tensor& x, const Tensor& weight, const OptTenso
 // B or C [..., G, S]; without groups, [..., S] is one.
 Tensor grouped(const Tensor& t, const Tensor& x) { return t.dim() == x.dim() ? t.unsqueeze(-2) : t; }
 
+// Rows of a sequence as the scan takes them: elements side by side, tokens less than 2^22 elements apart; others copied.
+Tensor scan_rows(const Tensor& t) {
+  const Tensor u = unit_rows(t);
+  return u.size(1) > 1 && u.stride(1) >= (int64_t(1) << 22) ? u.clone(at::MemoryFormat::Contiguous) : u;
+}
+int64_t step_along(const Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
 struct ScanOperands {
   Tensor x, delta, gate, B, C, A, skip, bias, initial, lengths;
   ScanOperands(const Tensor& x_, const Tensor& delta_, const Tensor& A_, const Tensor& B_, const Tensor& C_, const OptTensor& skip_,
                const OptTensor& gate_, const OptTensor& bias_, const OptTensor& initial_, const OptTensor& lengths_)
-      : x(unit_rows(x_)), delta(unit_rows(delta_)), gate(gate_ ? unit_rows(*gate_) : Tensor()), B(unit_rows(grouped(B_, x_))),
-        C(unit_rows(grouped(C_, x_))), A(table(A_)), skip(table(skip_)), bias(table(bias_)),
+      : x(scan_rows(x_)), delta(scan_rows(delta_)), gate(gate_ ? scan_rows(*gate_) : Tensor()), B(scan_rows(grouped(B_, x_))),
+        C(scan_rows(grouped(C_, x_))), A(table(A_)), skip(table(skip_)), bias(table(bias_)),
         initial(initial_ ? initial_->contiguous() : Tensor()), lengths(index_table(lengths_)) {}
   void fill(dwarf_selective_scan_fwd_args& a, bool softplus) const {
     a.B = size32(x.size(0));
@@ -528,16 +535,16 @@ struct ScanOperands {
     a.dtype = dtype_of(x, "x");
     a.softplus = softplus;
     a.x = x.const_data_ptr();
-    a.x_stride[0] = x.stride(0), a.x_stride[1] = x.stride(1);
+    a.x_stride[0] = step_along(x, 0), a.x_stride[1] = step_along(x, 1);
     a.delta = delta.const_data_ptr();
-    a.delta_stride[0] = delta.stride(0), a.delta_stride[1] = delta.stride(1);
+    a.delta_stride[0] = step_along(delta, 0), a.delta_stride[1] = step_along(delta, 1);
     if (gate.defined()) {
       a.gate = gate.const_data_ptr();
-      a.gate_stride[0] = gate.stride(0), a.gate_stride[1] = gate.stride(1);
+      a.gate_stride[0] = step_along(gate, 0), a.gate_stride[1] = step_along(gate, 1);
     }
     a.Bm = B.const_data_ptr();
     a.Cm = C.const_data_ptr();
-    for (int i = 0; i < 3; ++i) a.B_stride[i] = B.stride(i), a.C_stride[i] = C.stride(i);
+    for (int i = 0; i < 3; ++i) a.B_stride[i] = step_along(B, i), a.C_stride[i] = step_along(C, i);
     a.A = f32_ptr(A);
     a.skip = f32_ptr(skip);
     a.delta_bias = f32_ptr(bias);
@@ -581,7 +588,7 @@ ScanGrads scan_backward(const Tensor& dy_, const OptTensor& dstate, const Tensor
                         const OptTensor& initial, const OptTensor& lengths, const Tensor& checkpoints, bool softplus, bool need_A,
                         bool need_skip, bool need_bias, bool need_initial) {
   const ScanOperands in(x, delta, A, B, C, skip, gate, bias, initial, lengths);
-  const Tensor dy = unit_rows(dy_.to(x.scalar_type()));
+  const Tensor dy = scan_rows(dy_.to(x.scalar_type()));
   const Tensor df = dstate ? dstate->to(at::kFloat).contiguous() : Tensor();
   dwarf_selective_scan_bwd_args a{};
   in.fill(a.fwd, softplus);
@@ -589,7 +596,7 @@ ScanGrads scan_backward(const Tensor& dy_, const OptTensor& dstate, const Tensor
   a.fwd.checkpoints = const_cast<float*>(checkpoints.const_data_ptr<float>());
   a.fwd.checkpoint_bytes = static_cast<size_t>(checkpoints.numel()) * sizeof(float);
   a.dy = dy.const_data_ptr();
-  a.dy_stride[0] = dy.stride(0), a.dy_stride[1] = dy.stride(1);
+  a.dy_stride[0] = step_along(dy, 0), a.dy_stride[1] = step_along(dy, 1);
   a.dfinal = f32_ptr(df);
   ScanGrads g;
   g.dx = at::empty(x.sizes(), x.options());
@@ -693,6 +700,9 @@ void check_scan_inputs(const Tensor& x, const Tensor& delta, const Tensor& A, co
   TORCH_CHECK(S <= 64, "the scan is built for up to 64 states, got ", S);
   check_channels("skip", skip, D);
   check_channels("delta_bias", bias, D);
+}
+void check_scan_devices(const Tensor& x, const Tensor& delta, const Tensor& A, const Tensor& B, const Tensor& C, const OptTensor& skip,
+                        const OptTensor& gate, const OptTensor& bias) {
   check_cuda(x);
   check_beside("delta", delta, x);
   check_beside("A", A, x);
@@ -712,6 +722,7 @@ void check_scan(const Tensor& x, const Tensor& delta, const Tensor& A, const Ten
                       "initial_state must be fp32 [", x.size(0), ",", x.size(2), ",", A.size(1), "], got ", initial->sizes(), " ",
                       initial->scalar_type());
   check_lengths(lengths, x.size(0));
+  check_scan_devices(x, delta, A, B, C, skip, gate, bias);
   check_beside("initial_state", initial, x);
   check_beside("lengths", lengths, x);
 }
@@ -785,6 +796,7 @@ void check_scan_step(const Tensor& x, const Tensor& delta, const Tensor& A, cons
   check_scan_inputs(x, delta, A, B, C, skip, gate, bias, "rows");
   check_slots(slots, x.size(0));
   check_pools(state, new_state, slots, x.size(0), x.size(1), A.size(1), at::kFloat);
+  check_scan_devices(x, delta, A, B, C, skip, gate, bias);
   check_beside("state", state, x);
   check_beside("new_state", new_state, x);
   check_beside("slots", slots, x);

@@ -84,11 +84,12 @@ __device__ __forceinline__ float exp_f32(float x) {
 
 // log(1 + e^x) without a branch.  log(w) / (w - 1) changes slowly around the rounded w = 1 + e (and is 1 where w is next to
 // 1), so that times the exact e it is right however small e is: 3.5e-7 off at most over [-30, 21], 8e-8 on average.  Above 20
-// it is x.  (The library's calls, with their branches, took half of the forward's instructions.)
+// it is x, below -200, minus infinity included, 0.  (The library's calls, with their branches, took half of the forward's
+// instructions.)
 __device__ __forceinline__ float softplus_f32(float x) {
-  const float low = x > 20.f ? 20.f : x;
-  const float e = exp_f32(low), w = fmaxf(1.f + e, 1.00000012f);
-  return fmaf(__builtin_amdgcn_logf(w) * 0.693147181f, e * __builtin_amdgcn_rcpf(w - 1.f), x - low);
+  const float e = exp_f32(__builtin_amdgcn_fmed3f(x, -200.f, 20.f)), w = fmaxf(1.f + e, 1.00000012f);
+  const float above = (x < 20.f ? 20.f : x) - 20.f;   // NaN for a NaN
+  return fmaf(__builtin_amdgcn_logf(w) * 0.693147181f, e * __builtin_amdgcn_rcpf(w - 1.f), above);
 }
 // Chosen, not branched to: a branch for each quad of tokens keeps the compiler from working on several of them at once.
 __device__ __forceinline__ float step_of(float raw, bool softplus) {
@@ -241,7 +242,7 @@ struct WideRows {
   int64_t stride[kEach]; // bytes of a token
   int row[kEach], spot[kEach];
   bool ok[kEach];        // the vector is one of the tile's and its group's
-  __device__ __forceinline__ WideRows(const ScanRows (&rows)[NS], const ScanLane<LPC>& lane, int D, int t) {
+  __device__ __forceinline__ WideRows(const ScanRows* rows, const ScanLane<LPC>& lane, int D, int t) {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int i = e * kScanThreads + threadIdx.x, which = min(i / kVecs, NS - 1), vec = i % Tile::kNv;
@@ -272,7 +273,7 @@ struct ScanIn {   // WIDE
   T* lds;
   int mine;
   static constexpr int kSpan = NS * TOK * ScanTile<T, LPC>::kCh;   // of one of the two buffers
-  __device__ __forceinline__ ScanIn(const ScanRows (&in)[NS], const ScanLane<LPC>& lane, int D, int t, T* lds_)
+  __device__ __forceinline__ ScanIn(const ScanRows* in, const ScanLane<LPC>& lane, int D, int t, T* lds_)
       : rows(in, lane, D, t), lds(lds_), mine(ScanTile<T, LPC>::spot(lane.lane & 3, lane.local)) {}
   __device__ __forceinline__ void move(int tiles) { rows.move(tiles); }
   __device__ __forceinline__ void fetch(int live) {
@@ -301,9 +302,9 @@ struct ScanIn<T, TOK, LPC, NS, false> {
   T r[NS][TOK / 4];
   float v[NS][TOK / 4];
   template <int... I>
-  __device__ __forceinline__ ScanIn(const ScanRows (&in)[NS], const ScanLane<LPC>& lane, int t, std::integer_sequence<int, I...>)
+  __device__ __forceinline__ ScanIn(const ScanRows* in, const ScanLane<LPC>& lane, int t, std::integer_sequence<int, I...>)
       : q{QuadRows<T, TOK / 4>(in[I].p, in[I].sequence, in[I].stride, lane.d, t, lane.lane & 3)...}, given{in[I].p != nullptr...} {}
-  __device__ __forceinline__ ScanIn(const ScanRows (&in)[NS], const ScanLane<LPC>& lane, int, int t, T*)
+  __device__ __forceinline__ ScanIn(const ScanRows* in, const ScanLane<LPC>& lane, int, int t, T*)
       : ScanIn(in, lane, t, std::make_integer_sequence<int, NS>()) {}
   __device__ __forceinline__ void move(int tiles) {
 #pragma unroll
@@ -329,7 +330,7 @@ struct ScanOut {   // WIDE
   T* lds;
   int mine;
   static constexpr int kSpan = NS * TOK * ScanTile<T, LPC>::kCh;
-  __device__ __forceinline__ ScanOut(const ScanRows (&out)[NS], const ScanLane<LPC>& lane, int D, int t, T* lds_)
+  __device__ __forceinline__ ScanOut(const ScanRows* out, const ScanLane<LPC>& lane, int D, int t, T* lds_)
       : rows(out, lane, D, t), lds(lds_), mine(ScanTile<T, LPC>::spot(lane.lane & 3, lane.local)) {}
   __device__ __forceinline__ void move(int tiles) { rows.move(tiles); }
   __device__ __forceinline__ void put(int which, int buf, int k, float x) {
@@ -356,9 +357,9 @@ struct ScanOut<T, TOK, LPC, NS, false> {
   bool given[NS];
   float v[NS][TOK / 4];
   template <int... I>
-  __device__ __forceinline__ ScanOut(const ScanRows (&out)[NS], const ScanLane<LPC>& lane, int t, std::integer_sequence<int, I...>)
+  __device__ __forceinline__ ScanOut(const ScanRows* out, const ScanLane<LPC>& lane, int t, std::integer_sequence<int, I...>)
       : q{QuadRows<T, TOK / 4>(out[I].p, out[I].sequence, out[I].stride, lane.d, t, lane.lane & 3)...}, given{out[I].p != nullptr...} {}
-  __device__ __forceinline__ ScanOut(const ScanRows (&out)[NS], const ScanLane<LPC>& lane, int, int t, T*)
+  __device__ __forceinline__ ScanOut(const ScanRows* out, const ScanLane<LPC>& lane, int, int t, T*)
       : ScanOut(out, lane, t, std::make_integer_sequence<int, NS>()) {}
   __device__ __forceinline__ void move(int tiles) {
 #pragma unroll
@@ -413,11 +414,21 @@ __device__ __forceinline__ void store_user_states(float* p, int s0, int S, const
     if (s0 + s < S) p[s0 + s] = h[s];
 }
 
-// A in base 2, so that the decay is one exp2.
+// A in base 2, so that the decay is one exp2; finite where A is minus infinity, so that a step of 0 decays nothing.
+__device__ __forceinline__ float rate_of(float A) {
+  const float r = A * kLog2e;
+  return r < -3.4e38f ? -3.4e38f : r;
+}
 template <int SPL>
 __device__ __forceinline__ void load_rates(const float* A, int64_t d, int s0, int S, float* rate) {
 #pragma unroll
-  for (int s = 0; s < SPL; ++s) rate[s] = s0 + s < S ? A[d * S + s0 + s] * kLog2e : 0.f;
+  for (int s = 0; s < SPL; ++s) rate[s] = s0 + s < S ? rate_of(A[d * S + s0 + s]) : 0.f;
+}
+
+// The state (or adjoint) behind a segment from the one in front: nothing stays nothing, also where a growing segment's
+// factor is out of range.
+__device__ __forceinline__ float joined(float h, float sum, float rate, float add) {
+  return h == 0.f ? add : fmaf(__builtin_amdgcn_exp2f(sum * rate), h, add);
 }
 
 // LOCAL: what a segment adds from zero and its sum of steps, for all segments but the last; otherwise the rows.
@@ -447,7 +458,7 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
       load_states<SPL>(gm.local + row * SP + s0, add);
       const float sum = gm.steps[row];
 #pragma unroll
-      for (int s = 0; s < SPL; ++s) h[s] = fmaf(__builtin_amdgcn_exp2f(sum * rate[s]), h[s], add[s]);
+      for (int s = 0; s < SPL; ++s) h[s] = joined(h[s], sum, rate[s], add[s]);
     }
   }
   const bool gated = !LOCAL && a.gate, softplus = a.softplus, writes = at.in && at.sq < 4;
@@ -455,7 +466,7 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
   const ScanRows ins[3] = {{a.x, at.b * a.x_stride[0], a.x_stride[1]}, {a.delta, at.b * a.delta_stride[0], a.delta_stride[1]},
                            {gated ? a.gate : nullptr, at.b * a.gate_stride[0], a.gate_stride[1]}};
   const ScanRows outs[1] = {{a.y, at.b * a.y_stride[0], a.y_stride[1]}};
-  ScanIn<T, kTile, LPC, kIns, WIDE> in(reinterpret_cast<const ScanRows(&)[kIns]>(ins), at, a.D, t0, s_in);
+  ScanIn<T, kTile, LPC, kIns, WIDE> in(ins, at, a.D, t0, s_in);
   ScanOut<T, kTile, LPC, 1, WIDE> out(outs, at, a.D, t0, s_out);
   BcRows<T, SP, kTile> rb(static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2], a.B_stride[1], t0, a.S);
   BcRows<T, SP, kTile> rc(static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2], a.C_stride[1], t0, a.S);
@@ -718,7 +729,7 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
     load_states<SPL>(gm.local + row * SP + s0, add);
     const float sum = gm.steps[row];
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) ga[s] = fmaf(__builtin_amdgcn_exp2f(sum * rate[s]), ga[s], add[s]);
+    for (int s = 0; s < SPL; ++s) ga[s] = joined(ga[s], sum, rate[s], add[s]);
   }
   if (!at.in)
 #pragma unroll
@@ -1013,7 +1024,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(dwarf_selective
   if constexpr (WHOLE) {
     __builtin_memcpy(rate, a.A + d * a.S + s0, sizeof(rate));
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) rate[s] *= kLog2e;
+    for (int s = 0; s < SPL; ++s) rate[s] = rate_of(rate[s]);
   } else {
     load_rates<SPL>(a.A, d, s0, a.S, rate);
   }

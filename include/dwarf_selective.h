@@ -128,7 +128,8 @@ int dwarf_causal_conv_step(const dwarf_causal_conv_step_args* args, dwarf_stream
  *   h_t = a h_{t-1} + step x_t B_t[g],   y_t = (C_t[g] . h_t + skip x_t) silu(gate_t)
  * over the first lengths[b] tokens (all N where NULL; clamped to [0, N]), y zero behind them and nothing used there.
  * x, delta, gate (may be NULL: factor 1) and y [B][N][D] (batch stride, token stride, unit channel stride); Bm, Cm
- * [B][N][G][S] (batch, token, group stride, unit state stride), all in dtype.  A [D][S], skip and delta_bias [D]
+ * [B][N][G][S] (batch, token, group stride, unit state stride), all in dtype; token strides, the backward's too, lie in
+ * [0, 2^22) elements, D below 2^22.  A [D][S], skip and delta_bias [D]
  * (each may be NULL: 0) fp32.  h_{-1} = initial [B][D][S] fp32 (NULL: zero), final [B][D][S] = the state behind the
  * last live token (may be NULL).  checkpoints: dwarf_selective_scan_checkpoint_bytes() bytes that the backward reads,
  * NULL where there will be none.
