@@ -182,18 +182,24 @@ __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(dwarf_causal_con
     for (int j = 0; j < W; ++j)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) dp[j][e] = 0.f;
-    if (t0 < end || from < 0) {
+    if (n == 0 && from < 0) {   // no token is live: the state that enters leaves
+      for (int j = 0; j < W - 1; ++j) {
+        float f[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = 0.f;
+        if (df) load_any<T, VEC>(df + static_cast<int64_t>(j) * a.D, f);
+        store_any<T, VEC>(di + static_cast<int64_t>(j) * a.D, f);
+      }
+    } else if (t0 < end || from < 0) {
 #pragma unroll
       for (int j = 0; j < W - 1; ++j) conv_input<T, VEC, W>(a, x, at.b, d, t0 - W + 1 + j, win[j + 1]);
       // tokens up to W - 1 behind the strip, whose dp its last tokens' dx need; none behind the sequence's end
       const int stop = end + W - 1;
-      T rx[kConvAhead][VEC] = {}, rg[kConvAhead][VEC] = {};   // zeros where no token is live
+      T rx[kConvAhead][VEC], rg[kConvAhead][VEC];
       auto fetch = [&](int t, int i) {   // behind the sequence's last token: that again
-        const int64_t tt = min(t, max(n, 1) - 1);
-        if (n > 0) {
-          __builtin_memcpy(rx[i], x + tt * a.x_stride[1], sizeof(rx[i]));
-          __builtin_memcpy(rg[i], dy + tt * w_.dy_stride[1], sizeof(rg[i]));
-        }
+        const int64_t tt = min(t, n - 1);
+        __builtin_memcpy(rx[i], x + tt * a.x_stride[1], sizeof(rx[i]));
+        __builtin_memcpy(rg[i], dy + tt * w_.dy_stride[1], sizeof(rg[i]));
       };
 #pragma unroll
       for (int i = 0; i < kConvAhead; ++i) fetch(t0 + i, i);
