@@ -57,8 +57,14 @@ struct ScanGeom {
   float* part_d;             // [B][segs][2][D]: skip, bias
 };
 
-template <int J>
-__device__ __forceinline__ float quad_lane(float x) { return dpp_f<J * 0x55>(x); }
+// Lane j's value of each quad; j is known once loops are unrolled.  Next to what uses it, it is no instruction of its own
+// but an operand's.
+__device__ __forceinline__ float quad_lane(float x, int j) {
+  if (j == 0) return dpp_f<0x00>(x);
+  if (j == 1) return dpp_f<0x55>(x);
+  if (j == 2) return dpp_f<0xAA>(x);
+  return dpp_f<0xFF>(x);
+}
 
 // Lane i of each quad receives the sum of p[i] over the LPC lanes of its channel.
 template <int LPC>
@@ -86,14 +92,20 @@ __device__ __forceinline__ float exp_f32(float x) {
 // 1), so that times the exact e it is right however small e is: 3.5e-7 off at most over [-30, 21], 8e-8 on average.  Above 20
 // it is x, below -200, minus infinity included, 0.  (The library's calls, with their branches, took half of the forward's
 // instructions.)
-__device__ __forceinline__ float softplus_f32(float x) {
-  const float e = exp_f32(__builtin_amdgcn_fmed3f(x, -200.f, 20.f)), w = fmaxf(1.f + e, 1.00000012f);
-  const float above = (x < 20.f ? 20.f : x) - 20.f;   // NaN for a NaN
-  return fmaf(__builtin_amdgcn_logf(w) * 0.693147181f, e * __builtin_amdgcn_rcpf(w - 1.f), above);
-}
-// Chosen, not branched to: a branch for each quad of tokens keeps the compiler from working on several of them at once.
+struct Softplus {
+  float e, above;
+  __device__ __forceinline__ explicit Softplus(float x)
+      : e(exp_f32(__builtin_amdgcn_fmed3f(x, -200.f, 20.f))), above((x < 20.f ? 20.f : x) - 20.f) {}   // NaN for a NaN
+  __device__ __forceinline__ float value() const {
+    const float w = fmaxf(1.f + e, 1.00000012f);
+    return fmaf(__builtin_amdgcn_logf(w) * 0.693147181f, e * __builtin_amdgcn_rcpf(w - 1.f), above);
+  }
+  __device__ __forceinline__ float slope() const { return e * __builtin_amdgcn_rcpf(1.f + e); }   // 1 / (1 + e^-x)
+};
+// Chosen, not branched to: both sides are formed first.  A branch for each quad of tokens keeps the compiler from working on
+// several of them at once.
 __device__ __forceinline__ float step_of(float raw, bool softplus) {
-  const float s = softplus_f32(raw);
+  const float s = Softplus(raw).value();
   return softplus ? s : raw;
 }
 // What step_of makes a step of 0 of.
@@ -378,6 +390,18 @@ struct ScanOut<T, TOK, LPC, NS, false> {
 };
 
 template <int SPL>
+__device__ __forceinline__ void scaled(float f, const float* x, float* y) {
+#pragma unroll
+  for (int s = 0; s < SPL; ++s) y[s] = f * x[s];
+}
+template <int SPL>
+__device__ __forceinline__ void decays(float step, const float* rate, float* dec) {
+  scaled<SPL>(step, rate, dec);
+#pragma unroll
+  for (int s = 0; s < SPL; ++s) dec[s] = __builtin_amdgcn_exp2f(dec[s]);
+}
+
+template <int SPL>
 __device__ __forceinline__ void load_states(const float* p, float* h) {
   if constexpr (SPL == 2) {
     const float2 v = *reinterpret_cast<const float2*>(p);
@@ -461,7 +485,8 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
       for (int s = 0; s < SPL; ++s) h[s] = joined(h[s], sum, rate[s], add[s]);
     }
   }
-  const bool gated = !LOCAL && a.gate, softplus = a.softplus, writes = at.in && at.sq < 4;
+  const bool gated = !LOCAL && a.gate, writes = at.in && at.sq < 4;
+  const bool softplus = a.softplus;
   const float none = no_step(softplus);
   const ScanRows ins[3] = {{a.x, at.b * a.x_stride[0], a.x_stride[1]}, {a.delta, at.b * a.delta_stride[0], a.delta_stride[1]},
                            {gated ? a.gate : nullptr, at.b * a.gate_stride[0], a.gate_stride[1]}};
@@ -534,15 +559,16 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
         if (k + 1 < kQuads) begin(k + 1);
         if (k + 2 < kQuads) look(k + 2);
         const int i = k & 1;
-        const float stj[4] = {quad_lane<0>(st[i]), quad_lane<1>(st[i]), quad_lane<2>(st[i]), quad_lane<3>(st[i])};
-        const float suj[4] = {quad_lane<0>(su[i]), quad_lane<1>(su[i]), quad_lane<2>(su[i]), quad_lane<3>(su[i])};
         float p[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+          float dec[SPL], add[SPL];
+          decays<SPL>(quad_lane(st[i], j), rate, dec);
+          scaled<SPL>(quad_lane(su[i], j), B[i] + j * SPL, add);
           p[j] = 0.f;
 #pragma unroll
           for (int s = 0; s < SPL; ++s) {
-            h[s] = fmaf(__builtin_amdgcn_exp2f(stj[j] * rate[s]), h[s], suj[j] * B[i][j * SPL + s]);
+            h[s] = fmaf(dec[s], h[s], add[s]);
             if constexpr (!LOCAL) p[j] = fmaf(h[s], C[i][j * SPL + s], p[j]);
           }
         }
@@ -600,7 +626,8 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
   const float bias = a.delta_bias ? a.delta_bias[d] : 0.f;
 #pragma unroll
   for (int s = 0; s < SPL; ++s) ga[s] = 0.f;
-  const bool gated = a.gate != nullptr, softplus = a.softplus;
+  const bool gated = a.gate != nullptr;
+  const bool softplus = a.softplus;
   const float none = no_step(softplus);
   const int tiles = end > t0 ? (end - t0 + kTile - 1) / kTile : 0, last = t0 + (tiles - 1) * kTile;
   const ScanRows ins[3] = {{w.dy, at.b * w.dy_stride[0], w.dy_stride[1]}, {a.delta, at.b * a.delta_stride[0], a.delta_stride[1]},
@@ -646,12 +673,16 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
         if (k) begin(k - 1);
         if (k > 1) look(k - 2);
         const int m = k & 1;
-        const float stj[4] = {quad_lane<0>(st[m]), quad_lane<1>(st[m]), quad_lane<2>(st[m]), quad_lane<3>(st[m])};
-        const float goj[4] = {quad_lane<0>(go[m]), quad_lane<1>(go[m]), quad_lane<2>(go[m]), quad_lane<3>(go[m])};
 #pragma unroll
-        for (int j = 3; j >= 0; --j)
+        for (int j = 3; j >= 0; --j) {
+          float dec[SPL];
+          decays<SPL>(quad_lane(st[m], j), rate, dec);
+          const float goj = quad_lane(go[m], j);
 #pragma unroll
-          for (int s = 0; s < SPL; ++s) ga[s] = __builtin_amdgcn_exp2f(stj[j] * rate[s]) * fmaf(C[m][j * SPL + s], goj[j], ga[s]);
+          for (int s = 0; s < SPL; ++s) ga[s] = fmaf(goj, C[m][j * SPL + s], ga[s]);
+#pragma unroll
+          for (int s = 0; s < SPL; ++s) ga[s] *= dec[s];
+        }
       }
       if (i) {
         rc.store(s_c[buf ^ 1], kTile, a.S);
@@ -668,10 +699,20 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
   }
 }
 
-// Sums v[0 .. M-1] over the wave's channels (the lane bits above LPC's); lane l gets values which(l) .. which(l) + kLeft - 1.
-template <int LPC, int M>
+template <int N>
+__device__ __forceinline__ void store_left(float* p, const float* x) {
+  if constexpr (N == 1) p[0] = x[0];
+  else if constexpr (N == 2) *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
+  else *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+
+// Sums v[0 .. 2 SPL - 1] over the wave's channels, the lane bits above LPC's: bit 5 and bit 4 each leave a lane with half of
+// the values and add those of two lanes, bit 3 adds.  With four lanes to a channel bit 2 is left to the sum over the waves:
+// there an addition takes a thread's, here every lane's turn.
+template <int SPL, int LPC>
 struct ChannelSums {
-  static constexpr int kLeft = M >= 8 ? M / 8 : 1;   // values a lane ends with
+  static constexpr int M = 2 * SPL, kLeft = M / 4;   // values a lane ends with
+  static constexpr int kParts = LPC == 4 ? 2 : 1;    // partial sums a wave leaves
   static __device__ __forceinline__ float swap_add32(float a, float b) {
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
     return __builtin_bit_cast(float, static_cast<unsigned>(r[0])) + __builtin_bit_cast(float, static_cast<unsigned>(r[1]));
@@ -680,38 +721,27 @@ struct ChannelSums {
     const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
     return __builtin_bit_cast(float, static_cast<unsigned>(r[0])) + __builtin_bit_cast(float, static_cast<unsigned>(r[1]));
   }
-  // out[i] is value which(lane) + i: lane bit 5 chooses between the halves of v, bit 4 between the halves of that, bit 3
-  // (where there are more than two left) again
-  static __device__ __forceinline__ void sum(const float* v, float* out, int lane) {
+  // out[i] is value which(lane) + i
+  static __device__ __forceinline__ void sum(const float* v, float* out) {
     float w[M / 2];
 #pragma unroll
     for (int i = 0; i < M / 2; ++i) w[i] = swap_add32(v[i], v[i + M / 2]);
-    float x[M / 4];
 #pragma unroll
-    for (int i = 0; i < M / 4; ++i) x[i] = swap_add16(w[i], w[i + M / 4]);
-    if constexpr (M >= 8) {
-      const bool up = lane & 8;
-#pragma unroll
-      for (int i = 0; i < M / 8; ++i) out[i] = (up ? x[i + M / 8] : x[i]) + dpp_f<0x128>(up ? x[i] : x[i + M / 8]);
-    } else {
-      out[0] = x[0] + dpp_f<0x128>(x[0]);   // row_ror:8
-    }
-    if constexpr (LPC == 4) {
-#pragma unroll
-      for (int i = 0; i < kLeft; ++i) out[i] += dpp_f<0x1B>(dpp_f<0x141>(out[i]));   // lane ^ 7, then ^ 3: the other quad
+    for (int i = 0; i < M / 4; ++i) {
+      const float x = swap_add16(w[i], w[i + M / 4]);
+      out[i] = x + dpp_f<0x128>(x);   // row_ror:8
     }
   }
-  static __device__ __forceinline__ int which(int lane) {
-    return (lane >> 5 & 1) * (M / 2) + (lane >> 4 & 1) * (M / 4) + (M >= 8 ? (lane >> 3 & 1) * (M / 8) : 0);
-  }
+  static __device__ __forceinline__ int which(int lane) { return (lane >> 5 & 1) * (M / 2) + (lane >> 4 & 1) * (M / 4); }
+  static __device__ __forceinline__ int part(int lane) { return kParts == 2 ? lane >> 2 & 1 : 0; }
 };
 
 template <typename T, int SPL, int LPC, bool WIDE>
 __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void scan_bwd_kernel(dwarf_selective_scan_bwd_args w, ScanGeom gm) {
   constexpr int SP = SPL * LPC, kK = scan_chunk(SPL), kQuads = kK / 4;
-  using Sums = ChannelSums<LPC, 2 * SPL>;
+  using Sums = ChannelSums<SPL, LPC>;
   __shared__ __align__(16) float s_b[2][kK * SP], s_c[2][kK * SP];
-  __shared__ float s_sum[2][kScanWaves][kK][2 * SP];
+  __shared__ __align__(16) float s_sum[2][kScanWaves][kK][Sums::kParts][2 * SP];
   __shared__ __align__(16) T s_in[2 * ScanIn<T, kK, LPC, 4, WIDE>::kSpan];
   __shared__ __align__(16) T s_out[2 * ScanOut<T, kK, LPC, 3, WIDE>::kSpan];
   const dwarf_selective_scan_fwd_args& a = w.fwd;
@@ -734,7 +764,8 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
   if (!at.in)
 #pragma unroll
     for (int s = 0; s < SPL; ++s) ga[s] = 0.f;
-  const bool gated = a.gate != nullptr, softplus = a.softplus, writes = at.in && at.sq < 4;
+  const bool gated = a.gate != nullptr, writes = at.in && at.sq < 4;
+  const bool softplus = a.softplus;
   const float none = no_step(softplus);
   const int chunks = end > t0 ? (end - t0 + kK - 1) / kK : 0, last = t0 + (chunks - 1) * kK;
   const ScanRows ins[4] = {{a.x, at.b * a.x_stride[0], a.x_stride[1]}, {a.delta, at.b * a.delta_stride[0], a.delta_stride[1]},
@@ -762,27 +793,31 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
     part[i * part_step + threadIdx.x % (2 * SP)] = 0.f;
 
   float hn[SPL];
-  const int place = Sums::which(at.lane) / SPL * SP + s0 + Sums::which(at.lane) % SPL;   // lanes with the same sum write it alike
+  // lanes with the same sum write it alike
+  const int place = Sums::part(at.lane) * (2 * SP) + Sums::which(at.lane) / SPL * SP + s0 + Sums::which(at.lane) % SPL;
   // A chunk's results go to memory while the next one is worked on: read from LDS behind the barrier, stored later.
-  constexpr int kSums = kK * 2 * SP / kScanThreads;
-  float sums[kSums][kScanWaves];
+  constexpr int kSums = kK * 2 * SP / kScanThreads, kSumTokens = kScanThreads / (2 * SP);   // of a thread; of all at once
+  float* sums_to = part + (last + static_cast<int>(threadIdx.x) / (2 * SP)) * part_step + threadIdx.x % (2 * SP);
+  float sums[kSums][kScanWaves * Sums::kParts];
   auto collect = [&](int from) {
 #pragma unroll
     for (int e = 0; e < kSums; ++e)
 #pragma unroll
-      for (int v = 0; v < kScanWaves; ++v)
-        sums[e][v] = (&s_sum[from][v][0][0])[e * kScanThreads + threadIdx.x];
+      for (int v = 0; v < kScanWaves * Sums::kParts; ++v) {
+        const int at_ = e * kScanThreads + threadIdx.x;
+        sums[e][v] = s_sum[from][v / Sums::kParts][at_ / (2 * SP)][v % Sums::kParts][at_ % (2 * SP)];
+      }
     if constexpr (WIDE) out.collect(from);
   };
-  auto send = [&](int t, int live) {
+  auto send = [&](int live) {   // of chunk after chunk, from the last
 #pragma unroll
     for (int e = 0; e < kSums; ++e) {
-      const int at_ = e * kScanThreads + threadIdx.x, n = at_ / (2 * SP);
       float x = sums[e][0];
 #pragma unroll
-      for (int v = 1; v < kScanWaves; ++v) x += sums[e][v];
-      if (n < live) part[(t + n) * part_step + at_ % (2 * SP)] = x;
+      for (int v = 1; v < kScanWaves * Sums::kParts; ++v) x += sums[e][v];
+      if (e * kSumTokens + static_cast<int>(threadIdx.x) / (2 * SP) < live) sums_to[e * kSumTokens * part_step] = x;
     }
+    sums_to -= kK * part_step;
     if constexpr (WIDE) {
       out.send(live);
       out.move(-1);
@@ -800,7 +835,7 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
     __syncthreads();
     for (int i = chunks - 1; i >= 0; --i, buf ^= 1) {
       const int t = t0 + i * kK;
-      float h0[SPL], u[kQuads], raw[kQuads], z[kQuads], dy[kQuads], st[kQuads], su[kQuads], go[kQuads];
+      float h0[SPL], u[kQuads], raw[kQuads], z[kQuads], dy[kQuads], st[kQuads], slope[kQuads], su[kQuads], go[kQuads];
 #pragma unroll
       for (int s = 0; s < SPL; ++s) h0[s] = hn[s];
 #pragma unroll
@@ -809,6 +844,7 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
         const float vx = in.get(0, buf, k), vd = in.get(1, buf, k) + bias, vg = in.get(2, buf, k), vz = in.get(3, buf, k);
         u[k] = live ? vx : 0.f;
         raw[k] = live ? vd : none;
+        slope[k] = live ? 1.f : 0.f;   // the adjoint goes on through tokens behind the end, unchanged
         dy[k] = live ? vg : 0.f;
         z[k] = live && gated ? vz : 0.f;
       }
@@ -828,7 +864,10 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
       auto begin = [&](int k) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) load_states<SPL>(s_b[buf] + (4 * k + j) * SP + s0, R[k & 1] + j * SPL);
-        st[k] = step_of(raw[k], softplus);
+        const Softplus sp(raw[k]);
+        const float s = sp.value(), d = sp.slope();
+        st[k] = softplus ? s : raw[k];
+        slope[k] = softplus ? d : slope[k];
         su[k] = st[k] * u[k];
         go[k] = dy[k] * act_of(z[k], gated);
       };
@@ -837,19 +876,19 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
       for (int k = 0; k < kQuads; ++k) {
         __builtin_amdgcn_sched_barrier(0);
         if (k + 1 < kQuads) begin(k + 1);
-        const float stj[4] = {quad_lane<0>(st[k]), quad_lane<1>(st[k]), quad_lane<2>(st[k]), quad_lane<3>(st[k])};
-        const float suj[4] = {quad_lane<0>(su[k]), quad_lane<1>(su[k]), quad_lane<2>(su[k]), quad_lane<3>(su[k])};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int n = 4 * k + j;
+          float add[SPL];
+          decays<SPL>(quad_lane(st[k], j), rate, dec[n]);
+          scaled<SPL>(quad_lane(su[k], j), R[k & 1] + j * SPL, add);
 #pragma unroll
-          for (int s = 0; s < SPL; ++s) {
-            dec[n][s] = __builtin_amdgcn_exp2f(stj[j] * rate[s]);
-            hs[n][s] = fmaf(dec[n][s], n ? hs[n ? n - 1 : 0][s] : h0[s], suj[j] * R[k & 1][j * SPL + s]);
-          }
+          for (int s = 0; s < SPL; ++s) hs[n][s] = fmaf(dec[n][s], n ? hs[n ? n - 1 : 0][s] : h0[s], add[s]);
         }
       }
-      if (i + 1 < chunks) send(t + kK, min(kK, end - t - kK));
+#pragma unroll
+      for (int s = 0; s < SPL; ++s) asm volatile("" : "+v"(hs[kK - 1][s]));   // the pass ends here, not behind the branch
+      if (i + 1 < chunks) send(min(kK, end - t - kK));
       // and back through them; the rows of the two tokens in front are read meanwhile
       float cA[SPL], cskip = 0.f, cbias = 0.f, B[2][2 * SPL], C[2][2 * SPL];
 #pragma unroll
@@ -864,9 +903,8 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
       rows(kK / 2 - 1);
 #pragma unroll
       for (int k = kQuads - 1; k >= 0; --k) {
-        const float stj[4] = {quad_lane<0>(st[k]), quad_lane<1>(st[k]), quad_lane<2>(st[k]), quad_lane<3>(st[k])};
-        const float suj[4] = {quad_lane<0>(su[k]), quad_lane<1>(su[k]), quad_lane<2>(su[k]), quad_lane<3>(su[k])};
-        const float goj[4] = {quad_lane<0>(go[k]), quad_lane<1>(go[k]), quad_lane<2>(go[k]), quad_lane<3>(go[k])};
+        // other values to the compiler than the first pass's: their way to a quad's lanes is an operand's again, not kept
+        asm("" : "+v"(st[k]), "+v"(su[k]));
         float into[4], mA[4], o[4];
 #pragma unroll
         for (int j = 3; j >= 0; --j) {
@@ -877,32 +915,38 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
           }
           const float* Bn = B[pair & 1] + n % 2 * SPL;
           const float* Cn = C[pair & 1] + n % 2 * SPL;
-          float v[2 * SPL], left[Sums::kLeft];
+          float g[SPL], m[SPL], v[2 * SPL], left[Sums::kLeft];
+          const float goj = quad_lane(go[k], j);
+#pragma unroll
+          for (int s = 0; s < SPL; ++s) g[s] = fmaf(goj, Cn[s], ga[s]);
+          scaled<SPL>(goj, hs[n], v + SPL);
+          scaled<SPL>(quad_lane(su[k], j), g, v);
+#pragma unroll
+          for (int s = 0; s < SPL; ++s) {
+            ga[s] = g[s] * dec[n][s];
+            m[s] = ga[s] * (n ? hs[n ? n - 1 : 0][s] : h0[s]);
+          }
+          const float stj = quad_lane(st[k], j);
+#pragma unroll
+          for (int s = 0; s < SPL; ++s) cA[s] = fmaf(stj, m[s], cA[s]);
           into[j] = mA[j] = o[j] = 0.f;
 #pragma unroll
           for (int s = 0; s < SPL; ++s) {
-            const float g = fmaf(Cn[s], goj[j], ga[s]);
-            v[s] = g * suj[j];
-            v[SPL + s] = goj[j] * hs[n][s];
-            into[j] = fmaf(g, Bn[s], into[j]);
-            ga[s] = g * dec[n][s];
-            const float m = ga[s] * (n ? hs[n ? n - 1 : 0][s] : h0[s]);
-            cA[s] = fmaf(m, stj[j], cA[s]);
-            mA[j] = fmaf(m, rate[s], mA[j]);
+            into[j] = fmaf(g[s], Bn[s], into[j]);
+            mA[j] = fmaf(m[s], rate[s], mA[j]);
             o[j] = fmaf(hs[n][s], Cn[s], o[j]);
           }
-          Sums::sum(v, left, at.lane);
-#pragma unroll
-          for (int e = 0; e < Sums::kLeft; ++e) s_sum[buf][at.wave][n][place + e] = left[e];   // dB's states, then dC's
+          Sums::sum(v, left);
+          store_left<Sums::kLeft>(&s_sum[buf][at.wave][n][0][0] + place, left);   // dB's states, then dC's
         }
         const float gB = quad_sums<LPC>(into[0], into[1], into[2], into[3], at.lane);
         const float gA = quad_sums<LPC>(mA[0], mA[1], mA[2], mA[3], at.lane) * (1.f / kLog2e);
         const float scanned = fmaf(skip, u[k], quad_sums<LPC>(o[0], o[1], o[2], o[3], at.lane)), e = sigmoid_f32(z[k]);
-        const float slope = sigmoid_f32(raw[k]), all = fmaf(u[k], gB, gA);
-        // the adjoint goes on through tokens behind the end, unchanged
-        const float dd = t + 4 * k + quad < end ? softplus ? all * slope : all : 0.f;
+        const float dd = fmaf(u[k], gB, gA) * slope[k];
         cskip = fmaf(go[k], u[k], cskip);
         cbias += dd;
+#pragma unroll
+        for (int s = 0; s < SPL; ++s) asm("" : "+v"(cA[s]));   // summed here, not behind the chunk from products kept until then
         out.put(0, buf, k, fmaf(st[k], gB, skip * go[k]));
         out.put(1, buf, k, dd);
         out.put(2, buf, k, dy[k] * scanned * (e * fmaf(z[k], 1.f - e, 1.f)));
@@ -915,10 +959,8 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
       }
 #pragma unroll
       for (int s = 0; s < SPL; ++s) dA[s] += cA[s];
-      if (at.in) {   // lanes behind the group's end have computed its last channel's steps
-        dskip += cskip;
-        dbias += cbias;
-      }
+      dskip += cskip;
+      dbias += cbias;
       __syncthreads();   // one barrier a chunk: what it lets through writes the other buffers
       if constexpr (!WIDE) {
         out.flush(end - t, at);
@@ -926,7 +968,7 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
       }
     }
     collect(buf ^ 1);
-    send(t0, min(kK, end - t0));
+    send(min(kK, end - t0));
   }
   if (!at.in) return;
   const int64_t row = static_cast<int64_t>(at.b) * gm.segs + at.seg;
@@ -1029,18 +1071,19 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(dwarf_selective
     load_rates<SPL>(a.A, d, s0, a.S, rate);
   }
   const float bias = a.delta_bias ? a.delta_bias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
+  const bool softplus = a.softplus, gated = a.gate != nullptr;
   SameSlot same{false, a.R};
   if (a.slots) same = same_slot<kScanThreads>(a.slots, slot, row0, a.R, s_found);
   if (same.before) return;   // uniform
   for (int row = row0; row < a.R;) {
-    const float st = step_of(raw + bias, a.softplus), su = st * x;
+    const float st = step_of(raw + bias, softplus), su = st * x;
     float p = 0.f;
 #pragma unroll
     for (int s = 0; s < SPL; ++s) {
       h[s] = fmaf(__builtin_amdgcn_exp2f(st * rate[s]), h[s], su * B[s]);
       p = fmaf(h[s], C[s], p);
     }
-    const float o = fmaf(skip, x, lanes_sum<LPC>(p)) * act_of(z, a.gate != nullptr);
+    const float o = fmaf(skip, x, lanes_sum<LPC>(p)) * act_of(z, gated);
     if (in && sq == 0) static_cast<T*>(a.out)[row * a.out_stride + d] = from_f32<T>(o);
     row = same.next;
     if (row < a.R) {
