@@ -1283,9 +1283,9 @@ int dwarf_selective_scan_bwd(const dwarf_selective_scan_bwd_args* args, dwarf_st
     if (!rc) rc = zero_floats(a.dskip, a.fwd.D, s, "dwarf_selective_scan_bwd");
     return rc ? rc : zero_floats(a.ddelta_bias, a.fwd.D, s, "dwarf_selective_scan_bwd");
   }
-  // the threads that add the channel tiles' rows
-  if (static_cast<double>(a.fwd.B) * a.fwd.N * a.fwd.G * 128. >= 0x1p31)
-    return fail(DWARF_ERR_UNSUPPORTED, "gradients: B * N * G must stay below 2^24");
+  // the last launch counts its threads in 32 bits: 128 for a row of B and C, 8 for each of a channel's up to 66 sums
+  if (static_cast<double>(a.fwd.B) * a.fwd.N * a.fwd.G * 128. + a.fwd.D * 528. >= 0x1p31)
+    return fail(DWARF_ERR_UNSUPPORTED, "gradients: B * N * G + 4.2 D must stay below 2^24");
   if (a.fwd.N) {
     if ((rc = check_elements("dy", a.dy, a.fwd.dtype)) || (rc = check_elements("dx", a.dx, a.fwd.dtype)) ||
         (rc = check_elements("ddelta", a.ddelta, a.fwd.dtype)) || (rc = check_elements("dB", a.dB, a.fwd.dtype)) ||

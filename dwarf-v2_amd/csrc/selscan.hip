@@ -986,38 +986,51 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
   }
 }
 
-// dB and dC: the channel tiles' partial rows in order.  One thread to (token, group, B or C, state).
+// The last launch, in two parts.  The first row_blocks workgroups add dB and dC, the channel tiles' partial rows in order, a
+// thread to (token, group, B or C, state).  The others add dA, dskip and the bias's gradient, the batches' and segments'
+// partials, in 64 bits: 32 values each, eight threads to a value, each every eighth partial in order, then the eight (by one
+// thread B1 N2048, 128 partials, took 8 us).
+constexpr int kSumCols = 32, kSumRows = 256 / kSumCols;
+struct ScanSums {
+  const float* part; const float* part_A; const float* part_d;
+  void* dB; void* dC;
+  float* dA; float* dskip; float* dbias;
+  int64_t rows;
+  int tiles, row_blocks, parts, D, SP, S;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void scan_sum_rows(const float* __restrict__ part, T* __restrict__ dB, T* __restrict__ dC,
-                                                     int64_t rows, int tiles, int SP, int S) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= rows * 2 * SP) return;
-  float x = 0.f;
+__global__ __launch_bounds__(256) void scan_sum_kernel(ScanSums a) {
+  __shared__ double s_part[kSumRows][kSumCols];
+  if (static_cast<int>(blockIdx.x) < a.row_blocks) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, each = a.rows * 2 * a.SP;
+    if (i >= each) return;
+    float x = 0.f;
 #pragma unroll 8
-  for (int k = 0; k < tiles; ++k) x += part[k * rows * 2 * SP + i];
-  const int64_t row = i / (2 * SP);
-  const int q = static_cast<int>(i - row * (2 * SP)), s = q < SP ? q : q - SP;
-  if (s < S) (q < SP ? dB : dC)[row * S + s] = from_f32<T>(x);
-}
-
-// dA, dskip, ddelta_bias: the batches' and segments' partials in order, in 64 bits.
-__global__ __launch_bounds__(256) void scan_sum_channels(const float* __restrict__ part_A, const float* __restrict__ part_d,
-                                                         float* __restrict__ dA, float* __restrict__ dskip,
-                                                         float* __restrict__ dbias, int D, int SP, int S, int parts) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, nA = static_cast<int64_t>(D) * SP;
+    for (int k = 0; k < a.tiles; ++k) x += a.part[k * each + i];
+    const int64_t row = i / (2 * a.SP);
+    const int q = static_cast<int>(i - row * (2 * a.SP)), s = q < a.SP ? q : q - a.SP;
+    if (s < a.S) static_cast<T*>(q < a.SP ? a.dB : a.dC)[row * a.S + s] = from_f32<T>(x);
+    return;
+  }
+  const int col = threadIdx.x % kSumCols, first = threadIdx.x / kSumCols;
+  const int64_t i = static_cast<int64_t>(blockIdx.x - a.row_blocks) * kSumCols + col, nA = static_cast<int64_t>(a.D) * a.SP;
+  const bool in_A = i < nA, in = i < nA + 2 * static_cast<int64_t>(a.D);
+  const int64_t q = i - nA, step = in_A ? nA : 2 * static_cast<int64_t>(a.D);
+  const float* p = in_A ? a.part_A + i : a.part_d + q;
   double x = 0.;
-  if (i < nA) {
-    const int s = static_cast<int>(i % SP);
-    if (!dA || s >= S) return;
+  if (in)
 #pragma unroll 8
-    for (int k = 0; k < parts; ++k) x += part_A[k * nA + i];
-    dA[i / SP * S + s] = static_cast<float>(x);
-  } else if (i < nA + 2 * D) {
-    const int64_t q = i - nA;
-    float* out = q < D ? dskip : dbias;
-    if (!out) return;
-    for (int k = 0; k < parts; ++k) x += part_d[k * 2 * static_cast<int64_t>(D) + q];
-    out[q % D] = static_cast<float>(x);
+    for (int k = first; k < a.parts; k += kSumRows) x += p[k * step];
+  s_part[first][col] = x;
+  __syncthreads();
+  if (first || !in) return;
+#pragma unroll
+  for (int r = 1; r < kSumRows; ++r) x += s_part[r][col];
+  const int s = static_cast<int>(i % a.SP);
+  if (in_A) {
+    if (a.dA && s < a.S) a.dA[i / a.SP * a.S + s] = static_cast<float>(x);
+  } else if (float* out = q < a.D ? a.dskip : a.dbias) {
+    out[q % a.D] = static_cast<float>(x);
   }
 }
 
@@ -1162,12 +1175,13 @@ void scan_bwd_typed(const dwarf_selective_scan_bwd_args& w, const ScanGeom& gm, 
   else
     scan_bwd_laid<T, SPL, LPC, false>(w, gm, stream);
   const int64_t rows = static_cast<int64_t>(a.B) * a.N * a.G;
-  if (rows)
-    hipLaunchKernelGGL((scan_sum_rows<T>), dim3(static_cast<unsigned>((rows * 2 * SP + 255) / 256)), dim3(256), 0, stream,
-                       gm.part, static_cast<T*>(w.dB), static_cast<T*>(w.dC), rows, gm.tiles_of_group, SP, a.S);
-  if (w.dA || w.dskip || w.ddelta_bias)
-    hipLaunchKernelGGL(scan_sum_channels, dim3(static_cast<unsigned>((static_cast<int64_t>(a.D) * (SP + 2) + 255) / 256)),
-                       dim3(256), 0, stream, gm.part_A, gm.part_d, w.dA, w.dskip, w.ddelta_bias, a.D, SP, a.S, a.B * gm.segs);
+  const int row_blocks = static_cast<int>((rows * 2 * SP + 255) / 256);
+  const int sum_blocks = w.dA || w.dskip || w.ddelta_bias
+                             ? static_cast<int>((static_cast<int64_t>(a.D) * (SP + 2) + kSumCols - 1) / kSumCols) : 0;
+  if (row_blocks + sum_blocks)
+    hipLaunchKernelGGL((scan_sum_kernel<T>), dim3(row_blocks + sum_blocks), dim3(256), 0, stream,
+                       ScanSums{gm.part, gm.part_A, gm.part_d, w.dB, w.dC, w.dA, w.dskip, w.ddelta_bias, rows,
+                                gm.tiles_of_group, row_blocks, a.B * gm.segs, a.D, SP, a.S});
 }
 
 template <typename T, int SPL, int LPC>
