@@ -60,9 +60,25 @@ template <int VEC>
 struct ConvAt {
   int d, b, strip, col;
   bool in;
-  __device__ __forceinline__ ConvAt(int D, const ConvGeom& gm, int B) {
-    col = blockIdx.x % static_cast<uint32_t>(gm.col_blocks) * kConvCols + threadIdx.x % kConvCols;
-    const int64_t s = static_cast<int64_t>(blockIdx.x / static_cast<uint32_t>(gm.col_blocks)) * kConvStrips + threadIdx.x / kConvCols;
+  // FLAT: the threads in order over a strip's vectors, then the next strip's; otherwise a workgroup is a rectangle
+  template <bool FLAT>
+  static __device__ __forceinline__ ConvAt make(int D, const ConvGeom& gm, int B) {
+    ConvAt at;
+    // neighbours, which share a strip's first rows and the lines where their vectors meet, on one L2
+    const uint32_t block = xcd_remap(blockIdx.x, gridDim.x);
+    int64_t s;
+    if constexpr (FLAT) {
+      const uint32_t i = block * kConvThreads + threadIdx.x;   // a launch has fewer than 2^31 threads
+      s = i / static_cast<uint32_t>(gm.cols);
+      at.col = i - static_cast<uint32_t>(s) * static_cast<uint32_t>(gm.cols);
+    } else {
+      at.col = block % static_cast<uint32_t>(gm.col_blocks) * kConvCols + threadIdx.x % kConvCols;
+      s = static_cast<int64_t>(block / static_cast<uint32_t>(gm.col_blocks)) * kConvStrips + threadIdx.x / kConvCols;
+    }
+    at.place(s, D, gm, B);
+    return at;
+  }
+  __device__ __forceinline__ void place(int64_t s, int D, const ConvGeom& gm, int B) {
     in = col < gm.cols && s < static_cast<int64_t>(B) * gm.strips;
     b = in ? static_cast<int>(s / gm.strips) : 0;
     strip = in ? static_cast<int>(s - static_cast<int64_t>(b) * gm.strips) : 0;
@@ -97,7 +113,7 @@ __device__ __forceinline__ void conv_input(const dwarf_causal_conv_fwd_args& a, 
 
 template <typename T, int VEC, int W>
 __global__ __launch_bounds__(kConvThreads) void conv_fwd_kernel(dwarf_causal_conv_fwd_args a, ConvGeom gm) {
-  const ConvAt<VEC> at(a.D, gm, a.B);
+  const auto at = ConvAt<VEC>::template make<true>(a.D, gm, a.B);
   if (!at.in) return;
   const int d = at.d, n = conv_length(a, at.b);
   const int t0 = at.strip * gm.strip, t1 = min(a.N, t0 + gm.strip), end = min(t1, n);
@@ -109,7 +125,12 @@ __global__ __launch_bounds__(kConvThreads) void conv_fwd_kernel(dwarf_causal_con
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) conv_input<T, VEC, W>(a, x, at.b, d, t0 - W + 1 + j, win[j + 1]);
     T raw[kConvAhead][VEC];   // rows on the way; behind the sequence's end its last one again
-    auto fetch = [&](int t, int i) { __builtin_memcpy(raw[i], x + min(t, end - 1) * a.x_stride[1], sizeof(raw[i])); };
+    const T* from = x + t0 * a.x_stride[1];   // the pointers walk: a 64-bit product a row took the backward 49.4 us, not 47.9
+    T* to = y + t0 * a.y_stride[1];
+    auto fetch = [&](int t, int i) {
+      __builtin_memcpy(raw[i], from, sizeof(raw[i]));
+      from += t + 1 < end ? a.x_stride[1] : 0;
+    };
 #pragma unroll
     for (int i = 0; i < kConvAhead; ++i) fetch(t0 + i, i);
     for (int t = t0; t < end; t += kConvAhead) {
@@ -131,7 +152,8 @@ __global__ __launch_bounds__(kConvThreads) void conv_fwd_kernel(dwarf_causal_con
           const float s = p[e] * sigmoid_f32(p[e]);
           p[e] = a.silu ? s : p[e];
         }
-        if (t + i < end) store_any<T, VEC>(y + (t + i) * a.y_stride[1], p);
+        if (t + i < end) store_any<T, VEC>(to, p);
+        to += a.y_stride[1];
       }
     }
   }
@@ -159,7 +181,7 @@ template <typename T, int VEC, int W>
 __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(dwarf_causal_conv_bwd_args w_, ConvGeom gm, float* __restrict__ part) {
   __shared__ float s_red[kConvStrips][kConvCols * VEC];
   const dwarf_causal_conv_fwd_args& a = w_.fwd;
-  const ConvAt<VEC> at(a.D, gm, a.B);
+  const auto at = ConvAt<VEC>::template make<false>(a.D, gm, a.B);
   const int d = at.d;
   float dw[W + 1][VEC];   // dbias last
 #pragma unroll
@@ -196,10 +218,13 @@ __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(dwarf_causal_con
       // tokens up to W - 1 behind the strip, whose dp its last tokens' dx need; none behind the sequence's end
       const int stop = end + W - 1;
       T rx[kConvAhead][VEC], rg[kConvAhead][VEC];
+      const T *px = x + min(t0, n - 1) * a.x_stride[1], *pg = dy + min(t0, n - 1) * w_.dy_stride[1];
+      T* pd = dx + (t0 - (W - 1)) * w_.dx_stride[1];   // dx's row of the token W - 1 in front
       auto fetch = [&](int t, int i) {   // behind the sequence's last token: that again
-        const int64_t tt = min(t, n - 1);
-        __builtin_memcpy(rx[i], x + tt * a.x_stride[1], sizeof(rx[i]));
-        __builtin_memcpy(rg[i], dy + tt * w_.dy_stride[1], sizeof(rg[i]));
+        __builtin_memcpy(rx[i], px, sizeof(rx[i]));
+        __builtin_memcpy(rg[i], pg, sizeof(rg[i]));
+        px += t + 1 < n ? a.x_stride[1] : 0;
+        pg += t + 1 < n ? w_.dy_stride[1] : 0;
       };
 #pragma unroll
       for (int i = 0; i < kConvAhead; ++i) fetch(t0 + i, i);
@@ -246,9 +271,10 @@ __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(dwarf_causal_con
 #pragma unroll
               for (int e = 0; e < VEC; ++e) v[e] += f[e];
             }
-            if (to >= 0) store_any<T, VEC>(dx + to * w_.dx_stride[1], v);
+            if (to >= 0) store_any<T, VEC>(pd, v);
             else store_any<T, VEC>(di + static_cast<int64_t>(to + W - 1) * a.D, v);
           }
+          pd += w_.dx_stride[1];
         }
       }
     }
@@ -260,7 +286,7 @@ __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(dwarf_causal_con
   if (!part) return;   // uniform
   // the workgroup's strips in order; of channels that two vectors hold the first one's threads write
   const int row = threadIdx.x / kConvCols, col = threadIdx.x % kConvCols;
-  const int64_t group = blockIdx.x / static_cast<uint32_t>(gm.col_blocks);
+  const int64_t group = xcd_remap(blockIdx.x, gridDim.x) / static_cast<uint32_t>(gm.col_blocks);
 #pragma unroll 1
   for (int j = 0; j <= W; ++j) {
     __syncthreads();
@@ -396,7 +422,8 @@ int64_t conv_groups(const dwarf_causal_conv_fwd_args& a, const ConvGeom& gm) {
 template <typename T, int VEC, int W>
 void conv_fwd_typed(const dwarf_causal_conv_fwd_args& a, hipStream_t stream) {
   const ConvGeom gm = conv_geom(a, VEC);
-  hipLaunchKernelGGL((conv_fwd_kernel<T, VEC, W>), dim3(static_cast<unsigned>(conv_groups(a, gm) * gm.col_blocks)),
+  const int64_t threads = static_cast<int64_t>(a.B) * gm.strips * gm.cols;
+  hipLaunchKernelGGL((conv_fwd_kernel<T, VEC, W>), dim3(static_cast<unsigned>((threads + kConvThreads - 1) / kConvThreads)),
                      dim3(kConvThreads), 0, stream, a, gm);
 }
 template <typename T, int VEC, int W>
