@@ -3,20 +3,28 @@
 //   p_t = bias + sum_j w_j x_{t-W+1+j},   y_t = p_t or silu(p_t)
 //   dp = dy silu'(p),  dx_t = sum_j w_j dp_{t+W-1-j},  dw_j = sum dp_t x_{t-W+1+j},  dbias = sum dp
 //
-// Bound by memory.  A thread takes VEC adjacent channels (forward 16 bytes of
+// Forward bound by memory, backward by memory and the vector units (69% of their
+// cycles) together.  B15 N2048, 1,024 channels in bf16, W 4, inputs from memory:
+// forward 33.5 us (126 MB, 3.8 TB/s), backward 53 (189 MB, 3.6 TB/s), the sums
+// 4; from the last-level cache 26 and 48.  B20 of 1,031 channels in fp16, W 3:
+// 37 us (169 MB, 4.6 TB/s).
+//
+// A thread takes VEC adjacent channels (forward 16 bytes of
 // them, backward four: with eight, 148 registers left too few waves, 86 us
 // where four take 54) and walks a strip of tokens with the last W - 1 inputs in
-// registers, four rows on their way: each input is loaded once but for the
-// W - 1 rows in front of a strip, which another strip's thread loads at about
-// the same time.  Rows need no alignment but their elements':
-// gfx950 loads 16 bytes from any address, and a width that VEC does not divide
-// has its last vector moved back to the row's end, where two threads then store
-// the same values.  The backward forms p again from x, which it needs for dw
-// anyway, instead of reading a saved one; a strip goes W - 1 tokens further to
-// have the dp that its own dx need.  dw and dbias: a thread's sums over its
-// strip in registers, a workgroup's over its strips in LDS, then one partial
-// row for each workgroup and a last launch that adds those in order, in 64
-// bits.
+// registers, four rows on their way (two to eight: the same within 4%): each
+// input is loaded once but for the W - 1 rows in front of a strip, which another
+// strip's thread loads at about the same time, from the same L2.  Forward the
+// threads go over whole rows in order (in rectangles of 32 vectors, as the
+// backward's sums have it, the 1,031 channels took 43 us).  Rows need no
+// alignment but their elements': gfx950 loads 16 bytes from any address, and a
+// width that VEC does not divide has its last vector moved back to the row's
+// end, where two threads then store the same values.  The backward forms p
+// again from x, which it needs for dw anyway, instead of reading a saved one; a
+// strip goes W - 1 tokens further to have the dp that its own dx need.  dw and
+// dbias: a thread's sums over its strip in registers, a workgroup's over its
+// strips in LDS, then one partial row for each workgroup and a last launch that
+// adds those in order, in 64 bits.
 #include "selective.h"
 
 namespace dwarf {
@@ -338,7 +346,7 @@ __global__ __launch_bounds__(kConvSumCols * kConvSumRows) void conv_sum_kernel(c
   }
 }
 
-// One token of each row.  The first row of a slot takes the slot's later rows after it, in order.
+// One token of each row, bound by the launch (256 rows of 1,024 channels: 4.8 us, one row 2.9).  The first row of a slot takes the slot's later rows after it, in order.
 template <typename T, int VEC, int W>
 __global__ __launch_bounds__(kConvThreads) void conv_step_kernel(dwarf_causal_conv_step_args a, int col_blocks) {
   __shared__ int s_found[2];
@@ -408,8 +416,8 @@ ConvGeom conv_geom(const dwarf_causal_conv_fwd_args& a, int vec) {
   gm.cols = (a.D + vec - 1) / vec;
   gm.col_blocks = (gm.cols + kConvCols - 1) / kConvCols;
   // Strips of 16 to 64 tokens, as long as leave seven workgroups for each four CUs: a thread reads W - 1 rows in front of its
-  // strip and its weights once more for each (B15 N2048, 1,024 channels in bf16: strips of 16 tokens 29.5 us forward and
-  // 55 backward, of 32 27.0 and 51).
+  // strip and its weights once more for each (B15 N2048, 1,024 channels in bf16: forward strips of 16 tokens take 41 us, of 32
+  // 34, of 64 36; backward of 16 58, of 64 53).
   gm.strip = 16;
   while (gm.strip < 64 && static_cast<int64_t>(a.B) * a.N / (2 * gm.strip) / kConvStrips * gm.col_blocks >= 448) gm.strip *= 2;
   gm.strips = a.N > 0 ? (a.N + gm.strip - 1) / gm.strip : 1;
