@@ -345,3 +345,47 @@ def test_pools_count_as_written(pkg, device):
         pkg.selective_scan_step(rows, delta, p["A"], B, C, pool)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_results_past_32_bits(pkg, device):
+    """Results of more than 2^31 elements: one token over and over, whose rows and gradients are the same once the state has
+    settled (a decay of e^-8 forgets the way there)."""
+    N, D = (1 << 21) + 77, 1040
+    g = torch.Generator().manual_seed(11)
+    row, up = (randn(g, 1, 1, D, dtype=torch.bfloat16).to(device) for _ in range(2))
+    x, dy = row.expand(1, N, D), up.expand(1, N, D)
+    y, _ = pkg.rms_norm(x, residual=x)
+    assert torch.equal(y[:, -1], y[:, 0])
+    q, scale = pkg.rms_norm_fp8(x)
+    assert torch.equal(q[:, -1].float(), q[:, 0].float()) and torch.equal(scale[:, -1], scale[:, 0])
+    del y, q, scale
+    leaf = x.detach().requires_grad_(True)
+    y = pkg.causal_conv(leaf, randn(g, D, 4).to(device), activation="silu")
+    dx, = torch.autograd.grad(y, leaf, dy)
+    assert torch.equal(y[:, -1], y[:, 100]) and torch.equal(dx[:, -5], dx[:, 100])
+    del y, dx
+    one = torch.ones(1, 1, 1, dtype=torch.bfloat16, device=device).expand(1, N, 1)
+    y, state = pkg.selective_scan(leaf, one.expand(1, N, D), torch.full((D, 1), -8.0, device=device), one, one, return_state=True)
+    dx, = torch.autograd.grad(y, leaf, dy)
+    assert torch.equal(y[:, -1], y[:, 100]) and torch.equal(state[0, :, 0].bfloat16(), y[0, -1])
+    assert torch.equal(dx[:, -100], dx[:, 100])
+
+
+def test_inputs_changed_before_the_backward_are_noticed(pkg, device):
+    p, _ = traced_case(device)
+    for change_rows in (True, False):
+        t, lengths = leaves_of(p), torch.tensor([70, 3], dtype=torch.int32, device=device)
+        rows = t["x"][..., :D] * 1
+        y = pkg.causal_conv(rows, t["wc"], lengths=lengths)
+        (rows if change_rows else lengths).add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
+def test_compiled_norm_with_one_type(pkg, device):
+    """One gradient serves x and the residual in an eager call; a compiled one has two."""
+    x, r = (torch.randn(5, 64, device=device).bfloat16().requires_grad_(True) for _ in range(2))
+    up = [torch.randn(5, 64, device=device).bfloat16() for _ in range(2)]
+    want = torch.autograd.grad(pkg.rms_norm(x, residual=r), [x, r], up)
+    out = torch.compile(lambda x, r: pkg.rms_norm(x, residual=r), backend="aot_eager", fullgraph=True)(x, r)
+    same(torch.autograd.grad(out, [x, r], up), want)
