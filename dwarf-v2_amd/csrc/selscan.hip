@@ -45,13 +45,18 @@ namespace dwarf {
 namespace {
 
 constexpr int kScanWaves = 4, kScanThreads = kScanWaves * kWave;
-constexpr int kTile = 32;           // tokens of B and C in LDS at a time, forward
+constexpr int kTile = 32;           // tokens in LDS at a time, forward
 constexpr int kMaxSegments = 64;
 constexpr int kSegmentUnit = 32, kSegmentLeast = 64;   // tokens a segment is a multiple of, and has at least
 
 // States per lane and lanes per channel for S states.
 constexpr int scan_spl(int S) { return S <= 8 ? 2 : S <= 16 ? 4 : 8; }
 constexpr int scan_lpc(int S) { return S <= 32 ? 4 : 8; }
+// Tokens of the rows' tiles forward: twice as many where two workgroups still share a CU's LDS with them (a tile's barrier and
+// the waits behind it take 3% of the time in 64 tokens, 6 in 32: B15 N2048, 1,024 channels of 16 states in bf16 205 us, not 211;
+// the segments' sums have too many registers for it: 340 us, not 260, for B1 N65536).
+template <typename T, int SP, bool WIDE>
+constexpr int scan_rows_tile() { return WIDE && sizeof(T) == 2 && SP <= 16 ? 2 * kTile : kTile; }
 // Tokens of a backward chunk, whose states and decays a lane keeps: 64 of each.
 constexpr int scan_chunk(int spl) { return 64 / spl; }
 
@@ -466,12 +471,12 @@ __device__ __forceinline__ float joined(float h, float sum, float rate, float ad
 // LOCAL: what a segment adds from zero and its sum of steps, for all segments but the last; otherwise the rows.
 template <typename T, int SPL, int LPC, bool WIDE, bool LOCAL>
 __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void scan_fwd_kernel(dwarf_selective_scan_fwd_args a, ScanGeom gm) {
-  constexpr int SP = SPL * LPC, kQuads = kTile / 4, kK = scan_chunk(SPL);
-  __shared__ __align__(16) float s_b[2][kTile * SP];
-  __shared__ __align__(16) float s_c[LOCAL ? 1 : 2][LOCAL ? 4 : kTile * SP];
+  constexpr int SP = SPL * LPC, kTok = LOCAL ? kTile : scan_rows_tile<T, SP, WIDE>(), kQuads = kTok / 4, kK = scan_chunk(SPL);
+  __shared__ __align__(16) float s_b[2][kTok * SP];
+  __shared__ __align__(16) float s_c[LOCAL ? 1 : 2][LOCAL ? 4 : kTok * SP];
   constexpr int kIns = LOCAL ? 2 : 3;
-  __shared__ __align__(16) T s_in[2 * ScanIn<T, kTile, LPC, kIns, WIDE>::kSpan];
-  __shared__ __align__(16) T s_out[LOCAL ? 8 : 2 * ScanOut<T, kTile, LPC, 1, WIDE>::kSpan];
+  __shared__ __align__(16) T s_in[2 * ScanIn<T, kTok, LPC, kIns, WIDE>::kSpan];
+  __shared__ __align__(16) T s_out[LOCAL ? 8 : 2 * ScanOut<T, kTok, LPC, 1, WIDE>::kSpan];
   const ScanLane<LPC> at(a, gm, LOCAL ? gm.segs - 1 : gm.segs);
   const int s0 = at.sq * SPL, quad = at.lane & 3;
   const int64_t d = at.d;
@@ -499,10 +504,10 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
   const ScanRows ins[3] = {{a.x, at.b * a.x_stride[0], a.x_stride[1]}, {a.delta, at.b * a.delta_stride[0], a.delta_stride[1]},
                            {gated ? a.gate : nullptr, at.b * a.gate_stride[0], a.gate_stride[1]}};
   const ScanRows outs[1] = {{a.y, at.b * a.y_stride[0], a.y_stride[1]}};
-  ScanIn<T, kTile, LPC, kIns, WIDE> in(ins, at, a.D, t0, s_in);
-  ScanOut<T, kTile, LPC, 1, WIDE> out(outs, at, a.D, t0, s_out);
-  BcRows<T, SP, kTile> rb(static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2], a.B_stride[1], t0, a.S);
-  BcRows<T, SP, kTile> rc(static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2], a.C_stride[1], t0, a.S);
+  ScanIn<T, kTok, LPC, kIns, WIDE> in(ins, at, a.D, t0, s_in);
+  ScanOut<T, kTok, LPC, 1, WIDE> out(outs, at, a.D, t0, s_out);
+  BcRows<T, SP, kTok> rb(static_cast<const T*>(a.Bm) + at.b * a.B_stride[0] + at.g * a.B_stride[2], a.B_stride[1], t0, a.S);
+  BcRows<T, SP, kTok> rc(static_cast<const T*>(a.Cm) + at.b * a.C_stride[0] + at.g * a.C_stride[2], a.C_stride[1], t0, a.S);
   float* ck = !LOCAL && a.checkpoints && at.in
                   ? a.checkpoints + ((static_cast<int64_t>(at.b) * ((a.N + kK - 1) / kK) + t0 / kK) * a.D + d) * SP + s0 : nullptr;
   const int64_t ck_step = static_cast<int64_t>(a.D) * SP;
@@ -522,13 +527,13 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
     fetch(end - t0);
     take(0, end - t0);
     __syncthreads();
-    for (int t = t0; t < end; t += kTile, buf ^= 1) {
-      const bool more = t + kTile < end;
+    for (int t = t0; t < end; t += kTok, buf ^= 1) {
+      const bool more = t + kTok < end;
       if (more) {   // under way while this tile is worked on
         rb.move(1);
         rc.move(1);
         in.move(1);
-        fetch(end - t - kTile);
+        fetch(end - t - kTok);
       }
       // A quad at a time; the next one's rows and steps are formed meanwhile, from values read one quad earlier yet: the compiler
       // waits where it reads.
@@ -585,12 +590,12 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
       }
       if constexpr (WIDE && !LOCAL)
         if (t > t0) {
-          out.send(kTile);
+          out.send(kTok);
           out.move(1);
         }
       // The next tile's values are waited for in front of this one's stores: loads and stores are counted together, and
       // waiting behind them would wait for the stores too (an eighth of the time).
-      if (more) take(buf ^ 1, end - t - kTile);
+      if (more) take(buf ^ 1, end - t - kTok);
       __syncthreads();   // one barrier a tile: what it lets through writes the other buffers
       if constexpr (!WIDE && !LOCAL) {
         out.flush(end - t, at);
@@ -599,7 +604,7 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
     }
     if constexpr (WIDE && !LOCAL) {
       out.collect(buf ^ 1);
-      out.send(end - t0 - (end - t0 - 1) / kTile * kTile);
+      out.send(end - t0 - (end - t0 - 1) / kTok * kTok);
     }
   }
   if constexpr (LOCAL) {
