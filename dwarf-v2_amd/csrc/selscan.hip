@@ -9,10 +9,10 @@
 // Nothing here is a product of matrices: each (token, channel, state) has a
 // decay of its own, one exponential and four multiply-adds forward, 13 backward,
 // and that, not memory, bounds the kernels.  At B15 N2048, 1,024 channels of 16
-// states in bf16 (503 million of them): forward 211 us, 252 MB of rows and 126
+// states in bf16 (503 million of them): forward 205 us, 252 MB of rows and 126
 // MB of checkpoints; backward 540 us; the vector units issue in 70 and 76% of
-// the waves' cycles, a quarter to a third more instructions than those above
-// (84 and 210 us at an instruction every 4 cycles, 8 for the exponential).  So
+// the waves' cycles, and of those 62 and 55% are the operations above (84 and
+// 210 us at an instruction every 4 cycles, 8 for the exponential).  So
 // the work is laid out for the vector units: LPC adjacent lanes share a channel,
 // SPL states in the registers of each, and a wave holds 64 / LPC channels.  The
 // quads of lanes divide what a channel has once for each token (softplus, silu,
@@ -27,14 +27,15 @@
 // else it is cut into segments, which a launch in front reduces to the state
 // that each adds from zero and the sum of its steps (a segment's decay is
 // exp(A sum)); the rows' workgroups join the segments in front of their own
-// themselves (B1 N65536, 1,024 channels: 32 segments, 259 and 355 us).  The
+// themselves (B1 N65536, 1,024 channels: 32 segments, 260 and 351 us).  The
 // backward does the same with the adjoint, from the end.
 //
 // The backward walks chunks from the last to the first: it forms a chunk's
 // states again from the checkpoint the forward left in front of it, keeps them
 // and the decays in registers and walks back through them.  dB and dC are sums
-// over channels: over a wave's by lane exchanges, over a workgroup's waves in
-// LDS, over workgroups by partial rows that a last launch adds in order (12 us).
+// over channels: over a wave's by lane exchanges (by fp32 matrix instructions
+// the kernel took 744 us), over a workgroup's waves in LDS, over workgroups by
+// partial rows that a last launch adds in order (12 us).
 // Nothing is atomic: the same bits every time.  dA, dskip and the bias's
 // gradient, sums over all tokens, run in 64 bits from a chunk on.
 #include <utility>
