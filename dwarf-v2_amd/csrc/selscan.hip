@@ -956,7 +956,10 @@ __global__ __launch_bounds__(kScanThreads) __attribute__((amdgpu_waves_per_eu(1,
         const float gB = quad_sums<LPC>(into[0], into[1], into[2], into[3], at.lane);
         const float gA = quad_sums<LPC>(mA[0], mA[1], mA[2], mA[3], at.lane) * (1.f / kLog2e);
         const float scanned = fmaf(skip, u[k], quad_sums<LPC>(o[0], o[1], o[2], o[3], at.lane)), e = sigmoid_f32(z[k]);
-        const float dd = fmaf(u[k], gB, gA) * slope[k];
+        // Chosen, not multiplied by a slope of 0: a token without a step passes its state on, whose share in the step's gradient
+        // is out of range where a rate is minus infinity.  (A delta that is not a number has a slope of 0 too, but no step of 0.)
+        const bool still = st[k] == 0.f && slope[k] == 0.f;
+        const float dd = still ? 0.f : fmaf(u[k], gB, gA) * slope[k];
         cskip = fmaf(go[k], u[k], cskip);
         cbias += dd;
 #pragma unroll

@@ -208,6 +208,45 @@ def test_layouts_give_the_same_bits(pkg, device):
 
             def results(change):
                 d = {k: change(v.detach()).requires_grad_(True) if k in leaves_of(c) else v for k, v in c.items()}
+@pytest.mark.parametrize("S,D", [(8, 16), (16, 24), (5, 13), (40, 8)])
+@pytest.mark.parametrize("softplus", [False, True])
+def test_gradients_of_states_that_do_not_last(pkg, device, softplus, S, D):
+    """A of minus infinity beside every input, sequences that end inside a chunk, steps of 0 and large gradients of the state:
+    m = dstate h of a token whose step is 0 times a rate of -3.4e38 is out of range, and the token's part in the gradients of
+    its step and of the bias is still 0.  All are finite and those of a rate of -1e30."""
+    c = case(device, 4, 100, D, S, torch.float32, softplus=softplus, lengths=[100, 37, 64, 0])
+    c["dstate"] = 1e3 * c["dstate"]
+    if softplus:   # a step of 0; without the softplus only tokens behind the end have one
+        masked = torch.arange(100, device=device) % 7 == 3
+        c["delta"] = c["delta"].detach().masked_fill(masked[None, :, None], -float("inf")).requires_grad_(True)
+    results = []
+    for low in (-float("inf"), -1e30):
+        A = c["A"].detach().clone()
+        A[:, S // 2] = low
+        d = dict(c, A=A.requires_grad_(True))
+        out = call(pkg, d)
+        results.append([*out, *torch.autograd.grad(out, [d[k] for k in leaves_of(d)], [c["dy"], c["dstate"]])])
+    for k, s, t in zip(("y", "state", *leaves_of(c)), *results):
+        assert bool(s.isfinite().all()) and torch.equal(s, t), k
+
+
+@pytest.mark.parametrize("softplus", [False, True])
+def test_steps_that_are_not_numbers_show_in_every_gradient(pkg, device, softplus):
+    """A NaN among the steps reaches the outputs behind it and its channel's gradients; other channels' rows are untouched."""
+    c = case(device, 1, 60, 24, 16, torch.float32, softplus=softplus)
+    bad = c["delta"].detach().clone()
+    bad[0, 40, 5] = float("nan")
+    got = call(pkg, dict(c, delta=bad))
+    d = dict(c, delta=bad.requires_grad_(True))
+    names = ("x", "delta", "A", "delta_bias", "initial")
+    grads = dict(zip(names, torch.autograd.grad(call(pkg, d), [d[k] for k in names], [c["dy"], c["dstate"]])))
+    assert bool(got[0][0, 40:, 5].isnan().all()) and bool(got[0][0, :40].isfinite().all()) and bool(got[0][0, :, 6:].isfinite().all())
+    assert bool(grads["x"][0, :41, 5].isnan().all()) and bool(grads["delta"][0, :41, 5].isnan().all())
+    assert bool(grads["A"][5].isnan().all()) and bool(grads["delta_bias"][5].isnan()) and bool(grads["initial"][0, 5].isnan().all())
+    other = torch.arange(24, device=device) != 5
+    assert all(bool(grads[k][..., other].isfinite().all()) for k in ("x", "delta", "delta_bias"))
+
+
                 out = call(pkg, d)
                 return [*out, *torch.autograd.grad(out, [d[k] for k in leaves_of(c)], [change(c["dy"]), change(c["dstate"])])]
 
