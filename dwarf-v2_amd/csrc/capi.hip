@@ -1247,6 +1247,14 @@ size_t dwarf_selective_scan_fwd_workspace_bytes(const dwarf_selective_scan_fwd_a
   return scan_sized(a) ? dwarf::selective_scan_fwd_workspace(*a) : 0;
 }
 
+// The backward's last launch counts its threads in 32 bits: 128 for a row of B and C, 8 for each of a channel's up to 66 sums.
+// The forward refuses such a call too where it is asked for checkpoints: they are for a backward that would refuse them.
+static int check_scan_gradients(const dwarf_selective_scan_fwd_args& a) {
+  if (static_cast<double>(a.B) * a.N * a.G * 128. + a.D * 528. >= 0x1p31)
+    return fail(DWARF_ERR_UNSUPPORTED, "gradients: B * N * G + 4.2 D must stay below 2^24");
+  return DWARF_OK;
+}
+
 static int check_checkpoints(const dwarf_selective_scan_fwd_args& a) {
   const size_t need = dwarf::selective_scan_checkpoints(a);
   if (need && (!a.checkpoints || a.checkpoint_bytes < need || !aligned16(a.checkpoints)))
@@ -1260,7 +1268,7 @@ int dwarf_selective_scan_fwd(const dwarf_selective_scan_fwd_args* args, dwarf_st
   int rc = check_scan(a);
   if (rc || a.B == 0) return rc ? rc : ok();
   if (a.N && ((rc = check_elements("y", a.y, a.dtype)) || (rc = check_token_stride("y", a.y_stride[1])))) return rc;
-  if (a.checkpoints && (rc = check_checkpoints(a))) return rc;
+  if (a.checkpoints && ((rc = check_scan_gradients(a)) || (rc = check_checkpoints(a)))) return rc;
   if (a.N == 0 && !a.final) return ok();
   const size_t need = dwarf::selective_scan_fwd_workspace(a);
   if (need && (!a.workspace || a.workspace_bytes < need || !aligned16(a.workspace)))
@@ -1283,9 +1291,7 @@ int dwarf_selective_scan_bwd(const dwarf_selective_scan_bwd_args* args, dwarf_st
     if (!rc) rc = zero_floats(a.dskip, a.fwd.D, s, "dwarf_selective_scan_bwd");
     return rc ? rc : zero_floats(a.ddelta_bias, a.fwd.D, s, "dwarf_selective_scan_bwd");
   }
-  // the last launch counts its threads in 32 bits: 128 for a row of B and C, 8 for each of a channel's up to 66 sums
-  if (static_cast<double>(a.fwd.B) * a.fwd.N * a.fwd.G * 128. + a.fwd.D * 528. >= 0x1p31)
-    return fail(DWARF_ERR_UNSUPPORTED, "gradients: B * N * G + 4.2 D must stay below 2^24");
+  if ((rc = check_scan_gradients(a.fwd))) return rc;
   if (a.fwd.N) {
     if ((rc = check_elements("dy", a.dy, a.fwd.dtype)) || (rc = check_elements("dx", a.dx, a.fwd.dtype)) ||
         (rc = check_elements("ddelta", a.ddelta, a.fwd.dtype)) || (rc = check_elements("dB", a.dB, a.fwd.dtype)) ||

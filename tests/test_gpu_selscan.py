@@ -371,6 +371,16 @@ def test_steps(pkg, device, D, S, G, dtype, across):
 
 @pytest.mark.parametrize("D,S", [(40, 16), (13, 5)])
 def test_rows_of_one_slot_are_tokens_in_order(pkg, device, D, S):
+def test_gradients_that_cannot_be_formed_are_refused_in_front(pkg, device):
+    """B N G of 2^24: the call with gradients is refused before its forward runs, the one without them runs."""
+    x = torch.full((1, 1, 16), 0.5, device=device).expand(1, 1 << 20, 16)
+    A = -torch.ones(16, 1, device=device)
+    rows = x[..., None]
+    assert bool((pkg.selective_scan(x, x, A, rows, rows) > 0).all())
+    with pytest.raises(pkg._lib.NativeLibraryError, match="gradients"):
+        pkg.selective_scan(x, x, A.requires_grad_(True), rows, rows)
+
+
     c = case(device, 1, 9, D, S, torch.bfloat16)
     rows = {k: c[k].detach()[0] for k in ("x", "delta", "gate", "B", "C")}
     slots = torch.tensor([2, 0, 2, -1, 2, 1, 0, 2, 4], dtype=torch.int32, device=device)

@@ -178,6 +178,18 @@ def test_selective_scan_entry_points_refuse(pkg, lib):
         ("R", 0, L.DWARF_OK)])
 
 
+def test_checkpoints_of_gradients_that_cannot_be_formed_are_refused(pkg, lib):
+    """The forward refuses what the backward would: before it has run, where it is asked for checkpoints."""
+    L = pkg._lib
+    a = scan_args(L)
+    f = a.fwd
+    f.B, f.N = 1 << 10, 1 << 14
+    f.checkpoints, f.checkpoint_bytes = P, lib.dwarf_selective_scan_checkpoint_bytes(ctypes.byref(f))
+    for fn, args in ((lib.dwarf_selective_scan_fwd, f), (lib.dwarf_selective_scan_bwd, a)):
+        assert fn(ctypes.byref(args), None) == L.DWARF_ERR_UNSUPPORTED
+        assert b"gradients" in lib.dwarf_last_error()
+
+
 @pytest.mark.parametrize("S", [1, 8, 9, 16, 17, 32, 33, 64])
 @pytest.mark.parametrize("N", [1, 7, 8, 33, 257])
 def test_checkpoint_sizes_agree(pkg, lib, N, S):
