@@ -1140,7 +1140,8 @@ int dwarf_causal_conv_fwd(const dwarf_causal_conv_fwd_args* args, dwarf_stream_t
 }
 
 size_t dwarf_causal_conv_bwd_workspace_bytes(const dwarf_causal_conv_bwd_args* a) {
-  return a && a->fwd.B > 0 && a->fwd.N >= 0 && a->fwd.D > 0 && a->fwd.W > 0 && mixer_dtype(a->fwd.dtype)
+  return a && a->fwd.B > 0 && a->fwd.N >= 0 && a->fwd.N <= (1 << 24) && a->fwd.D > 0 && a->fwd.D <= (1 << 24) && a->fwd.W > 0 &&
+                 a->fwd.W <= 8 && mixer_dtype(a->fwd.dtype)
              ? dwarf::causal_conv_bwd_workspace(*a) : 0;
 }
 
@@ -1237,8 +1238,9 @@ static int check_scan(const dwarf_selective_scan_fwd_args& a) {
   return DWARF_OK;
 }
 
+// Sizes of calls that are not refused for theirs.
 static bool scan_sized(const dwarf_selective_scan_fwd_args* a) {
-  return a && a->B > 0 && a->N >= 0 && check_scan_sizes(a->D, a->G, a->S, a->dtype) == DWARF_OK;
+  return a && a->B > 0 && a->N >= 0 && a->N <= (1 << 24) && check_scan_sizes(a->D, a->G, a->S, a->dtype) == DWARF_OK;
 }
 size_t dwarf_selective_scan_checkpoint_bytes(const dwarf_selective_scan_fwd_args* a) {
   return scan_sized(a) ? dwarf::selective_scan_checkpoints(*a) : 0;

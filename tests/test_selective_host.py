@@ -199,6 +199,19 @@ def test_checkpoint_sizes_agree(pkg, lib, N, S):
     assert 4 * pkg.selscan.checkpoint_elements(2, N, 64, S) == lib.dwarf_selective_scan_checkpoint_bytes(ctypes.byref(f))
 
 
+@pytest.mark.parametrize("N", [(1 << 24) + 1, (1 << 31) - 1])
+def test_sizes_of_refused_calls_are_zero(pkg, lib, N):
+    """Token counts that the calls refuse, to the last that an int holds: no sizes are computed for them."""
+    a = scan_args(pkg._lib)
+    a.fwd.N = N
+    f, b = ctypes.byref(a.fwd), ctypes.byref(a)
+    assert lib.dwarf_selective_scan_checkpoint_bytes(f) == lib.dwarf_selective_scan_fwd_workspace_bytes(f) == 0
+    assert lib.dwarf_selective_scan_bwd_workspace_bytes(b) == 0
+    c = pkg._lib.CausalConvBwdArgs()
+    c.fwd.B, c.fwd.N, c.fwd.D, c.fwd.W, c.fwd.dtype, c.dweight = 2, N, 64, 4, pkg._lib.DWARF_BF16, P
+    assert lib.dwarf_causal_conv_bwd_workspace_bytes(ctypes.byref(c)) == 0
+
+
 def t(*shape, dtype=torch.bfloat16):
     return torch.zeros(shape, dtype=dtype)
 
