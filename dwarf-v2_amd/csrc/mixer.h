@@ -22,9 +22,10 @@ __device__ __forceinline__ f16 from_f32<f16>(float x) { return static_cast<f16>(
 template <>
 __device__ __forceinline__ float from_f32<float>(float x) { return x; }
 
-// VEC consecutive elements as one access: the whole vector is aligned to its size (16 bytes at most).
+// VEC consecutive elements as one access: the whole vector is aligned to its size, and to 16 bytes where it is longer (eight fp32
+// of a stream beside rows of 16 bits).
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Vec {
+struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Vec {
   T e[VEC];
 };
 template <typename T, int VEC>

@@ -18,6 +18,8 @@
 namespace dwarf {
 namespace {
 
+static_assert(alignof(Vec<float, 8>) == 16, "norm_vec_ok checks a stream's rows for 16 bytes");
+
 __device__ __forceinline__ float max2(float a, float b) { return a > b ? a : b; }
 
 template <int LANES>
