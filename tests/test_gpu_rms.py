@@ -182,6 +182,27 @@ def test_layouts_give_the_same_bits(pkg, device):
     assert torch.equal(pkg.rms_norm(x), pkg.rms_norm(x.contiguous()))
 
 
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=str)
+@pytest.mark.parametrize("D", [64, 512, 2048, 16384])
+def test_fp32_streams_at_16_bytes(pkg, device, dtype, D):
+    """A stream and its gradient at addresses that 16 divides and 32 does not, as all their rows or as every other one: the
+    bits of aligned ones, forward and backward."""
+    g = torch.Generator().manual_seed(D)
+    x, dy, r, ds = (randn(g, 6, D, dtype=t).to(device) for t in (dtype, dtype, torch.float32, torch.float32))
+    w = randn(g, D).to(device)
+    want = [*pkg.rms_norm(x, w, residual=r), *(t.view(torch.uint8) if t.element_size() == 1 else t for t in pkg.rms_norm_fp8(x, w, residual=r))]
+    back = pkg.norm.rms_backward(dy, ds, r, w, 1, 1e-5, True, True, True)
+    for between, start in ((0, 4), (4, 0), (4, 4)):
+        def moved(t):
+            return torch.empty(6 * (D + between) + start, device=device)[start:].view(6, D + between)[:, :D].copy_(t)
+        a, b = moved(r), moved(ds)
+        assert a.data_ptr() % 32 == 4 * start and (a.stride(0) * 4) % 32 == 4 * between
+        got = [*pkg.rms_norm(x, w, residual=a), *(t.view(torch.uint8) if t.element_size() == 1 else t for t in pkg.rms_norm_fp8(x, w, residual=a))]
+        assert all(torch.equal(s, t) for s, t in zip(got, want))
+        got = pkg.norm.rms_backward(dy, b, a, w, 1, 1e-5, True, True, True)
+        assert all(torch.equal(s, t) for s, t in zip(got, back))
+
+
 def test_empty_inputs(pkg, device):
     x = torch.empty(0, 64, device=device, requires_grad=True)
     w = torch.ones(64, device=device, requires_grad=True)
@@ -222,27 +243,6 @@ def test_differences(pkg, device):
 def test_far_rows(pkg, device):
     """Rows whose offsets pass 2^31 elements."""
     buf = torch.empty((1 << 31) + 4096, dtype=torch.bfloat16, device=device)
-@pytest.mark.parametrize("dtype", DTYPES[:2], ids=str)
-@pytest.mark.parametrize("D", [64, 512, 2048, 16384])
-def test_fp32_streams_at_16_bytes(pkg, device, dtype, D):
-    """A stream and its gradient at addresses that 16 divides and 32 does not, as all their rows or as every other one: the
-    bits of aligned ones, forward and backward."""
-    g = torch.Generator().manual_seed(D)
-    x, dy, r, ds = (randn(g, 6, D, dtype=t).to(device) for t in (dtype, dtype, torch.float32, torch.float32))
-    w = randn(g, D).to(device)
-    want = [*pkg.rms_norm(x, w, residual=r), *(t.view(torch.uint8) if t.element_size() == 1 else t for t in pkg.rms_norm_fp8(x, w, residual=r))]
-    back = pkg.norm.rms_backward(dy, ds, r, w, 1, 1e-5, True, True, True)
-    for between, start in ((0, 4), (4, 0), (4, 4)):
-        def moved(t):
-            return torch.empty(6 * (D + between) + start, device=device)[start:].view(6, D + between)[:, :D].copy_(t)
-        a, b = moved(r), moved(ds)
-        assert a.data_ptr() % 32 == 4 * start and (a.stride(0) * 4) % 32 == 4 * between
-        got = [*pkg.rms_norm(x, w, residual=a), *(t.view(torch.uint8) if t.element_size() == 1 else t for t in pkg.rms_norm_fp8(x, w, residual=a))]
-        assert all(torch.equal(s, t) for s, t in zip(got, want))
-        got = pkg.norm.rms_backward(dy, b, a, w, 1, 1e-5, True, True, True)
-        assert all(torch.equal(s, t) for s, t in zip(got, back))
-
-
     x = buf.as_strided((3, 256), ((1 << 30), 1)).normal_()
     assert torch.equal(pkg.rms_norm(x), pkg.rms_norm(x.clone()))
 

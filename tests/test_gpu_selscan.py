@@ -170,44 +170,6 @@ def test_states_that_do_not_last(pkg, device):
         assert all(torch.equal(s, t) and bool(s.isfinite().all()) for s, t in zip(*results))
 
 
-def test_growing_states_after_a_start_of_zeros(pkg, device):
-    """A above 0 whose growth over a segment is beyond fp32: where nothing has entered yet nothing is multiplied."""
-    c = case(device, 1, 200, 8, 4, torch.float32, parts=(), softplus=False)
-    with torch.no_grad():
-        c["A"].fill_(30.0)
-        c["delta"].fill_(0.2)
-        c["x"][:, :190] = 0
-        y, state = call(pkg, c)
-    assert segment_tokens(1, 200, 8, 1, 4)[1] and not bool(y[:, :190].any()) and bool(y.isfinite().all()) and bool(state.isfinite().all())
-
-
-def test_steps_of_any_size(pkg, device):
-    """delta from far below to far above: softplus against float64, through a scan of one token."""
-    raw = torch.cat((torch.linspace(-30, 30, 4001), torch.tensor([-87.0, -100.0, -1e4, 1e4, 60.0])))
-    D = raw.numel()
-    one = torch.ones(1, 1, 1)
-    y = pkg.selective_scan(torch.ones(1, 1, D, device=device), raw.view(1, 1, D).to(device), -torch.ones(D, 1, device=device),
-                           one.to(device), one.to(device), softplus=True)[0, 0].double().cpu()
-    want = torch.log1p(torch.exp(-raw.double().abs())) + raw.double().clamp(min=0)
-    assert bool(((y - want).abs() <= want * 8 * U + 1.2e-38).all())
-
-
-def same(a, b):
-    assert len(a) == len(b) and all(torch.equal(s, t) for s, t in zip(a, b))
-
-
-def test_layouts_give_the_same_bits(pkg, device):
-    """Strided, expanded, misaligned inputs and gradients against contiguous ones."""
-    odd = lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device=device)[1:].view(t.shape).copy_(t)   # noqa: E731
-    apart = lambda t: torch.stack((t, t), -1)[..., 0]                                                     # noqa: E731
-    wide = lambda t: torch.cat((t, t, t), -1)[..., t.shape[-1]:2 * t.shape[-1]]                            # noqa: E731
-    turned = lambda t: t if t.ndim < 2 else t.transpose(0, 1).contiguous().transpose(0, 1)                # noqa: E731
-    for dtype in DTYPES:
-        for D, S, G in ((32, 16, 2), (32, 5, None), (12, 8, 3)):
-            c = case(device, 3, 77, D, S, dtype, G=G, lengths=[77, 40, 0])
-
-            def results(change):
-                d = {k: change(v.detach()).requires_grad_(True) if k in leaves_of(c) else v for k, v in c.items()}
 @pytest.mark.parametrize("S,D", [(8, 16), (16, 24), (5, 13), (40, 8)])
 @pytest.mark.parametrize("softplus", [False, True])
 def test_gradients_of_states_that_do_not_last(pkg, device, softplus, S, D):
@@ -247,6 +209,44 @@ def test_steps_that_are_not_numbers_show_in_every_gradient(pkg, device, softplus
     assert all(bool(grads[k][..., other].isfinite().all()) for k in ("x", "delta", "delta_bias"))
 
 
+def test_growing_states_after_a_start_of_zeros(pkg, device):
+    """A above 0 whose growth over a segment is beyond fp32: where nothing has entered yet nothing is multiplied."""
+    c = case(device, 1, 200, 8, 4, torch.float32, parts=(), softplus=False)
+    with torch.no_grad():
+        c["A"].fill_(30.0)
+        c["delta"].fill_(0.2)
+        c["x"][:, :190] = 0
+        y, state = call(pkg, c)
+    assert segment_tokens(1, 200, 8, 1, 4)[1] and not bool(y[:, :190].any()) and bool(y.isfinite().all()) and bool(state.isfinite().all())
+
+
+def test_steps_of_any_size(pkg, device):
+    """delta from far below to far above: softplus against float64, through a scan of one token."""
+    raw = torch.cat((torch.linspace(-30, 30, 4001), torch.tensor([-87.0, -100.0, -1e4, 1e4, 60.0])))
+    D = raw.numel()
+    one = torch.ones(1, 1, 1)
+    y = pkg.selective_scan(torch.ones(1, 1, D, device=device), raw.view(1, 1, D).to(device), -torch.ones(D, 1, device=device),
+                           one.to(device), one.to(device), softplus=True)[0, 0].double().cpu()
+    want = torch.log1p(torch.exp(-raw.double().abs())) + raw.double().clamp(min=0)
+    assert bool(((y - want).abs() <= want * 8 * U + 1.2e-38).all())
+
+
+def same(a, b):
+    assert len(a) == len(b) and all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+def test_layouts_give_the_same_bits(pkg, device):
+    """Strided, expanded, misaligned inputs and gradients against contiguous ones."""
+    odd = lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device=device)[1:].view(t.shape).copy_(t)   # noqa: E731
+    apart = lambda t: torch.stack((t, t), -1)[..., 0]                                                     # noqa: E731
+    wide = lambda t: torch.cat((t, t, t), -1)[..., t.shape[-1]:2 * t.shape[-1]]                            # noqa: E731
+    turned = lambda t: t if t.ndim < 2 else t.transpose(0, 1).contiguous().transpose(0, 1)                # noqa: E731
+    for dtype in DTYPES:
+        for D, S, G in ((32, 16, 2), (32, 5, None), (12, 8, 3)):
+            c = case(device, 3, 77, D, S, dtype, G=G, lengths=[77, 40, 0])
+
+            def results(change):
+                d = {k: change(v.detach()).requires_grad_(True) if k in leaves_of(c) else v for k, v in c.items()}
                 out = call(pkg, d)
                 return [*out, *torch.autograd.grad(out, [d[k] for k in leaves_of(c)], [change(c["dy"]), change(c["dstate"])])]
 
@@ -333,6 +333,16 @@ def test_refusals(pkg, device):
         pkg.selective_scan(big, big, torch.zeros(1, 1, device=device).expand(1 << 22, 1), big[..., :1], big[..., :1])
 
 
+def test_gradients_that_cannot_be_formed_are_refused_in_front(pkg, device):
+    """B N G of 2^24: the call with gradients is refused before its forward runs, the one without them runs."""
+    x = torch.full((1, 1, 16), 0.5, device=device).expand(1, 1 << 20, 16)
+    A = -torch.ones(16, 1, device=device)
+    rows = x[..., None]
+    assert bool((pkg.selective_scan(x, x, A, rows, rows) > 0).all())
+    with pytest.raises(pkg._lib.NativeLibraryError, match="gradients"):
+        pkg.selective_scan(x, x, A.requires_grad_(True), rows, rows)
+
+
 def step_call(pkg, c, rows, pool, **kw):
     return pkg.selective_scan_step(*(rows[k] for k in ("x", "delta")), c["A"], rows["B"], rows["C"], pool, skip=c.get("skip"),
                                    gate=rows.get("gate"), delta_bias=c.get("delta_bias"), softplus=c["softplus"], **kw)
@@ -371,16 +381,6 @@ def test_steps(pkg, device, D, S, G, dtype, across):
 
 @pytest.mark.parametrize("D,S", [(40, 16), (13, 5)])
 def test_rows_of_one_slot_are_tokens_in_order(pkg, device, D, S):
-def test_gradients_that_cannot_be_formed_are_refused_in_front(pkg, device):
-    """B N G of 2^24: the call with gradients is refused before its forward runs, the one without them runs."""
-    x = torch.full((1, 1, 16), 0.5, device=device).expand(1, 1 << 20, 16)
-    A = -torch.ones(16, 1, device=device)
-    rows = x[..., None]
-    assert bool((pkg.selective_scan(x, x, A, rows, rows) > 0).all())
-    with pytest.raises(pkg._lib.NativeLibraryError, match="gradients"):
-        pkg.selective_scan(x, x, A.requires_grad_(True), rows, rows)
-
-
     c = case(device, 1, 9, D, S, torch.bfloat16)
     rows = {k: c[k].detach()[0] for k in ("x", "delta", "gate", "B", "C")}
     slots = torch.tensor([2, 0, 2, -1, 2, 1, 0, 2, 4], dtype=torch.int32, device=device)
