@@ -111,6 +111,44 @@ def test_one_segment_and_many(pkg, device, B, N, D, S):
     check(pkg, case(device, B, N, D, S, torch.float32, seed=N))
 
 
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=str)
+@pytest.mark.parametrize("S,parts", [(16, ALL), (8, ALL), (13, ("skip",))])
+def test_tiles_of_long_segments(pkg, device, S, parts, dtype):
+    """Rows of 16 bits in one segment of several tiles (64 tokens forward up to 16 states), the last one not whole; sequences
+    that end in the first, second and third tile."""
+    assert not segment_tokens(4, 150, 3080, 1, S)[1]
+    check(pkg, case(device, 4, 150, 3080, S, dtype, parts=parts, lengths=[150, 65, 64, 129], seed=S))
+    check(pkg, case(device, 4, 70, 3080, S, dtype, parts=parts, seed=S + 1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("N", [65, 127, 128, 129, 200])
+@pytest.mark.parametrize("S,parts", [(8, ALL), (16, ALL), (16, ("skip", "initial")), (24, ALL)])
+def test_one_call_is_its_parts_of_one_tile(pkg, device, S, parts, N, dtype):
+    """A segment of several tiles against calls of 64 tokens with the state and its gradient between them: the same bits of
+    everything but the sums over all tokens."""
+    B, D = 22, 520
+    assert not segment_tokens(B, N, D, 1, S)[1]
+    ends = [N, N - 1, 64, 65, 63, 1, 0, 128, 129]
+    c = case(device, B, N, D, S, dtype, parts=parts, lengths=[min(ends[i % len(ends)], N) for i in range(B)], seed=N)
+    rows = [k for k in ("x", "delta", "B", "C", "gate") if k in c]
+    out = call(pkg, c)
+    grads = dict(zip([*rows, "initial"], torch.autograd.grad(out, [c[k] for k in [*rows, "initial"]], [c["dy"], c["dstate"]])))
+    calls, state = [], c["initial"]
+    for a in range(0, N, 64):
+        d = dict(c, **{k: c[k].detach()[:, a:a + 64].contiguous().requires_grad_(True) for k in rows},
+                 initial=state.detach().requires_grad_(True), lengths=(c["lengths"] - a).clamp(min=0))
+        y, state = call(pkg, d)
+        calls.append((a, d, y, state))
+    same([torch.cat([y for _, _, y, _ in calls], 1), state], out)
+    dstate, parts_of = c["dstate"], {k: [] for k in rows}
+    for a, d, y, s in reversed(calls):
+        *g, dstate = torch.autograd.grad([y, s], [d[k] for k in [*rows, "initial"]], [c["dy"][:, a:a + 64].contiguous(), dstate])
+        for k, t in zip(rows, g):
+            parts_of[k].insert(0, t)
+    same([*(torch.cat(parts_of[k], 1) for k in rows), dstate], [grads[k] for k in [*rows, "initial"]])
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("D,S,parts", [(24, 16, ALL), (13, 5, ALL), (16, 40, ("gate",)), (24, 16, ())])
 @pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=str)
