@@ -50,6 +50,18 @@ def segment_tokens(b, n, D, G, S):
     return seg, n > seg
 
 
+def conv_strips(b, n, D, dtype):
+    """Tokens of the convolution's strips forward and backward, as the launches choose them."""
+    def strip(vec):
+        blocks = -(-(-(-D // vec)) // 32)
+        tokens = 16
+        while tokens < 64 and b * n // (2 * tokens) // 8 * blocks >= 448:
+            tokens *= 2
+        return tokens
+    per = 4 if dtype == torch.float32 else 8
+    return strip(per if D >= per else 1), strip(4 if D >= 4 else 1)
+
+
 def scan_bounds(a, softplus, lengths=None, dy=None, dstate=None):
     """Bounds in u for y, state and, with dy, every gradient of the scan of a (a dict of float64 inputs)."""
     x, delta, A, B, C = (a[k] for k in ("x", "delta", "A", "B", "C"))

@@ -10,7 +10,7 @@ import torch
 
 from oracle import selective_ref
 from tests.mixer_cases import DTYPES, randn
-from tests.selective_cases import U, f64, silu_off, slope_off, within
+from tests.selective_cases import U, conv_strips, f64, silu_off, slope_off, within
 
 pytestmark = pytest.mark.gpu
 
@@ -92,6 +92,17 @@ def test_sizes(pkg, device, N, D, dtype):
 @pytest.mark.parametrize("B,N,D", [(40, 700, 40), (3, 4000, 520), (300, 5, 8)])
 def test_longer_strips_and_many_sequences(pkg, device, B, N, D):
     check(pkg, case(device, B, N, D, 3, torch.bfloat16, initial=False), "silu")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("B,N,D,W,activation,strip,lengths", [
+    (4, 57400, 12, 4, "silu", 64, [57400, 19200, 19201, 33]), (4, 57400, 8, 3, None, 64, [57399, 64, 63, 57345]),
+    (2, 57400, 12, 8, "silu", 32, [31999, 32001]), (2300, 100, 9, 4, "silu", 64, None)])
+def test_strips_of_32_and_64_tokens(pkg, device, B, N, D, W, activation, strip, lengths, dtype):
+    """The strips of large batches, forward and backward: sequences that end at a strip's end, beside it and inside, strips
+    longer than what is left of a sequence."""
+    assert conv_strips(B, N, D, dtype) == (strip, strip)
+    check(pkg, case(device, B, N, D, W, dtype, seed=D, lengths=lengths), activation)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
