@@ -4,6 +4,8 @@ Bounds are sums of what each rounding can do, in units of u = 2^-24 (half a step
 rounded; ``within`` of mixer_cases adds the last rounding to the result's type.
 """
 
+import math
+
 import torch
 
 from oracle import selective_ref
@@ -60,6 +62,28 @@ def conv_strips(b, n, D, dtype):
         return tokens
     per = 4 if dtype == torch.float32 else 8
     return strip(per if D >= per else 1), strip(4 if D >= 4 else 1)
+
+
+def norm_grid(rows, groups, D, dtype, backward):
+    """Workgroups of the norm's register kernels on aligned rows, and the rows of each, as the launches choose them."""
+    per, threads = 4 if dtype == torch.float32 else 8, 512 if backward else 256
+    units = D // per if D % per == 0 else D
+    k = 1
+    for tpr in (8, 16, 32, 64):
+        if units <= tpr:
+            break
+    else:
+        if units <= 256:
+            k = 2 if units <= 128 else 4
+        else:
+            assert units <= 2048
+            tpr = threads if units <= 4 * threads else 512
+            k = 1 if units <= tpr else 2 if units <= 2 * tpr else 4
+    each = threads // tpr if tpr < threads else 1
+    most = 2048 if not backward else 256 if k >= 2 else 512
+    unit = groups // math.gcd(groups, each)
+    blocks = -(-min(-(-rows * groups // each), most) // unit) * unit
+    return blocks, each
 
 
 def scan_bounds(a, softplus, lengths=None, dy=None, dstate=None):

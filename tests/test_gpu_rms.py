@@ -13,7 +13,7 @@ import torch
 
 from oracle import selective_ref
 from tests.mixer_cases import DTYPES, randn
-from tests.selective_cases import U, within
+from tests.selective_cases import U, norm_grid, within
 
 pytestmark = pytest.mark.gpu
 STREAMS = [(d, d) for d in DTYPES] + [(d, torch.float32) for d in DTYPES[:2]]
@@ -112,6 +112,46 @@ def test_row_counts_and_table_types(pkg, device, rows):
     for wtype in DTYPES:
         run(pkg, device, (rows, 72), torch.bfloat16, torch.bfloat16, (72,), wtype=wtype, seed=rows)
     run(pkg, device, (rows, 72), torch.float16, torch.float32, None, seed=rows, use_sum=False)
+
+
+@pytest.mark.parametrize("shape,G,dtype,stream", [
+    ((9001, 512), 1, torch.bfloat16, torch.bfloat16), ((9001, 512), 1, torch.float16, torch.float32),
+    ((30720, 512), 1, torch.bfloat16, torch.float32), ((9001, 512), 1, torch.float32, torch.float32),
+    ((24001, 3, 40), 3, torch.bfloat16, torch.float32), ((9500, 8, 64), 8, torch.float16, torch.float16),
+    ((9001, 1000), 1, torch.bfloat16, torch.bfloat16), ((9001, 2048), 1, torch.bfloat16, torch.float32),
+    ((2500, 1031), 1, torch.float16, torch.float16), ((2500, 8200), 1, torch.bfloat16, torch.float32),
+    ((4500, 2000), 1, torch.float32, torch.float32)], ids=str)
+def test_more_rows_than_a_grid_holds(pkg, device, shape, G, dtype, stream):
+    """Threads that walk over several rows: the bits of calls whose grids hold all their rows.  The weight's gradient adds a
+    thread's rows, its workgroup's of the group, and the partial rows, 64 threads to a column and those in five steps, so it is
+    a chain of as many steps; each term has s r and the product's rounding."""
+    rows, D = shape[0], shape[-1]
+    g = torch.Generator().manual_seed(rows + D)
+    x, r, dy, ds = (randn(g, *shape, dtype=t).to(device) for t in (dtype, stream, dtype, stream))
+    w = (1 + 0.2 * randn(g, *shape[-1 - (G > 1):])).to(device)
+    each = 1400 // G
+    grids = {back: [norm_grid(n, G, D, dtype, back) for n in (rows, each)] for back in (False, True)}
+    assert all(blocks * held < rows * G for blocks, held in (grids[False][0], grids[True][0]))
+    assert grids[False][1][0] * grids[False][1][1] >= each * G
+
+    def results(a, b):
+        t = [v[a:b].clone().requires_grad_(True) for v in (x, r)] + [w.clone().requires_grad_(True)]
+        out = pkg.rms_norm(t[0], t[2], residual=t[1])
+        grads = torch.autograd.grad(out, t, [dy[a:b].clone(), ds[a:b].clone()])
+        with torch.no_grad():
+            q, scale, s = pkg.rms_norm_fp8(t[0], t[2], residual=t[1])
+        return [*out, q.view(torch.uint8), scale, s, *grads[:2]], grads[2]
+
+    whole, dw = results(0, rows)
+    for a in range(0, rows, each):
+        part, _ = results(a, a + each)
+        assert all(torch.equal(t[a:a + each], p) for t, p in zip(whole, part)), a
+    s, up = whole[1].double(), dy.double()
+    terms = up * s / torch.sqrt((s * s).mean(-1, keepdim=True) + 1e-5)
+    blocks, held = grids[True][0]
+    chain = -(-rows * G // (blocks * held)) + -(-held // G) + -(-blocks // 64) + 16 + 2
+    off_by = terms.abs().sum(0) * (off(D) + (chain + 2) * U)
+    assert bool(((dw.double() - terms.sum(0)).abs() <= off_by + dw.double().abs() * U).all())
 
 
 @pytest.mark.parametrize("eps,scale", [(0.0, 1.0), (1e-2, 1e-3), (1e-5, 300.0)])
