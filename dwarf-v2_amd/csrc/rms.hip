@@ -12,6 +12,15 @@
 // a residual of bf16: forward 23.6 us (126 MB, 5.3 TB/s), backward 24.2 (126 MB,
 // 5.2 TB/s), the weight's sum 3.9.  40,960 rows with an fp32 residual into e4m3:
 // 39.9 us (231 MB, 5.8 TB/s).  Seven rows of 1,031 in fp32: 3.3 us.
+//
+// Wider rows, forward and backward with the sums: 8,192 of 4,096 in bf16 44 and
+// 52 us (268 MB each), with an fp32 stream 75 (403 MB) and 108 (537 MB).  The
+// backward of four 16-bit vectors a thread (1,025 to 2,048 and 8,193 to 16,384
+// elements) does not fit its 256 registers: it holds the next row of three
+// inputs, and spills 27 to 40, with an fp32 stream 129 to 156.  16,384 rows of 2,048
+// in bf16: 66 us (268 MB, 4.1 TB/s), with an fp32 stream 173 (537 MB, 3.1
+// TB/s); 2,048 of 16,384 86 and 200.  Streamed rows, read twice or three times:
+// 1,024 of 20,000 in bf16 58 and 111 us (164 MB each).
 #include "norm_rows.h"
 #include "selective.h"
 

@@ -9,11 +9,12 @@
 // Nothing here is a product of matrices: each (token, channel, state) has a
 // decay of its own, one exponential and four multiply-adds forward, 13 backward,
 // and that, not memory, bounds the kernels.  At B15 N2048, 1,024 channels of 16
-// states in bf16 (503 million of them): forward 205 us, 252 MB of rows and 126
-// MB of checkpoints; backward 540 us; the vector units issue in 70 and 76% of
-// the waves' cycles, and of those 62 and 55% are the operations above (84 and
-// 210 us at an instruction every 4 cycles, 8 for the exponential).  So
-// the work is laid out for the vector units: LPC adjacent lanes share a channel,
+// states in bf16 (503 million of them): forward 187 us, 252 MB of rows and 126
+// MB of checkpoints; backward 503 us; the vector units issue in 72 and 76% of
+// the waves' cycles, and of those 62 and 55% are the operations above (79 and
+// 197 us at an instruction every 4 cycles, 8 for the exponential, and 2.34
+// GHz).  The clock rises for some 20 passes; the comparisons below are of 12,
+// 205 and 540 us in all then.  So the work is laid out for the vector units: LPC adjacent lanes share a channel,
 // SPL states in the registers of each, and a wave holds 64 / LPC channels.  The
 // quads of lanes divide what a channel has once for each token (softplus, silu,
 // loads, stores) by taking one of four tokens each; a token's step reaches the
@@ -27,8 +28,9 @@
 // else it is cut into segments, which a launch in front reduces to the state
 // that each adds from zero and the sum of its steps (a segment's decay is
 // exp(A sum)); the rows' workgroups join the segments in front of their own
-// themselves (B1 N65536, 1,024 channels: 32 segments, 260 and 351 us).  The
-// backward does the same with the adjoint, from the end.
+// themselves (B1 N65536, 1,024 channels: 32 segments, 233 and 313 us, the vector
+// units busy 90 and 87% of that).  The backward does the same with the adjoint,
+// from the end.
 //
 // The backward walks chunks from the last to the first: it forms a chunk's
 // states again from the checkpoint the forward left in front of it, keeps them
@@ -1137,7 +1139,17 @@ ScanGeom scan_geom(const dwarf_selective_scan_fwd_args& a) {
   gm.tiles = gm.tiles_of_group * a.G;
   const int64_t groups = static_cast<int64_t>(a.B) * gm.tiles;
   // One segment from three quarters of a workgroup (four waves, one for each vector unit) a CU on: more cost most of the
-  // forward's work a second time.  Below that, segments for two workgroups a CU.
+  // forward's work a second time.  Below that, segments for two workgroups a CU, which share it up to 256 registers: the
+  // forward's rows of up to 16 states (of 32 where they are aligned and of 16 bits), the segments' sums of up to 8 (of 16 where
+  // aligned and of 16 bits).  The others, every backward kernel among them, run in two rounds.  Against segments for one
+  // workgroup a CU, 1,024 channels, us:
+  //   states, type   B1 N65536 forward   B2 N2048 with gradients
+  //   16 bf16         544 against   642   150 against 150
+  //   16 fp32         613 against   668   160 against 151
+  //   32 bf16         992 against 1,076   252 against 244
+  //   32 fp32       1,104 against 1,094   270 against 247
+  //   64 bf16       2,182 against 2,175   490 against 474
+  //   64 fp32       2,174 against 2,162   483 against 467
   int64_t segs = groups >= 192 ? 1 : 512 / groups;
   if (segs > kMaxSegments) segs = kMaxSegments;
   gm.seg = static_cast<int>((a.N + segs - 1) / segs + kSegmentUnit - 1) / kSegmentUnit * kSegmentUnit;

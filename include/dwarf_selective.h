@@ -4,7 +4,9 @@
  * short causal convolution of each channel, and the selective scan, for
  * training and prompts and (convolution, scan) single tokens.  Conventions
  * (status codes, strides in elements, dwarf_stream_t) are those of
- * dwarf_dsqg.h, element types those of dwarf_mixer.h.
+ * dwarf_dsqg.h, element types those of dwarf_mixer.h.  Results share no memory
+ * with the inputs or with each other; but a step's new_state may be its state,
+ * and the pool that it writes shares none with the rest.
  */
 #ifndef DWARF_SELECTIVE_H
 #define DWARF_SELECTIVE_H
@@ -21,7 +23,6 @@ extern "C" {
  * unit element stride; residual and sum the same shape in residual_dtype (dtype or DWARF_F32).  weight
  * [groups][D] fp32, contiguous, may be NULL (1).  y in dtype, rounded once; where scale is given, y holds e4m3
  * bytes instead: y / scale, scale [rows][groups] fp32 = max|y| / 448 of the row, at least the smallest normal fp32.
- * sum and y share no memory with the others.
  */
 typedef struct {
   int64_t rows;
@@ -83,8 +84,8 @@ typedef struct {
 int dwarf_causal_conv_fwd(const dwarf_causal_conv_fwd_args* args, dwarf_stream_t stream);
 
 /*
- * The gradients for dy (and dfinal, NULL: zero): dx and dinitial in dtype (may be NULL), dweight [D][W] and dbias
- * [D] fp32 (each may be NULL), summed in a fixed order.  fwd.y and fwd.final are not used.
+ * The gradients for dy (and dfinal, NULL: zero): dx in dtype, dinitial in dtype (may be NULL), dweight [D][W] and
+ * dbias [D] fp32 (each may be NULL), summed in a fixed order.  fwd.y and fwd.final are not used.
  */
 typedef struct {
   dwarf_causal_conv_fwd_args fwd;
@@ -105,7 +106,7 @@ int dwarf_causal_conv_bwd(const dwarf_causal_conv_bwd_args* args, dwarf_stream_t
  * elements, each slot contiguous): row r takes slot slots[r] (r itself where slots is NULL).  The rows moved on by
  * one go to new_state (the pool itself, or another one of the same slot stride).  A slot outside [0, pool) marks a
  * row that pads the batch: no state is touched and its output is zero.  Rows of one slot are consecutive tokens of
- * its sequence, in row order.  x, out [R][D] by row stride; out shares no memory with the others.
+ * its sequence, in row order.  x, out [R][D] by row stride.
  */
 typedef struct {
   int32_t R, D, W, pool;
@@ -132,7 +133,9 @@ int dwarf_causal_conv_step(const dwarf_causal_conv_step_args* args, dwarf_stream
  * [0, 2^22) elements, D below 2^22.  A [D][S], skip and delta_bias [D]
  * (each may be NULL: 0) fp32.  h_{-1} = initial [B][D][S] fp32 (NULL: zero), final [B][D][S] = the state behind the
  * last live token (may be NULL).  checkpoints: dwarf_selective_scan_checkpoint_bytes() bytes that the backward reads,
- * NULL where there will be none.
+ * NULL where there will be none; with them the limit of the gradients, B G N + 4.2 D below 2^24, holds forward too.
+ * A step of 0 passes the state on, also where A is minus infinity, and has no part in the gradients of A; under the
+ * softplus, where a step of 0 has no slope, neither in those of delta and delta_bias.
  */
 typedef struct {
   int32_t B, N, D, G, S;
