@@ -125,7 +125,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
 
 def _check_scale(scale) -> float:
     scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
+    if not -math.inf < scale < math.inf:   # comparisons alone: where shapes are dynamic a trace has scale as a symbol
         raise ValueError("scale must be finite")
     return scale
 

@@ -74,7 +74,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 
 def _check(x, weight, bias, eps) -> int:
     """The native call's checks, for compiled and traced calls; returns the groups."""
-    if not (math.isfinite(eps) and eps >= 0):
+    if not 0 <= eps < math.inf:   # comparisons alone: where shapes are dynamic a trace has eps as a symbol
         raise ValueError("eps must be finite and not negative")
     if x.ndim < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must have a last dimension to normalise, got {tuple(x.shape)}")

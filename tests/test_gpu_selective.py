@@ -305,6 +305,34 @@ def test_compiled_block_with_gradients(pkg, device):
          want)
 
 
+def test_compiled_with_dynamic_shapes(pkg, device):
+    """One trace for several sizes and numbers: sizes, eps and scale are symbols there.  The checks still refuse."""
+    compile_ = lambda f: torch.compile(f, backend="aot_eager", fullgraph=True, dynamic=True)   # noqa: E731
+    whole = compile_(lambda *a: calls(pkg, dict(zip(PARAMETERS, a))))
+    token = compile_(lambda *a: one_token(pkg, dict(zip(PARAMETERS, a))))
+    for n in (70, 131):
+        p, ups = make(2, n, torch.bfloat16, n, device)
+        t = leaves_of(p)
+        want = [*calls(pkg, t)]
+        want = [*(w.detach() for w in want), *gradients(pkg, t, ups, want), *one_token(pkg, p)]
+        t = leaves_of(p)
+        outs = whole(*(t[k] for k in PARAMETERS))
+        same([*outs, *gradients(pkg, t, ups, outs), *token(*(p[k] for k in PARAMETERS))], want)
+    norms = compile_(lambda x, w, eps: [pkg.rms_norm(x, w, eps=eps), *pkg.rms_norm(x, w, residual=x, eps=eps), pkg.layer_norm(x, w, eps=eps)])
+    heads = compile_(lambda q, d, scale: pkg.linear_attention(q, q, q, d, scale=scale))
+    decay = torch.tensor([-0.1, -0.02], device=device)
+    for n, number in ((5, 1e-5), (5, 1e-2), (9, 0.5)):
+        x, w, q = torch.randn(n, 48, device=device), torch.randn(48, device=device), torch.randn(1, 2, 30 * n, 64, device=device)
+        same(norms(x, w, number), [pkg.rms_norm(x, w, eps=number), *pkg.rms_norm(x, w, residual=x, eps=number), pkg.layer_norm(x, w, eps=number)])
+        same([heads(q, decay, number)], [pkg.linear_attention(q, q, q, decay, scale=number)])
+    for bad in (-1.0, float("inf"), float("nan")):
+        with pytest.raises(Exception, match="eps"):
+            norms(x, w, bad)
+        if bad != -1.0:
+            with pytest.raises(Exception, match="scale"):
+                heads(q, decay, bad)
+
+
 def test_negated_and_zero_tensors(pkg, device):
     p, ups = traced_case(device)
     turned = {k: torch._neg_view(-v) for k, v in p.items()}
